@@ -68,6 +68,17 @@ SIGNATURES = [
     ("bg_kv_import_rows", _i32, [_vp, _i32, _i32, _i32, _i32, _vp, _vp]),
     ("bg_kv_save", _i32, [_vp, _i32, _i32, _vp, C.c_size_t, _vp]),
     ("bg_kv_load", _i32, [_vp, _i32, _i32, _vp, C.c_size_t, _vp]),
+    ("bg_paged_region_bytes", _i32, [_i32] * 7 + [C.POINTER(C.c_size_t)]),
+    ("bg_paged_create", _i32, [_i32] * 6 + [_vp] * 4 + [C.POINTER(_vp)]),
+    ("bg_paged_destroy", _i32, [_vp]),
+    ("bg_paged_set_q8_block", _i32, [_vp, _i32]),
+    ("bg_paged_batch_create", _i32, [_vp, _i32, _i32, _i32, _i32, C.POINTER(_vp)]),
+    ("bg_paged_batch_destroy", _i32, [_vp]),
+    ("bg_paged_batch_set", _i32, [_vp, _i32, _vp, _vp, _vp, _i32, _vp, _i32, _vp]),
+    ("bg_paged_batch_info", _i32, [_vp, C.POINTER(C.c_int64)]),
+    ("bg_paged_qkv_prologue", _i32, [_vp, _i32, _vp, _vp, _i32, _vp, _vp, _vp, _vp, _f32, _vp, _vp, _i32, _i32, _vp, _vp,
+                                     _vp]),
+    ("bg_paged_attention", _i32, [_vp, _i32, _vp, _vp, _f32, _vp, _i32, _vp, _vp]),
 ]
 
 

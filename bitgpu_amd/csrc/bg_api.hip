@@ -244,6 +244,13 @@ int32_t take_merge_error(bg_kv_cache* c, hipStream_t st) {
 
 }  // namespace
 
+// the same for the other files of entry points (bg_api_util.h)
+namespace bg {
+int32_t api_fail(int32_t code, const char* msg) { return fail(code, "%s", msg); }
+int32_t api_hip_fail(hipError_t e, const char* what) { return hip_fail(e, what); }
+bool api_capturing(hipStream_t st) { return capturing(st); }
+}  // namespace bg
+
 extern "C" {
 
 const char* bg_last_error_message(void) { return g_err.c_str(); }

@@ -1,0 +1,409 @@
+// The host side of a paged batch: checks of what a caller hands over (rows, lengths, page lists) and the
+// plan the kernels run by. Plain C++ (no HIP), so it is tested on the CPU.
+//
+// A batch is n_seqs sequences; sequence b holds lens[b] positions in pages of `page` slots, its last
+// rows[b] of them new in this call. Attention over it is cut into segments, a segment being a run of
+// positions in the same pages for all of its member rows:
+//   shared    the sequences' page lists form a tree (a node: sequences that list the same pages so far);
+//             every edge of it with two or more sequences is one segment, scanned once for the rows of
+//             all of them. Only pages that every row of the member sees whole are shared, so no mask.
+//   private   the rest of each sequence, causal
+// and a segment into units: a tile of its rows (row = (token, head of the kv head's group)) times a
+// chunk of its positions, one unit a workgroup and kv head. A row that meets several units gets a
+// partial (o, m, l) from each, joined by the merge kernel; a row of one unit is stored directly.
+#pragma once
+
+#include <stdint.h>
+#include <stdio.h>
+
+#include <algorithm>
+#include <string>
+#include <vector>
+
+namespace bg {
+
+// One workgroup's attention work, for every kv head. Positions [key0, key1) (key0 a multiple of 32) of
+// the page list at pages[table]; rows rho0 .. rho0 + n_rho - 1 of the tokens at toks[tok].
+struct PagedUnit {
+  int kind;    // 16-row sets a wave holds (1, 2), its four waves splitting the positions; 0: 128 rows,
+               // 32 a wave, the positions staged through LDS for all four
+  int tok;
+  int rho0, n_rho;
+  int table;
+  int key0, key1;
+  int mask0;   // positions below this are seen by every row of the unit
+  int chunk;   // which chunk of its segment: the partial slot is the token's `part` + chunk
+  int pad[3];
+};
+struct PagedTok {
+  int t;       // row of q and out
+  int pos;     // attends positions <= pos
+  int part;    // partial slot of the segment's first chunk; -1: the row's only unit, stored directly
+  int pad;
+};
+struct PagedMerge {
+  int t, part, n, pad;
+};
+
+struct PagedShape {
+  int kv_heads, G, D, dtype, page, n_pages;
+  int cus;
+  int max_seqs, max_tokens, max_pages;  // what the batch's arrays hold
+
+  // shared segments on one sequence's path at most (what is below them stays private)
+  static constexpr int kLevels = 4;
+  int max_toks() const { return max_tokens * (kLevels + 1); }
+  // units: a segment's row tiles unsplit (2 at most where they are fewer than 128 rows), and what a
+  // split adds, up to 8 units a CU
+  long max_units() const {
+    return (long)max_toks() * G / 128 + 2L * (2L * max_seqs) + 8L * cus;
+  }
+};
+// storage bytes of 32 values (bg_kv dtypes: 0 f32, 1 f16, 2 q8 with its scale)
+inline int paged_bytes32(int dtype) { return dtype == 0 ? 128 : dtype == 1 ? 64 : 36; }
+
+struct PagedPlan {
+  std::vector<PagedUnit> units;
+  std::vector<PagedTok> toks;
+  std::vector<PagedMerge> merges;
+  std::vector<int> pages;        // every sequence's page list, one after the other
+  std::vector<int> dst;          // per token: page * page size + slot
+  std::vector<int> v_single;     // tokens whose V row is stored alone
+  std::vector<int> v_group;      // first tokens of 16 that fill 16 aligned slots
+  int n_tokens = 0, n_parts = 0;
+  int shared_segments = 0;
+  int64_t keys = 0;              // positions scanned, a segment's once (a kv head)
+  int write_page = -1;           // a page whose new positions another sequence also lists (see below)
+};
+
+class PagedPlanner {
+ public:
+  // Fills `out`; "" or what is wrong with the arguments. table: [n_seqs][stride], the first
+  // ceil(lens[b] / page) entries of row b are read. `seen` is scratch kept between calls.
+  std::string build(const PagedShape& sh, int n_seqs, const int* rows, const int* lens, const int* table, int stride,
+                    PagedPlan& out) {
+    char msg[200];
+    sh_ = sh;
+    out_ = &out;
+    if (n_seqs < 0 || n_seqs > sh.max_seqs) {
+      snprintf(msg, sizeof(msg), "%d sequences in a batch of at most %d", n_seqs, sh.max_seqs);
+      return msg;
+    }
+    const int P = sh.page;
+    long tokens = 0, pages = 0;
+    for (int b = 0; b < n_seqs; b++) {
+      if (lens[b] < 0 || lens[b] > kMaxLen || rows[b] < 0 || rows[b] > lens[b]) {
+        snprintf(msg, sizeof(msg), "sequence %d: %d new rows of %d positions", b, rows[b], lens[b]);
+        return msg;
+      }
+      const int need = lens[b] / P + (lens[b] % P != 0);
+      if (need > stride) {
+        snprintf(msg, sizeof(msg), "sequence %d: %d positions need %d pages of %d, its list holds %d", b, lens[b], need, P, stride);
+        return msg;
+      }
+      tokens += rows[b];
+      pages += need;
+    }
+    if (tokens > sh.max_tokens || pages > sh.max_pages) {
+      snprintf(msg, sizeof(msg), "%ld new rows and %ld pages in a batch of at most %d and %d", tokens, pages, sh.max_tokens, sh.max_pages);
+      return msg;
+    }
+    // the page lists; ids checked before anything uses them
+    out.pages.clear();
+    off_.assign(n_seqs + 1, 0);
+    for (int b = 0; b < n_seqs; b++) {
+      const int need = lens[b] / P + (lens[b] % P != 0);
+      for (int i = 0; i < need; i++) {
+        const int id = table[(size_t)b * stride + i];
+        if (id < 0 || id >= sh.n_pages) {
+          snprintf(msg, sizeof(msg), "sequence %d: page %d of its list is %d, of %d", b, i, id, sh.n_pages);
+          return msg;
+        }
+        out.pages.push_back(id);
+      }
+      off_[b + 1] = (int)out.pages.size();
+    }
+    n_seqs_ = n_seqs;
+    rows_ = rows;
+    lens_ = lens;
+    out.n_tokens = (int)tokens;
+    append(out);
+    attend(out);
+    return "";
+  }
+
+ private:
+  static constexpr int kMaxLen = 1 << 30;  // positions of one sequence: the arithmetic below stays in int
+
+  struct Segment {
+    int table, key0, key1;  // positions; key1 the most any row sees
+    int tok, n_tok;
+    int rows;               // n_tok * G
+    bool shared;
+    int chunks = 1, chunk_len = 0;
+  };
+
+  // Where the new rows go, and the check that no two of them, and no other sequence's positions, share a
+  // slot: write_page is a page that one sequence writes while another (or itself, twice) lists it with
+  // written positions. The append refuses such a batch; attention alone may read it.
+  void append(PagedPlan& out) {
+    const int P = sh_.page;
+    out.dst.clear();
+    out.v_single.clear();
+    out.v_group.clear();
+    out.write_page = -1;
+    if ((int)stamp_.size() < sh_.n_pages) stamp_.resize(sh_.n_pages, 0);
+    if (epoch_ > 0x7ffffff0) {
+      std::fill(stamp_.begin(), stamp_.end(), 0);
+      epoch_ = 0;
+    }
+    const int written = ++epoch_;
+    int tok = 0;
+    for (int b = 0; b < n_seqs_; b++) {
+      if (!rows_[b]) continue;
+      const int p0 = lens_[b] - rows_[b], p1 = lens_[b];
+      for (int i = p0 / P; i <= (p1 - 1) / P; i++) {
+        const int id = out.pages[off_[b] + i];
+        if (stamp_[id] == written) out.write_page = id;
+        stamp_[id] = written;
+      }
+      for (int p = p0; p < p1; p++) out.dst.push_back(out.pages[off_[b] + p / P] * P + p % P);
+      int p = p0;
+      while (p < p1) {
+        if ((p & 15) == 0 && p + 16 <= p1) {
+          out.v_group.push_back(tok + p - p0);
+          p += 16;
+        } else {
+          out.v_single.push_back(tok + p - p0);
+          p++;
+        }
+      }
+      tok += rows_[b];
+    }
+    // a written page listed elsewhere so far that its written slots are read there
+    if (tok) {
+      for (int b = 0; b < n_seqs_; b++) {
+        const int n = off_[b + 1] - off_[b], first = rows_[b] ? (lens_[b] - rows_[b]) / P : n;
+        for (int i = 0; i < std::min(n, first); i++) {
+          const int id = out.pages[off_[b] + i];
+          if (stamp_[id] == written && reads_written(out, b, i, id)) out.write_page = id;
+        }
+      }
+    }
+  }
+  // sequence b reads page id (entry i of its list): does it read a slot that some sequence writes?
+  bool reads_written(const PagedPlan& out, int b, int i, int id) const {
+    const int P = sh_.page, upto = std::min(P, lens_[b] - i * P);
+    for (int c = 0; c < n_seqs_; c++) {
+      if (!rows_[c]) continue;
+      const int p0 = lens_[c] - rows_[c];
+      for (int j = p0 / P; j <= (lens_[c] - 1) / P; j++)
+        if (out.pages[off_[c] + j] == id && (b != c || j != i) && upto > std::max(0, p0 - j * P)) return true;
+    }
+    return false;
+  }
+
+  // a 128-row tile a sequence fills by itself gains nothing from other sequences' rows
+  bool shares(int b) const { return rows_[b] > 0 && rows_[b] * sh_.G < 128; }
+
+  void attend(PagedPlan& out) {
+    out.units.clear();
+    out.toks.clear();
+    out.merges.clear();
+    segs_.clear();
+    out.shared_segments = 0;
+    out.keys = 0;
+    first_.assign(n_seqs_, 0);
+    start_.assign(n_seqs_, 0);
+    std::vector<int> members;
+    int tok = 0;
+    for (int b = 0; b < n_seqs_; b++) {
+      first_[b] = tok;
+      tok += rows_[b];
+      if (shares(b)) members.push_back(b);
+    }
+    split(members, 0, 0, 0);
+    for (int b = 0; b < n_seqs_; b++) {
+      if (!rows_[b] || lens_[b] <= start_[b] * sh_.page) continue;
+      Segment s;
+      s.table = off_[b];
+      s.key0 = start_[b] * sh_.page;
+      s.key1 = lens_[b];
+      s.tok = (int)out.toks.size();
+      s.n_tok = rows_[b];
+      s.rows = rows_[b] * sh_.G;
+      s.shared = false;
+      push_tokens(b);
+      segs_.push_back(s);
+    }
+    chunk();
+    emit(out);
+  }
+
+  void push_tokens(int b) {
+    for (int i = 0; i < rows_[b]; i++)
+      out_->toks.push_back(PagedTok{first_[b] + i, lens_[b] - rows_[b] + i, -1, 0});
+  }
+  // pages of sequence b that all of its rows see whole
+  int whole(int b) const { return (lens_[b] - rows_[b] + 1) / sh_.page; }
+
+  // The tree below `members`, which list the same pages up to `depth`; those from `start` on are not yet
+  // in a segment.
+  void split(const std::vector<int>& members, int start, int depth, int level) {
+    if (members.size() < 2 || level == PagedShape::kLevels) {
+      for (int b : members) start_[b] = start;
+      return;
+    }
+    const std::vector<int>& pages = out_->pages;
+    std::vector<int> order(members);
+    auto key = [&](int b) { return depth < whole(b) ? pages[off_[b] + depth] : -1; };
+    std::stable_sort(order.begin(), order.end(), [&](int x, int y) { return key(x) < key(y); });
+    for (size_t i = 0; i < order.size();) {
+      size_t j = i + 1;
+      const int id = key(order[i]);
+      while (j < order.size() && key(order[j]) == id) j++;
+      if (id < 0 || j - i < 2) {
+        for (size_t m = i; m < j; m++) start_[order[m]] = start;
+        i = j;
+        continue;
+      }
+      const std::vector<int> cls(order.begin() + i, order.begin() + j);
+      int end = whole(cls[0]);
+      for (int b : cls) {
+        int e = depth + 1;
+        const int lim = std::min(end, whole(b));
+        while (e < lim && pages[off_[b] + e] == pages[off_[cls[0]] + e]) e++;
+        end = e;
+      }
+      // Worth a segment when the reads it saves outweigh the partials it adds: every row's o is
+      // written and read once more.
+      long rows = 0;
+      for (int b : cls) rows += rows_[b];
+      const long saved = (long)(cls.size() - 1) * (end - start) * sh_.page * 2 * (sh_.D / 32) * paged_bytes32(sh_.dtype);
+      const long added = rows * sh_.G * 2 * sh_.D * 4;
+      if (saved > added) {
+        Segment s;
+        s.table = off_[cls[0]];
+        s.key0 = start * sh_.page;
+        s.key1 = end * sh_.page;
+        s.tok = (int)out_->toks.size();
+        s.n_tok = (int)rows;
+        s.rows = (int)rows * sh_.G;
+        s.shared = true;
+        for (int b : cls) push_tokens(b);
+        segs_.push_back(s);
+        out_->shared_segments++;
+        split(cls, end, end, level + 1);
+      } else {
+        split(cls, start, end, level);
+      }
+      i = j;
+    }
+  }
+
+  // rows of one unit of a segment
+  int tile_rows(const Segment& s) const {
+    if (s.rows > 32) return 128;
+    return s.rows > 16 && sh_.dtype != 0 ? 32 : 16;
+  }
+  // The work of a row tile over 32 positions, in 1/8 us of a workgroup with the GPU full: the few-row
+  // kinds move the positions' bytes, the 128-row kind runs the matrix products.
+  int weight(const Segment& s) const {
+    if (s.rows <= 32) return sh_.dtype == 0 ? 22 : sh_.dtype == 1 ? 11 : 8;
+    return sh_.dtype == 0 ? 56 : sh_.dtype == 1 ? 8 : 12;
+  }
+
+  void chunk() {
+    const int per_cu = sh_.D == 128 ? 2 : 1;
+    const long slots = std::max(1L, (long)sh_.cus * per_cu);
+    double total = 0;
+    for (Segment& s : segs_) {
+      const int tiles = (s.key1 - s.key0 + 31) / 32, n = (s.rows + tile_rows(s) - 1) / tile_rows(s);
+      total += (double)tiles * n * weight(s) * sh_.kv_heads * (s.shared ? 1.0 : 0.5 + 0.5 * s.key0 / s.key1);
+    }
+    // half a workgroup slot's share of the work a unit, and as many units as the arrays hold
+    for (double share = total / slots / 2;; share = 2 * share + 64) {
+      long units = 0;
+      for (Segment& s : segs_) {
+        const int tiles = (s.key1 - s.key0 + 31) / 32, n = (s.rows + tile_rows(s) - 1) / tile_rows(s);
+        const long len = std::max(s.rows <= 32 ? 4L : 8L, (long)(share / weight(s)));
+        s.chunks = (int)((tiles + len - 1) / len);
+        s.chunk_len = ((tiles + s.chunks - 1) / s.chunks + 1) & ~1;
+        s.chunks = (tiles + s.chunk_len - 1) / s.chunk_len;
+        units += (long)s.chunks * n;
+      }
+      if (units <= sh_.max_units()) return;
+    }
+  }
+
+  void emit(PagedPlan& out) {
+    // partial slots: a token's parts are the chunks of the segments it is in, one after the other
+    count_.assign(out.n_tokens, 0);
+    for (const Segment& s : segs_)
+      for (int i = 0; i < s.n_tok; i++) count_[out.toks[s.tok + i].t] += s.chunks;
+    base_.assign(out.n_tokens, 0);
+    int parts = 0;
+    for (int t = 0; t < out.n_tokens; t++) {
+      if (count_[t] > 1) {
+        out.merges.push_back(PagedMerge{t, parts, count_[t], 0});
+        base_[t] = parts;
+        parts += count_[t];
+      } else {
+        base_[t] = -1;
+      }
+    }
+    out.n_parts = parts;
+    for (const Segment& s : segs_) {
+      for (int i = 0; i < s.n_tok; i++) {
+        PagedTok& k = out.toks[s.tok + i];
+        k.part = base_[k.t];
+        if (base_[k.t] >= 0) base_[k.t] += s.chunks;
+      }
+    }
+    // units, the heaviest first
+    cost_.clear();
+    for (const Segment& s : segs_) {
+      out.keys += s.key1 - s.key0;
+      const int R = tile_rows(s);
+      for (int c = 0; c < s.chunks; c++) {
+        for (int r0 = 0; r0 < s.rows; r0 += R) {
+          PagedUnit u{};
+          u.kind = R / 16 > 2 ? 0 : R / 16;
+          u.tok = s.tok;
+          u.rho0 = r0;
+          u.n_rho = std::min(R, s.rows - r0);
+          u.table = s.table;
+          u.chunk = c;
+          u.key0 = s.key0 + c * s.chunk_len * 32;
+          int lo = out.toks[s.tok + r0 / sh_.G].pos, hi = lo;
+          if (!s.shared) hi = out.toks[s.tok + (r0 + u.n_rho - 1) / sh_.G].pos;  // rows in order of position
+          u.key1 = std::min(s.key0 + (c + 1) * s.chunk_len * 32, s.shared ? s.key1 : hi + 1);
+          if (u.key1 < u.key0) u.key1 = u.key0;
+          u.mask0 = s.shared ? s.key1 : lo + 1;
+          out.units.push_back(u);
+          cost_.push_back((long)((u.key1 - u.key0 + 31) / 32) * weight(s));
+        }
+      }
+    }
+    order_.resize(out.units.size());
+    for (size_t i = 0; i < order_.size(); i++) order_[i] = (int)i;
+    std::stable_sort(order_.begin(), order_.end(), [&](int a, int b) { return cost_[a] > cost_[b]; });
+    sorted_.clear();
+    for (int i : order_) sorted_.push_back(out.units[i]);
+    out.units.swap(sorted_);
+  }
+
+  PagedShape sh_{};
+  PagedPlan* out_ = nullptr;
+  int n_seqs_ = 0;
+  const int* rows_ = nullptr;
+  const int* lens_ = nullptr;
+  std::vector<int> off_, first_, start_, count_, base_, order_;
+  std::vector<long> cost_;
+  std::vector<PagedUnit> sorted_;
+  std::vector<Segment> segs_;
+  std::vector<int> stamp_;
+  int epoch_ = 0;
+};
+
+}  // namespace bg

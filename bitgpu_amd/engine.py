@@ -15,6 +15,10 @@ The reference (stfurkan/bitgpu v0.19.1, src/engine.ts) records, per layer:
 * the fused decode block's qkv projection + prologue (1526-1540) -> :func:`qkv_proj_prologue`,
   and the block through o_proj + residual (1519-1547)          -> :func:`decode_attention_block`
 
+The reference holds one conversation an engine. For many at once, on one pool of pages that sequences may
+share: :class:`PagedKvCache`, :class:`PagedBatch`, :func:`paged_qkv_prologue`, :func:`paged_attention`, and
+the layer blocks :func:`paged_layer_attention` and :func:`paged_hybrid_attention`.
+
 Device memory is owned by torch tensors (``cuda`` device, float32, contiguous); only raw
 pointers cross the boundary. Every call is enqueued on torch's current stream. There is no CPU
 fallback: without the built HIP library these functions raise.
@@ -36,7 +40,8 @@ from ._lib import (BG_E_INVALID, BG_E_STATE, BG_K, BG_KSCALE, BG_ROPE_ABSOLUTE, 
 
 __all__ = ["KvCache", "attention", "qkv_prologue", "layer_attention", "hybrid_full_attention",
            "rope_tables", "evict_plan", "ring_map", "validate_snapshot", "OneBitWeight", "fused_mm", "resid_mm",
-           "qkv_proj_prologue", "decode_attention_block"]
+           "qkv_proj_prologue", "decode_attention_block", "PagedKvCache", "PagedBatch", "paged_qkv_prologue",
+           "paged_attention", "paged_layer_attention", "paged_hybrid_attention"]
 
 
 # A decode step makes two to four of these calls a layer on kernels of 4 to 13 us, so what a call
@@ -526,3 +531,241 @@ def decode_attention_block(cache: KvCache, li: int, n1, h, w_qkv: OneBitWeight, 
     qr = qkv_proj_prologue(cache, li, n1, w_qkv, H, q_norm, k_norm, eps, cos_tab, sin_tab, cache.head_dim, pos, slot)
     att = attention(cache, li, qr, 1, H, slot)
     return resid_mm(w_o, att.reshape(-1), h)
+
+
+# --------------------------------------------------------------------------------------------
+# many sequences on one pool of pages
+# --------------------------------------------------------------------------------------------
+class PagedKvCache:
+    """A pool of KV pages for many sequences (bg_paged_create): ``n_pages`` pages of ``page_size`` positions
+    (32, 64, 128 or 256) for each of ``n_layers`` layers. ``kv_cache`` and ``q8_block`` as in
+    :class:`KvCache`.
+
+    The pages are torch tensors, ``k`` [layers, pages, kv_heads, page_size, D], ``v`` [layers, pages,
+    kv_heads, page_size / 32, 4, D, 8] (slot 16a + 8c + 4b + r of a 32-slot tile at [2a + b, :, 4c + r])
+    and, for q8, ``k_scale`` / ``v_scale`` [layers, pages, kv_heads, page_size, D / 32] f32 (a value is
+    code * scale / 127): allocated uninitialized, or the caller's own. Which pages a sequence holds is the
+    caller's bookkeeping; a page's content is copied (a fork in the middle of a page) as
+    ``cache.k[:, dst] = cache.k[:, src]`` and the same for the other tensors."""
+
+    def __init__(self, n_layers: int, kv_heads: int, head_dim: int, kv_cache: str = "f32", *, n_pages: int,
+                 page_size: int = 64, q8_block: int = 32, k=None, v=None, k_scale=None, v_scale=None, device="cuda"):
+        if kv_cache not in KV_DTYPES:
+            raise ValueError(f"bitgpu_amd: kvCache must be one of {sorted(KV_DTYPES)}")
+        dtype = KV_DTYPES[kv_cache]
+        nbytes = C.c_size_t()  # the library's checks of the geometry, before anything is allocated
+        check(lib().bg_paged_region_bytes(n_layers, kv_heads, head_dim, dtype, page_size, n_pages, BG_K, C.byref(nbytes)))
+        elem = {"f32": torch.float32, "f16": torch.float16, "q8": torch.int8}[kv_cache]
+        lead = (n_layers, n_pages, kv_heads)
+        self._h = C.c_void_p()
+
+        def pool(t, name, shape, dt):
+            if t is None:
+                return torch.empty(shape, dtype=dt, device=device)
+            if t.dtype is not dt or t.shape != shape:
+                raise ValueError(f"bitgpu_amd: {name} must be {dt} {list(shape)}, got {t.dtype} {list(t.shape)}")
+            return t
+
+        self.k = pool(k, "k", (*lead, page_size, head_dim), elem)
+        self.v = pool(v, "v", (*lead, page_size // 32, 4, head_dim, 8), elem)
+        self.k_scale = self.v_scale = None
+        if kv_cache == "q8":
+            self.k_scale = pool(k_scale, "k_scale", (*lead, page_size, head_dim // 32), torch.float32)
+            self.v_scale = pool(v_scale, "v_scale", (*lead, page_size, head_dim // 32), torch.float32)
+        elif k_scale is not None or v_scale is not None:
+            raise ValueError("bitgpu_amd: k_scale and v_scale belong to a q8 cache")
+        self.n_layers, self.kv_heads, self.head_dim, self.kv_cache = n_layers, kv_heads, head_dim, kv_cache
+        self.n_pages, self.page_size, self.q8_block, self.device = n_pages, page_size, q8_block, self.k.device
+        with torch.cuda.device(self._one_device(self.k, self.v, self.k_scale, self.v_scale)):
+            check(lib().bg_paged_create(n_layers, kv_heads, head_dim, dtype, page_size, n_pages, _ptr(self.k), _ptr(self.v),
+                                        _ptr(self.k_scale), _ptr(self.v_scale), C.byref(self._h)))
+        if kv_cache == "q8" and q8_block != 32:
+            check(lib().bg_paged_set_q8_block(self._h, int(q8_block)))
+
+    def _one_device(self, *tensors):
+        """The pool's device; every tensor of a call has to be there."""
+        for t in tensors:
+            if t is not None and t.device != self.device:
+                raise ValueError(f"bitgpu_amd: expected tensors on {self.device}, got one on {t.device}")
+        if self.device.type != "cuda":
+            raise ValueError("bitgpu_amd: expected a device (cuda) tensor")
+        return self.device
+
+    def close(self):
+        if self._h:
+            lib().bg_paged_destroy(self._h)
+            self._h = C.c_void_p()
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+    @property
+    def handle(self):
+        return self._h
+
+
+class PagedBatch:
+    """What the paged calls work on (bg_paged_batch_create): up to ``max_seqs`` sequences with ``max_tokens``
+    new rows and ``max_pages`` listed pages in all. Set it once a step, before the layers' calls; all of
+    its GPU work belongs on one stream."""
+
+    def __init__(self, cache: PagedKvCache, H: int, max_seqs: int, max_tokens: int, max_pages: int):
+        self.cache, self.H, self.n_tokens = cache, H, 0
+        self._h = C.c_void_p()
+        check(lib().bg_paged_batch_create(cache._h, int(H), int(max_seqs), int(max_tokens), int(max_pages), C.byref(self._h)))
+
+    def set(self, rows, lens, tables, positions=None):
+        """Sequence s holds ``lens[s]`` positions, the last ``rows[s]`` of them new, in the pages
+        ``tables[s]`` (a list of page lists, or a [sequences, n] array of integers; entries past
+        ceil(lens[s] / page_size) are not read). ``positions`` [axes, new rows] (integers): the new
+        tokens' rotary positions, up to four axes; by default their positions in the sequence."""
+        rows, lens = _int32(rows, "rows", 1), _int32(lens, "lens", 1)
+        n = len(rows)
+        if len(lens) != n or len(tables) != n:
+            raise ValueError(f"bitgpu_amd: {n} rows, {len(lens)} lens and {len(tables)} tables")
+        if isinstance(tables, (list, tuple)):
+            lists = [_int32(t, "a table", 1) for t in tables]
+            tables = np.zeros((n, max((len(t) for t in lists), default=0)), np.int32)
+            for s, (t, length) in enumerate(zip(lists, lens)):
+                if len(t) * self.cache.page_size < length:
+                    raise ValueError(f"bitgpu_amd: sequence {s}: {length} positions need more than {len(t)} pages of "
+                                     f"{self.cache.page_size}")
+                tables[s, :len(t)] = t
+        else:
+            tables = _int32(tables, "tables", 2)
+        axes = 1
+        if positions is not None:
+            positions = _int32(positions, "positions", 2)
+            axes, total = positions.shape[0], int(rows.sum(dtype=np.int64))
+            if positions.shape[1] != total:
+                raise ValueError(f"bitgpu_amd: positions of {positions.shape[1]} tokens, the batch has {total} new rows")
+        check(lib().bg_paged_batch_set(self._h, n, rows.ctypes.data, lens.ctypes.data, tables.ctypes.data, tables.shape[1],
+                                       None if positions is None else positions.ctypes.data, axes, _stream()))
+        self.n_tokens = int(rows.sum())
+
+    def info(self) -> dict:
+        """What is set: new rows, the attention's workgroups, runs of shared pages, positions it scans (a
+        shared run's once), rows merged from partials, partials."""
+        out = (C.c_int64 * 6)()
+        check(lib().bg_paged_batch_info(self._h, out))
+        return dict(zip(("rows", "workgroups", "shared_runs", "positions", "merged_rows", "partials"), out))
+
+    def close(self):
+        if self._h:
+            lib().bg_paged_batch_destroy(self._h)
+            self._h = C.c_void_p()
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+    @property
+    def handle(self):
+        return self._h
+
+
+def _int32(x, name, dims):
+    """x (a sequence, array or host tensor of integers) as a contiguous int32 array."""
+    if torch is not None and isinstance(x, torch.Tensor):
+        x = x.numpy()
+    a = np.asarray(x)
+    if a.size == 0 and a.ndim == 1 and dims == 1:
+        return np.zeros(0, np.int32)
+    if a.ndim != dims or a.dtype.kind not in "iu":
+        raise ValueError(f"bitgpu_amd: {name} must hold integers in {dims} dimension{'s' if dims > 1 else ''}")
+    if a.dtype != np.int32:
+        if a.size and (a.max() > 0x7fffffff or a.min() < -0x80000000):
+            raise ValueError(f"bitgpu_amd: {name} exceeds 32 bits")
+        a = a.astype(np.int32)
+    return np.ascontiguousarray(a)
+
+
+def _rows_at_least(t, name, rows, width):
+    """t is f32 and holds `rows` rows of `width` values (more: a padded batch)."""
+    _f32(t, name)
+    if t.numel() < rows * width:
+        raise ValueError(f"bitgpu_amd: {name} holds {t.numel()} values, the batch needs {rows} rows of {width}")
+    return t
+
+
+def paged_qkv_prologue(cache: PagedKvCache, li: int, batch: PagedBatch, q, k, v, q_gamma, k_gamma, eps: float, cos_tab,
+                       sin_tab, rot_dim: int, pair_axis=None, q_stride: int | None = None, q_out=None):
+    """:func:`qkv_prologue` for a batch (bg_paged_qkv_prologue): q [rows, H, q_stride], k and v [rows, KV, D]
+    (any may be None) of the batch's new rows, sequence by sequence; returns the normed and roped q
+    [rows, H, D], with k and v written to their sequences' pages. ``pair_axis`` (rot_dim / 2 integers,
+    needed where the batch was set with several position axes): the axis each rotary pair takes its
+    position from."""
+    D, T, stride = cache.head_dim, batch.n_tokens, int(q_stride or cache.head_dim)
+    cache._one_device(*(t for t in (q, k, v, q_gamma, k_gamma, cos_tab, sin_tab, q_out) if t is not None))
+    for t, nm, rows, width in ((q, "q", T, batch.H * stride), (k, "k", T, cache.kv_heads * D), (v, "v", T, cache.kv_heads * D),
+                               (q_gamma, "q_gamma", 1, D), (k_gamma, "k_gamma", 1, D), (q_out, "q_out", T, batch.H * D)):
+        if t is not None:
+            _rows_at_least(t, nm, rows, width)
+    for t, nm in ((cos_tab, "cos"), (sin_tab, "sin")):
+        if t is not None and (_f32(t, nm).dim() != 2 or 2 * t.shape[1] != rot_dim or t.shape != cos_tab.shape):
+            raise ValueError(f"bitgpu_amd: {nm} must be [positions, rot_dim / 2 = {rot_dim // 2}], got {list(t.shape)}")
+    if q is not None and q_out is None:
+        q_out = q.new_empty((q.numel() // (batch.H * stride), batch.H, D))
+    if pair_axis is not None:
+        pair_axis = np.ascontiguousarray(pair_axis, np.uint8)
+        if pair_axis.shape != (rot_dim // 2,):
+            raise ValueError(f"bitgpu_amd: pair_axis must hold {rot_dim // 2} axes, got shape {list(pair_axis.shape)}")
+    rc = lib().bg_paged_qkv_prologue(cache._h, li, batch._h, _ptr(q), stride, _ptr(k), _ptr(v), _ptr(q_gamma), _ptr(k_gamma),
+                                     float(eps), _ptr(cos_tab), _ptr(sin_tab), cos_tab.shape[0] if cos_tab is not None else 0,
+                                     int(rot_dim), None if pair_axis is None else pair_axis.ctypes.data, _ptr(q_out), _stream())
+    if rc:
+        check(rc)
+    return q_out
+
+
+def paged_attention(cache: PagedKvCache, li: int, batch: PagedBatch, q, scale: float | None = None, gate=None,
+                    gate_stride: int | None = None, out=None):
+    """:func:`attention` for a batch (bg_paged_attention): every new row of q [rows, H, D] over its
+    sequence's pages up to its own position; pages that sequences share are scanned once for all. ``gate``
+    [rows, H, gate_stride] (a view into a wider row, such as the hybrid's query | gate projection, needs its
+    first row's first value at its start). Returns [rows, H, D]; rows beyond the batch's are not written."""
+    D, T = cache.head_dim, batch.n_tokens
+    _rows_at_least(q, "q", T, batch.H * D)
+    if out is None:
+        out = q.new_empty((q.numel() // (batch.H * D), batch.H, D))
+    _rows_at_least(out, "out", T, batch.H * D)
+    gs, gp = 0, None
+    if gate is not None:
+        gs = int(gate_stride if gate_stride is not None else D)
+        _f32(gate, "gate")
+        if not gate.is_cuda:
+            raise ValueError("bitgpu_amd: expected a device (cuda) tensor")
+        # rows [rows, H, D] whose heads are gs values apart, contiguous or a slice of rows of gs values
+        if T and (gate.dim() != 3 or gate.shape[0] < T or gate.shape[1] != batch.H or gate.shape[2] < D or gate.stride(2) != 1
+                  or (gate.stride(1) != gs and batch.H > 1) or (gate.stride(0) != batch.H * gs and gate.shape[0] > 1)):
+            raise ValueError(f"bitgpu_amd: gate must be [rows, {batch.H}, {D}] with heads {gs} values apart, got "
+                             f"{list(gate.shape)} with strides {list(gate.stride())}")
+        gp = gate.data_ptr()
+    cache._one_device(q, out, gate)
+    rc = lib().bg_paged_attention(cache._h, li, batch._h, _ptr(q), float(_dense_scale(D) if scale is None else scale), gp, gs,
+                                  _ptr(out), _stream())
+    if rc:
+        check(rc)
+    return out
+
+
+def paged_layer_attention(cache: PagedKvCache, li: int, batch: PagedBatch, q, k, v, q_norm, k_norm, eps: float, cos_tab,
+                          sin_tab, pair_axis=None):
+    """:func:`layer_attention` for a batch: q/k norm + rope, K/V into the pages, attention. q [rows, H, D],
+    k/v [rows, KV, D] projections; returns att [rows, H, D]."""
+    qr = paged_qkv_prologue(cache, li, batch, q, k, v, q_norm, k_norm, eps, cos_tab, sin_tab, cache.head_dim, pair_axis)
+    return paged_attention(cache, li, batch, qr)
+
+
+def paged_hybrid_attention(cache: PagedKvCache, li: int, batch: PagedBatch, qg, k, v, q_norm, k_norm, eps: float, cos_tab,
+                           sin_tab, rot_dim: int, pair_axis=None):
+    """:func:`hybrid_full_attention` for a batch: qg [rows, H, 2D] (query | gate), partial rope, attention
+    and the sigmoid gate; returns gated [rows, H, D]."""
+    D = cache.head_dim
+    qr = paged_qkv_prologue(cache, li, batch, qg, k, v, q_norm, k_norm, eps, cos_tab, sin_tab, rot_dim, pair_axis, 2 * D)
+    return paged_attention(cache, li, batch, qr, gate=qg.view(-1, batch.H, 2 * D)[..., D:], gate_stride=2 * D)

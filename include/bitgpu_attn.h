@@ -322,6 +322,75 @@ int32_t bg_kv_import_rows(bg_kv_cache* cache, int32_t layer, int32_t region, int
 int32_t bg_kv_save(bg_kv_cache* cache, int32_t base, int32_t count, void* host, size_t bytes, void* stream);
 int32_t bg_kv_load(bg_kv_cache* cache, int32_t base, int32_t count, const void* host, size_t bytes, void* stream);
 
+/* ---- paged KV cache: many sequences in one pool ---------------------------------------------
+ * No counterpart in the reference, whose engine holds one conversation: the same layers for a batch of
+ * conversations. A pool holds, per layer, n_pages pages of page_size positions (32, 64, 128 or 256); a
+ * sequence is a list of pages, and sequences may list the same leading pages (a common system prompt, a
+ * forked conversation), whose keys and values are then stored and, by bg_paged_attention, scanned once.
+ * The memory is the caller's (device, 16-byte aligned), one buffer a region for all layers:
+ *   BG_K       [layer][page][kv_head][slot][head_dim]                     of the storage type
+ *   BG_V       [layer][page][kv_head][slot / 32][4][head_dim][8]          of the storage type: slot
+ *              16 a + 8 c + 4 b + r of a 32-slot tile (a, b, c in 0..1, r in 0..3) at [2 a + b][dim][4 c + r]
+ *   BG_KSCALE, BG_VSCALE (q8) [layer][page][kv_head][slot][head_dim / 32] f32, a value code * scale / 127
+ * It need not be cleared: slots that no call wrote are never used, whatever they hold. Calls are not
+ * re-entrant on one batch, and all GPU work of one batch belongs on ONE stream (its launches share a
+ * workspace and read the arrays that bg_paged_batch_set uploads); batches of one pool may use different
+ * streams where none reads a page that another writes. Every call needs the pool's device current. */
+typedef struct bg_paged_kv bg_paged_kv;
+typedef struct bg_paged_batch bg_paged_batch;
+
+/* Bytes of a pool's region (BG_K, BG_V, BG_KSCALE, BG_VSCALE; the scales of f32 and f16: 0). Host-only. */
+int32_t bg_paged_region_bytes(int32_t n_layers, int32_t kv_heads, int32_t head_dim, int32_t dtype, int32_t page_size,
+                              int32_t n_pages, int32_t region, size_t* bytes);
+/* A pool over the caller's buffers, which outlive it (scales NULL unless q8). head_dim 128 or 256;
+ * n_pages * page_size below 2^31. */
+int32_t bg_paged_create(int32_t n_layers, int32_t kv_heads, int32_t head_dim, int32_t dtype, int32_t page_size,
+                        int32_t n_pages, void* k, void* v, float* k_scale, float* v_scale, bg_paged_kv** out);
+int32_t bg_paged_destroy(bg_paged_kv* kv);
+/* As bg_kv_set_q8_block. */
+int32_t bg_paged_set_q8_block(bg_paged_kv* kv, int32_t block);
+
+/* A batch of at most max_seqs sequences with max_tokens new rows and max_pages listed pages in all, for H
+ * query heads. Allocates its arrays (pinned and device); needs no pool but one of this geometry. */
+int32_t bg_paged_batch_create(const bg_paged_kv* kv, int32_t H, int32_t max_seqs, int32_t max_tokens, int32_t max_pages,
+                              bg_paged_batch** out);
+int32_t bg_paged_batch_destroy(bg_paged_batch* batch);
+/* What the next calls work on (host arrays, read before the call returns): sequence s holds lens[s]
+ * positions, its last rows[s] (0 to lens[s]) new, in the pages tables[s * table_stride ..] (the first
+ * ceil(lens[s] / page_size) are read). The batch's rows are numbered 0 .. sum(rows) - 1, sequence by
+ * sequence. positions: the new tokens' rotary positions [axes][sum(rows)], axes 1 to 4; NULL: their
+ * positions in the sequence. Checks everything (BG_E_INVALID, the batch before stays set), plans the
+ * attention (runs of pages that sequences share are found here) and uploads it on `stream`. May allocate
+ * the workspace of partials; not under graph capture (BG_E_STATE). Launches captured in a graph read the
+ * batch at replay, so a batch may be set between replays: with at most as many new rows as were captured,
+ * the same number of axes and positions inside the captured rope table (else BG_E_STATE). */
+int32_t bg_paged_batch_set(bg_paged_batch* batch, int32_t n_seqs, const int32_t* rows, const int32_t* lens,
+                           const int32_t* tables, int32_t table_stride, const int32_t* positions, int32_t axes, void* stream);
+/* Diagnostic of the batch that is set: out[0..5] = new rows, workgroups of the attention, runs of shared
+ * pages, positions scanned (a shared run's once), rows that are merged from partials, partials. */
+int32_t bg_paged_batch_info(const bg_paged_batch* batch, int64_t* out);
+
+/* bg_qkv_prologue for a batch: its rows' q [rows, H, q_stride], k and v [rows, kv_heads, head_dim] (any
+ * may be NULL); normed and roped q into q_out [rows, H, head_dim], normed and roped k and plain v into
+ * the sequences' pages at the rows' positions, the same bits as bg_qkv_prologue's. pair_axis (host,
+ * rot_dim / 2 entries, NULL where the batch has one axis): which axis of the batch's positions each rotary
+ * pair (dims j and j + rot_dim / 2) takes its angle from, e.g. time, height and width for images, in
+ * sections or interleaved. The tables need rope_positions rows above every position. A page that a
+ * sequence writes must not be listed, with the written positions, by another one or twice (BG_E_INVALID);
+ * rows of q_out and slots beyond the batch's are left as they are. */
+int32_t bg_paged_qkv_prologue(const bg_paged_kv* kv, int32_t layer, bg_paged_batch* batch, const float* q, int32_t q_stride,
+                              const float* k, const float* v, const float* q_gamma, const float* k_gamma, float eps,
+                              const float* cos_tab, const float* sin_tab, int32_t rope_positions, int32_t rot_dim,
+                              const uint8_t* pair_axis, float* q_out, void* stream);
+
+/* bg_attention for a batch: row i of sequence s attends positions 0 .. lens[s] - rows[s] + i of its pages
+ * (what they hold by then, the batch's own rows included). q, out [rows, H, head_dim] f32 (16-byte
+ * aligned, not the same buffer), gate [rows, H, gate_stride] or NULL, out = attn / (1 + exp(-gate)). Results
+ * are f32-accurate for every storage type and do not depend on which other sequences are in the batch
+ * beyond that rounding. Allocates nothing. Rows of out beyond the batch's are left as they are. */
+int32_t bg_paged_attention(const bg_paged_kv* kv, int32_t layer, bg_paged_batch* batch, const float* q, float scale,
+                           const float* gate, int32_t gate_stride, float* out, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
