@@ -71,6 +71,7 @@ struct PagedPlan {
   std::vector<int> v_single;     // tokens whose V row is stored alone
   std::vector<int> v_group;      // first tokens of 16 that fill 16 aligned slots
   int n_tokens = 0, n_parts = 0;
+  int n_many = 0, n_few1 = 0;    // units of 128 rows (the first ones) and of one 16-row set (the last ones)
   int shared_segments = 0;
   int64_t keys = 0;              // positions scanned, a segment's once (a kv head)
   int write_page = -1;           // a page whose new positions another sequence also lists (see below)
@@ -360,7 +361,7 @@ class PagedPlanner {
         if (base_[k.t] >= 0) base_[k.t] += s.chunks;
       }
     }
-    // units, the heaviest first
+    // units by kind (128 rows, two sets, one set), the heaviest first
     cost_.clear();
     for (const Segment& s : segs_) {
       out.keys += s.key1 - s.key0;
@@ -387,8 +388,16 @@ class PagedPlanner {
     }
     order_.resize(out.units.size());
     for (size_t i = 0; i < order_.size(); i++) order_[i] = (int)i;
-    std::stable_sort(order_.begin(), order_.end(), [&](int a, int b) { return cost_[a] > cost_[b]; });
+    auto rank = [&](int i) { return out.units[i].kind == 0 ? 0 : out.units[i].kind == 2 ? 1 : 2; };
+    std::stable_sort(order_.begin(), order_.end(), [&](int a, int b) {
+      return rank(a) != rank(b) ? rank(a) < rank(b) : cost_[a] > cost_[b];
+    });
     sorted_.clear();
+    out.n_many = out.n_few1 = 0;
+    for (int i : order_) {
+      out.n_many += out.units[i].kind == 0;
+      out.n_few1 += out.units[i].kind == 1;
+    }
     for (int i : order_) sorted_.push_back(out.units[i]);
     out.units.swap(sorted_);
   }

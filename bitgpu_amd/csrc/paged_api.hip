@@ -99,6 +99,8 @@ struct bg_paged_batch {
     b.captured = captured;
     if (!captured) {
       b.n_units = (int)plan.units.size();
+      b.n_many = plan.n_many;
+      b.n_few1 = plan.n_few1;
       b.n_merges = (int)plan.merges.size();
       b.n_tokens = plan.n_tokens;
       b.n_v_single = (int)plan.v_single.size();
@@ -339,6 +341,8 @@ int32_t bg_paged_batch_set(bg_paged_batch* b, int32_t n_seqs, const int32_t* row
   char* h = b->host[slot];
   bg::PagedHeader hdr{};
   hdr.n_units = (int)p.units.size();
+  hdr.n_many = p.n_many;
+  hdr.n_few1 = p.n_few1;
   hdr.n_merges = (int)p.merges.size();
   hdr.n_tokens = T;
   hdr.n_v_single = (int)p.v_single.size();

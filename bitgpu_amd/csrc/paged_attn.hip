@@ -61,7 +61,7 @@ struct PagedKernelArgs {
   float qscale;      // scale * log2(e)
   const float* gate; int gate_stride;
   float* out;
-  int n_blocks;      // units * kv heads; 0: read the header
+  int first, n_blocks;  // a launch's first unit and its units * kv heads; n_blocks 0: read the header
 };
 
 __device__ inline float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }
@@ -139,12 +139,6 @@ __device__ inline void store_o(const PagedKernelArgs& p, float* ws_o, const RowA
 // slot of register i (0..7) of lane group g in a 32-slot tile, 16-row matrix products: the V tile's own
 // order (tile_slot)
 __device__ inline int slot16(int g, int i) { return 16 * (g >> 1) + 8 * (i >> 2) + 4 * (g & 1) + (i & 3); }
-
-// a workgroup's LDS: four arrays of the same size
-struct Lds {
-  char *a, *b, *c, *d;
-  __device__ __forceinline__ char* of(int i) const { return i == 0 ? a : i == 1 ? b : i == 2 ? c : d; }
-};
 
 // ------------------------------------------------------------------------------------------ few
 template <int D, int DT>
@@ -225,13 +219,9 @@ __device__ __forceinline__ void few_load_v(const PagedKernelArgs& p, size_t row,
 
 constexpr int kFewPad = 4;  // floats between the LDS rows of the waves' o
 
-// LDS bytes of one wave's rows at the end of a few unit
-template <int D>
-constexpr int few_wave_bytes(int nset) { return 16 * nset * (D + kFewPad) * 4 + 16 * nset * 8; }
-
 template <int D, int DT, int NSET>
 __device__ __forceinline__ void few_unit(const PagedKernelArgs& p, const PagedUnit& u, int kvh, float* ws_o, float2* ws_ml,
-                                         const Lds& lds) {
+                                         float (*lo)[16 * NSET][D + kFewPad], float2 (*lml)[16 * NSET]) {
   constexpr int NK = DT == KV_F32 ? D / 16 : D / 32;
   const int wave = uniform(threadIdx.x >> 6), lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
   const int shift = p.b.page_shift, P = 1 << shift;
@@ -503,19 +493,15 @@ __device__ __forceinline__ void few_unit(const PagedKernelArgs& p, const PagedUn
 
   // ---- the four waves' results meet in LDS
   const float oscale = DT == KV_Q8 ? (vscale == 0.0f ? 0.0f : 1.0f / (127.0f * vscale)) : 1.0f;
-  {
-    float* wo = (float*)lds.of(wave);
-    float2* wml = (float2*)(lds.of(wave) + 16 * NSET * (D + kFewPad) * 4);
 #pragma unroll
-    for (int s = 0; s < NSET; s++) {
-      float2 r = pair16(l[s]);
-      l[s] = r.x + r.y;
-      r = pair32(l[s]);
-      l[s] = r.x + r.y;
-      if (g == 0) wml[16 * s + c] = make_float2(m[s], l[s]);
+  for (int s = 0; s < NSET; s++) {
+    float2 r = pair16(l[s]);
+    l[s] = r.x + r.y;
+    r = pair32(l[s]);
+    l[s] = r.x + r.y;
+    if (g == 0) lml[wave][16 * s + c] = make_float2(m[s], l[s]);
 #pragma unroll
-      for (int j = 0; j < D / 16; j++) *(f32x4*)(wo + (16 * s + c) * (D + kFewPad) + 16 * j + 4 * g) = o[s][j] * oscale;
-    }
+    for (int j = 0; j < D / 16; j++) *(f32x4*)(&lo[wave][16 * s + c][16 * j + 4 * g]) = o[s][j] * oscale;
   }
   __syncthreads();
   for (int x = threadIdx.x; x < u.n_rho * (D / 4); x += 256) {
@@ -523,7 +509,7 @@ __device__ __forceinline__ void few_unit(const PagedKernelArgs& p, const PagedUn
     float mw[4], lw[4], top = -INFINITY;
 #pragma unroll
     for (int w = 0; w < 4; w++) {
-      const float2 ml = ((const float2*)(lds.of(w) + 16 * NSET * (D + kFewPad) * 4))[i];
+      const float2 ml = lml[w][i];
       mw[w] = ml.x;
       lw[w] = ml.y;
       top = fmaxf(top, ml.x);
@@ -534,7 +520,7 @@ __device__ __forceinline__ void few_unit(const PagedKernelArgs& p, const PagedUn
     for (int w = 0; w < 4; w++) {
       const float f = mw[w] == -INFINITY ? 0.0f : exp2_hw(mw[w] - top);
       lsum += lw[w] * f;
-      sum += *(const f32x4*)((const float*)lds.of(w) + i * (D + kFewPad) + d) * f;
+      sum += *(const f32x4*)(&lo[w][i][d]) * f;
     }
     const RowAt r = row_at(p, u, kvh, i);
     store_o<D>(p, ws_o, r, d, sum, lsum);
@@ -620,7 +606,7 @@ __device__ __forceinline__ void many_store_q8(const ManyQ8<D>& r, char* kd, char
 
 template <int D, int DT>
 __device__ __forceinline__ void many_unit(const PagedKernelArgs& p, const PagedUnit& u, int kvh, float* ws_o, float2* ws_ml,
-                                          const Lds& lds, float* scales) {
+                                          char* k0, char* k1, char* v0, char* v1, float* scales) {
   using M = Many<D, DT>;
   constexpr int KT = M::KT, NSUB = M::NSUB;
   constexpr int NK = DT == KV_F32 ? D / 8 : D / 16;   // f32: 16-byte chunks a lane; else 16-dim products
@@ -851,7 +837,7 @@ __device__ __forceinline__ void many_unit(const PagedKernelArgs& p, const PagedU
     __syncthreads();
   };
 
-  // lds.a, lds.b: K of even and odd steps; lds.c, lds.d: V. scales: [step parity][K, V][block][KT]
+  // k0, k1: K of even and odd steps; v0, v1: V. scales: [step parity][K, V][block][KT]
   ManyQ8<D> r8[DT == KV_Q8 ? NSUB : 1];
   auto begin = [&](int st, char* kd, char* vd) __attribute__((always_inline)) {
 #pragma unroll
@@ -881,12 +867,12 @@ __device__ __forceinline__ void many_unit(const PagedKernelArgs& p, const PagedU
     if (more) finish(kn, vn, sn);
   };
   if (n_steps > 0) {
-    begin(0, lds.a, lds.c);
-    finish(lds.a, lds.c, scales);
+    begin(0, k0, v0);
+    finish(k0, v0, scales);
   }
   for (int st = 0; st < n_steps; st += 2) {
-    one(st, lds.a, lds.c, scales, lds.b, lds.d, scales + SC);
-    if (st + 1 < n_steps) one(st + 1, lds.b, lds.d, scales + SC, lds.a, lds.c, scales);
+    one(st, k0, v0, scales, k1, v1, scales + SC);
+    if (st + 1 < n_steps) one(st + 1, k1, v1, scales + SC, k0, v0, scales);
   }
   const float2 r = pair32(l);
   l = r.x + r.y;
@@ -902,40 +888,39 @@ __device__ __forceinline__ void many_unit(const PagedKernelArgs& p, const PagedU
   }
 }
 
+// Kernels: the 128-row units and the few-row units are launches of their own, each with its own registers.
 template <int D, int DT>
-constexpr int lds_array_bytes() {
-  const int many = Many<D, DT>::SUB * Many<D, DT>::NSUB;
-  const int few = few_wave_bytes<D>(DT == KV_F32 ? 1 : 2);
-  return many > few ? many : few;
-}
-
-template <int D, int DT>
-__global__ __launch_bounds__(256, D == 128 ? 2 : 1) void paged_attention_kernel(PagedKernelArgs p) {
+__global__ __launch_bounds__(256, D == 128 ? 2 : 1) void paged_many_kernel(PagedKernelArgs p) {
+  using M = Many<D, DT>;
   // four distinct arrays: a copy into one buffer then cannot alias the reads of another, and the
   // compiler adds no waits between them
-  __shared__ __align__(16) char l0[lds_array_bytes<D, DT>()];
-  __shared__ __align__(16) char l1[lds_array_bytes<D, DT>()];
-  __shared__ __align__(16) char l2[lds_array_bytes<D, DT>()];
-  __shared__ __align__(16) char l3[lds_array_bytes<D, DT>()];
-  __shared__ __align__(16) float scales[DT == KV_Q8 ? 4 * Many<D, DT>::KT * (D / 32) : 4];
-  Lds lds;
-  lds.a = l0;
-  lds.b = l1;
-  lds.c = l2;
-  lds.d = l3;
-  const int total = p.n_blocks ? p.n_blocks : p.b.hdr->n_units * p.kv_heads;
+  __shared__ __align__(16) char k0[M::SUB * M::NSUB];
+  __shared__ __align__(16) char k1[M::SUB * M::NSUB];
+  __shared__ __align__(16) char v0[M::SUB * M::NSUB];
+  __shared__ __align__(16) char v1[M::SUB * M::NSUB];
+  __shared__ __align__(16) float scales[DT == KV_Q8 ? 4 * M::KT * (D / 32) : 4];
+  const int total = p.n_blocks ? p.n_blocks : p.b.hdr->n_many * p.kv_heads;
   float* ws_o = p.b.hdr->ws_o;
   float2* ws_ml = p.b.hdr->ws_ml;
   for (int b = blockIdx.x; b < total; b += gridDim.x) {
     const PagedUnit u = p.b.units[b / p.kv_heads];
-    const int kvh = b % p.kv_heads;
-    if (u.kind == 0) {
-      many_unit<D, DT>(p, u, kvh, ws_o, ws_ml, lds, scales);
-    } else if (DT == KV_F32 || u.kind == 1) {
-      few_unit<D, DT, 1>(p, u, kvh, ws_o, ws_ml, lds);
-    } else {
-      if constexpr (DT != KV_F32) few_unit<D, DT, 2>(p, u, kvh, ws_o, ws_ml, lds);
-    }
+    many_unit<D, DT>(p, u, b % p.kv_heads, ws_o, ws_ml, k0, k1, v0, v1, scales);
+    __syncthreads();  // the unit's LDS is read before the next one's is written
+  }
+}
+
+template <int D, int DT, int NSET>
+__global__ __launch_bounds__(256, D == 128 ? 2 : 1) void paged_few_kernel(PagedKernelArgs p) {
+  __shared__ __align__(16) float lo[4][16 * NSET][D + kFewPad];
+  __shared__ float2 lml[4][16 * NSET];
+  const PagedHeader* h = p.b.hdr;
+  const int first = p.n_blocks ? p.first : NSET == 1 ? h->n_units - h->n_few1 : h->n_many;
+  const int total = p.n_blocks ? p.n_blocks : (NSET == 1 ? h->n_few1 : h->n_units - h->n_few1 - h->n_many) * p.kv_heads;
+  float* ws_o = h->ws_o;
+  float2* ws_ml = h->ws_ml;
+  for (int b = blockIdx.x; b < total; b += gridDim.x) {
+    const PagedUnit u = p.b.units[first + b / p.kv_heads];
+    few_unit<D, DT, NSET>(p, u, b % p.kv_heads, ws_o, ws_ml, lo, lml);
     __syncthreads();  // the unit's LDS is read before the next one's is written
   }
 }
@@ -980,10 +965,27 @@ template <int D, int DT>
 static hipError_t launch_attn(const PagedKernelArgs& k, const PagedAttnArgs& a, hipStream_t st) {
   const PagedBatchView& b = k.b;
   if (!b.captured && b.n_units == 0) return hipSuccess;
-  const long units = (long)b.n_units * k.kv_heads;
-  // under capture a grid that fills the GPU walks the units of whatever batch is set at replay
-  const unsigned grid = b.captured ? (unsigned)(a.num_cus * (D == 128 ? 2 : 1)) : (unsigned)units;
-  hipLaunchKernelGGL((paged_attention_kernel<D, DT>), dim3(grid), dim3(256), 0, st, k);
+  // Under capture a grid that fills the GPU walks the units of whatever batch is set at replay, of every
+  // kind. Units lie by kind: 128 rows, two sets, one set.
+  PagedKernelArgs x = k;
+  const unsigned full = (unsigned)(a.num_cus * (D == 128 ? 2 : 1));
+  if (b.captured || b.n_many) {
+    x.n_blocks = b.n_many * k.kv_heads;
+    hipLaunchKernelGGL((paged_many_kernel<D, DT>), dim3(b.captured ? full : (unsigned)x.n_blocks), dim3(256), 0, st, x);
+  }
+  if constexpr (DT != KV_F32) {
+    const int n2 = b.n_units - b.n_many - b.n_few1;
+    if (b.captured || n2) {
+      x.first = b.n_many;
+      x.n_blocks = n2 * k.kv_heads;
+      hipLaunchKernelGGL((paged_few_kernel<D, DT, 2>), dim3(b.captured ? full : (unsigned)x.n_blocks), dim3(256), 0, st, x);
+    }
+  }
+  if (b.captured || b.n_few1) {
+    x.first = b.n_units - b.n_few1;
+    x.n_blocks = b.n_few1 * k.kv_heads;
+    hipLaunchKernelGGL((paged_few_kernel<D, DT, 1>), dim3(b.captured ? full : (unsigned)x.n_blocks), dim3(256), 0, st, x);
+  }
   if (b.captured || b.n_merges) {
     const long rows = (long)b.n_merges * b.H;
     const unsigned mgrid = b.captured ? (unsigned)(a.num_cus * 4) : (unsigned)((rows + 3) / 4);
@@ -1014,7 +1016,7 @@ hipError_t launch_paged_attention(const LayerView& pool, const PagedBatchView& b
   k.gate = a.gate;
   k.gate_stride = a.gate_stride;
   k.out = a.out;
-  k.n_blocks = b.captured ? 0 : b.n_units * pool.kv_heads;
+  k.first = k.n_blocks = 0;
   return pool.D == 128 ? launch_attn_d<128>(pool, k, a, st) : launch_attn_d<256>(pool, k, a, st);
 }
 
