@@ -70,7 +70,7 @@ struct PagedPlan {
   std::vector<int> dst;          // per token: page * page size + slot
   std::vector<int> v_single;     // tokens whose V row is stored alone
   std::vector<int> v_group;      // first tokens of 16 that fill 16 aligned slots
-  int n_tokens = 0, n_parts = 0;
+  int n_tokens = 0, n_parts = 0, most_parts = 0;  // partials in all and of one row at most
   int n_many = 0, n_few1 = 0;    // units of 128 rows (the first ones) and of one 16-row set (the last ones)
   int shared_segments = 0;
   int64_t keys = 0;              // positions scanned, a segment's once (a kv head)
@@ -344,9 +344,11 @@ class PagedPlanner {
       for (int i = 0; i < s.n_tok; i++) count_[out.toks[s.tok + i].t] += s.chunks;
     base_.assign(out.n_tokens, 0);
     int parts = 0;
+    out.most_parts = 0;
     for (int t = 0; t < out.n_tokens; t++) {
       if (count_[t] > 1) {
         out.merges.push_back(PagedMerge{t, parts, count_[t], 0});
+        out.most_parts = std::max(out.most_parts, count_[t]);
         base_[t] = parts;
         parts += count_[t];
       } else {

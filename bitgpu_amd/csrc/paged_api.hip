@@ -102,6 +102,7 @@ struct bg_paged_batch {
       b.n_many = plan.n_many;
       b.n_few1 = plan.n_few1;
       b.n_merges = (int)plan.merges.size();
+      b.most_parts = plan.most_parts;
       b.n_tokens = plan.n_tokens;
       b.n_v_single = (int)plan.v_single.size();
       b.n_v_group = (int)plan.v_group.size();
@@ -343,6 +344,7 @@ int32_t bg_paged_batch_set(bg_paged_batch* b, int32_t n_seqs, const int32_t* row
   hdr.n_units = (int)p.units.size();
   hdr.n_many = p.n_many;
   hdr.n_few1 = p.n_few1;
+  hdr.most_parts = p.most_parts;
   hdr.n_merges = (int)p.merges.size();
   hdr.n_tokens = T;
   hdr.n_v_single = (int)p.v_single.size();

@@ -925,38 +925,80 @@ __global__ __launch_bounds__(256, D == 128 ? 2 : 1) void paged_few_kernel(PagedK
   }
 }
 
-// A row's partials joined: a wave a (token, head), D / 64 dims a lane.
+// lane groups that share a row's partials
+__host__ __device__ inline int merge_groups(int most_parts) { return most_parts <= 8 ? 1 : 4; }
+
+// A row's partials joined. D / 4 lanes hold a partial's row (16 bytes a lane); PP lane groups a row take
+// every PP-th partial, eight at a time, all loaded before any is used (a row of 55 partials: two rounds of
+// memory latency instead of 55), and meet in LDS. PP is 1 where no row has more than eight, else 4: the
+// same for a replay as for a call, so both give the same bits.
 template <int D>
-__global__ __launch_bounds__(256) void paged_merge_kernel(PagedKernelArgs p, int n_merges) {
-  constexpr int E = D / 64;
-  const int lane = threadIdx.x & 63;
-  const int n = n_merges ? n_merges : p.b.hdr->n_merges;
+__global__ __launch_bounds__(256) void paged_merge_kernel(PagedKernelArgs p, int n_merges, int most_parts) {
+  constexpr int LPR = D / 4, N = 8, MAXP = 4;
+  __shared__ f32x4 lo[256 / (LPR * MAXP)][MAXP][LPR];
+  __shared__ float2 lml[256 / (LPR * MAXP)][MAXP];
+  const int PP = merge_groups(n_merges ? most_parts : p.b.hdr->most_parts), RPW = 256 / (LPR * PP);
+  const int c = threadIdx.x % LPR, g = threadIdx.x / LPR % PP, rw = threadIdx.x / (LPR * PP);
+  const int H = p.b.H;
+  const long total = (long)(n_merges ? n_merges : p.b.hdr->n_merges) * H;
   const float* ws_o = p.b.hdr->ws_o;
   const float2* ws_ml = p.b.hdr->ws_ml;
-  for (long x = (long)blockIdx.x * 4 + uniform(threadIdx.x >> 6); x < (long)n * p.b.H; x += (long)gridDim.x * 4) {
-    const PagedMerge mg = p.b.merges[x / p.b.H];
-    const int head = (int)(x % p.b.H);
-    float top = -INFINITY, lsum = 0.0f;
-    for (int i = lane; i < mg.n; i += 64) top = fmaxf(top, ws_ml[(size_t)(mg.part + i) * p.b.H + head].x);
-    top = wave_max(top);
-    float acc[E];
+  for (long first = (long)blockIdx.x * RPW; first < total; first += (long)gridDim.x * RPW) {
+    const long x = min(first + rw, total - 1);  // past the end: the last row again, not stored
+    const PagedMerge mg = p.b.merges[x / H];
+    const int head = (int)(x % H);
+    float m = -INFINITY, l = 0.0f;
+    f32x4 acc = {0, 0, 0, 0};
+    for (int i0 = g; i0 < mg.n; i0 += N * PP) {
+      f32x4 o[N];
+      float2 ml[N];
+      float top = m;
 #pragma unroll
-    for (int e = 0; e < E; e++) acc[e] = 0.0f;
-    for (int i = 0; i < mg.n; i++) {
-      const size_t row = (size_t)(mg.part + i) * p.b.H + head;
-      const float2 ml = ws_ml[row];
-      const float f = ml.x == -INFINITY ? 0.0f : exp2_hw(ml.x - top);
-      lsum += ml.y * f;
+      for (int u = 0; u < N; u++) {
+        const size_t row = (size_t)(mg.part + min(i0 + u * PP, mg.n - 1)) * H + head;
+        ml[u] = ws_ml[row];
+        o[u] = *(const f32x4*)(ws_o + row * D + 4 * c);
+      }
 #pragma unroll
-      for (int e = 0; e < E; e++) acc[e] += ws_o[row * D + lane * E + e] * f;
+      for (int u = 0; u < N; u++) {
+        if (i0 + u * PP >= mg.n) ml[u] = make_float2(-INFINITY, 0.0f);
+        top = fmaxf(top, ml[u].x);
+      }
+      const float f0 = m == -INFINITY ? 0.0f : exp2_hw(m - top);
+      l *= f0;
+      acc *= f0;
+#pragma unroll
+      for (int u = 0; u < N; u++) {
+        const float f = ml[u].x == -INFINITY ? 0.0f : exp2_hw(ml[u].x - top);
+        l += ml[u].y * f;
+        if (ml[u].x != -INFINITY) acc += o[u] * f;  // an empty part's o is zero, a padding one's any row's
+      }
+      m = top;
     }
-    const size_t row = (size_t)mg.t * p.b.H + head;
-    const float inv = 1.0f / lsum;
+    if (PP > 1) {
+      lo[rw][g][c] = acc;
+      if (c == 0) lml[rw][g] = make_float2(m, l);
+      __syncthreads();
+      float top = -INFINITY;
 #pragma unroll
-    for (int e = 0; e < E; e++) {
-      float v = acc[e] * inv;
-      if (p.gate) v = v / (1.0f + __expf(-p.gate[row * p.gate_stride + lane * E + e]));
-      p.out[row * D + lane * E + e] = v;
+      for (int i = 0; i < MAXP; i++) top = fmaxf(top, lml[rw][i].x);
+      l = 0.0f;
+      acc = f32x4{0, 0, 0, 0};
+#pragma unroll
+      for (int i = 0; i < MAXP; i++) {
+        const float2 ml = lml[rw][i];
+        const float f = ml.x == -INFINITY ? 0.0f : exp2_hw(ml.x - top);
+        l += ml.y * f;
+        acc += lo[rw][i][c] * f;
+      }
+      __syncthreads();
+    }
+    if (g == 0 && first + rw < total) {
+      RowAt r;
+      r.t = mg.t;
+      r.head = head;
+      r.part = -1;
+      store_o<D>(p, nullptr, r, 4 * c, acc, l);
     }
   }
 }
@@ -987,9 +1029,9 @@ static hipError_t launch_attn(const PagedKernelArgs& k, const PagedAttnArgs& a, 
     hipLaunchKernelGGL((paged_few_kernel<D, DT, 1>), dim3(b.captured ? full : (unsigned)x.n_blocks), dim3(256), 0, st, x);
   }
   if (b.captured || b.n_merges) {
-    const long rows = (long)b.n_merges * b.H;
-    const unsigned mgrid = b.captured ? (unsigned)(a.num_cus * 4) : (unsigned)((rows + 3) / 4);
-    hipLaunchKernelGGL((paged_merge_kernel<D>), dim3(mgrid), dim3(256), 0, st, k, b.captured ? 0 : b.n_merges);
+    const int rpw = 256 / (D / 4 * merge_groups(b.most_parts));
+    const unsigned grid = b.captured ? (unsigned)(a.num_cus * 4) : (unsigned)(((long)b.n_merges * b.H + rpw - 1) / rpw);
+    hipLaunchKernelGGL((paged_merge_kernel<D>), dim3(grid), dim3(256), 0, st, k, b.captured ? 0 : b.n_merges, b.most_parts);
   }
   return hipGetLastError();
 }
