@@ -18,7 +18,7 @@ namespace bg {
 // replays is the one the replay runs.
 struct PagedHeader {
   int n_units, n_merges, n_tokens, n_v_single, n_v_group;
-  int n_many, n_few1, most_parts;  // units of 128 rows (the first ones) and of one 16-row set (the last ones)
+  int n_many, n_merge_few, pad;  // units of 128 rows and merges of few partials (the first ones)
   float* ws_o;      // [part][head][D] unnormalized output of a partial
   float2* ws_ml;    // [part][head] its (m, l), m in base 2
 };
@@ -38,7 +38,7 @@ struct PagedBatchView {
   int page_shift;
   int H, G;
   // the set counts; all zero for a launch under capture, which reads hdr
-  int n_units, n_many, n_few1, n_merges, most_parts, n_tokens, n_v_single, n_v_group;
+  int n_units, n_many, n_merges, n_merge_few, n_tokens, n_v_single, n_v_group;
   int captured;
 };
 

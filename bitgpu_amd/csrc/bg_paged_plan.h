@@ -25,8 +25,8 @@ namespace bg {
 // One workgroup's attention work, for every kv head. Positions [key0, key1) (key0 a multiple of 32) of
 // the page list at pages[table]; rows rho0 .. rho0 + n_rho - 1 of the tokens at toks[tok].
 struct PagedUnit {
-  int kind;    // 16-row sets a wave holds (1, 2), its four waves splitting the positions; 0: 128 rows,
-               // 32 a wave, the positions staged through LDS for all four
+  int kind;    // 1: 16 rows, the four waves splitting the positions; 0: 128 rows, 32 a wave, the positions
+               // staged through LDS for all four
   int tok;
   int rho0, n_rho;
   int table;
@@ -45,6 +45,8 @@ struct PagedMerge {
   int t, part, n, pad;
 };
 
+constexpr int kMergeFew = 8;
+
 struct PagedShape {
   int kv_heads, G, D, dtype, page, n_pages;
   int cus;
@@ -53,7 +55,7 @@ struct PagedShape {
   // shared segments on one sequence's path at most (what is below them stays private)
   static constexpr int kLevels = 4;
   int max_toks() const { return max_tokens * (kLevels + 1); }
-  // units: a segment's row tiles unsplit (2 at most where they are fewer than 128 rows), and what a
+  // units: a segment's row tiles unsplit (2 at most past the whole 128-row tiles), and what a
   // split adds, up to 8 units a CU
   long max_units() const {
     return (long)max_toks() * G / 128 + 2L * (2L * max_seqs) + 8L * cus;
@@ -70,8 +72,9 @@ struct PagedPlan {
   std::vector<int> dst;          // per token: page * page size + slot
   std::vector<int> v_single;     // tokens whose V row is stored alone
   std::vector<int> v_group;      // first tokens of 16 that fill 16 aligned slots
-  int n_tokens = 0, n_parts = 0, most_parts = 0;  // partials in all and of one row at most
-  int n_many = 0, n_few1 = 0;    // units of 128 rows (the first ones) and of one 16-row set (the last ones)
+  int n_tokens = 0, n_parts = 0;
+  int n_merge_few = 0;           // merges of at most kMergeFew partials (the first ones)
+  int n_many = 0;                // units of 128 rows (the first ones)
   int shared_segments = 0;
   int64_t keys = 0;              // positions scanned, a segment's once (a kv head)
   int write_page = -1;           // a page whose new positions another sequence also lists (see below)
@@ -302,38 +305,84 @@ class PagedPlanner {
     }
   }
 
-  // rows of one unit of a segment
-  int tile_rows(const Segment& s) const {
-    if (s.rows > 32) return 128;
-    return s.rows > 16 && sh_.dtype != 0 ? 32 : 16;
-  }
-  // The work of a row tile over 32 positions, in 1/8 us of a workgroup with the GPU full: the few-row
-  // kinds move the positions' bytes, the 128-row kind runs the matrix products.
-  int weight(const Segment& s) const {
-    if (s.rows <= 32) return sh_.dtype == 0 ? 22 : sh_.dtype == 1 ? 11 : 8;
-    return sh_.dtype == 0 ? 56 : sh_.dtype == 1 ? 8 : 12;
+  static constexpr int kFewRows = 32;  // rows up to which few-row units take a segment, or a tile's rest
+  // a segment's units: 0 of 128 rows, 1 of 16
+  int kind(const Segment& s) const { return s.rows > kFewRows ? 0 : 1; }
+  int n_tiles(const Segment& s) const {
+    const int rest = s.rows % 128;
+    return s.rows / 128 + (rest > kFewRows ? 1 : (rest + 15) / 16);
   }
 
+  // those of the segment's own kind: without a 128-row segment's few-row rest
+  int own_tiles(const Segment& s) const { return kind(s) ? n_tiles(s) : s.rows / 128 + (s.rows % 128 > kFewRows ? 1 : 0); }
+  // a segment's 32-position tiles
+  static int tiles(const Segment& s) { return (s.key1 - s.key0 + 31) / 32; }
+  static void cut(Segment& s, long len) {
+    s.chunks = (int)((tiles(s) + len - 1) / len);
+    s.chunk_len = ((tiles(s) + s.chunks - 1) / s.chunks + 1) & ~1;  // even: 64 positions a step
+    s.chunks = (tiles(s) + s.chunk_len - 1) / s.chunk_len;
+  }
+
+  // Chunk lengths, by kind (each is a launch): the candidate with the least estimated time, in us, from
+  // what the kernels measure. A launch of no more units than workgroup slots takes its longest unit, one
+  // of more the slots' share of the work and half a unit for the uneven end. A unit costs its start (its
+  // descriptor, rows and queries come one after the other) and its tiles; every row of a split or shared
+  // segment a partial a chunk, written and read.
   void chunk() {
-    const int per_cu = sh_.D == 128 ? 2 : 1;
-    const long slots = std::max(1L, (long)sh_.cus * per_cu);
-    double total = 0;
-    for (Segment& s : segs_) {
-      const int tiles = (s.key1 - s.key0 + 31) / 32, n = (s.rows + tile_rows(s) - 1) / tile_rows(s);
-      total += (double)tiles * n * weight(s) * sh_.kv_heads * (s.shared ? 1.0 : 0.5 + 0.5 * s.key0 / s.key1);
-    }
-    // half a workgroup slot's share of the work a unit, and as many units as the arrays hold
-    for (double share = total / slots / 2;; share = 2 * share + 64) {
-      long units = 0;
-      for (Segment& s : segs_) {
-        const int tiles = (s.key1 - s.key0 + 31) / 32, n = (s.rows + tile_rows(s) - 1) / tile_rows(s);
-        const long len = std::max(s.rows <= 32 ? 4L : 8L, (long)(share / weight(s)));
-        s.chunks = (int)((tiles + len - 1) / len);
-        s.chunk_len = ((tiles + s.chunks - 1) / s.chunks + 1) & ~1;
-        s.chunks = (tiles + s.chunk_len - 1) / s.chunk_len;
-        units += (long)s.chunks * n;
+    for (int kd = 0; kd < 2; kd++) {
+      const bool many = kd == 0;
+      // a 32-position tile of a 128-row unit, two workgroups a CU at head_dim 128 (one alone 1.26 / 2.5 /
+      // 4.7) and one at 256; of a few-row unit, all slots at work at 5.6 TB/s, and alone
+      static const double kMany[2][3] = {{9.3, 2.1, 3.55}, {11.2, 2.5, 5.3}};
+      const int wide = sh_.D == 256;
+      const int per_cu = many ? (wide ? 1 : 2) : sh_.dtype == 0 ? (wide ? 1 : 2) : wide ? 2 : 3;
+      const double slots = std::max(1.0, (double)sh_.cus * per_cu);
+      const double full = many ? kMany[wide][sh_.dtype] : 2.0 * (sh_.D / 32) * paged_bytes32(sh_.dtype) * 32 * slots / 5.6e6;
+      const double alone = many ? (wide ? full : full * (sh_.dtype == 0 ? 0.5 : sh_.dtype == 1 ? 0.6 : 0.7)) : 0.5;
+      const double start = many ? 6 : 5;
+      double work = 0;
+      long longest = 1, tiles1 = 0;
+      for (const Segment& s : segs_) {
+        if (kind(s) != kd) continue;
+        work += (s.shared ? tiles(s) : tiles(s) - s.n_tok / 64.0) * own_tiles(s) * sh_.kv_heads;
+        longest = std::max(longest, (long)tiles(s));
+        tiles1 += own_tiles(s);
       }
+      if (tiles1 == 0) continue;
+      double best = 1e30;
+      long best_len = longest;
+      for (long len = many && !wide ? 8 : 4; len < 2 * longest; len = len * 9 / 8 + 1) {
+        double units = 0, rows = 0;
+        long most = 1;
+        for (Segment& s : segs_) {
+          if (kind(s) != kd) continue;
+          cut(s, len);
+          units += (double)s.chunks * own_tiles(s) * sh_.kv_heads;
+          if (s.chunks > 1 || s.shared) rows += (double)s.chunks * s.rows * sh_.kv_heads;
+          most = std::max(most, (long)std::min(s.chunk_len, tiles(s)));
+        }
+        double t;
+        if (units <= slots) {
+          const double rate = many ? (units * per_cu <= slots ? alone : full) : std::max(alone, full * units / slots);
+          t = start + most * rate;
+        } else {
+          t = work * full / slots + start * (1 + units / slots) + (many ? 0.5 : 0.15) * most * full;
+        }
+        t += rows * (sh_.D + 2) * 4 * (1 / 5.0e6 + 1 / 4.0e6);
+        if (t < best) {
+          best = t;
+          best_len = len;
+        }
+      }
+      for (Segment& s : segs_)
+        if (kind(s) == kd) cut(s, best_len);
+    }
+    // as many units as the arrays hold
+    for (;;) {
+      long units = 0;
+      for (const Segment& s : segs_) units += (long)s.chunks * n_tiles(s);
       if (units <= sh_.max_units()) return;
+      for (Segment& s : segs_) cut(s, 2L * s.chunk_len);
     }
   }
 
@@ -343,18 +392,19 @@ class PagedPlanner {
     for (const Segment& s : segs_)
       for (int i = 0; i < s.n_tok; i++) count_[out.toks[s.tok + i].t] += s.chunks;
     base_.assign(out.n_tokens, 0);
+    // rows of at most eight partials first: the merge kernel takes the two groups differently
     int parts = 0;
-    out.most_parts = 0;
+    out.n_merge_few = 0;
     for (int t = 0; t < out.n_tokens; t++) {
-      if (count_[t] > 1) {
-        out.merges.push_back(PagedMerge{t, parts, count_[t], 0});
-        out.most_parts = std::max(out.most_parts, count_[t]);
-        base_[t] = parts;
-        parts += count_[t];
-      } else {
-        base_[t] = -1;
-      }
+      base_[t] = -1;
+      if (count_[t] < 2) continue;
+      base_[t] = parts;
+      parts += count_[t];
+      if (count_[t] <= kMergeFew) out.merges.push_back(PagedMerge{t, base_[t], count_[t], 0});
     }
+    out.n_merge_few = (int)out.merges.size();
+    for (int t = 0; t < out.n_tokens; t++)
+      if (count_[t] > kMergeFew) out.merges.push_back(PagedMerge{t, base_[t], count_[t], 0});
     out.n_parts = parts;
     for (const Segment& s : segs_) {
       for (int i = 0; i < s.n_tok; i++) {
@@ -363,15 +413,17 @@ class PagedPlanner {
         if (base_[k.t] >= 0) base_[k.t] += s.chunks;
       }
     }
-    // units by kind (128 rows, two sets, one set), the heaviest first
+    // units by kind (128 rows, 16 rows), the heaviest first
     cost_.clear();
     for (const Segment& s : segs_) {
       out.keys += s.key1 - s.key0;
-      const int R = tile_rows(s);
       for (int c = 0; c < s.chunks; c++) {
-        for (int r0 = 0; r0 < s.rows; r0 += R) {
+        for (int r0 = 0, R; r0 < s.rows; r0 += R) {
+          // what 128-row tiles leave over runs as few-row units where it is that few
+          const bool many = s.rows - r0 > kFewRows;
+          R = many ? 128 : 16;
           PagedUnit u{};
-          u.kind = R / 16 > 2 ? 0 : R / 16;
+          u.kind = many ? 0 : 1;
           u.tok = s.tok;
           u.rho0 = r0;
           u.n_rho = std::min(R, s.rows - r0);
@@ -384,22 +436,19 @@ class PagedPlanner {
           if (u.key1 < u.key0) u.key1 = u.key0;
           u.mask0 = s.shared ? s.key1 : lo + 1;
           out.units.push_back(u);
-          cost_.push_back((long)((u.key1 - u.key0 + 31) / 32) * weight(s));
+          cost_.push_back((u.key1 - u.key0 + 31) / 32);
         }
       }
     }
     order_.resize(out.units.size());
     for (size_t i = 0; i < order_.size(); i++) order_[i] = (int)i;
-    auto rank = [&](int i) { return out.units[i].kind == 0 ? 0 : out.units[i].kind == 2 ? 1 : 2; };
     std::stable_sort(order_.begin(), order_.end(), [&](int a, int b) {
-      return rank(a) != rank(b) ? rank(a) < rank(b) : cost_[a] > cost_[b];
+      const int ka = out.units[a].kind, kb = out.units[b].kind;
+      return ka != kb ? ka < kb : cost_[a] > cost_[b];
     });
     sorted_.clear();
-    out.n_many = out.n_few1 = 0;
-    for (int i : order_) {
-      out.n_many += out.units[i].kind == 0;
-      out.n_few1 += out.units[i].kind == 1;
-    }
+    out.n_many = 0;
+    for (int i : order_) out.n_many += out.units[i].kind == 0;
     for (int i : order_) sorted_.push_back(out.units[i]);
     out.units.swap(sorted_);
   }

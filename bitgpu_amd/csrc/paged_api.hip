@@ -100,9 +100,8 @@ struct bg_paged_batch {
     if (!captured) {
       b.n_units = (int)plan.units.size();
       b.n_many = plan.n_many;
-      b.n_few1 = plan.n_few1;
       b.n_merges = (int)plan.merges.size();
-      b.most_parts = plan.most_parts;
+      b.n_merge_few = plan.n_merge_few;
       b.n_tokens = plan.n_tokens;
       b.n_v_single = (int)plan.v_single.size();
       b.n_v_group = (int)plan.v_group.size();
@@ -343,8 +342,7 @@ int32_t bg_paged_batch_set(bg_paged_batch* b, int32_t n_seqs, const int32_t* row
   bg::PagedHeader hdr{};
   hdr.n_units = (int)p.units.size();
   hdr.n_many = p.n_many;
-  hdr.n_few1 = p.n_few1;
-  hdr.most_parts = p.most_parts;
+  hdr.n_merge_few = p.n_merge_few;
   hdr.n_merges = (int)p.merges.size();
   hdr.n_tokens = T;
   hdr.n_v_single = (int)p.v_single.size();

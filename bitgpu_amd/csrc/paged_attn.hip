@@ -20,8 +20,8 @@
 //   p       2^(s - m + 8), m raised only when a tile's maximum passes it by 6 (most tiles skip the
 //           rescale): p <= 2^14 stays below f16's 65504, and the smallest f16 step is 2^-32 of the
 //           largest p;
-//   q8 V    p is multiplied by the block scale of its position, over a power of two 2^ev that is at least
-//           every scale so far (raised like m).
+//   q8 V    p is multiplied by the block scale of its position; its exponent is lowered by ev, 2^ev above
+//           every scale so far (raised like m), so that the products stay as small.
 // S^T = K Q^T and O^T += V^T P^T: the score registers of a lane hold positions of one row, in exactly the
 // order in which the V tile stores them (bg_common.h), so P enters the second product as it lies.
 // Masked positions: scores are replaced, not added to; V beyond the positions written so far (a page's
@@ -67,13 +67,30 @@ struct PagedKernelArgs {
 __device__ inline float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }
 __device__ inline int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
 
+// x less the low (high) half of h: one mixed-precision fma, exact
+__device__ inline float less_lo(float x, uint32_t h) {
+  float r;
+  asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel_hi:[1,0,0]" : "=v"(r) : "v"(h), "v"(x));
+  return r;
+}
+__device__ inline float less_hi(float x, uint32_t h) {
+  float r;
+  asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(r) : "v"(h), "v"(x));
+  return r;
+}
+
 // x[0..7] as hi and lo f16 parts (each conversion truncates; lo holds what hi lost)
 __device__ inline void split8(const float (&x)[8], H8& hi, H8& lo) {
 #pragma unroll
   for (int i = 0; i < 4; i++) {
     hi.p[i] = __builtin_amdgcn_cvt_pkrtz(x[2 * i], x[2 * i + 1]);
-    lo.p[i] = __builtin_amdgcn_cvt_pkrtz(x[2 * i] - (float)hi.e[2 * i], x[2 * i + 1] - (float)hi.e[2 * i + 1]);
+    lo.p[i] = __builtin_amdgcn_cvt_pkrtz(less_lo(x[2 * i], hi.u[i]), less_hi(x[2 * i + 1], hi.u[i]));
   }
+}
+
+// A power of two 2^e above every q8 value scale up to `big` (zero and NaN: the least one kept)
+__device__ inline float scale_exponent(float big) {
+  return (float)(min(max((int)((__float_as_uint(big) >> 23) & 0xff) - 126, -60), 60));
 }
 
 // 2^e with 2^e * top in [2^10, 2^11) for a row's largest |value|; 1 for zero, infinite and NaN rows
@@ -140,395 +157,7 @@ __device__ inline void store_o(const PagedKernelArgs& p, float* ws_o, const RowA
 // order (tile_slot)
 __device__ inline int slot16(int g, int i) { return 16 * (g >> 1) + 8 * (i >> 2) + 4 * (g & 1) + (i & 3); }
 
-// ------------------------------------------------------------------------------------------ few
-template <int D, int DT>
-struct FewK {  // a lane's K operand of a 32-slot tile
-  static constexpr int N = DT == KV_F32 ? 2 * (D / 16) : 2 * (D / 32);
-  f32x4 f[DT == KV_F32 ? N : 1];
-  u32x4 h[DT == KV_F16 ? N : 1];
-  u32x2 c[DT == KV_Q8 ? N : 1];
-  f32x4 s[DT == KV_Q8 ? 8 * (D / 128) : 1];
-};
-template <int D, int DT>
-struct FewV {
-  static constexpr int N = D / 16;
-  f32x4 f[DT == KV_F32 ? 2 * N : 1];
-  u32x4 h[DT == KV_F16 ? N : 1];
-  u32x2 c[DT == KV_Q8 ? N : 1];
-  f32x4 s[DT == KV_Q8 ? 8 * (D / 128) : 1];
-};
-
-template <int D, int DT>
-__device__ __forceinline__ void few_load_k(const PagedKernelArgs& p, size_t row, int c, int g, FewK<D, DT>& k) {
-  // operand row c of product i is slot slot16(c / 4, 4 i + c % 4); the k dimension of a lane group is
-  // 8 g + e of every 32 dims (f32: 4 g + e of every 16)
-  const int s0 = 16 * (c >> 3) + 4 * ((c >> 2) & 1) + (c & 3);
-  if constexpr (DT == KV_F32) {
-    const float* b = (const float*)p.k + row * D + (size_t)s0 * D + 4 * g;
-#pragma unroll
-    for (int i = 0; i < 2; i++)
-#pragma unroll
-      for (int j = 0; j < D / 16; j++) k.f[i * (D / 16) + j] = *(const f32x4*)(b + 8 * i * D + 16 * j);
-  } else if constexpr (DT == KV_F16) {
-    const _Float16* b = (const _Float16*)p.k + row * D + (size_t)s0 * D + 8 * g;
-#pragma unroll
-    for (int i = 0; i < 2; i++)
-#pragma unroll
-      for (int j = 0; j < D / 32; j++) k.h[i * (D / 32) + j] = *(const u32x4*)(b + 8 * i * D + 32 * j);
-  } else {
-    const int8_t* b = (const int8_t*)p.k + row * D + (size_t)s0 * D + 8 * g;
-#pragma unroll
-    for (int i = 0; i < 2; i++)
-#pragma unroll
-      for (int j = 0; j < D / 32; j++) k.c[i * (D / 32) + j] = *(const u32x2*)(b + 8 * i * D + 32 * j);
-    // the scales of the 8 slots this lane's scores are of
-    const float* sc = p.ks + (row + slot16(g, 0)) * (D / 32);
-#pragma unroll
-    for (int e = 0; e < 8; e++)
-#pragma unroll
-      for (int j = 0; j < D / 128; j++)
-        k.s[e * (D / 128) + j] = *(const f32x4*)(sc + (size_t)(8 * (e >> 2) + (e & 3)) * (D / 32) + 4 * j);
-  }
-}
-
-template <int D, int DT>
-__device__ __forceinline__ void few_load_v(const PagedKernelArgs& p, size_t row, int c, int g, FewV<D, DT>& v) {
-  if constexpr (DT == KV_F32) {
-    const float* b = (const float*)p.v + row * D + (size_t)(g * D + c) * 8;
-#pragma unroll
-    for (int j = 0; j < D / 16; j++) {
-      v.f[2 * j] = *(const f32x4*)(b + 128 * j);
-      v.f[2 * j + 1] = *(const f32x4*)(b + 128 * j + 4);
-    }
-  } else if constexpr (DT == KV_F16) {
-    const _Float16* b = (const _Float16*)p.v + row * D + (size_t)(g * D + c) * 8;
-#pragma unroll
-    for (int j = 0; j < D / 16; j++) v.h[j] = *(const u32x4*)(b + 128 * j);
-  } else {
-    const int8_t* b = (const int8_t*)p.v + row * D + (size_t)(g * D + c) * 8;
-#pragma unroll
-    for (int j = 0; j < D / 16; j++) v.c[j] = *(const u32x2*)(b + 128 * j);
-    const float* sc = p.vs + (row + slot16(g, 0)) * (D / 32);
-#pragma unroll
-    for (int e = 0; e < 8; e++)
-#pragma unroll
-      for (int j = 0; j < D / 128; j++)
-        v.s[e * (D / 128) + j] = *(const f32x4*)(sc + (size_t)(8 * (e >> 2) + (e & 3)) * (D / 32) + 4 * j);
-  }
-}
-
-constexpr int kFewPad = 4;  // floats between the LDS rows of the waves' o
-
-template <int D, int DT, int NSET>
-__device__ __forceinline__ void few_unit(const PagedKernelArgs& p, const PagedUnit& u, int kvh, float* ws_o, float2* ws_ml,
-                                         float (*lo)[16 * NSET][D + kFewPad], float2 (*lml)[16 * NSET]) {
-  constexpr int NK = DT == KV_F32 ? D / 16 : D / 32;
-  const int wave = uniform(threadIdx.x >> 6), lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
-  const int shift = p.b.page_shift, P = 1 << shift;
-  const int n_tiles = (u.key1 - u.key0 + 31) >> 5;
-  const int* pages = p.b.pages + u.table;
-
-  // ---- the queries
-  int pos[NSET];
-  float qs[NSET];
-  H8 qh[NSET][DT == KV_F32 ? 1 : NK], ql[NSET][DT == KV_F32 ? 1 : NK];
-  f32x4 qf[NSET][DT == KV_F32 ? NK : 1];
-#pragma unroll
-  for (int s = 0; s < NSET; s++) {
-    const int i = 16 * s + c;
-    const bool on = i < u.n_rho;
-    const int rho = u.rho0 + (on ? i : 0);
-    const int j = rho / p.b.G;
-    const PagedTok tok = p.b.toks[u.tok + j];
-    pos[s] = tok.pos;
-    const float* q = p.q + ((size_t)tok.t * p.b.H + kvh * p.b.G + rho - j * p.b.G) * D;
-    if constexpr (DT == KV_F32) {
-#pragma unroll
-      for (int n = 0; n < NK; n++) qf[s][n] = *(const f32x4*)(q + 16 * n + 4 * g);
-      qs[s] = p.qscale;
-    } else {
-      float x[NK][8];
-      float top = 0.0f;
-#pragma unroll
-      for (int n = 0; n < NK; n++) {
-        const f32x4 a = *(const f32x4*)(q + 32 * n + 8 * g), b = *(const f32x4*)(q + 32 * n + 8 * g + 4);
-#pragma unroll
-        for (int e = 0; e < 4; e++) {
-          x[n][e] = a[e];
-          x[n][4 + e] = b[e];
-          top = fmaxf(top, fmaxf(fabsf(a[e]), fabsf(b[e])));
-        }
-      }
-      float2 r = pair16(top);
-      top = fmaxf(r.x, r.y);
-      r = pair32(top);
-      top = fmaxf(r.x, r.y);
-      float undo;
-      const float f = row_factor(top, &undo);
-      qs[s] = p.qscale * undo;
-#pragma unroll
-      for (int n = 0; n < NK; n++) {
-#pragma unroll
-        for (int e = 0; e < 8; e++) x[n][e] *= f;
-        split8(x[n], qh[s][n], ql[s][n]);
-      }
-    }
-    if constexpr (DT == KV_Q8) qs[s] *= 1.0f / 127.0f;
-  }
-
-  f32x4 o[NSET][D / 16];
-  float m[NSET], l[NSET];
-#pragma unroll
-  for (int s = 0; s < NSET; s++) {
-    m[s] = -INFINITY;
-    l[s] = 0.0f;
-#pragma unroll
-    for (int j = 0; j < D / 16; j++) o[s][j] = f32x4{0, 0, 0, 0};
-  }
-  float vscale = 0.0f;   // q8: 2^-ev, 0 before the first tile
-
-  auto row_of = [&](int t) -> size_t {
-    const int key = u.key0 + 32 * t;
-    const int id = uniform(pages[key >> shift]);
-    return ((size_t)id * p.kv_heads + kvh) * P + (key & (P - 1));
-  };
-  FewK<D, DT> k;
-  FewV<D, DT> v;
-  if (wave < n_tiles) {
-    const size_t row = row_of(wave);
-    few_load_k<D, DT>(p, row, c, g, k);
-    few_load_v<D, DT>(p, row, c, g, v);
-  }
-  for (int t = wave; t < n_tiles; t += 4) {
-    const int key = u.key0 + 32 * t;
-    const int tn = min(t + 4, n_tiles - 1);   // past the end: a tile of the unit, unused
-    const size_t next = row_of(tn);
-    // ---- scores: s[set][e] of slot slot16(g, e), row c
-    float sc[NSET][8];
-    if constexpr (DT == KV_F32) {
-#pragma unroll
-      for (int s = 0; s < NSET; s++) {
-        f32x4 a[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
-#pragma unroll
-        for (int n = 0; n < NK; n++)
-#pragma unroll
-          for (int e = 0; e < 4; e++)
-#pragma unroll
-            for (int i = 0; i < 2; i++)
-              a[i] = __builtin_amdgcn_mfma_f32_16x16x4f32(k.f[i * NK + n][e], qf[s][n][e], a[i], 0, 0, 0);
-#pragma unroll
-        for (int e = 0; e < 8; e++) sc[s][e] = a[e >> 2][e & 3];
-      }
-    } else if constexpr (DT == KV_F16) {
-      f32x4 a[NSET][2];
-#pragma unroll
-      for (int s = 0; s < NSET; s++) a[s][0] = a[s][1] = f32x4{0, 0, 0, 0};
-#pragma unroll
-      for (int n = 0; n < NK; n++) {
-        H8 k0, k1;
-        k0.u = k.h[n];
-        k1.u = k.h[NK + n];
-#pragma unroll
-        for (int s = 0; s < NSET; s++) {
-          a[s][0] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k0.h, qh[s][n].h, a[s][0], 0, 0, 0);
-          a[s][1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k1.h, qh[s][n].h, a[s][1], 0, 0, 0);
-          a[s][0] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k0.h, ql[s][n].h, a[s][0], 0, 0, 0);
-          a[s][1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k1.h, ql[s][n].h, a[s][1], 0, 0, 0);
-        }
-      }
-#pragma unroll
-      for (int s = 0; s < NSET; s++)
-#pragma unroll
-        for (int e = 0; e < 8; e++) sc[s][e] = a[s][e >> 2][e & 3];
-    } else {
-      // a product's 32 dims are one scale block: its exact code sums, then the block scale in f32
-#pragma unroll
-      for (int s = 0; s < NSET; s++)
-#pragma unroll
-        for (int e = 0; e < 8; e++) sc[s][e] = 0.0f;
-#pragma unroll
-      for (int n = 0; n < NK; n++) {
-        const half8 k0 = codes8(k.c[n]), k1 = codes8(k.c[NK + n]);
-#pragma unroll
-        for (int s = 0; s < NSET; s++) {
-          f32x4 a0 = {0, 0, 0, 0}, a1 = {0, 0, 0, 0};
-          a0 = __builtin_amdgcn_mfma_f32_16x16x32_f16(k0, qh[s][n].h, a0, 0, 0, 0);
-          a1 = __builtin_amdgcn_mfma_f32_16x16x32_f16(k1, qh[s][n].h, a1, 0, 0, 0);
-          a0 = __builtin_amdgcn_mfma_f32_16x16x32_f16(k0, ql[s][n].h, a0, 0, 0, 0);
-          a1 = __builtin_amdgcn_mfma_f32_16x16x32_f16(k1, ql[s][n].h, a1, 0, 0, 0);
-#pragma unroll
-          for (int e = 0; e < 8; e++)
-            sc[s][e] = fmaf(e < 4 ? a0[e & 3] : a1[e & 3], k.s[e * (D / 128) + n / 4][n & 3], sc[s][e]);
-        }
-      }
-    }
-    few_load_k<D, DT>(p, next, c, g, k);
-    const bool masked = key + 32 > u.mask0;
-    if (masked) {
-#pragma unroll
-      for (int s = 0; s < NSET; s++)
-#pragma unroll
-        for (int e = 0; e < 8; e++) sc[s][e] = key + slot16(g, e) <= pos[s] ? sc[s][e] : -INFINITY;
-    }
-    const bool stale = key + 32 > u.key1;  // slots past the written positions
-    if (stale) {
-      if constexpr (DT == KV_F32) {
-#pragma unroll
-        for (int j = 0; j < D / 16; j++)
-#pragma unroll
-          for (int e = 0; e < 8; e++)
-            v.f[2 * j + (e >> 2)][e & 3] = key + slot16(g, e) < u.key1 ? v.f[2 * j + (e >> 2)][e & 3] : 0.0f;
-      } else if constexpr (DT == KV_F16) {
-        u32x4 keep;
-#pragma unroll
-        for (int w = 0; w < 4; w++)
-          keep[w] = (key + slot16(g, 2 * w) < u.key1 ? 0xffffu : 0u) | (key + slot16(g, 2 * w + 1) < u.key1 ? 0xffff0000u : 0u);
-#pragma unroll
-        for (int j = 0; j < D / 16; j++) v.h[j] &= keep;
-      } else {
-#pragma unroll
-        for (int e = 0; e < 8; e++)
-#pragma unroll
-          for (int j = 0; j < D / 128; j++)
-            if (key + slot16(g, e) >= u.key1) v.s[e * (D / 128) + j] = f32x4{0, 0, 0, 0};
-      }
-    }
-    // ---- running maximum and sum
-    float pr[NSET][8];
-#pragma unroll
-    for (int s = 0; s < NSET; s++) {
-      float top = sc[s][0];
-#pragma unroll
-      for (int e = 1; e < 8; e++) top = fmaxf(top, sc[s][e]);
-      float2 r = pair16(top);
-      top = fmaxf(r.x, r.y);
-      r = pair32(top);
-      top = fmaxf(r.x, r.y) * qs[s];
-      if (__any(top > m[s] + kLazy)) {
-        const float mn = fmaxf(m[s], top);
-        const float f = mn == -INFINITY ? 1.0f : exp2_hw(m[s] - mn);
-        m[s] = mn;
-        l[s] *= f;
-#pragma unroll
-        for (int j = 0; j < D / 16; j++) o[s][j] *= f;
-      }
-      const float base = m[s] == -INFINITY ? 0.0f : kPShift - m[s];
-#pragma unroll
-      for (int e = 0; e < 8; e++) {
-        pr[s][e] = exp2_hw(fmaf(sc[s][e], qs[s], base));
-        l[s] += pr[s][e];
-      }
-    }
-    // ---- o
-    if constexpr (DT == KV_F32) {
-#pragma unroll
-      for (int s = 0; s < NSET; s++)
-#pragma unroll
-        for (int e = 0; e < 8; e++)
-#pragma unroll
-          for (int j = 0; j < D / 16; j++)
-            o[s][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(v.f[2 * j + (e >> 2)][e & 3], pr[s][e], o[s][j], 0, 0, 0);
-    } else if constexpr (DT == KV_F16) {
-      H8 ph[NSET], pl[NSET];
-#pragma unroll
-      for (int s = 0; s < NSET; s++) split8(pr[s], ph[s], pl[s]);
-#pragma unroll
-      for (int s = 0; s < NSET; s++) {
-#pragma unroll
-        for (int j = 0; j < D / 16; j++) {
-          H8 a;
-          a.u = v.h[j];
-          o[s][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a.h, ph[s].h, o[s][j], 0, 0, 0);
-        }
-#pragma unroll
-        for (int j = 0; j < D / 16; j++) {
-          H8 a;
-          a.u = v.h[j];
-          o[s][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a.h, pl[s].h, o[s][j], 0, 0, 0);
-        }
-      }
-    } else {
-      // 2^ev at least every scale of the tile (and of those before): p * scale / 2^ev <= p
-      float top = 0.0f;
-#pragma unroll
-      for (int e = 0; e < 8 * (D / 128); e++)
-#pragma unroll
-        for (int w = 0; w < 4; w++) top = fmaxf(top, v.s[e][w]);
-      float2 r = pair16(top);
-      top = fmaxf(r.x, r.y);
-      r = pair32(top);
-      top = fmaxf(r.x, r.y);
-      if (vscale == 0.0f || top * vscale > 1.0f) {  // the same in every lane
-        const int ex = min(max((int)((__float_as_uint(top) >> 23) & 0xff) + 1, 28), 226);
-        const float vn = __uint_as_float((uint32_t)(254 - ex) << 23);
-        const float f = vscale == 0.0f ? 1.0f : vn / vscale;
-        vscale = vn;
-#pragma unroll
-        for (int s = 0; s < NSET; s++)
-#pragma unroll
-          for (int j = 0; j < D / 16; j++) o[s][j] *= f;
-      }
-#pragma unroll
-      for (int n = 0; n < D / 32; n++) {
-        const half8 a0 = codes8(v.c[2 * n]), a1 = codes8(v.c[2 * n + 1]);
-        float w[8];
-#pragma unroll
-        for (int e = 0; e < 8; e++) w[e] = v.s[e * (D / 128) + n / 4][n & 3] * vscale;
-#pragma unroll
-        for (int s = 0; s < NSET; s++) {
-          float x[8];
-#pragma unroll
-          for (int e = 0; e < 8; e++) x[e] = pr[s][e] * w[e];
-          H8 ph, pl;
-          split8(x, ph, pl);
-          o[s][2 * n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a0, ph.h, o[s][2 * n], 0, 0, 0);
-          o[s][2 * n + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a1, ph.h, o[s][2 * n + 1], 0, 0, 0);
-          o[s][2 * n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a0, pl.h, o[s][2 * n], 0, 0, 0);
-          o[s][2 * n + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a1, pl.h, o[s][2 * n + 1], 0, 0, 0);
-        }
-      }
-    }
-    few_load_v<D, DT>(p, next, c, g, v);
-  }
-
-  // ---- the four waves' results meet in LDS
-  const float oscale = DT == KV_Q8 ? (vscale == 0.0f ? 0.0f : 1.0f / (127.0f * vscale)) : 1.0f;
-#pragma unroll
-  for (int s = 0; s < NSET; s++) {
-    float2 r = pair16(l[s]);
-    l[s] = r.x + r.y;
-    r = pair32(l[s]);
-    l[s] = r.x + r.y;
-    if (g == 0) lml[wave][16 * s + c] = make_float2(m[s], l[s]);
-#pragma unroll
-    for (int j = 0; j < D / 16; j++) *(f32x4*)(&lo[wave][16 * s + c][16 * j + 4 * g]) = o[s][j] * oscale;
-  }
-  __syncthreads();
-  for (int x = threadIdx.x; x < u.n_rho * (D / 4); x += 256) {
-    const int i = x / (D / 4), d = 4 * (x % (D / 4));
-    float mw[4], lw[4], top = -INFINITY;
-#pragma unroll
-    for (int w = 0; w < 4; w++) {
-      const float2 ml = lml[w][i];
-      mw[w] = ml.x;
-      lw[w] = ml.y;
-      top = fmaxf(top, ml.x);
-    }
-    f32x4 sum = {0, 0, 0, 0};
-    float lsum = 0.0f;
-#pragma unroll
-    for (int w = 0; w < 4; w++) {
-      const float f = mw[w] == -INFINITY ? 0.0f : exp2_hw(mw[w] - top);
-      lsum += lw[w] * f;
-      sum += *(const f32x4*)(&lo[w][i][d]) * f;
-    }
-    const RowAt r = row_at(p, u, kvh, i);
-    store_o<D>(p, ws_o, r, d, sum, lsum);
-    if (d == 0 && r.part >= 0) ws_ml[(size_t)r.part * p.b.H + r.head] = make_float2(top, lsum);
-  }
-}
-
-// ------------------------------------------------------------------------------------------ many
+// a 128-row unit's staging
 template <int D, int DT>
 struct Many {
   static constexpr int EB = DT == KV_F32 ? 4 : 2;               // bytes of a staged value (q8 codes as f16)
@@ -539,9 +168,417 @@ struct Many {
   static constexpr int SCALES = DT == KV_Q8 ? KT * (D / 32) * 4 : 0;  // bytes of a step's K (or V) scales
 };
 
-// where a staged K row keeps its chunk x: rows of one bank phase spread over all banks
+// ------------------------------------------------------------------------------------------ few
+// A wave's 32-position tile in matrix operand registers. All loads are buffer loads over the tile's 32
+// rows: one descriptor a tile (scalars), constant lane offsets, and a tile past the wave's last one has a
+// descriptor of no bytes, so that the loop needs no branch around its loads and moves nothing for them.
+template <int D, int DT>
+struct FewTile {
+  static constexpr int NK = DT == KV_F32 ? 2 * (D / 16) : 2 * (D / 32), NV = D / 16;
+  u32x4 k[DT == KV_Q8 ? 1 : NK], v[DT == KV_F32 ? 2 * NV : DT == KV_F16 ? NV : 1];
+  u32x2 kc[DT == KV_Q8 ? NK : 1], vc[DT == KV_Q8 ? NV : 1];
+  float ks[DT == KV_Q8 ? D / 64 : 1], vs[DT == KV_Q8 ? D / 64 : 1];  // the lane's share of the tile's scales
+};
+
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t tile_rsrc(const void* base, int bytes) {
+  return __builtin_amdgcn_make_buffer_rsrc((void*)base, (short)0, bytes, 0x00020000);
+}
+__device__ __forceinline__ u32x4 ld16(__amdgpu_buffer_rsrc_t r, int off, int more) {
+  return __builtin_amdgcn_raw_buffer_load_b128(r, off, more, 0);
+}
+__device__ __forceinline__ u32x2 ld8(__amdgpu_buffer_rsrc_t r, int off, int more) {
+  return __builtin_amdgcn_raw_buffer_load_b64(r, off, more, 0);
+}
+
+template <int D, int DT>
+__device__ __forceinline__ void few_load_scales(const float* base, size_t row, bool on, int lane, float (&s)[D / 64]) {
+  const __amdgpu_buffer_rsrc_t r = tile_rsrc(base + row * (D / 32), on ? D * 4 : 0);
+  if constexpr (D == 128) {
+    const u32x2 w = ld8(r, lane * 8, 0);
+    s[0] = __uint_as_float(w[0]);
+    s[1] = __uint_as_float(w[1]);
+  } else {
+    const u32x4 w = ld16(r, lane * 16, 0);
+#pragma unroll
+    for (int i = 0; i < 4; i++) s[i] = __uint_as_float(w[i]);
+  }
+}
+
+template <int D, int DT>
+__device__ __forceinline__ void few_load_k(const PagedKernelArgs& p, size_t row, bool on, int c, int g, FewTile<D, DT>& t) {
+  // operand row c of product i is slot slot16(c / 4, 4 i + c % 4); the k dimension of a lane group is
+  // 8 g + e of every 32 dims (f32: 4 g + e of every 16)
+  constexpr int EB = DT == KV_F32 ? 4 : DT == KV_F16 ? 2 : 1;
+  const int s0 = 16 * (c >> 3) + 4 * ((c >> 2) & 1) + (c & 3);
+  const __amdgpu_buffer_rsrc_t r = tile_rsrc(p.k + row * D * EB, on ? 32 * D * EB : 0);
+  if constexpr (DT == KV_F32) {
+#pragma unroll
+    for (int i = 0; i < 2; i++)
+#pragma unroll
+      for (int j = 0; j < D / 16; j++) t.k[i * (D / 16) + j] = ld16(r, (s0 * D + 4 * g) * 4, (8 * i * D + 16 * j) * 4);
+  } else if constexpr (DT == KV_F16) {
+#pragma unroll
+    for (int i = 0; i < 2; i++)
+#pragma unroll
+      for (int j = 0; j < D / 32; j++) t.k[i * (D / 32) + j] = ld16(r, (s0 * D + 8 * g) * 2, (8 * i * D + 32 * j) * 2);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 2; i++)
+#pragma unroll
+      for (int j = 0; j < D / 32; j++) t.kc[i * (D / 32) + j] = ld8(r, s0 * D + 8 * g, 8 * i * D + 32 * j);
+    few_load_scales<D, DT>(p.ks, row, on, c + 16 * g, t.ks);
+  }
+}
+
+template <int D, int DT>
+__device__ __forceinline__ void few_load_v(const PagedKernelArgs& p, size_t row, bool on, int c, int g, FewTile<D, DT>& t) {
+  constexpr int EB = DT == KV_F32 ? 4 : DT == KV_F16 ? 2 : 1;
+  const __amdgpu_buffer_rsrc_t r = tile_rsrc(p.v + row * D * EB, on ? 32 * D * EB : 0);
+  const int off = (g * D + c) * 8 * EB;
+  if constexpr (DT == KV_F32) {
+#pragma unroll
+    for (int j = 0; j < D / 16; j++) {
+      t.v[2 * j] = ld16(r, off, 128 * 4 * j);
+      t.v[2 * j + 1] = ld16(r, off, 128 * 4 * j + 16);
+    }
+  } else if constexpr (DT == KV_F16) {
+#pragma unroll
+    for (int j = 0; j < D / 16; j++) t.v[j] = ld16(r, off, 128 * 2 * j);
+  } else {
+#pragma unroll
+    for (int j = 0; j < D / 16; j++) t.vc[j] = ld8(r, off, 128 * j);
+    few_load_scales<D, DT>(p.vs, row, on, c + 16 * g, t.vs);
+  }
+}
+
+// where an LDS row keeps its 16-byte chunk x: 16 rows of one chunk spread over all banks
 __device__ inline int swz(int r, int x) { return x ^ (r & 15); }
 
+// LDS of a few-row unit
+template <int D, int DT>
+union FewLds {
+  static constexpr int NQ = DT == KV_F32 ? D / 16 : 2 * (D / 32);
+  struct {
+    u32x4 q[NQ][64];                           // the queries as matrix operands, the same for every wave
+    float s[DT == KV_Q8 ? 4 : 1][2][DT == KV_Q8 ? D : 1];  // q8: K and V scales of the tile a wave is at
+  } in;
+  struct {
+    float o[4][16 * D];                        // the waves' results
+    float2 ml[4][16];
+  } out;
+};
+
+// workgroups of few-row units a CU holds (waves a SIMD)
+template <int D, int DT>
+constexpr int few_waves() { return D == 256 ? (DT == KV_F32 ? 1 : 2) : DT == KV_F32 ? 2 : 3; }
+
+template <int D, int DT>
+__device__ __forceinline__ void few_unit(const PagedKernelArgs& p, const PagedUnit& u, int kvh, float* ws_o, float2* ws_ml,
+                                         FewLds<D, DT>& lds) {
+  constexpr int NK = DT == KV_F32 ? D / 16 : D / 32;
+    const int wave = uniform(threadIdx.x >> 6), lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
+  const int shift = p.b.page_shift, P = 1 << shift;
+  const int n_tiles = (u.key1 - u.key0 + 31) >> 5;
+  const int* pages = p.b.pages + u.table;
+
+  auto row_of = [&](int t) -> size_t {
+    const int key = u.key0 + 32 * min(t, n_tiles - 1);
+    const int id = uniform(pages[key >> shift]);
+    return ((size_t)id * p.kv_heads + kvh) * P + (key & (P - 1));
+  };
+  // the first tiles are on their way before the queries are looked at
+  FewTile<D, DT> tl;
+  if (n_tiles > 0) {
+    const size_t row = row_of(wave);
+    few_load_k<D, DT>(p, row, wave < n_tiles, c, g, tl);
+    few_load_v<D, DT>(p, row, wave < n_tiles, c, g, tl);
+  }
+
+  // ---- the queries: every wave looks at all of them (each row's factor), prepares its share
+  int pos;
+  float qs;
+  {
+    const int rho = u.rho0 + (c < u.n_rho ? c : 0);
+    const int j = rho / p.b.G;
+    const PagedTok tok = p.b.toks[u.tok + j];
+    pos = tok.pos;
+    const float* q = p.q + ((size_t)tok.t * p.b.H + kvh * p.b.G + rho - j * p.b.G) * D;
+    if constexpr (DT == KV_F32) {
+#pragma unroll
+      for (int n = 0; n < NK; n++)
+        if ((n & 3) == wave) lds.in.q[n][lane] = *(const u32x4*)(q + 16 * n + 4 * g);
+      qs = p.qscale;
+    } else {
+      f32x4 x[NK][2];
+      float top = 0.0f;
+#pragma unroll
+      for (int n = 0; n < NK; n++) {
+        x[n][0] = *(const f32x4*)(q + 32 * n + 8 * g);
+        x[n][1] = *(const f32x4*)(q + 32 * n + 8 * g + 4);
+#pragma unroll
+        for (int e = 0; e < 4; e++) top = fmaxf(top, fmaxf(fabsf(x[n][0][e]), fabsf(x[n][1][e])));
+      }
+      float2 r = pair16(top);
+      top = fmaxf(r.x, r.y);
+      r = pair32(top);
+      top = fmaxf(r.x, r.y);
+      float undo;
+      const float f = row_factor(top, &undo);
+      qs = p.qscale * undo * (DT == KV_Q8 ? 1.0f / 127.0f : 1.0f);
+#pragma unroll
+      for (int n = 0; n < NK; n++) {
+        if ((n & 3) == wave) {
+          float y[8];
+#pragma unroll
+          for (int e = 0; e < 8; e++) y[e] = x[n][e >> 2][e & 3] * f;
+          H8 hi, lo;
+          split8(y, hi, lo);
+          lds.in.q[2 * n][lane] = hi.u;
+          lds.in.q[2 * n + 1][lane] = lo.u;
+        }
+      }
+    }
+  }
+  __syncthreads();
+  // part 0: hi (f32: the values), 1: lo
+  auto q_at = [&](int n, int part) __attribute__((always_inline)) {
+    H8 h;
+    h.u = lds.in.q[2 * n + part][lane];
+    return h.h;
+  };
+
+  f32x4 o[D / 16];
+  float m = -INFINITY, l = 0.0f;
+#pragma unroll
+  for (int j = 0; j < D / 16; j++) o[j] = f32x4{0, 0, 0, 0};
+  float ev = -60.0f;     // q8: 2^ev is above every value scale so far
+
+  for (int t = wave; t < n_tiles; t += 4) {
+    const int key = u.key0 + 32 * t;
+    const bool more = t + 4 < n_tiles;
+    const size_t next = row_of(t + 4);
+    float* lk = lds.in.s[DT == KV_Q8 ? wave : 0][0];
+    float* lv = lds.in.s[DT == KV_Q8 ? wave : 0][1];
+    if constexpr (DT == KV_Q8) {
+      // a wave's LDS accesses complete in order: the tile before is done with them
+#pragma unroll
+      for (int i = 0; i < D / 64; i++) {
+        lk[lane * (D / 64) + i] = tl.ks[i];
+        lv[lane * (D / 64) + i] = tl.vs[i];
+      }
+      __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+      __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    }
+    // ---- scores: sc[e] of slot slot16(g, e), row c
+    float sc[8];
+    if constexpr (DT == KV_F32) {
+      f32x4 a[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
+#pragma unroll
+      for (int n = 0; n < NK; n++) {
+        const f32x4 qn = *(const f32x4*)&lds.in.q[n][lane];
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+#pragma unroll
+          for (int i = 0; i < 2; i++)
+            a[i] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(tl.k[i * NK + n][e]), qn[e], a[i], 0, 0, 0);
+      }
+#pragma unroll
+      for (int e = 0; e < 8; e++) sc[e] = a[e >> 2][e & 3];
+    } else if constexpr (DT == KV_F16) {
+      f32x4 a[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}}, b[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
+#pragma unroll
+      for (int n = 0; n < NK; n++) {
+        H8 k0, k1;
+        k0.u = tl.k[n];
+        k1.u = tl.k[NK + n];
+        const half8 qh = q_at(n, 0), ql = q_at(n, 1);
+        a[0] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k0.h, qh, a[0], 0, 0, 0);
+        a[1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k1.h, qh, a[1], 0, 0, 0);
+        b[0] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k0.h, ql, b[0], 0, 0, 0);
+        b[1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k1.h, ql, b[1], 0, 0, 0);
+      }
+#pragma unroll
+      for (int e = 0; e < 8; e++) sc[e] = a[e >> 2][e & 3] + b[e >> 2][e & 3];
+    } else {
+      // a product's 32 dims are one scale block: its exact code sums, then the block scale in f32
+#pragma unroll
+      for (int e = 0; e < 8; e++) sc[e] = 0.0f;
+#pragma unroll
+      for (int n4 = 0; n4 < NK; n4 += 4) {
+        f32x4 a[4][2];
+#pragma unroll
+        for (int n = 0; n < 4; n++) {
+          const half8 k0 = codes8(tl.kc[n4 + n]), k1 = codes8(tl.kc[NK + n4 + n]);
+          const half8 qh = q_at(n4 + n, 0), ql = q_at(n4 + n, 1);
+          a[n][0] = a[n][1] = f32x4{0, 0, 0, 0};
+          a[n][0] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k0, qh, a[n][0], 0, 0, 0);
+          a[n][1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k1, qh, a[n][1], 0, 0, 0);
+          a[n][0] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k0, ql, a[n][0], 0, 0, 0);
+          a[n][1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k1, ql, a[n][1], 0, 0, 0);
+        }
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+          const f32x4 z = *(const f32x4*)(lk + slot16(g, e) * (D / 32) + n4);
+#pragma unroll
+          for (int n = 0; n < 4; n++) sc[e] = fmaf(a[n][e >> 2][e & 3], z[n], sc[e]);
+        }
+      }
+    }
+    __builtin_amdgcn_sched_barrier(0);  // into the registers just used: not before, which would take a second set
+    few_load_k<D, DT>(p, next, more, c, g, tl);
+    __builtin_amdgcn_sched_barrier(0);
+    if (key + 32 > u.mask0) {
+#pragma unroll
+      for (int e = 0; e < 8; e++) sc[e] = key + slot16(g, e) <= pos ? sc[e] : -INFINITY;
+    }
+    const bool stale = key + 32 > u.key1;  // slots past the written positions
+    if (stale) {
+      if constexpr (DT == KV_F32) {
+#pragma unroll
+        for (int j = 0; j < D / 16; j++)
+#pragma unroll
+          for (int e = 0; e < 8; e++)
+            tl.v[2 * j + (e >> 2)][e & 3] = key + slot16(g, e) < u.key1 ? tl.v[2 * j + (e >> 2)][e & 3] : 0u;
+      } else if constexpr (DT == KV_F16) {
+        u32x4 keep;
+#pragma unroll
+        for (int w = 0; w < 4; w++)
+          keep[w] = (key + slot16(g, 2 * w) < u.key1 ? 0xffffu : 0u) | (key + slot16(g, 2 * w + 1) < u.key1 ? 0xffff0000u : 0u);
+#pragma unroll
+        for (int j = 0; j < D / 16; j++) tl.v[j] &= keep;
+      } else {
+#pragma unroll
+        for (int i = 0; i < D / 64; i++) {  // this lane's scales are of slot (lane * D / 64 + i) / (D / 32)
+          if (key + (lane * (D / 64) + i) / (D / 32) >= u.key1) {
+            tl.vs[i] = 0.0f;
+            lv[lane * (D / 64) + i] = 0.0f;
+          }
+        }
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+      }
+    }
+    // ---- running maximum and sum
+    float top = sc[0];
+#pragma unroll
+    for (int e = 1; e < 8; e++) top = fmaxf(top, sc[e]);
+    float2 r = pair16(top);
+    top = fmaxf(r.x, r.y);
+    r = pair32(top);
+    top = fmaxf(r.x, r.y) * qs;
+    float en = ev;
+    if constexpr (DT == KV_Q8) {
+      float big = tl.vs[0];
+#pragma unroll
+      for (int i = 1; i < D / 64; i++) big = fmaxf(big, tl.vs[i]);
+      en = fmaxf(ev, scale_exponent(wave_max(big)));
+    }
+    if (__any(top > m + kLazy || en > ev)) {
+      const float mn = top > m + kLazy ? top : m;
+      const float f = m == -INFINITY ? 1.0f : exp2_hw(m - mn + (DT == KV_Q8 ? ev - en : 0.0f));
+      m = mn;
+      ev = en;
+      l *= f;
+#pragma unroll
+      for (int j = 0; j < D / 16; j++) o[j] *= f;
+    }
+    const float base = m == -INFINITY ? 0.0f : kPShift - m - (DT == KV_Q8 ? ev : 0.0f);
+    float pr[8];
+#pragma unroll
+    for (int e = 0; e < 8; e++) {
+      pr[e] = exp2_hw(fmaf(sc[e], qs, base));
+      l += pr[e];
+    }
+    // ---- o
+    if constexpr (DT == KV_F32) {
+#pragma unroll
+      for (int e = 0; e < 8; e++)
+#pragma unroll
+        for (int j = 0; j < D / 16; j++)
+          o[j] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(tl.v[2 * j + (e >> 2)][e & 3]), pr[e], o[j], 0, 0, 0);
+    } else if constexpr (DT == KV_F16) {
+      H8 ph, pl;
+      split8(pr, ph, pl);
+#pragma unroll
+      for (int j = 0; j < D / 16; j++) {
+        H8 a;
+        a.u = tl.v[j];
+        o[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a.h, ph.h, o[j], 0, 0, 0);
+      }
+#pragma unroll
+      for (int j = 0; j < D / 16; j++) {
+        H8 a;
+        a.u = tl.v[j];
+        o[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a.h, pl.h, o[j], 0, 0, 0);
+      }
+    } else {
+#pragma unroll
+      for (int n4 = 0; n4 < D / 32; n4 += 4) {
+        f32x4 z[8];
+#pragma unroll
+        for (int e = 0; e < 8; e++) z[e] = *(const f32x4*)(lv + slot16(g, e) * (D / 32) + n4);
+#pragma unroll
+        for (int n = 0; n < 4; n++) {
+          const half8 a0 = codes8(tl.vc[2 * (n4 + n)]), a1 = codes8(tl.vc[2 * (n4 + n) + 1]);
+          float x[8];
+#pragma unroll
+          for (int e = 0; e < 8; e++) x[e] = pr[e] * z[e][n];
+          H8 ph, pl;
+          split8(x, ph, pl);
+          f32x4 &o0 = o[2 * (n4 + n)], &o1 = o[2 * (n4 + n) + 1];
+          o0 = __builtin_amdgcn_mfma_f32_16x16x32_f16(a0, ph.h, o0, 0, 0, 0);
+          o1 = __builtin_amdgcn_mfma_f32_16x16x32_f16(a1, ph.h, o1, 0, 0, 0);
+          o0 = __builtin_amdgcn_mfma_f32_16x16x32_f16(a0, pl.h, o0, 0, 0, 0);
+          o1 = __builtin_amdgcn_mfma_f32_16x16x32_f16(a1, pl.h, o1, 0, 0, 0);
+        }
+      }
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    few_load_v<D, DT>(p, next, more, c, g, tl);
+    __builtin_amdgcn_sched_barrier(0);
+  }
+
+  // ---- the four waves' results meet in LDS
+  const float oscale = DT == KV_Q8 ? 1.0f / 127.0f : 1.0f;
+  if constexpr (DT == KV_Q8) m += ev;
+  __syncthreads();  // every wave is done with the queries and its scales
+  {
+    float2 r = pair16(l);
+    l = r.x + r.y;
+    r = pair32(l);
+    l = r.x + r.y;
+    if (g == 0) lds.out.ml[wave][c] = make_float2(m, l);
+#pragma unroll
+    for (int j = 0; j < D / 16; j++) *(f32x4*)&lds.out.o[wave][c * D + swz(c, 4 * j + g) * 4] = o[j] * oscale;
+  }
+  __syncthreads();
+  for (int x = threadIdx.x; x < u.n_rho * (D / 4); x += 256) {
+    const int i = x / (D / 4), ch = x % (D / 4);
+    float mw[4], lw[4], top = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < 4; w++) {
+      const float2 z = lds.out.ml[w][i];
+      mw[w] = z.x;
+      lw[w] = z.y;
+      top = fmaxf(top, z.x);
+    }
+    f32x4 sum = {0, 0, 0, 0};
+    float lsum = 0.0f;
+#pragma unroll
+    for (int w = 0; w < 4; w++) {
+      const float f = mw[w] == -INFINITY ? 0.0f : exp2_hw(mw[w] - top);
+      lsum += lw[w] * f;
+      sum += *(const f32x4*)&lds.out.o[w][i * D + swz(i, ch) * 4] * f;
+    }
+    const RowAt r = row_at(p, u, kvh, i);
+    store_o<D>(p, ws_o, r, 4 * ch, sum, lsum);
+    if (ch == 0 && r.part >= 0) ws_ml[(size_t)r.part * p.b.H + r.head] = make_float2(top, lsum);
+  }
+}
+
+// ------------------------------------------------------------------------------------------ many
 template <int D, int DT>
 __device__ __forceinline__ void many_stage(const PagedKernelArgs& p, size_t row, char* kd, char* vd) {
   // f16 / f32: 16-byte chunks copied straight into LDS, no registers. A wave instruction fills 64
@@ -660,7 +697,7 @@ __device__ __forceinline__ void many_unit(const PagedKernelArgs& p, const PagedU
   for (int j = 0; j < D / 32; j++)
 #pragma unroll
     for (int e = 0; e < 16; e++) o[j][e] = 0.0f;
-  float m = -INFINITY, l = 0.0f, vscale = 0.0f;
+  float m = -INFINITY, l = 0.0f, ev = -60.0f;  // q8: 2^ev is above every value scale so far
 
   auto row_of = [&](int t) -> size_t {
     const int key = u.key0 + 32 * min(t, n_tiles - 1);  // past the end: staged again, masked
@@ -671,6 +708,36 @@ __device__ __forceinline__ void many_unit(const PagedKernelArgs& p, const PagedU
   // one step over staged tiles; key: its first position
   auto step = [&](const char* kb, const char* vb, const float* ksb, const float* vsb, int key) __attribute__((always_inline)) {
     float s[NSUB][16];
+    if constexpr (DT == KV_F16) {
+      // both sub-tiles' chains side by side, their operands read two chunks ahead
+      f32x16 a[NSUB];
+#pragma unroll
+      for (int sub = 0; sub < NSUB; sub++)
+#pragma unroll
+        for (int e = 0; e < 16; e++) a[sub][e] = 0.0f;
+      int at = c * M::CPR * 16 + swz(c, h) * 16;  // chunk 2 n + h lies at at ^ 32 n
+      asm volatile("" : "+v"(at));                // made here, not kept in a register a chunk
+#pragma unroll
+      for (int n = 0; n < NK; n++) {
+        H8 x[NSUB];
+#pragma unroll
+        for (int sub = 0; sub < NSUB; sub++) x[sub].u = *(const u32x4*)(kb + sub * M::SUB + (at ^ (32 * n)));
+#pragma unroll
+        for (int sub = 0; sub < NSUB; sub++) a[sub] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x[sub].h, qh[n].h, a[sub], 0, 0, 0);
+#pragma unroll
+        for (int sub = 0; sub < NSUB; sub++) a[sub] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x[sub].h, ql[n].h, a[sub], 0, 0, 0);
+      }
+      __builtin_amdgcn_sched_group_barrier(0x100, 2 * NSUB, 0);
+#pragma unroll
+      for (int n = 0; n < NK; n++) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 2 * NSUB, 0);
+        __builtin_amdgcn_sched_group_barrier(0x100, NSUB, 0);
+      }
+#pragma unroll
+      for (int sub = 0; sub < NSUB; sub++)
+#pragma unroll
+        for (int e = 0; e < 16; e++) s[sub][e] = a[sub][e];
+    }
 #pragma unroll
     for (int sub = 0; sub < NSUB; sub++) {
       const char* kt = kb + sub * M::SUB + c * M::CPR * 16;
@@ -686,20 +753,7 @@ __device__ __forceinline__ void many_unit(const PagedKernelArgs& p, const PagedU
         }
 #pragma unroll
         for (int e = 0; e < 16; e++) s[sub][e] = a[e];
-      } else if constexpr (DT == KV_F16) {
-        f32x16 a, b;
-#pragma unroll
-        for (int e = 0; e < 16; e++) a[e] = b[e] = 0.0f;
-#pragma unroll
-        for (int n = 0; n < NK; n++) {
-          H8 x;
-          x.u = *(const u32x4*)(kt + swz(c, 2 * n + h) * 16);
-          a = __builtin_amdgcn_mfma_f32_32x32x16_f16(x.h, qh[n].h, a, 0, 0, 0);
-          b = __builtin_amdgcn_mfma_f32_32x32x16_f16(x.h, ql[n].h, b, 0, 0, 0);
-        }
-#pragma unroll
-        for (int e = 0; e < 16; e++) s[sub][e] = a[e] + b[e];
-      } else {
+      } else if constexpr (DT == KV_Q8) {
 #pragma unroll
         for (int e = 0; e < 16; e++) s[sub][e] = 0.0f;
 #pragma unroll
@@ -739,15 +793,23 @@ __device__ __forceinline__ void many_unit(const PagedKernelArgs& p, const PagedU
       for (int e = 0; e < 16; e++) top = fmaxf(top, s[sub][e]);
     const float2 r = pair32(top);
     top = fmaxf(r.x, r.y) * qs;
-    if (__any(top > m + kLazy)) {
-      const float mn = fmaxf(m, top);
-      const float f = mn == -INFINITY ? 1.0f : exp2_hw(m - mn);
+    float en = ev;
+    if constexpr (DT == KV_Q8) {
+      float big = 0.0f;
+#pragma unroll
+      for (int i = 0; i < KT * (D / 32) / 64; i++) big = fmaxf(big, vsb[lane + 64 * i]);
+      en = fmaxf(ev, scale_exponent(wave_max(big)));
+    }
+    if (__any(top > m + kLazy || en > ev)) {
+      const float mn = top > m + kLazy ? top : m;
+      const float f = m == -INFINITY ? 1.0f : exp2_hw(m - mn + (DT == KV_Q8 ? ev - en : 0.0f));
       m = mn;
+      ev = en;
       l *= f;
 #pragma unroll
       for (int j = 0; j < D / 32; j++) o[j] *= f;
     }
-    const float base = m == -INFINITY ? 0.0f : kPShift - m;
+    const float base = m == -INFINITY ? 0.0f : kPShift - m - (DT == KV_Q8 ? ev : 0.0f);
 #pragma unroll
     for (int sub = 0; sub < NSUB; sub++)
 #pragma unroll
@@ -755,21 +817,6 @@ __device__ __forceinline__ void many_unit(const PagedKernelArgs& p, const PagedU
         s[sub][e] = exp2_hw(fmaf(s[sub][e], qs, base));
         l += s[sub][e];
       }
-    if constexpr (DT == KV_Q8) {
-      // 2^ev at least every scale of the step
-      float big = 0.0f;
-#pragma unroll
-      for (int i = 0; i < KT * (D / 32) / 64; i++) big = fmaxf(big, vsb[lane + 64 * i]);
-      big = wave_max(big);
-      if (vscale == 0.0f || big * vscale > 1.0f) {
-        const int ex = min(max((int)((__float_as_uint(big) >> 23) & 0xff) + 1, 28), 226);
-        const float vn = __uint_as_float((uint32_t)(254 - ex) << 23);
-        const float f = vscale == 0.0f ? 1.0f : vn / vscale;
-        vscale = vn;
-#pragma unroll
-        for (int j = 0; j < D / 32; j++) o[j] *= f;
-      }
-    }
 #pragma unroll
     for (int sub = 0; sub < NSUB; sub++) {
       const char* vt = vb + sub * M::SUB;
@@ -792,11 +839,14 @@ __device__ __forceinline__ void many_unit(const PagedKernelArgs& p, const PagedU
           H8 ph, pl;
           split8(w, ph, pl);
 #pragma unroll
-          for (int j = 0; j < D / 32; j++) {
-            H8 a;
+          for (int j = 0; j < D / 32; j += 2) {
+            H8 a, b;
             a.u = *(const u32x4*)(vt + ((2 * x + h) * D + 32 * j + c) * 16);
+            b.u = *(const u32x4*)(vt + ((2 * x + h) * D + 32 * j + 32 + c) * 16);
             o[j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a.h, ph.h, o[j], 0, 0, 0);
+            o[j + 1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(b.h, ph.h, o[j + 1], 0, 0, 0);
             o[j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a.h, pl.h, o[j], 0, 0, 0);
+            o[j + 1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(b.h, pl.h, o[j + 1], 0, 0, 0);
           }
         }
       } else {
@@ -809,7 +859,7 @@ __device__ __forceinline__ void many_unit(const PagedKernelArgs& p, const PagedU
             for (int y = 0; y < 2; y++) {
               const f32x4 z = *(const f32x4*)(vsb + j * KT + 32 * sub + 16 * x + 8 * y + 4 * h);
 #pragma unroll
-              for (int e = 0; e < 4; e++) w[4 * y + e] = s[sub][8 * x + 4 * y + e] * (z[e] * vscale);
+              for (int e = 0; e < 4; e++) w[4 * y + e] = s[sub][8 * x + 4 * y + e] * z[e];
             }
             H8 ph, pl, a;
             split8(w, ph, pl);
@@ -876,7 +926,8 @@ __device__ __forceinline__ void many_unit(const PagedKernelArgs& p, const PagedU
   }
   const float2 r = pair32(l);
   l = r.x + r.y;
-  const float oscale = DT == KV_Q8 ? (vscale == 0.0f ? 0.0f : 1.0f / (127.0f * vscale)) : 1.0f;
+  const float oscale = DT == KV_Q8 ? 1.0f / 127.0f : 1.0f;
+  if constexpr (DT == KV_Q8) m += ev;
   if (ra.on) {
 #pragma unroll
     for (int j = 0; j < D / 32; j++)
@@ -888,12 +939,12 @@ __device__ __forceinline__ void many_unit(const PagedKernelArgs& p, const PagedU
   }
 }
 
-// Kernels: the 128-row units and the few-row units are launches of their own, each with its own registers.
+// The 128-row units and the few-row units are launches of their own, each with its own registers and LDS.
 template <int D, int DT>
 __global__ __launch_bounds__(256, D == 128 ? 2 : 1) void paged_many_kernel(PagedKernelArgs p) {
   using M = Many<D, DT>;
-  // four distinct arrays: a copy into one buffer then cannot alias the reads of another, and the
-  // compiler adds no waits between them
+  // K and V tiles of even and odd steps. Distinct arrays: a copy into one buffer then cannot alias the
+  // reads of another, and the compiler adds no waits between them.
   __shared__ __align__(16) char k0[M::SUB * M::NSUB];
   __shared__ __align__(16) char k1[M::SUB * M::NSUB];
   __shared__ __align__(16) char v0[M::SUB * M::NSUB];
@@ -909,41 +960,50 @@ __global__ __launch_bounds__(256, D == 128 ? 2 : 1) void paged_many_kernel(Paged
   }
 }
 
-template <int D, int DT, int NSET>
-__global__ __launch_bounds__(256, D == 128 ? 2 : 1) void paged_few_kernel(PagedKernelArgs p) {
-  __shared__ __align__(16) float lo[4][16 * NSET][D + kFewPad];
-  __shared__ float2 lml[4][16 * NSET];
+template <int D, int DT>
+__global__ __launch_bounds__(256, (few_waves<D, DT>())) void paged_few_kernel(PagedKernelArgs p) {
+  __shared__ FewLds<D, DT> lds;
   const PagedHeader* h = p.b.hdr;
-  const int first = p.n_blocks ? p.first : NSET == 1 ? h->n_units - h->n_few1 : h->n_many;
-  const int total = p.n_blocks ? p.n_blocks : (NSET == 1 ? h->n_few1 : h->n_units - h->n_few1 - h->n_many) * p.kv_heads;
+  const int first = p.n_blocks ? p.first : h->n_many;
+  const int total = p.n_blocks ? p.n_blocks : (h->n_units - h->n_many) * p.kv_heads;
   float* ws_o = h->ws_o;
   float2* ws_ml = h->ws_ml;
   for (int b = blockIdx.x; b < total; b += gridDim.x) {
     const PagedUnit u = p.b.units[first + b / p.kv_heads];
-    few_unit<D, DT, NSET>(p, u, b % p.kv_heads, ws_o, ws_ml, lo, lml);
+    few_unit<D, DT>(p, u, b % p.kv_heads, ws_o, ws_ml, lds);
     __syncthreads();  // the unit's LDS is read before the next one's is written
   }
 }
 
-// lane groups that share a row's partials
-__host__ __device__ inline int merge_groups(int most_parts) { return most_parts <= 8 ? 1 : 4; }
+template <int D>
+__host__ __device__ inline long merge_blocks(long rows, int groups) {
+  const int rpw = 256 / (D / 4 * groups);
+  return (rows + rpw - 1) / rpw;
+}
 
 // A row's partials joined. D / 4 lanes hold a partial's row (16 bytes a lane); PP lane groups a row take
 // every PP-th partial, eight at a time, all loaded before any is used (a row of 55 partials: two rounds of
-// memory latency instead of 55), and meet in LDS. PP is 1 where no row has more than eight, else 4: the
-// same for a replay as for a call, so both give the same bits.
+// memory latency instead of 55), and meet in LDS. The merges of at most kMergeFew partials come first and
+// take one group a row (a row of two would leave three of four groups idle), the others four; a workgroup
+// has rows of one kind.
 template <int D>
-__global__ __launch_bounds__(256) void paged_merge_kernel(PagedKernelArgs p, int n_merges, int most_parts) {
+__global__ __launch_bounds__(256) void paged_merge_kernel(PagedKernelArgs p) {
   constexpr int LPR = D / 4, N = 8, MAXP = 4;
+  static_assert(N >= kMergeFew, "one round takes a row of few partials");
   __shared__ f32x4 lo[256 / (LPR * MAXP)][MAXP][LPR];
   __shared__ float2 lml[256 / (LPR * MAXP)][MAXP];
-  const int PP = merge_groups(n_merges ? most_parts : p.b.hdr->most_parts), RPW = 256 / (LPR * PP);
-  const int c = threadIdx.x % LPR, g = threadIdx.x / LPR % PP, rw = threadIdx.x / (LPR * PP);
   const int H = p.b.H;
-  const long total = (long)(n_merges ? n_merges : p.b.hdr->n_merges) * H;
+  const PagedHeader* hdr = p.b.hdr;
+  const long n_few = (long)(p.b.captured ? hdr->n_merge_few : p.b.n_merge_few) * H;
+  const long n_all = (long)(p.b.captured ? hdr->n_merges : p.b.n_merges) * H;
+  const long few_blocks = merge_blocks<D>(n_few, 1), blocks = few_blocks + merge_blocks<D>(n_all - n_few, MAXP);
   const float* ws_o = p.b.hdr->ws_o;
   const float2* ws_ml = p.b.hdr->ws_ml;
-  for (long first = (long)blockIdx.x * RPW; first < total; first += (long)gridDim.x * RPW) {
+  for (long blk = blockIdx.x; blk < blocks; blk += gridDim.x) {
+    const bool few = blk < few_blocks;
+    const int PP = few ? 1 : MAXP, RPW = 256 / (LPR * PP);
+    const int c = threadIdx.x % LPR, g = few ? 0 : threadIdx.x / LPR % MAXP, rw = threadIdx.x / (LPR * PP);
+    const long first = few ? blk * RPW : n_few + (blk - few_blocks) * RPW, total = few ? n_few : n_all;
     const long x = min(first + rw, total - 1);  // past the end: the last row again, not stored
     const PagedMerge mg = p.b.merges[x / H];
     const int head = (int)(x % H);
@@ -1007,31 +1067,24 @@ template <int D, int DT>
 static hipError_t launch_attn(const PagedKernelArgs& k, const PagedAttnArgs& a, hipStream_t st) {
   const PagedBatchView& b = k.b;
   if (!b.captured && b.n_units == 0) return hipSuccess;
-  // Under capture a grid that fills the GPU walks the units of whatever batch is set at replay, of every
-  // kind. Units lie by kind: 128 rows, two sets, one set.
+  // Under capture a grid that fills the GPU walks the units of whatever batch is set at replay, of both
+  // kinds.
   PagedKernelArgs x = k;
-  const unsigned full = (unsigned)(a.num_cus * (D == 128 ? 2 : 1));
   if (b.captured || b.n_many) {
     x.n_blocks = b.n_many * k.kv_heads;
-    hipLaunchKernelGGL((paged_many_kernel<D, DT>), dim3(b.captured ? full : (unsigned)x.n_blocks), dim3(256), 0, st, x);
+    const unsigned grid = (unsigned)(b.captured ? a.num_cus * (D == 128 ? 2 : 1) : x.n_blocks);
+    hipLaunchKernelGGL((paged_many_kernel<D, DT>), dim3(grid), dim3(256), 0, st, x);
   }
-  if constexpr (DT != KV_F32) {
-    const int n2 = b.n_units - b.n_many - b.n_few1;
-    if (b.captured || n2) {
-      x.first = b.n_many;
-      x.n_blocks = n2 * k.kv_heads;
-      hipLaunchKernelGGL((paged_few_kernel<D, DT, 2>), dim3(b.captured ? full : (unsigned)x.n_blocks), dim3(256), 0, st, x);
-    }
-  }
-  if (b.captured || b.n_few1) {
-    x.first = b.n_units - b.n_few1;
-    x.n_blocks = b.n_few1 * k.kv_heads;
-    hipLaunchKernelGGL((paged_few_kernel<D, DT, 1>), dim3(b.captured ? full : (unsigned)x.n_blocks), dim3(256), 0, st, x);
+  if (b.captured || b.n_units > b.n_many) {
+    x.first = b.n_many;
+    x.n_blocks = (b.n_units - b.n_many) * k.kv_heads;
+    const unsigned grid = (unsigned)(b.captured ? a.num_cus * few_waves<D, DT>() : x.n_blocks);
+    hipLaunchKernelGGL((paged_few_kernel<D, DT>), dim3(grid), dim3(256), 0, st, x);
   }
   if (b.captured || b.n_merges) {
-    const int rpw = 256 / (D / 4 * merge_groups(b.most_parts));
-    const unsigned grid = b.captured ? (unsigned)(a.num_cus * 4) : (unsigned)(((long)b.n_merges * b.H + rpw - 1) / rpw);
-    hipLaunchKernelGGL((paged_merge_kernel<D>), dim3(grid), dim3(256), 0, st, k, b.captured ? 0 : b.n_merges, b.most_parts);
+    const long few = (long)b.n_merge_few * b.H, all = (long)b.n_merges * b.H;
+    const long grid = b.captured ? a.num_cus * 4L : merge_blocks<D>(few, 1) + merge_blocks<D>(all - few, 4);
+    hipLaunchKernelGGL((paged_merge_kernel<D>), dim3((unsigned)grid), dim3(256), 0, st, k);
   }
   return hipGetLastError();
 }

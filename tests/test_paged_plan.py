@@ -47,8 +47,8 @@ def check(p, rows, lens, tables, G, page, dtype):
     taken = sorted((part, part + n) for part, n in merged.values())
     assert all(a[1] <= b[0] for a, b in zip(taken, taken[1:])) and (not taken or taken[-1][1] <= n_parts)
     for u in p["units"]:
-        width = {0: 128, 1: 16, 2: 32}[u["kind"]]
-        assert 1 <= u["n_rho"] <= width and not (dtype == 0 and u["kind"] == 2)
+        width = {0: 128, 1: 16}[u["kind"]]
+        assert 1 <= u["n_rho"] <= width
         assert u["key0"] % 32 == 0 and u["key0"] <= u["key1"]
         if u["kind"] == 0 and u["key1"] > u["key0"]:      # a step of 64 holds no half of another chunk
             assert (u["key1"] - u["key0"]) % 64 == 0 or u["mask0"] <= u["key1"]
