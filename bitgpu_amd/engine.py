@@ -25,6 +25,7 @@ fallback: without the built HIP library these functions raise.
 """
 from __future__ import annotations
 
+import array
 import ctypes as C
 import math
 
@@ -576,6 +577,7 @@ class PagedKvCache:
             raise ValueError("bitgpu_amd: k_scale and v_scale belong to a q8 cache")
         self.n_layers, self.kv_heads, self.head_dim, self.kv_cache = n_layers, kv_heads, head_dim, kv_cache
         self.n_pages, self.page_size, self.q8_block, self.device = n_pages, page_size, q8_block, self.k.device
+        self.index = self.k.get_device()
         with torch.cuda.device(self._one_device(self.k, self.v, self.k_scale, self.v_scale)):
             check(lib().bg_paged_create(n_layers, kv_heads, head_dim, dtype, page_size, n_pages, _ptr(self.k), _ptr(self.v),
                                         _ptr(self.k_scale), _ptr(self.v_scale), C.byref(self._h)))
@@ -671,6 +673,11 @@ class PagedBatch:
 
 def _int32(x, name, dims):
     """x (a sequence, array or host tensor of integers) as a contiguous int32 array."""
+    if isinstance(x, (list, tuple)) and dims == 1:
+        try:  # a list of Python integers, several times faster than through np.asarray
+            return np.frombuffer(array.array("i", x), np.int32) if x else np.zeros(0, np.int32)
+        except (TypeError, OverflowError):
+            pass
     if torch is not None and isinstance(x, torch.Tensor):
         x = x.numpy()
     a = np.asarray(x)
@@ -685,12 +692,20 @@ def _int32(x, name, dims):
     return np.ascontiguousarray(a)
 
 
-def _rows_at_least(t, name, rows, width):
-    """t is f32 and holds `rows` rows of `width` values (more: a padded batch)."""
-    _f32(t, name)
+def _rows_ptr(t, name, rows, width, device):
+    """Pointer of an f32 tensor of at least `rows` contiguous rows of `width` values (more: a padded batch)
+    on the pool's device; None for None."""
+    if t is None:
+        return None
+    if t.dtype is not torch.float32:
+        raise TypeError(f"bitgpu_amd: {name} must be float32, got {t.dtype}")
+    if t.get_device() != device:
+        raise ValueError(f"bitgpu_amd: expected {name} on cuda:{device}, got {t.device}")
+    if not t.is_contiguous():
+        raise ValueError(f"bitgpu_amd: expected a contiguous tensor ({name})")
     if t.numel() < rows * width:
         raise ValueError(f"bitgpu_amd: {name} holds {t.numel()} values, the batch needs {rows} rows of {width}")
-    return t
+    return t.data_ptr()
 
 
 def paged_qkv_prologue(cache: PagedKvCache, li: int, batch: PagedBatch, q, k, v, q_gamma, k_gamma, eps: float, cos_tab,
@@ -700,24 +715,29 @@ def paged_qkv_prologue(cache: PagedKvCache, li: int, batch: PagedBatch, q, k, v,
     [rows, H, D], with k and v written to their sequences' pages. ``pair_axis`` (rot_dim / 2 integers,
     needed where the batch was set with several position axes): the axis each rotary pair takes its
     position from."""
-    D, T, stride = cache.head_dim, batch.n_tokens, int(q_stride or cache.head_dim)
-    cache._one_device(*(t for t in (q, k, v, q_gamma, k_gamma, cos_tab, sin_tab, q_out) if t is not None))
-    for t, nm, rows, width in ((q, "q", T, batch.H * stride), (k, "k", T, cache.kv_heads * D), (v, "v", T, cache.kv_heads * D),
-                               (q_gamma, "q_gamma", 1, D), (k_gamma, "k_gamma", 1, D), (q_out, "q_out", T, batch.H * D)):
-        if t is not None:
-            _rows_at_least(t, nm, rows, width)
-    for t, nm in ((cos_tab, "cos"), (sin_tab, "sin")):
-        if t is not None and (_f32(t, nm).dim() != 2 or 2 * t.shape[1] != rot_dim or t.shape != cos_tab.shape):
-            raise ValueError(f"bitgpu_amd: {nm} must be [positions, rot_dim / 2 = {rot_dim // 2}], got {list(t.shape)}")
+    D, H, T, dev = cache.head_dim, batch.H, batch.n_tokens, cache.index
+    stride, kw = int(q_stride or D), cache.kv_heads * D
+    qp = _rows_ptr(q, "q", T, H * stride, dev)
+    positions = 0
+    if cos_tab is not None or sin_tab is not None:
+        for t, nm in ((cos_tab, "cos"), (sin_tab, "sin")):
+            if t is None or t.dim() != 2 or 2 * t.shape[1] != rot_dim or t.shape != cos_tab.shape:
+                raise ValueError(f"bitgpu_amd: {nm} must be [positions, rot_dim / 2 = {rot_dim // 2}], got "
+                                 f"{None if t is None else list(t.shape)}")
+        positions = cos_tab.shape[0]
     if q is not None and q_out is None:
-        q_out = q.new_empty((q.numel() // (batch.H * stride), batch.H, D))
+        q_out = torch.empty_like(q) if stride == D and q.dim() == 3 else q.new_empty((q.numel() // (H * stride), H, D))
+    ap = None
     if pair_axis is not None:
         pair_axis = np.ascontiguousarray(pair_axis, np.uint8)
         if pair_axis.shape != (rot_dim // 2,):
             raise ValueError(f"bitgpu_amd: pair_axis must hold {rot_dim // 2} axes, got shape {list(pair_axis.shape)}")
-    rc = lib().bg_paged_qkv_prologue(cache._h, li, batch._h, _ptr(q), stride, _ptr(k), _ptr(v), _ptr(q_gamma), _ptr(k_gamma),
-                                     float(eps), _ptr(cos_tab), _ptr(sin_tab), cos_tab.shape[0] if cos_tab is not None else 0,
-                                     int(rot_dim), None if pair_axis is None else pair_axis.ctypes.data, _ptr(q_out), _stream())
+        ap = pair_axis.ctypes.data
+    rc = lib().bg_paged_qkv_prologue(
+        cache._h, li, batch._h, qp, stride, _rows_ptr(k, "k", T, kw, dev), _rows_ptr(v, "v", T, kw, dev),
+        _rows_ptr(q_gamma, "q_gamma", 1, D, dev), _rows_ptr(k_gamma, "k_gamma", 1, D, dev), eps,
+        _rows_ptr(cos_tab, "cos", 0, 0, dev), _rows_ptr(sin_tab, "sin", 0, 0, dev), positions, rot_dim, ap,
+        _rows_ptr(q_out, "q_out", T, H * D, dev), _stream())
     if rc:
         check(rc)
     return q_out
@@ -727,28 +747,24 @@ def paged_attention(cache: PagedKvCache, li: int, batch: PagedBatch, q, scale: f
                     gate_stride: int | None = None, out=None):
     """:func:`attention` for a batch (bg_paged_attention): every new row of q [rows, H, D] over its
     sequence's pages up to its own position; pages that sequences share are scanned once for all. ``gate``
-    [rows, H, gate_stride] (a view into a wider row, such as the hybrid's query | gate projection, needs its
-    first row's first value at its start). Returns [rows, H, D]; rows beyond the batch's are not written."""
-    D, T = cache.head_dim, batch.n_tokens
-    _rows_at_least(q, "q", T, batch.H * D)
+    [rows, H, D], its heads ``gate_stride`` values apart (D: contiguous; 2D: the gate half of the hybrid's
+    query | gate rows). Returns [rows, H, D]; rows beyond the batch's are not written."""
+    D, H, T, dev = cache.head_dim, batch.H, batch.n_tokens, cache.index
+    qp = _rows_ptr(q, "q", T, H * D, dev)
     if out is None:
-        out = q.new_empty((q.numel() // (batch.H * D), batch.H, D))
-    _rows_at_least(out, "out", T, batch.H * D)
+        out = torch.empty_like(q) if q.dim() == 3 else q.new_empty((q.numel() // (H * D), H, D))
     gs, gp = 0, None
     if gate is not None:
         gs = int(gate_stride if gate_stride is not None else D)
         _f32(gate, "gate")
-        if not gate.is_cuda:
-            raise ValueError("bitgpu_amd: expected a device (cuda) tensor")
-        # rows [rows, H, D] whose heads are gs values apart, contiguous or a slice of rows of gs values
-        if T and (gate.dim() != 3 or gate.shape[0] < T or gate.shape[1] != batch.H or gate.shape[2] < D or gate.stride(2) != 1
-                  or (gate.stride(1) != gs and batch.H > 1) or (gate.stride(0) != batch.H * gs and gate.shape[0] > 1)):
-            raise ValueError(f"bitgpu_amd: gate must be [rows, {batch.H}, {D}] with heads {gs} values apart, got "
+        cache._one_device(gate)
+        if T and (gate.dim() != 3 or gate.shape[0] < T or gate.shape[1] != H or gate.shape[2] < D or gate.stride(2) != 1
+                  or (gate.stride(1) != gs and H > 1) or (gate.stride(0) != H * gs and gate.shape[0] > 1)):
+            raise ValueError(f"bitgpu_amd: gate must be [rows, {H}, {D}] with heads {gs} values apart, got "
                              f"{list(gate.shape)} with strides {list(gate.stride())}")
         gp = gate.data_ptr()
-    cache._one_device(q, out, gate)
-    rc = lib().bg_paged_attention(cache._h, li, batch._h, _ptr(q), float(_dense_scale(D) if scale is None else scale), gp, gs,
-                                  _ptr(out), _stream())
+    rc = lib().bg_paged_attention(cache._h, li, batch._h, qp, _dense_scale(D) if scale is None else scale, gp, gs,
+                                  _rows_ptr(out, "out", T, H * D, dev), _stream())
     if rc:
         check(rc)
     return out
