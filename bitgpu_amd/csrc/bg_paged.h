@@ -18,7 +18,7 @@ namespace bg {
 // replays is the one the replay runs.
 struct PagedHeader {
   int n_units, n_merges, n_tokens, n_v_single, n_v_group;
-  int n_many, n_merge_few, pad;  // units of 128 rows and merges of few partials (the first ones)
+  int n_many, n_mid, n_merge_few;  // units of 128 rows (the first) and of 32; merges of few partials (the first)
   float* ws_o;      // [part][head][D] unnormalized output of a partial
   float2* ws_ml;    // [part][head] its (m, l), m in base 2
 };
@@ -38,7 +38,8 @@ struct PagedBatchView {
   int page_shift;
   int H, G;
   // the set counts; all zero for a launch under capture, which reads hdr
-  int n_units, n_many, n_merges, n_merge_few, n_tokens, n_v_single, n_v_group;
+  int n_units, n_many, n_mid, n_merges, n_merge_few, n_tokens, n_v_single, n_v_group;
+  int stream_few;        // the few-row units' pages are read once, and too many to stay in a cache
   int captured;
 };
 

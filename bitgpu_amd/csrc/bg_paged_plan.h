@@ -25,8 +25,8 @@ namespace bg {
 // One workgroup's attention work, for every kv head. Positions [key0, key1) (key0 a multiple of 32) of
 // the page list at pages[table]; rows rho0 .. rho0 + n_rho - 1 of the tokens at toks[tok].
 struct PagedUnit {
-  int kind;    // 1: 16 rows, the four waves splitting the positions; 0: 128 rows, 32 a wave, the positions
-               // staged through LDS for all four
+  int kind;    // 0: 128 rows, 32 a wave, the positions staged through LDS for all four; 1, 2: 32 and 16 rows,
+               // the four waves splitting the positions
   int tok;
   int rho0, n_rho;
   int table;
@@ -55,14 +55,17 @@ struct PagedShape {
   // shared segments on one sequence's path at most (what is below them stays private)
   static constexpr int kLevels = 4;
   int max_toks() const { return max_tokens * (kLevels + 1); }
-  // units: a segment's row tiles unsplit (2 at most past the whole 128-row tiles), and what a
+  // units: a segment's row tiles unsplit (of 32 rows and more, and 2 at most for the rest), and what a
   // split adds, up to 8 units a CU
   long max_units() const {
-    return (long)max_toks() * G / 128 + 2L * (2L * max_seqs) + 8L * cus;
+    return (long)max_toks() * G / 32 + 2L * (2L * max_seqs) + 8L * cus;
   }
 };
 // storage bytes of 32 values (bg_kv dtypes: 0 f32, 1 f16, 2 q8 with its scale)
 inline int paged_bytes32(int dtype) { return dtype == 0 ? 128 : dtype == 1 ? 64 : 36; }
+
+// whether there is a kernel of 128-row units (elsewhere the 32-row ones are faster at every size)
+constexpr bool paged_has_many(int D, int dtype) { return dtype == 1 || (dtype == 0 && D == 256); }
 
 struct PagedPlan {
   std::vector<PagedUnit> units;
@@ -74,8 +77,9 @@ struct PagedPlan {
   std::vector<int> v_group;      // first tokens of 16 that fill 16 aligned slots
   int n_tokens = 0, n_parts = 0;
   int n_merge_few = 0;           // merges of at most kMergeFew partials (the first ones)
-  int n_many = 0;                // units of 128 rows (the first ones)
+  int n_many = 0, n_mid = 0;     // units of 128 rows (the first) and of 32 (the next)
   int shared_segments = 0;
+  bool stream_few = false;       // 16-row units read their pages once, over 64 MB a layer
   int64_t keys = 0;              // positions scanned, a segment's once (a kv head)
   int write_page = -1;           // a page whose new positions another sequence also lists (see below)
 };
@@ -305,16 +309,35 @@ class PagedPlanner {
     }
   }
 
-  static constexpr int kFewRows = 32;  // rows up to which few-row units take a segment, or a tile's rest
-  // a segment's units: 0 of 128 rows, 1 of 16
-  int kind(const Segment& s) const { return s.rows > kFewRows ? 0 : 1; }
-  int n_tiles(const Segment& s) const {
-    const int rest = s.rows % 128;
-    return s.rows / 128 + (rest > kFewRows ? 1 : (rest + 15) / 16);
+  // A segment's kind of units. 128-row units stage their positions once for four waves and reach the
+  // matrix cores' rate; 32-row ones need a quarter of the workgroups' partials for the same parallelism.
+  // Where both exist the work decides, rows x positions x kv heads (us, 128-row / 32-row units with their
+  // merges: f16 at 128, 8 kv heads, 128 rows over 2,048 / 8,192 / 32,768 20 / 28 / 56 and 17 / 28 / 60, 512
+  // rows 32 / 56 / 139 and 30 / 61 / 192; f16 at 256, 4 kv heads, 29 / 37 / 66 and 24 / 33 / 74; f32 at 256
+  // 54 / 68 / 207 and 37 / 85 / 274).
+  int kind(const Segment& s) const {
+    if (s.rows <= 16) return 2;
+    if (!paged_has_many(sh_.D, sh_.dtype)) return 1;
+    const double work = (double)s.rows * (s.shared ? s.key1 - s.key0 : s.key1 - s.key0 - s.n_tok / 2) * sh_.kv_heads;
+    return work > (sh_.dtype == 0 ? 2e6 : sh_.D == 128 ? 8e6 : 12e6) ? 0 : 1;
   }
-
-  // those of the segment's own kind: without a 128-row segment's few-row rest
-  int own_tiles(const Segment& s) const { return kind(s) ? n_tiles(s) : s.rows / 128 + (s.rows % 128 > kFewRows ? 1 : 0); }
+  // the unit that takes a segment's rows from r0 on: its kind and rows. What whole tiles leave over goes to
+  // the smallest kind that takes it at once.
+  int unit_kind(const Segment& s, int r0) const {
+    const int left = s.rows - r0, k = kind(s);
+    return left <= 16 ? 2 : k == 0 && left <= 32 ? 1 : k;
+  }
+  static int unit_rows(int kind) { return kind == 0 ? 128 : kind == 1 ? 32 : 16; }
+  // row tiles in all, and those of the segment's own kind
+  int n_tiles(const Segment& s) const {
+    int n = 0;
+    for (int r0 = 0; r0 < s.rows; r0 += unit_rows(unit_kind(s, r0))) n++;
+    return n;
+  }
+  int own_tiles(const Segment& s) const {
+    const int w = unit_rows(kind(s)), rest = s.rows % w;
+    return s.rows / w + (rest && unit_kind(s, s.rows - rest) == kind(s));
+  }
   // a segment's 32-position tiles
   static int tiles(const Segment& s) { return (s.key1 - s.key0 + 31) / 32; }
   static void cut(Segment& s, long len) {
@@ -325,21 +348,22 @@ class PagedPlanner {
 
   // Chunk lengths, by kind (each is a launch): the candidate with the least estimated time, in us, from
   // what the kernels measure. A launch of no more units than workgroup slots takes its longest unit, one
-  // of more the slots' share of the work and half a unit for the uneven end. A unit costs its start (its
+  // of more the slots' share of the work and part of a unit for the uneven end. A unit costs its start (its
   // descriptor, rows and queries come one after the other) and its tiles; every row of a split or shared
   // segment a partial a chunk, written and read.
   void chunk() {
-    for (int kd = 0; kd < 2; kd++) {
-      const bool many = kd == 0;
-      // a 32-position tile of a 128-row unit, two workgroups a CU at head_dim 128 (one alone 1.26 / 2.5 /
-      // 4.7) and one at 256; of a few-row unit, all slots at work at 5.6 TB/s, and alone
-      static const double kMany[2][3] = {{9.3, 2.1, 3.55}, {11.2, 2.5, 5.3}};
-      const int wide = sh_.D == 256;
-      const int per_cu = many ? (wide ? 1 : 2) : sh_.dtype == 0 ? (wide ? 1 : 2) : wide ? 2 : 3;
+    // [kind][head_dim 128, 256][dtype]: workgroups a CU, us of a 32-position tile of one unit with all of
+    // them at work, and alone on a CU. 16-row units: 5.6 TB/s, and a wave's latency.
+    static const int kSlots[3][2][3] = {{{2, 2, 2}, {1, 1, 1}}, {{2, 2, 2}, {1, 1, 2}}, {{2, 3, 3}, {1, 2, 2}}};
+    static const double kFull[2][2][3] = {{{0, 2.1, 0}, {11.2, 2.5, 0}}, {{2.5, 0.72, 0.89}, {4.2, 0.92, 2.0}}};
+    static const double kAlone[2][2][3] = {{{0, 1.26, 0}, {11.2, 2.5, 0}}, {{1.26, 0.39, 0.56}, {4.2, 0.92, 1.4}}};
+    for (int kd = 0; kd < 3; kd++) {
+      const bool few = kd == 2;
+      const int wide = sh_.D == 256, per_cu = kSlots[kd][wide][sh_.dtype];
       const double slots = std::max(1.0, (double)sh_.cus * per_cu);
-      const double full = many ? kMany[wide][sh_.dtype] : 2.0 * (sh_.D / 32) * paged_bytes32(sh_.dtype) * 32 * slots / 5.6e6;
-      const double alone = many ? (wide ? full : full * (sh_.dtype == 0 ? 0.5 : sh_.dtype == 1 ? 0.6 : 0.7)) : 0.5;
-      const double start = many ? 6 : 5;
+      const double full = few ? 2.0 * (sh_.D / 32) * paged_bytes32(sh_.dtype) * 32 * slots / 5.6e6 : kFull[kd][wide][sh_.dtype];
+      const double alone = few ? 0.5 : kAlone[kd][wide][sh_.dtype];
+      const double start = kd == 0 ? 6 : kd == 1 ? 7 : 5;
       double work = 0;
       long longest = 1, tiles1 = 0;
       for (const Segment& s : segs_) {
@@ -351,7 +375,7 @@ class PagedPlanner {
       if (tiles1 == 0) continue;
       double best = 1e30;
       long best_len = longest;
-      for (long len = many && !wide ? 8 : 4; len < 2 * longest; len = len * 9 / 8 + 1) {
+      for (long len = kd == 0 && !wide ? 8 : 4; len < 2 * longest; len = len * 9 / 8 + 1) {
         double units = 0, rows = 0;
         long most = 1;
         for (Segment& s : segs_) {
@@ -363,10 +387,10 @@ class PagedPlanner {
         }
         double t;
         if (units <= slots) {
-          const double rate = many ? (units * per_cu <= slots ? alone : full) : std::max(alone, full * units / slots);
+          const double rate = !few ? (units * per_cu <= slots ? alone : full) : std::max(alone, full * units / slots);
           t = start + most * rate;
         } else {
-          t = work * full / slots + start * (1 + units / slots) + (many ? 0.5 : 0.15) * most * full;
+          t = work * full / slots + start * (1 + units / slots) + (few ? 0.15 : 0.5) * most * full;
         }
         t += rows * (sh_.D + 2) * 4 * (1 / 5.0e6 + 1 / 4.0e6);
         if (t < best) {
@@ -413,17 +437,15 @@ class PagedPlanner {
         if (base_[k.t] >= 0) base_[k.t] += s.chunks;
       }
     }
-    // units by kind (128 rows, 16 rows), the heaviest first
+    // units by kind (128, 32, 16 rows), the heaviest first
     cost_.clear();
     for (const Segment& s : segs_) {
       out.keys += s.key1 - s.key0;
       for (int c = 0; c < s.chunks; c++) {
         for (int r0 = 0, R; r0 < s.rows; r0 += R) {
-          // what 128-row tiles leave over runs as few-row units where it is that few
-          const bool many = s.rows - r0 > kFewRows;
-          R = many ? 128 : 16;
           PagedUnit u{};
-          u.kind = many ? 0 : 1;
+          u.kind = unit_kind(s, r0);
+          R = unit_rows(u.kind);
           u.tok = s.tok;
           u.rho0 = r0;
           u.n_rho = std::min(R, s.rows - r0);
@@ -447,8 +469,19 @@ class PagedPlanner {
       return ka != kb ? ka < kb : cost_[a] > cost_[b];
     });
     sorted_.clear();
-    out.n_many = 0;
-    for (int i : order_) out.n_many += out.units[i].kind == 0;
+    out.n_many = out.n_mid = 0;
+    for (int i : order_) {
+      out.n_many += out.units[i].kind == 0;
+      out.n_mid += out.units[i].kind == 1;
+    }
+    // 16-row units: pages of their own, or the rest of a segment whose other units read the same
+    bool once = true;
+    double bytes = 0;
+    for (const Segment& s : segs_) {
+      if (kind(s) == 2) bytes += (double)(s.key1 - s.key0) * sh_.kv_heads * 2 * (sh_.D / 32) * paged_bytes32(sh_.dtype);
+      else if (own_tiles(s) < n_tiles(s)) once = false;
+    }
+    out.stream_few = once && bytes > 64e6;
     for (int i : order_) sorted_.push_back(out.units[i]);
     out.units.swap(sorted_);
   }

@@ -97,9 +97,11 @@ struct bg_paged_batch {
     b.H = H;
     b.G = shape.G;
     b.captured = captured;
+    b.stream_few = plan.stream_few;
     if (!captured) {
       b.n_units = (int)plan.units.size();
       b.n_many = plan.n_many;
+      b.n_mid = plan.n_mid;
       b.n_merges = (int)plan.merges.size();
       b.n_merge_few = plan.n_merge_few;
       b.n_tokens = plan.n_tokens;
@@ -342,6 +344,7 @@ int32_t bg_paged_batch_set(bg_paged_batch* b, int32_t n_seqs, const int32_t* row
   bg::PagedHeader hdr{};
   hdr.n_units = (int)p.units.size();
   hdr.n_many = p.n_many;
+  hdr.n_mid = p.n_mid;
   hdr.n_merge_few = p.n_merge_few;
   hdr.n_merges = (int)p.merges.size();
   hdr.n_tokens = T;

@@ -27,6 +27,7 @@
 // Masked positions: scores are replaced, not added to; V beyond the positions written so far (a page's
 // stale or never written slots, possibly NaN) is replaced by zero, its q8 scales too.
 #include <algorithm>
+#include <type_traits>
 
 #include "bg_paged.h"
 
@@ -160,12 +161,11 @@ __device__ inline int slot16(int g, int i) { return 16 * (g >> 1) + 8 * (i >> 2)
 // a 128-row unit's staging
 template <int D, int DT>
 struct Many {
-  static constexpr int EB = DT == KV_F32 ? 4 : 2;               // bytes of a staged value (q8 codes as f16)
+  static constexpr int EB = DT == KV_F32 ? 4 : 2;               // bytes of a staged value
   static constexpr int KT = DT == KV_F32 || D == 256 ? 32 : 64; // positions a step
   static constexpr int NSUB = KT / 32;
   static constexpr int SUB = 32 * D * EB;                       // bytes of a staged 32-position tile of K (or V)
   static constexpr int CPR = D * EB / 16;                       // 16-byte chunks of a K row
-  static constexpr int SCALES = DT == KV_Q8 ? KT * (D / 32) * 4 : 0;  // bytes of a step's K (or V) scales
 };
 
 // ------------------------------------------------------------------------------------------ few
@@ -183,8 +183,9 @@ struct FewTile {
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t tile_rsrc(const void* base, int bytes) {
   return __builtin_amdgcn_make_buffer_rsrc((void*)base, (short)0, bytes, 0x00020000);
 }
+template <int AUX = 0>
 __device__ __forceinline__ u32x4 ld16(__amdgpu_buffer_rsrc_t r, int off, int more) {
-  return __builtin_amdgcn_raw_buffer_load_b128(r, off, more, 0);
+  return __builtin_amdgcn_raw_buffer_load_b128(r, off, more, AUX);
 }
 __device__ __forceinline__ u32x2 ld8(__amdgpu_buffer_rsrc_t r, int off, int more) {
   return __builtin_amdgcn_raw_buffer_load_b64(r, off, more, 0);
@@ -204,7 +205,7 @@ __device__ __forceinline__ void few_load_scales(const float* base, size_t row, b
   }
 }
 
-template <int D, int DT>
+template <int D, int DT, int AUX>
 __device__ __forceinline__ void few_load_k(const PagedKernelArgs& p, size_t row, bool on, int c, int g, FewTile<D, DT>& t) {
   // operand row c of product i is slot slot16(c / 4, 4 i + c % 4); the k dimension of a lane group is
   // 8 g + e of every 32 dims (f32: 4 g + e of every 16)
@@ -215,12 +216,12 @@ __device__ __forceinline__ void few_load_k(const PagedKernelArgs& p, size_t row,
 #pragma unroll
     for (int i = 0; i < 2; i++)
 #pragma unroll
-      for (int j = 0; j < D / 16; j++) t.k[i * (D / 16) + j] = ld16(r, (s0 * D + 4 * g) * 4, (8 * i * D + 16 * j) * 4);
+      for (int j = 0; j < D / 16; j++) t.k[i * (D / 16) + j] = ld16<AUX>(r, (s0 * D + 4 * g) * 4, (8 * i * D + 16 * j) * 4);
   } else if constexpr (DT == KV_F16) {
 #pragma unroll
     for (int i = 0; i < 2; i++)
 #pragma unroll
-      for (int j = 0; j < D / 32; j++) t.k[i * (D / 32) + j] = ld16(r, (s0 * D + 8 * g) * 2, (8 * i * D + 32 * j) * 2);
+      for (int j = 0; j < D / 32; j++) t.k[i * (D / 32) + j] = ld16<AUX>(r, (s0 * D + 8 * g) * 2, (8 * i * D + 32 * j) * 2);
   } else {
 #pragma unroll
     for (int i = 0; i < 2; i++)
@@ -230,7 +231,7 @@ __device__ __forceinline__ void few_load_k(const PagedKernelArgs& p, size_t row,
   }
 }
 
-template <int D, int DT>
+template <int D, int DT, int AUX>
 __device__ __forceinline__ void few_load_v(const PagedKernelArgs& p, size_t row, bool on, int c, int g, FewTile<D, DT>& t) {
   constexpr int EB = DT == KV_F32 ? 4 : DT == KV_F16 ? 2 : 1;
   const __amdgpu_buffer_rsrc_t r = tile_rsrc(p.v + row * D * EB, on ? 32 * D * EB : 0);
@@ -238,12 +239,12 @@ __device__ __forceinline__ void few_load_v(const PagedKernelArgs& p, size_t row,
   if constexpr (DT == KV_F32) {
 #pragma unroll
     for (int j = 0; j < D / 16; j++) {
-      t.v[2 * j] = ld16(r, off, 128 * 4 * j);
-      t.v[2 * j + 1] = ld16(r, off, 128 * 4 * j + 16);
+      t.v[2 * j] = ld16<AUX>(r, off, 128 * 4 * j);
+      t.v[2 * j + 1] = ld16<AUX>(r, off, 128 * 4 * j + 16);
     }
   } else if constexpr (DT == KV_F16) {
 #pragma unroll
-    for (int j = 0; j < D / 16; j++) t.v[j] = ld16(r, off, 128 * 2 * j);
+    for (int j = 0; j < D / 16; j++) t.v[j] = ld16<AUX>(r, off, 128 * 2 * j);
   } else {
 #pragma unroll
     for (int j = 0; j < D / 16; j++) t.vc[j] = ld8(r, off, 128 * j);
@@ -272,7 +273,7 @@ union FewLds {
 template <int D, int DT>
 constexpr int few_waves() { return D == 256 ? (DT == KV_F32 ? 1 : 2) : DT == KV_F32 ? 2 : 3; }
 
-template <int D, int DT>
+template <int D, int DT, int AUX>
 __device__ __forceinline__ void few_unit(const PagedKernelArgs& p, const PagedUnit& u, int kvh, float* ws_o, float2* ws_ml,
                                          FewLds<D, DT>& lds) {
   constexpr int NK = DT == KV_F32 ? D / 16 : D / 32;
@@ -290,8 +291,8 @@ __device__ __forceinline__ void few_unit(const PagedKernelArgs& p, const PagedUn
   FewTile<D, DT> tl;
   if (n_tiles > 0) {
     const size_t row = row_of(wave);
-    few_load_k<D, DT>(p, row, wave < n_tiles, c, g, tl);
-    few_load_v<D, DT>(p, row, wave < n_tiles, c, g, tl);
+    few_load_k<D, DT, AUX>(p, row, wave < n_tiles, c, g, tl);
+    few_load_v<D, DT, AUX>(p, row, wave < n_tiles, c, g, tl);
   }
 
   // ---- the queries: every wave looks at all of them (each row's factor), prepares its share
@@ -426,7 +427,7 @@ __device__ __forceinline__ void few_unit(const PagedKernelArgs& p, const PagedUn
       }
     }
     __builtin_amdgcn_sched_barrier(0);  // into the registers just used: not before, which would take a second set
-    few_load_k<D, DT>(p, next, more, c, g, tl);
+    few_load_k<D, DT, AUX>(p, next, more, c, g, tl);
     __builtin_amdgcn_sched_barrier(0);
     if (key + 32 > u.mask0) {
 #pragma unroll
@@ -536,7 +537,7 @@ __device__ __forceinline__ void few_unit(const PagedKernelArgs& p, const PagedUn
       }
     }
     __builtin_amdgcn_sched_barrier(0);
-    few_load_v<D, DT>(p, next, more, c, g, tl);
+    few_load_v<D, DT, AUX>(p, next, more, c, g, tl);
     __builtin_amdgcn_sched_barrier(0);
   }
 
@@ -578,6 +579,397 @@ __device__ __forceinline__ void few_unit(const PagedKernelArgs& p, const PagedUn
   }
 }
 
+// ------------------------------------------------------------------------------------------ mid
+// A wave's 32-position tile as operands of the 32-row products (descriptors as for the few-row units): K
+// row c, dims 16 n + 8 h + e (f32 8 n + 4 h + e, q8 32 n + 16 h + e); V dim 32 j + c, panel 2 x + h.
+template <int D, int DT>
+struct MidTile {
+  static constexpr int NK = DT == KV_F32 ? D / 8 : DT == KV_F16 ? D / 16 : D / 32;
+  static constexpr int NV = 2 * (D / 32);
+  u32x4 k[NK], v[DT == KV_F32 ? 2 * NV : DT == KV_F16 ? NV : 1];
+  u32x2 vc[DT == KV_Q8 ? NV : 1];
+  float ks[DT == KV_Q8 ? D / 64 : 1], vs[DT == KV_Q8 ? D / 64 : 1];
+};
+
+template <int D, int DT>
+__device__ __forceinline__ void mid_load_k(const PagedKernelArgs& p, size_t row, bool on, int c, int h, MidTile<D, DT>& t) {
+  constexpr int EB = DT == KV_F32 ? 4 : DT == KV_F16 ? 2 : 1;
+  const __amdgpu_buffer_rsrc_t r = tile_rsrc(p.k + row * D * EB, on ? 32 * D * EB : 0);
+#pragma unroll
+  for (int n = 0; n < MidTile<D, DT>::NK; n++) t.k[n] = ld16(r, c * D * EB + 16 * h, 32 * n);
+  if constexpr (DT == KV_Q8) few_load_scales<D, DT>(p.ks, row, on, c + 32 * h, t.ks);
+}
+template <int D, int DT>
+__device__ __forceinline__ void mid_load_v(const PagedKernelArgs& p, size_t row, bool on, int c, int h, MidTile<D, DT>& t) {
+  constexpr int EB = DT == KV_F32 ? 4 : DT == KV_F16 ? 2 : 1;
+  const __amdgpu_buffer_rsrc_t r = tile_rsrc(p.v + row * D * EB, on ? 32 * D * EB : 0);
+  const int off = (h * D + c) * 8 * EB;
+#pragma unroll
+  for (int x = 0; x < 2; x++)
+#pragma unroll
+    for (int j = 0; j < D / 32; j++) {
+      const int at = (2 * x * D + 32 * j) * 8 * EB;
+      if constexpr (DT == KV_F32) {
+        t.v[2 * (x * (D / 32) + j)] = ld16(r, off, at);
+        t.v[2 * (x * (D / 32) + j) + 1] = ld16(r, off, at + 16);
+      } else if constexpr (DT == KV_F16) {
+        t.v[x * (D / 32) + j] = ld16(r, off, at);
+      } else {
+        t.vc[x * (D / 32) + j] = ld8(r, off, at);
+      }
+    }
+  if constexpr (DT == KV_Q8) few_load_scales<D, DT>(p.vs, row, on, c + 32 * h, t.vs);
+}
+
+template <int D, int DT>
+union MidLds {
+  static constexpr int NQ = DT == KV_F32 ? D / 8 : 2 * (D / 16);
+  struct {
+    u32x4 q[NQ][64];                           // the queries as matrix operands, the same for every wave
+    float s[DT == KV_Q8 ? 4 : 1][2][DT == KV_Q8 ? D : 1];  // q8: K and V scales of the tile a wave is at
+  } in;
+  f32x4 x[4][D / 64 * 4][64];                  // half of every wave's o, on its way to another wave
+};
+
+template <int D, int DT>
+__device__ __forceinline__ void mid_unit(const PagedKernelArgs& p, const PagedUnit& u, int kvh, float* ws_o, float2* ws_ml,
+                                         MidLds<D, DT>& lds, float2 (*lml)[32]) {
+  using T = MidTile<D, DT>;
+  constexpr int ND = D / 32;
+  const int wave = uniform(threadIdx.x >> 6), lane = threadIdx.x & 63, c = lane & 31, h = lane >> 5;
+  const int shift = p.b.page_shift, P = 1 << shift;
+  const int n_tiles = (u.key1 - u.key0 + 31) >> 5;
+  const int* pages = p.b.pages + u.table;
+  auto row_of = [&](int t) -> size_t {
+    const int key = u.key0 + 32 * min(t, n_tiles - 1);
+    const int id = uniform(pages[key >> shift]);
+    return ((size_t)id * p.kv_heads + kvh) * P + (key & (P - 1));
+  };
+  T tl;
+  if (n_tiles > 0) {
+    const size_t row = row_of(wave);
+    mid_load_k<D, DT>(p, row, wave < n_tiles, c, h, tl);
+    mid_load_v<D, DT>(p, row, wave < n_tiles, c, h, tl);
+  }
+  // ---- the queries: every wave looks at all of them (each row's factor), prepares its share
+  const RowAt ra = row_at(p, u, kvh, c);
+  int pos;
+  float qs;
+  {
+    const int rho = u.rho0 + (ra.on ? c : 0);
+    pos = p.b.toks[u.tok + rho / p.b.G].pos;
+    const float* q = p.q + ((size_t)ra.t * p.b.H + ra.head) * D;
+    if constexpr (DT == KV_F32) {
+#pragma unroll
+      for (int n = 0; n < D / 8; n++)
+        if ((n & 3) == wave) lds.in.q[n][lane] = *(const u32x4*)(q + 8 * n + 4 * h);
+      qs = p.qscale;
+    } else {
+      float top = 0.0f;
+#pragma unroll 4
+      for (int n = 0; n < D / 8; n++) {
+        const f32x4 a = *(const f32x4*)(q + 8 * n + 4 * h);
+#pragma unroll
+        for (int e = 0; e < 4; e++) top = fmaxf(top, fabsf(a[e]));
+      }
+      const float2 r = pair32(top);
+      top = fmaxf(r.x, r.y);
+      float undo;
+      const float f = row_factor(top, &undo);
+      qs = p.qscale * undo * (DT == KV_Q8 ? 1.0f / 127.0f : 1.0f);
+#pragma unroll
+      for (int n = 0; n < D / 16; n++) {  // product n: f16 dims 16 n + 8 h; q8 block n / 2, dims 16 h + 8 (n & 1)
+        if ((n & 3) == wave) {
+          const float* at = q + (DT == KV_F16 ? 16 * n + 8 * h : 32 * (n >> 1) + 16 * h + 8 * (n & 1));
+          const f32x4 a = *(const f32x4*)at, b = *(const f32x4*)(at + 4);
+          float y[8];
+#pragma unroll
+          for (int e = 0; e < 4; e++) {
+            y[e] = a[e] * f;
+            y[4 + e] = b[e] * f;
+          }
+          H8 hi, lo;
+          split8(y, hi, lo);
+          lds.in.q[2 * n][lane] = hi.u;
+          lds.in.q[2 * n + 1][lane] = lo.u;
+        }
+      }
+    }
+  }
+  __syncthreads();
+  auto q_at = [&](int n, int part) __attribute__((always_inline)) {
+    H8 x;
+    x.u = lds.in.q[2 * n + part][lane];
+    return x.h;
+  };
+
+  f32x16 o[ND];
+#pragma unroll
+  for (int j = 0; j < ND; j++)
+#pragma unroll
+    for (int e = 0; e < 16; e++) o[j][e] = 0.0f;
+  float m = -INFINITY, l = 0.0f, ev = -60.0f;  // q8: 2^ev is above every value scale so far
+
+  for (int t = wave; t < n_tiles; t += 4) {
+    const int key = u.key0 + 32 * t;
+    const bool more = t + 4 < n_tiles;
+    const size_t next = row_of(t + 4);
+    float* lk = lds.in.s[DT == KV_Q8 ? wave : 0][0];
+    float* lv = lds.in.s[DT == KV_Q8 ? wave : 0][1];
+    if constexpr (DT == KV_Q8) {
+      // [block][position], so that a lane reads the four positions of a register group at once; a wave's
+      // LDS accesses complete in order: the tile before is done with them
+#pragma unroll
+      for (int i = 0; i < D / 64; i++) {
+        const int x = lane * (D / 64) + i, at = x % (D / 32) * 32 + x / (D / 32);
+        lk[at] = tl.ks[i];
+        lv[at] = tl.vs[i];
+      }
+      __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+      __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    }
+    // ---- scores: s[e] of slot 8 (e / 4) + 4 h + e % 4, row c
+    float s[16];
+    if constexpr (DT == KV_F32) {
+      f32x16 a;
+#pragma unroll
+      for (int e = 0; e < 16; e++) a[e] = 0.0f;
+#pragma unroll
+      for (int n = 0; n < D / 8; n++) {
+        const f32x4 qn = *(const f32x4*)&lds.in.q[n][lane];
+#pragma unroll
+        for (int e = 0; e < 4; e++) a = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(tl.k[n][e]), qn[e], a, 0, 0, 0);
+      }
+#pragma unroll
+      for (int e = 0; e < 16; e++) s[e] = a[e];
+    } else if constexpr (DT == KV_F16) {
+      f32x16 a;
+#pragma unroll
+      for (int e = 0; e < 16; e++) a[e] = 0.0f;
+#pragma unroll
+      for (int n = 0; n < D / 16; n++) {
+        H8 x;
+        x.u = tl.k[n];
+        a = __builtin_amdgcn_mfma_f32_32x32x16_f16(x.h, q_at(n, 0), a, 0, 0, 0);
+        a = __builtin_amdgcn_mfma_f32_32x32x16_f16(x.h, q_at(n, 1), a, 0, 0, 0);
+      }
+#pragma unroll
+      for (int e = 0; e < 16; e++) s[e] = a[e];
+    } else {
+#pragma unroll
+      for (int e = 0; e < 16; e++) s[e] = 0.0f;
+#pragma unroll
+      for (int b = 0; b < ND; b++) {
+        const half8 x0 = codes8(u32x2{tl.k[b][0], tl.k[b][1]}), x1 = codes8(u32x2{tl.k[b][2], tl.k[b][3]});
+        f32x16 a;
+#pragma unroll
+        for (int e = 0; e < 16; e++) a[e] = 0.0f;
+        a = __builtin_amdgcn_mfma_f32_32x32x16_f16(x0, q_at(2 * b, 0), a, 0, 0, 0);
+        a = __builtin_amdgcn_mfma_f32_32x32x16_f16(x0, q_at(2 * b, 1), a, 0, 0, 0);
+        a = __builtin_amdgcn_mfma_f32_32x32x16_f16(x1, q_at(2 * b + 1, 0), a, 0, 0, 0);
+        a = __builtin_amdgcn_mfma_f32_32x32x16_f16(x1, q_at(2 * b + 1, 1), a, 0, 0, 0);
+#pragma unroll
+        for (int w = 0; w < 4; w++) {
+          const f32x4 z = *(const f32x4*)(lk + 32 * b + 8 * w + 4 * h);
+#pragma unroll
+          for (int e = 0; e < 4; e++) s[4 * w + e] = fmaf(a[4 * w + e], z[e], s[4 * w + e]);
+        }
+      }
+    }
+    __builtin_amdgcn_sched_barrier(0);  // into the registers just used: not before, which would take a second set
+    mid_load_k<D, DT>(p, next, more, c, h, tl);
+    __builtin_amdgcn_sched_barrier(0);
+    if (key + 32 > u.mask0) {
+#pragma unroll
+      for (int e = 0; e < 16; e++) s[e] = key + 8 * (e >> 2) + 4 * h + (e & 3) <= pos ? s[e] : -INFINITY;
+    }
+    if (key + 32 > u.key1) {  // slots past the written positions
+      if constexpr (DT == KV_F32) {
+#pragma unroll
+        for (int x = 0; x < 2; x++)
+#pragma unroll
+          for (int j = 0; j < ND; j++)
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+              const int i = 2 * (x * ND + j) + (e >> 2);
+              tl.v[i][e & 3] = key + 16 * x + 8 * (e >> 2) + 4 * h + (e & 3) < u.key1 ? tl.v[i][e & 3] : 0u;
+            }
+      } else if constexpr (DT == KV_F16) {
+#pragma unroll
+        for (int x = 0; x < 2; x++) {
+          u32x4 keep;
+#pragma unroll
+          for (int w = 0; w < 4; w++) {
+            const int at = key + 16 * x + 8 * (w >> 1) + 4 * h + 2 * (w & 1);
+            keep[w] = (at < u.key1 ? 0xffffu : 0u) | (at + 1 < u.key1 ? 0xffff0000u : 0u);
+          }
+#pragma unroll
+          for (int j = 0; j < ND; j++) tl.v[x * ND + j] &= keep;
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < D / 64; i++) {
+          const int x = lane * (D / 64) + i;
+          if (key + x / (D / 32) >= u.key1) {
+            tl.vs[i] = 0.0f;
+            lv[x % (D / 32) * 32 + x / (D / 32)] = 0.0f;
+          }
+        }
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+      }
+    }
+    // ---- running maximum and sum
+    float top = s[0];
+#pragma unroll
+    for (int e = 1; e < 16; e++) top = fmaxf(top, s[e]);
+    const float2 r = pair32(top);
+    top = fmaxf(r.x, r.y) * qs;
+    float en = ev;
+    if constexpr (DT == KV_Q8) {
+      float big = tl.vs[0];
+#pragma unroll
+      for (int i = 1; i < D / 64; i++) big = fmaxf(big, tl.vs[i]);
+      en = fmaxf(ev, scale_exponent(wave_max(big)));
+    }
+    if (__any(top > m + kLazy || en > ev)) {
+      const float mn = top > m + kLazy ? top : m;
+      const float f = m == -INFINITY ? 1.0f : exp2_hw(m - mn + (DT == KV_Q8 ? ev - en : 0.0f));
+      m = mn;
+      ev = en;
+      l *= f;
+#pragma unroll
+      for (int j = 0; j < ND; j++) o[j] *= f;
+    }
+    const float base = m == -INFINITY ? 0.0f : kPShift - m - (DT == KV_Q8 ? ev : 0.0f);
+#pragma unroll
+    for (int e = 0; e < 16; e++) {
+      s[e] = exp2_hw(fmaf(s[e], qs, base));
+      l += s[e];
+    }
+    // ---- o
+#pragma unroll
+    for (int x = 0; x < 2; x++) {
+      if constexpr (DT == KV_F32) {
+#pragma unroll
+        for (int e = 0; e < 8; e++)
+#pragma unroll
+          for (int j = 0; j < ND; j++)
+            o[j] = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(tl.v[2 * (x * ND + j) + (e >> 2)][e & 3]), s[8 * x + e],
+                                                        o[j], 0, 0, 0);
+      } else if constexpr (DT == KV_F16) {
+        float w[8];
+#pragma unroll
+        for (int e = 0; e < 8; e++) w[e] = s[8 * x + e];
+        H8 ph, pl;
+        split8(w, ph, pl);
+#pragma unroll
+        for (int j = 0; j < ND; j++) {
+          H8 a;
+          a.u = tl.v[x * ND + j];
+          o[j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a.h, ph.h, o[j], 0, 0, 0);
+        }
+#pragma unroll
+        for (int j = 0; j < ND; j++) {
+          H8 a;
+          a.u = tl.v[x * ND + j];
+          o[j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a.h, pl.h, o[j], 0, 0, 0);
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < ND; j++) {
+          float w[8];
+#pragma unroll
+          for (int y = 0; y < 2; y++) {
+            const f32x4 z = *(const f32x4*)(lv + 32 * j + 16 * x + 8 * y + 4 * h);
+#pragma unroll
+            for (int e = 0; e < 4; e++) w[4 * y + e] = s[8 * x + 4 * y + e] * z[e];
+          }
+          H8 ph, pl;
+          split8(w, ph, pl);
+          const half8 a = codes8(tl.vc[x * ND + j]);
+          o[j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, ph.h, o[j], 0, 0, 0);
+          o[j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, pl.h, o[j], 0, 0, 0);
+        }
+      }
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    mid_load_v<D, DT>(p, next, more, c, h, tl);
+    __builtin_amdgcn_sched_barrier(0);
+  }
+
+  // ---- the four waves' results: all weighted by one maximum, then halves of o exchanged with the wave
+  // two away and quarters with the next one, so that each ends with the sum of a quarter of the dims
+  if constexpr (DT == KV_Q8) m += ev;
+  {
+    const float2 r = pair32(l);
+    l = r.x + r.y;
+  }
+  if (h == 0) lml[wave][c] = make_float2(m, l);
+  __syncthreads();  // and every wave is done with the queries and its scales
+  float top = -INFINITY, lsum = 0.0f;
+  float2 z[4];
+#pragma unroll
+  for (int w = 0; w < 4; w++) {
+    z[w] = lml[w][c];
+    top = fmaxf(top, z[w].x);
+  }
+#pragma unroll
+  for (int w = 0; w < 4; w++) lsum += z[w].x == -INFINITY ? 0.0f : z[w].y * exp2_hw(z[w].x - top);
+  const float mine = (m == -INFINITY ? 0.0f : exp2_hw(m - top)) * (DT == KV_Q8 ? 1.0f / 127.0f : 1.0f);
+#pragma unroll
+  for (int j = 0; j < ND; j++) o[j] *= mine;
+  auto send = [&](auto from, auto n) __attribute__((always_inline)) {
+#pragma unroll
+    for (int j = 0; j < n; j++)
+#pragma unroll
+      for (int w = 0; w < 4; w++)
+        lds.x[wave][4 * j + w][lane] = f32x4{o[from + j][4 * w], o[from + j][4 * w + 1], o[from + j][4 * w + 2], o[from + j][4 * w + 3]};
+  };
+  auto add = [&](auto to, auto n, int other) __attribute__((always_inline)) {
+#pragma unroll
+    for (int j = 0; j < n; j++)
+#pragma unroll
+      for (int w = 0; w < 4; w++) {
+        const f32x4 y = lds.x[other][4 * j + w][lane];
+#pragma unroll
+        for (int e = 0; e < 4; e++) o[to + j][4 * w + e] += y[e];
+      }
+  };
+  auto put = [&](auto at, auto n) __attribute__((always_inline)) {
+    if (!ra.on) return;
+#pragma unroll
+    for (int j = 0; j < n; j++)
+#pragma unroll
+      for (int w = 0; w < 4; w++)
+        store_o<D>(p, ws_o, ra, 32 * (at + j) + 8 * w + 4 * h,
+                   f32x4{o[at + j][4 * w], o[at + j][4 * w + 1], o[at + j][4 * w + 2], o[at + j][4 * w + 3]}, lsum);
+  };
+  constexpr int Q = ND / 4;  // 32-dim groups a wave ends with
+  using I0 = std::integral_constant<int, 0>;
+  using I1 = std::integral_constant<int, Q>;
+  using I2 = std::integral_constant<int, 2 * Q>;
+  using I3 = std::integral_constant<int, 3 * Q>;
+  if (wave < 2) send(I2{}, I2{});
+  else send(I0{}, I2{});
+  __syncthreads();
+  if (wave < 2) add(I0{}, I2{}, wave + 2);
+  else add(I2{}, I2{}, wave - 2);
+  __syncthreads();
+  if (wave == 0) send(I1{}, I1{});
+  else if (wave == 1) send(I0{}, I1{});
+  else if (wave == 2) send(I3{}, I1{});
+  else send(I2{}, I1{});
+  __syncthreads();
+  if (wave == 0) { add(I0{}, I1{}, 1); put(I0{}, I1{}); }
+  else if (wave == 1) { add(I1{}, I1{}, 0); put(I1{}, I1{}); }
+  else if (wave == 2) { add(I2{}, I1{}, 3); put(I2{}, I1{}); }
+  else { add(I3{}, I1{}, 2); put(I3{}, I1{}); }
+  if (wave == 0 && h == 0 && ra.on && ra.part >= 0) ws_ml[(size_t)ra.part * p.b.H + ra.head] = make_float2(top, lsum);
+}
+
 // ------------------------------------------------------------------------------------------ many
 template <int D, int DT>
 __device__ __forceinline__ void many_stage(const PagedKernelArgs& p, size_t row, char* kd, char* vd) {
@@ -597,53 +989,9 @@ __device__ __forceinline__ void many_stage(const PagedKernelArgs& p, size_t row,
   }
 }
 
-// q8: a thread's share of a staged 32-position tile, through registers
-template <int D>
-struct ManyQ8 {
-  static constexpr int N = 32 * D / 16 / 256 > 0 ? 32 * D / 16 / 256 : 1;
-  u32x4 k[N], v[N];
-  float ks, vs;
-};
-template <int D>
-__device__ __forceinline__ void many_load_q8(const PagedKernelArgs& p, size_t row, ManyQ8<D>& r) {
-  const int t = threadIdx.x;
-#pragma unroll
-  for (int i = 0; i < ManyQ8<D>::N; i++) {
-    r.k[i] = *(const u32x4*)(p.k + row * D + (size_t)(t + 256 * i) * 16);
-    r.v[i] = *(const u32x4*)(p.v + row * D + (size_t)(t + 256 * i) * 16);
-  }
-  const int n = t & (D - 1);  // 32 positions x D / 32 scales
-  r.ks = p.ks[row * (D / 32) + n];
-  r.vs = p.vs[row * (D / 32) + n];
-}
-// scales are staged [block][position], so that a lane reads the four positions of a register group at once
-template <int D>
-__device__ __forceinline__ void many_store_q8(const ManyQ8<D>& r, char* kd, char* vd, float* ksd, float* vsd, int KT) {
-  const int t = threadIdx.x;
-#pragma unroll
-  for (int i = 0; i < ManyQ8<D>::N; i++) {
-    const int x = t + 256 * i;              // 16 codes: half a K row's 32 ..., two dims' 8 slots of V
-    const int row = x / (D / 16), c0 = 2 * (x % (D / 16));
-    H8 a, b;
-    a.h = codes8(u32x2{r.k[i][0], r.k[i][1]});
-    b.h = codes8(u32x2{r.k[i][2], r.k[i][3]});
-    *(u32x4*)(kd + (row * (D / 8) + swz(row, c0)) * 16) = a.u;
-    *(u32x4*)(kd + (row * (D / 8) + swz(row, c0 + 1)) * 16) = b.u;
-    a.h = codes8(u32x2{r.v[i][0], r.v[i][1]});
-    b.h = codes8(u32x2{r.v[i][2], r.v[i][3]});
-    *(u32x4*)(vd + (size_t)x * 32) = a.u;
-    *(u32x4*)(vd + (size_t)x * 32 + 16) = b.u;
-  }
-  if (t < D) {
-    const int s = t / (D / 32), blk = t % (D / 32);
-    ksd[blk * KT + s] = r.ks;
-    vsd[blk * KT + s] = r.vs;
-  }
-}
-
 template <int D, int DT>
 __device__ __forceinline__ void many_unit(const PagedKernelArgs& p, const PagedUnit& u, int kvh, float* ws_o, float2* ws_ml,
-                                          char* k0, char* k1, char* v0, char* v1, float* scales) {
+                                          char* k0, char* k1, char* v0, char* v1) {
   using M = Many<D, DT>;
   constexpr int KT = M::KT, NSUB = M::NSUB;
   constexpr int NK = DT == KV_F32 ? D / 8 : D / 16;   // f32: 16-byte chunks a lane; else 16-dim products
@@ -678,7 +1026,7 @@ __device__ __forceinline__ void many_unit(const PagedKernelArgs& p, const PagedU
       top = fmaxf(r.x, r.y);
       float undo;
       const float f = row_factor(top, &undo);
-      qs = p.qscale * undo * (DT == KV_Q8 ? 1.0f / 127.0f : 1.0f);
+      qs = p.qscale * undo;
 #pragma unroll
       for (int n = 0; n < NK; n++) {  // read again: half the registers of holding the row in f32
         const f32x4 a = *(const f32x4*)(q + 16 * n + 8 * h), b = *(const f32x4*)(q + 16 * n + 8 * h + 4);
@@ -697,7 +1045,7 @@ __device__ __forceinline__ void many_unit(const PagedKernelArgs& p, const PagedU
   for (int j = 0; j < D / 32; j++)
 #pragma unroll
     for (int e = 0; e < 16; e++) o[j][e] = 0.0f;
-  float m = -INFINITY, l = 0.0f, ev = -60.0f;  // q8: 2^ev is above every value scale so far
+  float m = -INFINITY, l = 0.0f;
 
   auto row_of = [&](int t) -> size_t {
     const int key = u.key0 + 32 * min(t, n_tiles - 1);  // past the end: staged again, masked
@@ -706,7 +1054,7 @@ __device__ __forceinline__ void many_unit(const PagedKernelArgs& p, const PagedU
   };
 
   // one step over staged tiles; key: its first position
-  auto step = [&](const char* kb, const char* vb, const float* ksb, const float* vsb, int key) __attribute__((always_inline)) {
+  auto step = [&](const char* kb, const char* vb, int key) __attribute__((always_inline)) {
     float s[NSUB][16];
     if constexpr (DT == KV_F16) {
       // both sub-tiles' chains side by side, their operands read two chunks ahead
@@ -753,28 +1101,6 @@ __device__ __forceinline__ void many_unit(const PagedKernelArgs& p, const PagedU
         }
 #pragma unroll
         for (int e = 0; e < 16; e++) s[sub][e] = a[e];
-      } else if constexpr (DT == KV_Q8) {
-#pragma unroll
-        for (int e = 0; e < 16; e++) s[sub][e] = 0.0f;
-#pragma unroll
-        for (int blk = 0; blk < D / 32; blk++) {
-          f32x16 a;
-#pragma unroll
-          for (int e = 0; e < 16; e++) a[e] = 0.0f;
-#pragma unroll
-          for (int n = 2 * blk; n < 2 * blk + 2; n++) {
-            H8 x;
-            x.u = *(const u32x4*)(kt + swz(c, 2 * n + h) * 16);
-            a = __builtin_amdgcn_mfma_f32_32x32x16_f16(x.h, qh[n].h, a, 0, 0, 0);
-            a = __builtin_amdgcn_mfma_f32_32x32x16_f16(x.h, ql[n].h, a, 0, 0, 0);
-          }
-#pragma unroll
-          for (int w = 0; w < 4; w++) {
-            const f32x4 z = *(const f32x4*)(ksb + blk * KT + 32 * sub + 8 * w + 4 * h);
-#pragma unroll
-            for (int e = 0; e < 4; e++) s[sub][4 * w + e] = fmaf(a[4 * w + e], z[e], s[sub][4 * w + e]);
-          }
-        }
       }
     }
     if (key + KT > u.mask0) {
@@ -793,23 +1119,15 @@ __device__ __forceinline__ void many_unit(const PagedKernelArgs& p, const PagedU
       for (int e = 0; e < 16; e++) top = fmaxf(top, s[sub][e]);
     const float2 r = pair32(top);
     top = fmaxf(r.x, r.y) * qs;
-    float en = ev;
-    if constexpr (DT == KV_Q8) {
-      float big = 0.0f;
-#pragma unroll
-      for (int i = 0; i < KT * (D / 32) / 64; i++) big = fmaxf(big, vsb[lane + 64 * i]);
-      en = fmaxf(ev, scale_exponent(wave_max(big)));
-    }
-    if (__any(top > m + kLazy || en > ev)) {
+    if (__any(top > m + kLazy)) {
       const float mn = top > m + kLazy ? top : m;
-      const float f = m == -INFINITY ? 1.0f : exp2_hw(m - mn + (DT == KV_Q8 ? ev - en : 0.0f));
+      const float f = m == -INFINITY ? 1.0f : exp2_hw(m - mn);
       m = mn;
-      ev = en;
       l *= f;
 #pragma unroll
       for (int j = 0; j < D / 32; j++) o[j] *= f;
     }
-    const float base = m == -INFINITY ? 0.0f : kPShift - m - (DT == KV_Q8 ? ev : 0.0f);
+    const float base = m == -INFINITY ? 0.0f : kPShift - m;
 #pragma unroll
     for (int sub = 0; sub < NSUB; sub++)
 #pragma unroll
@@ -849,92 +1167,47 @@ __device__ __forceinline__ void many_unit(const PagedKernelArgs& p, const PagedU
             o[j + 1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(b.h, pl.h, o[j + 1], 0, 0, 0);
           }
         }
-      } else {
-#pragma unroll
-        for (int j = 0; j < D / 32; j++) {
-#pragma unroll
-          for (int x = 0; x < 2; x++) {
-            float w[8];
-#pragma unroll
-            for (int y = 0; y < 2; y++) {
-              const f32x4 z = *(const f32x4*)(vsb + j * KT + 32 * sub + 16 * x + 8 * y + 4 * h);
-#pragma unroll
-              for (int e = 0; e < 4; e++) w[4 * y + e] = s[sub][8 * x + 4 * y + e] * z[e];
-            }
-            H8 ph, pl, a;
-            split8(w, ph, pl);
-            a.u = *(const u32x4*)(vt + ((2 * x + h) * D + 32 * j + c) * 16);
-            o[j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a.h, ph.h, o[j], 0, 0, 0);
-            o[j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a.h, pl.h, o[j], 0, 0, 0);
-          }
-        }
       }
     }
   };
-  // V (or its q8 scales) past the written positions becomes zero
-  auto clear_stale = [&](char* vb, float* vsb, int key) __attribute__((always_inline)) {
-    for (int x = threadIdx.x; x < KT * (DT == KV_Q8 ? D / 32 : D); x += 256) {
-      if constexpr (DT == KV_Q8) {
-        if (key + x % KT >= u.key1) vsb[x] = 0.0f;
-      } else {
-        const int sub = x / (32 * D), y = x % (32 * D), panel = y / (8 * D), e = y % 8;
-        if (key + 32 * sub + tile_slot(panel, e) >= u.key1) {
-          if constexpr (DT == KV_F32) ((float*)vb)[x] = 0.0f;
-          else ((uint16_t*)vb)[x] = 0;
-        }
+  // V past the written positions becomes zero
+  auto clear_stale = [&](char* vb, int key) __attribute__((always_inline)) {
+    for (int x = threadIdx.x; x < KT * D; x += 256) {
+      const int sub = x / (32 * D), y = x % (32 * D), panel = y / (8 * D), e = y % 8;
+      if (key + 32 * sub + tile_slot(panel, e) >= u.key1) {
+        if constexpr (DT == KV_F32) ((float*)vb)[x] = 0.0f;
+        else ((uint16_t*)vb)[x] = 0;
       }
     }
     __syncthreads();
   };
-
-  // k0, k1: K of even and odd steps; v0, v1: V. scales: [step parity][K, V][block][KT]
-  ManyQ8<D> r8[DT == KV_Q8 ? NSUB : 1];
   auto begin = [&](int st, char* kd, char* vd) __attribute__((always_inline)) {
 #pragma unroll
-    for (int sub = 0; sub < NSUB; sub++) {
-      const size_t row = row_of(NSUB * st + sub);
-      if constexpr (DT == KV_Q8) many_load_q8<D>(p, row, r8[sub]);
-      else many_stage<D, DT>(p, row, kd + sub * M::SUB, vd + sub * M::SUB);
-    }
+    for (int sub = 0; sub < NSUB; sub++) many_stage<D, DT>(p, row_of(NSUB * st + sub), kd + sub * M::SUB, vd + sub * M::SUB);
   };
-  auto finish = [&](char* kd, char* vd, float* sc) __attribute__((always_inline)) {
-    if constexpr (DT == KV_Q8) {
-#pragma unroll
-      for (int sub = 0; sub < NSUB; sub++)
-        many_store_q8<D>(r8[sub], kd + sub * M::SUB, vd + sub * M::SUB, sc + 32 * sub, sc + KT * (D / 32) + 32 * sub, KT);
-    }
-  };
-  constexpr int SC = DT == KV_Q8 ? 2 * KT * (D / 32) : 0;
-  auto one = [&](int st, char* kb, char* vb, float* sb, char* kn, char* vn, float* sn) __attribute__((always_inline)) {
+  auto one = [&](int st, char* kb, char* vb, char* kn, char* vn) __attribute__((always_inline)) {
     // the step's tiles have landed; the other buffers' readers are done
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
-    const bool more = st + 1 < n_steps;
-    if (more) begin(st + 1, kn, vn);
+    if (st + 1 < n_steps) begin(st + 1, kn, vn);
     const int key = u.key0 + KT * st;
-    if (key + KT > u.key1) clear_stale(vb, sb + SC / 2, key);
-    if (active) step(kb, vb, sb, sb + SC / 2, key);
-    if (more) finish(kn, vn, sn);
+    if (key + KT > u.key1) clear_stale(vb, key);
+    if (active) step(kb, vb, key);
   };
-  if (n_steps > 0) {
-    begin(0, k0, v0);
-    finish(k0, v0, scales);
-  }
+  if (n_steps > 0) begin(0, k0, v0);
   for (int st = 0; st < n_steps; st += 2) {
-    one(st, k0, v0, scales, k1, v1, scales + SC);
-    if (st + 1 < n_steps) one(st + 1, k1, v1, scales + SC, k0, v0, scales);
+    one(st, k0, v0, k1, v1);
+    if (st + 1 < n_steps) one(st + 1, k1, v1, k0, v0);
   }
   const float2 r = pair32(l);
   l = r.x + r.y;
-  const float oscale = DT == KV_Q8 ? 1.0f / 127.0f : 1.0f;
-  if constexpr (DT == KV_Q8) m += ev;
   if (ra.on) {
 #pragma unroll
     for (int j = 0; j < D / 32; j++)
 #pragma unroll
       for (int w = 0; w < 4; w++)
         store_o<D>(p, ws_o, ra, 32 * j + 8 * w + 4 * h,
-                   f32x4{o[j][4 * w], o[j][4 * w + 1], o[j][4 * w + 2], o[j][4 * w + 3]} * oscale, l);
+                   f32x4{o[j][4 * w], o[j][4 * w + 1], o[j][4 * w + 2], o[j][4 * w + 3]}, l);
     if (h == 0 && ra.part >= 0) ws_ml[(size_t)ra.part * p.b.H + ra.head] = make_float2(m, l);
   }
 }
@@ -949,28 +1222,48 @@ __global__ __launch_bounds__(256, D == 128 ? 2 : 1) void paged_many_kernel(Paged
   __shared__ __align__(16) char k1[M::SUB * M::NSUB];
   __shared__ __align__(16) char v0[M::SUB * M::NSUB];
   __shared__ __align__(16) char v1[M::SUB * M::NSUB];
-  __shared__ __align__(16) float scales[DT == KV_Q8 ? 4 * M::KT * (D / 32) : 4];
   const int total = p.n_blocks ? p.n_blocks : p.b.hdr->n_many * p.kv_heads;
   float* ws_o = p.b.hdr->ws_o;
   float2* ws_ml = p.b.hdr->ws_ml;
   for (int b = blockIdx.x; b < total; b += gridDim.x) {
     const PagedUnit u = p.b.units[b / p.kv_heads];
-    many_unit<D, DT>(p, u, b % p.kv_heads, ws_o, ws_ml, k0, k1, v0, v1, scales);
+    many_unit<D, DT>(p, u, b % p.kv_heads, ws_o, ws_ml, k0, k1, v0, v1);
     __syncthreads();  // the unit's LDS is read before the next one's is written
   }
 }
 
+// workgroups of 32-row units a CU holds
 template <int D, int DT>
-__global__ __launch_bounds__(256, (few_waves<D, DT>())) void paged_few_kernel(PagedKernelArgs p) {
-  __shared__ FewLds<D, DT> lds;
+constexpr int mid_waves() { return D == 256 && DT != KV_Q8 ? 1 : 2; }
+
+template <int D, int DT>
+__global__ __launch_bounds__(256, (mid_waves<D, DT>())) void paged_mid_kernel(PagedKernelArgs p) {
+  __shared__ MidLds<D, DT> lds;
+  __shared__ float2 ml[4][32];
   const PagedHeader* h = p.b.hdr;
   const int first = p.n_blocks ? p.first : h->n_many;
-  const int total = p.n_blocks ? p.n_blocks : (h->n_units - h->n_many) * p.kv_heads;
+  const int total = p.n_blocks ? p.n_blocks : h->n_mid * p.kv_heads;
   float* ws_o = h->ws_o;
   float2* ws_ml = h->ws_ml;
   for (int b = blockIdx.x; b < total; b += gridDim.x) {
     const PagedUnit u = p.b.units[first + b / p.kv_heads];
-    few_unit<D, DT>(p, u, b % p.kv_heads, ws_o, ws_ml, lds);
+    mid_unit<D, DT>(p, u, b % p.kv_heads, ws_o, ws_ml, lds, ml);
+    __syncthreads();  // the unit's LDS is read before the next one's is written
+  }
+}
+
+// AUX: cache policy of the page loads (2: nontemporal)
+template <int D, int DT, int AUX>
+__global__ __launch_bounds__(256, (few_waves<D, DT>())) void paged_few_kernel(PagedKernelArgs p) {
+  __shared__ FewLds<D, DT> lds;
+  const PagedHeader* h = p.b.hdr;
+  const int first = p.n_blocks ? p.first : h->n_many + h->n_mid;
+  const int total = p.n_blocks ? p.n_blocks : (h->n_units - first) * p.kv_heads;
+  float* ws_o = h->ws_o;
+  float2* ws_ml = h->ws_ml;
+  for (int b = blockIdx.x; b < total; b += gridDim.x) {
+    const PagedUnit u = p.b.units[first + b / p.kv_heads];
+    few_unit<D, DT, AUX>(p, u, b % p.kv_heads, ws_o, ws_ml, lds);
     __syncthreads();  // the unit's LDS is read before the next one's is written
   }
 }
@@ -1070,16 +1363,33 @@ static hipError_t launch_attn(const PagedKernelArgs& k, const PagedAttnArgs& a, 
   // Under capture a grid that fills the GPU walks the units of whatever batch is set at replay, of both
   // kinds.
   PagedKernelArgs x = k;
-  if (b.captured || b.n_many) {
-    x.n_blocks = b.n_many * k.kv_heads;
-    const unsigned grid = (unsigned)(b.captured ? a.num_cus * (D == 128 ? 2 : 1) : x.n_blocks);
-    hipLaunchKernelGGL((paged_many_kernel<D, DT>), dim3(grid), dim3(256), 0, st, x);
+  if constexpr (paged_has_many(D, DT)) {
+    if (b.captured || b.n_many) {
+      x.n_blocks = b.n_many * k.kv_heads;
+      const unsigned grid = (unsigned)(b.captured ? a.num_cus * (D == 128 ? 2 : 1) : x.n_blocks);
+      hipLaunchKernelGGL((paged_many_kernel<D, DT>), dim3(grid), dim3(256), 0, st, x);
+    }
   }
-  if (b.captured || b.n_units > b.n_many) {
+  if (b.captured || b.n_mid) {
     x.first = b.n_many;
-    x.n_blocks = (b.n_units - b.n_many) * k.kv_heads;
+    x.n_blocks = b.n_mid * k.kv_heads;
+    const unsigned grid = (unsigned)(b.captured ? a.num_cus * mid_waves<D, DT>() : x.n_blocks);
+    hipLaunchKernelGGL((paged_mid_kernel<D, DT>), dim3(grid), dim3(256), 0, st, x);
+  }
+  if (b.captured || b.n_units > b.n_many + b.n_mid) {
+    x.first = b.n_many + b.n_mid;
+    x.n_blocks = (b.n_units - x.first) * k.kv_heads;
     const unsigned grid = (unsigned)(b.captured ? a.num_cus * few_waves<D, DT>() : x.n_blocks);
-    hipLaunchKernelGGL((paged_few_kernel<D, DT>), dim3(grid), dim3(256), 0, st, x);
+    // Pages that one unit reads once, more of them than caches keep from call to call: nontemporal, which
+    // leaves the shared pages there (64 sequences of 2,000, 524 MB: 94 -> 83 us; a shared 16k document
+    // beside tails of 71 MB 61 -> 57). Two row tiles that share a page want it kept (115 -> 149), and q8's
+    // 8-byte and head_dim 256's strided pieces of a line come one after the other (138 -> 157, 137 -> 151).
+    bool stream = false;
+    if constexpr (D == 128 && DT == KV_F16) {
+      stream = b.stream_few;
+      if (stream) hipLaunchKernelGGL((paged_few_kernel<D, DT, 2>), dim3(grid), dim3(256), 0, st, x);
+    }
+    if (!stream) hipLaunchKernelGGL((paged_few_kernel<D, DT, 0>), dim3(grid), dim3(256), 0, st, x);
   }
   if (b.captured || b.n_merges) {
     const long few = (long)b.n_merge_few * b.H, all = (long)b.n_merges * b.H;
