@@ -33,6 +33,8 @@ struct PagedUnit {
   int key0, key1;
   int mask0;   // positions below this are seen by every row of the unit
   int chunk;   // which chunk of its segment: the partial slot is the token's `part` + chunk
+  int page[4]; // the pages of the first four tiles, with which a wave each begins (one load in the chain
+               // less before its first keys are on their way)
   int pad[3];
 };
 struct PagedTok {
@@ -244,6 +246,18 @@ class PagedPlanner {
       push_tokens(b);
       segs_.push_back(s);
     }
+    // Few-row segments join the 32-row units of others rather than take a launch of their own (16
+    // sequences of 300 positions behind 4,096 f16 25 -> 19 us, 24 of 600 behind 8,192 40 -> 30), but where
+    // they are most of the work: the 16-row kernel moves their pages faster at head_dim 128 (32 of 4,000
+    // behind 2,048 f16 105, joined 110, f32 209 / 238, q8 79 / 92).
+    few_as_mid_ = false;
+    bool mid = false;
+    double few = 0;
+    for (const Segment& s : segs_) {
+      if (kind(s) == 1) mid = true;
+      if (kind(s) == 2) few += (double)(s.key1 - s.key0) * sh_.kv_heads;
+    }
+    few_as_mid_ = mid && (sh_.D == 256 || few < 5e5);
     chunk();
     emit(out);
   }
@@ -310,22 +324,23 @@ class PagedPlanner {
   }
 
   // A segment's kind of units. 128-row units stage their positions once for four waves and reach the
-  // matrix cores' rate; 32-row ones need a quarter of the workgroups' partials for the same parallelism.
-  // Where both exist the work decides, rows x positions x kv heads (us, 128-row / 32-row units with their
-  // merges: f16 at 128, 8 kv heads, 128 rows over 2,048 / 8,192 / 32,768 20 / 28 / 56 and 17 / 28 / 60, 512
-  // rows 32 / 56 / 139 and 30 / 61 / 192; f16 at 256, 4 kv heads, 29 / 37 / 66 and 24 / 33 / 74; f32 at 256
-  // 54 / 68 / 207 and 37 / 85 / 274).
+  // matrix cores' rate; 32-row ones need a quarter of the workgroups' partials for the same parallelism,
+  // and take a batch's few-row segments into the same launch. Where both exist the work decides, rows x
+  // positions x kv heads (us in all, 128-row / 32-row units. f16 at 128, 8 kv heads, 32 sequences of 4
+  // heads behind 16,384 positions 54 / 45, behind 32,768 72 / 79, a prompt of 777 34 / 47, of 100 19 / 15;
+  // f16 at 256, 4 kv heads, 64 behind 4,096 65 / 59, behind 16,384 116 / 135; f32 at 256, 32 of 4 heads
+  // behind 2,048 54 / 37, 64 of 6 behind 4,096 138 / 227).
   int kind(const Segment& s) const {
-    if (s.rows <= 16) return 2;
+    if (s.rows <= 16) return few_as_mid_ ? 1 : 2;
     if (!paged_has_many(sh_.D, sh_.dtype)) return 1;
     const double work = (double)s.rows * (s.shared ? s.key1 - s.key0 : s.key1 - s.key0 - s.n_tok / 2) * sh_.kv_heads;
-    return work > (sh_.dtype == 0 ? 2e6 : sh_.D == 128 ? 8e6 : 12e6) ? 0 : 1;
+    return work > (sh_.dtype == 0 ? 2e6 : !s.shared ? 3e6 : sh_.D == 128 ? 20e6 : 12e6) ? 0 : 1;
   }
   // the unit that takes a segment's rows from r0 on: its kind and rows. What whole tiles leave over goes to
   // the smallest kind that takes it at once.
   int unit_kind(const Segment& s, int r0) const {
     const int left = s.rows - r0, k = kind(s);
-    return left <= 16 ? 2 : k == 0 && left <= 32 ? 1 : k;
+    return left <= 16 && !few_as_mid_ ? 2 : k == 0 && left <= 32 ? 1 : k;
   }
   static int unit_rows(int kind) { return kind == 0 ? 128 : kind == 1 ? 32 : 16; }
   // row tiles in all, and those of the segment's own kind
@@ -457,6 +472,10 @@ class PagedPlanner {
           u.key1 = std::min(s.key0 + (c + 1) * s.chunk_len * 32, s.shared ? s.key1 : hi + 1);
           if (u.key1 < u.key0) u.key1 = u.key0;
           u.mask0 = s.shared ? s.key1 : lo + 1;
+          for (int w = 0; w < 4; w++) {
+            const int key = std::max(u.key0, std::min(u.key0 + 32 * w, (u.key1 - 1) & ~31));
+            u.page[w] = out.pages[s.table + std::min(key, s.key1 - 1) / sh_.page];
+          }
           out.units.push_back(u);
           cost_.push_back((u.key1 - u.key0 + 31) / 32);
         }
@@ -486,6 +505,7 @@ class PagedPlanner {
     out.units.swap(sorted_);
   }
 
+  bool few_as_mid_ = false;
   PagedShape sh_{};
   PagedPlan* out_ = nullptr;
   int n_seqs_ = 0;

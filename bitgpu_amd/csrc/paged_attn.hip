@@ -136,6 +136,13 @@ __device__ inline RowAt row_at(const PagedKernelArgs& p, const PagedUnit& u, int
   return r;
 }
 
+// row (of D values) at which tile t of a unit begins, t one of the first four
+__device__ inline size_t first_row(const PagedKernelArgs& p, const PagedUnit& u, int kvh, int t) {
+  const int key = u.key0 + 32 * t, P = 1 << p.b.page_shift;
+  const int id = t == 0 ? u.page[0] : t == 1 ? u.page[1] : t == 2 ? u.page[2] : u.page[3];
+  return ((size_t)id * p.kv_heads + kvh) * P + (key & (P - 1));
+}
+
 // a row's o at dims d .. d+3: the output (normalized, gated) or the unit's partial
 template <int D>
 __device__ inline void store_o(const PagedKernelArgs& p, float* ws_o, const RowAt& r, int d, f32x4 o, float l) {
@@ -290,7 +297,7 @@ __device__ __forceinline__ void few_unit(const PagedKernelArgs& p, const PagedUn
   // the first tiles are on their way before the queries are looked at
   FewTile<D, DT> tl;
   if (n_tiles > 0) {
-    const size_t row = row_of(wave);
+    const size_t row = first_row(p, u, kvh, wave);
     few_load_k<D, DT, AUX>(p, row, wave < n_tiles, c, g, tl);
     few_load_v<D, DT, AUX>(p, row, wave < n_tiles, c, g, tl);
   }
@@ -583,24 +590,29 @@ __device__ __forceinline__ void few_unit(const PagedKernelArgs& p, const PagedUn
 // A wave's 32-position tile as operands of the 32-row products (descriptors as for the few-row units): K
 // row c, dims 16 n + 8 h + e (f32 8 n + 4 h + e, q8 32 n + 16 h + e); V dim 32 j + c, panel 2 x + h.
 template <int D, int DT>
-struct MidTile {
-  static constexpr int NK = DT == KV_F32 ? D / 8 : DT == KV_F16 ? D / 16 : D / 32;
-  static constexpr int NV = 2 * (D / 32);
-  u32x4 k[NK], v[DT == KV_F32 ? 2 * NV : DT == KV_F16 ? NV : 1];
-  u32x2 vc[DT == KV_Q8 ? NV : 1];
-  float ks[DT == KV_Q8 ? D / 64 : 1], vs[DT == KV_Q8 ? D / 64 : 1];
+struct MidK {
+  static constexpr int N = DT == KV_F32 ? D / 8 : DT == KV_F16 ? D / 16 : D / 32;
+  u32x4 k[N];
+  float ks[DT == KV_Q8 ? D / 64 : 1];
+};
+template <int D, int DT>
+struct MidV {
+  static constexpr int N = 2 * (D / 32);
+  u32x4 v[DT == KV_F32 ? 2 * N : DT == KV_F16 ? N : 1];
+  u32x2 vc[DT == KV_Q8 ? N : 1];
+  float vs[DT == KV_Q8 ? D / 64 : 1];
 };
 
 template <int D, int DT>
-__device__ __forceinline__ void mid_load_k(const PagedKernelArgs& p, size_t row, bool on, int c, int h, MidTile<D, DT>& t) {
+__device__ __forceinline__ void mid_load_k(const PagedKernelArgs& p, size_t row, bool on, int c, int h, MidK<D, DT>& t) {
   constexpr int EB = DT == KV_F32 ? 4 : DT == KV_F16 ? 2 : 1;
   const __amdgpu_buffer_rsrc_t r = tile_rsrc(p.k + row * D * EB, on ? 32 * D * EB : 0);
 #pragma unroll
-  for (int n = 0; n < MidTile<D, DT>::NK; n++) t.k[n] = ld16(r, c * D * EB + 16 * h, 32 * n);
+  for (int n = 0; n < MidK<D, DT>::N; n++) t.k[n] = ld16(r, c * D * EB + 16 * h, 32 * n);
   if constexpr (DT == KV_Q8) few_load_scales<D, DT>(p.ks, row, on, c + 32 * h, t.ks);
 }
 template <int D, int DT>
-__device__ __forceinline__ void mid_load_v(const PagedKernelArgs& p, size_t row, bool on, int c, int h, MidTile<D, DT>& t) {
+__device__ __forceinline__ void mid_load_v(const PagedKernelArgs& p, size_t row, bool on, int c, int h, MidV<D, DT>& t) {
   constexpr int EB = DT == KV_F32 ? 4 : DT == KV_F16 ? 2 : 1;
   const __amdgpu_buffer_rsrc_t r = tile_rsrc(p.v + row * D * EB, on ? 32 * D * EB : 0);
   const int off = (h * D + c) * 8 * EB;
@@ -634,7 +646,6 @@ union MidLds {
 template <int D, int DT>
 __device__ __forceinline__ void mid_unit(const PagedKernelArgs& p, const PagedUnit& u, int kvh, float* ws_o, float2* ws_ml,
                                          MidLds<D, DT>& lds, float2 (*lml)[32]) {
-  using T = MidTile<D, DT>;
   constexpr int ND = D / 32;
   const int wave = uniform(threadIdx.x >> 6), lane = threadIdx.x & 63, c = lane & 31, h = lane >> 5;
   const int shift = p.b.page_shift, P = 1 << shift;
@@ -645,11 +656,12 @@ __device__ __forceinline__ void mid_unit(const PagedKernelArgs& p, const PagedUn
     const int id = uniform(pages[key >> shift]);
     return ((size_t)id * p.kv_heads + kvh) * P + (key & (P - 1));
   };
-  T tl;
+  MidK<D, DT> tk;
+  MidV<D, DT> tv;
   if (n_tiles > 0) {
-    const size_t row = row_of(wave);
-    mid_load_k<D, DT>(p, row, wave < n_tiles, c, h, tl);
-    mid_load_v<D, DT>(p, row, wave < n_tiles, c, h, tl);
+    const size_t row = first_row(p, u, kvh, wave);
+    mid_load_k<D, DT>(p, row, wave < n_tiles, c, h, tk);
+    mid_load_v<D, DT>(p, row, wave < n_tiles, c, h, tv);
   }
   // ---- the queries: every wave looks at all of them (each row's factor), prepares its share
   const RowAt ra = row_at(p, u, kvh, c);
@@ -665,12 +677,16 @@ __device__ __forceinline__ void mid_unit(const PagedKernelArgs& p, const PagedUn
         if ((n & 3) == wave) lds.in.q[n][lane] = *(const u32x4*)(q + 8 * n + 4 * h);
       qs = p.qscale;
     } else {
+      // product n: f16 dims 16 n + 8 h + e; q8 block n / 2, dims 16 h + 8 (n & 1) + e
+      f32x4 x[D / 16][2];
       float top = 0.0f;
-#pragma unroll 4
-      for (int n = 0; n < D / 8; n++) {
-        const f32x4 a = *(const f32x4*)(q + 8 * n + 4 * h);
 #pragma unroll
-        for (int e = 0; e < 4; e++) top = fmaxf(top, fabsf(a[e]));
+      for (int n = 0; n < D / 16; n++) {
+        const float* at = q + (DT == KV_F16 ? 16 * n + 8 * h : 32 * (n >> 1) + 16 * h + 8 * (n & 1));
+        x[n][0] = *(const f32x4*)at;
+        x[n][1] = *(const f32x4*)(at + 4);
+#pragma unroll
+        for (int e = 0; e < 4; e++) top = fmaxf(top, fmaxf(fabsf(x[n][0][e]), fabsf(x[n][1][e])));
       }
       const float2 r = pair32(top);
       top = fmaxf(r.x, r.y);
@@ -678,16 +694,11 @@ __device__ __forceinline__ void mid_unit(const PagedKernelArgs& p, const PagedUn
       const float f = row_factor(top, &undo);
       qs = p.qscale * undo * (DT == KV_Q8 ? 1.0f / 127.0f : 1.0f);
 #pragma unroll
-      for (int n = 0; n < D / 16; n++) {  // product n: f16 dims 16 n + 8 h; q8 block n / 2, dims 16 h + 8 (n & 1)
+      for (int n = 0; n < D / 16; n++) {
         if ((n & 3) == wave) {
-          const float* at = q + (DT == KV_F16 ? 16 * n + 8 * h : 32 * (n >> 1) + 16 * h + 8 * (n & 1));
-          const f32x4 a = *(const f32x4*)at, b = *(const f32x4*)(at + 4);
           float y[8];
 #pragma unroll
-          for (int e = 0; e < 4; e++) {
-            y[e] = a[e] * f;
-            y[4 + e] = b[e] * f;
-          }
+          for (int e = 0; e < 8; e++) y[e] = x[n][e >> 2][e & 3] * f;
           H8 hi, lo;
           split8(y, hi, lo);
           lds.in.q[2 * n][lane] = hi.u;
@@ -722,8 +733,8 @@ __device__ __forceinline__ void mid_unit(const PagedKernelArgs& p, const PagedUn
 #pragma unroll
       for (int i = 0; i < D / 64; i++) {
         const int x = lane * (D / 64) + i, at = x % (D / 32) * 32 + x / (D / 32);
-        lk[at] = tl.ks[i];
-        lv[at] = tl.vs[i];
+        lk[at] = tk.ks[i];
+        lv[at] = tv.vs[i];
       }
       __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
       __builtin_amdgcn_wave_barrier();
@@ -739,7 +750,7 @@ __device__ __forceinline__ void mid_unit(const PagedKernelArgs& p, const PagedUn
       for (int n = 0; n < D / 8; n++) {
         const f32x4 qn = *(const f32x4*)&lds.in.q[n][lane];
 #pragma unroll
-        for (int e = 0; e < 4; e++) a = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(tl.k[n][e]), qn[e], a, 0, 0, 0);
+        for (int e = 0; e < 4; e++) a = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(tk.k[n][e]), qn[e], a, 0, 0, 0);
       }
 #pragma unroll
       for (int e = 0; e < 16; e++) s[e] = a[e];
@@ -750,7 +761,7 @@ __device__ __forceinline__ void mid_unit(const PagedKernelArgs& p, const PagedUn
 #pragma unroll
       for (int n = 0; n < D / 16; n++) {
         H8 x;
-        x.u = tl.k[n];
+        x.u = tk.k[n];
         a = __builtin_amdgcn_mfma_f32_32x32x16_f16(x.h, q_at(n, 0), a, 0, 0, 0);
         a = __builtin_amdgcn_mfma_f32_32x32x16_f16(x.h, q_at(n, 1), a, 0, 0, 0);
       }
@@ -761,7 +772,7 @@ __device__ __forceinline__ void mid_unit(const PagedKernelArgs& p, const PagedUn
       for (int e = 0; e < 16; e++) s[e] = 0.0f;
 #pragma unroll
       for (int b = 0; b < ND; b++) {
-        const half8 x0 = codes8(u32x2{tl.k[b][0], tl.k[b][1]}), x1 = codes8(u32x2{tl.k[b][2], tl.k[b][3]});
+        const half8 x0 = codes8(u32x2{tk.k[b][0], tk.k[b][1]}), x1 = codes8(u32x2{tk.k[b][2], tk.k[b][3]});
         f32x16 a;
 #pragma unroll
         for (int e = 0; e < 16; e++) a[e] = 0.0f;
@@ -778,7 +789,7 @@ __device__ __forceinline__ void mid_unit(const PagedKernelArgs& p, const PagedUn
       }
     }
     __builtin_amdgcn_sched_barrier(0);  // into the registers just used: not before, which would take a second set
-    mid_load_k<D, DT>(p, next, more, c, h, tl);
+    mid_load_k<D, DT>(p, next, more, c, h, tk);
     __builtin_amdgcn_sched_barrier(0);
     if (key + 32 > u.mask0) {
 #pragma unroll
@@ -793,7 +804,7 @@ __device__ __forceinline__ void mid_unit(const PagedKernelArgs& p, const PagedUn
 #pragma unroll
             for (int e = 0; e < 8; e++) {
               const int i = 2 * (x * ND + j) + (e >> 2);
-              tl.v[i][e & 3] = key + 16 * x + 8 * (e >> 2) + 4 * h + (e & 3) < u.key1 ? tl.v[i][e & 3] : 0u;
+              tv.v[i][e & 3] = key + 16 * x + 8 * (e >> 2) + 4 * h + (e & 3) < u.key1 ? tv.v[i][e & 3] : 0u;
             }
       } else if constexpr (DT == KV_F16) {
 #pragma unroll
@@ -805,14 +816,14 @@ __device__ __forceinline__ void mid_unit(const PagedKernelArgs& p, const PagedUn
             keep[w] = (at < u.key1 ? 0xffffu : 0u) | (at + 1 < u.key1 ? 0xffff0000u : 0u);
           }
 #pragma unroll
-          for (int j = 0; j < ND; j++) tl.v[x * ND + j] &= keep;
+          for (int j = 0; j < ND; j++) tv.v[x * ND + j] &= keep;
         }
       } else {
 #pragma unroll
         for (int i = 0; i < D / 64; i++) {
           const int x = lane * (D / 64) + i;
           if (key + x / (D / 32) >= u.key1) {
-            tl.vs[i] = 0.0f;
+            tv.vs[i] = 0.0f;
             lv[x % (D / 32) * 32 + x / (D / 32)] = 0.0f;
           }
         }
@@ -829,9 +840,9 @@ __device__ __forceinline__ void mid_unit(const PagedKernelArgs& p, const PagedUn
     top = fmaxf(r.x, r.y) * qs;
     float en = ev;
     if constexpr (DT == KV_Q8) {
-      float big = tl.vs[0];
+      float big = tv.vs[0];
 #pragma unroll
-      for (int i = 1; i < D / 64; i++) big = fmaxf(big, tl.vs[i]);
+      for (int i = 1; i < D / 64; i++) big = fmaxf(big, tv.vs[i]);
       en = fmaxf(ev, scale_exponent(wave_max(big)));
     }
     if (__any(top > m + kLazy || en > ev)) {
@@ -857,7 +868,7 @@ __device__ __forceinline__ void mid_unit(const PagedKernelArgs& p, const PagedUn
         for (int e = 0; e < 8; e++)
 #pragma unroll
           for (int j = 0; j < ND; j++)
-            o[j] = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(tl.v[2 * (x * ND + j) + (e >> 2)][e & 3]), s[8 * x + e],
+            o[j] = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(tv.v[2 * (x * ND + j) + (e >> 2)][e & 3]), s[8 * x + e],
                                                         o[j], 0, 0, 0);
       } else if constexpr (DT == KV_F16) {
         float w[8];
@@ -868,13 +879,13 @@ __device__ __forceinline__ void mid_unit(const PagedKernelArgs& p, const PagedUn
 #pragma unroll
         for (int j = 0; j < ND; j++) {
           H8 a;
-          a.u = tl.v[x * ND + j];
+          a.u = tv.v[x * ND + j];
           o[j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a.h, ph.h, o[j], 0, 0, 0);
         }
 #pragma unroll
         for (int j = 0; j < ND; j++) {
           H8 a;
-          a.u = tl.v[x * ND + j];
+          a.u = tv.v[x * ND + j];
           o[j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a.h, pl.h, o[j], 0, 0, 0);
         }
       } else {
@@ -889,14 +900,14 @@ __device__ __forceinline__ void mid_unit(const PagedKernelArgs& p, const PagedUn
           }
           H8 ph, pl;
           split8(w, ph, pl);
-          const half8 a = codes8(tl.vc[x * ND + j]);
+          const half8 a = codes8(tv.vc[x * ND + j]);
           o[j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, ph.h, o[j], 0, 0, 0);
           o[j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, pl.h, o[j], 0, 0, 0);
         }
       }
     }
     __builtin_amdgcn_sched_barrier(0);
-    mid_load_v<D, DT>(p, next, more, c, h, tl);
+    mid_load_v<D, DT>(p, next, more, c, h, tv);
     __builtin_amdgcn_sched_barrier(0);
   }
 

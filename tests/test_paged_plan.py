@@ -24,8 +24,8 @@ def plan(tmp_path_factory):
         if out.startswith("error "):
             return out[6:].strip()
         got = {ln.split()[0]: [int(x) for x in ln.split()[1:]] for ln in out.splitlines()}
-        names = ("kind", "tok", "rho0", "n_rho", "table", "key0", "key1", "mask0", "chunk")
-        got["units"] = [dict(zip(names, got["units"][i:i + 12])) for i in range(0, len(got["units"]), 12)]
+        names = ("kind", "tok", "rho0", "n_rho", "table", "key0", "key1", "mask0", "chunk", "p0", "p1", "p2", "p3")
+        got["units"] = [dict(zip(names, got["units"][i:i + 16])) for i in range(0, len(got["units"]), 16)]
         got["toks"] = [tuple(got["toks"][i:i + 3]) for i in range(0, len(got["toks"]), 4)]
         got["merges"] = [tuple(got["merges"][i:i + 3]) for i in range(0, len(got["merges"]), 4)]
         return got
@@ -65,6 +65,9 @@ def check(p, rows, lens, tables, G, page, dtype):
                 for i in range(lo // page, (hi - 1) // page + 1):
                     assert p["pages"][u["table"] + i] == own[i]
                 seen[t][rho % G].append((lo, hi))
+            for w in range(4):                                # the pages of a unit's first tiles
+                if u["key0"] + 32 * w < u["key1"]:
+                    assert u[f"p{w}"] == p["pages"][u["table"] + (u["key0"] + 32 * w) // page]
             # what the kernels read past the row's positions is still inside a listed page
             assert u["key1"] == 0 or u["table"] + (u["key1"] - 1) // page < len(p["pages"])
             if t in merged:
