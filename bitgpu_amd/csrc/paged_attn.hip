@@ -119,18 +119,25 @@ __device__ inline half8 codes8(u32x2 w) {
   return o.h + bias;
 }
 
+// A value the compiler takes as new here: what is computed from it for a unit's end is not computed before
+// the walk over units and held (or spilled) through all of it.
+__device__ __forceinline__ int afresh(int x) {
+  asm volatile("" : "+v"(x));
+  return x;
+}
+
 // what a unit's body needs to know of one of its rows
 struct RowAt {
-  int t, head, part;
-  bool on;
+  int t, head, part, pos;
 };
+// (rows past the unit's: its first one)
 __device__ inline RowAt row_at(const PagedKernelArgs& p, const PagedUnit& u, int kvh, int i) {
   RowAt r;
-  r.on = i < u.n_rho;
-  const int rho = u.rho0 + (r.on ? i : 0);
+  const int rho = u.rho0 + (i < u.n_rho ? i : 0);
   const int j = rho / p.b.G;
   const PagedTok tok = p.b.toks[u.tok + j];
   r.t = tok.t;
+  r.pos = tok.pos;
   r.part = tok.part < 0 ? -1 : tok.part + u.chunk;
   r.head = kvh * p.b.G + rho - j * p.b.G;
   return r;
@@ -160,6 +167,31 @@ __device__ inline void store_o(const PagedKernelArgs& p, float* ws_o, const RowA
   }
   *(f32x4*)(p.out + row * D + d) = o;
 }
+
+// 32 rows of o between waves and threads, in LDS: 16-byte chunk ch of row c lies in line ch / 2, where the
+// lanes of a matrix result (row c, dims 8 w + 4 h + e of every 32) write it without bank conflicts, and 16
+// chunks of one row are read without.
+__device__ inline int chunk_at(int c, int line, int h) { return line * 64 + ((c + 2 * (line & 7) + h) & 31) + 32 * h; }
+template <int J>
+__device__ __forceinline__ void put_o(f32x4* x, const f32x16* o, int c, int h) {
+#pragma unroll
+  for (int j = 0; j < J; j++)
+#pragma unroll
+    for (int w = 0; w < 4; w++)
+      x[chunk_at(c, 4 * j + w, h)] = f32x4{o[j][4 * w], o[j][4 * w + 1], o[j][4 * w + 2], o[j][4 * w + 3]};
+}
+template <int J>
+__device__ __forceinline__ void add_o(const f32x4* x, f32x16* o, int c, int h) {
+#pragma unroll
+  for (int j = 0; j < J; j++)
+#pragma unroll
+    for (int w = 0; w < 4; w++) {
+      const f32x4 y = x[chunk_at(c, 4 * j + w, h)];
+#pragma unroll
+      for (int e = 0; e < 4; e++) o[j][4 * w + e] += y[e];
+    }
+}
+__device__ inline f32x4 get_o(const f32x4* x, int c, int ch) { return x[chunk_at(c, ch >> 1, ch & 1)]; }
 
 // slot of register i (0..7) of lane group g in a 32-slot tile, 16-row matrix products: the V tile's own
 // order (tile_slot)
@@ -264,16 +296,20 @@ __device__ inline int swz(int r, int x) { return x ^ (r & 15); }
 
 // LDS of a few-row unit
 template <int D, int DT>
-union FewLds {
+struct FewLds {
   static constexpr int NQ = DT == KV_F32 ? D / 16 : 2 * (D / 32);
-  struct {
-    u32x4 q[NQ][64];                           // the queries as matrix operands, the same for every wave
-    float s[DT == KV_Q8 ? 4 : 1][2][DT == KV_Q8 ? D : 1];  // q8: K and V scales of the tile a wave is at
-  } in;
-  struct {
-    float o[4][16 * D];                        // the waves' results
-    float2 ml[4][16];
-  } out;
+  union {
+    struct {
+      u32x4 q[NQ][64];                         // the queries as matrix operands, the same for every wave
+      float s[DT == KV_Q8 ? 4 : 1][2][DT == KV_Q8 ? D : 1];  // q8: K and V scales of the tile a wave is at
+    } in;
+    struct {
+      float o[4][16 * D];                      // the waves' results
+      float2 ml[4][16];
+    } out;
+  };
+  float top[4][16];                            // largest |q| of a wave's dims
+  RowAt row[16];
 };
 
 // workgroups of few-row units a CU holds (waves a SIMD)
@@ -302,48 +338,46 @@ __device__ __forceinline__ void few_unit(const PagedKernelArgs& p, const PagedUn
     few_load_v<D, DT, AUX>(p, row, wave < n_tiles, c, g, tl);
   }
 
-  // ---- the queries: every wave looks at all of them (each row's factor), prepares its share
+  // ---- the queries: a wave prepares every fourth operand; a row's factor needs all of them
   int pos;
-  float qs;
+  float qs = p.qscale;
   {
-    const int rho = u.rho0 + (c < u.n_rho ? c : 0);
-    const int j = rho / p.b.G;
-    const PagedTok tok = p.b.toks[u.tok + j];
-    pos = tok.pos;
-    const float* q = p.q + ((size_t)tok.t * p.b.H + kvh * p.b.G + rho - j * p.b.G) * D;
+    const int tid = afresh(threadIdx.x), c = tid & 15, g = (tid >> 4) & 3, lane = tid & 63;
+    const RowAt ra = row_at(p, u, kvh, c);
+    pos = ra.pos;
+    if (wave == 0 && g == 0) lds.row[c] = ra;
+    const float* q = p.q + ((size_t)ra.t * p.b.H + ra.head) * D;
     if constexpr (DT == KV_F32) {
 #pragma unroll
-      for (int n = 0; n < NK; n++)
-        if ((n & 3) == wave) lds.in.q[n][lane] = *(const u32x4*)(q + 16 * n + 4 * g);
-      qs = p.qscale;
+      for (int i = 0; i < NK / 4; i++) lds.in.q[4 * i + wave][lane] = *(const u32x4*)(q + 16 * (4 * i + wave) + 4 * g);
     } else {
-      f32x4 x[NK][2];
+      f32x4 x[NK / 4][2];
       float top = 0.0f;
 #pragma unroll
-      for (int n = 0; n < NK; n++) {
-        x[n][0] = *(const f32x4*)(q + 32 * n + 8 * g);
-        x[n][1] = *(const f32x4*)(q + 32 * n + 8 * g + 4);
+      for (int i = 0; i < NK / 4; i++) {
+        const float* at = q + 32 * (4 * i + wave) + 8 * g;
+        x[i][0] = *(const f32x4*)at;
+        x[i][1] = *(const f32x4*)(at + 4);
 #pragma unroll
-        for (int e = 0; e < 4; e++) top = fmaxf(top, fmaxf(fabsf(x[n][0][e]), fabsf(x[n][1][e])));
+        for (int e = 0; e < 4; e++) top = fmaxf(top, fmaxf(fabsf(x[i][0][e]), fabsf(x[i][1][e])));
       }
       float2 r = pair16(top);
       top = fmaxf(r.x, r.y);
       r = pair32(top);
-      top = fmaxf(r.x, r.y);
+      lds.top[wave][c] = fmaxf(r.x, r.y);
+      __syncthreads();
       float undo;
-      const float f = row_factor(top, &undo);
-      qs = p.qscale * undo * (DT == KV_Q8 ? 1.0f / 127.0f : 1.0f);
+      const float f = row_factor(fmaxf(fmaxf(lds.top[0][c], lds.top[1][c]), fmaxf(lds.top[2][c], lds.top[3][c])), &undo);
+      qs *= undo * (DT == KV_Q8 ? 1.0f / 127.0f : 1.0f);
 #pragma unroll
-      for (int n = 0; n < NK; n++) {
-        if ((n & 3) == wave) {
-          float y[8];
+      for (int i = 0; i < NK / 4; i++) {
+        float y[8];
 #pragma unroll
-          for (int e = 0; e < 8; e++) y[e] = x[n][e >> 2][e & 3] * f;
-          H8 hi, lo;
-          split8(y, hi, lo);
-          lds.in.q[2 * n][lane] = hi.u;
-          lds.in.q[2 * n + 1][lane] = lo.u;
-        }
+        for (int e = 0; e < 8; e++) y[e] = x[i][e >> 2][e & 3] * f;
+        H8 hi, lo;
+        split8(y, hi, lo);
+        lds.in.q[2 * (4 * i + wave)][lane] = hi.u;
+        lds.in.q[2 * (4 * i + wave) + 1][lane] = lo.u;
       }
     }
   }
@@ -549,6 +583,7 @@ __device__ __forceinline__ void few_unit(const PagedKernelArgs& p, const PagedUn
   }
 
   // ---- the four waves' results meet in LDS
+  const int tid = afresh(threadIdx.x), ec = tid & 15, eg = (tid >> 4) & 3;
   const float oscale = DT == KV_Q8 ? 1.0f / 127.0f : 1.0f;
   if constexpr (DT == KV_Q8) m += ev;
   __syncthreads();  // every wave is done with the queries and its scales
@@ -557,12 +592,12 @@ __device__ __forceinline__ void few_unit(const PagedKernelArgs& p, const PagedUn
     l = r.x + r.y;
     r = pair32(l);
     l = r.x + r.y;
-    if (g == 0) lds.out.ml[wave][c] = make_float2(m, l);
+    if (eg == 0) lds.out.ml[wave][ec] = make_float2(m, l);
 #pragma unroll
-    for (int j = 0; j < D / 16; j++) *(f32x4*)&lds.out.o[wave][c * D + swz(c, 4 * j + g) * 4] = o[j] * oscale;
+    for (int j = 0; j < D / 16; j++) *(f32x4*)&lds.out.o[wave][ec * D + swz(ec, 4 * j + eg) * 4] = o[j] * oscale;
   }
   __syncthreads();
-  for (int x = threadIdx.x; x < u.n_rho * (D / 4); x += 256) {
+  for (int x = tid; x < u.n_rho * (D / 4); x += 256) {
     const int i = x / (D / 4), ch = x % (D / 4);
     float mw[4], lw[4], top = -INFINITY;
 #pragma unroll
@@ -580,7 +615,7 @@ __device__ __forceinline__ void few_unit(const PagedKernelArgs& p, const PagedUn
       lsum += lw[w] * f;
       sum += *(const f32x4*)&lds.out.o[w][i * D + swz(i, ch) * 4] * f;
     }
-    const RowAt r = row_at(p, u, kvh, i);
+    const RowAt r = lds.row[i];
     store_o<D>(p, ws_o, r, 4 * ch, sum, lsum);
     if (ch == 0 && r.part >= 0) ws_ml[(size_t)r.part * p.b.H + r.head] = make_float2(top, lsum);
   }
@@ -634,18 +669,24 @@ __device__ __forceinline__ void mid_load_v(const PagedKernelArgs& p, size_t row,
 }
 
 template <int D, int DT>
-union MidLds {
+struct MidLds {
   static constexpr int NQ = DT == KV_F32 ? D / 8 : 2 * (D / 16);
-  struct {
-    u32x4 q[NQ][64];                           // the queries as matrix operands, the same for every wave
-    float s[DT == KV_Q8 ? 4 : 1][2][DT == KV_Q8 ? D : 1];  // q8: K and V scales of the tile a wave is at
-  } in;
-  f32x4 x[4][D / 64 * 4][64];                  // half of every wave's o, on its way to another wave
+  union {
+    struct {
+      u32x4 q[NQ][64];                         // the queries as matrix operands, the same for every wave
+      float s[DT == KV_Q8 ? 4 : 1][2][DT == KV_Q8 ? D : 1];  // q8: K and V scales of the tile a wave is at
+    } in;
+    f32x4 x[2][D / 8 * 64];                    // two waves' o
+  };
+  float2 ml[4][32];                            // the waves' (m, l)
+  float2 all[32];                              // the rows' (m, l)
+  RowAt row[32];
+  float top[4][32];                            // largest |q| of a wave's dims
 };
 
 template <int D, int DT>
 __device__ __forceinline__ void mid_unit(const PagedKernelArgs& p, const PagedUnit& u, int kvh, float* ws_o, float2* ws_ml,
-                                         MidLds<D, DT>& lds, float2 (*lml)[32]) {
+                                         MidLds<D, DT>& lds) {
   constexpr int ND = D / 32;
   const int wave = uniform(threadIdx.x >> 6), lane = threadIdx.x & 63, c = lane & 31, h = lane >> 5;
   const int shift = p.b.page_shift, P = 1 << shift;
@@ -663,47 +704,46 @@ __device__ __forceinline__ void mid_unit(const PagedKernelArgs& p, const PagedUn
     mid_load_k<D, DT>(p, row, wave < n_tiles, c, h, tk);
     mid_load_v<D, DT>(p, row, wave < n_tiles, c, h, tv);
   }
-  // ---- the queries: every wave looks at all of them (each row's factor), prepares its share
-  const RowAt ra = row_at(p, u, kvh, c);
+  // ---- the queries: a wave prepares every fourth operand; a row's factor needs all of them
   int pos;
-  float qs;
+  float qs = p.qscale;
   {
-    const int rho = u.rho0 + (ra.on ? c : 0);
-    pos = p.b.toks[u.tok + rho / p.b.G].pos;
+    const int tid = afresh(threadIdx.x), c = tid & 31, h = (tid >> 5) & 1, lane = tid & 63;
+    const RowAt ra = row_at(p, u, kvh, c);
+    pos = ra.pos;
+    if (wave == 0 && h == 0) lds.row[c] = ra;
     const float* q = p.q + ((size_t)ra.t * p.b.H + ra.head) * D;
     if constexpr (DT == KV_F32) {
 #pragma unroll
-      for (int n = 0; n < D / 8; n++)
-        if ((n & 3) == wave) lds.in.q[n][lane] = *(const u32x4*)(q + 8 * n + 4 * h);
-      qs = p.qscale;
+      for (int i = 0; i < D / 32; i++) lds.in.q[4 * i + wave][lane] = *(const u32x4*)(q + 8 * (4 * i + wave) + 4 * h);
     } else {
       // product n: f16 dims 16 n + 8 h + e; q8 block n / 2, dims 16 h + 8 (n & 1) + e
-      f32x4 x[D / 16][2];
+      f32x4 x[D / 64][2];
       float top = 0.0f;
 #pragma unroll
-      for (int n = 0; n < D / 16; n++) {
+      for (int i = 0; i < D / 64; i++) {
+        const int n = 4 * i + wave;
         const float* at = q + (DT == KV_F16 ? 16 * n + 8 * h : 32 * (n >> 1) + 16 * h + 8 * (n & 1));
-        x[n][0] = *(const f32x4*)at;
-        x[n][1] = *(const f32x4*)(at + 4);
+        x[i][0] = *(const f32x4*)at;
+        x[i][1] = *(const f32x4*)(at + 4);
 #pragma unroll
-        for (int e = 0; e < 4; e++) top = fmaxf(top, fmaxf(fabsf(x[n][0][e]), fabsf(x[n][1][e])));
+        for (int e = 0; e < 4; e++) top = fmaxf(top, fmaxf(fabsf(x[i][0][e]), fabsf(x[i][1][e])));
       }
       const float2 r = pair32(top);
-      top = fmaxf(r.x, r.y);
+      lds.top[wave][c] = fmaxf(r.x, r.y);
+      __syncthreads();
       float undo;
-      const float f = row_factor(top, &undo);
-      qs = p.qscale * undo * (DT == KV_Q8 ? 1.0f / 127.0f : 1.0f);
+      const float f = row_factor(fmaxf(fmaxf(lds.top[0][c], lds.top[1][c]), fmaxf(lds.top[2][c], lds.top[3][c])), &undo);
+      qs *= undo * (DT == KV_Q8 ? 1.0f / 127.0f : 1.0f);
 #pragma unroll
-      for (int n = 0; n < D / 16; n++) {
-        if ((n & 3) == wave) {
-          float y[8];
+      for (int i = 0; i < D / 64; i++) {
+        float y[8];
 #pragma unroll
-          for (int e = 0; e < 8; e++) y[e] = x[n][e >> 2][e & 3] * f;
-          H8 hi, lo;
-          split8(y, hi, lo);
-          lds.in.q[2 * n][lane] = hi.u;
-          lds.in.q[2 * n + 1][lane] = lo.u;
-        }
+        for (int e = 0; e < 8; e++) y[e] = x[i][e >> 2][e & 3] * f;
+        H8 hi, lo;
+        split8(y, hi, lo);
+        lds.in.q[2 * (4 * i + wave)][lane] = hi.u;
+        lds.in.q[2 * (4 * i + wave) + 1][lane] = lo.u;
       }
     }
   }
@@ -911,74 +951,43 @@ __device__ __forceinline__ void mid_unit(const PagedKernelArgs& p, const PagedUn
     __builtin_amdgcn_sched_barrier(0);
   }
 
-  // ---- the four waves' results: all weighted by one maximum, then halves of o exchanged with the wave
-  // two away and quarters with the next one, so that each ends with the sum of a quarter of the dims
+  // ---- the four waves' results, weighted by one maximum: two waves' o through LDS to the other two, their
+  // sums through LDS to all threads, which store whole rows
+  const int tid = afresh(threadIdx.x), ec = tid & 31, eh = (tid >> 5) & 1;
   if constexpr (DT == KV_Q8) m += ev;
   {
     const float2 r = pair32(l);
     l = r.x + r.y;
   }
-  if (h == 0) lml[wave][c] = make_float2(m, l);
+  if (eh == 0) lds.ml[wave][ec] = make_float2(m, l);
   __syncthreads();  // and every wave is done with the queries and its scales
   float top = -INFINITY, lsum = 0.0f;
-  float2 z[4];
+#pragma unroll
+  for (int w = 0; w < 4; w++) top = fmaxf(top, lds.ml[w][ec].x);
 #pragma unroll
   for (int w = 0; w < 4; w++) {
-    z[w] = lml[w][c];
-    top = fmaxf(top, z[w].x);
+    const float2 z = lds.ml[w][ec];
+    lsum += z.x == -INFINITY ? 0.0f : z.y * exp2_hw(z.x - top);
   }
-#pragma unroll
-  for (int w = 0; w < 4; w++) lsum += z[w].x == -INFINITY ? 0.0f : z[w].y * exp2_hw(z[w].x - top);
   const float mine = (m == -INFINITY ? 0.0f : exp2_hw(m - top)) * (DT == KV_Q8 ? 1.0f / 127.0f : 1.0f);
 #pragma unroll
   for (int j = 0; j < ND; j++) o[j] *= mine;
-  auto send = [&](auto from, auto n) __attribute__((always_inline)) {
-#pragma unroll
-    for (int j = 0; j < n; j++)
-#pragma unroll
-      for (int w = 0; w < 4; w++)
-        lds.x[wave][4 * j + w][lane] = f32x4{o[from + j][4 * w], o[from + j][4 * w + 1], o[from + j][4 * w + 2], o[from + j][4 * w + 3]};
-  };
-  auto add = [&](auto to, auto n, int other) __attribute__((always_inline)) {
-#pragma unroll
-    for (int j = 0; j < n; j++)
-#pragma unroll
-      for (int w = 0; w < 4; w++) {
-        const f32x4 y = lds.x[other][4 * j + w][lane];
-#pragma unroll
-        for (int e = 0; e < 4; e++) o[to + j][4 * w + e] += y[e];
-      }
-  };
-  auto put = [&](auto at, auto n) __attribute__((always_inline)) {
-    if (!ra.on) return;
-#pragma unroll
-    for (int j = 0; j < n; j++)
-#pragma unroll
-      for (int w = 0; w < 4; w++)
-        store_o<D>(p, ws_o, ra, 32 * (at + j) + 8 * w + 4 * h,
-                   f32x4{o[at + j][4 * w], o[at + j][4 * w + 1], o[at + j][4 * w + 2], o[at + j][4 * w + 3]}, lsum);
-  };
-  constexpr int Q = ND / 4;  // 32-dim groups a wave ends with
-  using I0 = std::integral_constant<int, 0>;
-  using I1 = std::integral_constant<int, Q>;
-  using I2 = std::integral_constant<int, 2 * Q>;
-  using I3 = std::integral_constant<int, 3 * Q>;
-  if (wave < 2) send(I2{}, I2{});
-  else send(I0{}, I2{});
+  if (wave == 0 && eh == 0) lds.all[ec] = make_float2(top, lsum);
+  if (wave >= 2) put_o<ND>(lds.x[wave - 2], o, ec, eh);
   __syncthreads();
-  if (wave < 2) add(I0{}, I2{}, wave + 2);
-  else add(I2{}, I2{}, wave - 2);
+  if (wave < 2) {
+    add_o<ND>(lds.x[wave], o, ec, eh);
+    put_o<ND>(lds.x[wave], o, ec, eh);  // a lane's own places
+  }
   __syncthreads();
-  if (wave == 0) send(I1{}, I1{});
-  else if (wave == 1) send(I0{}, I1{});
-  else if (wave == 2) send(I3{}, I1{});
-  else send(I2{}, I1{});
-  __syncthreads();
-  if (wave == 0) { add(I0{}, I1{}, 1); put(I0{}, I1{}); }
-  else if (wave == 1) { add(I1{}, I1{}, 0); put(I1{}, I1{}); }
-  else if (wave == 2) { add(I2{}, I1{}, 3); put(I2{}, I1{}); }
-  else { add(I3{}, I1{}, 2); put(I3{}, I1{}); }
-  if (wave == 0 && h == 0 && ra.on && ra.part >= 0) ws_ml[(size_t)ra.part * p.b.H + ra.head] = make_float2(top, lsum);
+#pragma unroll 1
+  for (int x = tid; x < u.n_rho * (D / 4); x += 256) {
+    const int i = x / (D / 4), ch = x % (D / 4);
+    const RowAt r = lds.row[i];
+    const float2 z = lds.all[i];
+    store_o<D>(p, ws_o, r, 4 * ch, get_o(lds.x[0], i, ch) + get_o(lds.x[1], i, ch), z.y);
+    if (ch == 0 && r.part >= 0) ws_ml[(size_t)r.part * p.b.H + r.head] = z;
+  }
 }
 
 // ------------------------------------------------------------------------------------------ many
@@ -1018,8 +1027,7 @@ __device__ __forceinline__ void many_unit(const PagedKernelArgs& p, const PagedU
   H8 qh[DT == KV_F32 ? 1 : NK], ql[DT == KV_F32 ? 1 : NK];
   f32x4 qf[DT == KV_F32 ? NK : 1];
   {
-    const int rho = u.rho0 + (ra.on ? 32 * wave + c : 0);
-    pos = p.b.toks[u.tok + rho / p.b.G].pos;
+    pos = ra.pos;
     const float* q = p.q + ((size_t)ra.t * p.b.H + ra.head) * D;
     if constexpr (DT == KV_F32) {
 #pragma unroll
@@ -1212,7 +1220,7 @@ __device__ __forceinline__ void many_unit(const PagedKernelArgs& p, const PagedU
   }
   const float2 r = pair32(l);
   l = r.x + r.y;
-  if (ra.on) {
+  if (32 * wave + c < u.n_rho) {
 #pragma unroll
     for (int j = 0; j < D / 32; j++)
 #pragma unroll
@@ -1250,7 +1258,6 @@ constexpr int mid_waves() { return D == 256 && DT != KV_Q8 ? 1 : 2; }
 template <int D, int DT>
 __global__ __launch_bounds__(256, (mid_waves<D, DT>())) void paged_mid_kernel(PagedKernelArgs p) {
   __shared__ MidLds<D, DT> lds;
-  __shared__ float2 ml[4][32];
   const PagedHeader* h = p.b.hdr;
   const int first = p.n_blocks ? p.first : h->n_many;
   const int total = p.n_blocks ? p.n_blocks : h->n_mid * p.kv_heads;
@@ -1258,7 +1265,7 @@ __global__ __launch_bounds__(256, (mid_waves<D, DT>())) void paged_mid_kernel(Pa
   float2* ws_ml = h->ws_ml;
   for (int b = blockIdx.x; b < total; b += gridDim.x) {
     const PagedUnit u = p.b.units[first + b / p.kv_heads];
-    mid_unit<D, DT>(p, u, b % p.kv_heads, ws_o, ws_ml, lds, ml);
+    mid_unit<D, DT>(p, u, b % p.kv_heads, ws_o, ws_ml, lds);
     __syncthreads();  // the unit's LDS is read before the next one's is written
   }
 }
