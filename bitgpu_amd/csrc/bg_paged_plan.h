@@ -369,7 +369,7 @@ class PagedPlanner {
   void chunk() {
     // [kind][head_dim 128, 256][dtype]: workgroups a CU, us of a 32-position tile of one unit with all of
     // them at work, and alone on a CU. 16-row units: 5.6 TB/s, and a wave's latency.
-    static const int kSlots[3][2][3] = {{{2, 2, 2}, {1, 1, 1}}, {{2, 2, 2}, {1, 1, 2}}, {{2, 3, 3}, {1, 2, 2}}};
+    static const int kSlots[3][2][3] = {{{2, 2, 2}, {1, 1, 1}}, {{2, 2, 3}, {1, 1, 2}}, {{2, 3, 3}, {1, 2, 2}}};
     static const double kFull[2][2][3] = {{{0, 2.1, 0}, {11.2, 2.5, 0}}, {{2.5, 0.72, 0.89}, {4.2, 0.92, 2.0}}};
     static const double kAlone[2][2][3] = {{{0, 1.26, 0}, {11.2, 2.5, 0}}, {{1.26, 0.39, 0.56}, {4.2, 0.92, 1.4}}};
     for (int kd = 0; kd < 3; kd++) {

@@ -1253,7 +1253,7 @@ __global__ __launch_bounds__(256, D == 128 ? 2 : 1) void paged_many_kernel(Paged
 
 // workgroups of 32-row units a CU holds
 template <int D, int DT>
-constexpr int mid_waves() { return D == 256 && DT != KV_Q8 ? 1 : 2; }
+constexpr int mid_waves() { return D == 256 && DT != KV_Q8 ? 1 : D == 128 && DT == KV_Q8 ? 3 : 2; }
 
 template <int D, int DT>
 __global__ __launch_bounds__(256, (mid_waves<D, DT>())) void paged_mid_kernel(PagedKernelArgs p) {
