@@ -9,6 +9,7 @@
 #include <cstdarg>
 #include <cstdio>
 #include <cstring>
+#include <exception>
 #include <new>
 #include <string>
 #include <vector>
@@ -228,7 +229,7 @@ int32_t bg_paged_batch_create(const bg_paged_kv* c, int32_t H, int32_t max_seqs,
   if (!out) return fail(BG_E_INVALID, "bg_paged_batch_create: out is NULL");
   *out = nullptr;
   if (!c) return fail(BG_E_INVALID, "bg_paged_batch_create: NULL cache");
-  if (H < c->kv_heads || H % c->kv_heads) return fail(BG_E_INVALID, "heads %d must be a multiple of kv_heads %d", H, c->kv_heads);
+  if (H < c->kv_heads || H % c->kv_heads) return fail(BG_E_INVALID, "bg_paged_batch_create: heads %d must be a multiple of kv_heads %d", H, c->kv_heads);
   if (max_seqs < 1 || max_tokens < 1 || max_pages < 1)
     return fail(BG_E_INVALID, "bg_paged_batch_create: max_seqs %d, max_tokens %d, max_pages %d must be >= 1", max_seqs,
                 max_tokens, max_pages);
@@ -292,7 +293,7 @@ int32_t bg_paged_batch_set(bg_paged_batch* b, int32_t n_seqs, const int32_t* row
   try {
     const std::string wrong = b->planner.build(b->shape, n_seqs, rows, lens, tables, table_stride, b->next);
     if (!wrong.empty()) return fail(BG_E_INVALID, "bg_paged_batch_set: %s", wrong.c_str());
-  } catch (const std::bad_alloc&) {
+  } catch (const std::exception&) {  // the plan's arrays
     return fail(BG_E_OOM, "bg_paged_batch_set: out of host memory");
   }
   const bg::PagedPlan& p = b->next;
@@ -330,6 +331,7 @@ int32_t bg_paged_batch_set(bg_paged_batch* b, int32_t n_seqs, const int32_t* row
     if (b->ws) {  // launches before this set, in any stream, are done with the old one
       (void)hipDeviceSynchronize();
       (void)hipFree(b->ws);
+      b->set = false;  // should the upload of the new one fail
     }
     b->ws = ws;
     b->ws_bytes = bytes;
@@ -470,6 +472,7 @@ int32_t bg_paged_attention(const bg_paged_kv* c, int32_t layer, bg_paged_batch* 
   const bool captured = bg::api_capturing(st);
   if (!captured && b->plan.n_tokens == 0) return BG_OK;
   if (!q || !out) return fail(BG_E_INVALID, "bg_paged_attention: NULL argument");
+  if (q == out) return fail(BG_E_INVALID, "bg_paged_attention: out is q");
   if (((uintptr_t)q | (uintptr_t)out) & 15) return fail(BG_E_INVALID, "bg_paged_attention: q and out must be 16-byte aligned");
   if (captured) b->cap_tokens = std::min(b->cap_tokens, b->plan.n_tokens);
   bg::PagedAttnArgs a{};

@@ -565,6 +565,8 @@ class PagedKvCache:
                 return torch.empty(shape, dtype=dt, device=device)
             if t.dtype is not dt or t.shape != shape:
                 raise ValueError(f"bitgpu_amd: {name} must be {dt} {list(shape)}, got {t.dtype} {list(t.shape)}")
+            if not t.is_contiguous():
+                raise ValueError(f"bitgpu_amd: expected a contiguous tensor ({name})")
             return t
 
         self.k = pool(k, "k", (*lead, page_size, head_dim), elem)
@@ -729,6 +731,10 @@ def paged_qkv_prologue(cache: PagedKvCache, li: int, batch: PagedBatch, q, k, v,
         q_out = torch.empty_like(q) if stride == D and q.dim() == 3 else q.new_empty((q.numel() // (H * stride), H, D))
     ap = None
     if pair_axis is not None:
+        if not (isinstance(pair_axis, np.ndarray) and pair_axis.dtype == np.uint8 and pair_axis.ndim == 1):
+            pair_axis = _int32(pair_axis, "pair_axis", 1)
+            if pair_axis.size and (pair_axis.min() < 0 or pair_axis.max() > 255):
+                raise ValueError("bitgpu_amd: pair_axis holds axes, 0 to 3")
         pair_axis = np.ascontiguousarray(pair_axis, np.uint8)
         if pair_axis.shape != (rot_dim // 2,):
             raise ValueError(f"bitgpu_amd: pair_axis must hold {rot_dim // 2} axes, got shape {list(pair_axis.shape)}")
@@ -748,7 +754,9 @@ def paged_attention(cache: PagedKvCache, li: int, batch: PagedBatch, q, scale: f
     """:func:`attention` for a batch (bg_paged_attention): every new row of q [rows, H, D] over its
     sequence's pages up to its own position; pages that sequences share are scanned once for all. ``gate``
     [rows, H, D], its heads ``gate_stride`` values apart (D: contiguous; 2D: the gate half of the hybrid's
-    query | gate rows). Returns [rows, H, D]; rows beyond the batch's are not written."""
+    query | gate rows). Returns [rows, H, D]; rows beyond the batch's are not written. ``out`` may not be q.
+    A value in the pages that is not finite reaches all new rows of the sequences that list it, those
+    before its position too."""
     D, H, T, dev = cache.head_dim, batch.H, batch.n_tokens, cache.index
     qp = _rows_ptr(q, "q", T, H * D, dev)
     if out is None:

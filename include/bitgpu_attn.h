@@ -387,7 +387,9 @@ int32_t bg_paged_qkv_prologue(const bg_paged_kv* kv, int32_t layer, bg_paged_bat
  * (what they hold by then, the batch's own rows included). q, out [rows, H, head_dim] f32 (16-byte
  * aligned, not the same buffer), gate [rows, H, gate_stride] or NULL, out = attn / (1 + exp(-gate)). Results
  * are f32-accurate for every storage type and do not depend on which other sequences are in the batch
- * beyond that rounding. Allocates nothing. Rows of out beyond the batch's are left as they are. */
+ * beyond that rounding. A value in the pages that is not finite reaches all new rows of the sequences that
+ * list it (its factor of zero makes it NaN in rows before it). Allocates nothing. Rows of out beyond the
+ * batch's are left as they are. */
 int32_t bg_paged_attention(const bg_paged_kv* kv, int32_t layer, bg_paged_batch* batch, const float* q, float scale,
                            const float* gate, int32_t gate_stride, float* out, void* stream);
 
