@@ -114,3 +114,18 @@ def test_integers_taken(x, dims, want):
 def test_integers_refused(x, dims):
     with pytest.raises(ValueError):
         E._int32(x, "x", dims)
+
+
+@pytest.mark.parametrize("lists", [[], [[]], [[], [3]], [[1, 2], [3]], [(1, 2), [3, 4]], [np.array([1, 2]), [3]], [[np.int64(7)], [True, 9]],
+                                   [torch.tensor([5, 6]), (1,)], [[2**31 - 1, -2**31]]])
+def test_tables_of_lists(lists):
+    got = E._int32_rows(lists)
+    width = max(map(len, lists), default=0)
+    assert got.dtype == np.int32 and got.shape == (len(lists), width) and got.flags.c_contiguous
+    assert got.tolist() == [[int(x) for x in t] + [0] * (width - len(t)) for t in lists]
+
+
+@pytest.mark.parametrize("lists", [[[1.0]], [[1], [2.5]], [["a"]], [[2**31]], [[[1]]], [np.array([1.5])], [[None]]])
+def test_tables_refused(lists):
+    with pytest.raises(ValueError):
+        E._int32_rows(lists)
