@@ -8,9 +8,10 @@
 //             every edge of it with two or more sequences is one segment, scanned once for the rows of
 //             all of them. Only pages that every row of the member sees whole are shared, so no mask.
 //   private   the rest of each sequence, causal
-// and a segment into units: a tile of its rows (row = (token, head of the kv head's group)) times a
-// chunk of its positions, one unit a workgroup and kv head. A row that meets several units gets a
-// partial (o, m, l) from each, joined by the merge kernel; a row of one unit is stored directly.
+// and a segment into units: a tile of 128, 32 or 16 of its rows (row = (token, head of the kv head's
+// group)) times a chunk of its positions, one unit a workgroup and kv head. A row that meets several units
+// gets a partial (o, m, l) from each, joined by the merge kernel; a row of one unit is stored directly.
+// Everything is chosen by sizes and types alone, with the kernels' measured costs (kind, chunk).
 #pragma once
 
 #include <stdint.h>

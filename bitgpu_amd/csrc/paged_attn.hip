@@ -2,14 +2,26 @@
 // pages that sequences share scanned once for the rows of all of them.
 //
 // The plan (bg_paged_plan.h) hands every workgroup a unit: a tile of rows (row = (token, head of one kv
-// head's group), so a loaded key serves G heads of every member token) times a chunk of positions. Two
-// bodies, chosen by the unit's segment:
-//   few     <= 32 rows (a token, a verify): bound by the cache's bytes. Each of the four waves takes
-//           every fourth 32-position tile straight from the pages into matrix-core operand registers (no
-//           LDS, no barrier), the next tile's K in flight under the softmax and its V under the next
-//           scores; the waves' (o, m, l) meet in LDS at the end.
-//   many    more rows (a shared prefix, a prompt): bound by the matrix cores. 128 rows, 32 a wave; the
-//           positions staged through LDS once for all four waves, double-buffered.
+// head's group), so a loaded key serves G heads of every member token) times a chunk of positions, for one
+// kv head. Kv heads are the fastest index of the grid: with eight of them each XCD's L2 sees one head's
+// pages. Three kinds of units, each a kernel with its own registers and LDS (one kernel of all bodies
+// spilled: 64 ragged q8 sequences 278 us against 191):
+//   few     16 rows, a token's or two's. Bound by the pages' bytes: four waves take every fourth 32-position
+//           tile straight from the pages into matrix operand registers, the next tile's K in flight under
+//           the softmax and its V under the next scores. Three workgroups a CU (queries and q8 scales in
+//           LDS) keep enough of them in flight: 64 sequences of up to 8,192 q8 positions, 712 MB in
+//           136-142 us, 5.0-5.2 TB/s (two a CU 180 us; a device copy 5.1).
+//   mid     32 rows: verifies, short prompts, a prefix that a batch shares. As few, on the 32-row matrix
+//           products; one unit's four waves split the positions, so a chunk of them costs a quarter of the
+//           partials that four waves of different rows would need for the same parallelism. 128 rows behind
+//           16,384 shared f16 positions and their own tails, 144 MB: 48 us; bound by its waves' chains
+//           (two a SIMD; matrix cores a quarter, loads alone 31 us, products alone 27) and a start and an
+//           end of 9 us (descriptor, queries, first tile, exchange). Tried and slower: double-buffered K,
+//           64 rows over the same registers (50 us), three workgroups a CU for f16 (spills, 67).
+//   many    128 rows, 32 a wave: prompts, and prefixes with enough work for them. Positions staged through
+//           LDS once for all four waves, double-buffered by asynchronous copies. Bound by the matrix
+//           cores: two prompts of 777 and their 2,048 shared positions, 113 GFLOP in two parts a product,
+//           120 us, 0.94 PFLOP/s (a plain f16 product of 8,192 cubed: 1.1).
 //
 // Results are f32-accurate, as the f32 activations and outputs are: an f16 operand holds 11 bits, so the
 // query and the probabilities enter the f16 matrix cores as two parts each (hi = f16(x), lo = f16(x -
@@ -27,7 +39,6 @@
 // Masked positions: scores are replaced, not added to; V beyond the positions written so far (a page's
 // stale or never written slots, possibly NaN) is replaced by zero, its q8 scales too.
 #include <algorithm>
-#include <type_traits>
 
 #include "bg_paged.h"
 
@@ -1231,7 +1242,7 @@ __device__ __forceinline__ void many_unit(const PagedKernelArgs& p, const PagedU
   }
 }
 
-// The 128-row units and the few-row units are launches of their own, each with its own registers and LDS.
+// A workgroup a unit and kv head; a launch under capture walks the units of whatever batch is set.
 template <int D, int DT>
 __global__ __launch_bounds__(256, D == 128 ? 2 : 1) void paged_many_kernel(PagedKernelArgs p) {
   using M = Many<D, DT>;
@@ -1378,8 +1389,7 @@ template <int D, int DT>
 static hipError_t launch_attn(const PagedKernelArgs& k, const PagedAttnArgs& a, hipStream_t st) {
   const PagedBatchView& b = k.b;
   if (!b.captured && b.n_units == 0) return hipSuccess;
-  // Under capture a grid that fills the GPU walks the units of whatever batch is set at replay, of both
-  // kinds.
+  // Under capture grids that fill the GPU walk the units of whatever batch is set at replay, of every kind.
   PagedKernelArgs x = k;
   if constexpr (paged_has_many(D, DT)) {
     if (b.captured || b.n_many) {
