@@ -78,6 +78,11 @@ struct bg_paged_batch {
   bg::PagedPlan plan, next;
   int axes = 1, max_pos = -1;
   bool set = false;
+  // The stream of the last call. A call on another one first waits there for what the batch has enqueued:
+  // its launches read the arrays an upload writes, and share a workspace.
+  hipStream_t last = nullptr;
+  bool used = false;
+  hipEvent_t moved = nullptr;
   // what launches under capture rely on and later sets have to keep
   int cap_tokens = INT_MAX, cap_rope = INT_MAX, cap_axes = 0;
   bool cap_append = false;
@@ -146,11 +151,27 @@ int32_t check_pair(const char* who, const bg_paged_kv* c, const bg_paged_batch* 
   return BG_OK;
 }
 
+// Orders a call on `st` behind the batch's calls so far. (A launch under capture runs at replay: its order is
+// the caller's.)
+int32_t join_stream(const char* who, bg_paged_batch* b, hipStream_t st) {
+  if (b->used && b->last != st) {
+    if (bg::api_capturing(b->last))
+      return fail(BG_E_STATE, "%s: the batch worked on a stream that is being captured now", who);
+    hipError_t e = hipEventRecord(b->moved, b->last);
+    if (e == hipSuccess) e = hipStreamWaitEvent(st, b->moved, 0);
+    if (e != hipSuccess) return bg::api_hip_fail(e, "paged batch: the stream of its last call");
+  }
+  b->last = st;
+  b->used = true;
+  return BG_OK;
+}
+
 void free_batch(bg_paged_batch* b) {
   for (int i = 0; i < kSlots; i++) {
     if (b->host[i]) (void)hipHostFree(b->host[i]);
     if (b->done[i]) (void)hipEventDestroy(b->done[i]);
   }
+  if (b->moved) (void)hipEventDestroy(b->moved);
   if (b->dev) (void)hipFree(b->dev);
   if (b->ws) (void)hipFree(b->ws);
   delete b;
@@ -257,6 +278,7 @@ int32_t bg_paged_batch_create(const bg_paged_kv* c, int32_t H, int32_t max_seqs,
                                     (size_t)max_tokens * 4};
   for (int i = 0; i < N_SECTIONS; i++) b->at[i + 1] = b->at[i] + round256(bytes[i]);
   hipError_t e = hipMalloc((void**)&b->dev, b->at[N_SECTIONS]);
+  if (e == hipSuccess) e = hipEventCreateWithFlags(&b->moved, hipEventDisableTiming);
   for (int i = 0; i < kSlots && e == hipSuccess; i++) {
     e = hipHostMalloc((void**)&b->host[i], b->at[N_SECTIONS], hipHostMallocMapped | hipHostMallocCoherent);
     if (e == hipSuccess) e = hipEventCreateWithFlags(&b->done[i], hipEventDisableTiming);
@@ -318,6 +340,8 @@ int32_t bg_paged_batch_set(bg_paged_batch* b, int32_t n_seqs, const int32_t* row
     if (p.write_page >= 0)
       return fail(BG_E_STATE, "bg_paged_batch_set: page %d is written and listed elsewhere, and a prologue of this batch was captured", p.write_page);
   }
+  const int32_t rc = join_stream("bg_paged_batch_set", b, st);
+  if (rc != BG_OK) return rc;
   // the workspace of partials
   const size_t ml = round256((size_t)p.n_parts * b->H * sizeof(float2)), need = ml + (size_t)p.n_parts * b->H * b->shape.D * sizeof(float);
   if (need > b->ws_bytes) {
@@ -444,6 +468,9 @@ int32_t bg_paged_qkv_prologue(const bg_paged_kv* c, int32_t layer, bg_paged_batc
     b->cap_append = true;
   } else if (b->plan.n_tokens == 0) {
     return BG_OK;
+  } else {
+    const int32_t moved = join_stream("bg_paged_qkv_prologue", b, st);
+    if (moved != BG_OK) return moved;
   }
   a.q = q;
   a.q_stride = q_stride;
@@ -474,7 +501,12 @@ int32_t bg_paged_attention(const bg_paged_kv* c, int32_t layer, bg_paged_batch* 
   if (!q || !out) return fail(BG_E_INVALID, "bg_paged_attention: NULL argument");
   if (q == out) return fail(BG_E_INVALID, "bg_paged_attention: out is q");
   if (((uintptr_t)q | (uintptr_t)out) & 15) return fail(BG_E_INVALID, "bg_paged_attention: q and out must be 16-byte aligned");
-  if (captured) b->cap_tokens = std::min(b->cap_tokens, b->plan.n_tokens);
+  if (captured) {
+    b->cap_tokens = std::min(b->cap_tokens, b->plan.n_tokens);
+  } else {
+    const int32_t moved = join_stream("bg_paged_attention", b, st);
+    if (moved != BG_OK) return moved;
+  }
   bg::PagedAttnArgs a{};
   a.q = q;
   a.scale = scale;

@@ -613,8 +613,9 @@ class PagedKvCache:
 
 class PagedBatch:
     """What the paged calls work on (bg_paged_batch_create): up to ``max_seqs`` sequences with ``max_tokens``
-    new rows and ``max_pages`` listed pages in all. Set it once a step, before the layers' calls; all of
-    its GPU work belongs on one stream."""
+    new rows and ``max_pages`` listed pages in all. Set it once a step, before the layers' calls. Its calls
+    run in their order whatever streams they are made on; replays of a graph that holds them are the
+    caller's to order with the rest."""
 
     def __init__(self, cache: PagedKvCache, H: int, max_seqs: int, max_tokens: int, max_pages: int):
         self.cache, self.H, self.n_tokens = cache, H, 0

@@ -333,9 +333,11 @@ int32_t bg_kv_load(bg_kv_cache* cache, int32_t base, int32_t count, const void* 
  *              16 a + 8 c + 4 b + r of a 32-slot tile (a, b, c in 0..1, r in 0..3) at [2 a + b][dim][4 c + r]
  *   BG_KSCALE, BG_VSCALE (q8) [layer][page][kv_head][slot][head_dim / 32] f32, a value code * scale / 127
  * It need not be cleared: slots that no call wrote are never used, whatever they hold. Calls are not
- * re-entrant on one batch, and all GPU work of one batch belongs on ONE stream (its launches share a
- * workspace and read the arrays that bg_paged_batch_set uploads); batches of one pool may use different
- * streams where none reads a page that another writes. Every call needs the pool's device current. */
+ * re-entrant on one batch, whose launches share a workspace and read the arrays that bg_paged_batch_set
+ * uploads: a call on another stream than the batch's last one waits there for what the batch enqueued before
+ * (that stream still exists, and is not being captured), and replays of a graph that holds its launches are
+ * the caller's to order with its other calls. Batches of one pool may use different streams where none reads
+ * a page that another writes. Every call needs the pool's device current. */
 typedef struct bg_paged_kv bg_paged_kv;
 typedef struct bg_paged_batch bg_paged_batch;
 
