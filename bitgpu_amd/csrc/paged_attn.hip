@@ -978,7 +978,7 @@ __device__ __forceinline__ void mid_unit(const PagedKernelArgs& p, const PagedUn
 #pragma unroll
   for (int w = 0; w < 4; w++) {
     const float2 z = lds.ml[w][ec];
-    lsum += z.x == -INFINITY ? 0.0f : z.y * exp2_hw(z.x - top);
+    lsum += z.y * (z.x == -INFINITY ? 0.0f : exp2_hw(z.x - top));  // a sum that is NaN stays one
   }
   const float mine = (m == -INFINITY ? 0.0f : exp2_hw(m - top)) * (DT == KV_Q8 ? 1.0f / 127.0f : 1.0f);
 #pragma unroll
