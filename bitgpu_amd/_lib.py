@@ -76,6 +76,7 @@ SIGNATURES = [
     ("bg_paged_batch_destroy", _i32, [_vp]),
     ("bg_paged_batch_set", _i32, [_vp, _i32, _vp, _vp, _vp, _i32, _vp, _i32, _vp]),
     ("bg_paged_batch_info", _i32, [_vp, C.POINTER(C.c_int64)]),
+    ("bg_paged_batch_units", _i32, [_vp, C.POINTER(C.c_int64)]),
     ("bg_paged_qkv_prologue", _i32, [_vp, _i32, _vp, _vp, _i32, _vp, _vp, _vp, _vp, _f32, _vp, _vp, _i32, _i32, _vp, _vp,
                                      _vp]),
     ("bg_paged_attention", _i32, [_vp, _i32, _vp, _vp, _f32, _vp, _i32, _vp, _vp]),

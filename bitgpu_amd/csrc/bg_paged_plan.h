@@ -70,6 +70,9 @@ inline int paged_bytes32(int dtype) { return dtype == 0 ? 128 : dtype == 1 ? 64 
 // whether there is a kernel of 128-row units (elsewhere the 32-row ones are faster at every size)
 constexpr bool paged_has_many(int D, int dtype) { return dtype == 1 || (dtype == 0 && D == 256); }
 
+// and a kernel of 16-row units whose page loads are nontemporal
+constexpr bool paged_has_stream(int D, int dtype) { return D == 128 && dtype == 1; }
+
 struct PagedPlan {
   std::vector<PagedUnit> units;
   std::vector<PagedTok> toks;

@@ -429,6 +429,17 @@ int32_t bg_paged_batch_info(const bg_paged_batch* b, int64_t* out) {
   return BG_OK;
 }
 
+int32_t bg_paged_batch_units(const bg_paged_batch* b, int64_t* out) {
+  if (!b || !out) return fail(BG_E_INVALID, "bg_paged_batch_units: NULL argument");
+  if (!b->set) return fail(BG_E_STATE, "bg_paged_batch_units: the batch has not been set");
+  const bg::PagedPlan& p = b->plan;
+  out[0] = (int64_t)p.n_many * b->shape.kv_heads;
+  out[1] = (int64_t)p.n_mid * b->shape.kv_heads;
+  out[2] = ((int64_t)p.units.size() - p.n_many - p.n_mid) * b->shape.kv_heads;
+  out[3] = p.stream_few && bg::paged_has_stream(b->shape.D, b->shape.dtype);
+  return BG_OK;
+}
+
 int32_t bg_paged_qkv_prologue(const bg_paged_kv* c, int32_t layer, bg_paged_batch* b, const float* q, int32_t q_stride,
                               const float* k, const float* v, const float* q_gamma, const float* k_gamma, float eps,
                               const float* cos_tab, const float* sin_tab, int32_t rope_positions, int32_t rot_dim,

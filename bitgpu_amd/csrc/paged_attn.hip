@@ -1413,7 +1413,7 @@ static hipError_t launch_attn(const PagedKernelArgs& k, const PagedAttnArgs& a, 
     // beside tails of 71 MB 61 -> 57). Two row tiles that share a page want it kept (115 -> 149), and q8's
     // 8-byte and head_dim 256's strided pieces of a line come one after the other (138 -> 157, 137 -> 151).
     bool stream = false;
-    if constexpr (D == 128 && DT == KV_F16) {
+    if constexpr (paged_has_stream(D, DT)) {
       stream = b.stream_few;
       if (stream) hipLaunchKernelGGL((paged_few_kernel<D, DT, 2>), dim3(grid), dim3(256), 0, st, x);
     }

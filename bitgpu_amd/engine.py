@@ -651,10 +651,13 @@ class PagedBatch:
 
     def info(self) -> dict:
         """What is set: new rows, the attention's workgroups, runs of shared pages, positions it scans (a
-        shared run's once), rows merged from partials, partials."""
-        out = (C.c_int64 * 6)()
+        shared run's once), rows merged from partials, partials; and of the workgroups those of 128, 32 and
+        16 rows, and whether the last kind's pages pass the caches by."""
+        out, units = (C.c_int64 * 6)(), (C.c_int64 * 4)()
         check(lib().bg_paged_batch_info(self._h, out))
-        return dict(zip(("rows", "workgroups", "shared_runs", "positions", "merged_rows", "partials"), out))
+        check(lib().bg_paged_batch_units(self._h, units))
+        return dict(zip(("rows", "workgroups", "shared_runs", "positions", "merged_rows", "partials", "units128", "units32",
+                         "units16", "streamed"), (*out, *units)))
 
     def close(self):
         if self._h:

@@ -371,6 +371,9 @@ int32_t bg_paged_batch_set(bg_paged_batch* batch, int32_t n_seqs, const int32_t*
 /* Diagnostic of the batch that is set: out[0..5] = new rows, workgroups of the attention, runs of shared
  * pages, positions scanned (a shared run's once), rows that are merged from partials, partials. */
 int32_t bg_paged_batch_info(const bg_paged_batch* batch, int64_t* out);
+/* As bg_paged_batch_info, out[0..3] = workgroups of 128, of 32 and of 16 rows, and 1 where the last kind's pages
+ * (read once, more than caches keep) pass the caches by. */
+int32_t bg_paged_batch_units(const bg_paged_batch* batch, int64_t* out);
 
 /* bg_qkv_prologue for a batch: its rows' q [rows, H, q_stride], k and v [rows, kv_heads, head_dim] (any
  * may be NULL); normed and roped q into q_out [rows, H, head_dim], normed and roped k and plain v into
