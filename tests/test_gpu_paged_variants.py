@@ -1,0 +1,96 @@
+"""GPU: kernel variants that a rule on sizes picks for batches larger than the other tests': the prologue of
+many rows (four loads a wave), and single tokens over more f16 pages than caches keep."""
+import random
+
+import numpy as np
+import pytest
+import torch
+
+from bitgpu_amd import engine as E
+from tests.gpu_helpers import export_k_v, rope_dev
+from tests.paged_helpers import DEV, Pool, attention64, make_batch, set_batch
+from tests.test_gpu_paged_attention import close
+from tests.test_gpu_paged_prologue import inputs, stored
+
+pytestmark = pytest.mark.gpu
+
+MANY = 8192  # rows of q and k from which the prologue takes four loads a wave
+
+
+@pytest.mark.parametrize("kv,block", [("f32", 32), ("f16", 32), ("q8", 32), ("q8", 0)])
+@pytest.mark.parametrize("H,KV,D,rot", [(16, 8, 128, 128), (24, 4, 256, 64), (7, 7, 128, 20), (5, 5, 256, 256)])
+def test_many_rows_have_the_bits_of_one_sequence(dev, kv, block, H, KV, D, rot):
+    """Head counts that fill no item of four loads too; unwritten slots are checked by the smaller test."""
+    page, wanted = 64, -(-MANY // (H + KV)) + 40
+    rows, lens, tables, n_pages = make_batch(random.Random(D + rot), 4, page, lambda b: [wanted - 54, 1, 0, 53][b], 1, wanted + 90)
+    assert sum(rows) * (H + KV) > MANY
+    pool = Pool(KV, D, kv, page, n_pages, q8_block=block or D)
+    width = 2 * D if rot == 64 else D
+    q, k, v, gq, gk = inputs(sum(rows), H, KV, D, 1, width)
+    cos, sin, _, _ = rope_dev(1e6, rot, max(lens))
+    batch = set_batch(pool.cache, H, rows, lens, tables)
+    got = E.paged_qkv_prologue(pool.cache, 0, batch, q, k, v, gq, gk, 1e-6, cos, sin, rot, q_stride=width)
+    at = 0
+    for r, n, table in zip(rows, lens, tables):
+        if not r:
+            continue
+        one = E.KvCache(1, KV, D, kv, max_seq_len=n, capacity=n, q8_block=block or D)
+        want = E.qkv_prologue(one, 0, q[at:at + r], k[at:at + r], v[at:at + r], r, H, gq, gk, 1e-6, cos, sin, rot, n - r, n - r,
+                              q_stride=width)
+        assert torch.equal(got[at:at + r], want)
+        for a, b in zip(stored(pool, table, n - r, n), export_k_v(one, 0, n - r, r)):
+            assert np.array_equal(a, b)
+        one.close()
+        at += r
+
+
+@pytest.mark.parametrize("kv", ["f32", "f16", "q8"])
+@pytest.mark.parametrize("H,KV,D,rot", [(16, 8, 128, 128), (24, 4, 256, 64), (6, 2, 128, 36)])
+def test_many_rows_with_axes_are_those_of_small_batches(dev, kv, H, KV, D, rot):
+    """Three axes: the same bits as the rows give in batches of a few, which the smaller tests hold to
+    float64."""
+    page, T, half = 64, -(-MANY // (H + KV)) + 77, rot // 2
+    rng = np.random.default_rng(rot)
+    pos = rng.integers(0, 600, (3, T)).astype(np.int32)
+    axis = rng.integers(0, 3, half).astype(np.uint8)
+    need = -(-T // page)
+    q, k, v, gq, gk = inputs(T, H, KV, D, 3)
+    cos, sin, _, _ = rope_dev(1e4, rot, 600)
+    table = list(range(need))
+    whole, parts = Pool(KV, D, kv, page, need), Pool(KV, D, kv, page, need)
+    batch = set_batch(whole.cache, H, [T], [T], [table], positions=pos)
+    got = E.paged_qkv_prologue(whole.cache, 0, batch, q, k, v, gq, gk, 1e-6, cos, sin, rot, pair_axis=axis)
+    step = MANY // (H + KV) // 2
+    batch = E.PagedBatch(parts.cache, H, 1, step, need)
+    for a in range(0, T, step):
+        b = min(a + step, T)
+        batch.set([b - a], [b], [table], positions=pos[:, a:b])
+        part = E.paged_qkv_prologue(parts.cache, 0, batch, q[a:b], k[a:b], v[a:b], gq, gk, 1e-6, cos, sin, rot, pair_axis=axis)
+        assert torch.equal(got[a:b], part)
+    for a, b in zip(stored(whole, table, 0, T), stored(parts, table, 0, T)):
+        assert np.array_equal(a, b)
+
+
+@pytest.mark.parametrize("B,n", [(9, 2100), (40, 500)])
+def test_single_tokens_over_more_pages_than_caches_keep(dev, B, n):
+    """f16 pages of one reader, over 64 MB of them, pass the caches by; a part of the rows against float64, and
+    the same results from a batch of few sequences, which does not."""
+    H, KV, page = 32, 8, 64
+    rows, lens = [1] * B, [n - b % 7 for b in range(B)]
+    need = -(-n // page)
+    tables = [list(range(b * need, (b + 1) * need)) for b in range(B)]
+    pool = Pool(KV, 128, "f16", page, B * need)
+    for t, m in zip(tables, lens):
+        pool.fill(t, m)
+    batch = set_batch(pool.cache, H, rows, lens, tables)
+    info = batch.info()
+    assert info["streamed"] == 1 and info["units16"] == info["workgroups"]
+    q = torch.randn(B, H, 128, device=DEV)
+    got = E.paged_attention(pool.cache, 0, batch, q)
+    for b in (0, B // 2, B - 1):
+        want, tol = attention64(q[b:b + 1].cpu(), [pool.values(tables[b], lens[b])], [1], lens[b:b + 1])
+        close(got[b:b + 1].cpu().double(), want, tol)
+        one = set_batch(pool.cache, H, [1], lens[b:b + 1], tables[b:b + 1])
+        assert one.info()["streamed"] == 0
+        alone = E.paged_attention(pool.cache, 0, one, q[b:b + 1])
+        close(alone.cpu().double(), want, tol)
