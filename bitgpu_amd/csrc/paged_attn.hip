@@ -32,8 +32,9 @@
 //   p       2^(s - m + 8), m raised only when a tile's maximum passes it by 6 (most tiles skip the
 //           rescale): p <= 2^14 stays below f16's 65504, and the smallest f16 step is 2^-32 of the
 //           largest p;
-//   q8 V    p is multiplied by the block scale of its position; its exponent is lowered by ev, 2^ev above
-//           every scale so far (raised like m), so that the products stay as small.
+//   q8 V    p is multiplied by the block scale of its position in units of 2^e, e the block's own, 2^e above
+//           every scale of that block so far (o counts in the same units, rescaled when e is raised): the
+//           products stay as small, and a block keeps its bits whatever the other blocks hold.
 // S^T = K Q^T and O^T += V^T P^T: the score registers of a lane hold positions of one row, in exactly the
 // order in which the V tile stores them (bg_common.h), so P enters the second product as it lies.
 // Masked positions: scores are replaced, not added to; V beyond the positions written so far (a page's
@@ -100,9 +101,45 @@ __device__ inline void split8(const float (&x)[8], H8& hi, H8& lo) {
   }
 }
 
-// A power of two 2^e above every q8 value scale up to `big` (zero and NaN: the least one kept)
-__device__ inline float scale_exponent(float big) {
-  return (float)(min(max((int)((__float_as_uint(big) >> 23) & 0xff) - 126, -60), 60));
+// ---- q8 value scales. A lane loads D / 64 of a tile's, of blocks (lane * D / 64 + i) % (D / 32): the same
+// ones for every second lane. unit[i] holds 2^-e of its block, 2^e above every scale of the block so far. e
+// from -120 (zeros) to 126 (a scale of up to 2^128 is then below 4, its products below 2^16: two f16 parts
+// still hold them).
+constexpr float kUnit0 = 0x1p120f;
+constexpr int kDppRor4 = 0x124, kDppRor8 = 0x128;  // row_ror, within 16 lanes
+// o's blocks to the units that this tile's scales need: a power of two each, seldom anything
+template <int D, class V>
+__device__ __forceinline__ void raise_units(const float (&vs)[D / 64], float (&unit)[D / 64], V* o) {
+  constexpr int N = D / 64, PER = sizeof(V) == 16 ? 2 : 1;  // vectors of o a block
+  bool over = false;
+#pragma unroll
+  for (int i = 0; i < N; i++) over |= vs[i] * unit[i] > 1.0f;
+  if (!__any(over)) return;
+  float f[N];
+#pragma unroll
+  for (int i = 0; i < N; i++) {
+    float big = fmaxf(vs[i], dpp_mov<kDppXor2>(vs[i]));  // over the lanes of this one's parity
+    big = fmaxf(big, dpp_mov<kDppRor4>(big));
+    big = fmaxf(big, dpp_mov<kDppRor8>(big));
+    float2 r = pair16(big);
+    r = pair32(fmaxf(r.x, r.y));
+    const int e = min(max((int)((__float_as_uint(fmaxf(r.x, r.y)) >> 23) & 0xff) - 126, -120), 126);
+    const float up = fminf(unit[i], __uint_as_float((uint32_t)(127 - e) << 23));
+    f[i] = __int_as_float(max((127 << 23) + __float_as_int(up) - __float_as_int(unit[i]), 0));  // up / unit
+    unit[i] = up;
+  }
+#pragma unroll
+  for (int b = 0; b < D / 32; b++) {
+    const float fb = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(f[b % N]), b / N));
+#pragma unroll
+    for (int j = 0; j < PER; j++) o[PER * b + j] *= fb;
+  }
+}
+// what block b of o is to be multiplied by in the end (a value is code * scale / 127)
+template <int D>
+__device__ __forceinline__ float unit_of(const float (&unit)[D / 64], int b) {
+  const int u = __builtin_amdgcn_readlane(__float_as_int(unit[b % (D / 64)]), b / (D / 64));
+  return __int_as_float((254 << 23) - u) * (1.0f / 127.0f);
 }
 
 // 2^e with 2^e * top in [2^10, 2^11) for a row's largest |value|; 1 for zero, infinite and NaN rows
@@ -404,7 +441,11 @@ __device__ __forceinline__ void few_unit(const PagedKernelArgs& p, const PagedUn
   float m = -INFINITY, l = 0.0f;
 #pragma unroll
   for (int j = 0; j < D / 16; j++) o[j] = f32x4{0, 0, 0, 0};
-  float ev = -60.0f;     // q8: 2^ev is above every value scale so far
+  float unit[DT == KV_Q8 ? D / 64 : 1];  // q8: of the value scales
+  if constexpr (DT == KV_Q8) {
+#pragma unroll
+    for (int i = 0; i < D / 64; i++) unit[i] = kUnit0;
+  }
 
   for (int t = wave; t < n_tiles; t += 4) {
     const int key = u.key0 + 32 * t;
@@ -413,11 +454,17 @@ __device__ __forceinline__ void few_unit(const PagedKernelArgs& p, const PagedUn
     float* lk = lds.in.s[DT == KV_Q8 ? wave : 0][0];
     float* lv = lds.in.s[DT == KV_Q8 ? wave : 0][1];
     if constexpr (DT == KV_Q8) {
+      if (key + 32 > u.key1) {  // slots past the written positions; this lane's scales are of slot x / (D / 32)
+#pragma unroll
+        for (int i = 0; i < D / 64; i++)
+          if (key + (lane * (D / 64) + i) / (D / 32) >= u.key1) tl.vs[i] = 0.0f;
+      }
+      raise_units<D>(tl.vs, unit, o);
       // a wave's LDS accesses complete in order: the tile before is done with them
 #pragma unroll
       for (int i = 0; i < D / 64; i++) {
         lk[lane * (D / 64) + i] = tl.ks[i];
-        lv[lane * (D / 64) + i] = tl.vs[i];
+        lv[lane * (D / 64) + i] = tl.vs[i] * unit[i];
       }
       __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
       __builtin_amdgcn_wave_barrier();
@@ -485,8 +532,7 @@ __device__ __forceinline__ void few_unit(const PagedKernelArgs& p, const PagedUn
 #pragma unroll
       for (int e = 0; e < 8; e++) sc[e] = key + slot16(g, e) <= pos ? sc[e] : -INFINITY;
     }
-    const bool stale = key + 32 > u.key1;  // slots past the written positions
-    if (stale) {
+    if (DT != KV_Q8 && key + 32 > u.key1) {  // slots past the written positions
       if constexpr (DT == KV_F32) {
 #pragma unroll
         for (int j = 0; j < D / 16; j++)
@@ -500,17 +546,6 @@ __device__ __forceinline__ void few_unit(const PagedKernelArgs& p, const PagedUn
           keep[w] = (key + slot16(g, 2 * w) < u.key1 ? 0xffffu : 0u) | (key + slot16(g, 2 * w + 1) < u.key1 ? 0xffff0000u : 0u);
 #pragma unroll
         for (int j = 0; j < D / 16; j++) tl.v[j] &= keep;
-      } else {
-#pragma unroll
-        for (int i = 0; i < D / 64; i++) {  // this lane's scales are of slot (lane * D / 64 + i) / (D / 32)
-          if (key + (lane * (D / 64) + i) / (D / 32) >= u.key1) {
-            tl.vs[i] = 0.0f;
-            lv[lane * (D / 64) + i] = 0.0f;
-          }
-        }
-        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-        __builtin_amdgcn_wave_barrier();
-        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
       }
     }
     // ---- running maximum and sum
@@ -521,23 +556,15 @@ __device__ __forceinline__ void few_unit(const PagedKernelArgs& p, const PagedUn
     top = fmaxf(r.x, r.y);
     r = pair32(top);
     top = fmaxf(r.x, r.y) * qs;
-    float en = ev;
-    if constexpr (DT == KV_Q8) {
-      float big = tl.vs[0];
-#pragma unroll
-      for (int i = 1; i < D / 64; i++) big = fmaxf(big, tl.vs[i]);
-      en = fmaxf(ev, scale_exponent(wave_max(big)));
-    }
-    if (__any(top > m + kLazy || en > ev)) {
+    if (__any(top > m + kLazy)) {
       const float mn = top > m + kLazy ? top : m;
-      const float f = m == -INFINITY ? 1.0f : exp2_hw(m - mn + (DT == KV_Q8 ? ev - en : 0.0f));
+      const float f = m == -INFINITY ? 1.0f : exp2_hw(m - mn);
       m = mn;
-      ev = en;
       l *= f;
 #pragma unroll
       for (int j = 0; j < D / 16; j++) o[j] *= f;
     }
-    const float base = m == -INFINITY ? 0.0f : kPShift - m - (DT == KV_Q8 ? ev : 0.0f);
+    const float base = m == -INFINITY ? 0.0f : kPShift - m;
     float pr[8];
 #pragma unroll
     for (int e = 0; e < 8; e++) {
@@ -595,8 +622,10 @@ __device__ __forceinline__ void few_unit(const PagedKernelArgs& p, const PagedUn
 
   // ---- the four waves' results meet in LDS
   const int tid = afresh(threadIdx.x), ec = tid & 15, eg = (tid >> 4) & 3;
-  const float oscale = DT == KV_Q8 ? 1.0f / 127.0f : 1.0f;
-  if constexpr (DT == KV_Q8) m += ev;
+  if constexpr (DT == KV_Q8) {
+#pragma unroll
+    for (int j = 0; j < D / 16; j++) o[j] *= unit_of<D>(unit, j / 2);
+  }
   __syncthreads();  // every wave is done with the queries and its scales
   {
     float2 r = pair16(l);
@@ -605,7 +634,7 @@ __device__ __forceinline__ void few_unit(const PagedKernelArgs& p, const PagedUn
     l = r.x + r.y;
     if (eg == 0) lds.out.ml[wave][ec] = make_float2(m, l);
 #pragma unroll
-    for (int j = 0; j < D / 16; j++) *(f32x4*)&lds.out.o[wave][ec * D + swz(ec, 4 * j + eg) * 4] = o[j] * oscale;
+    for (int j = 0; j < D / 16; j++) *(f32x4*)&lds.out.o[wave][ec * D + swz(ec, 4 * j + eg) * 4] = o[j];
   }
   __syncthreads();
   for (int x = tid; x < u.n_rho * (D / 4); x += 256) {
@@ -770,7 +799,12 @@ __device__ __forceinline__ void mid_unit(const PagedKernelArgs& p, const PagedUn
   for (int j = 0; j < ND; j++)
 #pragma unroll
     for (int e = 0; e < 16; e++) o[j][e] = 0.0f;
-  float m = -INFINITY, l = 0.0f, ev = -60.0f;  // q8: 2^ev is above every value scale so far
+  float m = -INFINITY, l = 0.0f;
+  float unit[DT == KV_Q8 ? D / 64 : 1];  // q8: of the value scales
+  if constexpr (DT == KV_Q8) {
+#pragma unroll
+    for (int i = 0; i < D / 64; i++) unit[i] = kUnit0;
+  }
 
   for (int t = wave; t < n_tiles; t += 4) {
     const int key = u.key0 + 32 * t;
@@ -779,13 +813,19 @@ __device__ __forceinline__ void mid_unit(const PagedKernelArgs& p, const PagedUn
     float* lk = lds.in.s[DT == KV_Q8 ? wave : 0][0];
     float* lv = lds.in.s[DT == KV_Q8 ? wave : 0][1];
     if constexpr (DT == KV_Q8) {
+      if (key + 32 > u.key1) {  // slots past the written positions
+#pragma unroll
+        for (int i = 0; i < D / 64; i++)
+          if (key + (lane * (D / 64) + i) / (D / 32) >= u.key1) tv.vs[i] = 0.0f;
+      }
+      raise_units<D>(tv.vs, unit, o);
       // [block][position], so that a lane reads the four positions of a register group at once; a wave's
       // LDS accesses complete in order: the tile before is done with them
 #pragma unroll
       for (int i = 0; i < D / 64; i++) {
         const int x = lane * (D / 64) + i, at = x % (D / 32) * 32 + x / (D / 32);
         lk[at] = tk.ks[i];
-        lv[at] = tv.vs[i];
+        lv[at] = tv.vs[i] * unit[i];
       }
       __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
       __builtin_amdgcn_wave_barrier();
@@ -846,7 +886,7 @@ __device__ __forceinline__ void mid_unit(const PagedKernelArgs& p, const PagedUn
 #pragma unroll
       for (int e = 0; e < 16; e++) s[e] = key + 8 * (e >> 2) + 4 * h + (e & 3) <= pos ? s[e] : -INFINITY;
     }
-    if (key + 32 > u.key1) {  // slots past the written positions
+    if (DT != KV_Q8 && key + 32 > u.key1) {  // slots past the written positions
       if constexpr (DT == KV_F32) {
 #pragma unroll
         for (int x = 0; x < 2; x++)
@@ -869,18 +909,6 @@ __device__ __forceinline__ void mid_unit(const PagedKernelArgs& p, const PagedUn
 #pragma unroll
           for (int j = 0; j < ND; j++) tv.v[x * ND + j] &= keep;
         }
-      } else {
-#pragma unroll
-        for (int i = 0; i < D / 64; i++) {
-          const int x = lane * (D / 64) + i;
-          if (key + x / (D / 32) >= u.key1) {
-            tv.vs[i] = 0.0f;
-            lv[x % (D / 32) * 32 + x / (D / 32)] = 0.0f;
-          }
-        }
-        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-        __builtin_amdgcn_wave_barrier();
-        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
       }
     }
     // ---- running maximum and sum
@@ -889,23 +917,15 @@ __device__ __forceinline__ void mid_unit(const PagedKernelArgs& p, const PagedUn
     for (int e = 1; e < 16; e++) top = fmaxf(top, s[e]);
     const float2 r = pair32(top);
     top = fmaxf(r.x, r.y) * qs;
-    float en = ev;
-    if constexpr (DT == KV_Q8) {
-      float big = tv.vs[0];
-#pragma unroll
-      for (int i = 1; i < D / 64; i++) big = fmaxf(big, tv.vs[i]);
-      en = fmaxf(ev, scale_exponent(wave_max(big)));
-    }
-    if (__any(top > m + kLazy || en > ev)) {
+    if (__any(top > m + kLazy)) {
       const float mn = top > m + kLazy ? top : m;
-      const float f = m == -INFINITY ? 1.0f : exp2_hw(m - mn + (DT == KV_Q8 ? ev - en : 0.0f));
+      const float f = m == -INFINITY ? 1.0f : exp2_hw(m - mn);
       m = mn;
-      ev = en;
       l *= f;
 #pragma unroll
       for (int j = 0; j < ND; j++) o[j] *= f;
     }
-    const float base = m == -INFINITY ? 0.0f : kPShift - m - (DT == KV_Q8 ? ev : 0.0f);
+    const float base = m == -INFINITY ? 0.0f : kPShift - m;
 #pragma unroll
     for (int e = 0; e < 16; e++) {
       s[e] = exp2_hw(fmaf(s[e], qs, base));
@@ -965,7 +985,6 @@ __device__ __forceinline__ void mid_unit(const PagedKernelArgs& p, const PagedUn
   // ---- the four waves' results, weighted by one maximum: two waves' o through LDS to the other two, their
   // sums through LDS to all threads, which store whole rows
   const int tid = afresh(threadIdx.x), ec = tid & 31, eh = (tid >> 5) & 1;
-  if constexpr (DT == KV_Q8) m += ev;
   {
     const float2 r = pair32(l);
     l = r.x + r.y;
@@ -980,9 +999,12 @@ __device__ __forceinline__ void mid_unit(const PagedKernelArgs& p, const PagedUn
     const float2 z = lds.ml[w][ec];
     lsum += z.y * (z.x == -INFINITY ? 0.0f : exp2_hw(z.x - top));  // a sum that is NaN stays one
   }
-  const float mine = (m == -INFINITY ? 0.0f : exp2_hw(m - top)) * (DT == KV_Q8 ? 1.0f / 127.0f : 1.0f);
+  const float mine = m == -INFINITY ? 0.0f : exp2_hw(m - top);
 #pragma unroll
-  for (int j = 0; j < ND; j++) o[j] *= mine;
+  for (int j = 0; j < ND; j++) {
+    if constexpr (DT == KV_Q8) o[j] *= mine * unit_of<D>(unit, j);
+    else o[j] *= mine;
+  }
   if (wave == 0 && eh == 0) lds.all[ec] = make_float2(top, lsum);
   if (wave >= 2) put_o<ND>(lds.x[wave - 2], o, ec, eh);
   __syncthreads();

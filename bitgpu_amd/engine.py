@@ -779,6 +779,7 @@ def paged_attention(cache: PagedKvCache, li: int, batch: PagedBatch, q, scale: f
     sequence's pages up to its own position; pages that sequences share are scanned once for all. ``gate``
     [rows, H, D], its heads ``gate_stride`` values apart (D: contiguous; 2D: the gate half of the hybrid's
     query | gate rows). Returns [rows, H, D]; rows beyond the batch's are not written. ``out`` may not be q.
+    f32-accurate (bitgpu_attn.h says to what, for q8 values of very unequal sizes too).
     A value in the pages that is not finite reaches all new rows of the sequences that list it, those
     before its position too."""
     D, H, T, dev = cache.head_dim, batch.H, batch.n_tokens, cache.index

@@ -392,7 +392,9 @@ int32_t bg_paged_qkv_prologue(const bg_paged_kv* kv, int32_t layer, bg_paged_bat
  * (what they hold by then, the batch's own rows included). q, out [rows, H, head_dim] f32 (16-byte
  * aligned, not the same buffer), gate [rows, H, gate_stride] or NULL, out = attn / (1 + exp(-gate)). Results
  * are f32-accurate for every storage type and do not depend on which other sequences are in the batch
- * beyond that rounding. A value in the pages that is not finite reaches all new rows of the sequences that
+ * beyond that rounding: a probability counts with 22 bits or to 2^-32 of the largest, whichever is more, of
+ * its position's value (f16) or of the largest scale that its 32-dim block has in the row's positions (q8);
+ * f32 pages round as f32 sums do. |values| from 2^100 on may overflow in the sums. A value in the pages that is not finite reaches all new rows of the sequences that
  * list it (its factor of zero makes it NaN in rows before it). Allocates nothing. Rows of out beyond the
  * batch's are left as they are. */
 int32_t bg_paged_attention(const bg_paged_kv* kv, int32_t layer, bg_paged_batch* batch, const float* q, float scale,

@@ -13,13 +13,15 @@ pytestmark = pytest.mark.gpu
 KINDS = [("f16", 128), ("f16", 256), ("f32", 256)]  # types with a kernel of 128-row units
 
 
-def attention64_on(q, kvs, rows, lens, scale=None, gate=None):
+def attention64_on(q, kvs, rows, lens, scale=None, gate=None, block=None):
     """The definition in float64 and its tolerance (paged_helpers.tolerance), a kv head at a time on the
-    queries' device: q [T, H, D] f32, kvs one (k, v) [lens, KV, D] float64 a sequence."""
+    queries' device: q [T, H, D] f32, kvs one (k, v) [lens, KV, D] float64 a sequence. The tolerance is
+    relative to the largest |v| of the `block` dims that a result's dim is in (all: None)."""
     T, H, D = q.shape
+    block = block or D
     scale = 1 / math.sqrt(D) if scale is None else scale
     out = torch.zeros(T, H, D, dtype=torch.float64, device=q.device)
-    tol = torch.zeros(T, H, 1, dtype=torch.float64, device=q.device)
+    tol = torch.zeros(T, H, D, dtype=torch.float64, device=q.device)
     t = 0
     for (k, v), r, n in zip(kvs, rows, lens):
         if not r:
@@ -34,9 +36,9 @@ def attention64_on(q, kvs, rows, lens, scale=None, gate=None):
             s = (x @ kt * scale).masked_fill(~mask, -math.inf)
             out[t:t + r, h * G:(h + 1) * G] = (torch.softmax(s, -1) @ vh).view(r, G, D)
             size = (x.abs() @ kt.abs() * scale).masked_fill(~mask, 0).amax(-1)
-            top = vh.abs().amax(-1).cummax(0).values[n - r:].repeat_interleave(G)
+            top = vh.abs().view(n, D // block, block).amax(-1).cummax(0).values[n - r:].repeat_interleave(G, 0)  # [r G, blocks]
             err = torch.tensor([tolerance(a, D, b) for a, b in zip(size.tolist(), m.tolist())], dtype=torch.float64, device=q.device)
-            tol[t:t + r, h * G:(h + 1) * G, 0] = (err * top).view(r, G)
+            tol[t:t + r, h * G:(h + 1) * G] = (err[:, None] * top).repeat_interleave(block, -1).view(r, G, D)
         t += r
     if gate is not None:
         out = out / (1 + torch.exp(-gate.double()))
