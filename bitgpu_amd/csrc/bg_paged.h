@@ -37,7 +37,7 @@ struct PagedBatchView {
   int pos_stride;
   int page_shift;
   int H, G;
-  // the set counts; all zero for a launch under capture, which reads hdr
+  // the set counts and their choices; all zero for a launch under capture, which reads hdr
   int n_units, n_many, n_mid, n_merges, n_merge_few, n_tokens, n_v_single, n_v_group;
   int stream_few;        // the few-row units' pages are read once, and too many to stay in a cache
   int captured;

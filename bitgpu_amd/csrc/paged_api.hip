@@ -103,8 +103,8 @@ struct bg_paged_batch {
     b.H = H;
     b.G = shape.G;
     b.captured = captured;
-    b.stream_few = plan.stream_few;
     if (!captured) {
+      b.stream_few = plan.stream_few;
       b.n_units = (int)plan.units.size();
       b.n_many = plan.n_many;
       b.n_mid = plan.n_mid;

@@ -94,3 +94,28 @@ def test_single_tokens_over_more_pages_than_caches_keep(dev, B, n):
         assert one.info()["streamed"] == 0
         alone = E.paged_attention(pool.cache, 0, one, q[b:b + 1])
         close(alone.cpu().double(), want, tol)
+
+
+def test_a_graph_keeps_to_the_caches(dev):
+    """Captured while such a batch is set, a launch takes the other variant (the batch of a later replay may
+    share pages), with the same bits."""
+    H, KV, page, B, n = 32, 8, 64, 9, 2100
+    tables = [list(range(33 * b, 33 * b + 33)) for b in range(B)]
+    pool = Pool(KV, 128, "f16", page, 33 * B)
+    for t in tables:
+        pool.fill(t, n)
+    batch = set_batch(pool.cache, H, [1] * B, [n] * B, tables)
+    assert batch.info()["streamed"] == 1
+    q, out = torch.randn(B, H, 128, device=DEV), torch.zeros(B, H, 128, device=DEV)
+    eager = E.paged_attention(pool.cache, 0, batch, q)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        E.paged_attention(pool.cache, 0, batch, q, out=out)
+    for rows, tabs in (([1] * B, tables), ([1] * B, [tables[0]] * B), ([1] * B, tables)):
+        batch.set(rows, [n] * B, tabs)
+        eager = E.paged_attention(pool.cache, 0, batch, q)
+        out.fill_(-1)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, eager)
