@@ -344,27 +344,25 @@ int32_t bg_paged_batch_set(bg_paged_batch* b, int32_t n_seqs, const int32_t* row
   if (rc != BG_OK) return rc;
   // the workspace of partials
   const size_t ml = round256((size_t)p.n_parts * b->H * sizeof(float2)), need = ml + (size_t)p.n_parts * b->H * b->shape.D * sizeof(float);
-  if (need > b->ws_bytes) {
-    float* ws = nullptr;
-    const size_t bytes = std::max(need, 2 * b->ws_bytes);  // at least twofold: few are ever replaced
-    hipError_t e = hipMalloc((void**)&ws, bytes);
-    if (e != hipSuccess) {
-      (void)hipGetLastError();
-      return bg::api_hip_fail(e, "paged attention workspace allocation");
-    }
-    if (b->ws) {  // launches before this set, in any stream, are done with the old one
-      (void)hipDeviceSynchronize();
-      (void)hipFree(b->ws);
-      b->set = false;  // should the upload of the new one fail
-    }
-    b->ws = ws;
-    b->ws_bytes = bytes;
-  }
   const int slot = b->slot;
   if (b->pending[slot]) {
     const hipError_t e = hipEventSynchronize(b->done[slot]);
     if (e != hipSuccess) return bg::api_hip_fail(e, "paged batch staging");
     b->pending[slot] = false;
+  }
+  float* ws = b->ws;
+  size_t ws_bytes = b->ws_bytes;
+  if (need > ws_bytes) {
+    ws_bytes = std::max(need, 2 * ws_bytes);  // at least twofold, where there is room: few are ever replaced
+    hipError_t e = hipMalloc((void**)&ws, ws_bytes);
+    if (e != hipSuccess && ws_bytes > need) {
+      (void)hipGetLastError();
+      e = hipMalloc((void**)&ws, ws_bytes = need);
+    }
+    if (e != hipSuccess) {
+      (void)hipGetLastError();
+      return bg::api_hip_fail(e, "paged attention workspace allocation");
+    }
   }
   char* h = b->host[slot];
   bg::PagedHeader hdr{};
@@ -376,8 +374,8 @@ int32_t bg_paged_batch_set(bg_paged_batch* b, int32_t n_seqs, const int32_t* row
   hdr.n_tokens = T;
   hdr.n_v_single = (int)p.v_single.size();
   hdr.n_v_group = (int)p.v_group.size();
-  hdr.ws_ml = (float2*)b->ws;
-  hdr.ws_o = b->ws ? (float*)((char*)b->ws + ml) : nullptr;
+  hdr.ws_ml = (float2*)ws;
+  hdr.ws_o = ws ? (float*)((char*)ws + ml) : nullptr;
   bg::PagedUpload up{};
   auto put = [&](int section, size_t offset, const void* src, size_t bytes) {
     if (bytes) memcpy(h + b->at[section] + offset, src, bytes);
@@ -406,7 +404,20 @@ int32_t bg_paged_batch_set(bg_paged_batch* b, int32_t n_seqs, const int32_t* row
     up.n16[S_POS] = (unsigned)(((size_t)T * 4 + 15) / 16);
   }
   hipError_t e = bg::launch_paged_upload(up, st);
-  if (e == hipSuccess) e = hipEventRecord(b->done[slot], st);
+  if (e != hipSuccess) {
+    if (ws != b->ws) (void)hipFree(ws);  // no launch knows it; those of before and captured ones keep the old
+    b->set = false;
+    return bg::api_hip_fail(e, "paged batch upload");
+  }
+  if (ws != b->ws) {
+    std::swap(ws, b->ws);
+    b->ws_bytes = ws_bytes;
+    if (ws) {  // the old one: launches, and replays that began before the new header was there, are done with it
+      (void)hipDeviceSynchronize();
+      (void)hipFree(ws);
+    }
+  }
+  e = hipEventRecord(b->done[slot], st);
   if (e != hipSuccess) return bg::api_hip_fail(e, "paged batch upload");
   b->pending[slot] = true;
   b->slot = (slot + 1) % kSlots;

@@ -362,8 +362,9 @@ int32_t bg_paged_batch_destroy(bg_paged_batch* batch);
  * ceil(lens[s] / page_size) are read). The batch's rows are numbered 0 .. sum(rows) - 1, sequence by
  * sequence. positions: the new tokens' rotary positions [axes][sum(rows)], axes 1 to 4; NULL: their
  * positions in the sequence. Checks everything (BG_E_INVALID, the batch before stays set), plans the
- * attention (runs of pages that sequences share are found here) and uploads it on `stream`. May allocate
- * the workspace of partials; not under graph capture (BG_E_STATE). Launches captured in a graph read the
+ * attention (runs of pages that sequences share are found here) and uploads it on `stream` (BG_E_DEVICE from
+ * the upload: to be set again). May allocate the workspace of partials (BG_E_OOM, the batch before stays set);
+ * not under graph capture (BG_E_STATE). Launches captured in a graph read the
  * batch at replay, so a batch may be set between replays: with at most as many new rows as were captured,
  * the same number of axes and positions inside the captured rope table (else BG_E_STATE). */
 int32_t bg_paged_batch_set(bg_paged_batch* batch, int32_t n_seqs, const int32_t* rows, const int32_t* lens,

@@ -4,8 +4,17 @@
 #include <hip/hip_runtime.h>
 
 #define main paged_api_main
+#define hipMalloc plain_malloc
 #include "paged_api.cpp"
+#undef hipMalloc
 #undef main
+
+static size_t room = ~(size_t)0;  // the largest block that the device has
+extern "C" hipError_t hipMalloc(void** p, size_t n) {
+  if (n > room) return hipErrorOutOfMemory;
+  note("malloc %zu", n);
+  return plain_malloc(p, n);
+}
 
 // f16 pages past 64 MB a layer that one row each reads: nontemporal, but not in a graph, whose batch changes
 static void cache_policy_under_capture() {
@@ -27,7 +36,58 @@ static void cache_policy_under_capture() {
   calls.clear();
 }
 
+// the workspace of partials, as the uploaded header (which captured launches read) has it
+static bool workspace_stands(size_t bytes = 4) { return inside(bg::seen.hdr->ws_o, bytes); }
+
+static void workspace_growth() {
+  Batch x;
+  CHECK(x.set({4}, {8000}, {range(0, 250)}, 0) == BG_OK && x.attend(0) == BG_OK);
+  CHECK(bg::seen.n_merges > 0 && workspace_stands());
+  size_t first = 0;
+  for (auto& c : calls)
+    if (sscanf(c.c_str(), "malloc %zu", &first) == 1) break;
+  const float* old = bg::seen.hdr->ws_o;
+  // an upload that fails: what the header names is still there
+  fail_upload = 1;
+  CHECK(x.set({64}, {60000}, {range(0, 1875)}, 0) == BG_E_DEVICE);
+  fail_upload = 0;
+  CHECK(bg::seen.hdr->ws_o == old && workspace_stands());
+  CHECK(x.attend(0) == BG_E_STATE);
+  // no room at all: the batch before stays set
+  CHECK(x.set({4}, {8000}, {range(0, 250)}, 0) == BG_OK);
+  calls.clear();
+  room = 1;
+  CHECK(x.set({64}, {60000}, {range(0, 1875)}, 0) != BG_OK);
+  calls.clear();
+  room = first;
+  CHECK(x.attend(0) == BG_OK && bg::seen.hdr->ws_o == old && workspace_stands());
+  EXPECT("attention on 0");
+  // room for what is needed, not for twice the old one
+  int len = 8000;
+  size_t bytes = 0;
+  room = 2 * first - 1;
+  while (len < 60000 && !bytes) {
+    len += 32;
+    calls.clear();
+    CHECK(x.set({4}, {len}, {range(0, (len + 31) / 32)}, 0) == BG_OK);
+    for (auto& c : calls) sscanf(c.c_str(), "malloc %zu", &bytes);
+  }
+  CHECK(bytes > first && bytes < 2 * first);
+  CHECK(x.attend(0) == BG_OK && workspace_stands());
+  // the old block goes behind the upload that replaces it
+  room = ~(size_t)0;
+  CHECK(x.set({1}, {40}, {{0, 1}}, 0) == BG_OK);
+  calls.clear();
+  CHECK(x.set({64}, {60000}, {range(0, 1875)}, 0) == BG_OK);
+  std::vector<std::string> order;
+  for (auto& c : calls)
+    if (c[0] == 'u' || c == "sync" || c == "free") order.push_back(c);
+  CHECK((order == std::vector<std::string>{"upload on 0", "sync", "free"}));
+  CHECK(x.attend(0) == BG_OK && workspace_stands());
+}
+
 int main() {
+  workspace_growth();
   cache_policy_under_capture();
   if (!blocks.empty()) line_of_fault(__LINE__, "blocks left");
   printf("ok\n");
