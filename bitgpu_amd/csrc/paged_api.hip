@@ -418,7 +418,11 @@ int32_t bg_paged_batch_set(bg_paged_batch* b, int32_t n_seqs, const int32_t* row
     }
   }
   e = hipEventRecord(b->done[slot], st);
-  if (e != hipSuccess) return bg::api_hip_fail(e, "paged batch upload");
+  if (e != hipSuccess) {  // the arrays are another plan's than `plan`, and nothing says when the slot is free
+    (void)hipDeviceSynchronize();
+    b->set = false;
+    return bg::api_hip_fail(e, "paged batch upload");
+  }
   b->pending[slot] = true;
   b->slot = (slot + 1) % kSlots;
   std::swap(b->plan, b->next);

@@ -86,7 +86,22 @@ static void workspace_growth() {
   CHECK(x.attend(0) == BG_OK && workspace_stands());
 }
 
+// an event that fails behind an upload: the arrays are no longer those of the plan that was set
+static void failed_event() {
+  Batch x;
+  CHECK(x.set({1, 1, 1}, {40, 40, 40}, {{0, 1}, {2, 3}, {4, 5}}, 0) == BG_OK && x.attend(0) == BG_OK);
+  calls.clear();
+  fail_record = 1;
+  CHECK(x.set({1}, {40}, {{0, 1}}, 0) == BG_E_DEVICE);
+  fail_record = 0;
+  EXPECT("upload on 0", "sync");
+  CHECK(x.attend(0) == BG_E_STATE && x.append(0) == BG_E_STATE);
+  CHECK(x.set({1}, {40}, {{0, 1}}, 0) == BG_OK && x.attend(0) == BG_OK);
+  CHECK(bg::seen.n_tokens == 1 && bg::seen.hdr->n_tokens == 1);
+}
+
 int main() {
+  failed_event();
   workspace_growth();
   cache_policy_under_capture();
   if (!blocks.empty()) line_of_fault(__LINE__, "blocks left");
