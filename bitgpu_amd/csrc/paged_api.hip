@@ -84,8 +84,8 @@ struct bg_paged_batch {
   bool used = false;
   hipEvent_t moved = nullptr;
   // what launches under capture rely on and later sets have to keep
-  int cap_tokens = INT_MAX, cap_rope = INT_MAX, cap_axes = 0;
-  bool cap_append = false;
+  int cap_tokens = INT_MAX, cap_rope = INT_MAX, cap_axes = 0;  // (cap_axes 0: nothing that rotates)
+  bool cap_write = false;                                      // something that writes pages
 
   bg::PagedBatchView view(bool captured) const {
     bg::PagedBatchView b{};
@@ -332,14 +332,12 @@ int32_t bg_paged_batch_set(bg_paged_batch* b, int32_t n_seqs, const int32_t* row
   }
   if (T > b->cap_tokens)
     return fail(BG_E_STATE, "bg_paged_batch_set: %d new rows, but launches of this batch were captured with %d", T, b->cap_tokens);
-  if (b->cap_append) {
-    if (n_axes != b->cap_axes)
-      return fail(BG_E_STATE, "bg_paged_batch_set: %d position axes, but a prologue of this batch was captured with %d", n_axes, b->cap_axes);
-    if (T && max_pos >= b->cap_rope)
-      return fail(BG_E_STATE, "bg_paged_batch_set: position %d outside the %d-row rope table of a captured prologue", max_pos, b->cap_rope);
-    if (p.write_page >= 0)
-      return fail(BG_E_STATE, "bg_paged_batch_set: page %d is written and listed elsewhere, and a prologue of this batch was captured", p.write_page);
-  }
+  if (b->cap_axes && n_axes != b->cap_axes)
+    return fail(BG_E_STATE, "bg_paged_batch_set: %d position axes, but a prologue of this batch was captured with %d", n_axes, b->cap_axes);
+  if (T && max_pos >= b->cap_rope)
+    return fail(BG_E_STATE, "bg_paged_batch_set: position %d outside the %d-row rope table of a captured prologue", max_pos, b->cap_rope);
+  if (b->cap_write && p.write_page >= 0)
+    return fail(BG_E_STATE, "bg_paged_batch_set: page %d is written and listed elsewhere, and a prologue of this batch was captured", p.write_page);
   const int32_t rc = join_stream("bg_paged_batch_set", b, st);
   if (rc != BG_OK) return rc;
   // the workspace of partials
@@ -487,14 +485,8 @@ int32_t bg_paged_qkv_prologue(const bg_paged_kv* c, int32_t layer, bg_paged_batc
                               "by another (or twice): give the writer a page of its own", b->plan.write_page);
   hipStream_t st = (hipStream_t)stream;
   const bool captured = bg::api_capturing(st);
-  if (captured) {
-    b->cap_tokens = std::min(b->cap_tokens, b->plan.n_tokens);
-    b->cap_rope = std::min(b->cap_rope, q || k ? rope_positions : INT_MAX);
-    b->cap_axes = b->axes;
-    b->cap_append = true;
-  } else if (b->plan.n_tokens == 0) {
-    return BG_OK;
-  } else {
+  if (!captured) {
+    if (b->plan.n_tokens == 0) return BG_OK;
     const int32_t moved = join_stream("bg_paged_qkv_prologue", b, st);
     if (moved != BG_OK) return moved;
   }
@@ -512,7 +504,16 @@ int32_t bg_paged_qkv_prologue(const bg_paged_kv* c, int32_t layer, bg_paged_batc
   a.q_out = q_out;
   a.num_cus = c->num_cus;
   const hipError_t e = bg::launch_paged_prologue(layer_view(c, layer), b->view(captured), a, st);
-  return e == hipSuccess ? BG_OK : bg::api_hip_fail(e, "paged prologue launch");
+  if (e != hipSuccess) return bg::api_hip_fail(e, "paged prologue launch");
+  if (captured) {
+    b->cap_tokens = std::min(b->cap_tokens, b->plan.n_tokens);
+    if (q || k) {
+      b->cap_rope = std::min(b->cap_rope, rope_positions);
+      b->cap_axes = b->axes;
+    }
+    b->cap_write |= k || v;
+  }
+  return BG_OK;
 }
 
 int32_t bg_paged_attention(const bg_paged_kv* c, int32_t layer, bg_paged_batch* b, const float* q, float scale,
@@ -527,9 +528,7 @@ int32_t bg_paged_attention(const bg_paged_kv* c, int32_t layer, bg_paged_batch* 
   if (!q || !out) return fail(BG_E_INVALID, "bg_paged_attention: NULL argument");
   if (q == out) return fail(BG_E_INVALID, "bg_paged_attention: out is q");
   if (((uintptr_t)q | (uintptr_t)out) & 15) return fail(BG_E_INVALID, "bg_paged_attention: q and out must be 16-byte aligned");
-  if (captured) {
-    b->cap_tokens = std::min(b->cap_tokens, b->plan.n_tokens);
-  } else {
+  if (!captured) {
     const int32_t moved = join_stream("bg_paged_attention", b, st);
     if (moved != BG_OK) return moved;
   }
@@ -541,7 +540,9 @@ int32_t bg_paged_attention(const bg_paged_kv* c, int32_t layer, bg_paged_batch* 
   a.out = out;
   a.num_cus = c->num_cus;
   const hipError_t e = bg::launch_paged_attention(layer_view(c, layer), b->view(captured), a, st);
-  return e == hipSuccess ? BG_OK : bg::api_hip_fail(e, "paged attention launch");
+  if (e != hipSuccess) return bg::api_hip_fail(e, "paged attention launch");
+  if (captured) b->cap_tokens = std::min(b->cap_tokens, b->plan.n_tokens);
+  return BG_OK;
 }
 
 }  // extern "C"

@@ -100,7 +100,38 @@ static void failed_event() {
   CHECK(bg::seen.n_tokens == 1 && bg::seen.hdr->n_tokens == 1);
 }
 
+// what a captured launch keeps later sets to is what that launch uses
+static void captured_parts() {
+  const int32_t pos[2] = {300, 300};
+  auto shared = [](Batch& x) { return x.set({1, 1}, {40, 40}, {{0, 1}, {2, 1}}, 0); };  // page 1 written by both
+  auto far = [](Batch& x) { return x.set({1}, {301}, {range(0, 10)}, 0); };
+  auto two = [&](Batch& x) { return x.set({1}, {40}, {{0, 1}}, 0, pos, 2); };
+  auto many = [](Batch& x) { return x.set({4}, {40}, {{0, 1}}, 0); };
+  struct { bool q, k, v; int32_t shared, far, two; } cases[] = {
+      {true, false, false, BG_OK, BG_E_STATE, BG_E_STATE}, {false, true, false, BG_E_STATE, BG_E_STATE, BG_E_STATE},
+      {false, false, true, BG_E_STATE, BG_OK, BG_OK}, {true, false, true, BG_E_STATE, BG_E_STATE, BG_E_STATE}};
+  for (auto& c : cases) {
+    Batch x;
+    CHECK(x.set({2}, {40}, {{0, 1}}, 0) == BG_OK);
+    capturing_now.insert(stream(6));
+    CHECK(bg_paged_qkv_prologue(x.kv, 0, x.b, c.q ? buf : nullptr, 128, c.k ? buf : nullptr, c.v ? buf : nullptr, buf, buf, 1e-6f, buf,
+                                buf, 100, 128, nullptr, buf, stream(6)) == BG_OK);
+    capturing_now.clear();
+    CHECK(shared(x) == c.shared && far(x) == c.far && two(x) == c.two && many(x) == BG_E_STATE);
+  }
+  {  // attention reads what it is given; a launch that was refused binds nothing
+    Batch x;
+    CHECK(x.set({2}, {40}, {{0, 1}}, 0) == BG_OK);
+    capturing_now.insert(stream(6));
+    CHECK(x.attend(6) == BG_OK && x.append(6, 39) == BG_E_INVALID);
+    capturing_now.clear();
+    CHECK(shared(x) == BG_OK && far(x) == BG_OK && two(x) == BG_OK && many(x) == BG_E_STATE);
+  }
+  calls.clear();
+}
+
 int main() {
+  captured_parts();
   failed_event();
   workspace_growth();
   cache_policy_under_capture();
