@@ -480,6 +480,13 @@ int32_t bg_paged_qkv_prologue(const bg_paged_kv* c, int32_t layer, bg_paged_batc
                          (uintptr_t)k_gamma | (uintptr_t)cos_tab | (uintptr_t)sin_tab) & 15;
   if (mis || (q && (q_stride & 3)))
     return fail(BG_E_INVALID, "bg_paged_qkv_prologue: buffers must be 16-byte aligned and q_stride a multiple of 4");
+  if (q && b->plan.n_tokens) {  // q in place: its own rows, each read whole before it is written
+    const size_t rows = (size_t)b->plan.n_tokens * b->H;
+    const char *q0 = (const char*)q, *o0 = (const char*)q_out;
+    const bool apart = q0 + ((rows - 1) * q_stride + c->D) * sizeof(float) <= o0 || o0 + rows * c->D * sizeof(float) <= q0;
+    if (!apart && !(q == q_out && q_stride == c->D))
+      return fail(BG_E_INVALID, "bg_paged_qkv_prologue: q_out overlaps q and is not q with q_stride head_dim");
+  }
   if ((k || v) && b->plan.write_page >= 0)
     return fail(BG_E_INVALID, "bg_paged_qkv_prologue: page %d would be written by one sequence and is listed with these positions "
                               "by another (or twice): give the writer a page of its own", b->plan.write_page);

@@ -731,16 +731,21 @@ def _rows_ptr(t, name, rows, width, device):
     return t.data_ptr()
 
 
+def _overlap(a, na, b, nb):
+    """Whether na f32 values at pointer a and nb at b share memory (pointers may be None)."""
+    return bool(a and b and na > 0 and nb > 0 and a < b + 4 * nb and b < a + 4 * na)
+
+
 def paged_qkv_prologue(cache: PagedKvCache, li: int, batch: PagedBatch, q, k, v, q_gamma, k_gamma, eps: float, cos_tab,
                        sin_tab, rot_dim: int, pair_axis=None, q_stride: int | None = None, q_out=None):
     """:func:`qkv_prologue` for a batch (bg_paged_qkv_prologue): q [rows, H, q_stride], k and v [rows, KV, D]
     (any may be None) of the batch's new rows, sequence by sequence; returns the normed and roped q
     [rows, H, D], with k and v written to their sequences' pages. ``pair_axis`` (rot_dim / 2 integers,
     needed where the batch was set with several position axes): the axis each rotary pair takes its
-    position from."""
+    position from. ``q_out`` may be q where its heads are D apart; otherwise it overlaps no input."""
     D, H, T, dev = cache.head_dim, batch.H, batch.n_tokens, cache.index
     stride, kw = int(q_stride or D), cache.kv_heads * D
-    qp = _rows_ptr(q, "q", T, H * stride, dev)
+    qp, kp, vp = _rows_ptr(q, "q", T, H * stride, dev), _rows_ptr(k, "k", T, kw, dev), _rows_ptr(v, "v", T, kw, dev)
     positions = 0
     if cos_tab is not None or sin_tab is not None:
         shapes = [None if t is None else t.shape for t in (cos_tab, sin_tab)]
@@ -750,6 +755,8 @@ def paged_qkv_prologue(cache: PagedKvCache, li: int, batch: PagedBatch, q, k, v,
         positions = shapes[0][0]
     if q is None or q_out is not None:
         op = _rows_ptr(q_out, "q_out", T, H * D, dev)
+        if qp and (_overlap(op, T * H * D, kp, T * kw) or _overlap(op, T * H * D, vp, T * kw)):
+            raise ValueError("bitgpu_amd: q_out overlaps k or v")
     else:
         q_out = torch.empty_like(q) if stride == D and q.dim() == 3 else q.new_empty((q.numel() // (H * stride), H, D))
         op = q_out.data_ptr()
@@ -764,7 +771,7 @@ def paged_qkv_prologue(cache: PagedKvCache, li: int, batch: PagedBatch, q, k, v,
             raise ValueError(f"bitgpu_amd: pair_axis must hold {rot_dim // 2} axes, got shape {list(pair_axis.shape)}")
         ap = pair_axis.ctypes.data
     rc = lib().bg_paged_qkv_prologue(
-        cache._h, li, batch._h, qp, stride, _rows_ptr(k, "k", T, kw, dev), _rows_ptr(v, "v", T, kw, dev),
+        cache._h, li, batch._h, qp, stride, kp, vp,
         _rows_ptr(q_gamma, "q_gamma", 1, D, dev), _rows_ptr(k_gamma, "k_gamma", 1, D, dev), eps,
         _rows_ptr(cos_tab, "cos", 0, 0, dev), _rows_ptr(sin_tab, "sin", 0, 0, dev), positions, rot_dim, ap,
         op, _stream())
@@ -778,10 +785,11 @@ def paged_attention(cache: PagedKvCache, li: int, batch: PagedBatch, q, scale: f
     """:func:`attention` for a batch (bg_paged_attention): every new row of q [rows, H, D] over its
     sequence's pages up to its own position; pages that sequences share are scanned once for all. ``gate``
     [rows, H, D], its heads ``gate_stride`` values apart (D: contiguous; 2D: the gate half of the hybrid's
-    query | gate rows). Returns [rows, H, D]; rows beyond the batch's are not written. ``out`` may not be q.
+    query | gate rows). Returns [rows, H, D]; rows beyond the batch's are not written.
+    ``out`` may be a contiguous gate; otherwise it overlaps no input.
     f32-accurate (bitgpu_attn.h says to what, for q8 values of very unequal sizes too).
-    A value in the pages that is not finite reaches all new rows of the sequences that list it, those
-    before its position too."""
+    A key in the pages that is not finite reaches the rows that attend it, a value those and new rows of
+    its sequence before it."""
     D, H, T, dev = cache.head_dim, batch.H, batch.n_tokens, cache.index
     qp = _rows_ptr(q, "q", T, H * D, dev)
     if out is not None:
@@ -799,6 +807,12 @@ def paged_attention(cache: PagedKvCache, li: int, batch: PagedBatch, q, scale: f
             raise ValueError(f"bitgpu_amd: gate must be [rows, {H}, {D}] with heads {gs} values apart, got "
                              f"{list(gate.shape)} with strides {list(gate.stride())}")
         gp = gate.data_ptr()
+    if out is not None and T:
+        n = T * H * D
+        if qp != op and _overlap(op, n, qp, n):  # (out = q: the library's error)
+            raise ValueError("bitgpu_amd: out overlaps q")
+        if _overlap(op, n, gp, (T * H - 1) * gs + D) and not (op == gp and gs == D):
+            raise ValueError("bitgpu_amd: out overlaps gate")
     rc = lib().bg_paged_attention(cache._h, li, batch._h, qp, _dense_scale(D) if scale is None else scale, gp, gs, op,
                                   _stream())
     if rc:

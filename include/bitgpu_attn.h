@@ -382,7 +382,8 @@ int32_t bg_paged_batch_units(const bg_paged_batch* batch, int64_t* out);
  * the sequences' pages at the rows' positions, the same bits as bg_qkv_prologue's. pair_axis (host,
  * rot_dim / 2 entries, NULL where the batch has one axis): which axis of the batch's positions each rotary
  * pair (dims j and j + rot_dim / 2) takes its angle from, e.g. time, height and width for images, in
- * sections or interleaved. The tables need rope_positions rows above every position. A page that a
+ * sections or interleaved. q_out may be q where q_stride is head_dim, and overlaps no other input. The tables
+ * need rope_positions rows above every position. A page that a
  * sequence writes must not be listed, with the written positions, by another one or twice (BG_E_INVALID);
  * rows of q_out and slots beyond the batch's are left as they are. */
 int32_t bg_paged_qkv_prologue(const bg_paged_kv* kv, int32_t layer, bg_paged_batch* batch, const float* q, int32_t q_stride,
@@ -392,13 +393,15 @@ int32_t bg_paged_qkv_prologue(const bg_paged_kv* kv, int32_t layer, bg_paged_bat
 
 /* bg_attention for a batch: row i of sequence s attends positions 0 .. lens[s] - rows[s] + i of its pages
  * (what they hold by then, the batch's own rows included). q, out [rows, H, head_dim] f32 (16-byte
- * aligned, not the same buffer), gate [rows, H, gate_stride] or NULL, out = attn / (1 + exp(-gate)). Results
- * are f32-accurate for every storage type and do not depend on which other sequences are in the batch
- * beyond that rounding: a probability counts with 22 bits or to 2^-32 of the largest, whichever is more, of
- * its position's value (f16) or of the largest scale that its 32-dim block has in the row's positions (q8);
- * f32 pages round as f32 sums do. |values| from 2^100 on may overflow in the sums. A value in the pages that is not finite reaches all new rows of the sequences that
- * list it (its factor of zero makes it NaN in rows before it). Allocates nothing. Rows of out beyond the
- * batch's are left as they are. */
+ * aligned), gate [rows, H, gate_stride] or NULL, out = attn / (1 + exp(-gate)). out may be a gate of
+ * gate_stride head_dim, and overlaps no other input. Allocates nothing. Rows of out beyond the batch's are
+ * left as they are.
+ * Results are f32-accurate for every storage type and do not depend on which other sequences are in the
+ * batch beyond that rounding: a probability counts with 22 bits or to 2^-32 of the largest, whichever is
+ * more, of its position's value (f16) or of the largest scale that its 32-dim block has in the row's
+ * positions (q8); f32 pages round as f32 sums do. |values| from 2^100 on may overflow in the sums. A key that
+ * is not finite reaches the rows that attend it, a value those and, by its factor of zero, new rows of the
+ * sequence before it. */
 int32_t bg_paged_attention(const bg_paged_kv* kv, int32_t layer, bg_paged_batch* batch, const float* q, float scale,
                            const float* gate, int32_t gate_stride, float* out, void* stream);
 

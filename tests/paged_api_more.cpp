@@ -130,7 +130,26 @@ static void captured_parts() {
   calls.clear();
 }
 
+// q_out over q: in place, or not at all
+static void overlaps() {
+  Batch x;  // 8 heads
+  CHECK(x.set({2}, {40}, {{0, 1}}, 0) == BG_OK);
+  static float mem[2 * 8 * 256 * 3];
+  float* m = (float*)(((uintptr_t)mem + 63) & ~(uintptr_t)63);
+  auto call = [&](const float* q, int stride, float* out) {
+    return bg_paged_qkv_prologue(x.kv, 0, x.b, q, stride, nullptr, nullptr, buf, nullptr, 1e-6f, buf, buf, 4096, 128, nullptr, out, stream(0));
+  };
+  const int dense = 2 * 8 * 128, wide = 15 * 256 + 128;
+  CHECK(call(m, 128, m) == BG_OK && call(m, 128, m + dense) == BG_OK && call(m + dense, 128, m) == BG_OK);
+  CHECK(call(m, 256, m + wide) == BG_OK && call(m + dense, 256, m) == BG_OK);
+  CHECK(call(m, 256, m) == BG_E_INVALID);                  // a head's row is written before the next is read
+  CHECK(call(m, 128, m + 128) == BG_E_INVALID && call(m + 128, 128, m) == BG_E_INVALID);
+  CHECK(call(m, 128, m + dense - 4) == BG_E_INVALID && call(m + dense - 4, 128, m) == BG_E_INVALID);
+  CHECK(call(m, 256, m + wide - 4) == BG_E_INVALID && call(m, 256, m + 128) == BG_E_INVALID);
+}
+
 int main() {
+  overlaps();
   captured_parts();
   failed_event();
   workspace_growth();

@@ -119,3 +119,29 @@ def test_a_graph_keeps_to_the_caches(dev):
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(out, eager)
+
+
+@pytest.mark.parametrize("T", [3, 700])
+@pytest.mark.parametrize("H,KV,D,rot", [(16, 8, 128, 128), (5, 5, 256, 64)])
+def test_q_normed_in_place(dev, T, H, KV, D, rot):
+    need = -(-T // 64)
+    pool = Pool(KV, D, "f16", 64, need)
+    q, k, v, gq, gk = inputs(T, H, KV, D, 11)
+    cos, sin, _, _ = rope_dev(1e6, rot, T)
+    batch = set_batch(pool.cache, H, [T], [T], [list(range(need))])
+    for kk, vv in ((k, v), (None, None)):
+        want = E.paged_qkv_prologue(pool.cache, 0, batch, q, kk, vv, gq, gk, 1e-6, cos, sin, rot)
+        mine = q.clone()
+        assert E.paged_qkv_prologue(pool.cache, 0, batch, mine, kk, vv, gq, gk, 1e-6, cos, sin, rot, q_out=mine) is mine
+        assert torch.equal(mine, want)
+
+
+@pytest.mark.parametrize("rows", [1, 60])
+def test_a_gate_that_becomes_the_output(dev, rows):
+    pool = Pool(2, 128, "f16", 64, 8)
+    table = list(range(8))
+    pool.fill(table, 500)
+    batch = set_batch(pool.cache, 8, [rows], [500], [table])
+    q, gate = torch.randn(rows, 8, 128, device=DEV), torch.randn(rows, 8, 128, device=DEV)
+    want = E.paged_attention(pool.cache, 0, batch, q, gate=gate)
+    assert torch.equal(E.paged_attention(pool.cache, 0, batch, q, gate=gate, out=gate), want)
