@@ -58,6 +58,8 @@ int32_t check_pool(const char* who, int32_t n_layers, int32_t kv_heads, int32_t 
     return fail(BG_E_UNSUPPORTED, "%s: page_size %d unsupported (32, 64, 128 or 256)", who, page_size);
   if ((long long)n_pages * page_size > INT_MAX)
     return fail(BG_E_UNSUPPORTED, "%s: %d pages of %d positions, beyond 2^31 - 1 positions", who, n_pages, page_size);
+  if ((long long)n_layers * kv_heads > 1 << 22)  // with the line above: a region's bytes stay below 2^63
+    return fail(BG_E_UNSUPPORTED, "%s: n_layers %d x kv_heads %d too large", who, n_layers, kv_heads);
   return BG_OK;
 }
 

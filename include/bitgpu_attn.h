@@ -345,7 +345,7 @@ typedef struct bg_paged_batch bg_paged_batch;
 int32_t bg_paged_region_bytes(int32_t n_layers, int32_t kv_heads, int32_t head_dim, int32_t dtype, int32_t page_size,
                               int32_t n_pages, int32_t region, size_t* bytes);
 /* A pool over the caller's buffers, which outlive it (scales NULL unless q8). head_dim 128 or 256;
- * n_pages * page_size below 2^31. */
+ * n_pages * page_size below 2^31, n_layers * kv_heads up to 2^22. */
 int32_t bg_paged_create(int32_t n_layers, int32_t kv_heads, int32_t head_dim, int32_t dtype, int32_t page_size,
                         int32_t n_pages, void* k, void* v, float* k_scale, float* v_scale, bg_paged_kv** out);
 int32_t bg_paged_destroy(bg_paged_kv* kv);

@@ -65,3 +65,15 @@ def test_outputs_beside_their_inputs(monkeypatch):
         E.paged_attention(cache, 0, batch, apart, gate=q, out=q)
     with pytest.raises(E.BitgpuError, match="NULL cache"):
         E.paged_qkv_prologue(cache, 0, batch, q, None, None, None, None, 1e-6, None, None, 128, q_out=q)
+
+
+@pytest.mark.parametrize("layers,KV", [(2**31 - 1, 2**31 - 1), (2**20, 5), (1, 2**22 + 1)])
+def test_a_pool_of_more_bytes_than_64_bits_count(layers, KV):
+    size, h = C.c_size_t(7), C.c_void_p(1)
+    for dtype in (_lib.BG_KV_F32, _lib.BG_KV_Q8):
+        assert _lib.lib().bg_paged_region_bytes(layers, KV, 256, dtype, 256, 2**23 - 1, _lib.BG_K, C.byref(size)) == _lib.BG_E_UNSUPPORTED
+        assert "too large" in message() and size.value == 7
+        assert _lib.lib().bg_paged_create(layers, KV, 256, dtype, 256, 2**23 - 1, 256, 256, None, None, C.byref(h)) == _lib.BG_E_UNSUPPORTED
+        assert not h
+    assert _lib.lib().bg_paged_region_bytes(2**20, 4, 256, _lib.BG_KV_F32, 256, 2**23 - 1, _lib.BG_K, C.byref(size)) == 0
+    assert size.value == 2**22 * (2**23 - 1) * 256 * 256 * 4
