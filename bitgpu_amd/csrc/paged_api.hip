@@ -529,7 +529,7 @@ int32_t bg_paged_attention(const bg_paged_kv* c, int32_t layer, bg_paged_batch* 
                            const float* gate, int32_t gate_stride, float* out, void* stream) {
   const int32_t rc = check_pair("bg_paged_attention", c, b, layer);
   if (rc != BG_OK) return rc;
-  if (!(scale > 0.0f) || !std::isfinite(scale)) return fail(BG_E_INVALID, "bg_paged_attention: scale must be positive");
+  if (!(scale > 0.0f) || !(scale < 0x1p127f)) return fail(BG_E_INVALID, "bg_paged_attention: scale must be positive and below 2^127");
   if (gate && gate_stride < c->D) return fail(BG_E_INVALID, "bg_paged_attention: gate_stride %d < head_dim", gate_stride);
   hipStream_t st = (hipStream_t)stream;
   const bool captured = bg::api_capturing(st);

@@ -154,6 +154,9 @@ __device__ inline float row_factor(float top, float* undo) {
   return __uint_as_float((uint32_t)(127 + s) << 23);
 }
 
+// A score's factor from the products' one. Never zero, which a masked score (-inf) would turn into NaN.
+__device__ inline float score_factor(float qs, float undo) { return fmaxf(qs * undo, 0x1p-149f); }
+
 // 8 int8 codes as exact f16 values: byte + 128 placed under the exponent of 1024, less 1152
 __device__ inline half8 codes8(u32x2 w) {
   H8 o;
@@ -416,7 +419,7 @@ __device__ __forceinline__ void few_unit(const PagedKernelArgs& p, const PagedUn
       __syncthreads();
       float undo;
       const float f = row_factor(fmaxf(fmaxf(lds.top[0][c], lds.top[1][c]), fmaxf(lds.top[2][c], lds.top[3][c])), &undo);
-      qs *= undo * (DT == KV_Q8 ? 1.0f / 127.0f : 1.0f);
+      qs = score_factor(qs, undo * (DT == KV_Q8 ? 1.0f / 127.0f : 1.0f));
 #pragma unroll
       for (int i = 0; i < NK / 4; i++) {
         float y[8];
@@ -774,7 +777,7 @@ __device__ __forceinline__ void mid_unit(const PagedKernelArgs& p, const PagedUn
       __syncthreads();
       float undo;
       const float f = row_factor(fmaxf(fmaxf(lds.top[0][c], lds.top[1][c]), fmaxf(lds.top[2][c], lds.top[3][c])), &undo);
-      qs *= undo * (DT == KV_Q8 ? 1.0f / 127.0f : 1.0f);
+      qs = score_factor(qs, undo * (DT == KV_Q8 ? 1.0f / 127.0f : 1.0f));
 #pragma unroll
       for (int i = 0; i < D / 64; i++) {
         float y[8];
@@ -1078,7 +1081,7 @@ __device__ __forceinline__ void many_unit(const PagedKernelArgs& p, const PagedU
       top = fmaxf(r.x, r.y);
       float undo;
       const float f = row_factor(top, &undo);
-      qs = p.qscale * undo;
+      qs = score_factor(p.qscale, undo);
 #pragma unroll
       for (int n = 0; n < NK; n++) {  // read again: half the registers of holding the row in f32
         const f32x4 a = *(const f32x4*)(q + 16 * n + 8 * h), b = *(const f32x4*)(q + 16 * n + 8 * h + 4);

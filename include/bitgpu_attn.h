@@ -393,9 +393,9 @@ int32_t bg_paged_qkv_prologue(const bg_paged_kv* kv, int32_t layer, bg_paged_bat
 
 /* bg_attention for a batch: row i of sequence s attends positions 0 .. lens[s] - rows[s] + i of its pages
  * (what they hold by then, the batch's own rows included). q, out [rows, H, head_dim] f32 (16-byte
- * aligned), gate [rows, H, gate_stride] or NULL, out = attn / (1 + exp(-gate)). out may be a gate of
- * gate_stride head_dim, and overlaps no other input. Allocates nothing. Rows of out beyond the batch's are
- * left as they are.
+ * aligned), scale positive and below 2^127, gate [rows, H, gate_stride] or NULL, out = attn / (1 +
+ * exp(-gate)). out may be a gate of gate_stride head_dim, and overlaps no other input. Allocates nothing. Rows
+ * of out beyond the batch's are left as they are.
  * Results are f32-accurate for every storage type and do not depend on which other sequences are in the
  * batch beyond that rounding: a probability counts with 22 bits or to 2^-32 of the largest, whichever is
  * more, of its position's value (f16) or of the largest scale that its 32-dim block has in the row's

@@ -145,3 +145,32 @@ def test_a_gate_that_becomes_the_output(dev, rows):
     q, gate = torch.randn(rows, 8, 128, device=DEV), torch.randn(rows, 8, 128, device=DEV)
     want = E.paged_attention(pool.cache, 0, batch, q, gate=gate)
     assert torch.equal(E.paged_attention(pool.cache, 0, batch, q, gate=gate, out=gate), want)
+
+
+@pytest.mark.parametrize("kv,D", [("f32", 128), ("f16", 128), ("q8", 128), ("f32", 256), ("f16", 256), ("q8", 256)])
+@pytest.mark.parametrize("rows", [1, 40, 600])
+@pytest.mark.parametrize("scale", [1.5e-45, 1e-38, 1e-30])
+def test_a_scale_that_makes_all_scores_equal(dev, kv, D, rows, scale):
+    """The smallest scales there are: every row is the mean of the values it sees, whatever is masked, for
+    queries of any size."""
+    n = 601
+    pool = Pool(2, D, kv, 64, 10)
+    table = list(range(10))
+    pool.fill(table, n)
+    batch = set_batch(pool.cache, 24, [rows], [n], [table])
+    q = torch.randn(rows, 24, D, device=DEV)
+    q[..., 12:, :] *= 1e-33
+    got = E.paged_attention(pool.cache, 0, batch, q, scale=scale).cpu().double()
+    v = pool.values(table, n)[1]
+    mean = (v.cumsum(0) / torch.arange(1, n + 1)[:, None, None])[n - rows:].repeat_interleave(12, 1)
+    # sums of n values and of n ones in f32 (sqrt(n) 2^-24), the parts of p (2^-21), the largest of many: 4
+    tol = 4 * (2 * n ** 0.5 * 2.0 ** -24 + 2.0 ** -21) * v.abs().max()
+    assert ((got - mean).abs() <= tol).all()
+
+
+def test_scales_refused(dev):
+    pool = Pool(1, 128, "f16", 32, 2)
+    batch = set_batch(pool.cache, 1, [1], [3], [[0]])
+    for scale in (2.0 ** 127, 3e38, float("inf"), 0.0, -1e-45):
+        with pytest.raises(E.BitgpuError, match="scale must be positive"):
+            E.paged_attention(pool.cache, 0, batch, torch.zeros(1, 1, 128, device=DEV), scale=scale)
