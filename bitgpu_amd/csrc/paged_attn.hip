@@ -113,12 +113,13 @@ __device__ __forceinline__ void raise_units(const float (&vs)[D / 64], float (&u
   constexpr int N = D / 64, PER = sizeof(V) == 16 ? 2 : 1;  // vectors of o a block
   bool over = false;
 #pragma unroll
-  for (int i = 0; i < N; i++) over |= vs[i] * unit[i] > 1.0f;
+  for (int i = 0; i < N; i++) over |= fabsf(vs[i] * unit[i]) > 1.0f;
   if (!__any(over)) return;
   float f[N];
 #pragma unroll
   for (int i = 0; i < N; i++) {
-    float big = fmaxf(vs[i], dpp_mov<kDppXor2>(vs[i]));  // over the lanes of this one's parity
+    float big = fabsf(vs[i]);
+    big = fmaxf(big, dpp_mov<kDppXor2>(big));  // over the lanes of this one's parity
     big = fmaxf(big, dpp_mov<kDppRor4>(big));
     big = fmaxf(big, dpp_mov<kDppRor8>(big));
     float2 r = pair16(big);

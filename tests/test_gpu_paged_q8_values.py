@@ -90,3 +90,14 @@ def test_a_scale_that_is_nan_stays_in_its_block(dev, kind):
     first = max(0, 35 - (lens[0] - rows[0]))
     assert got[first:, :, 64:96].isnan().all()
     assert torch.isfinite(got[first:][..., :64]).all() and torch.isfinite(got[first:][..., 96:]).all()
+
+
+@pytest.mark.parametrize("D", [128, 256])
+@pytest.mark.parametrize("kind", ["one", "shared", "verify", "prompt"])
+@pytest.mark.parametrize("some", [False, True])
+def test_scales_below_zero(dev, D, kind, some):
+    """Pages of the caller's own making: a value is code * scale / 127 whatever the scale's sign."""
+    def change(s):
+        sign = torch.where(torch.rand(s.shape, device=DEV) < 0.5, -1.0, 1.0) if some else -1.0
+        s.mul_(sign)
+    check(D, kind, change)
