@@ -174,3 +174,29 @@ def test_scales_refused(dev):
     for scale in (2.0 ** 127, 3e38, float("inf"), 0.0, -1e-45):
         with pytest.raises(E.BitgpuError, match="scale must be positive"):
             E.paged_attention(pool.cache, 0, batch, torch.zeros(1, 1, 128, device=DEV), scale=scale)
+
+
+@pytest.mark.parametrize("kv", ["f16", "q8"])
+def test_an_append_to_far_pages(dev, kv):
+    """Pages whose byte offset passes 2^32, in the second of two layers: the bits that near ones get, and what
+    the attention then reads."""
+    KV, D, page, H = 2, 128, 64, 8
+    n_pages = 5 * 2 ** 30 // (page * KV * D * (2 if kv == "f16" else 1))
+    far = [n_pages - 1, 2 ** 32 // (page * KV * D * 2) + 1, n_pages // 2 + 3, n_pages - 2]
+    near = list(range(4))
+    rows, lens = [1, 120], [65, 120]
+    cos, sin, _, _ = rope_dev(1e6, D, 128)
+    q, k, v, gq, gk = inputs(sum(rows), H, KV, D, 3)
+    outs = []
+    for n, ids in ((4, near), (n_pages, far)):
+        pool = Pool.__new__(Pool)
+        pool.cache = E.PagedKvCache(2, KV, D, kv, n_pages=n, page_size=page)
+        pool.KV, pool.D, pool.kv, pool.page, pool.gen = KV, D, kv, page, torch.Generator().manual_seed(1)
+        tables = [ids[:2], ids[2:]]
+        pool.fill(tables[0], 64, layer=1)
+        batch = set_batch(pool.cache, H, rows, lens, tables)
+        qr = E.paged_qkv_prologue(pool.cache, 1, batch, q, k, v, gq, gk, 1e-6, cos, sin, D)
+        outs.append([qr.cpu().numpy(), E.paged_attention(pool.cache, 1, batch, qr).cpu().numpy(), *stored(pool, tables[0], 64, 65, 1),
+                     *stored(pool, tables[1], 0, 120, 1)])
+        del pool, batch
+    assert all(np.array_equal(a, b) for a, b in zip(*outs))
