@@ -1415,7 +1415,8 @@ template <int D, int DT>
 static hipError_t launch_attn(const PagedKernelArgs& k, const PagedAttnArgs& a, hipStream_t st) {
   const PagedBatchView& b = k.b;
   if (!b.captured && b.n_units == 0) return hipSuccess;
-  // Under capture grids that fill the GPU walk the units of whatever batch is set at replay, of every kind.
+  // Under capture grids that fill the GPU walk the units of whatever batch is set at replay, of every kind (a
+  // kind without units takes 0.7-1.6 us, q8's few rows 4.5).
   PagedKernelArgs x = k;
   if constexpr (paged_has_many(D, DT)) {
     if (b.captured || b.n_many) {

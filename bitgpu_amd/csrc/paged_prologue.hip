@@ -204,7 +204,8 @@ __global__ __launch_bounds__(64) void paged_prologue_kernel(LayerView pool, Page
 }
 
 // Under capture: the items of whatever batch is set at replay, counted on the device, walked by a grid
-// that fills the GPU (the walk holds about 100 registers where one item holds 30 to 60).
+// that fills the GPU (the walk holds about 100 registers where one item holds 30 to 60: one token and 64 take as
+// long as outside a capture, 3,241 f32 rows 27-28 us instead of 21.6).
 template <int D, int DT, bool AXES>
 __global__ __launch_bounds__(64) void paged_prologue_walk_kernel(LayerView pool, PagedBatchView b, PagedAppendArgs a) {
   constexpr int RB = 64 / (D / 4);
