@@ -792,11 +792,6 @@ def paged_attention(cache: PagedKvCache, li: int, batch: PagedBatch, q, scale: f
     its sequence before it."""
     D, H, T, dev = cache.head_dim, batch.H, batch.n_tokens, cache.index
     qp = _rows_ptr(q, "q", T, H * D, dev)
-    if out is not None:
-        op = _rows_ptr(out, "out", T, H * D, dev)
-    else:
-        out = torch.empty_like(q) if q.dim() == 3 else q.new_empty((q.numel() // (H * D), H, D))
-        op = out.data_ptr()
     gs, gp = 0, None
     if gate is not None:
         gs = int(gate_stride if gate_stride is not None else D)
@@ -807,8 +802,11 @@ def paged_attention(cache: PagedKvCache, li: int, batch: PagedBatch, q, scale: f
             raise ValueError(f"bitgpu_amd: gate must be [rows, {H}, {D}] with heads {gs} values apart, got "
                              f"{list(gate.shape)} with strides {list(gate.stride())}")
         gp = gate.data_ptr()
-    if out is not None and T:
-        n = T * H * D
+    if out is None:
+        out = torch.empty_like(q) if q.dim() == 3 else q.new_empty((q.numel() // (H * D), H, D))
+        op = out.data_ptr()
+    else:
+        op, n = _rows_ptr(out, "out", T, H * D, dev), T * H * D
         if qp != op and _overlap(op, n, qp, n):  # (out = q: the library's error)
             raise ValueError("bitgpu_amd: out overlaps q")
         if _overlap(op, n, gp, (T * H - 1) * gs + D) and not (op == gp and gs == D):

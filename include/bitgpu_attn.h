@@ -367,7 +367,7 @@ int32_t bg_paged_batch_destroy(bg_paged_batch* batch);
  * not under graph capture (BG_E_STATE). Launches captured in a graph read the
  * batch at replay, so a batch may be set between replays: with at most as many new rows as were captured and,
  * where a prologue was, the same number of axes and positions inside its rope table (of q or k) and no page
- * that it may not write (of k or v), else BG_E_STATE; for as long as the batch lives. */
+ * that it may not write (of k or v), else BG_E_STATE; for as long as the batch lives, and it outlives the graph. */
 int32_t bg_paged_batch_set(bg_paged_batch* batch, int32_t n_seqs, const int32_t* rows, const int32_t* lens,
                            const int32_t* tables, int32_t table_stride, const int32_t* positions, int32_t axes, void* stream);
 /* Diagnostic of the batch that is set: out[0..5] = new rows, workgroups of the attention, runs of shared
