@@ -398,8 +398,8 @@ int32_t bg_paged_qkv_prologue(const bg_paged_kv* kv, int32_t layer, bg_paged_bat
  * of out beyond the batch's are left as they are.
  * Results are f32-accurate for every storage type and do not depend on which other sequences are in the
  * batch beyond that rounding: a probability counts with 22 bits or to 2^-32 of the largest, whichever is
- * more, of its position's value (f16) or of the largest scale that its 32-dim block has in the row's
- * positions (q8); f32 pages round as f32 sums do. |values| from 2^100 on may overflow in the sums. A key that
+ * more, of its position's value (f16) or of the largest scale that its 32-dim block has in the sequence
+ * (q8); f32 pages round as f32 sums do. |values| from 2^100 on may overflow in the sums. A key that
  * is not finite reaches the rows that attend it, a value those and, by its factor of zero, new rows of the
  * sequence before it. */
 int32_t bg_paged_attention(const bg_paged_kv* kv, int32_t layer, bg_paged_batch* batch, const float* q, float scale,
