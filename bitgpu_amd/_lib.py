@@ -80,6 +80,15 @@ SIGNATURES = [
     ("bg_paged_qkv_prologue", _i32, [_vp, _i32, _vp, _vp, _i32, _vp, _vp, _vp, _vp, _f32, _vp, _vp, _i32, _i32, _vp, _vp,
                                      _vp]),
     ("bg_paged_attention", _i32, [_vp, _i32, _vp, _vp, _f32, _vp, _i32, _vp, _vp]),
+    ("bg_linear_create", _i32, [_i32] * 7 + [_vp, _vp, C.POINTER(_vp)]),
+    ("bg_linear_destroy", _i32, [_vp]),
+    ("bg_linear_batch_create", _i32, [_vp, _i32, _i32, C.POINTER(_vp)]),
+    ("bg_linear_batch_destroy", _i32, [_vp]),
+    ("bg_linear_batch_set", _i32, [_vp, _i32, _vp, _vp, _vp, _vp]),
+    ("bg_linear_prologue", _i32, [_vp, _i32, _vp, _vp, _vp, _vp, _vp, _i32] + [_vp] * 8),
+    ("bg_linear_attention", _i32, [_vp, _i32, _vp, _vp, _vp, _vp, _vp, _i32, _vp, _f32, _vp, _vp, _f32, _vp, _vp]),
+    ("bg_gemv4_split", _i32, [_vp, _i32, _i32, _vp, _vp, _vp, _i32, _i32, _i32, _i32, _i32, _vp, _vp, _vp, _vp]),
+    ("bg_gemv4_resid", _i32, [_vp, _i32, _i32, _vp, _vp, _vp, _i32, _i32, _i32, _vp, _vp, _vp]),
 ]
 
 

@@ -1,0 +1,81 @@
+// Linear attention with a decay for each head: what its kernels (linear_prologue.hip, linear_attn.hip) and
+// its entry points (linear_api.hip) share.
+//
+// Per layer, slot and value head one f32 matrix [v_dim][k_dim] (the state, transposed: a row holds what one
+// value dim has gathered over the key dims), and per layer and slot the convolution's last inputs,
+// [conv_width - 1][channels], channels = q heads | k heads | v heads.
+#pragma once
+
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+namespace bg {
+
+constexpr int kLinChunk = 64;     // rows of a unit
+
+// A sequence of the batch: its new rows are rows row0 .. row0 + rows - 1 of the call's tensors; its state is
+// read from slot src (-1: zeros) and left in slot dst.
+struct LinSeq {
+  int row0, rows, src, dst;
+  int unit0, n_units;             // its units: runs of 64 rows, in order
+  int pad[2];
+};
+struct LinUnit {
+  int seq, row0, n, chunk;        // rows row0 .. row0 + n - 1, the chunk-th 64 of sequence `seq`
+};
+// What a captured launch reads of the batch instead of its arguments, so that a batch set again between
+// replays is the one the replay runs.
+struct LinHeader {
+  int n_seqs, n_tokens, n_units;
+  int pad;
+};
+
+// The batch as the kernels see it: device arrays at fixed addresses, written by one upload a set. The counts
+// are upper bounds for a launch under capture, whose kernels compare with hdr.
+struct LinBatchView {
+  const LinHeader* hdr;
+  const LinSeq* seqs;
+  const LinUnit* units;
+  int n_seqs, n_tokens, n_units;
+  int most;                       // rows of the longest sequence
+};
+
+// One layer of the caller's state.
+struct LinLayer {
+  float* state;                   // [slot][v_head][DV][DK]
+  float* conv;                    // [slot][taps - 1][channels]
+  int k_heads, v_heads, DK, DV, taps, channels;
+};
+
+struct LinPrologueArgs {
+  const float* qkv;               // [rows][channels]
+  const float* w;                 // [channels][taps]
+  const float* a; const float* b; int ab_stride;
+  const float* a_log; const float* dt_bias;
+  float *q, *k, *v, *g, *beta;
+};
+hipError_t launch_linear_prologue(const LinLayer& L, const LinBatchView& b, const LinPrologueArgs& a, hipStream_t st);
+
+struct LinAttnArgs {
+  const float *q, *k, *v;
+  const float* g; int g_stride;   // 0: one decay a head
+  const float* beta;              // NULL: a plain sum
+  float scale;
+  const float* gate; const float* norm; float eps;
+  float* out;
+};
+hipError_t launch_linear_attention(const LinLayer& L, const LinBatchView& b, const LinAttnArgs& a, hipStream_t st);
+
+// gemv4.hip: 4-bit projections. Code k of row n is bits 4 (k % 8) .. of codes[n][k / 8]; a weight is
+// (code - 8) * scale, or code * scale + min where mins is given, one scale (and min) per `group` weights.
+struct Gemv4Args {
+  const float* x; int M, K;
+  const uint32_t* codes; const void* scales; const void* mins;
+  int scale_f16, group;
+  int N0, N1, N2;
+  float *out0, *out1, *out2;
+  const float* resid;
+};
+hipError_t launch_gemv4(const Gemv4Args& a, hipStream_t st);
+
+}  // namespace bg

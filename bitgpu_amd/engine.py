@@ -17,7 +17,8 @@ The reference (stfurkan/bitgpu v0.19.1, src/engine.ts) records, per layer:
 
 The reference holds one conversation an engine. For many at once, on one pool of pages that sequences may
 share: :class:`PagedKvCache`, :class:`PagedBatch`, :func:`paged_qkv_prologue`, :func:`paged_attention`, and
-the layer blocks :func:`paged_layer_attention` and :func:`paged_hybrid_attention`.
+the layer blocks :func:`paged_layer_attention` and :func:`paged_hybrid_attention`. The hybrid's linear-attention
+layers and 4-bit projections are in linear.py and have their names here too.
 
 Device memory is owned by torch tensors (``cuda`` device, float32, contiguous); only raw
 pointers cross the boundary. Every call is enqueued on torch's current stream. There is no CPU
@@ -36,44 +37,17 @@ try:
 except ImportError:  # the host-only functions (tables, plans, snapshot checks) need no torch
     torch = None
 
+from ._args import _f32, _int32, _ptr, _rows_ptr, _stream
 from ._lib import (BG_E_INVALID, BG_E_STATE, BG_K, BG_KSCALE, BG_ROPE_ABSOLUTE, BG_ROPE_SLOT, BG_V, BG_VSCALE,
                    KV_DTYPES, BitgpuError, check, lib)
+from .linear import (FourBitWeight, LinearBatch, LinearStateCache, _fused_mm4, _resid_mm4, linear_attention,
+                     linear_layer_attention, linear_prologue)
 
 __all__ = ["KvCache", "attention", "qkv_prologue", "layer_attention", "hybrid_full_attention",
            "rope_tables", "evict_plan", "ring_map", "validate_snapshot", "OneBitWeight", "fused_mm", "resid_mm",
            "qkv_proj_prologue", "decode_attention_block", "PagedKvCache", "PagedBatch", "paged_qkv_prologue",
-           "paged_attention", "paged_layer_attention", "paged_hybrid_attention"]
-
-
-# A decode step makes two to four of these calls a layer on kernels of 4 to 13 us, so what a call
-# costs on the host is the step's time: pointers and streams go to ctypes as plain integers and the
-# current stream is asked for as one, not through a Stream object (2.9 us). layer_attention 22.7 ->
-# 13.9 us a call (the two C calls alone 7).
-_getDevice = getattr(getattr(torch, "_C", None), "_cuda_getDevice", None)
-_getRawStream = getattr(getattr(torch, "_C", None), "_cuda_getCurrentRawStream", None)
-
-
-def _stream() -> int:
-    """The current device's current stream (hipStream_t as an integer)."""
-    if _getRawStream is None or not torch.cuda.is_initialized():
-        return torch.cuda.current_stream().cuda_stream
-    return _getRawStream(_getDevice())
-
-
-def _ptr(t):
-    if t is None:
-        return None
-    if not t.is_cuda:
-        raise ValueError("bitgpu_amd: expected a device (cuda) tensor")
-    if not t.is_contiguous():
-        raise ValueError("bitgpu_amd: expected a contiguous tensor")
-    return t.data_ptr()
-
-
-def _f32(t, name):
-    if t.dtype is not torch.float32:
-        raise TypeError(f"bitgpu_amd: {name} must be float32, got {t.dtype}")
-    return t
+           "paged_attention", "paged_layer_attention", "paged_hybrid_attention", "FourBitWeight", "LinearStateCache",
+           "LinearBatch", "linear_prologue", "linear_attention", "linear_layer_attention", "linear_block"]
 
 
 def _rows_like(t, S, H, D):
@@ -481,10 +455,13 @@ class OneBitWeight:
         return self.N0 + self.N1 + self.N2
 
 
-def fused_mm(w: OneBitWeight, x, outs):
+def fused_mm(w, x, outs):
     """fusedMM at S = 1 (src/engine.ts:1344-1350, matmul_split_sg.wgsl): rows of W x into up to
-    three outputs by range."""
+    three outputs by range. A :class:`FourBitWeight` takes x [K] or up to 16 rows [rows, K], and outputs
+    [rows, N] alike."""
     _f32(x, "x")
+    if type(w) is not OneBitWeight and isinstance(w, FourBitWeight):
+        return _fused_mm4(w, x, outs)
     o = list(outs) + [None] * (3 - len(outs))
     rc = lib().bg_gemv_split(_ptr(x), w.K, _ptr(w.sign), _ptr(w.scales), w.N0, w.N1, w.N2, _ptr(o[0]), _ptr(o[1]),
                              _ptr(o[2]), _stream())
@@ -492,10 +469,14 @@ def fused_mm(w: OneBitWeight, x, outs):
         check(rc)
 
 
-def resid_mm(w: OneBitWeight, x, resid, out=None):
-    """residMM at S = 1 (src/engine.ts:1364-1369, matmul_resid_mr_sg.wgsl): W x + resid."""
+def resid_mm(w, x, resid, out=None):
+    """residMM at S = 1 (src/engine.ts:1364-1369, matmul_resid_mr_sg.wgsl): W x + resid. A
+    :class:`FourBitWeight` takes x [K] or up to 16 rows [rows, K], resid and out [rows, N] alike (out may be
+    resid)."""
     _f32(x, "x")
     _f32(resid, "resid")
+    if type(w) is not OneBitWeight and isinstance(w, FourBitWeight):
+        return _resid_mm4(w, x, resid, out)
     if out is None:
         out = x.new_empty(w.N)
     rc = lib().bg_gemv_resid(_ptr(x), w.K, _ptr(w.sign), _ptr(w.scales), w.N, _ptr(resid), _ptr(out), _stream())
@@ -675,27 +656,6 @@ class PagedBatch:
         return self._h
 
 
-def _int32(x, name, dims):
-    """x (a sequence, array or host tensor of integers) as a contiguous int32 array."""
-    if isinstance(x, (list, tuple)) and dims == 1:
-        try:  # a list of Python integers, several times faster than through np.asarray
-            return np.frombuffer(array.array("i", x), np.int32) if x else np.zeros(0, np.int32)
-        except (TypeError, OverflowError):
-            pass
-    if torch is not None and isinstance(x, torch.Tensor):
-        x = x.numpy()
-    a = np.asarray(x)
-    if a.size == 0 and a.ndim == 1 and dims == 1:
-        return np.zeros(0, np.int32)
-    if a.ndim != dims or a.dtype.kind not in "iu":
-        raise ValueError(f"bitgpu_amd: {name} must hold integers in {dims} dimension{'s' if dims > 1 else ''}")
-    if a.dtype != np.int32:
-        if a.size and (a.max() > 0x7fffffff or a.min() < -0x80000000):
-            raise ValueError(f"bitgpu_amd: {name} exceeds 32 bits")
-        a = a.astype(np.int32)
-    return np.ascontiguousarray(a)
-
-
 def _int32_rows(lists):
     """Lists of integers as the rows of one int32 array, zeros behind the shorter ones."""
     n, width = len(lists), max(map(len, lists), default=0)
@@ -713,22 +673,6 @@ def _int32_rows(lists):
     for s, t in enumerate(lists):
         rows[s, :len(t)] = _int32(t, "a table", 1)
     return rows
-
-
-def _rows_ptr(t, name, rows, width, device):
-    """Pointer of an f32 tensor of at least `rows` contiguous rows of `width` values (more: a padded batch)
-    on the pool's device; None for None."""
-    if t is None:
-        return None
-    if t.dtype is not torch.float32:
-        raise TypeError(f"bitgpu_amd: {name} must be float32, got {t.dtype}")
-    if t.get_device() != device:
-        raise ValueError(f"bitgpu_amd: expected {name} on cuda:{device}, got {t.device}")
-    if not t.is_contiguous():
-        raise ValueError(f"bitgpu_amd: expected a contiguous tensor ({name})")
-    if t.numel() < rows * width:
-        raise ValueError(f"bitgpu_amd: {name} holds {t.numel()} values, the batch needs {rows} rows of {width}")
-    return t.data_ptr()
 
 
 def _overlap(a, na, b, nb):
@@ -833,3 +777,26 @@ def paged_hybrid_attention(cache: PagedKvCache, li: int, batch: PagedBatch, qg, 
     D = cache.head_dim
     qr = paged_qkv_prologue(cache, li, batch, qg, k, v, q_norm, k_norm, eps, cos_tab, sin_tab, rot_dim, pair_axis, 2 * D)
     return paged_attention(cache, li, batch, qr, gate=qg.view(-1, batch.H, 2 * D)[..., D:], gate_stride=2 * D)
+
+
+# --------------------------------------------------------------------------------------------
+# linear-attention layers (the rest in linear.py)
+# --------------------------------------------------------------------------------------------
+def linear_block(cache: LinearStateCache, li: int, batch: LinearBatch, n1, h, w_in, w_out, conv_weight, a_log, dt_bias, norm,
+                 eps: float):
+    """A linear-attention layer's attention block: in-projection, prologue, attention with its output norm,
+    out-projection and residual. n1: the input-layernormed hidden rows [rows, K] (up to 16 with 4-bit weights,
+    one with 1-bit ones); ``w_in``'s row ranges are channels (q | k | v), v_heads v_dim (z) and 2 v_heads (b | a);
+    h [rows, hidden] the residual. Returns h + w_out att."""
+    Hv, DV = cache.v_heads, cache.v_dim
+    if (w_in.N0, w_in.N1, w_in.N2) != (cache.channels, Hv * DV, 2 * Hv) or w_out.K != Hv * DV:
+        raise ValueError(f"bitgpu_amd: the weights' rows must be {cache.channels} | {Hv * DV} | {2 * Hv} from the hidden state "
+                         f"and the hidden state from {Hv * DV}")
+    M = 1 if n1.dim() == 1 else n1.shape[0]
+    if M != batch.n_tokens:
+        raise ValueError(f"bitgpu_amd: n1 holds {M} rows, the batch has {batch.n_tokens} new rows")
+    new = n1.new_empty
+    qkv, z, ba = new((M, cache.channels)), new((M, Hv, DV)), new((M, 2 * Hv))
+    fused_mm(w_in, n1, [qkv, z, ba])
+    att = linear_layer_attention(cache, li, batch, qkv, ba[:, Hv:], ba[:, :Hv], conv_weight, a_log, dt_bias, z, norm, eps)
+    return resid_mm(w_out, att.view(*n1.shape[:-1], Hv * DV), h)

@@ -405,6 +405,72 @@ int32_t bg_paged_qkv_prologue(const bg_paged_kv* kv, int32_t layer, bg_paged_bat
 int32_t bg_paged_attention(const bg_paged_kv* kv, int32_t layer, bg_paged_batch* batch, const float* q, float scale,
                            const float* gate, int32_t gate_stride, float* out, void* stream);
 
+/* ---- linear attention with a decay for each head ---------------------------------------------------------
+ * The hybrid's other layers (three in four): no keys and values are kept but, per conversation and value head,
+ * one matrix. For a row with key k, query q (of key head h / (v_heads / k_heads)), value v, decay g <= 0 and
+ * write strength beta:
+ *   S <- e^g S + k (beta (v - e^g S^T k))^T     beta NULL: S <- e^g S + k v^T        out = scale S^T q
+ * A cache holds them for n_slots conversations (slots) of n_layers layers, in the caller's device memory (f32,
+ * 16-byte aligned), with the last inputs of the layer's causal convolution:
+ *   state  [layer][slot][v_head][v_dim][k_dim]            (a row: what a value dim has of every key dim)
+ *   conv   [layer][slot][conv_width - 1][channels]        channels = q heads | k heads | v heads, oldest first
+ * Slots need not be cleared. A batch names the sequences of the next calls; its calls are not re-entrant and
+ * follow each other on whatever streams they are made, as the paged batch's do (above), and it may be set again
+ * between replays of a graph that holds its launches, with at most as many new rows as were captured; replays
+ * are the caller's to order with the batch's other calls. Batches of one cache may use different streams where
+ * none reads a slot that another writes. Every call needs the cache's device current. */
+typedef struct bg_linear_cache bg_linear_cache;
+typedef struct bg_linear_batch bg_linear_batch;
+
+/* k_dim, v_dim 64 or 128; v_heads a multiple of k_heads; conv_width 2 to 4, or 0 and conv NULL: no convolution. */
+int32_t bg_linear_create(int32_t n_layers, int32_t k_heads, int32_t v_heads, int32_t k_dim, int32_t v_dim, int32_t conv_width,
+                         int32_t n_slots, float* state, float* conv, bg_linear_cache** out);
+int32_t bg_linear_destroy(bg_linear_cache* cache);
+
+/* A batch of at most max_seqs sequences with max_tokens new rows in all. Allocates (pinned and device). */
+int32_t bg_linear_batch_create(const bg_linear_cache* cache, int32_t max_seqs, int32_t max_tokens, bg_linear_batch** out);
+int32_t bg_linear_batch_destroy(bg_linear_batch* batch);
+/* What the next calls work on (host arrays, read before the call returns): sequence s has rows[s] new rows, goes
+ * on from the state in slot sources[s] (NULL: slots[s]; -1: a new conversation, zeros) and leaves it in slot
+ * slots[s]. Sequences may share a source (a fork); no slot is written by two, or written by one and read by
+ * another (BG_E_INVALID, the batch before stays set). A sequence without new rows touches no slot. Rows are
+ * numbered sequence by sequence. Not under graph capture (BG_E_STATE). */
+int32_t bg_linear_batch_set(bg_linear_batch* batch, int32_t n_seqs, const int32_t* rows, const int32_t* slots,
+                            const int32_t* sources, void* stream);
+
+/* The layer's prologue for a batch: qkv [rows, channels] through the causal depthwise convolution conv_weight
+ * [channels][conv_width] (the last tap on the row itself) and SiLU, then q, k [rows, k_heads, k_dim] each head over
+ * sqrt(its sum of squares + 1e-6), v [rows, v_heads, v_dim] as it is; g = -exp(a_log) softplus(a + dt_bias) and beta =
+ * 1 / (1 + exp(-b)) [rows, v_heads] of a, b (rows ab_stride values apart), a_log, dt_bias [v_heads]; g or beta
+ * may be NULL. The slots' last inputs are read from the sequences' sources and left in their slots. qkv,
+ * conv_weight, q, k, v 16-byte aligned; no output overlaps an input or another. Rows of the outputs beyond the
+ * batch's are left as they are. */
+int32_t bg_linear_prologue(const bg_linear_cache* cache, int32_t layer, bg_linear_batch* batch, const float* qkv,
+                           const float* conv_weight, const float* a, const float* b, int32_t ab_stride, const float* a_log,
+                           const float* dt_bias, float* q, float* k, float* v, float* g, float* beta, void* stream);
+
+/* The recurrence above over every sequence's new rows, its state read and left as the batch says: q, k [rows,
+ * k_heads, k_dim], v, out [rows, v_heads, v_dim], g [rows, v_heads] with rows g_stride values apart (0: [v_heads], one
+ * decay a head), beta [rows, v_heads] or NULL. norm (nullable, [v_dim]): out = o / sqrt(mean o^2 + eps) * norm, and
+ * with gate [rows, v_heads, v_dim] times gate / (1 + exp(-gate)). q, k, v, gate, norm, out 16-byte aligned; out
+ * overlaps no input. Rows of out beyond the batch's are left as they are. A value that is not finite reaches its own
+ * head's later rows and state. */
+int32_t bg_linear_attention(const bg_linear_cache* cache, int32_t layer, bg_linear_batch* batch, const float* q, const float* k,
+                            const float* v, const float* g, int32_t g_stride, const float* beta, float scale, const float* gate,
+                            const float* norm, float eps, float* out, void* stream);
+
+/* ---- 4-bit projections ------------------------------------------------------------------------------------
+ * bg_gemv_split and bg_gemv_resid for 4-bit weights and up to 16 rows x [rows, K]: weight k of row n has the code
+ * c = bits 4 (k % 8) .. + 3 of codes[n][k / 8] (u32) and, with the scale (and min) [n][k / group], the value
+ * (c - 8) * scale, or c * scale + min where mins is not NULL. scale_type (scales and mins): BG_KV_F32 or BG_KV_F16.
+ * K a multiple of 128, group 32, 64 or 128; x, codes, scales and mins 16-byte aligned. Outputs [rows, N0], [rows, N1],
+ * [rows, N2]; resid, y [rows, N], y may be resid; otherwise no output overlaps an input or another. */
+int32_t bg_gemv4_split(const float* x, int32_t rows, int32_t K, const uint32_t* codes, const void* scales, const void* mins,
+                       int32_t scale_type, int32_t group, int32_t N0, int32_t N1, int32_t N2, float* out0, float* out1, float* out2,
+                       void* stream);
+int32_t bg_gemv4_resid(const float* x, int32_t rows, int32_t K, const uint32_t* codes, const void* scales, const void* mins,
+                       int32_t scale_type, int32_t group, int32_t N, const float* resid, float* y, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
