@@ -12,6 +12,16 @@
 namespace bg {
 
 constexpr int kLinChunk = 64;     // rows of a unit
+// Sequences of at least this many new rows are done in chunks of 64, shorter ones row by row.
+constexpr int kLinChunkFrom = 24;
+constexpr size_t kLinSpace = (size_t)256 << 20;  // most bytes of chunk operands at a time
+
+// a row's decay as hi + lo: the rounding of one float would add up over the rows of a constant decay
+__device__ inline void fade_of(float g, float& hi, float& lo) {
+  const double e = exp((double)g);
+  hi = (float)e;
+  lo = hi < __builtin_inff() ? (float)(e - (double)hi) : 0.0f;
+}
 
 // A sequence of the batch: its new rows are rows row0 .. row0 + rows - 1 of the call's tensors; its state is
 // read from slot src (-1: zeros) and left in slot dst.
@@ -27,7 +37,9 @@ struct LinUnit {
 // replays is the one the replay runs.
 struct LinHeader {
   int n_seqs, n_tokens, n_units;
+  int n_chunked, n_chunk_units;   // the first ones
   int pad;
+  char* ws;                       // operands of `window` chunks
 };
 
 // The batch as the kernels see it: device arrays at fixed addresses, written by one upload a set. The counts
@@ -38,6 +50,9 @@ struct LinBatchView {
   const LinUnit* units;
   int n_seqs, n_tokens, n_units;
   int most;                       // rows of the longest sequence
+  int n_chunked, n_chunk_units;
+  int window;                     // chunks that the workspace holds
+  char* ws;                       // NULL under capture: hdr's
 };
 
 // One layer of the caller's state.
@@ -64,7 +79,10 @@ struct LinAttnArgs {
   const float* gate; const float* norm; float eps;
   float* out;
 };
-hipError_t launch_linear_attention(const LinLayer& L, const LinBatchView& b, const LinAttnArgs& a, hipStream_t st);
+hipError_t launch_linear_rows(const LinLayer& L, const LinBatchView& b, const LinAttnArgs& a, hipStream_t st);
+
+hipError_t launch_linear_chunks(const LinLayer& L, const LinBatchView& b, const LinAttnArgs& a, hipStream_t st);
+size_t linear_unit_bytes(int DK, int k_heads, int v_heads);  // a chunk's operands in the workspace
 
 // gemv4.hip: 4-bit projections. Code k of row n is bits 4 (k % 8) .. of codes[n][k / 8]; a weight is
 // (code - 8) * scale, or code * scale + min where mins is given, one scale (and min) per `group` weights.

@@ -44,6 +44,7 @@ struct Plan {
   std::vector<bg::LinSeq> seqs;    // those with new rows, the longest first
   std::vector<bg::LinUnit> units;
   int n_tokens = 0, most = 0;
+  int n_chunked = 0, n_chunk_units = 0;
 };
 
 // whether na f32 values at a and nb at b share memory
@@ -56,6 +57,10 @@ bool overlap(const void* a, size_t na, const void* b, size_t nb) {
 
 struct bg_linear_batch {
   int k_heads, v_heads, DK, DV, n_slots, max_seqs, max_tokens, max_units, device;
+  size_t unit_bytes;                // of a chunk in the workspace
+  int window;                       // chunks of a pass, at most
+  char* ws = nullptr;
+  size_t ws_bytes = 0;
   char* dev = nullptr;              // the device block of all sections
   char* host[kSlots] = {};          // pinned staging, one block a slot
   hipEvent_t done[kSlots] = {};     // recorded behind the slot's upload
@@ -81,6 +86,15 @@ struct bg_linear_batch {
     b.n_seqs = captured ? std::min(max_seqs, plan.n_tokens) : (int)plan.seqs.size();
     b.n_units = captured ? b.n_seqs + plan.n_tokens / bg::kLinChunk : (int)plan.units.size();
     b.most = plan.most;
+    b.window = window;
+    if (captured) {
+      b.n_chunked = std::min(max_seqs, plan.n_tokens / bg::kLinChunkFrom);
+      b.n_chunk_units = b.n_chunked ? b.n_chunked + plan.n_tokens / bg::kLinChunk : 0;
+    } else {
+      b.n_chunked = plan.n_chunked;
+      b.n_chunk_units = plan.n_chunk_units;
+      b.ws = ws;
+    }
     return b;
   }
 };
@@ -136,6 +150,7 @@ void free_batch(bg_linear_batch* b) {
   }
   if (b->moved) (void)hipEventDestroy(b->moved);
   if (b->dev) (void)hipFree(b->dev);
+  if (b->ws) (void)hipFree(b->ws);
   delete b;
 }
 
@@ -144,7 +159,7 @@ int32_t make_plan(bg_linear_batch* b, int32_t n_seqs, const int32_t* rows, const
   Plan& p = b->next;
   p.seqs.clear();
   p.units.clear();
-  p.most = 0;
+  p.most = p.n_chunked = p.n_chunk_units = 0;
   long long T = 0;
   b->writer.assign(b->n_slots, -1);
   for (int s = 0; s < n_seqs; s++) {
@@ -176,6 +191,10 @@ int32_t make_plan(bg_linear_batch* b, int32_t n_seqs, const int32_t* rows, const
     for (int r = 0; r < q.rows; r += bg::kLinChunk)
       p.units.push_back(bg::LinUnit{(int)i, q.row0 + r, std::min(bg::kLinChunk, q.rows - r), r / bg::kLinChunk});
     q.n_units = (int)p.units.size() - q.unit0;
+    if (q.rows >= bg::kLinChunkFrom) {
+      p.n_chunked = (int)i + 1;
+      p.n_chunk_units = (int)p.units.size();
+    }
   }
   p.n_tokens = (int)T;
   return BG_OK;
@@ -250,6 +269,8 @@ int32_t bg_linear_batch_create(const bg_linear_cache* c, int32_t max_seqs, int32
   b->max_tokens = max_tokens;
   b->max_units = std::min(max_seqs, max_tokens) + max_tokens / bg::kLinChunk;
   b->device = dev;
+  b->unit_bytes = bg::linear_unit_bytes(c->DK, c->k_heads, c->v_heads);
+  b->window = (int)std::max<size_t>(1, bg::kLinSpace / b->unit_bytes);
   const size_t bytes[N_SECTIONS] = {sizeof(bg::LinHeader), (size_t)std::min(max_seqs, max_tokens) * sizeof(bg::LinSeq),
                                     (size_t)b->max_units * sizeof(bg::LinUnit)};
   for (int i = 0; i < N_SECTIONS; i++) b->at[i + 1] = b->at[i] + round256(bytes[i]);
@@ -303,8 +324,23 @@ int32_t bg_linear_batch_set(bg_linear_batch* b, int32_t n_seqs, const int32_t* r
     if (e != hipSuccess) return bg::api_hip_fail(e, "linear batch staging");
     b->pending[slot] = false;
   }
+  const size_t need = std::min(p.n_chunk_units, b->window) * b->unit_bytes;
+  char* ws = b->ws;
+  size_t ws_bytes = b->ws_bytes;
+  if (need > ws_bytes) {
+    ws_bytes = std::min(std::max(need, 2 * ws_bytes), b->window * b->unit_bytes);  // at least twofold: few are ever replaced
+    hipError_t e = hipMalloc((void**)&ws, ws_bytes);
+    if (e != hipSuccess && ws_bytes > need) {
+      (void)hipGetLastError();
+      e = hipMalloc((void**)&ws, ws_bytes = need);
+    }
+    if (e != hipSuccess) {
+      (void)hipGetLastError();
+      return bg::api_hip_fail(e, "linear attention workspace allocation");
+    }
+  }
   char* h = b->host[slot];
-  bg::LinHeader hdr{(int)p.seqs.size(), p.n_tokens, (int)p.units.size(), 0};
+  bg::LinHeader hdr{(int)p.seqs.size(), p.n_tokens, (int)p.units.size(), p.n_chunked, p.n_chunk_units, 0, ws};
   bg::PagedUpload up{};
   auto put = [&](int section, const void* src, size_t bytes) {
     if (bytes) memcpy(h + b->at[section], src, bytes);
@@ -317,8 +353,17 @@ int32_t bg_linear_batch_set(bg_linear_batch* b, int32_t n_seqs, const int32_t* r
   put(S_UNITS, p.units.data(), p.units.size() * sizeof(bg::LinUnit));
   hipError_t e = bg::launch_paged_upload(up, st);
   if (e != hipSuccess) {
+    if (ws != b->ws) (void)hipFree(ws);  // no launch knows it; those of before and captured ones keep the old
     b->set = false;
     return bg::api_hip_fail(e, "linear batch upload");
+  }
+  if (ws != b->ws) {
+    std::swap(ws, b->ws);
+    b->ws_bytes = ws_bytes;
+    if (ws) {  // the old one: launches, and replays that began before the new header was there, are done with it
+      (void)hipDeviceSynchronize();
+      (void)hipFree(ws);
+    }
   }
   e = hipEventRecord(b->done[slot], st);
   if (e != hipSuccess) {  // the arrays are another plan's than `plan`, and nothing says when the slot is free
@@ -403,7 +448,11 @@ int32_t bg_linear_attention(const bg_linear_cache* c, int32_t layer, bg_linear_b
     if (moved != BG_OK) return moved;
   }
   const bg::LinAttnArgs args{q, k, v, g, g_stride, beta, scale, gate, norm, eps, out};
-  const hipError_t e = bg::launch_linear_attention(layer_view(c, layer), b->view(captured), args, st);
+  const bg::LinLayer view = layer_view(c, layer);
+  const bg::LinBatchView batch = b->view(captured);
+  hipError_t e = hipSuccess;
+  if (captured || batch.n_seqs > batch.n_chunked) e = bg::launch_linear_rows(view, batch, args, st);
+  if (e == hipSuccess && batch.n_chunk_units) e = bg::launch_linear_chunks(view, batch, args, st);
   if (e != hipSuccess) return bg::api_hip_fail(e, "linear attention launch");
   if (captured) b->cap_tokens = std::min(b->cap_tokens, b->plan.n_tokens);
   return BG_OK;

@@ -1,4 +1,4 @@
-// Linear attention with a decay for each head, one row after the other.
+// Linear attention with a decay for each head, one row after the other (sequences of few new rows).
 //
 //   S <- e^g S + k (beta (v - e^g S^T k))^T   ("sum": S <- e^g S + k v^T),   o = scale S^T q
 // and behind it, where asked for, the layer's output norm o / rms(o) * weight * silu(gate).
@@ -23,16 +23,15 @@ struct RowIn {
 };
 
 template <int DK, int DV, bool DELTA>
-__global__ __launch_bounds__(kThreads) void linear_recurrent_kernel(LinLayer L, LinBatchView b, LinAttnArgs a) {
+__global__ __launch_bounds__(kThreads) void linear_recurrent_kernel(LinLayer L, LinBatchView b, LinAttnArgs a, int first) {
   constexpr int CPL = DV * 8 / kThreads;  // columns of a lane group
   constexpr int NI = DK / 32;
   constexpr int WAVES = kThreads / 64;
   static_assert(CPL >= 1 && NI >= 1, "state split");
   __shared__ float part[2][WAVES];
-  const int s_at = blockIdx.y;
-  if (s_at >= b.hdr->n_seqs) return;
+  const int s_at = first + blockIdx.y;
   const LinSeq s = b.seqs[s_at];
-  if (s.rows <= 0) return;
+  if (s_at >= b.hdr->n_seqs || s.rows >= kLinChunkFrom) return;
   const int h = blockIdx.x, kh = h / (L.v_heads / L.k_heads);
   const int l = threadIdx.x & 7, col = (threadIdx.x >> 3) * CPL, wave = threadIdx.x >> 6;
 
@@ -80,7 +79,9 @@ __global__ __launch_bounds__(kThreads) void linear_recurrent_kernel(LinLayer L, 
       vv[c] = v[c];
       zz[c] = z[c];
     }
-    const float fade = expf(g), strength = beta;
+    float fade, rest;
+    fade_of(g, fade, rest);
+    const float strength = beta;
     if (t + 1 < s.rows) load(t + 1);
     float ks[CPL], qs[CPL], qk = 0.0f;
 #pragma unroll
@@ -108,7 +109,7 @@ __global__ __launch_bounds__(kThreads) void linear_recurrent_kernel(LinLayer L, 
 #pragma unroll
       for (int i = 0; i < NI; i++)
 #pragma unroll
-        for (int e = 0; e < 4; e++) S[c][i][e] = fmaf(x.k[i][e], delta, fade * S[c][i][e]);
+        for (int e = 0; e < 4; e++) S[c][i][e] = fmaf(fade, S[c][i][e], fmaf(rest, S[c][i][e], x.k[i][e] * delta));
     }
     if (a.norm) {
       // the eight lanes of a column hold the same value: sum over the wave's eight groups, then its waves
@@ -143,15 +144,16 @@ __global__ __launch_bounds__(kThreads) void linear_recurrent_kernel(LinLayer L, 
 
 template <int DK, int DV>
 hipError_t launch_t(const LinLayer& L, const LinBatchView& b, const LinAttnArgs& a, hipStream_t st) {
-  const dim3 g(L.v_heads, b.n_seqs);
-  if (a.beta) hipLaunchKernelGGL((linear_recurrent_kernel<DK, DV, true>), g, dim3(kThreads), 0, st, L, b, a);
-  else hipLaunchKernelGGL((linear_recurrent_kernel<DK, DV, false>), g, dim3(kThreads), 0, st, L, b, a);
+  const int first = b.ws || !b.n_chunked ? b.n_chunked : 0;  // (under capture the counts are of the replay)
+  const dim3 g(L.v_heads, b.n_seqs - first);
+  if (a.beta) hipLaunchKernelGGL((linear_recurrent_kernel<DK, DV, true>), g, dim3(kThreads), 0, st, L, b, a, first);
+  else hipLaunchKernelGGL((linear_recurrent_kernel<DK, DV, false>), g, dim3(kThreads), 0, st, L, b, a, first);
   return hipGetLastError();
 }
 
 }  // namespace
 
-hipError_t launch_linear_attention(const LinLayer& L, const LinBatchView& b, const LinAttnArgs& a, hipStream_t st) {
+hipError_t launch_linear_rows(const LinLayer& L, const LinBatchView& b, const LinAttnArgs& a, hipStream_t st) {
   if (L.DK == 64) return L.DV == 64 ? launch_t<64, 64>(L, b, a, st) : launch_t<64, 128>(L, b, a, st);
   return L.DV == 64 ? launch_t<128, 64>(L, b, a, st) : launch_t<128, 128>(L, b, a, st);
 }

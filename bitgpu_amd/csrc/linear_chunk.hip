@@ -1,0 +1,760 @@
+// Linear attention with a decay for each head, 64 rows at a time (prompts).
+//
+// Within a chunk, with G_i the sum of its log decays up to row i and S the state before it:
+//   A_ij = beta_i e^(G_i - G_j) k_i . k_j  (i > j)       T = (I + A)^-1 diag(beta)
+//   V'   = T (V - e^G K S)                               P_ij = e^(G_i - G_j) q_i . k_j  (i >= j)
+//   O    = scale (e^G Q S + P V')                        S  <- e^(G_n) S + K^T (e^(G_n - G) V')
+// ("sum": V' = V). Everything that does not need S is one launch over all chunks (linear_chunk_prepare); the
+// scan (linear_chunk_scan) then walks a sequence's chunks with 32 value dims of a head a workgroup.
+//
+// Precision: products run on the f16 matrix cores with each f32 operand as two f16 parts, x = hi + lo, three
+// products of four (22 bits of the larger operands; what is left out is 2^-22 of a product), summed in f32.
+// Powers of two bring an operand's largest value to 2^14, so values down to 2^-16 of it keep all 22 bits: one
+// for a tile of K, Q, T, P; one for a value dim of S, Y = V - e^G K S and V', whose columns are independent and
+// may be of any size. Those follow from bounds (the column's largest |S| and |V|, K's largest value, T's largest
+// row sum), which may be 2^16 too large before that costs a bit. The decays' sums are taken in f64: their
+// differences over a chunk would lose 2^-24 of the sums. T is found in f32: its diagonal blocks of 16 rows by
+// substitution, the others from them with f32 matrix products.
+//
+// A column whose V or S is not finite, or so large that a bound would overflow, and every column of a chunk
+// whose K, Q, decays or strengths are not finite, is done again row by row: zero times infinity would reach
+// rows before it. Its other columns keep their results (a matrix product's columns do not mix).
+#include <algorithm>
+
+#include "bg_common.h"
+#include "bg_linear.h"
+
+namespace bg {
+
+namespace {
+
+typedef _Float16 half8 __attribute__((ext_vector_type(8)));
+typedef _Float16 half4 __attribute__((ext_vector_type(4)));
+typedef float f4 __attribute__((ext_vector_type(4)));
+
+constexpr int kTop = 14;      // an operand's largest value is below 2^kTop
+constexpr int kCols = 32;     // value dims of a scan workgroup
+constexpr int kPad = 68;      // row stride of 64 x 64 matrices in LDS
+constexpr double kLowest = -1e4;  // of a log decay: e^g is 0 in f32 from -104 on
+
+// What the scan needs of a chunk and head beside its operands. Operands are held times 2^shift.
+struct ChunkMeta {
+  int kshift, qshift[4], tshift[4], pshift[4];
+  float kmax;                  // largest |K|
+  float tsum;                  // largest row sum of |T|
+  float gmax, fmax, whole;     // largest e^G_i and e^(G_n - G_i), e^G_n
+  int bad;                     // something is not finite: row by row
+  int pad[13];
+};
+static_assert(sizeof(ChunkMeta) == 128, "meta");
+
+// Operands of a chunk in the order the matrix instructions take them: [tile of 16 rows][32 of k][hi, lo][lane], a
+// lane's k values being 16 (j / 4) + 4 g + j % 4 of the 32 for j = 0..7 (g = lane / 16), so that a product's
+// result (rows 4 g + r of a tile) is the next one's operand without leaving its lane.
+template <int DK>
+struct ChunkSpace {
+  static constexpr int NKB = DK / 32;
+  static constexpr int K = 0, Q = K + 4 * NKB * 2 * 64, KT = Q + 4 * NKB * 2 * 64, PER_K = KT + (DK / 16) * 2 * 2 * 64;  // in half8
+  static constexpr int T = 0, P = T + 4 * 2 * 2 * 64, G = P + 4 * 2 * 2 * 64, META = G + 128 / 4, PER_H = META + 8;       // in 16 bytes
+};
+
+__device__ inline int top_exponent(float x) { return __builtin_amdgcn_frexp_expf(x); }  // x < 2^e; 0 for 0
+__device__ inline int shift_for(float most) { return kTop - top_exponent(most); }
+__device__ inline uint32_t mag(float x) { return __float_as_uint(x) & 0x7fffffffu; }
+constexpr uint32_t kInf = 0x7f800000u;
+
+__device__ inline void split4(const float (&x)[4], half4& hi, half4& lo) {
+#pragma unroll
+  for (int i = 0; i < 4; i++) hi[i] = (_Float16)x[i];
+#pragma unroll
+  for (int i = 0; i < 4; i++) lo[i] = (_Float16)(x[i] - (float)hi[i]);
+}
+__device__ inline void split8(const float (&x)[8], half8& hi, half8& lo) {
+#pragma unroll
+  for (int i = 0; i < 8; i++) hi[i] = (_Float16)x[i];
+#pragma unroll
+  for (int i = 0; i < 8; i++) lo[i] = (_Float16)(x[i] - (float)hi[i]);
+}
+// c += (ah + al)(bh + bl) less al bl
+__device__ inline f4 product3(half8 ah, half8 al, half8 bh, half8 bl, f4 c) {
+  c = __builtin_amdgcn_mfma_f32_16x16x32_f16(al, bh, c, 0, 0, 0);
+  c = __builtin_amdgcn_mfma_f32_16x16x32_f16(ah, bl, c, 0, 0, 0);
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(ah, bh, c, 0, 0, 0);
+}
+// over the four lane groups that hold a column's rows (or a row's k values)
+__device__ inline uint32_t groups_max(uint32_t v) {
+  auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+  v = max(r[0], r[1]);
+  r = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+  return max(r[0], r[1]);
+}
+__device__ inline float groups_sum(float v) {
+  float2 r = pair16(v);
+  r = pair32(r.x + r.y);
+  return r.x + r.y;
+}
+__device__ inline uint32_t wave_umax(uint32_t v) {
+#pragma unroll
+  for (int m = 1; m < 16; m <<= 1) v = max(v, (uint32_t)__shfl_xor((int)v, m));
+  return groups_max(v);
+}
+
+// One chunk and key head (and its value heads): blockIdx.x a unit from u0 on, blockIdx.y the key head.
+template <int DK, bool DELTA>
+__global__ __launch_bounds__(256) void linear_chunk_prepare(LinLayer L, LinBatchView b, LinAttnArgs a, int u0) {
+  using W = ChunkSpace<DK>;
+  constexpr int NKB = W::NKB;
+  constexpr int kMat = 64 * kPad * 4, kFrag = 4 * NKB * 2 * 64 * 16;
+  __shared__ __align__(16) char mem[2 * kMat > kFrag ? 2 * kMat : kFrag];
+  __shared__ double gsum[64];
+  __shared__ float strength[64];
+  __shared__ uint32_t most[4], bits[4];
+  __shared__ float sums[4];
+  half8* frag = (half8*)mem;                 // K, while products with it run
+  float* Am = (float*)mem;                   // then A
+  float* Tm = (float*)(mem + kMat);          // P, then T
+  const LinUnit u = b.units[u0 + blockIdx.x];
+  if (u0 + (int)blockIdx.x >= b.hdr->n_chunk_units) return;
+  const int kh = blockIdx.y, rep = L.v_heads / L.k_heads;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, m = lane & 15, g = lane >> 4;
+  char* space = b.ws ? b.ws : b.hdr->ws;
+  half8* wk = (half8*)space + (size_t)blockIdx.x * (L.k_heads * W::PER_K + L.v_heads * W::PER_H);
+  half8* wh0 = wk + (size_t)L.k_heads * W::PER_K;
+  wk += (size_t)kh * W::PER_K;
+
+  // this wave's 16 rows of K and Q as operands
+  const int row = 16 * wave + m;
+  const bool live = row < u.n;
+  const size_t at = ((size_t)(u.row0 + (live ? row : 0)) * L.k_heads + kh) * DK + 4 * g;
+  float kx[NKB][8], qx[NKB][8];
+  uint32_t km = 0, qm = 0;
+#pragma unroll
+  for (int kb = 0; kb < NKB; kb++)
+#pragma unroll
+    for (int half = 0; half < 2; half++) {
+      const f4 k = *(const f4*)(a.k + at + 32 * kb + 16 * half), q = *(const f4*)(a.q + at + 32 * kb + 16 * half);
+#pragma unroll
+      for (int e = 0; e < 4; e++) {
+        kx[kb][4 * half + e] = live ? k[e] : 0.0f;
+        qx[kb][4 * half + e] = live ? q[e] : 0.0f;
+        km = max(km, mag(kx[kb][4 * half + e]));
+        qm = max(qm, mag(qx[kb][4 * half + e]));
+      }
+    }
+  km = wave_umax(km);
+  qm = wave_umax(qm);
+  if (lane == 0) {
+    most[wave] = km;
+    bits[wave] = qm;
+  }
+  __syncthreads();
+  const uint32_t kall = max(max(most[0], most[1]), max(most[2], most[3]));
+  const uint32_t qall = max(max(bits[0], bits[1]), max(bits[2], bits[3]));
+  const bool bad_k = kall >= kInf || qall >= kInf;
+  const float kmax = __uint_as_float(kall);
+  const int ks = shift_for(kmax), qs = shift_for(__uint_as_float(qm));
+  half8 qh[NKB], ql[NKB], kh8[NKB], kl8[NKB];
+#pragma unroll
+  for (int kb = 0; kb < NKB; kb++) {
+#pragma unroll
+    for (int e = 0; e < 8; e++) {
+      kx[kb][e] = ldexpf(kx[kb][e], ks);
+      qx[kb][e] = ldexpf(qx[kb][e], qs);
+    }
+    split8(kx[kb], kh8[kb], kl8[kb]);
+    split8(qx[kb], qh[kb], ql[kb]);
+    const int i = (wave * NKB + kb) * 2 * 64 + lane;
+    frag[i] = kh8[kb];
+    frag[i + 64] = kl8[kb];
+    if constexpr (DELTA) {
+      wk[W::K + i] = kh8[kb];
+      wk[W::K + i + 64] = kl8[kb];
+    }
+    wk[W::Q + i] = qh[kb];
+    wk[W::Q + i + 64] = ql[kb];
+  }
+  __syncthreads();
+  // K^T: this wave's tiles of 16 key dims
+  {
+    const _Float16* e = (const _Float16*)frag;
+#pragma unroll
+    for (int i = 0; i < DK / 64; i++) {
+      const int td = wave * (DK / 64) + i;
+#pragma unroll
+      for (int kb2 = 0; kb2 < 2; kb2++)
+#pragma unroll
+        for (int hl = 0; hl < 2; hl++) {
+          half8 x;
+#pragma unroll
+          for (int j = 0; j < 8; j++) {
+            const int tile = 2 * kb2 + (j >> 2), from = 4 * g + (j & 3) + 16 * (m >> 2);
+            x[j] = e[(((tile * NKB + (td >> 1)) * 2 + hl) * 64 + from) * 8 + 4 * (td & 1) + (m & 3)];
+          }
+          wk[W::KT + ((td * 2 + kb2) * 2 + hl) * 64 + lane] = x;
+        }
+    }
+  }
+  // row tile `wave` of K K^T and Q K^T
+  f4 kk[4], qk[4];
+#pragma unroll
+  for (int ct = 0; ct < 4; ct++) {
+    kk[ct] = qk[ct] = f4{0, 0, 0, 0};
+    if (ct > wave) continue;
+#pragma unroll
+    for (int kb = 0; kb < NKB; kb++) {
+      const half8 bh = frag[((ct * NKB + kb) * 2 + 0) * 64 + lane], bl = frag[((ct * NKB + kb) * 2 + 1) * 64 + lane];
+      if constexpr (DELTA) kk[ct] = product3(kh8[kb], kl8[kb], bh, bl, kk[ct]);
+      qk[ct] = product3(qh[kb], ql[kb], bh, bl, qk[ct]);
+    }
+#pragma unroll
+    for (int r = 0; r < 4; r++) {
+      kk[ct][r] = ldexpf(kk[ct][r], -2 * ks);
+      qk[ct][r] = ldexpf(qk[ct][r], -ks - qs);
+    }
+  }
+
+  for (int i = 0; i < rep; i++) {
+    const int h = kh * rep + i;
+    half8* wh = wh0 + (size_t)h * W::PER_H;
+    __syncthreads();  // the frag reads, or the head before
+    float gmax = 1.0f, fmax_ = 1.0f, whole = 1.0f;
+    bool bad = bad_k;
+    if (wave == 0) {  // the decays' sums: lane = row
+      const bool on = lane < u.n;
+      const size_t rr = u.row0 + (on ? lane : 0);
+      const float gv = on ? a.g[(a.g_stride ? rr * a.g_stride : 0) + h] : 0.0f;
+      double s = gv < (float)kLowest ? kLowest : (double)gv;
+#pragma unroll
+      for (int d = 1; d < 64; d <<= 1) {
+        const double o = __shfl_up(s, d);
+        if (lane >= d) s += o;
+      }
+      const double end = __shfl(s, 63);
+      const float be = DELTA ? (on ? a.beta[rr * L.v_heads + h] : 0.0f) : 1.0f;
+      gsum[lane] = s;
+      strength[lane] = be;
+      const float eg = expf((float)s), fg = expf((float)(end - s));
+      ((float*)(wh + W::G))[lane] = eg;
+      ((float*)(wh + W::G))[64 + lane] = on ? fg : 0.0f;
+      gmax = __uint_as_float(wave_umax(mag(eg)));
+      fmax_ = __uint_as_float(wave_umax(mag(fg)));
+      whole = expf((float)end);
+      bad = bad || __any(mag(eg) >= kInf || mag(fg) >= kInf || mag(be) >= kInf);
+    }
+    __syncthreads();
+    // A and P of this wave's rows
+    uint32_t pm = 0;
+#pragma unroll
+    for (int ct = 0; ct < 4; ct++) {
+      if (ct > wave) continue;
+      const int c = 16 * ct + m;
+      const double gc = gsum[c];
+#pragma unroll
+      for (int r = 0; r < 4; r++) {
+        const int w = 16 * wave + 4 * g + r;
+        const float fade = c <= w ? expf((float)(gsum[w] - gc)) : 0.0f;
+        const float p = c <= w ? fade * qk[ct][r] : 0.0f;
+        Tm[w * kPad + c] = p;
+        pm = max(pm, mag(p));
+        if constexpr (DELTA) Am[w * kPad + c] = c < w ? strength[w] * (fade * kk[ct][r]) : 0.0f;
+      }
+    }
+    pm = wave_umax(pm);
+    const int ps = shift_for(__uint_as_float(pm));
+    if (lane == 0) bits[wave] = pm;
+    // P's operands: rows written by this wave itself
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    auto operand = [&](const float* M, int kb, bool strong, float& sum, uint32_t& big, float (&x)[8]) {
+#pragma unroll
+      for (int half = 0; half < 2; half++) {
+        const int ct = 2 * kb + half;
+        f4 v = f4{0, 0, 0, 0};
+        if (ct <= wave) v = *(const f4*)(M + row * kPad + 16 * ct + 4 * g);
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+          const float y = ct <= wave && strong ? v[e] * strength[16 * ct + 4 * g + e] : v[e];
+          x[4 * half + e] = y;
+          sum += fabsf(y);
+          big = max(big, mag(y));
+        }
+      }
+    };
+    auto put = [&](int base, int kb, int shift, float (&x)[8]) {
+      half8 hi, lo;
+#pragma unroll
+      for (int e = 0; e < 8; e++) x[e] = ldexpf(x[e], shift);
+      split8(x, hi, lo);
+      wh[base + ((wave * 2 + kb) * 2 + 0) * 64 + lane] = hi;
+      wh[base + ((wave * 2 + kb) * 2 + 1) * 64 + lane] = lo;
+    };
+#pragma unroll
+    for (int kb = 0; kb < 2; kb++) {
+      float x[8], none = 0;
+      uint32_t nil = 0;
+      if (2 * kb > wave) continue;
+      operand(Tm, kb, false, none, nil, x);
+      put(W::P, kb, ps, x);
+    }
+    int ts = 0;
+    float tsum = 1.0f;
+    if constexpr (DELTA) {
+      __syncthreads();  // P is read; A is there
+      {  // the diagonal block of this wave, a column a lane (four lanes alike)
+        float x[16];
+#pragma unroll
+        for (int r = 0; r < 16; r++) {
+          float y = r == m ? 1.0f : 0.0f;
+#pragma unroll
+          for (int j = 0; j < r; j++) y = fmaf(-Am[(16 * wave + r) * kPad + 16 * wave + j], x[j], y);
+          x[r] = y;
+        }
+#pragma unroll
+        for (int r = 0; r < 16; r++)
+          if ((r >> 2) == g) Tm[(16 * wave + r) * kPad + 16 * wave + m] = x[r];
+      }
+      __syncthreads();
+      {  // the blocks below it: column block `wave`
+        f4 t[4];
+#pragma unroll
+        for (int r = 0; r < 4; r++) t[0][r] = Tm[(16 * wave + 4 * g + r) * kPad + 16 * wave + m];
+#pragma unroll
+        for (int d = 1; d < 4; d++) {
+          const int I = wave + d;
+          if (I > 3) break;
+          f4 acc = f4{0, 0, 0, 0};
+#pragma unroll
+          for (int k = 0; k < d; k++) {
+            const f4 x = *(const f4*)(Am + (16 * I + m) * kPad + 16 * (wave + k) + 4 * g);
+#pragma unroll
+            for (int r = 0; r < 4; r++) acc = __builtin_amdgcn_mfma_f32_16x16x4f32(x[r], t[k][r], acc, 0, 0, 0);
+          }
+          const f4 x = *(const f4*)(Tm + (16 * I + m) * kPad + 16 * I + 4 * g);
+          t[d] = f4{0, 0, 0, 0};
+#pragma unroll
+          for (int r = 0; r < 4; r++) t[d] = __builtin_amdgcn_mfma_f32_16x16x4f32(x[r], -acc[r], t[d], 0, 0, 0);
+#pragma unroll
+          for (int r = 0; r < 4; r++) Tm[(16 * I + 4 * g + r) * kPad + 16 * wave + m] = t[d][r];
+        }
+      }
+      __syncthreads();
+      float x[2][8], sum = 0.0f;
+      uint32_t big = 0;
+#pragma unroll
+      for (int kb = 0; kb < 2; kb++)
+        if (2 * kb <= wave) operand(Tm, kb, true, sum, big, x[kb]);
+      big = wave_umax(big);
+      ts = shift_for(__uint_as_float(big));
+#pragma unroll
+      for (int kb = 0; kb < 2; kb++)
+        if (2 * kb <= wave) put(W::T, kb, ts, x[kb]);
+      sum = __uint_as_float(wave_umax(mag(groups_sum(sum))));  // (a NaN counts as the largest)
+      if (lane == 0) sums[wave] = sum;
+      __syncthreads();
+      tsum = fmaxf(fmaxf(sums[0], sums[1]), fmaxf(sums[2], sums[3]));
+      for (int w = 0; w < 4; w++) bad = bad || !(sums[w] < 0x1p60f);
+    } else {
+      __syncthreads();
+    }
+    for (int w = 0; w < 4; w++) bad = bad || !(__uint_as_float(bits[w]) < 0x1p60f);
+    ChunkMeta* meta = (ChunkMeta*)(wh + W::META);
+    if (lane == 0) {
+      meta->qshift[wave] = qs;
+      meta->tshift[wave] = ts;
+      meta->pshift[wave] = ps;
+      if (wave == 0) {
+        meta->kshift = ks;
+        meta->kmax = kmax;
+        meta->tsum = tsum;
+        meta->gmax = gmax;
+        meta->fmax = fmax_;
+        meta->whole = whole;
+        meta->bad = bad;
+      }
+    }
+  }
+}
+
+// A chunk's operands of one wave: its 16 rows of K, Q, T, P, its key dims of K^T, and its rows of V.
+template <int DK>
+struct Fragments {
+  half8 k[DK / 32][2], q[DK / 32][2], t[2][2], p[2][2], kt[DK / 64][2][2];
+  float v[2][4], eg[4], fg[4];
+};
+
+// A sequence's chunks from u0 up to u1 (its window of the workspace) for 32 value dims of a head.
+template <int DK, int DV, bool DELTA>
+__global__ __launch_bounds__(256, 2) void linear_chunk_scan(LinLayer L, LinBatchView b, LinAttnArgs a, int u0, int u1) {
+  using W = ChunkSpace<DK>;
+  constexpr int NKB = W::NKB, MT = DK / 64, SLICES = DV / kCols;
+  __shared__ half8 Sb[NKB * 2 * 2 * 64];        // the state as an operand
+  __shared__ half8 Yb[2 * 2 * 2 * 64], Vb[2 * 2 * 2 * 64], Fb[2 * 2 * 2 * 64];  // Y, V', e^(G_n - G) V'
+  __shared__ uint32_t smax[4][kCols], vmax[4][kCols];
+  __shared__ float plain[kCols][DK + 4];        // the state of columns that are done row by row
+  // a key head's value heads and slices, which read the same operands, run on one XCD
+  const int rep = L.v_heads / L.k_heads, members = rep * SLICES;
+  const int x = blockIdx.x & 7, j = blockIdx.x >> 3;
+  const int group = x + 8 * (j / members), member = j % members;
+  const int seq = group / L.k_heads, kh = group % L.k_heads;
+  if (seq >= b.hdr->n_chunked) return;
+  const LinSeq s = b.seqs[seq];
+  const int first = max(s.unit0, u0), last = min(s.unit0 + s.n_units, u1);
+  if (first >= last) return;
+  const int h = kh * rep + member / SLICES, col0 = (member % SLICES) * kCols;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
+  const char* space = b.ws ? b.ws : b.hdr->ws;
+  const size_t per_unit = (size_t)L.k_heads * W::PER_K + (size_t)L.v_heads * W::PER_H;
+  const half8* wk0 = (const half8*)space + (size_t)kh * W::PER_K;
+  const half8* wh0 = (const half8*)space + (size_t)L.k_heads * W::PER_K + (size_t)h * W::PER_H;
+
+  f4 S[MT][2];
+  const int from = first == s.unit0 ? s.src : s.dst;
+#pragma unroll
+  for (int i = 0; i < MT; i++)
+#pragma unroll
+    for (int nt = 0; nt < 2; nt++)
+      S[i][nt] = from >= 0 ? *(const f4*)(L.state + (((size_t)from * L.v_heads + h) * DV + col0 + 16 * nt + n) * DK + 16 * (wave * MT + i) + 4 * g)
+                           : f4{0, 0, 0, 0};
+
+  Fragments<DK> F;
+  auto load_kq = [&](int u) {
+    const half8* wk = wk0 + (size_t)(u - u0) * per_unit;
+#pragma unroll
+    for (int kb = 0; kb < NKB; kb++)
+#pragma unroll
+      for (int hl = 0; hl < 2; hl++) {
+        if constexpr (DELTA) F.k[kb][hl] = wk[W::K + ((wave * NKB + kb) * 2 + hl) * 64 + lane];
+        F.q[kb][hl] = wk[W::Q + ((wave * NKB + kb) * 2 + hl) * 64 + lane];
+      }
+  };
+  auto load_t = [&](int u) {
+    const half8* wh = wh0 + (size_t)(u - u0) * per_unit;
+    if constexpr (DELTA)
+#pragma unroll
+      for (int kb = 0; kb < 2; kb++)
+#pragma unroll
+        for (int hl = 0; hl < 2; hl++)
+          if (2 * kb <= wave) F.t[kb][hl] = wh[W::T + ((wave * 2 + kb) * 2 + hl) * 64 + lane];
+  };
+  auto load_p = [&](int u) {
+    const half8* wh = wh0 + (size_t)(u - u0) * per_unit;
+#pragma unroll
+    for (int kb = 0; kb < 2; kb++)
+#pragma unroll
+      for (int hl = 0; hl < 2; hl++)
+        if (2 * kb <= wave) F.p[kb][hl] = wh[W::P + ((wave * 2 + kb) * 2 + hl) * 64 + lane];
+  };
+  auto load_kt = [&](int u) {
+    const half8* wk = wk0 + (size_t)(u - u0) * per_unit;
+#pragma unroll
+    for (int i = 0; i < MT; i++)
+#pragma unroll
+      for (int kb = 0; kb < 2; kb++)
+#pragma unroll
+        for (int hl = 0; hl < 2; hl++) F.kt[i][kb][hl] = wk[W::KT + (((wave * MT + i) * 2 + kb) * 2 + hl) * 64 + lane];
+  };
+  auto load_v = [&](int u) {
+    const LinUnit w = b.units[u];
+#pragma unroll
+    for (int r = 0; r < 4; r++) {
+      const int row = 16 * wave + 4 * g + r;
+      const size_t at = ((size_t)(w.row0 + (row < w.n ? row : 0)) * L.v_heads + h) * DV + col0 + n;
+#pragma unroll
+      for (int nt = 0; nt < 2; nt++) F.v[nt][r] = row < w.n ? a.v[at + 16 * nt] : 0.0f;
+    }
+    const float* gg = (const float*)(wh0 + (size_t)(u - u0) * per_unit + W::G) + 16 * wave + 4 * g;
+#pragma unroll
+    for (int r = 0; r < 4; r++) {
+      F.eg[r] = gg[r];
+      F.fg[r] = gg[64 + r];
+    }
+  };
+  load_kq(first);
+  load_t(first);
+  load_p(first);
+  load_kt(first);
+  load_v(first);
+
+  auto note_state = [&]() {  // the largest |S| of each column over this wave's key dims
+#pragma unroll
+    for (int nt = 0; nt < 2; nt++) {
+      uint32_t t = 0;
+#pragma unroll
+      for (int i = 0; i < MT; i++)
+#pragma unroll
+        for (int r = 0; r < 4; r++) t = max(t, mag(S[i][nt][r]));
+      t = groups_max(t);
+      if (g == 0) smax[wave][16 * nt + n] = t;
+    }
+  };
+  auto note_v = [&]() {
+#pragma unroll
+    for (int nt = 0; nt < 2; nt++) {
+      uint32_t t = 0;
+#pragma unroll
+      for (int r = 0; r < 4; r++) t = max(t, mag(F.v[nt][r]));
+      t = groups_max(t);
+      if (g == 0) vmax[wave][16 * nt + n] = t;
+    }
+  };
+  auto put4 = [&](half8* to, int tile, int nt, const float (&x)[4], int shift) {
+    float y[4];
+    half4 hi, lo;
+#pragma unroll
+    for (int r = 0; r < 4; r++) y[r] = ldexpf(x[r], shift);
+    split4(y, hi, lo);
+    char* p = (char*)(to + (((tile >> 1) * 2 + nt) * 2) * 64 + lane) + 8 * (tile & 1);
+    *(half4*)p = hi;
+    *(half4*)(p + 64 * 16) = lo;
+  };
+  int sshift[2];
+  auto put_state = [&]() {
+#pragma unroll
+    for (int i = 0; i < MT; i++)
+#pragma unroll
+      for (int nt = 0; nt < 2; nt++) {
+        const float y[4] = {S[i][nt][0], S[i][nt][1], S[i][nt][2], S[i][nt][3]};
+        put4(Sb, wave * MT + i, nt, y, sshift[nt]);
+      }
+  };
+  note_state();
+  note_v();
+  __syncthreads();
+#pragma unroll
+  for (int nt = 0; nt < 2; nt++) {
+    const int c = 16 * nt + n;
+    sshift[nt] = shift_for(__uint_as_float(max(max(smax[0][c], smax[1][c]), max(smax[2][c], smax[3][c]))));
+  }
+  put_state();
+
+  for (int u = first; u < last; u++) {
+    const LinUnit w = b.units[u];
+    const ChunkMeta* meta = (const ChunkMeta*)(wh0 + (size_t)(u - u0) * per_unit + W::META);
+    const int kshift = meta->kshift, qshift = meta->qshift[wave], tshift = meta->tshift[wave], pshift = meta->pshift[wave];
+    const float whole = meta->whole;
+    const int next = min(u + 1, last - 1);
+    __syncthreads();  // the state, and what is noted of it and of V
+    int yshift[2], vshift[2], fshift[2], sshift_next[2];
+    bool odd = meta->bad;
+    uint32_t todo = 0;  // columns for the row-by-row pass
+#pragma unroll
+    for (int nt = 0; nt < 2; nt++) {
+      const int c = 16 * nt + n;
+      const float sm = __uint_as_float(max(max(smax[0][c], smax[1][c]), max(smax[2][c], smax[3][c])));
+      const float vm = __uint_as_float(max(max(vmax[0][c], vmax[1][c]), max(vmax[2][c], vmax[3][c])));
+      const float ym = vm + (DELTA ? meta->gmax * (DK * meta->kmax) * sm : 0.0f);
+      const float vpm = meta->tsum * ym, fm = meta->fmax * vpm;
+      const float next_m = whole * sm + kLinChunk * meta->kmax * fm;
+      yshift[nt] = shift_for(ym);
+      vshift[nt] = shift_for(vpm);
+      fshift[nt] = shift_for(fm);
+      sshift_next[nt] = shift_for(next_m);
+      const bool out = odd || !(next_m < 0x1p120f) || !(ym < 0x1p120f) || !(vpm < 0x1p120f) || !(sm < 0x1p120f);
+      todo |= (uint32_t)(__ballot(out) & 0xffffu) << (16 * nt);
+    }
+    todo = __builtin_amdgcn_readfirstlane(todo);
+    if (todo) {
+#pragma unroll
+      for (int i = 0; i < MT; i++)
+#pragma unroll
+        for (int nt = 0; nt < 2; nt++) *(f4*)&plain[16 * nt + n][16 * (wave * MT + i) + 4 * g] = S[i][nt];
+    }
+
+    // K S and Q S
+    f4 ks[2], o[2];
+#pragma unroll
+    for (int nt = 0; nt < 2; nt++) ks[nt] = o[nt] = f4{0, 0, 0, 0};
+#pragma unroll
+    for (int kb = 0; kb < NKB; kb++)
+#pragma unroll
+      for (int nt = 0; nt < 2; nt++) {
+        const half8 sh = Sb[((kb * 2 + nt) * 2 + 0) * 64 + lane], sl = Sb[((kb * 2 + nt) * 2 + 1) * 64 + lane];
+        if constexpr (DELTA) ks[nt] = product3(F.k[kb][0], F.k[kb][1], sh, sl, ks[nt]);
+        o[nt] = product3(F.q[kb][0], F.q[kb][1], sh, sl, o[nt]);
+      }
+    load_kq(next);
+#pragma unroll
+    for (int nt = 0; nt < 2; nt++)
+#pragma unroll
+      for (int r = 0; r < 4; r++) o[nt][r] = F.eg[r] * ldexpf(o[nt][r], -qshift - sshift[nt]);
+    f4 vp[2];
+    if constexpr (DELTA) {
+#pragma unroll
+      for (int nt = 0; nt < 2; nt++) {
+        float y[4];
+#pragma unroll
+        for (int r = 0; r < 4; r++) y[r] = F.v[nt][r] - F.eg[r] * ldexpf(ks[nt][r], -kshift - sshift[nt]);
+        put4(Yb, wave, nt, y, yshift[nt]);
+      }
+      __syncthreads();
+#pragma unroll
+      for (int nt = 0; nt < 2; nt++) {
+        vp[nt] = f4{0, 0, 0, 0};
+#pragma unroll
+        for (int kb = 0; kb < 2; kb++)
+          if (2 * kb <= wave)
+            vp[nt] = product3(F.t[kb][0], F.t[kb][1], Yb[((kb * 2 + nt) * 2 + 0) * 64 + lane], Yb[((kb * 2 + nt) * 2 + 1) * 64 + lane], vp[nt]);
+#pragma unroll
+        for (int r = 0; r < 4; r++) vp[nt][r] = ldexpf(vp[nt][r], -tshift - yshift[nt]);
+      }
+      load_t(next);
+    } else {
+#pragma unroll
+      for (int nt = 0; nt < 2; nt++)
+#pragma unroll
+        for (int r = 0; r < 4; r++) vp[nt][r] = F.v[nt][r];
+    }
+#pragma unroll
+    for (int nt = 0; nt < 2; nt++) {
+      const float y[4] = {vp[nt][0], vp[nt][1], vp[nt][2], vp[nt][3]};
+      const float z[4] = {F.fg[0] * y[0], F.fg[1] * y[1], F.fg[2] * y[2], F.fg[3] * y[3]};
+      put4(Vb, wave, nt, y, vshift[nt]);
+      put4(Fb, wave, nt, z, fshift[nt]);
+    }
+    load_v(next);
+    __syncthreads();
+    // the state
+#pragma unroll
+    for (int i = 0; i < MT; i++)
+#pragma unroll
+      for (int nt = 0; nt < 2; nt++) {
+        f4 acc = f4{0, 0, 0, 0};
+#pragma unroll
+        for (int kb = 0; kb < 2; kb++)
+          acc = product3(F.kt[i][kb][0], F.kt[i][kb][1], Fb[((kb * 2 + nt) * 2 + 0) * 64 + lane], Fb[((kb * 2 + nt) * 2 + 1) * 64 + lane], acc);
+#pragma unroll
+        for (int r = 0; r < 4; r++) S[i][nt][r] = fmaf(whole, S[i][nt][r], ldexpf(acc[r], -kshift - fshift[nt]));
+      }
+    load_kt(next);
+    // the output
+#pragma unroll
+    for (int nt = 0; nt < 2; nt++) {
+      f4 acc = f4{0, 0, 0, 0};
+#pragma unroll
+      for (int kb = 0; kb < 2; kb++)
+        if (2 * kb <= wave)
+          acc = product3(F.p[kb][0], F.p[kb][1], Vb[((kb * 2 + nt) * 2 + 0) * 64 + lane], Vb[((kb * 2 + nt) * 2 + 1) * 64 + lane], acc);
+#pragma unroll
+      for (int r = 0; r < 4; r++) {
+        const int row = 16 * wave + 4 * g + r;
+        const float y = a.scale * (o[nt][r] + ldexpf(acc[r], -pshift - vshift[nt]));
+        if (row < w.n && !(todo >> (16 * nt + n) & 1)) a.out[((size_t)(w.row0 + row) * L.v_heads + h) * DV + col0 + 16 * nt + n] = y;
+      }
+    }
+    load_p(next);
+    if (todo) {  // eight lanes a column, as linear_attn.hip's
+      __syncthreads();
+      const int c = threadIdx.x >> 3, l = threadIdx.x & 7;
+      float* sp = &plain[c][4 * l];
+      f4 st[DK / 32];
+#pragma unroll
+      for (int i = 0; i < DK / 32; i++) st[i] = *(const f4*)(sp + 32 * i);
+#pragma unroll 1
+      for (int t = 0; t < w.n; t++) {
+        const size_t r = w.row0 + t;
+        const float* kp = a.k + (r * L.k_heads + kh) * DK + 4 * l;
+        const float* qp = a.q + (r * L.k_heads + kh) * DK + 4 * l;
+        float hi, lo;
+        fade_of(a.g[(a.g_stride ? r * a.g_stride : 0) + h], hi, lo);
+        float sum = 0.0f;
+        f4 kx[DK / 32];
+#pragma unroll
+        for (int i = 0; i < DK / 32; i++) {
+          kx[i] = *(const f4*)(kp + 32 * i);
+#pragma unroll
+          for (int e = 0; e < 4; e++) sum = fmaf(st[i][e], kx[i][e], sum);
+        }
+        float d = a.v[(r * L.v_heads + h) * DV + col0 + c];
+        if constexpr (DELTA) d = a.beta[r * L.v_heads + h] * (d - hi * group_sum<8>(sum));
+        sum = 0.0f;
+#pragma unroll
+        for (int i = 0; i < DK / 32; i++) {
+          const f4 q = *(const f4*)(qp + 32 * i);
+#pragma unroll
+          for (int e = 0; e < 4; e++) {
+            st[i][e] = fmaf(hi, st[i][e], fmaf(lo, st[i][e], kx[i][e] * d));
+            sum = fmaf(st[i][e], q[e], sum);
+          }
+        }
+        sum = group_sum<8>(sum);
+        if (l == 0 && (todo >> c & 1)) a.out[(r * L.v_heads + h) * DV + col0 + c] = a.scale * sum;
+      }
+#pragma unroll
+      for (int i = 0; i < DK / 32; i++) *(f4*)(sp + 32 * i) = st[i];
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < MT; i++)
+#pragma unroll
+        for (int nt = 0; nt < 2; nt++)
+          if (todo >> (16 * nt + n) & 1) S[i][nt] = *(const f4*)&plain[16 * nt + n][16 * (wave * MT + i) + 4 * g];
+    }
+    note_state();
+    note_v();
+#pragma unroll
+    for (int nt = 0; nt < 2; nt++) sshift[nt] = sshift_next[nt];
+    put_state();
+  }
+#pragma unroll
+  for (int i = 0; i < MT; i++)
+#pragma unroll
+    for (int nt = 0; nt < 2; nt++)
+      *(f4*)(L.state + (((size_t)s.dst * L.v_heads + h) * DV + col0 + 16 * nt + n) * DK + 16 * (wave * MT + i) + 4 * g) = S[i][nt];
+}
+
+// The output norm of the chunks' rows, in place: DV / 4 lanes a row and head.
+template <int DV>
+__global__ __launch_bounds__(256) void linear_norm_kernel(LinLayer L, LinBatchView b, LinAttnArgs a) {
+  constexpr int LG = DV / 4;
+  const LinUnit u = b.units[blockIdx.x];
+  if ((int)blockIdx.x >= b.hdr->n_chunk_units) return;
+  const int grp = threadIdx.x / LG, c = 4 * (threadIdx.x % LG);
+  const f4 w = *(const f4*)(a.norm + c);
+  for (int i = blockIdx.y * (256 / LG) + grp; i < u.n * L.v_heads; i += gridDim.y * (256 / LG)) {
+    const size_t at = ((size_t)u.row0 * L.v_heads + i) * DV + c;
+    f4 o = *(const f4*)(a.out + at);
+    const float inv = 1.0f / sqrtf(group_sum<LG>(fmaf(o[0], o[0], fmaf(o[1], o[1], fmaf(o[2], o[2], o[3] * o[3])))) / DV + a.eps);
+#pragma unroll
+    for (int e = 0; e < 4; e++) o[e] = o[e] * inv * w[e];
+    if (a.gate) {
+      const f4 z = *(const f4*)(a.gate + at);
+#pragma unroll
+      for (int e = 0; e < 4; e++) o[e] *= z[e] / (1.0f + expf(-z[e]));
+    }
+    *(f4*)(a.out + at) = o;
+  }
+}
+
+template <int DK, int DV, bool DELTA>
+hipError_t launch_t(const LinLayer& L, const LinBatchView& b, const LinAttnArgs& a, hipStream_t st) {
+  const int groups = b.n_chunked * L.k_heads, members = L.v_heads / L.k_heads * (DV / kCols);
+  for (int u0 = 0; u0 < b.n_chunk_units; u0 += b.window) {
+    const int u1 = std::min(u0 + b.window, b.n_chunk_units);
+    hipLaunchKernelGGL((linear_chunk_prepare<DK, DELTA>), dim3(u1 - u0, L.k_heads), dim3(256), 0, st, L, b, a, u0);
+    hipLaunchKernelGGL((linear_chunk_scan<DK, DV, DELTA>), dim3(8 * ((groups + 7) / 8) * members), dim3(256), 0, st, L, b, a, u0, u1);
+  }
+  if (a.norm) hipLaunchKernelGGL((linear_norm_kernel<DV>), dim3(b.n_chunk_units, std::min(8, L.v_heads)), dim3(256), 0, st, L, b, a);
+  return hipGetLastError();
+}
+
+template <int DK>
+size_t unit_bytes(int k_heads, int v_heads) {
+  return 16 * ((size_t)k_heads * ChunkSpace<DK>::PER_K + (size_t)v_heads * ChunkSpace<DK>::PER_H);
+}
+
+}  // namespace
+
+size_t linear_unit_bytes(int DK, int k_heads, int v_heads) {
+  return DK == 64 ? unit_bytes<64>(k_heads, v_heads) : unit_bytes<128>(k_heads, v_heads);
+}
+
+hipError_t launch_linear_chunks(const LinLayer& L, const LinBatchView& b, const LinAttnArgs& a, hipStream_t st) {
+  if (a.beta) {
+    if (L.DK == 64) return L.DV == 64 ? launch_t<64, 64, true>(L, b, a, st) : launch_t<64, 128, true>(L, b, a, st);
+    return L.DV == 64 ? launch_t<128, 64, true>(L, b, a, st) : launch_t<128, 128, true>(L, b, a, st);
+  }
+  if (L.DK == 64) return L.DV == 64 ? launch_t<64, 64, false>(L, b, a, st) : launch_t<64, 128, false>(L, b, a, st);
+  return L.DV == 64 ? launch_t<128, 64, false>(L, b, a, st) : launch_t<128, 128, false>(L, b, a, st);
+}
+
+}  // namespace bg

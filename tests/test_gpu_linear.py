@@ -124,15 +124,19 @@ def test_sizes_of_values(dev, rows, size):
 
 @pytest.mark.parametrize("rows", [[5, 4], [120, 70]])
 def test_values_that_are_not_finite(dev, rows):
-    """A NaN or an infinity reaches its own head's columns of later rows, and nothing else."""
+    """A NaN or an infinity reaches its own head's column of later rows, and nothing else: other columns keep their
+    bits, the column's earlier rows (a prompt does such a column row by row) stay within the bound."""
     for rule in ("delta", "sum"):
         c = Case(rows, rule=rule, seed=2)
         clean_out, clean_state = c.run()
+        want, bound = c.reference()[:2]
         c.v[2, 1, 7], c.v[3, 2, 5] = np.nan, np.inf
         out, state = c.run()
         hit = np.zeros(out.shape, bool)
         hit[2:rows[0], 1, 7] = hit[3:rows[0], 2, 5] = True
         assert not np.isfinite(out[hit]).any()
+        assert np.all(np.abs(out - want)[~hit] <= bound[~hit])
+        hit[:rows[0], 1, 7] = hit[:rows[0], 2, 5] = True
         assert np.array_equal(out[~hit], clean_out[~hit])
         s = c.slots[0]
         assert not np.isfinite(state[0, s, 1, 7]).any() and not np.isfinite(state[0, s, 2, 5]).any()
