@@ -20,6 +20,7 @@
 // whose K, Q, decays or strengths are not finite, is done again row by row: zero times infinity would reach
 // rows before it. Its other columns keep their results (a matrix product's columns do not mix).
 #include <algorithm>
+#include <cstddef>
 
 #include "bg_common.h"
 #include "bg_linear.h"
@@ -57,6 +58,12 @@ struct ChunkSpace {
   static constexpr int K = 0, Q = K + 4 * NKB * 2 * 64, KT = Q + 4 * NKB * 2 * 64, PER_K = KT + (DK / 16) * 2 * 2 * 64;  // in half8
   static constexpr int T = 0, P = T + 4 * 2 * 2 * 64, G = P + 4 * 2 * 2 * 64, META = G + 128 / 4, PER_H = META + 8;       // in 16 bytes
 };
+
+// The workspace, as memory that is known to be the device's: through a pointer of no known kind its loads would
+// count as LDS accesses too, and every barrier wait for them.
+#define BG_GLOBAL __attribute__((address_space(1)))
+typedef BG_GLOBAL half8 ghalf8;
+__device__ inline ghalf8* workspace(const LinBatchView& b) { return (ghalf8*)(b.ws ? b.ws : b.hdr->ws); }
 
 __device__ inline int top_exponent(float x) { return __builtin_amdgcn_frexp_expf(x); }  // x < 2^e; 0 for 0
 __device__ inline int shift_for(float most) { return kTop - top_exponent(most); }
@@ -117,9 +124,8 @@ __global__ __launch_bounds__(256) void linear_chunk_prepare(LinLayer L, LinBatch
   if (u0 + (int)blockIdx.x >= b.hdr->n_chunk_units) return;
   const int kh = blockIdx.y, rep = L.v_heads / L.k_heads;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, m = lane & 15, g = lane >> 4;
-  char* space = b.ws ? b.ws : b.hdr->ws;
-  half8* wk = (half8*)space + (size_t)blockIdx.x * (L.k_heads * W::PER_K + L.v_heads * W::PER_H);
-  half8* wh0 = wk + (size_t)L.k_heads * W::PER_K;
+  ghalf8* wk = workspace(b) + (size_t)blockIdx.x * (L.k_heads * W::PER_K + L.v_heads * W::PER_H);
+  ghalf8* wh0 = wk + (size_t)L.k_heads * W::PER_K;
   wk += (size_t)kh * W::PER_K;
 
   // this wave's 16 rows of K and Q as operands
@@ -215,7 +221,7 @@ __global__ __launch_bounds__(256) void linear_chunk_prepare(LinLayer L, LinBatch
 
   for (int i = 0; i < rep; i++) {
     const int h = kh * rep + i;
-    half8* wh = wh0 + (size_t)h * W::PER_H;
+    ghalf8* wh = wh0 + (size_t)h * W::PER_H;
     __syncthreads();  // the frag reads, or the head before
     float gmax = 1.0f, fmax_ = 1.0f, whole = 1.0f;
     bool bad = bad_k;
@@ -234,8 +240,8 @@ __global__ __launch_bounds__(256) void linear_chunk_prepare(LinLayer L, LinBatch
       gsum[lane] = s;
       strength[lane] = be;
       const float eg = expf((float)s), fg = expf((float)(end - s));
-      ((float*)(wh + W::G))[lane] = eg;
-      ((float*)(wh + W::G))[64 + lane] = on ? fg : 0.0f;
+      ((BG_GLOBAL float*)(wh + W::G))[lane] = eg;
+      ((BG_GLOBAL float*)(wh + W::G))[64 + lane] = on ? fg : 0.0f;
       gmax = __uint_as_float(wave_umax(mag(eg)));
       fmax_ = __uint_as_float(wave_umax(mag(fg)));
       whole = expf((float)end);
@@ -358,7 +364,7 @@ __global__ __launch_bounds__(256) void linear_chunk_prepare(LinLayer L, LinBatch
       __syncthreads();
     }
     for (int w = 0; w < 4; w++) bad = bad || !(__uint_as_float(bits[w]) < 0x1p60f);
-    ChunkMeta* meta = (ChunkMeta*)(wh + W::META);
+    BG_GLOBAL ChunkMeta* meta = (BG_GLOBAL ChunkMeta*)(wh + W::META);
     if (lane == 0) {
       meta->qshift[wave] = qs;
       meta->tshift[wave] = ts;
@@ -380,10 +386,33 @@ __global__ __launch_bounds__(256) void linear_chunk_prepare(LinLayer L, LinBatch
 template <int DK>
 struct Fragments {
   half8 k[DK / 32][2], q[DK / 32][2], t[2][2], p[2][2], kt[DK / 64][2][2];
-  float v[2][4], eg[4], fg[4];
+  float v[2][4];
+  f4 eg, fg;
+  int meta;  // lane i: word i of the chunk's ChunkMeta
 };
+enum { M_KSHIFT = 0, M_QSHIFT = 1, M_TSHIFT = 5, M_PSHIFT = 9, M_KMAX = 13, M_TSUM, M_GMAX, M_FMAX, M_WHOLE, M_BAD };
+static_assert(offsetof(ChunkMeta, bad) == 4 * M_BAD && offsetof(ChunkMeta, kmax) == 4 * M_KMAX, "meta words");
 
-// A sequence's chunks from u0 up to u1 (its window of the workspace) for 32 value dims of a head.
+__device__ inline int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
+__device__ inline __amdgpu_buffer_rsrc_t buffer(const void* p, uint32_t bytes) {
+  const uint64_t a = (uint64_t)p;
+  const uint64_t u = (uint64_t)(uint32_t)uniform((int)(uint32_t)a) | (uint64_t)(uint32_t)uniform((int)(uint32_t)(a >> 32)) << 32;
+  return __builtin_amdgcn_make_buffer_rsrc((void*)u, (short)0, (int)bytes, 0x00020000);
+}
+__device__ inline half8 load8(__amdgpu_buffer_rsrc_t r, int offset, int at) {  // `at` half8s behind byte `offset`
+  return __builtin_bit_cast(half8, __builtin_amdgcn_raw_buffer_load_b128(r, offset, 16 * at, 0));
+}
+// x, which the compiler may not keep ready beside its multiples for the whole loop (those spilled)
+__device__ inline int afresh(int x) {
+  asm volatile("" : "+v"(x));
+  return x;
+}
+
+// A sequence's chunks from u0 up to u1 (its window of the workspace) for 32 value dims of a head. The next chunk's
+// operands are loaded into the registers of this one's as soon as their last product has been issued: by
+// buffer loads, whose one lane offset and scalar rest leave the registers to the operands. (A register too many
+// costs a wait for everything in flight when it is read back: with 64-bit addresses in vector registers 14 us a
+// chunk, with the row offsets of V and the output kept through the loop 6.8.)
 template <int DK, int DV, bool DELTA>
 __global__ __launch_bounds__(256, 2) void linear_chunk_scan(LinLayer L, LinBatchView b, LinAttnArgs a, int u0, int u1) {
   using W = ChunkSpace<DK>;
@@ -391,25 +420,25 @@ __global__ __launch_bounds__(256, 2) void linear_chunk_scan(LinLayer L, LinBatch
   __shared__ half8 Sb[NKB * 2 * 2 * 64];        // the state as an operand
   __shared__ half8 Yb[2 * 2 * 2 * 64], Vb[2 * 2 * 2 * 64], Fb[2 * 2 * 2 * 64];  // Y, V', e^(G_n - G) V'
   __shared__ uint32_t smax[4][kCols], vmax[4][kCols];
-  __shared__ float plain[kCols][DK + 4];        // the state of columns that are done row by row
+  __shared__ float plain[kCols][DK + 4];        // columns that are done row by row: the state before
+  __shared__ int slow_from[kCols];              // this chunk of the sequence
   // a key head's value heads and slices, which read the same operands, run on one XCD
   const int rep = L.v_heads / L.k_heads, members = rep * SLICES;
   const int x = blockIdx.x & 7, j = blockIdx.x >> 3;
   const int group = x + 8 * (j / members), member = j % members;
   const int seq = group / L.k_heads, kh = group % L.k_heads;
   if (seq >= b.hdr->n_chunked) return;
-  const LinSeq s = b.seqs[seq];
-  const int first = max(s.unit0, u0), last = min(s.unit0 + s.n_units, u1);
+  const LinSeq* sp = b.seqs + seq;
+  const int row0 = uniform(sp->row0), rows = uniform(sp->rows), unit0 = uniform(sp->unit0);
+  const int first = max(unit0, u0), last = min(unit0 + uniform(sp->n_units), u1);
   if (first >= last) return;
   const int h = kh * rep + member / SLICES, col0 = (member % SLICES) * kCols;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
-  const char* space = b.ws ? b.ws : b.hdr->ws;
+  const int wave = uniform(threadIdx.x >> 6), lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
   const size_t per_unit = (size_t)L.k_heads * W::PER_K + (size_t)L.v_heads * W::PER_H;
-  const half8* wk0 = (const half8*)space + (size_t)kh * W::PER_K;
-  const half8* wh0 = (const half8*)space + (size_t)L.k_heads * W::PER_K + (size_t)h * W::PER_H;
+  const half8* ws = (const half8*)(b.ws ? b.ws : b.hdr->ws);
 
   f4 S[MT][2];
-  const int from = first == s.unit0 ? s.src : s.dst;
+  const int from = uniform(first == unit0 ? sp->src : sp->dst);
 #pragma unroll
   for (int i = 0; i < MT; i++)
 #pragma unroll
@@ -418,63 +447,75 @@ __global__ __launch_bounds__(256, 2) void linear_chunk_scan(LinLayer L, LinBatch
                            : f4{0, 0, 0, 0};
 
   Fragments<DK> F;
+  const int at_k = 16 * lane + wave * (NKB * 2 * 64 * 16), at_t = 16 * lane + wave * (2 * 2 * 64 * 16);
+  static_assert(NKB == 2 * MT, "the operands of a wave's rows and of its key dims lie alike");
+  auto keys = [&](int u) { return buffer(ws + (size_t)(u - u0) * per_unit + (size_t)kh * W::PER_K, 16 * W::PER_K); };
+  auto head = [&](int u) {
+    return buffer(ws + (size_t)(u - u0) * per_unit + (size_t)L.k_heads * W::PER_K + (size_t)h * W::PER_H, 16 * W::PER_H);
+  };
+  const int vrow = L.v_heads * DV * 4;  // bytes of a row of V and of the output
+  const int vlane = (16 * wave + 4 * g) * vrow + 4 * n;
+  auto values = [&](const float* p, int u) {  // the chunk's rows: those behind them read as zero and are not stored
+    const int r = kLinChunk * (u - unit0);
+    return buffer(p + ((size_t)(row0 + r) * L.v_heads + h) * DV + col0, (min(kLinChunk, rows - r) - 1) * vrow + 4 * kCols);
+  };
   auto load_kq = [&](int u) {
-    const half8* wk = wk0 + (size_t)(u - u0) * per_unit;
+    const auto r = keys(u);
 #pragma unroll
     for (int kb = 0; kb < NKB; kb++)
 #pragma unroll
       for (int hl = 0; hl < 2; hl++) {
-        if constexpr (DELTA) F.k[kb][hl] = wk[W::K + ((wave * NKB + kb) * 2 + hl) * 64 + lane];
-        F.q[kb][hl] = wk[W::Q + ((wave * NKB + kb) * 2 + hl) * 64 + lane];
+        if constexpr (DELTA) F.k[kb][hl] = load8(r, at_k, W::K + (kb * 2 + hl) * 64);
+        F.q[kb][hl] = load8(r, at_k, W::Q + (kb * 2 + hl) * 64);
       }
   };
   auto load_t = [&](int u) {
-    const half8* wh = wh0 + (size_t)(u - u0) * per_unit;
+    const auto r = head(u);
     if constexpr (DELTA)
 #pragma unroll
       for (int kb = 0; kb < 2; kb++)
 #pragma unroll
         for (int hl = 0; hl < 2; hl++)
-          if (2 * kb <= wave) F.t[kb][hl] = wh[W::T + ((wave * 2 + kb) * 2 + hl) * 64 + lane];
+          if (2 * kb <= wave) F.t[kb][hl] = load8(r, at_t, W::T + (kb * 2 + hl) * 64);
   };
   auto load_p = [&](int u) {
-    const half8* wh = wh0 + (size_t)(u - u0) * per_unit;
+    const auto r = head(u);
 #pragma unroll
     for (int kb = 0; kb < 2; kb++)
 #pragma unroll
       for (int hl = 0; hl < 2; hl++)
-        if (2 * kb <= wave) F.p[kb][hl] = wh[W::P + ((wave * 2 + kb) * 2 + hl) * 64 + lane];
+        if (2 * kb <= wave) F.p[kb][hl] = load8(r, at_t, W::P + (kb * 2 + hl) * 64);
   };
   auto load_kt = [&](int u) {
-    const half8* wk = wk0 + (size_t)(u - u0) * per_unit;
+    const auto r = keys(u);
 #pragma unroll
     for (int i = 0; i < MT; i++)
 #pragma unroll
       for (int kb = 0; kb < 2; kb++)
 #pragma unroll
-        for (int hl = 0; hl < 2; hl++) F.kt[i][kb][hl] = wk[W::KT + (((wave * MT + i) * 2 + kb) * 2 + hl) * 64 + lane];
+        for (int hl = 0; hl < 2; hl++) F.kt[i][kb][hl] = load8(r, at_k, W::KT + ((i * 2 + kb) * 2 + hl) * 64);
   };
   auto load_v = [&](int u) {
-    const LinUnit w = b.units[u];
+    const auto r = values(a.v, u);
+    int at = afresh(vlane);
 #pragma unroll
-    for (int r = 0; r < 4; r++) {
-      const int row = 16 * wave + 4 * g + r;
-      const size_t at = ((size_t)(w.row0 + (row < w.n ? row : 0)) * L.v_heads + h) * DV + col0 + n;
+    for (int e = 0; e < 4; e++, at += vrow)
 #pragma unroll
-      for (int nt = 0; nt < 2; nt++) F.v[nt][r] = row < w.n ? a.v[at + 16 * nt] : 0.0f;
-    }
-    const float* gg = (const float*)(wh0 + (size_t)(u - u0) * per_unit + W::G) + 16 * wave + 4 * g;
-#pragma unroll
-    for (int r = 0; r < 4; r++) {
-      F.eg[r] = gg[r];
-      F.fg[r] = gg[64 + r];
-    }
+      for (int nt = 0; nt < 2; nt++) F.v[nt][e] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(r, at + 64 * nt, 0, 0));
   };
+  auto load_meta = [&](int u) {
+    const auto r = head(u);
+    const int l = afresh(lane), at = 64 * wave + 16 * (l >> 4);
+    F.eg = __builtin_bit_cast(f4, __builtin_amdgcn_raw_buffer_load_b128(r, at, 16 * W::G, 0));
+    F.fg = __builtin_bit_cast(f4, __builtin_amdgcn_raw_buffer_load_b128(r, at, 16 * W::G + 256, 0));
+    F.meta = __builtin_amdgcn_raw_buffer_load_b32(r, 4 * (l & 31), 16 * W::META, 0);
+  };
+  auto word = [&](int i) { return __builtin_amdgcn_readlane(F.meta, i); };
+  auto fword = [&](int i) { return __builtin_bit_cast(float, __builtin_amdgcn_readlane(F.meta, i)); };
+  load_meta(first);
   load_kq(first);
-  load_t(first);
-  load_p(first);
-  load_kt(first);
   load_v(first);
+  load_kt(first);
 
   auto note_state = [&]() {  // the largest |S| of each column over this wave's key dims
 #pragma unroll
@@ -485,7 +526,8 @@ __global__ __launch_bounds__(256, 2) void linear_chunk_scan(LinLayer L, LinBatch
 #pragma unroll
         for (int r = 0; r < 4; r++) t = max(t, mag(S[i][nt][r]));
       t = groups_max(t);
-      if (g == 0) smax[wave][16 * nt + n] = t;
+      const int l = afresh(lane);
+      if (l < 16) smax[wave][16 * nt + l] = t;
     }
   };
   auto note_v = [&]() {
@@ -495,7 +537,8 @@ __global__ __launch_bounds__(256, 2) void linear_chunk_scan(LinLayer L, LinBatch
 #pragma unroll
       for (int r = 0; r < 4; r++) t = max(t, mag(F.v[nt][r]));
       t = groups_max(t);
-      if (g == 0) vmax[wave][16 * nt + n] = t;
+      const int l = afresh(lane);
+      if (l < 16) vmax[wave][16 * nt + l] = t;
     }
   };
   auto put4 = [&](half8* to, int tile, int nt, const float (&x)[4], int shift) {
@@ -528,39 +571,52 @@ __global__ __launch_bounds__(256, 2) void linear_chunk_scan(LinLayer L, LinBatch
   }
   put_state();
 
+  uint32_t slow = 0;  // the columns that are done row by row
+#pragma unroll 1
   for (int u = first; u < last; u++) {
-    const LinUnit w = b.units[u];
-    const ChunkMeta* meta = (const ChunkMeta*)(wh0 + (size_t)(u - u0) * per_unit + W::META);
-    const int kshift = meta->kshift, qshift = meta->qshift[wave], tshift = meta->tshift[wave], pshift = meta->pshift[wave];
-    const float whole = meta->whole;
     const int next = min(u + 1, last - 1);
+    const int kshift = word(M_KSHIFT), qshift = word(M_QSHIFT + wave), tshift = word(M_TSHIFT + wave), pshift = word(M_PSHIFT + wave);
+    const float whole = fword(M_WHOLE);
     __syncthreads();  // the state, and what is noted of it and of V
     int yshift[2], vshift[2], fshift[2], sshift_next[2];
-    bool odd = meta->bad;
-    uint32_t todo = 0;  // columns for the row-by-row pass
+    uint32_t todo = 0;  // columns that are not for these products
+    {
+      const bool bad = word(M_BAD);
+      const float kmax = fword(M_KMAX), tsum = fword(M_TSUM), gmax = fword(M_GMAX), fmax_ = fword(M_FMAX);
 #pragma unroll
-    for (int nt = 0; nt < 2; nt++) {
-      const int c = 16 * nt + n;
-      const float sm = __uint_as_float(max(max(smax[0][c], smax[1][c]), max(smax[2][c], smax[3][c])));
-      const float vm = __uint_as_float(max(max(vmax[0][c], vmax[1][c]), max(vmax[2][c], vmax[3][c])));
-      const float ym = vm + (DELTA ? meta->gmax * (DK * meta->kmax) * sm : 0.0f);
-      const float vpm = meta->tsum * ym, fm = meta->fmax * vpm;
-      const float next_m = whole * sm + kLinChunk * meta->kmax * fm;
-      yshift[nt] = shift_for(ym);
-      vshift[nt] = shift_for(vpm);
-      fshift[nt] = shift_for(fm);
-      sshift_next[nt] = shift_for(next_m);
-      const bool out = odd || !(next_m < 0x1p120f) || !(ym < 0x1p120f) || !(vpm < 0x1p120f) || !(sm < 0x1p120f);
-      todo |= (uint32_t)(__ballot(out) & 0xffffu) << (16 * nt);
+      for (int nt = 0; nt < 2; nt++) {
+        const int c = 16 * nt + n;
+        const float sm = __uint_as_float(max(max(smax[0][c], smax[1][c]), max(smax[2][c], smax[3][c])));
+        const float vm = __uint_as_float(max(max(vmax[0][c], vmax[1][c]), max(vmax[2][c], vmax[3][c])));
+        const float ym = vm + (DELTA ? gmax * (DK * kmax) * sm : 0.0f);
+        const float vpm = tsum * ym, fm = fmax_ * vpm;
+        const float next_m = whole * sm + kLinChunk * kmax * fm;
+        yshift[nt] = shift_for(ym);
+        vshift[nt] = shift_for(vpm);
+        fshift[nt] = shift_for(fm);
+        sshift_next[nt] = shift_for(next_m);
+        const bool out = bad || !(next_m < 0x1p120f) || !(ym < 0x1p120f) || !(vpm < 0x1p120f) || !(sm < 0x1p120f);
+        todo |= (uint32_t)(__ballot(out) & 0xffffu) << (16 * nt);
+      }
+      todo = uniform(todo);
     }
-    todo = __builtin_amdgcn_readfirstlane(todo);
-    if (todo) {
+    todo &= ~slow;
+    if (todo) {  // columns that leave the chunks here
+      const int l = afresh(lane);
 #pragma unroll
-      for (int i = 0; i < MT; i++)
+      for (int nt = 0; nt < 2; nt++) {
+        const int c = 16 * nt + (l & 15);
+        if (!(todo >> c & 1)) continue;
 #pragma unroll
-        for (int nt = 0; nt < 2; nt++) *(f4*)&plain[16 * nt + n][16 * (wave * MT + i) + 4 * g] = S[i][nt];
+        for (int i = 0; i < MT; i++) *(f4*)&plain[c][16 * (wave * MT + i) + 4 * (l >> 4)] = S[i][nt];
+        if (wave == 0) slow_from[c] = u - unit0;
+      }
+      slow |= todo;
     }
 
+    __builtin_amdgcn_sched_barrier(0);
+    load_t(u);
+    __builtin_amdgcn_sched_barrier(0);
     // K S and Q S
     f4 ks[2], o[2];
 #pragma unroll
@@ -573,11 +629,10 @@ __global__ __launch_bounds__(256, 2) void linear_chunk_scan(LinLayer L, LinBatch
         if constexpr (DELTA) ks[nt] = product3(F.k[kb][0], F.k[kb][1], sh, sl, ks[nt]);
         o[nt] = product3(F.q[kb][0], F.q[kb][1], sh, sl, o[nt]);
       }
+    __builtin_amdgcn_sched_barrier(0);
+    load_p(u);
     load_kq(next);
-#pragma unroll
-    for (int nt = 0; nt < 2; nt++)
-#pragma unroll
-      for (int r = 0; r < 4; r++) o[nt][r] = F.eg[r] * ldexpf(o[nt][r], -qshift - sshift[nt]);
+    __builtin_amdgcn_sched_barrier(0);
     f4 vp[2];
     if constexpr (DELTA) {
 #pragma unroll
@@ -595,10 +650,11 @@ __global__ __launch_bounds__(256, 2) void linear_chunk_scan(LinLayer L, LinBatch
         for (int kb = 0; kb < 2; kb++)
           if (2 * kb <= wave)
             vp[nt] = product3(F.t[kb][0], F.t[kb][1], Yb[((kb * 2 + nt) * 2 + 0) * 64 + lane], Yb[((kb * 2 + nt) * 2 + 1) * 64 + lane], vp[nt]);
+      }
+#pragma unroll
+      for (int nt = 0; nt < 2; nt++)
 #pragma unroll
         for (int r = 0; r < 4; r++) vp[nt][r] = ldexpf(vp[nt][r], -tshift - yshift[nt]);
-      }
-      load_t(next);
     } else {
 #pragma unroll
       for (int nt = 0; nt < 2; nt++)
@@ -612,7 +668,14 @@ __global__ __launch_bounds__(256, 2) void linear_chunk_scan(LinLayer L, LinBatch
       put4(Vb, wave, nt, y, vshift[nt]);
       put4(Fb, wave, nt, z, fshift[nt]);
     }
+#pragma unroll
+    for (int nt = 0; nt < 2; nt++)
+#pragma unroll
+      for (int r = 0; r < 4; r++) o[nt][r] = F.eg[r] * ldexpf(o[nt][r], -qshift - sshift[nt]);
+    __builtin_amdgcn_sched_barrier(0);
     load_v(next);
+    load_meta(next);
+    __builtin_amdgcn_sched_barrier(0);
     __syncthreads();
     // the state
 #pragma unroll
@@ -626,8 +689,11 @@ __global__ __launch_bounds__(256, 2) void linear_chunk_scan(LinLayer L, LinBatch
 #pragma unroll
         for (int r = 0; r < 4; r++) S[i][nt][r] = fmaf(whole, S[i][nt][r], ldexpf(acc[r], -kshift - fshift[nt]));
       }
+    __builtin_amdgcn_sched_barrier(0);
     load_kt(next);
+    __builtin_amdgcn_sched_barrier(0);
     // the output
+    const auto ro = values(a.out, u);
 #pragma unroll
     for (int nt = 0; nt < 2; nt++) {
       f4 acc = f4{0, 0, 0, 0};
@@ -636,58 +702,16 @@ __global__ __launch_bounds__(256, 2) void linear_chunk_scan(LinLayer L, LinBatch
         if (2 * kb <= wave)
           acc = product3(F.p[kb][0], F.p[kb][1], Vb[((kb * 2 + nt) * 2 + 0) * 64 + lane], Vb[((kb * 2 + nt) * 2 + 1) * 64 + lane], acc);
 #pragma unroll
-      for (int r = 0; r < 4; r++) {
-        const int row = 16 * wave + 4 * g + r;
-        const float y = a.scale * (o[nt][r] + ldexpf(acc[r], -pshift - vshift[nt]));
-        if (row < w.n && !(todo >> (16 * nt + n) & 1)) a.out[((size_t)(w.row0 + row) * L.v_heads + h) * DV + col0 + 16 * nt + n] = y;
-      }
+      for (int r = 0; r < 4; r++) o[nt][r] = a.scale * (o[nt][r] + ldexpf(acc[r], -pshift - vshift[nt]));
     }
-    load_p(next);
-    if (todo) {  // eight lanes a column, as linear_attn.hip's
-      __syncthreads();
-      const int c = threadIdx.x >> 3, l = threadIdx.x & 7;
-      float* sp = &plain[c][4 * l];
-      f4 st[DK / 32];
+    {
+      int at = afresh(vlane);
+      const bool on[2] = {!(slow >> n & 1), !(slow >> (16 + n) & 1)};
 #pragma unroll
-      for (int i = 0; i < DK / 32; i++) st[i] = *(const f4*)(sp + 32 * i);
-#pragma unroll 1
-      for (int t = 0; t < w.n; t++) {
-        const size_t r = w.row0 + t;
-        const float* kp = a.k + (r * L.k_heads + kh) * DK + 4 * l;
-        const float* qp = a.q + (r * L.k_heads + kh) * DK + 4 * l;
-        float hi, lo;
-        fade_of(a.g[(a.g_stride ? r * a.g_stride : 0) + h], hi, lo);
-        float sum = 0.0f;
-        f4 kx[DK / 32];
-#pragma unroll
-        for (int i = 0; i < DK / 32; i++) {
-          kx[i] = *(const f4*)(kp + 32 * i);
-#pragma unroll
-          for (int e = 0; e < 4; e++) sum = fmaf(st[i][e], kx[i][e], sum);
-        }
-        float d = a.v[(r * L.v_heads + h) * DV + col0 + c];
-        if constexpr (DELTA) d = a.beta[r * L.v_heads + h] * (d - hi * group_sum<8>(sum));
-        sum = 0.0f;
-#pragma unroll
-        for (int i = 0; i < DK / 32; i++) {
-          const f4 q = *(const f4*)(qp + 32 * i);
-#pragma unroll
-          for (int e = 0; e < 4; e++) {
-            st[i][e] = fmaf(hi, st[i][e], fmaf(lo, st[i][e], kx[i][e] * d));
-            sum = fmaf(st[i][e], q[e], sum);
-          }
-        }
-        sum = group_sum<8>(sum);
-        if (l == 0 && (todo >> c & 1)) a.out[(r * L.v_heads + h) * DV + col0 + c] = a.scale * sum;
-      }
-#pragma unroll
-      for (int i = 0; i < DK / 32; i++) *(f4*)(sp + 32 * i) = st[i];
-      __syncthreads();
-#pragma unroll
-      for (int i = 0; i < MT; i++)
+      for (int r = 0; r < 4; r++, at += vrow)
 #pragma unroll
         for (int nt = 0; nt < 2; nt++)
-          if (todo >> (16 * nt + n) & 1) S[i][nt] = *(const f4*)&plain[16 * nt + n][16 * (wave * MT + i) + 4 * g];
+          if (on[nt]) __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(o[nt][r]), ro, at + 64 * nt, 0, 0);
     }
     note_state();
     note_v();
@@ -695,11 +719,53 @@ __global__ __launch_bounds__(256, 2) void linear_chunk_scan(LinLayer L, LinBatch
     for (int nt = 0; nt < 2; nt++) sshift[nt] = sshift_next[nt];
     put_state();
   }
+  float* left = L.state + (((size_t)uniform(sp->dst) * L.v_heads + h) * DV + col0) * DK;
 #pragma unroll
   for (int i = 0; i < MT; i++)
 #pragma unroll
     for (int nt = 0; nt < 2; nt++)
-      *(f4*)(L.state + (((size_t)s.dst * L.v_heads + h) * DV + col0 + 16 * nt + n) * DK + 16 * (wave * MT + i) + 4 * g) = S[i][nt];
+      if (!(slow >> (16 * nt + n) & 1)) *(f4*)(left + (16 * nt + n) * DK + 16 * (wave * MT + i) + 4 * g) = S[i][nt];
+  if (!slow) return;
+  // the other columns, eight lanes each, as linear_attn.hip does them
+  __syncthreads();
+  const int c = threadIdx.x >> 3, l = threadIdx.x & 7;
+  if (!(slow >> c & 1)) return;
+  f4 st[DK / 32];
+#pragma unroll
+  for (int i = 0; i < DK / 32; i++) st[i] = *(const f4*)&plain[c][32 * i + 4 * l];
+  const int end = min(rows, kLinChunk * (last - unit0));
+#pragma unroll 1
+  for (int t = kLinChunk * slow_from[c]; t < end; t++) {
+    const size_t r = row0 + t;
+    const float* kp = a.k + (r * L.k_heads + kh) * DK + 4 * l;
+    const float* qp = a.q + (r * L.k_heads + kh) * DK + 4 * l;
+    float hi, lo;
+    fade_of(a.g[(a.g_stride ? r * a.g_stride : 0) + h], hi, lo);
+    float sum = 0.0f;
+    f4 kx[DK / 32];
+#pragma unroll
+    for (int i = 0; i < DK / 32; i++) {
+      kx[i] = *(const f4*)(kp + 32 * i);
+#pragma unroll
+      for (int e = 0; e < 4; e++) sum = fmaf(st[i][e], kx[i][e], sum);
+    }
+    float d = a.v[(r * L.v_heads + h) * DV + col0 + c];
+    if constexpr (DELTA) d = a.beta[r * L.v_heads + h] * (d - hi * group_sum<8>(sum));
+    sum = 0.0f;
+#pragma unroll
+    for (int i = 0; i < DK / 32; i++) {
+      const f4 q = *(const f4*)(qp + 32 * i);
+#pragma unroll
+      for (int e = 0; e < 4; e++) {
+        st[i][e] = fmaf(hi, st[i][e], fmaf(lo, st[i][e], kx[i][e] * d));
+        sum = fmaf(st[i][e], q[e], sum);
+      }
+    }
+    sum = group_sum<8>(sum);
+    if (l == 0) a.out[(r * L.v_heads + h) * DV + col0 + c] = a.scale * sum;
+  }
+#pragma unroll
+  for (int i = 0; i < DK / 32; i++) *(f4*)(left + c * DK + 32 * i + 4 * l) = st[i];
 }
 
 // The output norm of the chunks' rows, in place: DV / 4 lanes a row and head.
