@@ -30,21 +30,21 @@ namespace bg {
 namespace {
 
 typedef _Float16 half8 __attribute__((ext_vector_type(8)));
-typedef _Float16 half4 __attribute__((ext_vector_type(4)));
 typedef float f4 __attribute__((ext_vector_type(4)));
 
 constexpr int kTop = 14;      // an operand's largest value is below 2^kTop
 constexpr int kCols = 32;     // value dims of a scan workgroup
+constexpr int kBad = 1 << 20;
 constexpr int kPad = 68;      // row stride of 64 x 64 matrices in LDS
 constexpr double kLowest = -1e4;  // of a log decay: e^g is 0 in f32 from -104 on
 
 // What the scan needs of a chunk and head beside its operands. Operands are held times 2^shift.
 struct ChunkMeta {
   int kshift, qshift[4], tshift[4], pshift[4];
-  float kmax;                  // largest |K|
-  float tsum;                  // largest row sum of |T|
-  float gmax, fmax, whole;     // largest e^G_i and e^(G_n - G_i), e^G_n
-  int bad;                     // something is not finite: row by row
+  float whole;                 // e^G_n
+  // What the scan's bounds are made of, as powers of two: y of gmax DK kmax (of a state's share of Y), t of T's
+  // largest row sum, f of the largest e^(G_n - G_i), s of e^G_n, k of 64 kmax. bad in y: something is not finite
+  int ey, et, ef, es, ek;
   int pad[13];
 };
 static_assert(sizeof(ChunkMeta) == 128, "meta");
@@ -70,23 +70,56 @@ __device__ inline int shift_for(float most) { return kTop - top_exponent(most); 
 __device__ inline uint32_t mag(float x) { return __float_as_uint(x) & 0x7fffffffu; }
 constexpr uint32_t kInf = 0x7f800000u;
 
-__device__ inline void split4(const float (&x)[4], half4& hi, half4& lo) {
-#pragma unroll
-  for (int i = 0; i < 4; i++) hi[i] = (_Float16)x[i];
-#pragma unroll
-  for (int i = 0; i < 4; i++) lo[i] = (_Float16)(x[i] - (float)hi[i]);
+// x less the low (high) half of h: one mixed-precision fma, exact
+__device__ inline float less_lo(float x, uint32_t h) {
+  float r;
+  asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel_hi:[1,0,0]" : "=v"(r) : "v"(h), "v"(x));
+  return r;
+}
+__device__ inline float less_hi(float x, uint32_t h) {
+  float r;
+  asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(r) : "v"(h), "v"(x));
+  return r;
+}
+// a, b as hi and lo f16 parts, each rounded to nearest
+__device__ inline void split2(float a, float b, uint32_t& hi, uint32_t& lo) {
+  typedef _Float16 half2_t __attribute__((ext_vector_type(2)));
+  const half2_t h = {(_Float16)a, (_Float16)b};
+  hi = __builtin_bit_cast(uint32_t, h);
+  const half2_t l = {(_Float16)less_lo(a, hi), (_Float16)less_hi(b, hi)};
+  lo = __builtin_bit_cast(uint32_t, l);
+}
+typedef uint32_t u2 __attribute__((ext_vector_type(2)));
+typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+__device__ inline void split4(float a, float b, float c, float d, u2& hi, u2& lo) {
+  uint32_t h[2], l[2];
+  split2(a, b, h[0], l[0]);
+  split2(c, d, h[1], l[1]);
+  hi = u2{h[0], h[1]};
+  lo = u2{l[0], l[1]};
 }
 __device__ inline void split8(const float (&x)[8], half8& hi, half8& lo) {
+  uint32_t h[4], l[4];
 #pragma unroll
-  for (int i = 0; i < 8; i++) hi[i] = (_Float16)x[i];
-#pragma unroll
-  for (int i = 0; i < 8; i++) lo[i] = (_Float16)(x[i] - (float)hi[i]);
+  for (int i = 0; i < 4; i++) split2(x[2 * i], x[2 * i + 1], h[i], l[i]);
+  hi = __builtin_bit_cast(half8, u4{h[0], h[1], h[2], h[3]});
+  lo = __builtin_bit_cast(half8, u4{l[0], l[1], l[2], l[3]});
 }
 // c += (ah + al)(bh + bl) less al bl
 __device__ inline f4 product3(half8 ah, half8 al, half8 bh, half8 bl, f4 c) {
   c = __builtin_amdgcn_mfma_f32_16x16x32_f16(al, bh, c, 0, 0, 0);
   c = __builtin_amdgcn_mfma_f32_16x16x32_f16(ah, bl, c, 0, 0, 0);
   return __builtin_amdgcn_mfma_f32_16x16x32_f16(ah, bh, c, 0, 0, 0);
+}
+// the same for N tiles of columns, their chains side by side
+template <int N>
+__device__ inline void products3(half8 ah, half8 al, const half8 (&bh)[N], const half8 (&bl)[N], f4 (&c)[N]) {
+#pragma unroll
+  for (int i = 0; i < N; i++) c[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(al, bh[i], c[i], 0, 0, 0);
+#pragma unroll
+  for (int i = 0; i < N; i++) c[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ah, bl[i], c[i], 0, 0, 0);
+#pragma unroll
+  for (int i = 0; i < N; i++) c[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ah, bh[i], c[i], 0, 0, 0);
 }
 // over the four lane groups that hold a column's rows (or a row's k values)
 __device__ inline uint32_t groups_max(uint32_t v) {
@@ -106,15 +139,37 @@ __device__ inline uint32_t wave_umax(uint32_t v) {
   return groups_max(v);
 }
 
+__device__ inline int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
+__device__ inline __amdgpu_buffer_rsrc_t buffer(const void* p, uint32_t bytes) {
+  const uint64_t a = (uint64_t)p;
+  const uint64_t u = (uint64_t)(uint32_t)uniform((int)(uint32_t)a) | (uint64_t)(uint32_t)uniform((int)(uint32_t)(a >> 32)) << 32;
+  return __builtin_amdgcn_make_buffer_rsrc((void*)u, (short)0, (int)bytes, 0x00020000);
+}
+__device__ inline half8 load8(__amdgpu_buffer_rsrc_t r, int offset, int at) {  // `at` half8s behind byte `offset`
+  return __builtin_bit_cast(half8, __builtin_amdgcn_raw_buffer_load_b128(r, offset, 16 * at, 0));
+}
+// x, copied here: a copy that the compiler puts at its next use would wait there for what x is loaded with anew
+__device__ inline float moved(float x) {
+  float y;
+  asm volatile("v_mov_b32 %0, %1" : "=v"(y) : "v"(x));
+  return y;
+}
+// x, which the compiler may not keep ready beside its multiples for the whole loop (those spilled)
+__device__ inline int afresh(int x) {
+  asm volatile("" : "+v"(x));
+  return x;
+}
+
 // One chunk and key head (and its value heads): blockIdx.x a unit from u0 on, blockIdx.y the key head.
 template <int DK, bool DELTA>
-__global__ __launch_bounds__(256) void linear_chunk_prepare(LinLayer L, LinBatchView b, LinAttnArgs a, int u0) {
+__global__ __launch_bounds__(256, 4) void linear_chunk_prepare(LinLayer L, LinBatchView b, LinAttnArgs a, int u0) {
   using W = ChunkSpace<DK>;
   constexpr int NKB = W::NKB;
   constexpr int kMat = 64 * kPad * 4, kFrag = 4 * NKB * 2 * 64 * 16;
   __shared__ __align__(16) char mem[2 * kMat > kFrag ? 2 * kMat : kFrag];
-  __shared__ double gsum[64];
-  __shared__ float strength[64];
+  __shared__ double gsums[4][64];            // of four value heads at a time, a wave each
+  __shared__ float strengths[4][64], gtop[4][3];
+  __shared__ int gbad[4];
   __shared__ uint32_t most[4], bits[4];
   __shared__ float sums[4];
   half8* frag = (half8*)mem;                 // K, while products with it run
@@ -123,11 +178,17 @@ __global__ __launch_bounds__(256) void linear_chunk_prepare(LinLayer L, LinBatch
   const LinUnit u = b.units[u0 + blockIdx.x];
   if (u0 + (int)blockIdx.x >= b.hdr->n_chunk_units) return;
   const int kh = blockIdx.y, rep = L.v_heads / L.k_heads;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, m = lane & 15, g = lane >> 4;
+  const int wave = uniform(threadIdx.x >> 6), lane_ = threadIdx.x & 63;
   ghalf8* wk = workspace(b) + (size_t)blockIdx.x * (L.k_heads * W::PER_K + L.v_heads * W::PER_H);
   ghalf8* wh0 = wk + (size_t)L.k_heads * W::PER_K;
   wk += (size_t)kh * W::PER_K;
 
+  f4 kk[4], qk[4];
+  float kmax;
+  int ks, qs;
+  bool bad_k;
+  {
+  const int lane = lane_, m = lane & 15, g = lane >> 4;
   // this wave's 16 rows of K and Q as operands
   const int row = 16 * wave + m;
   const bool live = row < u.n;
@@ -156,9 +217,10 @@ __global__ __launch_bounds__(256) void linear_chunk_prepare(LinLayer L, LinBatch
   __syncthreads();
   const uint32_t kall = max(max(most[0], most[1]), max(most[2], most[3]));
   const uint32_t qall = max(max(bits[0], bits[1]), max(bits[2], bits[3]));
-  const bool bad_k = kall >= kInf || qall >= kInf;
-  const float kmax = __uint_as_float(kall);
-  const int ks = shift_for(kmax), qs = shift_for(__uint_as_float(qm));
+  bad_k = kall >= kInf || qall >= kInf;
+  kmax = __uint_as_float(kall);
+  ks = shift_for(kmax);
+  qs = shift_for(__uint_as_float(qm));
   half8 qh[NKB], ql[NKB], kh8[NKB], kl8[NKB];
 #pragma unroll
   for (int kb = 0; kb < NKB; kb++) {
@@ -190,6 +252,7 @@ __global__ __launch_bounds__(256) void linear_chunk_prepare(LinLayer L, LinBatch
       for (int kb2 = 0; kb2 < 2; kb2++)
 #pragma unroll
         for (int hl = 0; hl < 2; hl++) {
+          asm volatile("" ::: "memory");
           half8 x;
 #pragma unroll
           for (int j = 0; j < 8; j++) {
@@ -201,11 +264,11 @@ __global__ __launch_bounds__(256) void linear_chunk_prepare(LinLayer L, LinBatch
     }
   }
   // row tile `wave` of K K^T and Q K^T
-  f4 kk[4], qk[4];
 #pragma unroll
   for (int ct = 0; ct < 4; ct++) {
     kk[ct] = qk[ct] = f4{0, 0, 0, 0};
     if (ct > wave) continue;
+    asm volatile("" ::: "memory");  // (one tile's operands at a time in registers)
 #pragma unroll
     for (int kb = 0; kb < NKB; kb++) {
       const half8 bh = frag[((ct * NKB + kb) * 2 + 0) * 64 + lane], bl = frag[((ct * NKB + kb) * 2 + 1) * 64 + lane];
@@ -218,36 +281,50 @@ __global__ __launch_bounds__(256) void linear_chunk_prepare(LinLayer L, LinBatch
       qk[ct][r] = ldexpf(qk[ct][r], -ks - qs);
     }
   }
+  }
 
+#pragma unroll 1
   for (int i = 0; i < rep; i++) {
     const int h = kh * rep + i;
     ghalf8* wh = wh0 + (size_t)h * W::PER_H;
+    const auto rh = buffer((const void*)wh, 16 * W::PER_H);
+    const int lane = afresh(lane_), m = lane & 15, g = lane >> 4, row = 16 * wave + m;
     __syncthreads();  // the frag reads, or the head before
-    float gmax = 1.0f, fmax_ = 1.0f, whole = 1.0f;
-    bool bad = bad_k;
-    if (wave == 0) {  // the decays' sums: lane = row
-      const bool on = lane < u.n;
-      const size_t rr = u.row0 + (on ? lane : 0);
-      const float gv = on ? a.g[(a.g_stride ? rr * a.g_stride : 0) + h] : 0.0f;
-      double s = gv < (float)kLowest ? kLowest : (double)gv;
+    if ((i & 3) == 0) {
+      if (i + wave < rep) {  // the decays' sums: lane = row
+        const bool on = lane < u.n;
+        const size_t rr = u.row0 + (on ? lane : 0);
+        const int hh = h + wave;
+        const float gv = on ? a.g[(a.g_stride ? rr * a.g_stride : 0) + hh] : 0.0f;
+        double s = gv < (float)kLowest ? kLowest : (double)gv;
 #pragma unroll
-      for (int d = 1; d < 64; d <<= 1) {
-        const double o = __shfl_up(s, d);
-        if (lane >= d) s += o;
+        for (int d = 1; d < 64; d <<= 1) {
+          const double o = __shfl_up(s, d);
+          if (lane >= d) s += o;
+        }
+        const double end = __shfl(s, 63);
+        const float be = DELTA ? (on ? a.beta[rr * L.v_heads + hh] : 0.0f) : 1.0f;
+        gsums[wave][lane] = s;
+        strengths[wave][lane] = be;
+        const float eg = expf((float)s), fg = expf((float)(end - s));
+        BG_GLOBAL float* gg = (BG_GLOBAL float*)(wh + (size_t)wave * W::PER_H + W::G);
+        gg[lane] = eg;
+        gg[64 + lane] = on ? fg : 0.0f;
+        const float gm = __uint_as_float(wave_umax(mag(eg))), fm = __uint_as_float(wave_umax(mag(fg)));
+        const bool odd = __any(mag(eg) >= kInf || mag(fg) >= kInf || mag(be) >= kInf);
+        if (lane == 0) {
+          gtop[wave][0] = gm;
+          gtop[wave][1] = fm;
+          gtop[wave][2] = expf((float)end);
+          gbad[wave] = odd;
+        }
       }
-      const double end = __shfl(s, 63);
-      const float be = DELTA ? (on ? a.beta[rr * L.v_heads + h] : 0.0f) : 1.0f;
-      gsum[lane] = s;
-      strength[lane] = be;
-      const float eg = expf((float)s), fg = expf((float)(end - s));
-      ((BG_GLOBAL float*)(wh + W::G))[lane] = eg;
-      ((BG_GLOBAL float*)(wh + W::G))[64 + lane] = on ? fg : 0.0f;
-      gmax = __uint_as_float(wave_umax(mag(eg)));
-      fmax_ = __uint_as_float(wave_umax(mag(fg)));
-      whole = expf((float)end);
-      bad = bad || __any(mag(eg) >= kInf || mag(fg) >= kInf || mag(be) >= kInf);
+      __syncthreads();
     }
-    __syncthreads();
+    const double* gsum = gsums[i & 3];
+    const float* strength = strengths[i & 3];
+    const float gmax = gtop[i & 3][0], fmax_ = gtop[i & 3][1], whole = gtop[i & 3][2];
+    bool bad = bad_k || gbad[i & 3];
     // A and P of this wave's rows
     uint32_t pm = 0;
 #pragma unroll
@@ -258,7 +335,7 @@ __global__ __launch_bounds__(256) void linear_chunk_prepare(LinLayer L, LinBatch
 #pragma unroll
       for (int r = 0; r < 4; r++) {
         const int w = 16 * wave + 4 * g + r;
-        const float fade = c <= w ? expf((float)(gsum[w] - gc)) : 0.0f;
+        const float fade = expf(c <= w ? (float)(gsum[w] - gc) : -__builtin_inff());  // 0 above the diagonal
         const float p = c <= w ? fade * qk[ct][r] : 0.0f;
         Tm[w * kPad + c] = p;
         pm = max(pm, mag(p));
@@ -292,8 +369,9 @@ __global__ __launch_bounds__(256) void linear_chunk_prepare(LinLayer L, LinBatch
 #pragma unroll
       for (int e = 0; e < 8; e++) x[e] = ldexpf(x[e], shift);
       split8(x, hi, lo);
-      wh[base + ((wave * 2 + kb) * 2 + 0) * 64 + lane] = hi;
-      wh[base + ((wave * 2 + kb) * 2 + 1) * 64 + lane] = lo;
+      const int at = 16 * lane + 4096 * wave;
+      __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u4, hi), rh, at, 16 * (base + kb * 128), 0);
+      __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u4, lo), rh, at, 16 * (base + kb * 128 + 64), 0);
     };
 #pragma unroll
     for (int kb = 0; kb < 2; kb++) {
@@ -310,11 +388,22 @@ __global__ __launch_bounds__(256) void linear_chunk_prepare(LinLayer L, LinBatch
       {  // the diagonal block of this wave, a column a lane (four lanes alike)
         float x[16];
 #pragma unroll
-        for (int r = 0; r < 16; r++) {
-          float y = r == m ? 1.0f : 0.0f;
+        for (int q = 0; q < 8; q++) {
+          // two rows' values at a time: all sixteen rows' at once do not fit
+          asm volatile("" ::: "memory");
+          f4 w[2][4];
 #pragma unroll
-          for (int j = 0; j < r; j++) y = fmaf(-Am[(16 * wave + r) * kPad + 16 * wave + j], x[j], y);
-          x[r] = y;
+          for (int r = 0; r < 2; r++)
+#pragma unroll
+            for (int c = 0; c <= q / 2; c++) w[r][c] = *(const f4*)(Am + (16 * wave + 2 * q + r) * kPad + 16 * wave + 4 * c);
+#pragma unroll
+          for (int r = 0; r < 2; r++) {
+            float y = 2 * q + r == m ? 1.0f : 0.0f;
+#pragma unroll
+            for (int c = 0; c < 2 * q + r; c++) y = fmaf(-w[r][c >> 2][c & 3], x[c], y);
+            asm volatile("" : "+v"(y));  // here, and not where a lane stores it: the values it is made of go
+            x[2 * q + r] = y;
+          }
         }
 #pragma unroll
         for (int r = 0; r < 16; r++)
@@ -371,54 +460,34 @@ __global__ __launch_bounds__(256) void linear_chunk_prepare(LinLayer L, LinBatch
       meta->pshift[wave] = ps;
       if (wave == 0) {
         meta->kshift = ks;
-        meta->kmax = kmax;
-        meta->tsum = tsum;
-        meta->gmax = gmax;
-        meta->fmax = fmax_;
         meta->whole = whole;
-        meta->bad = bad;
+        meta->ey = bad ? kBad : top_exponent(gmax) + top_exponent(DK * kmax);
+        meta->et = top_exponent(tsum);
+        meta->ef = top_exponent(fmax_);
+        meta->es = whole > 0.0f ? top_exponent(whole) : -200;
+        meta->ek = kmax > 0.0f ? top_exponent(kLinChunk * kmax) : -200;
       }
     }
   }
 }
 
-// A chunk's operands of one wave: its 16 rows of K, Q, T, P, its key dims of K^T, and its rows of V.
-template <int DK>
-struct Fragments {
-  half8 k[DK / 32][2], q[DK / 32][2], t[2][2], p[2][2], kt[DK / 64][2][2];
-  float v[2][4];
-  f4 eg, fg;
-  int meta;  // lane i: word i of the chunk's ChunkMeta
-};
-enum { M_KSHIFT = 0, M_QSHIFT = 1, M_TSHIFT = 5, M_PSHIFT = 9, M_KMAX = 13, M_TSUM, M_GMAX, M_FMAX, M_WHOLE, M_BAD };
-static_assert(offsetof(ChunkMeta, bad) == 4 * M_BAD && offsetof(ChunkMeta, kmax) == 4 * M_KMAX, "meta words");
+enum { M_KSHIFT = 0, M_QSHIFT = 1, M_TSHIFT = 5, M_PSHIFT = 9, M_WHOLE = 13, M_EY, M_ET, M_EF, M_ES, M_EK };
+static_assert(offsetof(ChunkMeta, ek) == 4 * M_EK && offsetof(ChunkMeta, pshift) == 4 * M_PSHIFT, "meta words");
 
-__device__ inline int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
-__device__ inline __amdgpu_buffer_rsrc_t buffer(const void* p, uint32_t bytes) {
-  const uint64_t a = (uint64_t)p;
-  const uint64_t u = (uint64_t)(uint32_t)uniform((int)(uint32_t)a) | (uint64_t)(uint32_t)uniform((int)(uint32_t)(a >> 32)) << 32;
-  return __builtin_amdgcn_make_buffer_rsrc((void*)u, (short)0, (int)bytes, 0x00020000);
-}
-__device__ inline half8 load8(__amdgpu_buffer_rsrc_t r, int offset, int at) {  // `at` half8s behind byte `offset`
-  return __builtin_bit_cast(half8, __builtin_amdgcn_raw_buffer_load_b128(r, offset, 16 * at, 0));
-}
-// x, which the compiler may not keep ready beside its multiples for the whole loop (those spilled)
-__device__ inline int afresh(int x) {
-  asm volatile("" : "+v"(x));
-  return x;
-}
-
-// A sequence's chunks from u0 up to u1 (its window of the workspace) for 32 value dims of a head. The next chunk's
-// operands are loaded into the registers of this one's as soon as their last product has been issued: by
-// buffer loads, whose one lane offset and scalar rest leave the registers to the operands. (A register too many
-// costs a wait for everything in flight when it is read back: with 64-bit addresses in vector registers 14 us a
-// chunk, with the row offsets of V and the output kept through the loop 6.8.)
+// A sequence's chunks from u0 up to u1 (its window of the workspace) for 32 value dims of a head. Four waves carry
+// the state: wave w has rows 16 w .. of K S, Y and V' and a quarter of the key dims of S, all in registers; what
+// the next product needs of the others goes through LDS, three barriers a chunk. Four more waves, a SIMD's second,
+// make the output from what lies in LDS between those barriers. The next chunk's operands are loaded into the
+// registers of this one's as soon as their last product has been issued: by buffer loads, whose one lane
+// offset and scalar rest leave the registers to the operands. (A register too many costs a wait for everything
+// in flight when it is read back: with 64-bit addresses in vector registers 14 us a chunk, with the row offsets
+// of V and the output kept through the loop 6.8, without 4.0; one set of waves for all of it.)
 template <int DK, int DV, bool DELTA>
-__global__ __launch_bounds__(256, 2) void linear_chunk_scan(LinLayer L, LinBatchView b, LinAttnArgs a, int u0, int u1) {
+__global__ __launch_bounds__(512, 2) void linear_chunk_scan(LinLayer L, LinBatchView b, LinAttnArgs a, int u0, int u1) {
   using W = ChunkSpace<DK>;
   constexpr int NKB = W::NKB, MT = DK / 64, SLICES = DV / kCols;
   __shared__ half8 Sb[NKB * 2 * 2 * 64];        // the state as an operand
-  __shared__ half8 Yb[2 * 2 * 2 * 64], Vb[2 * 2 * 2 * 64], Fb[2 * 2 * 2 * 64];  // Y, V', e^(G_n - G) V'
+  __shared__ half8 Yb[2 * 2 * 2 * 64], Vb[2][2 * 2 * 2 * 64], Fb[2 * 2 * 2 * 64];  // Y, V' (of this chunk and the one before), e^(G_n - G) V'
   __shared__ uint32_t smax[4][kCols], vmax[4][kCols];
   __shared__ float plain[kCols][DK + 4];        // columns that are done row by row: the state before
   __shared__ int slow_from[kCols];              // this chunk of the sequence
@@ -433,20 +502,11 @@ __global__ __launch_bounds__(256, 2) void linear_chunk_scan(LinLayer L, LinBatch
   const int first = max(unit0, u0), last = min(unit0 + uniform(sp->n_units), u1);
   if (first >= last) return;
   const int h = kh * rep + member / SLICES, col0 = (member % SLICES) * kCols;
-  const int wave = uniform(threadIdx.x >> 6), lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
+  const int role = uniform(threadIdx.x >> 8), wave = uniform((threadIdx.x >> 6) & 3);
+  const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
   const size_t per_unit = (size_t)L.k_heads * W::PER_K + (size_t)L.v_heads * W::PER_H;
   const half8* ws = (const half8*)(b.ws ? b.ws : b.hdr->ws);
 
-  f4 S[MT][2];
-  const int from = uniform(first == unit0 ? sp->src : sp->dst);
-#pragma unroll
-  for (int i = 0; i < MT; i++)
-#pragma unroll
-    for (int nt = 0; nt < 2; nt++)
-      S[i][nt] = from >= 0 ? *(const f4*)(L.state + (((size_t)from * L.v_heads + h) * DV + col0 + 16 * nt + n) * DK + 16 * (wave * MT + i) + 4 * g)
-                           : f4{0, 0, 0, 0};
-
-  Fragments<DK> F;
   const int at_k = 16 * lane + wave * (NKB * 2 * 64 * 16), at_t = 16 * lane + wave * (2 * 2 * 64 * 16);
   static_assert(NKB == 2 * MT, "the operands of a wave's rows and of its key dims lie alike");
   auto keys = [&](int u) { return buffer(ws + (size_t)(u - u0) * per_unit + (size_t)kh * W::PER_K, 16 * W::PER_K); };
@@ -459,65 +519,128 @@ __global__ __launch_bounds__(256, 2) void linear_chunk_scan(LinLayer L, LinBatch
     const int r = kLinChunk * (u - unit0);
     return buffer(p + ((size_t)(row0 + r) * L.v_heads + h) * DV + col0, (min(kLinChunk, rows - r) - 1) * vrow + 4 * kCols);
   };
-  auto load_kq = [&](int u) {
-    const auto r = keys(u);
-#pragma unroll
-    for (int kb = 0; kb < NKB; kb++)
-#pragma unroll
-      for (int hl = 0; hl < 2; hl++) {
-        if constexpr (DELTA) F.k[kb][hl] = load8(r, at_k, W::K + (kb * 2 + hl) * 64);
-        F.q[kb][hl] = load8(r, at_k, W::Q + (kb * 2 + hl) * 64);
-      }
+  int meta;  // lane i: word i of the chunk's ChunkMeta
+  auto load_meta = [&](int u) { meta = __builtin_amdgcn_raw_buffer_load_b32(head(u), 4 * (afresh(lane) & 31), 16 * W::META, 0); };
+  auto load_fade = [&](int u, int at) {  // this wave's rows' e^G (at 0) or e^(G_n - G) (256)
+    return __builtin_bit_cast(f4, __builtin_amdgcn_raw_buffer_load_b128(head(u), 64 * wave + 16 * (afresh(lane) >> 4), 16 * W::G + at, 0));
   };
-  auto load_t = [&](int u) {
-    const auto r = head(u);
-    if constexpr (DELTA)
-#pragma unroll
-      for (int kb = 0; kb < 2; kb++)
-#pragma unroll
-        for (int hl = 0; hl < 2; hl++)
-          if (2 * kb <= wave) F.t[kb][hl] = load8(r, at_t, W::T + (kb * 2 + hl) * 64);
+  auto word = [&](int i) { return __builtin_amdgcn_readlane(meta, i); };
+  auto fword = [&](int i) { return __builtin_bit_cast(float, __builtin_amdgcn_readlane(meta, i)); };
+  // The powers of two of a chunk's columns (this lane's two), from what is noted of S and V; next_m bounds the
+  // next state. `out`: columns that are not for these products.
+  struct Shifts {
+    int y[2], v[2], f[2], s_next[2];
+    uint32_t out;
   };
-  auto load_p = [&](int u) {
-    const auto r = head(u);
+  auto shifts = [&]() {
+    Shifts t;
+    t.out = 0;
+    const int cy = word(M_EY), ct = word(M_ET), cf = word(M_EF), cs = word(M_ES), ck = word(M_EK);
 #pragma unroll
-    for (int kb = 0; kb < 2; kb++)
-#pragma unroll
-      for (int hl = 0; hl < 2; hl++)
-        if (2 * kb <= wave) F.p[kb][hl] = load8(r, at_t, W::P + (kb * 2 + hl) * 64);
+    for (int nt = 0; nt < 2; nt++) {
+      const int c = 16 * nt + n;
+      const uint32_t sm = max(max(smax[0][c], smax[1][c]), max(smax[2][c], smax[3][c]));
+      const uint32_t vm = max(max(vmax[0][c], vmax[1][c]), max(vmax[2][c], vmax[3][c]));
+      // powers of two above them (of nothing: what adds nothing to a maximum)
+      const int es = sm ? top_exponent(__uint_as_float(sm)) : -200, ev = vm ? top_exponent(__uint_as_float(vm)) : -200;
+      const int ey = DELTA ? max(ev, es + cy) + 1 : ev, evp = ey + ct, ef = evp + cf, en = max(es + cs, ef + ck) + 1;
+      t.y[nt] = kTop - ey;
+      t.v[nt] = kTop - evp;
+      t.f[nt] = kTop - ef;
+      t.s_next[nt] = kTop - en;
+      const bool out = max(sm, vm) >= kInf || max(max(es, ey), max(evp, en)) >= 120 || cy >= kBad / 2;
+      t.out |= (uint32_t)(__ballot(out) & 0xffffu) << (16 * nt);
+    }
+    t.out = uniform(t.out);
+    return t;
   };
-  auto load_kt = [&](int u) {
-    const auto r = keys(u);
-#pragma unroll
-    for (int i = 0; i < MT; i++)
-#pragma unroll
-      for (int kb = 0; kb < 2; kb++)
-#pragma unroll
-        for (int hl = 0; hl < 2; hl++) F.kt[i][kb][hl] = load8(r, at_k, W::KT + ((i * 2 + kb) * 2 + hl) * 64);
+  auto first_shift = [&](int nt) {
+    const int c = 16 * nt + n;
+    return shift_for(__uint_as_float(max(max(smax[0][c], smax[1][c]), max(smax[2][c], smax[3][c]))));
   };
-  auto load_v = [&](int u) {
+  auto load_v = [&](int u, float (&to)[2][4]) {
     const auto r = values(a.v, u);
     int at = afresh(vlane);
 #pragma unroll
     for (int e = 0; e < 4; e++, at += vrow)
 #pragma unroll
-      for (int nt = 0; nt < 2; nt++) F.v[nt][e] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(r, at + 64 * nt, 0, 0));
+      for (int nt = 0; nt < 2; nt++) to[nt][e] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(r, at + 64 * nt, 0, 0));
   };
-  auto load_meta = [&](int u) {
-    const auto r = head(u);
-    const int l = afresh(lane), at = 64 * wave + 16 * (l >> 4);
-    F.eg = __builtin_bit_cast(f4, __builtin_amdgcn_raw_buffer_load_b128(r, at, 16 * W::G, 0));
-    F.fg = __builtin_bit_cast(f4, __builtin_amdgcn_raw_buffer_load_b128(r, at, 16 * W::G + 256, 0));
-    F.meta = __builtin_amdgcn_raw_buffer_load_b32(r, 4 * (l & 31), 16 * W::META, 0);
+  auto operands = [&](const half8* from, int kb, half8 (&hi)[2], half8 (&lo)[2]) {  // both column tiles
+#pragma unroll
+    for (int nt = 0; nt < 2; nt++) {
+      hi[nt] = from[((kb * 2 + nt) * 2 + 0) * 64 + lane];
+      lo[nt] = from[((kb * 2 + nt) * 2 + 1) * 64 + lane];
+    }
   };
-  auto word = [&](int i) { return __builtin_amdgcn_readlane(F.meta, i); };
-  auto fword = [&](int i) { return __builtin_bit_cast(float, __builtin_amdgcn_readlane(F.meta, i)); };
-  load_meta(first);
-  load_kq(first);
-  load_v(first);
-  load_kt(first);
+  uint32_t slow = 0;  // the columns that are done row by row
+  int sshift[2];
+  f4 S[MT][2];
 
-  auto note_state = [&]() {  // the largest |S| of each column over this wave's key dims
+  if (role == 0) {
+    __builtin_amdgcn_s_setprio(2);  // the state is what everything waits for
+    half8 fk[NKB][2], ft[2][2], fkt[MT][2][2];
+    float v[2][2][4];  // this chunk's and the next one's
+    f4 eg, fg;
+    auto load_k = [&](int u) {
+      const auto r = keys(u);
+      if constexpr (DELTA)
+#pragma unroll
+        for (int kb = 0; kb < NKB; kb++)
+#pragma unroll
+          for (int hl = 0; hl < 2; hl++) fk[kb][hl] = load8(r, at_k, W::K + (kb * 2 + hl) * 64);
+    };
+    auto load_t = [&](int u) {
+      const auto r = head(u);
+      if constexpr (DELTA)
+#pragma unroll
+        for (int kb = 0; kb < 2; kb++)
+#pragma unroll
+          for (int hl = 0; hl < 2; hl++)
+            if (2 * kb <= wave) ft[kb][hl] = load8(r, at_t, W::T + (kb * 2 + hl) * 64);
+    };
+    auto load_kt = [&](int u) {
+      const auto r = keys(u);
+#pragma unroll
+      for (int i = 0; i < MT; i++)
+#pragma unroll
+        for (int kb = 0; kb < 2; kb++)
+#pragma unroll
+          for (int hl = 0; hl < 2; hl++) fkt[i][kb][hl] = load8(r, at_k, W::KT + ((i * 2 + kb) * 2 + hl) * 64);
+    };
+    auto note = [&](int nt, uint32_t t) {  // a column's largest over this wave's key dims
+      t = groups_max(t);
+      const int l = afresh(lane);
+      if (l < 16) smax[wave][16 * nt + l] = t;
+    };
+    auto put4 = [&](half8* to, int tile, int nt, float a, float b, float c, float d) {
+      u2 hi, lo;
+      split4(a, b, c, d, hi, lo);
+      char* p = (char*)(to + (((tile >> 1) * 2 + nt) * 2) * 64 + lane) + 8 * (tile & 1);
+      *(u2*)p = hi;
+      *(u2*)(p + 64 * 16) = lo;
+    };
+    auto put_state = [&]() {
+#pragma unroll
+      for (int i = 0; i < MT; i++)
+#pragma unroll
+        for (int nt = 0; nt < 2; nt++) put4(Sb, wave * MT + i, nt, S[i][nt][0], S[i][nt][1], S[i][nt][2], S[i][nt][3]);
+    };
+    const int from = uniform(first == unit0 ? sp->src : sp->dst);
+#pragma unroll
+    for (int i = 0; i < MT; i++)
+#pragma unroll
+      for (int nt = 0; nt < 2; nt++)
+        S[i][nt] = from >= 0 ? *(const f4*)(L.state + (((size_t)from * L.v_heads + h) * DV + col0 + 16 * nt + n) * DK + 16 * (wave * MT + i) + 4 * g)
+                             : f4{0, 0, 0, 0};
+    load_v(first, v[0]);
+    load_meta(first);
+    load_k(first);
+    eg = load_fade(first, 0);
+    fg = load_fade(first, 256);
+    load_t(first);
+    load_kt(first);
+    load_v(min(first + 1, last - 1), v[1]);
 #pragma unroll
     for (int nt = 0; nt < 2; nt++) {
       uint32_t t = 0;
@@ -525,211 +648,260 @@ __global__ __launch_bounds__(256, 2) void linear_chunk_scan(LinLayer L, LinBatch
       for (int i = 0; i < MT; i++)
 #pragma unroll
         for (int r = 0; r < 4; r++) t = max(t, mag(S[i][nt][r]));
-      t = groups_max(t);
-      const int l = afresh(lane);
-      if (l < 16) smax[wave][16 * nt + l] = t;
+      note(nt, t);
     }
-  };
-  auto note_v = [&]() {
-#pragma unroll
-    for (int nt = 0; nt < 2; nt++) {
-      uint32_t t = 0;
-#pragma unroll
-      for (int r = 0; r < 4; r++) t = max(t, mag(F.v[nt][r]));
-      t = groups_max(t);
-      const int l = afresh(lane);
-      if (l < 16) vmax[wave][16 * nt + l] = t;
-    }
-  };
-  auto put4 = [&](half8* to, int tile, int nt, const float (&x)[4], int shift) {
-    float y[4];
-    half4 hi, lo;
-#pragma unroll
-    for (int r = 0; r < 4; r++) y[r] = ldexpf(x[r], shift);
-    split4(y, hi, lo);
-    char* p = (char*)(to + (((tile >> 1) * 2 + nt) * 2) * 64 + lane) + 8 * (tile & 1);
-    *(half4*)p = hi;
-    *(half4*)(p + 64 * 16) = lo;
-  };
-  int sshift[2];
-  auto put_state = [&]() {
-#pragma unroll
-    for (int i = 0; i < MT; i++)
-#pragma unroll
-      for (int nt = 0; nt < 2; nt++) {
-        const float y[4] = {S[i][nt][0], S[i][nt][1], S[i][nt][2], S[i][nt][3]};
-        put4(Sb, wave * MT + i, nt, y, sshift[nt]);
-      }
-  };
-  note_state();
-  note_v();
-  __syncthreads();
-#pragma unroll
-  for (int nt = 0; nt < 2; nt++) {
-    const int c = 16 * nt + n;
-    sshift[nt] = shift_for(__uint_as_float(max(max(smax[0][c], smax[1][c]), max(smax[2][c], smax[3][c]))));
-  }
-  put_state();
-
-  uint32_t slow = 0;  // the columns that are done row by row
-#pragma unroll 1
-  for (int u = first; u < last; u++) {
-    const int next = min(u + 1, last - 1);
-    const int kshift = word(M_KSHIFT), qshift = word(M_QSHIFT + wave), tshift = word(M_TSHIFT + wave), pshift = word(M_PSHIFT + wave);
-    const float whole = fword(M_WHOLE);
-    __syncthreads();  // the state, and what is noted of it and of V
-    int yshift[2], vshift[2], fshift[2], sshift_next[2];
-    uint32_t todo = 0;  // columns that are not for these products
-    {
-      const bool bad = word(M_BAD);
-      const float kmax = fword(M_KMAX), tsum = fword(M_TSUM), gmax = fword(M_GMAX), fmax_ = fword(M_FMAX);
-#pragma unroll
-      for (int nt = 0; nt < 2; nt++) {
-        const int c = 16 * nt + n;
-        const float sm = __uint_as_float(max(max(smax[0][c], smax[1][c]), max(smax[2][c], smax[3][c])));
-        const float vm = __uint_as_float(max(max(vmax[0][c], vmax[1][c]), max(vmax[2][c], vmax[3][c])));
-        const float ym = vm + (DELTA ? gmax * (DK * kmax) * sm : 0.0f);
-        const float vpm = tsum * ym, fm = fmax_ * vpm;
-        const float next_m = whole * sm + kLinChunk * kmax * fm;
-        yshift[nt] = shift_for(ym);
-        vshift[nt] = shift_for(vpm);
-        fshift[nt] = shift_for(fm);
-        sshift_next[nt] = shift_for(next_m);
-        const bool out = bad || !(next_m < 0x1p120f) || !(ym < 0x1p120f) || !(vpm < 0x1p120f) || !(sm < 0x1p120f);
-        todo |= (uint32_t)(__ballot(out) & 0xffffu) << (16 * nt);
-      }
-      todo = uniform(todo);
-    }
-    todo &= ~slow;
-    if (todo) {  // columns that leave the chunks here
-      const int l = afresh(lane);
-#pragma unroll
-      for (int nt = 0; nt < 2; nt++) {
-        const int c = 16 * nt + (l & 15);
-        if (!(todo >> c & 1)) continue;
-#pragma unroll
-        for (int i = 0; i < MT; i++) *(f4*)&plain[c][16 * (wave * MT + i) + 4 * (l >> 4)] = S[i][nt];
-        if (wave == 0) slow_from[c] = u - unit0;
-      }
-      slow |= todo;
-    }
-
-    __builtin_amdgcn_sched_barrier(0);
-    load_t(u);
-    __builtin_amdgcn_sched_barrier(0);
-    // K S and Q S
-    f4 ks[2], o[2];
-#pragma unroll
-    for (int nt = 0; nt < 2; nt++) ks[nt] = o[nt] = f4{0, 0, 0, 0};
-#pragma unroll
-    for (int kb = 0; kb < NKB; kb++)
-#pragma unroll
-      for (int nt = 0; nt < 2; nt++) {
-        const half8 sh = Sb[((kb * 2 + nt) * 2 + 0) * 64 + lane], sl = Sb[((kb * 2 + nt) * 2 + 1) * 64 + lane];
-        if constexpr (DELTA) ks[nt] = product3(F.k[kb][0], F.k[kb][1], sh, sl, ks[nt]);
-        o[nt] = product3(F.q[kb][0], F.q[kb][1], sh, sl, o[nt]);
-      }
-    __builtin_amdgcn_sched_barrier(0);
-    load_p(u);
-    load_kq(next);
-    __builtin_amdgcn_sched_barrier(0);
-    f4 vp[2];
-    if constexpr (DELTA) {
-#pragma unroll
-      for (int nt = 0; nt < 2; nt++) {
-        float y[4];
-#pragma unroll
-        for (int r = 0; r < 4; r++) y[r] = F.v[nt][r] - F.eg[r] * ldexpf(ks[nt][r], -kshift - sshift[nt]);
-        put4(Yb, wave, nt, y, yshift[nt]);
-      }
-      __syncthreads();
-#pragma unroll
-      for (int nt = 0; nt < 2; nt++) {
-        vp[nt] = f4{0, 0, 0, 0};
-#pragma unroll
-        for (int kb = 0; kb < 2; kb++)
-          if (2 * kb <= wave)
-            vp[nt] = product3(F.t[kb][0], F.t[kb][1], Yb[((kb * 2 + nt) * 2 + 0) * 64 + lane], Yb[((kb * 2 + nt) * 2 + 1) * 64 + lane], vp[nt]);
-      }
-#pragma unroll
-      for (int nt = 0; nt < 2; nt++)
-#pragma unroll
-        for (int r = 0; r < 4; r++) vp[nt][r] = ldexpf(vp[nt][r], -tshift - yshift[nt]);
-    } else {
-#pragma unroll
-      for (int nt = 0; nt < 2; nt++)
-#pragma unroll
-        for (int r = 0; r < 4; r++) vp[nt][r] = F.v[nt][r];
-    }
-#pragma unroll
-    for (int nt = 0; nt < 2; nt++) {
-      const float y[4] = {vp[nt][0], vp[nt][1], vp[nt][2], vp[nt][3]};
-      const float z[4] = {F.fg[0] * y[0], F.fg[1] * y[1], F.fg[2] * y[2], F.fg[3] * y[3]};
-      put4(Vb, wave, nt, y, vshift[nt]);
-      put4(Fb, wave, nt, z, fshift[nt]);
-    }
-#pragma unroll
-    for (int nt = 0; nt < 2; nt++)
-#pragma unroll
-      for (int r = 0; r < 4; r++) o[nt][r] = F.eg[r] * ldexpf(o[nt][r], -qshift - sshift[nt]);
-    __builtin_amdgcn_sched_barrier(0);
-    load_v(next);
-    load_meta(next);
-    __builtin_amdgcn_sched_barrier(0);
     __syncthreads();
-    // the state
-#pragma unroll
-    for (int i = 0; i < MT; i++)
-#pragma unroll
-      for (int nt = 0; nt < 2; nt++) {
-        f4 acc = f4{0, 0, 0, 0};
-#pragma unroll
-        for (int kb = 0; kb < 2; kb++)
-          acc = product3(F.kt[i][kb][0], F.kt[i][kb][1], Fb[((kb * 2 + nt) * 2 + 0) * 64 + lane], Fb[((kb * 2 + nt) * 2 + 1) * 64 + lane], acc);
-#pragma unroll
-        for (int r = 0; r < 4; r++) S[i][nt][r] = fmaf(whole, S[i][nt][r], ldexpf(acc[r], -kshift - fshift[nt]));
-      }
-    __builtin_amdgcn_sched_barrier(0);
-    load_kt(next);
-    __builtin_amdgcn_sched_barrier(0);
-    // the output
-    const auto ro = values(a.out, u);
+    // from here on S holds the state times 2^sshift
 #pragma unroll
     for (int nt = 0; nt < 2; nt++) {
-      f4 acc = f4{0, 0, 0, 0};
+      sshift[nt] = first_shift(nt);
+#pragma unroll
+      for (int i = 0; i < MT; i++)
+#pragma unroll
+        for (int r = 0; r < 4; r++) S[i][nt][r] = ldexpf(S[i][nt][r], sshift[nt]);
+    }
+    put_state();
+#pragma unroll 1
+    for (int u = first; u < last; u++) {
+      const int next = min(u + 1, last - 1);
+      const int kshift = word(M_KSHIFT), tshift = word(M_TSHIFT + wave);
+      const float whole = fword(M_WHOLE);
+      __syncthreads();  // the state, and what is noted of it and of V
+      const Shifts sh = shifts();
+      load_meta(next);
+      f4 vp[2];
+      if constexpr (DELTA) {
+        f4 ks[2] = {f4{0, 0, 0, 0}, f4{0, 0, 0, 0}};
+#pragma unroll
+        for (int kb = 0; kb < NKB; kb++) {
+          half8 hi[2], lo[2];
+          operands(Sb, kb, hi, lo);
+          products3(fk[kb][0], fk[kb][1], hi, lo, ks);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        load_k(next);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int nt = 0; nt < 2; nt++) {
+          // Y 2^y, the product's own powers in one factor: below 2^-149 its share is nothing beside Y's bound
+          const float f = ldexpf(1.0f, sh.y[nt] - kshift - sshift[nt]);
+          float y[4];
+#pragma unroll
+          for (int r = 0; r < 4; r++) y[r] = fmaf(-(eg[r] * f), ks[nt][r], ldexpf(v[0][nt][r], sh.y[nt]));
+          put4(Yb, wave, nt, y[0], y[1], y[2], y[3]);
+        }
+        eg = load_fade(next, 0);
+        __syncthreads();
+        vp[0] = vp[1] = f4{0, 0, 0, 0};
+#pragma unroll
+        for (int kb = 0; kb < 2; kb++)
+          if (2 * kb <= wave) {
+            half8 hi[2], lo[2];
+            operands(Yb, kb, hi, lo);
+            products3(ft[kb][0], ft[kb][1], hi, lo, vp);
+          }
+        __builtin_amdgcn_sched_barrier(0);
+        load_t(next);
+        __builtin_amdgcn_sched_barrier(0);
+      } else {
+#pragma unroll
+        for (int nt = 0; nt < 2; nt++)
+#pragma unroll
+          for (int r = 0; r < 4; r++) vp[nt][r] = v[0][nt][r];
+      }
+      // V' as it is held: times 2^held
+      const int held[2] = {DELTA ? tshift + sh.y[0] : 0, DELTA ? tshift + sh.y[1] : 0};
+#pragma unroll
+      for (int nt = 0; nt < 2; nt++) {
+        const float f = ldexpf(1.0f, sh.f[nt] - held[nt]);
+        put4(Fb, wave, nt, fg[0] * f * vp[nt][0], fg[1] * f * vp[nt][1], fg[2] * f * vp[nt][2], fg[3] * f * vp[nt][3]);
+      }
+      fg = load_fade(next, 256);
+      __syncthreads();
+      f4 acc[MT][2];
+#pragma unroll
+      for (int i = 0; i < MT; i++) acc[i][0] = acc[i][1] = f4{0, 0, 0, 0};
+#pragma unroll
+      for (int kb = 0; kb < 2; kb++) {
+        half8 hi[2], lo[2];
+        operands(Fb, kb, hi, lo);
+#pragma unroll
+        for (int i = 0; i < MT; i++) products3(fkt[i][kb][0], fkt[i][kb][1], hi, lo, acc[i]);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+      load_kt(next);
+      __builtin_amdgcn_sched_barrier(0);
+      if (const uint32_t todo = sh.out & ~slow) {  // columns that leave the chunks here
+        const int l = afresh(lane);
+#pragma unroll
+        for (int nt = 0; nt < 2; nt++) {
+          const int c = 16 * nt + (l & 15);
+          if (!(todo >> c & 1)) continue;
+#pragma unroll
+          for (int i = 0; i < MT; i++)
+#pragma unroll
+            for (int r = 0; r < 4; r++) plain[c][16 * (wave * MT + i) + 4 * (l >> 4) + r] = ldexpf(S[i][nt][r], -sshift[nt]);
+          if (wave == 0) slow_from[c] = u - unit0;
+        }
+        slow |= todo;
+      }
+#pragma unroll
+      for (int nt = 0; nt < 2; nt++) {
+        const float f = ldexpf(1.0f, sh.s_next[nt] - kshift - sh.f[nt]), w = ldexpf(whole, sh.s_next[nt] - sshift[nt]);
+        float t = 0.0f;
+#pragma unroll
+        for (int i = 0; i < MT; i++) {
+#pragma unroll
+          for (int r = 0; r < 4; r++) S[i][nt][r] = fmaf(f, acc[i][nt][r], w * S[i][nt][r]);
+#pragma unroll
+          for (int r = 0; r < 4; r++) t = fmaxf(t, fabsf(S[i][nt][r]));
+        }
+        sshift[nt] = sh.s_next[nt];
+        note(nt, __float_as_uint(ldexpf(t, -sshift[nt])));
+#pragma unroll
+        for (int r = 0; r < 4; r++) v[0][nt][r] = moved(v[1][nt][r]);
+      }
+      put_state();
+      // V' for the output waves, which take it behind the next barrier
+#pragma unroll
+      for (int nt = 0; nt < 2; nt++) {
+        const int e = sh.v[nt] - held[nt];
+        put4(Vb[u & 1], wave, nt, ldexpf(vp[nt][0], e), ldexpf(vp[nt][1], e), ldexpf(vp[nt][2], e), ldexpf(vp[nt][3], e));
+      }
+      __builtin_amdgcn_sched_barrier(0);
+      load_v(min(u + 2, last - 1), v[1]);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    __syncthreads();
+  } else {
+    half8 fq[NKB][2], fp[2][2];
+    f4 eg;
+    auto load_q = [&](int u) {
+      const auto r = keys(u);
+#pragma unroll
+      for (int kb = 0; kb < NKB; kb++)
+#pragma unroll
+        for (int hl = 0; hl < 2; hl++) fq[kb][hl] = load8(r, at_k, W::Q + (kb * 2 + hl) * 64);
+    };
+    auto load_p = [&](int u) {
+      const auto r = head(u);
 #pragma unroll
       for (int kb = 0; kb < 2; kb++)
-        if (2 * kb <= wave)
-          acc = product3(F.p[kb][0], F.p[kb][1], Vb[((kb * 2 + nt) * 2 + 0) * 64 + lane], Vb[((kb * 2 + nt) * 2 + 1) * 64 + lane], acc);
 #pragma unroll
-      for (int r = 0; r < 4; r++) o[nt][r] = a.scale * (o[nt][r] + ldexpf(acc[r], -pshift - vshift[nt]));
-    }
-    {
+        for (int hl = 0; hl < 2; hl++)
+          if (2 * kb <= wave) fp[kb][hl] = load8(r, at_t, W::P + (kb * 2 + hl) * 64);
+    };
+    auto note_v = [&](const float (&of)[2][4]) {
+#pragma unroll
+      for (int nt = 0; nt < 2; nt++) {
+        uint32_t t = 0;
+#pragma unroll
+        for (int r = 0; r < 4; r++) t = max(t, mag(of[nt][r]));
+        t = groups_max(t);
+        const int l = afresh(lane);
+        if (l < 16) vmax[wave][16 * nt + l] = t;
+      }
+    };
+    float v[2][4];
+    f4 o[2];
+    // what V' adds to the rows of chunk u, and their store, but for the columns `left_out`
+    auto finish = [&](int u, int pshift, const int (&vshift)[2], uint32_t left_out) {
+      const auto ro = values(a.out, u);
+      f4 acc[2] = {f4{0, 0, 0, 0}, f4{0, 0, 0, 0}};
+#pragma unroll
+      for (int kb = 0; kb < 2; kb++)
+        if (2 * kb <= wave) {
+          half8 hi[2], lo[2];
+          operands(Vb[u & 1], kb, hi, lo);
+          products3(fp[kb][0], fp[kb][1], hi, lo, acc);
+        }
+#pragma unroll
+      for (int nt = 0; nt < 2; nt++) {
+        const float f = a.scale * ldexpf(1.0f, -pshift - vshift[nt]);
+#pragma unroll
+        for (int r = 0; r < 4; r++) acc[nt][r] = fmaf(f, acc[nt][r], o[nt][r]);
+      }
       int at = afresh(vlane);
-      const bool on[2] = {!(slow >> n & 1), !(slow >> (16 + n) & 1)};
+      const bool on[2] = {!(left_out >> n & 1), !(left_out >> (16 + n) & 1)};
 #pragma unroll
       for (int r = 0; r < 4; r++, at += vrow)
 #pragma unroll
         for (int nt = 0; nt < 2; nt++)
-          if (on[nt]) __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(o[nt][r]), ro, at + 64 * nt, 0, 0);
-    }
-    note_state();
-    note_v();
+          if (on[nt]) __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(acc[nt][r]), ro, at + 64 * nt, 0, 0);
+    };
+    load_v(first, v);
+    load_meta(first);
+    load_q(first);
+    eg = load_fade(first, 0);
+    load_p(first);
+    note_v(v);
+    load_v(min(first + 1, last - 1), v);
+    __syncthreads();
 #pragma unroll
-    for (int nt = 0; nt < 2; nt++) sshift[nt] = sshift_next[nt];
-    put_state();
+    for (int nt = 0; nt < 2; nt++) sshift[nt] = first_shift(nt);
+    int vshift[2] = {0, 0}, pshift = 0;
+#pragma unroll 1
+    for (int u = first; u < last; u++) {
+      const int next = min(u + 1, last - 1);
+      __syncthreads();
+      const Shifts sh = shifts();
+      const int qshift = word(M_QSHIFT + wave), pshift_now = word(M_PSHIFT + wave);
+      load_meta(next);
+      f4 now[2] = {f4{0, 0, 0, 0}, f4{0, 0, 0, 0}};
+#pragma unroll
+      for (int kb = 0; kb < NKB; kb++) {
+        half8 hi[2], lo[2];
+        operands(Sb, kb, hi, lo);
+        products3(fq[kb][0], fq[kb][1], hi, lo, now);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+      load_q(next);
+      __builtin_amdgcn_sched_barrier(0);
+      if constexpr (DELTA) __syncthreads();
+      // the state waves hurry from here to the third barrier: the chunk before is finished behind it
+#pragma unroll
+      for (int nt = 0; nt < 2; nt++) {
+        const float f = a.scale * ldexpf(1.0f, -qshift - sshift[nt]);
+#pragma unroll
+        for (int r = 0; r < 4; r++) now[nt][r] = eg[r] * (f * now[nt][r]);
+      }
+      eg = load_fade(next, 0);
+      __syncthreads();
+      note_v(v);
+      __builtin_amdgcn_sched_barrier(0);
+      load_v(min(u + 2, last - 1), v);
+      __builtin_amdgcn_sched_barrier(0);
+      if (u > first) {
+        finish(u - 1, pshift, vshift, slow);
+        __builtin_amdgcn_sched_barrier(0);
+        load_p(u);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+#pragma unroll
+      for (int nt = 0; nt < 2; nt++) {
+        o[nt] = now[nt];
+        vshift[nt] = sh.v[nt];
+        sshift[nt] = sh.s_next[nt];
+      }
+      pshift = pshift_now;
+      slow |= sh.out;
+    }
+    __syncthreads();
+    finish(last - 1, pshift, vshift, slow);
   }
   float* left = L.state + (((size_t)uniform(sp->dst) * L.v_heads + h) * DV + col0) * DK;
+  if (role == 0)
 #pragma unroll
-  for (int i = 0; i < MT; i++)
+    for (int i = 0; i < MT; i++)
 #pragma unroll
-    for (int nt = 0; nt < 2; nt++)
-      if (!(slow >> (16 * nt + n) & 1)) *(f4*)(left + (16 * nt + n) * DK + 16 * (wave * MT + i) + 4 * g) = S[i][nt];
+      for (int nt = 0; nt < 2; nt++)
+        if (!(slow >> (16 * nt + n) & 1)) *(f4*)(left + (16 * nt + n) * DK + 16 * (wave * MT + i) + 4 * g) =
+              f4{ldexpf(S[i][nt][0], -sshift[nt]), ldexpf(S[i][nt][1], -sshift[nt]), ldexpf(S[i][nt][2], -sshift[nt]), ldexpf(S[i][nt][3], -sshift[nt])};
   if (!slow) return;
   // the other columns, eight lanes each, as linear_attn.hip does them
   __syncthreads();
   const int c = threadIdx.x >> 3, l = threadIdx.x & 7;
-  if (!(slow >> c & 1)) return;
+  if (role || !(slow >> c & 1)) return;
   f4 st[DK / 32];
 #pragma unroll
   for (int i = 0; i < DK / 32; i++) st[i] = *(const f4*)&plain[c][32 * i + 4 * l];
@@ -797,7 +969,7 @@ hipError_t launch_t(const LinLayer& L, const LinBatchView& b, const LinAttnArgs&
   for (int u0 = 0; u0 < b.n_chunk_units; u0 += b.window) {
     const int u1 = std::min(u0 + b.window, b.n_chunk_units);
     hipLaunchKernelGGL((linear_chunk_prepare<DK, DELTA>), dim3(u1 - u0, L.k_heads), dim3(256), 0, st, L, b, a, u0);
-    hipLaunchKernelGGL((linear_chunk_scan<DK, DV, DELTA>), dim3(8 * ((groups + 7) / 8) * members), dim3(256), 0, st, L, b, a, u0, u1);
+    hipLaunchKernelGGL((linear_chunk_scan<DK, DV, DELTA>), dim3(8 * ((groups + 7) / 8) * members), dim3(512), 0, st, L, b, a, u0, u1);
   }
   if (a.norm) hipLaunchKernelGGL((linear_norm_kernel<DV>), dim3(b.n_chunk_units, std::min(8, L.v_heads)), dim3(256), 0, st, L, b, a);
   return hipGetLastError();
