@@ -33,7 +33,7 @@ typedef _Float16 half8 __attribute__((ext_vector_type(8)));
 typedef float f4 __attribute__((ext_vector_type(4)));
 
 constexpr int kTop = 14;      // an operand's largest value is below 2^kTop
-constexpr int kCols = 32;     // value dims of a scan workgroup
+constexpr int kFewScans = 256;   // workgroups of 32 value dims of the sum rule's scan
 constexpr int kBad = 1 << 20;
 constexpr int kPad = 68;      // row stride of 64 x 64 matrices in LDS
 constexpr double kLowest = -1e4;  // of a log decay: e^g is 0 in f32 from -104 on
@@ -474,7 +474,7 @@ __global__ __launch_bounds__(256, 4) void linear_chunk_prepare(LinLayer L, LinBa
 enum { M_KSHIFT = 0, M_QSHIFT = 1, M_TSHIFT = 5, M_PSHIFT = 9, M_WHOLE = 13, M_EY, M_ET, M_EF, M_ES, M_EK };
 static_assert(offsetof(ChunkMeta, ek) == 4 * M_EK && offsetof(ChunkMeta, pshift) == 4 * M_PSHIFT, "meta words");
 
-// A sequence's chunks from u0 up to u1 (its window of the workspace) for 32 value dims of a head. Four waves carry
+// A sequence's chunks from u0 up to u1 (its window of the workspace) for 16 NT value dims of a head. Four waves carry
 // the state: wave w has rows 16 w .. of K S, Y and V' and a quarter of the key dims of S, all in registers; what
 // the next product needs of the others goes through LDS, three barriers a chunk. Four more waves, a SIMD's second,
 // make the output from what lies in LDS between those barriers. The next chunk's operands are loaded into the
@@ -482,12 +482,12 @@ static_assert(offsetof(ChunkMeta, ek) == 4 * M_EK && offsetof(ChunkMeta, pshift)
 // offset and scalar rest leave the registers to the operands. (A register too many costs a wait for everything
 // in flight when it is read back: with 64-bit addresses in vector registers 14 us a chunk, with the row offsets
 // of V and the output kept through the loop 6.8, without 4.0; one set of waves for all of it.)
-template <int DK, int DV, bool DELTA>
-__global__ __launch_bounds__(512, 2) void linear_chunk_scan(LinLayer L, LinBatchView b, LinAttnArgs a, int u0, int u1) {
+template <int DK, int DV, bool DELTA, int NT>
+__global__ __launch_bounds__(512, NT == 1 ? 4 : 2) void linear_chunk_scan(LinLayer L, LinBatchView b, LinAttnArgs a, int u0, int u1) {
   using W = ChunkSpace<DK>;
-  constexpr int NKB = W::NKB, MT = DK / 64, SLICES = DV / kCols;
-  __shared__ half8 Sb[NKB * 2 * 2 * 64];        // the state as an operand
-  __shared__ half8 Yb[2 * 2 * 2 * 64], Vb[2][2 * 2 * 2 * 64], Fb[2 * 2 * 2 * 64];  // Y, V' (of this chunk and the one before), e^(G_n - G) V'
+  constexpr int NKB = W::NKB, MT = DK / 64, kCols = 16 * NT, SLICES = DV / kCols;
+  __shared__ half8 Sb[NKB * NT * 2 * 64];        // the state as an operand
+  __shared__ half8 Yb[2 * NT * 2 * 64], Vb[2][2 * NT * 2 * 64], Fb[2 * NT * 2 * 64];  // Y, V' (of this chunk and the one before), e^(G_n - G) V'
   __shared__ uint32_t smax[4][kCols], vmax[4][kCols];
   __shared__ float plain[kCols][DK + 4];        // columns that are done row by row: the state before
   __shared__ int slow_from[kCols];              // this chunk of the sequence
@@ -529,7 +529,7 @@ __global__ __launch_bounds__(512, 2) void linear_chunk_scan(LinLayer L, LinBatch
   // The powers of two of a chunk's columns (this lane's two), from what is noted of S and V; next_m bounds the
   // next state. `out`: columns that are not for these products.
   struct Shifts {
-    int y[2], v[2], f[2], s_next[2];
+    int y[NT], v[NT], f[NT], s_next[NT];
     uint32_t out;
   };
   auto shifts = [&]() {
@@ -537,7 +537,7 @@ __global__ __launch_bounds__(512, 2) void linear_chunk_scan(LinLayer L, LinBatch
     t.out = 0;
     const int cy = word(M_EY), ct = word(M_ET), cf = word(M_EF), cs = word(M_ES), ck = word(M_EK);
 #pragma unroll
-    for (int nt = 0; nt < 2; nt++) {
+    for (int nt = 0; nt < NT; nt++) {
       const int c = 16 * nt + n;
       const uint32_t sm = max(max(smax[0][c], smax[1][c]), max(smax[2][c], smax[3][c]));
       const uint32_t vm = max(max(vmax[0][c], vmax[1][c]), max(vmax[2][c], vmax[3][c]));
@@ -558,29 +558,29 @@ __global__ __launch_bounds__(512, 2) void linear_chunk_scan(LinLayer L, LinBatch
     const int c = 16 * nt + n;
     return shift_for(__uint_as_float(max(max(smax[0][c], smax[1][c]), max(smax[2][c], smax[3][c]))));
   };
-  auto load_v = [&](int u, float (&to)[2][4]) {
+  auto load_v = [&](int u, float (&to)[NT][4]) {
     const auto r = values(a.v, u);
     int at = afresh(vlane);
 #pragma unroll
     for (int e = 0; e < 4; e++, at += vrow)
 #pragma unroll
-      for (int nt = 0; nt < 2; nt++) to[nt][e] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(r, at + 64 * nt, 0, 0));
+      for (int nt = 0; nt < NT; nt++) to[nt][e] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(r, at + 64 * nt, 0, 0));
   };
-  auto operands = [&](const half8* from, int kb, half8 (&hi)[2], half8 (&lo)[2]) {  // both column tiles
+  auto operands = [&](const half8* from, int kb, half8 (&hi)[NT], half8 (&lo)[NT]) {  // both column tiles
 #pragma unroll
-    for (int nt = 0; nt < 2; nt++) {
-      hi[nt] = from[((kb * 2 + nt) * 2 + 0) * 64 + lane];
-      lo[nt] = from[((kb * 2 + nt) * 2 + 1) * 64 + lane];
+    for (int nt = 0; nt < NT; nt++) {
+      hi[nt] = from[((kb * NT + nt) * 2 + 0) * 64 + lane];
+      lo[nt] = from[((kb * NT + nt) * 2 + 1) * 64 + lane];
     }
   };
   uint32_t slow = 0;  // the columns that are done row by row
-  int sshift[2];
-  f4 S[MT][2];
+  int sshift[NT];
+  f4 S[MT][NT];
 
   if (role == 0) {
     __builtin_amdgcn_s_setprio(2);  // the state is what everything waits for
     half8 fk[NKB][2], ft[2][2], fkt[MT][2][2];
-    float v[2][2][4];  // this chunk's and the next one's
+    float v[2][NT][4];  // this chunk's and the next one's
     f4 eg, fg;
     auto load_k = [&](int u) {
       const auto r = keys(u);
@@ -616,7 +616,7 @@ __global__ __launch_bounds__(512, 2) void linear_chunk_scan(LinLayer L, LinBatch
     auto put4 = [&](half8* to, int tile, int nt, float a, float b, float c, float d) {
       u2 hi, lo;
       split4(a, b, c, d, hi, lo);
-      char* p = (char*)(to + (((tile >> 1) * 2 + nt) * 2) * 64 + lane) + 8 * (tile & 1);
+      char* p = (char*)(to + (((tile >> 1) * NT + nt) * 2) * 64 + lane) + 8 * (tile & 1);
       *(u2*)p = hi;
       *(u2*)(p + 64 * 16) = lo;
     };
@@ -624,13 +624,13 @@ __global__ __launch_bounds__(512, 2) void linear_chunk_scan(LinLayer L, LinBatch
 #pragma unroll
       for (int i = 0; i < MT; i++)
 #pragma unroll
-        for (int nt = 0; nt < 2; nt++) put4(Sb, wave * MT + i, nt, S[i][nt][0], S[i][nt][1], S[i][nt][2], S[i][nt][3]);
+        for (int nt = 0; nt < NT; nt++) put4(Sb, wave * MT + i, nt, S[i][nt][0], S[i][nt][1], S[i][nt][2], S[i][nt][3]);
     };
     const int from = uniform(first == unit0 ? sp->src : sp->dst);
 #pragma unroll
     for (int i = 0; i < MT; i++)
 #pragma unroll
-      for (int nt = 0; nt < 2; nt++)
+      for (int nt = 0; nt < NT; nt++)
         S[i][nt] = from >= 0 ? *(const f4*)(L.state + (((size_t)from * L.v_heads + h) * DV + col0 + 16 * nt + n) * DK + 16 * (wave * MT + i) + 4 * g)
                              : f4{0, 0, 0, 0};
     load_v(first, v[0]);
@@ -642,7 +642,7 @@ __global__ __launch_bounds__(512, 2) void linear_chunk_scan(LinLayer L, LinBatch
     load_kt(first);
     load_v(min(first + 1, last - 1), v[1]);
 #pragma unroll
-    for (int nt = 0; nt < 2; nt++) {
+    for (int nt = 0; nt < NT; nt++) {
       uint32_t t = 0;
 #pragma unroll
       for (int i = 0; i < MT; i++)
@@ -653,7 +653,7 @@ __global__ __launch_bounds__(512, 2) void linear_chunk_scan(LinLayer L, LinBatch
     __syncthreads();
     // from here on S holds the state times 2^sshift
 #pragma unroll
-    for (int nt = 0; nt < 2; nt++) {
+    for (int nt = 0; nt < NT; nt++) {
       sshift[nt] = first_shift(nt);
 #pragma unroll
       for (int i = 0; i < MT; i++)
@@ -669,12 +669,12 @@ __global__ __launch_bounds__(512, 2) void linear_chunk_scan(LinLayer L, LinBatch
       __syncthreads();  // the state, and what is noted of it and of V
       const Shifts sh = shifts();
       load_meta(next);
-      f4 vp[2];
+      f4 vp[NT];
       if constexpr (DELTA) {
-        f4 ks[2] = {f4{0, 0, 0, 0}, f4{0, 0, 0, 0}};
+        f4 ks[NT] = {};
 #pragma unroll
         for (int kb = 0; kb < NKB; kb++) {
-          half8 hi[2], lo[2];
+          half8 hi[NT], lo[NT];
           operands(Sb, kb, hi, lo);
           products3(fk[kb][0], fk[kb][1], hi, lo, ks);
         }
@@ -682,7 +682,7 @@ __global__ __launch_bounds__(512, 2) void linear_chunk_scan(LinLayer L, LinBatch
         load_k(next);
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int nt = 0; nt < 2; nt++) {
+        for (int nt = 0; nt < NT; nt++) {
           // Y 2^y, the product's own powers in one factor: below 2^-149 its share is nothing beside Y's bound
           const float f = ldexpf(1.0f, sh.y[nt] - kshift - sshift[nt]);
           float y[4];
@@ -692,11 +692,11 @@ __global__ __launch_bounds__(512, 2) void linear_chunk_scan(LinLayer L, LinBatch
         }
         eg = load_fade(next, 0);
         __syncthreads();
-        vp[0] = vp[1] = f4{0, 0, 0, 0};
+        for (int nt = 0; nt < NT; nt++) vp[nt] = f4{0, 0, 0, 0};
 #pragma unroll
         for (int kb = 0; kb < 2; kb++)
           if (2 * kb <= wave) {
-            half8 hi[2], lo[2];
+            half8 hi[NT], lo[NT];
             operands(Yb, kb, hi, lo);
             products3(ft[kb][0], ft[kb][1], hi, lo, vp);
           }
@@ -705,25 +705,25 @@ __global__ __launch_bounds__(512, 2) void linear_chunk_scan(LinLayer L, LinBatch
         __builtin_amdgcn_sched_barrier(0);
       } else {
 #pragma unroll
-        for (int nt = 0; nt < 2; nt++)
+        for (int nt = 0; nt < NT; nt++)
 #pragma unroll
           for (int r = 0; r < 4; r++) vp[nt][r] = v[0][nt][r];
       }
       // V' as it is held: times 2^held
-      const int held[2] = {DELTA ? tshift + sh.y[0] : 0, DELTA ? tshift + sh.y[1] : 0};
+      int held[NT];
 #pragma unroll
-      for (int nt = 0; nt < 2; nt++) {
+      for (int nt = 0; nt < NT; nt++) held[nt] = DELTA ? tshift + sh.y[nt] : 0;
+#pragma unroll
+      for (int nt = 0; nt < NT; nt++) {
         const float f = ldexpf(1.0f, sh.f[nt] - held[nt]);
         put4(Fb, wave, nt, fg[0] * f * vp[nt][0], fg[1] * f * vp[nt][1], fg[2] * f * vp[nt][2], fg[3] * f * vp[nt][3]);
       }
       fg = load_fade(next, 256);
       __syncthreads();
-      f4 acc[MT][2];
-#pragma unroll
-      for (int i = 0; i < MT; i++) acc[i][0] = acc[i][1] = f4{0, 0, 0, 0};
+      f4 acc[MT][NT] = {};
 #pragma unroll
       for (int kb = 0; kb < 2; kb++) {
-        half8 hi[2], lo[2];
+        half8 hi[NT], lo[NT];
         operands(Fb, kb, hi, lo);
 #pragma unroll
         for (int i = 0; i < MT; i++) products3(fkt[i][kb][0], fkt[i][kb][1], hi, lo, acc[i]);
@@ -734,7 +734,7 @@ __global__ __launch_bounds__(512, 2) void linear_chunk_scan(LinLayer L, LinBatch
       if (const uint32_t todo = sh.out & ~slow) {  // columns that leave the chunks here
         const int l = afresh(lane);
 #pragma unroll
-        for (int nt = 0; nt < 2; nt++) {
+        for (int nt = 0; nt < NT; nt++) {
           const int c = 16 * nt + (l & 15);
           if (!(todo >> c & 1)) continue;
 #pragma unroll
@@ -746,7 +746,7 @@ __global__ __launch_bounds__(512, 2) void linear_chunk_scan(LinLayer L, LinBatch
         slow |= todo;
       }
 #pragma unroll
-      for (int nt = 0; nt < 2; nt++) {
+      for (int nt = 0; nt < NT; nt++) {
         const float f = ldexpf(1.0f, sh.s_next[nt] - kshift - sh.f[nt]), w = ldexpf(whole, sh.s_next[nt] - sshift[nt]);
         float t = 0.0f;
 #pragma unroll
@@ -764,7 +764,7 @@ __global__ __launch_bounds__(512, 2) void linear_chunk_scan(LinLayer L, LinBatch
       put_state();
       // V' for the output waves, which take it behind the next barrier
 #pragma unroll
-      for (int nt = 0; nt < 2; nt++) {
+      for (int nt = 0; nt < NT; nt++) {
         const int e = sh.v[nt] - held[nt];
         put4(Vb[u & 1], wave, nt, ldexpf(vp[nt][0], e), ldexpf(vp[nt][1], e), ldexpf(vp[nt][2], e), ldexpf(vp[nt][3], e));
       }
@@ -791,9 +791,9 @@ __global__ __launch_bounds__(512, 2) void linear_chunk_scan(LinLayer L, LinBatch
         for (int hl = 0; hl < 2; hl++)
           if (2 * kb <= wave) fp[kb][hl] = load8(r, at_t, W::P + (kb * 2 + hl) * 64);
     };
-    auto note_v = [&](const float (&of)[2][4]) {
+    auto note_v = [&](const float (&of)[NT][4]) {
 #pragma unroll
-      for (int nt = 0; nt < 2; nt++) {
+      for (int nt = 0; nt < NT; nt++) {
         uint32_t t = 0;
 #pragma unroll
         for (int r = 0; r < 4; r++) t = max(t, mag(of[nt][r]));
@@ -802,32 +802,31 @@ __global__ __launch_bounds__(512, 2) void linear_chunk_scan(LinLayer L, LinBatch
         if (l < 16) vmax[wave][16 * nt + l] = t;
       }
     };
-    float v[2][4];
-    f4 o[2];
+    float v[NT][4];
+    f4 o[NT];
     // what V' adds to the rows of chunk u, and their store, but for the columns `left_out`
-    auto finish = [&](int u, int pshift, const int (&vshift)[2], uint32_t left_out) {
+    auto finish = [&](int u, int pshift, const int (&vshift)[NT], uint32_t left_out) {
       const auto ro = values(a.out, u);
-      f4 acc[2] = {f4{0, 0, 0, 0}, f4{0, 0, 0, 0}};
+      f4 acc[NT] = {};
 #pragma unroll
       for (int kb = 0; kb < 2; kb++)
         if (2 * kb <= wave) {
-          half8 hi[2], lo[2];
+          half8 hi[NT], lo[NT];
           operands(Vb[u & 1], kb, hi, lo);
           products3(fp[kb][0], fp[kb][1], hi, lo, acc);
         }
 #pragma unroll
-      for (int nt = 0; nt < 2; nt++) {
+      for (int nt = 0; nt < NT; nt++) {
         const float f = a.scale * ldexpf(1.0f, -pshift - vshift[nt]);
 #pragma unroll
         for (int r = 0; r < 4; r++) acc[nt][r] = fmaf(f, acc[nt][r], o[nt][r]);
       }
       int at = afresh(vlane);
-      const bool on[2] = {!(left_out >> n & 1), !(left_out >> (16 + n) & 1)};
 #pragma unroll
       for (int r = 0; r < 4; r++, at += vrow)
 #pragma unroll
-        for (int nt = 0; nt < 2; nt++)
-          if (on[nt]) __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(acc[nt][r]), ro, at + 64 * nt, 0, 0);
+        for (int nt = 0; nt < NT; nt++)
+          if (!(left_out >> (16 * nt + n) & 1)) __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(acc[nt][r]), ro, at + 64 * nt, 0, 0);
     };
     load_v(first, v);
     load_meta(first);
@@ -838,8 +837,8 @@ __global__ __launch_bounds__(512, 2) void linear_chunk_scan(LinLayer L, LinBatch
     load_v(min(first + 1, last - 1), v);
     __syncthreads();
 #pragma unroll
-    for (int nt = 0; nt < 2; nt++) sshift[nt] = first_shift(nt);
-    int vshift[2] = {0, 0}, pshift = 0;
+    for (int nt = 0; nt < NT; nt++) sshift[nt] = first_shift(nt);
+    int vshift[NT] = {}, pshift = 0;
 #pragma unroll 1
     for (int u = first; u < last; u++) {
       const int next = min(u + 1, last - 1);
@@ -847,10 +846,10 @@ __global__ __launch_bounds__(512, 2) void linear_chunk_scan(LinLayer L, LinBatch
       const Shifts sh = shifts();
       const int qshift = word(M_QSHIFT + wave), pshift_now = word(M_PSHIFT + wave);
       load_meta(next);
-      f4 now[2] = {f4{0, 0, 0, 0}, f4{0, 0, 0, 0}};
+      f4 now[NT] = {};
 #pragma unroll
       for (int kb = 0; kb < NKB; kb++) {
-        half8 hi[2], lo[2];
+        half8 hi[NT], lo[NT];
         operands(Sb, kb, hi, lo);
         products3(fq[kb][0], fq[kb][1], hi, lo, now);
       }
@@ -860,7 +859,7 @@ __global__ __launch_bounds__(512, 2) void linear_chunk_scan(LinLayer L, LinBatch
       if constexpr (DELTA) __syncthreads();
       // the state waves hurry from here to the third barrier: the chunk before is finished behind it
 #pragma unroll
-      for (int nt = 0; nt < 2; nt++) {
+      for (int nt = 0; nt < NT; nt++) {
         const float f = a.scale * ldexpf(1.0f, -qshift - sshift[nt]);
 #pragma unroll
         for (int r = 0; r < 4; r++) now[nt][r] = eg[r] * (f * now[nt][r]);
@@ -878,7 +877,7 @@ __global__ __launch_bounds__(512, 2) void linear_chunk_scan(LinLayer L, LinBatch
         __builtin_amdgcn_sched_barrier(0);
       }
 #pragma unroll
-      for (int nt = 0; nt < 2; nt++) {
+      for (int nt = 0; nt < NT; nt++) {
         o[nt] = now[nt];
         vshift[nt] = sh.v[nt];
         sshift[nt] = sh.s_next[nt];
@@ -894,14 +893,14 @@ __global__ __launch_bounds__(512, 2) void linear_chunk_scan(LinLayer L, LinBatch
 #pragma unroll
     for (int i = 0; i < MT; i++)
 #pragma unroll
-      for (int nt = 0; nt < 2; nt++)
+      for (int nt = 0; nt < NT; nt++)
         if (!(slow >> (16 * nt + n) & 1)) *(f4*)(left + (16 * nt + n) * DK + 16 * (wave * MT + i) + 4 * g) =
               f4{ldexpf(S[i][nt][0], -sshift[nt]), ldexpf(S[i][nt][1], -sshift[nt]), ldexpf(S[i][nt][2], -sshift[nt]), ldexpf(S[i][nt][3], -sshift[nt])};
   if (!slow) return;
   // the other columns, eight lanes each, as linear_attn.hip does them
   __syncthreads();
   const int c = threadIdx.x >> 3, l = threadIdx.x & 7;
-  if (role || !(slow >> c & 1)) return;
+  if (c >= kCols || !(slow >> c & 1)) return;
   f4 st[DK / 32];
 #pragma unroll
   for (int i = 0; i < DK / 32; i++) st[i] = *(const f4*)&plain[c][32 * i + 4 * l];
@@ -963,15 +962,28 @@ __global__ __launch_bounds__(256) void linear_norm_kernel(LinLayer L, LinBatchVi
   }
 }
 
+template <int DK, int DV, bool DELTA, int NT>
+void launch_scan(const LinLayer& L, const LinBatchView& b, const LinAttnArgs& a, int u0, int u1, hipStream_t st) {
+  const int groups = b.n_chunked * L.k_heads, members = L.v_heads / L.k_heads * (DV / (16 * NT));
+  hipLaunchKernelGGL((linear_chunk_scan<DK, DV, DELTA, NT>), dim3(8 * ((groups + 7) / 8) * members), dim3(512), 0, st, L, b, a, u0, u1);
+}
+
 template <int DK, int DV, bool DELTA>
 hipError_t launch_t(const LinLayer& L, const LinBatchView& b, const LinAttnArgs& a, hipStream_t st) {
-  const int groups = b.n_chunked * L.k_heads, members = L.v_heads / L.k_heads * (DV / kCols);
   for (int u0 = 0; u0 < b.n_chunk_units; u0 += b.window) {
     const int u1 = std::min(u0 + b.window, b.n_chunk_units);
     hipLaunchKernelGGL((linear_chunk_prepare<DK, DELTA>), dim3(u1 - u0, L.k_heads), dim3(256), 0, st, L, b, a, u0);
-    hipLaunchKernelGGL((linear_chunk_scan<DK, DV, DELTA>), dim3(8 * ((groups + 7) / 8) * members), dim3(512), 0, st, L, b, a, u0, u1);
+    // 32 value dims a workgroup; of the sum rule, whose chain is short, 16 where that still fits the GPU twice (2 x
+    // 2048 rows of 16 heads, 128 workgroups of 32: 59 us, 256 of 16: 50; more workgroups than 512 of 16, each
+    // reading the same operands, take longer). The delta rule's 192 of 32 over 8192 rows 435 us, 384 of 16 496.
+    bool narrow = false;
+    if constexpr (!DELTA) narrow = b.n_chunked * L.v_heads * (DV / 32) <= kFewScans;
+    if constexpr (!DELTA)
+      if (narrow) launch_scan<DK, DV, DELTA, 1>(L, b, a, u0, u1, st);
+    if (!narrow) launch_scan<DK, DV, DELTA, 2>(L, b, a, u0, u1, st);
   }
-  if (a.norm) hipLaunchKernelGGL((linear_norm_kernel<DV>), dim3(b.n_chunk_units, std::min(8, L.v_heads)), dim3(256), 0, st, L, b, a);
+  if (a.norm)
+    hipLaunchKernelGGL((linear_norm_kernel<DV>), dim3(b.n_chunk_units, (kLinChunk * L.v_heads * DV / 4 + 1023) / 1024), dim3(256), 0, st, L, b, a);
   return hipGetLastError();
 }
 
