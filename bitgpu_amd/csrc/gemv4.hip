@@ -6,16 +6,16 @@
 //           a word give its odd codes and, shifted, its even ones). The operand of x has four rows a token, one a
 //           digit, so a product takes four tokens; its result leaves lane 16 g + n with the four digit sums of
 //           weight row n and token g, exact integers that are joined in f32 once a scale group, scaled back and
-//           multiplied by the group's scale. With minima, a weight is (c - 8) s + (8 s + m): the groups' sums of
-//           x come from the same products over all-ones weights. What a row of x gives does not depend on the
-//           rows beside it: how K is split depends on K alone, and the rest is exact.
+//           multiplied by the group's scale. With minima, codes enter as they are (c), and the minima times the
+//           groups' sums of x, 16 tokens at once, are a product on the f32 matrix cores. What a row of x gives does
+//           not depend on the rows beside it: how K is split depends on K alone, and the rest is exact.
 //   lanes   16 weight rows x 128 weights: lane 16 g + n holds words 4 g .. 4 g + 3 of row n (one 16-byte load). A
 //           product contracts one word of each of the four lane groups: of the same scale group with groups of 128;
 //           for 64 and 32 the words change lane groups (v_permlane32_swap, v_permlane16_swap) until that holds. The
 //           digits of x are read in the order that this gives.
-//   split   the waves of a workgroup split K, each taking 512 weights at a time and preparing x for those alone, in
-//           LDS; every wave runs the workgroup's tiles over its part, and the parts meet in LDS. A wave's loads of
-//           weights and scales are in flight before x is prepared.
+//   split   the waves of a workgroup split K, 512 weights at a time. A wave prepares x for its 512 once, through LDS
+//           into registers, and runs the workgroup's tiles of 16 rows over it, the next tile's weights and scales in
+//           flight while one is multiplied; the parts meet in LDS at the end.
 //   values  a block of x with an infinity or a NaN is summed directly in f32.
 #include <hip/hip_fp16.h>
 
@@ -35,6 +35,8 @@ typedef float f32x4_t __attribute__((ext_vector_type(4)));
 
 constexpr int kStep = 512;            // weights of a wave's step: four blocks of 128
 constexpr int kWaves = 8;
+constexpr int kTarget = 512;          // workgroups that a launch aims at, with up to kMaxTiles tiles of 16 rows each
+constexpr int kMaxTiles = 4;
 constexpr int kDigit = 528;           // bytes of a digit's row: 64 words of 8, and a pad that spreads 16 rows over the banks
 constexpr int kToken = 4 * kDigit;
 
@@ -60,9 +62,11 @@ __device__ inline void exchange(u32x4_t& w) {
   }
 }
 
-// a word's eight codes as signed bytes 16 (c - 8): its even ones, then its odd ones
+// a word's eight codes as signed bytes, its even ones, then its odd ones: 16 (c - 8), or c where there are minima
+template <bool MINS>
 __device__ inline long weight_operand(uint32_t w) {
-  const uint32_t even = (w << 4 ^ 0x80808080u) & 0xf0f0f0f0u, odd = (w ^ 0x80808080u) & 0xf0f0f0f0u;
+  const uint32_t even = MINS ? w & 0x0f0f0f0fu : (w << 4 ^ 0x80808080u) & 0xf0f0f0f0u;
+  const uint32_t odd = MINS ? w >> 4 & 0x0f0f0f0fu : (w ^ 0x80808080u) & 0xf0f0f0f0u;
   return (long)((uint64_t)odd << 32 | even);
 }
 
@@ -74,151 +78,120 @@ __device__ inline int round_i32(float v) {
 }
 
 // One group's scale of a row (or its minimum)
-__device__ inline float scale_at(const void* p, size_t at, int f16) {
-  return f16 ? __half2float(((const __half*)p)[at]) : ((const float*)p)[at];
+template <bool F16>
+__device__ inline float scale_at(const void* p, size_t at) {
+  return F16 ? __half2float(((const __half*)p)[at]) : ((const float*)p)[at];
 }
-// The 128 / G scales of a block, as loaded: 2 to 16 bytes
-template <int G>
+// The 128 / G scales of a block, as loaded: 2 to 16 bytes (rows hold a multiple of 128 / G groups: aligned)
+template <int G, bool F16>
 struct Scales {
-  uint32_t raw[128 / G];
-};
-template <int G>
-__device__ inline void load_scales(Scales<G>& s, const void* p, size_t at, int f16) {
-  constexpr int N = 128 / G;
-  if (f16) {  // (rows hold a multiple of 128 / G groups: aligned)
-    if constexpr (N == 1) s.raw[0] = ((const uint16_t*)p)[at];
-    if constexpr (N == 2) s.raw[0] = *(const uint32_t*)((const uint16_t*)p + at);
-    if constexpr (N == 4) {
-      const uint2 v = *(const uint2*)((const uint16_t*)p + at);
-      s.raw[0] = v.x;
-      s.raw[1] = v.y;
-    }
-  } else {
-    if constexpr (N == 1) s.raw[0] = ((const uint32_t*)p)[at];
-    if constexpr (N == 2) {
-      const uint2 v = *(const uint2*)((const uint32_t*)p + at);
-      s.raw[0] = v.x;
-      s.raw[1] = v.y;
-    }
-    if constexpr (N == 4) {
-      const uint4 v = *(const uint4*)((const uint32_t*)p + at);
-      s.raw[0] = v.x;
-      s.raw[1] = v.y;
-      s.raw[2] = v.z;
-      s.raw[3] = v.w;
+  static constexpr int N = 128 / G, W = F16 ? (N + 1) / 2 : N;
+  uint32_t raw[W];
+  __device__ __forceinline__ void load(__amdgpu_buffer_rsrc_t r, int at, int more) {  // bytes
+    if constexpr (F16 && N == 1) {
+      raw[0] = __builtin_amdgcn_raw_buffer_load_b16(r, at, more, 0);
+    } else if constexpr (W == 1) {
+      raw[0] = __builtin_amdgcn_raw_buffer_load_b32(r, at, more, 0);
+    } else if constexpr (W == 2) {
+      const auto v = __builtin_amdgcn_raw_buffer_load_b64(r, at, more, 0);
+      raw[0] = v[0];
+      raw[1] = v[1];
+    } else {
+      const auto v = __builtin_amdgcn_raw_buffer_load_b128(r, at, more, 0);
+      raw[0] = v[0];
+      raw[1] = v[1];
+      raw[2] = v[2];
+      raw[3] = v[3];
     }
   }
-}
-template <int G>
-__device__ inline float scale_of(const Scales<G>& s, int i, int f16) {
-  if (!f16) return __uint_as_float(s.raw[i]);
-  return __half2float(__ushort_as_half((unsigned short)(s.raw[i >> 1] >> (16 * (i & 1)))));
-}
+  __device__ __forceinline__ float get(int i) const {
+    if constexpr (!F16) return __uint_as_float(raw[i]);
+    else return __half2float(__ushort_as_half((unsigned short)(raw[i >> 1] >> (16 * (i & 1)))));
+  }
+};
 
 // A block of 128 weights in f32, for a row of x that holds an infinity or a NaN there
-__device__ __noinline__ float block_f32(const float* x, const uint32_t* words, const void* scales, const void* mins, size_t at, int group,
-                                        int f16) {
+template <int G, bool F16>
+__device__ __forceinline__ float block_f32(const float* x, const uint32_t* words, const void* scales, const void* mins, size_t at) {
   float sum = 0.0f;
 #pragma unroll 1
   for (int k = 0; k < 128; k++) {
-    const float s = scale_at(scales, at + k / group, f16);
-    const float lo = mins ? scale_at(mins, at + k / group, f16) : -8.0f * s;
+    const float s = scale_at<F16>(scales, at + k / G);
+    const float lo = mins ? scale_at<F16>(mins, at + k / G) : -8.0f * s;
     sum = fmaf(fmaf((float)(words[k >> 3] >> (4 * (k & 7)) & 15), s, lo), x[k], sum);
   }
   return sum;
 }
 
-constexpr int kOdd = 1 << 20;  // in the place of a block's exponent: it is not finite
+__device__ inline __amdgpu_buffer_rsrc_t buffer(const void* p, size_t bytes) {
+  return __builtin_amdgcn_make_buffer_rsrc((void*)p, (short)0, (int)(uint32_t)(bytes < 0xffffffffu ? bytes : 0xffffffffu), 0x00020000);
+}
 
-// Rows of x as loaded: lane 16 b + l has weights 8 l .. + 7 of the step's block b.
-template <int MT>
-struct XLoad {
-  f32x4_t v[MT][2];
-};
-
-// T tiles of 16 weight rows a workgroup, P passes of MT tokens over a step's weights (MT 1: one token).
-template <int T, int MT, int P, int G>
-__global__ __launch_bounds__(64 * kWaves) void gemv4_kernel(Gemv4Args a) {
+// P: groups of four tokens.
+template <int P, int G, bool MINS, bool F16>
+__global__ __launch_bounds__(64 * kWaves, P == 1 ? 4 : 2) void gemv4_kernel(Gemv4Args a, int T) {
   constexpr int NG = 128 / G;
-  constexpr int kBytes = MT * kToken + kDigit;  // a wave's digits, then zeros for the tokens that are not there
-  constexpr int kRed = T * 16 * MT * P * 4;     // a wave's sums
-  __shared__ __align__(16) char lds[kWaves * (kBytes > kRed ? kBytes : kRed)];
-  __shared__ int exps[kWaves][MT][4];
+  extern __shared__ __align__(16) char lds[];
+  __shared__ int exps[kWaves][4][4];
+  __shared__ float xsum[MINS ? kWaves : 1][16][4 * NG];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int n = lane & 15, g = lane >> 4;
   const int N = a.N0 + a.N1 + a.N2, n0 = blockIdx.x * 16 * T;
   const int steps = (a.K + kStep - 1) / kStep, waves = blockDim.x >> 6;
   const int blocks = a.K >> 7, words = a.K >> 3, groups = a.K / G;
-  char* dig = lds + wave * kBytes;
-  float* red = (float*)lds;
+  const int held = min(a.M, 4);                         // tokens of the digits in LDS, then zeros for the others
+  char* dig = lds + wave * (held * kToken + kDigit);
+  float* red = (float*)(lds + waves * (held * kToken + kDigit));  // [wave][tile][16 rows][M]
 
-  size_t row[T];
+  long xd[P == 1 ? 1 : P][4][4];  // the operand of x: four words of each of the step's blocks (of one pass: read where used)
+  int ex[P][4];        // the blocks' powers of two, of this lane's token 4 p + g
+  float xs[NG];        // the groups' sums of x: token 4 (n % 4) + n / 4, group 4 i + g of the step
+  bool odd_any = false;
+  f32x4_t x0[4], x1[4];  // a pass's rows of x as loaded: lane 16 b + l has weights 8 l .. + 7 of block b
+  auto load_x = [&](int step, int p) {
 #pragma unroll
-  for (int t = 0; t < T; t++) row[t] = min(n0 + 16 * t + n, N - 1);
-  auto load_x = [&](XLoad<MT>& x, int step, int m0) {
-    const int blk = min(4 * step + g, blocks - 1);
-#pragma unroll
-    for (int m = 0; m < MT; m++) {
-      const float* p = a.x + (size_t)min(m0 + m, a.M - 1) * a.K + 128 * blk + 8 * n;
-      x.v[m][0] = *(const f32x4_t*)p;
-      x.v[m][1] = *(const f32x4_t*)(p + 4);
+    for (int m = 0; m < 4; m++) {
+      if (4 * p + m >= a.M) break;
+      const float* xp = a.x + (size_t)(4 * p + m) * a.K + 128 * min(4 * step + g, blocks - 1) + 8 * n;
+      x0[m] = *(const f32x4_t*)xp;
+      x1[m] = *(const f32x4_t*)(xp + 4);
     }
   };
-  float acc[P][T];
-#pragma unroll
-  for (int p = 0; p < P; p++)
-#pragma unroll
-    for (int t = 0; t < T; t++) acc[p][t] = 0.0f;
-  for (int i = lane; i < kDigit / 4; i += 64) ((int*)(dig + MT * kToken))[i] = 0;
-
-  for (int step = wave; step < steps; step += waves) {
-    // x first: it is needed first, and loads arrive in order
-    XLoad<MT> x;
-    load_x(x, step, 0);
-    __builtin_amdgcn_sched_barrier(0);
-    u32x4_t w[T][4];
-    Scales<G> sc[T][4], mn[T][4];
-#pragma unroll
-    for (int b = 0; b < 4; b++) {
-      const int blk = min(4 * step + b, blocks - 1);  // past the end: x counts as zero there
-#pragma unroll
-      for (int t = 0; t < T; t++) {
-        w[t][b] = *(const u32x4_t*)(a.codes + row[t] * words + 16 * blk + 4 * g);
-        load_scales<G>(sc[t][b], a.scales, row[t] * groups + NG * blk, a.scale_f16);
-        if (a.mins) load_scales<G>(mn[t][b], a.mins, row[t] * groups + NG * blk, a.scale_f16);
-      }
-    }
-    __builtin_amdgcn_sched_barrier(0);
+  auto prepare = [&](int step) {  // x of its first pass is loaded
+    for (int i = lane; i < kDigit / 4; i += 64) ((int*)(dig + held * kToken))[i] = 0;
 #pragma unroll
     for (int p = 0; p < P; p++) {
-      const int m0 = p * MT;
-      if (p && m0 >= a.M) break;
-      bool bad = false;
-      // the reads of the pass before are done; a wave's LDS accesses complete in order
-      __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-      __builtin_amdgcn_wave_barrier();
 #pragma unroll
-      for (int m = 0; m < MT; m++) {
-        const bool on = 4 * step + g < blocks && m0 + m < a.M;
-        const f32x4_t x0 = x.v[m][0], x1 = x.v[m][1];
+      for (int m = 0; m < 4; m++) {
+        if (4 * p + m >= a.M) {
+          if constexpr (MINS)
+            if (lane < 4 * NG) xsum[wave][4 * m + p][lane] = 0.0f;
+          continue;
+        }
+        const bool on = 4 * step + g < blocks;
         uint32_t top = 0;
 #pragma unroll
-        for (int e = 0; e < 4; e++) top = max(top, max(__float_as_uint(x0[e]) & 0x7fffffffu, __float_as_uint(x1[e]) & 0x7fffffffu));
+        for (int e = 0; e < 4; e++) top = max(top, max(__float_as_uint(x0[m][e]) & 0x7fffffffu, __float_as_uint(x1[m][e]) & 0x7fffffffu));
         auto dppmax = [&](auto ctrl) { top = max(top, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)top, decltype(ctrl)::value, 0xf, 0xf, false)); };
         dppmax(std::integral_constant<int, kDppXor1>{});
         dppmax(std::integral_constant<int, kDppXor2>{});
         dppmax(std::integral_constant<int, kDppHalfMirror>{});
         dppmax(std::integral_constant<int, kDppMirror>{});
         const bool odd = top >= 0x7f800000u;
-        bad = bad || (on && odd);
+        odd_any = odd_any || (on && odd);
         const int e = (int)(top >> 23) - 126;  // |x| < 2^e
-        const int shift = on && !odd ? 30 - e : -1024;  // (an infinity or NaN leaves some integer, cleared below)
+        const uint32_t use = on && !odd ? ~0u : 0u;  // (an infinity or NaN leaves some integer)
         uint32_t y[2][4];  // even weights, odd weights
 #pragma unroll
         for (int i = 0; i < 4; i++) {
-          const float u = i < 2 ? x0[2 * i] : x1[2 * i - 4], v = i < 2 ? x0[2 * i + 1] : x1[2 * i - 3];
-          y[0][i] = ((uint32_t)(odd ? 0 : round_i32(ldexpf(u, shift))) + 0x80808080u) ^ 0x80808080u;  // signed base-256 digits
-          y[1][i] = ((uint32_t)(odd ? 0 : round_i32(ldexpf(v, shift))) + 0x80808080u) ^ 0x80808080u;
+          const float u = i < 2 ? x0[m][2 * i] : x1[m][2 * i - 4], v = i < 2 ? x0[m][2 * i + 1] : x1[m][2 * i - 3];
+          y[0][i] = (((uint32_t)round_i32(ldexpf(u, 30 - e)) & use) + 0x80808080u) ^ 0x80808080u;  // signed base-256 digits
+          y[1][i] = (((uint32_t)round_i32(ldexpf(v, 30 - e)) & use) + 0x80808080u) ^ 0x80808080u;
+        }
+        if constexpr (MINS) {
+          float t = ((x0[m][0] + x0[m][1]) + (x0[m][2] + x0[m][3])) + ((x1[m][0] + x1[m][1]) + (x1[m][2] + x1[m][3]));
+          t = group_sum<G / 8>(t);
+          if (n % (G / 8) == 0) xsum[wave][4 * m + p][NG * g + n / (G / 8)] = use ? t : 0.0f;
         }
         uint32_t d[2][4];
 #pragma unroll
@@ -234,76 +207,156 @@ __global__ __launch_bounds__(64 * kWaves) void gemv4_kernel(Gemv4Args a) {
         }
 #pragma unroll
         for (int q = 0; q < 4; q++) *(uint2*)(dig + m * kToken + q * kDigit + 128 * g + 8 * n) = make_uint2(d[0][q], d[1][q]);
-        if (n == 0) exps[wave][m][g] = odd ? kOdd : e - 34;
+        if (n == 0) exps[wave][m][g] = odd ? 0 : e - (MINS ? 30 : 34);
       }
       __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
       __builtin_amdgcn_wave_barrier();
       __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-      if (p + 1 < P) load_x(x, step, m0 + MT);
+      if (p + 1 < P) load_x(step, p + 1);
       const int token = n >> 2;  // of the operand's row n; its digit is n & 3
-      const char* src = dig + (token < MT ? token * kToken + (n & 3) * kDigit : MT * kToken);
-      const int mine = g < MT ? g : 0;  // the token of this lane's results
+      const bool there = token < held && 4 * p + token < a.M;
+      const char* src = dig + (there ? token * kToken + (n & 3) * kDigit : held * kToken);
 #pragma unroll
       for (int b = 0; b < 4; b++) {
-        long xd[4];
 #pragma unroll
-        for (int j = 0; j < 4; j++) xd[j] = *(const long*)(src + 128 * b + 8 * word_of<G>(j, g));
-        const int e = exps[wave][mine][b];
-        auto joined = [&](const i32x4_t& d) {  // digits 0, 1 and 2, 3 as integers (|d| <= 2^21), then in f32
-          return ldexpf(fmaf((float)(d[2] + (d[3] << 8)), 65536.0f, (float)(d[0] + (d[1] << 8))), e);
-        };
-        float sums[NG];  // of x, by group
-        if (a.mins) {
+        for (int j = 0; j < 4; j++)
+          if constexpr (P > 1) xd[p][b][j] = *(const long*)(src + 128 * b + 8 * word_of<G>(j, g));
+        ex[p][b] = 4 * p + g < a.M ? exps[wave][g][b] : 0;
+      }
+      __builtin_amdgcn_sched_barrier(0);
+      // read before the next pass writes: a wave's LDS accesses complete in order
+      __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+    }
+    if constexpr (MINS) {
+      __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 #pragma unroll
-          for (int i = 0; i < NG; i++) {
-            i32x4_t d = {0, 0, 0, 0};
+      for (int i = 0; i < NG; i++) xs[i] = (n & 3) < P ? xsum[wave][n][4 * i + g] : 0.0f;  // (row n: token 4 (n % 4) + n / 4)
+    }
+  };
+
+  struct Tile {
+    u32x4_t w[4];
+    Scales<G, F16> s[4];
+    Scales<128, F16> lo[MINS ? NG : 1];
+  };
+  // The workgroup's rows as buffers: 32-bit offsets from its first (rows behind the last are the last again)
+  const int rows = min(16 * T, N - n0);
+  constexpr int kScale = F16 ? 2 : 4;
+  const auto rw = buffer(a.codes + (size_t)n0 * words, (size_t)rows * words * 4);
+  const auto rs = buffer((const char*)a.scales + (size_t)n0 * groups * kScale, (size_t)rows * groups * kScale);
+  const auto rm = buffer((const char*)(MINS ? a.mins : a.scales) + (size_t)n0 * groups * kScale, (size_t)rows * groups * kScale);
+  auto load = [&](Tile& x, int step, int t, int b) {
+    const int r = min(16 * t + n, rows - 1), blk = min(4 * step + b, blocks - 1);  // past the end: x counts as zero there
+    x.w[b] = __builtin_bit_cast(u32x4_t, __builtin_amdgcn_raw_buffer_load_b128(rw, r * words * 4 + 16 * g, 64 * blk, 0));
+    x.s[b].load(rs, r * groups * kScale, NG * kScale * blk);
+  };
+  auto load_lo = [&](Tile& x, int step, int t) {
+    const int r = min(16 * t + n, rows - 1);
+    if constexpr (MINS)
 #pragma unroll
-            for (int j = i * G / 32; j < (i + 1) * G / 32; j++)
-              d = __builtin_amdgcn_mfma_i32_16x16x32_i8(xd[j], 0x1010101010101010l, d, 0, 0, 0);
-            sums[i] = joined(d);
-          }
-        }
+      for (int i = 0; i < NG; i++) x.lo[i].load(rm, kScale * (r * groups + min(4 * NG * step + 4 * i + g, groups - 1)), 0);
+  };
+  // A tile's products; the next one's (step1, t1) loads go into the registers of each block as it is done
+  auto multiply = [&](Tile& x, int step, int t, int step1, int t1) {
+    float acc[P];
 #pragma unroll
-        for (int t = 0; t < T; t++) {
-          u32x4_t v = w[t][b];
-          exchange<G>(v);
+    for (int p = 0; p < P; p++) acc[p] = 0.0f;
+    if constexpr (MINS) {
+      f32x4_t d = {0, 0, 0, 0};
 #pragma unroll
-          for (int i = 0; i < NG; i++) {
-            i32x4_t d = {0, 0, 0, 0};
+      for (int i = 0; i < NG; i++) d = __builtin_amdgcn_mfma_f32_16x16x4f32(xs[i], x.lo[i].get(0), d, 0, 0, 0);
 #pragma unroll
-            for (int j = i * G / 32; j < (i + 1) * G / 32; j++)
-              d = __builtin_amdgcn_mfma_i32_16x16x32_i8(xd[j], weight_operand(v[j]), d, 0, 0, 0);
-            const float s = scale_of<G>(sc[t][b], i, a.scale_f16);
-            acc[p][t] = fmaf(joined(d), s, acc[p][t]);
-            if (a.mins) acc[p][t] = fmaf(sums[i], fmaf(8.0f, s, scale_of<G>(mn[t][b], i, a.scale_f16)), acc[p][t]);
-          }
+      for (int p = 0; p < P; p++) acc[p] = d[p];
+      if (step1 < steps) load_lo(x, step1, t1);
+    }
+#pragma unroll
+    for (int b = 0; b < 4; b++) {
+      u32x4_t v = x.w[b];
+      exchange<G>(v);
+      long w[4];
+#pragma unroll
+      for (int j = 0; j < 4; j++) w[j] = weight_operand<MINS>(v[j]);
+      if constexpr (P == 1) {
+        const char* src = dig + ((n >> 2) < held ? (n >> 2) * kToken + (n & 3) * kDigit : held * kToken);
+#pragma unroll
+        for (int j = 0; j < 4; j++) xd[0][b][j] = *(const long*)(src + 128 * b + 8 * word_of<G>(j, g));
+      }
+#pragma unroll
+      for (int i = 0; i < NG; i++) {
+        const float s = x.s[b].get(i);
+        i32x4_t d[P];
+#pragma unroll
+        for (int p = 0; p < P; p++) d[p] = i32x4_t{0, 0, 0, 0};
+#pragma unroll
+        for (int j = i * G / 32; j < (i + 1) * G / 32; j++)
+#pragma unroll
+          for (int p = 0; p < P; p++) d[p] = __builtin_amdgcn_mfma_i32_16x16x32_i8(xd[p][b][j], w[j], d[p], 0, 0, 0);
+#pragma unroll
+        for (int p = 0; p < P; p++) {  // digits 0, 1 and 2, 3 as integers (|d| <= 2^21), then in f32
+          const float lo = (float)(d[p][0] + (d[p][1] << 8)), hi = (float)(d[p][2] + (d[p][3] << 8));
+          acc[p] = fmaf(ldexpf(fmaf(hi, 65536.0f, lo), ex[p][b]), s, acc[p]);
         }
       }
-      if (__any(bad)) {
-#pragma unroll 1
-        for (int b = 0; b < 4; b++) {
-          const int k = 4 * step + b;
-          if (k >= blocks || g >= MT || m0 + g >= a.M || exps[wave][mine][b] != kOdd) continue;
+      // the sums of a block here, and not where a lane stores its part: all blocks' digits at once do not fit
 #pragma unroll
-          for (int t = 0; t < T; t++)
-            acc[p][t] += block_f32(a.x + (size_t)(m0 + g) * a.K + 128 * k, a.codes + row[t] * words + 16 * k, a.scales, a.mins,
-                                   row[t] * groups + NG * k, G, a.scale_f16);
+      for (int p = 0; p < P; p++) asm volatile("" : "+v"(acc[p]));
+      if (step1 < steps) load(x, step1, t1, b);
+    }
+    float* to = red + (size_t)((wave * T + t) * 16 + n) * a.M + g;
+#pragma unroll
+    for (int p = 0; p < P; p++)
+      if (4 * p + g < a.M) to[4 * p] = step == wave ? acc[p] : to[4 * p] + acc[p];
+  };
+
+  if (wave < steps) {
+    // x first: it is needed first, and loads arrive in order
+    Tile x;
+    load_x(wave, 0);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int b = 0; b < 4; b++) load(x, wave, 0, b);
+    load_lo(x, wave, 0);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll 1
+    for (int step = wave, t = 0; step < steps;) {
+      if (t == 0) {
+        if (step != wave) load_x(step, 0);
+        prepare(step);
+      }
+      const bool end = t + 1 == T;
+      const int step1 = end ? step + waves : step, t1 = end ? 0 : t + 1;
+      multiply(x, step, t, step1, t1);
+      step = step1;
+      t = t1;
+    }
+    if (__any(odd_any)) {  // the blocks of x that hold an infinity or a NaN, left out so far
+#pragma unroll 1
+      for (int blk = 0; blk < blocks; blk++) {
+        if ((blk >> 2) % waves != wave) continue;
+#pragma unroll 1
+        for (int m = g; m < a.M; m += 4) {
+          const float* xp = a.x + (size_t)m * a.K + 128 * blk;
+          uint32_t top = 0;
+#pragma unroll 1
+          for (int k = 0; k < 128; k++) top = max(top, __float_as_uint(xp[k]) & 0x7fffffffu);
+          if (top < 0x7f800000u) continue;
+#pragma unroll 1
+          for (int u = 0; u < T; u++) {
+            const size_t r = min(n0 + 16 * u + n, N - 1);
+            red[(size_t)((wave * T + u) * 16 + n) * a.M + m] +=
+                block_f32<G, F16>(xp, a.codes + r * words + 16 * blk, a.scales, MINS ? a.mins : nullptr, r * groups + NG * blk);
+          }
         }
       }
     }
   }
-  __syncthreads();  // every wave is done with its digits
-  if (g < MT)
-#pragma unroll
-    for (int p = 0; p < P; p++)
-#pragma unroll
-      for (int t = 0; t < T; t++) red[(wave * T * 16 + 16 * t + n) * (MT * P) + p * MT + g] = acc[p][t];
   __syncthreads();
-  for (int i = threadIdx.x; i < T * 16 * MT * P; i += blockDim.x) {
+  for (int i = threadIdx.x; i < T * 16 * a.M; i += blockDim.x) {
     const int m = i / (T * 16), r = i % (T * 16), at = n0 + r;
-    if (at >= N || m >= a.M) continue;
+    if (at >= N) continue;
     float y = 0.0f;
-    for (int k = 0; k < waves; k++) y += red[(k * T * 16 + r) * (MT * P) + m];
+    for (int k = 0; k < waves; k++) y += red[(size_t)(k * T * 16 + r) * a.M + m];
     if (a.resid) y += a.resid[(size_t)m * N + at];
     if (at < a.N0) a.out0[(size_t)m * a.N0 + at] = y;
     else if (at < a.N0 + a.N1) a.out1[(size_t)m * a.N1 + at - a.N0] = y;
@@ -311,20 +364,29 @@ __global__ __launch_bounds__(64 * kWaves) void gemv4_kernel(Gemv4Args a) {
   }
 }
 
-template <int T, int MT, int P, int G>
+template <int P, int G, bool MINS, bool F16>
 hipError_t launch_t(const Gemv4Args& a, hipStream_t st) {
-  const int N = a.N0 + a.N1 + a.N2, steps = (a.K + kStep - 1) / kStep;
-  hipLaunchKernelGGL((gemv4_kernel<T, MT, P, G>), dim3((N + 16 * T - 1) / (16 * T)), dim3(64 * std::min(steps, kWaves)), 0, st, a);
+  const int tiles = (a.N0 + a.N1 + a.N2 + 15) / 16, waves = std::min((a.K + kStep - 1) / kStep, kWaves);
+  const int T = std::min(kMaxTiles, (tiles + kTarget - 1) / kTarget);
+  const size_t lds = waves * ((size_t)(std::min(a.M, 4) * kToken + kDigit) + (size_t)T * 16 * a.M * sizeof(float));
+  hipLaunchKernelGGL((gemv4_kernel<P, G, MINS, F16>), dim3((tiles + T - 1) / T), dim3(64 * waves), lds, st, a, T);
   return hipGetLastError();
+}
+
+template <int P, int G>
+hipError_t launch_p(const Gemv4Args& a, hipStream_t st) {
+  if (a.mins) return a.scale_f16 ? launch_t<P, G, true, true>(a, st) : launch_t<P, G, true, false>(a, st);
+  return a.scale_f16 ? launch_t<P, G, false, true>(a, st) : launch_t<P, G, false, false>(a, st);
 }
 
 template <int G>
 hipError_t launch_g(const Gemv4Args& a, hipStream_t st) {
-  const bool few = (a.N0 + a.N1 + a.N2 + 15) / 16 <= 512;
-  if (a.M == 1) return few ? launch_t<1, 1, 1, G>(a, st) : launch_t<2, 1, 1, G>(a, st);
-  if (a.M <= 4) return few ? launch_t<1, 4, 1, G>(a, st) : launch_t<2, 4, 1, G>(a, st);
-  if (a.M <= 8) return few ? launch_t<1, 4, 2, G>(a, st) : launch_t<2, 4, 2, G>(a, st);
-  return few ? launch_t<1, 4, 4, G>(a, st) : launch_t<2, 4, 4, G>(a, st);
+  switch ((a.M + 3) / 4) {
+    case 1: return launch_p<1, G>(a, st);
+    case 2: return launch_p<2, G>(a, st);
+    case 3: return launch_p<3, G>(a, st);
+    default: return launch_p<4, G>(a, st);
+  }
 }
 
 }  // namespace
