@@ -35,8 +35,8 @@ typedef float f32x4_t __attribute__((ext_vector_type(4)));
 
 constexpr int kStep = 512;            // weights of a wave's step: four blocks of 128
 constexpr int kWaves = 8;
-constexpr int kTarget = 512;          // workgroups that a launch aims at, with up to kMaxTiles tiles of 16 rows each
-constexpr int kMaxTiles = 4;
+// Workgroups that a launch aims at, with up to kMaxTiles tiles of 16 rows each: two a CU for one token, one otherwise
+constexpr int kTargetOne = 512, kTarget = 256, kMaxTiles = 8;
 constexpr int kDigit = 528;           // bytes of a digit's row: 64 words of 8, and a pad that spreads 16 rows over the banks
 constexpr int kToken = 4 * kDigit;
 
@@ -68,6 +68,10 @@ __device__ inline long weight_operand(uint32_t w) {
   const uint32_t even = MINS ? w & 0x0f0f0f0fu : (w << 4 ^ 0x80808080u) & 0xf0f0f0f0u;
   const uint32_t odd = MINS ? w >> 4 & 0x0f0f0f0fu : (w ^ 0x80808080u) & 0xf0f0f0f0u;
   return (long)((uint64_t)odd << 32 | even);
+}
+
+__device__ inline i32x4_t pair(long a, long b) {
+  return i32x4_t{(int)(uint32_t)(uint64_t)a, (int)(uint32_t)((uint64_t)a >> 32), (int)(uint32_t)(uint64_t)b, (int)(uint32_t)((uint64_t)b >> 32)};
 }
 
 // floor(v + 0.5) in one instruction
@@ -123,8 +127,96 @@ __device__ __forceinline__ float block_f32(const float* x, const uint32_t* words
   return sum;
 }
 
+// A lane's eight values of x (its block's other 15 lanes hold the rest) as digits: d[0] of its even ones, d[1] of its
+// odd ones, digit q in d[.][q]; |x| < 2^e in the block, and a digit of weight 2^0 counts 2^(e - 30). Where not `on`, or
+// the block is not finite (returned), all are zero.
+__device__ inline bool digits(f32x4_t x0, f32x4_t x1, bool on, uint32_t (&d)[2][4], int& e) {
+  uint32_t top = 0;
+#pragma unroll
+  for (int i = 0; i < 4; i++) top = max(top, max(__float_as_uint(x0[i]) & 0x7fffffffu, __float_as_uint(x1[i]) & 0x7fffffffu));
+  auto dppmax = [&](auto ctrl) { top = max(top, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)top, decltype(ctrl)::value, 0xf, 0xf, false)); };
+  dppmax(std::integral_constant<int, kDppXor1>{});
+  dppmax(std::integral_constant<int, kDppXor2>{});
+  dppmax(std::integral_constant<int, kDppHalfMirror>{});
+  dppmax(std::integral_constant<int, kDppMirror>{});
+  const bool odd = top >= 0x7f800000u;
+  e = (int)(top >> 23) - 126;
+  const uint32_t use = on && !odd ? ~0u : 0u;  // (an infinity or NaN leaves some integer)
+  uint32_t y[2][4];
+#pragma unroll
+  for (int i = 0; i < 4; i++) {
+    const float u = i < 2 ? x0[2 * i] : x1[2 * i - 4], v = i < 2 ? x0[2 * i + 1] : x1[2 * i - 3];
+    y[0][i] = (((uint32_t)round_i32(ldexpf(u, 30 - e)) & use) + 0x80808080u) ^ 0x80808080u;  // signed base-256 digits
+    y[1][i] = (((uint32_t)round_i32(ldexpf(v, 30 - e)) & use) + 0x80808080u) ^ 0x80808080u;
+  }
+#pragma unroll
+  for (int u = 0; u < 2; u++) {  // dword of digit q = byte q of the four
+    const uint32_t p01 = __builtin_amdgcn_perm(y[u][1], y[u][0], 0x05010400u);
+    const uint32_t p23 = __builtin_amdgcn_perm(y[u][3], y[u][2], 0x05010400u);
+    const uint32_t q01 = __builtin_amdgcn_perm(y[u][1], y[u][0], 0x07030602u);
+    const uint32_t q23 = __builtin_amdgcn_perm(y[u][3], y[u][2], 0x07030602u);
+    d[u][0] = __builtin_amdgcn_perm(p23, p01, 0x05040100u);
+    d[u][1] = __builtin_amdgcn_perm(p23, p01, 0x07060302u);
+    d[u][2] = __builtin_amdgcn_perm(q23, q01, 0x05040100u);
+    d[u][3] = __builtin_amdgcn_perm(q23, q01, 0x07060302u);
+  }
+  return odd;
+}
+
+// four registers of the four lane groups transposed: afterwards w[i] of group g is what w[g] of group i was
+__device__ inline void transpose(uint32_t& a, uint32_t& b, uint32_t& c, uint32_t& d) {
+  auto ac = __builtin_amdgcn_permlane32_swap(a, c, false, false);
+  auto bd = __builtin_amdgcn_permlane32_swap(b, d, false, false);
+  auto lo = __builtin_amdgcn_permlane16_swap(ac[0], bd[0], false, false);
+  auto hi = __builtin_amdgcn_permlane16_swap(ac[1], bd[1], false, false);
+  a = lo[0];
+  b = lo[1];
+  c = hi[0];
+  d = hi[1];
+}
+
 __device__ inline __amdgpu_buffer_rsrc_t buffer(const void* p, size_t bytes) {
   return __builtin_amdgcn_make_buffer_rsrc((void*)p, (short)0, (int)(uint32_t)(bytes < 0xffffffffu ? bytes : 0xffffffffu), 0x00020000);
+}
+
+// The blocks of x that hold an infinity or a NaN, left out of a wave's sums red[wave][tile][16 rows][M] so far
+template <int G, bool MINS, bool F16>
+__device__ __forceinline__ void odd_blocks(const Gemv4Args& a, float* red, int T, int n0, int wave, int waves, int lane) {
+  const int n = lane & 15, g = lane >> 4, N = a.N0 + a.N1 + a.N2;
+  const int blocks = a.K >> 7, words = a.K >> 3, groups = a.K / G;
+#pragma unroll 1
+  for (int blk = 0; blk < blocks; blk++) {
+    if ((blk >> 2) % waves != wave) continue;
+#pragma unroll 1
+    for (int m = g; m < a.M; m += 4) {
+      const float* xp = a.x + (size_t)m * a.K + 128 * blk;
+      uint32_t top = 0;
+#pragma unroll 1
+      for (int k = 0; k < 128; k++) top = max(top, __float_as_uint(xp[k]) & 0x7fffffffu);
+      if (top < 0x7f800000u) continue;
+#pragma unroll 1
+      for (int u = 0; u < T; u++) {
+        const size_t r = min(n0 + 16 * u + n, N - 1);
+        red[(size_t)((wave * T + u) * 16 + n) * a.M + m] +=
+            block_f32<G, F16>(xp, a.codes + r * words + 16 * blk, a.scales, MINS ? a.mins : nullptr, r * groups + 128 / G * blk);
+      }
+    }
+  }
+}
+
+// The workgroup's rows: the waves' sums in their order
+__device__ __forceinline__ void store(const Gemv4Args& a, const float* red, int T, int n0, int waves) {
+  const int N = a.N0 + a.N1 + a.N2;
+  for (int i = threadIdx.x; i < T * 16 * a.M; i += blockDim.x) {
+    const int m = i / (T * 16), r = i % (T * 16), at = n0 + r;
+    if (at >= N) continue;
+    float y = 0.0f;
+    for (int k = 0; k < waves; k++) y += red[(size_t)(k * T * 16 + r) * a.M + m];
+    if (a.resid) y += a.resid[(size_t)m * N + at];
+    if (at < a.N0) a.out0[(size_t)m * a.N0 + at] = y;
+    else if (at < a.N0 + a.N1) a.out1[(size_t)m * a.N1 + at - a.N0] = y;
+    else a.out2[(size_t)m * a.N2 + at - a.N0 - a.N1] = y;
+  }
 }
 
 // P: groups of four tokens.
@@ -145,7 +237,7 @@ __global__ __launch_bounds__(64 * kWaves, P == 1 ? 4 : 2) void gemv4_kernel(Gemv
 
   long xd[P == 1 ? 1 : P][4][4];  // the operand of x: four words of each of the step's blocks (of one pass: read where used)
   int ex[P][4];        // the blocks' powers of two, of this lane's token 4 p + g
-  float xs[NG];        // the groups' sums of x: token 4 (n % 4) + n / 4, group 4 i + g of the step
+  float xs[NG];        // the groups' sums of x: token 4 (n % 4) + n / 4, group i of the step's block g
   bool odd_any = false;
   f32x4_t x0[4], x1[4];  // a pass's rows of x as loaded: lane 16 b + l has weights 8 l .. + 7 of block b
   auto load_x = [&](int step, int p) {
@@ -169,41 +261,14 @@ __global__ __launch_bounds__(64 * kWaves, P == 1 ? 4 : 2) void gemv4_kernel(Gemv
           continue;
         }
         const bool on = 4 * step + g < blocks;
-        uint32_t top = 0;
-#pragma unroll
-        for (int e = 0; e < 4; e++) top = max(top, max(__float_as_uint(x0[m][e]) & 0x7fffffffu, __float_as_uint(x1[m][e]) & 0x7fffffffu));
-        auto dppmax = [&](auto ctrl) { top = max(top, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)top, decltype(ctrl)::value, 0xf, 0xf, false)); };
-        dppmax(std::integral_constant<int, kDppXor1>{});
-        dppmax(std::integral_constant<int, kDppXor2>{});
-        dppmax(std::integral_constant<int, kDppHalfMirror>{});
-        dppmax(std::integral_constant<int, kDppMirror>{});
-        const bool odd = top >= 0x7f800000u;
+        uint32_t d[2][4];
+        int e;
+        const bool odd = digits(x0[m], x1[m], on, d, e);
         odd_any = odd_any || (on && odd);
-        const int e = (int)(top >> 23) - 126;  // |x| < 2^e
-        const uint32_t use = on && !odd ? ~0u : 0u;  // (an infinity or NaN leaves some integer)
-        uint32_t y[2][4];  // even weights, odd weights
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-          const float u = i < 2 ? x0[m][2 * i] : x1[m][2 * i - 4], v = i < 2 ? x0[m][2 * i + 1] : x1[m][2 * i - 3];
-          y[0][i] = (((uint32_t)round_i32(ldexpf(u, 30 - e)) & use) + 0x80808080u) ^ 0x80808080u;  // signed base-256 digits
-          y[1][i] = (((uint32_t)round_i32(ldexpf(v, 30 - e)) & use) + 0x80808080u) ^ 0x80808080u;
-        }
         if constexpr (MINS) {
           float t = ((x0[m][0] + x0[m][1]) + (x0[m][2] + x0[m][3])) + ((x1[m][0] + x1[m][1]) + (x1[m][2] + x1[m][3]));
           t = group_sum<G / 8>(t);
-          if (n % (G / 8) == 0) xsum[wave][4 * m + p][NG * g + n / (G / 8)] = use ? t : 0.0f;
-        }
-        uint32_t d[2][4];
-#pragma unroll
-        for (int u = 0; u < 2; u++) {  // dword of digit q = byte q of the four
-          const uint32_t p01 = __builtin_amdgcn_perm(y[u][1], y[u][0], 0x05010400u);
-          const uint32_t p23 = __builtin_amdgcn_perm(y[u][3], y[u][2], 0x05010400u);
-          const uint32_t q01 = __builtin_amdgcn_perm(y[u][1], y[u][0], 0x07030602u);
-          const uint32_t q23 = __builtin_amdgcn_perm(y[u][3], y[u][2], 0x07030602u);
-          d[u][0] = __builtin_amdgcn_perm(p23, p01, 0x05040100u);
-          d[u][1] = __builtin_amdgcn_perm(p23, p01, 0x07060302u);
-          d[u][2] = __builtin_amdgcn_perm(q23, q01, 0x05040100u);
-          d[u][3] = __builtin_amdgcn_perm(q23, q01, 0x07060302u);
+          if (n % (G / 8) == 0) xsum[wave][4 * m + p][NG * g + n / (G / 8)] = on && !odd ? t : 0.0f;
         }
 #pragma unroll
         for (int q = 0; q < 4; q++) *(uint2*)(dig + m * kToken + q * kDigit + 128 * g + 8 * n) = make_uint2(d[0][q], d[1][q]);
@@ -231,14 +296,14 @@ __global__ __launch_bounds__(64 * kWaves, P == 1 ? 4 : 2) void gemv4_kernel(Gemv
     if constexpr (MINS) {
       __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 #pragma unroll
-      for (int i = 0; i < NG; i++) xs[i] = (n & 3) < P ? xsum[wave][n][4 * i + g] : 0.0f;  // (row n: token 4 (n % 4) + n / 4)
+      for (int i = 0; i < NG; i++) xs[i] = (n & 3) < P ? xsum[wave][n][NG * g + i] : 0.0f;  // (row n: token 4 (n % 4) + n / 4)
     }
   };
 
   struct Tile {
     u32x4_t w[4];
     Scales<G, F16> s[4];
-    Scales<128, F16> lo[MINS ? NG : 1];
+    Scales<G, F16> lo;  // of block g
   };
   // The workgroup's rows as buffers: 32-bit offsets from its first (rows behind the last are the last again)
   const int rows = min(16 * T, N - n0);
@@ -253,21 +318,15 @@ __global__ __launch_bounds__(64 * kWaves, P == 1 ? 4 : 2) void gemv4_kernel(Gemv
   };
   auto load_lo = [&](Tile& x, int step, int t) {
     const int r = min(16 * t + n, rows - 1);
-    if constexpr (MINS)
-#pragma unroll
-      for (int i = 0; i < NG; i++) x.lo[i].load(rm, kScale * (r * groups + min(4 * NG * step + 4 * i + g, groups - 1)), 0);
+    if constexpr (MINS) x.lo.load(rm, kScale * (r * groups + NG * min(4 * step + g, blocks - 1)), 0);
   };
   // A tile's products; the next one's (step1, t1) loads go into the registers of each block as it is done
   auto multiply = [&](Tile& x, int step, int t, int step1, int t1) {
-    float acc[P];
-#pragma unroll
-    for (int p = 0; p < P; p++) acc[p] = 0.0f;
+    float acc[P], two[P];  // of the blocks so far; of the pair of blocks under way
+    f32x4_t lo = {0, 0, 0, 0};
     if constexpr (MINS) {
-      f32x4_t d = {0, 0, 0, 0};
 #pragma unroll
-      for (int i = 0; i < NG; i++) d = __builtin_amdgcn_mfma_f32_16x16x4f32(xs[i], x.lo[i].get(0), d, 0, 0, 0);
-#pragma unroll
-      for (int p = 0; p < P; p++) acc[p] = d[p];
+      for (int i = 0; i < NG; i++) lo = __builtin_amdgcn_mfma_f32_16x16x4f32(xs[i], x.lo.get(i), lo, 0, 0, 0);
       if (step1 < steps) load_lo(x, step1, t1);
     }
 #pragma unroll
@@ -282,27 +341,45 @@ __global__ __launch_bounds__(64 * kWaves, P == 1 ? 4 : 2) void gemv4_kernel(Gemv
 #pragma unroll
         for (int j = 0; j < 4; j++) xd[0][b][j] = *(const long*)(src + 128 * b + 8 * word_of<G>(j, g));
       }
+      float sum[P];
 #pragma unroll
       for (int i = 0; i < NG; i++) {
         const float s = x.s[b].get(i);
         i32x4_t d[P];
 #pragma unroll
         for (int p = 0; p < P; p++) d[p] = i32x4_t{0, 0, 0, 0};
+        if constexpr (G == 32) {
 #pragma unroll
-        for (int j = i * G / 32; j < (i + 1) * G / 32; j++)
+          for (int p = 0; p < P; p++) d[p] = __builtin_amdgcn_mfma_i32_16x16x32_i8(xd[p][b][i], w[i], d[p], 0, 0, 0);
+        } else {  // two words a lane at once
 #pragma unroll
-          for (int p = 0; p < P; p++) d[p] = __builtin_amdgcn_mfma_i32_16x16x32_i8(xd[p][b][j], w[j], d[p], 0, 0, 0);
+          for (int j = i * G / 32; j < (i + 1) * G / 32; j += 2)
+#pragma unroll
+            for (int p = 0; p < P; p++)
+              d[p] = __builtin_amdgcn_mfma_i32_16x16x64_i8(pair(xd[p][b][j], xd[p][b][j + 1]), pair(w[j], w[j + 1]), d[p], 0, 0, 0);
+        }
 #pragma unroll
         for (int p = 0; p < P; p++) {  // digits 0, 1 and 2, 3 as integers (|d| <= 2^21), then in f32
-          const float lo = (float)(d[p][0] + (d[p][1] << 8)), hi = (float)(d[p][2] + (d[p][3] << 8));
-          acc[p] = fmaf(ldexpf(fmaf(hi, 65536.0f, lo), ex[p][b]), s, acc[p]);
+          const float low = (float)(d[p][0] + (d[p][1] << 8)), hi = (float)(d[p][2] + (d[p][3] << 8));
+          const float all = fmaf(hi, 65536.0f, low);
+          sum[p] = i ? fmaf(all, s, sum[p]) : all * s;
         }
+      }
+#pragma unroll
+      for (int p = 0; p < P; p++) {  // (blocks 0 + 1) + (2 + 3)
+        const float v = ldexpf(sum[p], ex[p][b]);
+        two[p] = b & 1 ? two[p] + v : v;
+        if (b == 1) acc[p] = two[p];
+        if (b == 3) acc[p] += two[p];
       }
       // the sums of a block here, and not where a lane stores its part: all blocks' digits at once do not fit
 #pragma unroll
-      for (int p = 0; p < P; p++) asm volatile("" : "+v"(acc[p]));
+      for (int p = 0; p < P; p++) asm volatile("" : "+v"(two[p]));
       if (step1 < steps) load(x, step1, t1, b);
     }
+    if constexpr (MINS)
+#pragma unroll
+      for (int p = 0; p < P; p++) acc[p] += lo[p];
     float* to = red + (size_t)((wave * T + t) * 16 + n) * a.M + g;
 #pragma unroll
     for (int p = 0; p < P; p++)
@@ -330,38 +407,143 @@ __global__ __launch_bounds__(64 * kWaves, P == 1 ? 4 : 2) void gemv4_kernel(Gemv
       step = step1;
       t = t1;
     }
-    if (__any(odd_any)) {  // the blocks of x that hold an infinity or a NaN, left out so far
-#pragma unroll 1
-      for (int blk = 0; blk < blocks; blk++) {
-        if ((blk >> 2) % waves != wave) continue;
-#pragma unroll 1
-        for (int m = g; m < a.M; m += 4) {
-          const float* xp = a.x + (size_t)m * a.K + 128 * blk;
-          uint32_t top = 0;
-#pragma unroll 1
-          for (int k = 0; k < 128; k++) top = max(top, __float_as_uint(xp[k]) & 0x7fffffffu);
-          if (top < 0x7f800000u) continue;
-#pragma unroll 1
-          for (int u = 0; u < T; u++) {
-            const size_t r = min(n0 + 16 * u + n, N - 1);
-            red[(size_t)((wave * T + u) * 16 + n) * a.M + m] +=
-                block_f32<G, F16>(xp, a.codes + r * words + 16 * blk, a.scales, MINS ? a.mins : nullptr, r * groups + NG * blk);
-          }
-        }
-      }
-    }
+    if (__any(odd_any)) odd_blocks<G, MINS, F16>(a, red, T, n0, wave, waves, lane);
   }
   __syncthreads();
-  for (int i = threadIdx.x; i < T * 16 * a.M; i += blockDim.x) {
-    const int m = i / (T * 16), r = i % (T * 16), at = n0 + r;
-    if (at >= N) continue;
-    float y = 0.0f;
-    for (int k = 0; k < waves; k++) y += red[(size_t)(k * T * 16 + r) * a.M + m];
-    if (a.resid) y += a.resid[(size_t)m * N + at];
-    if (at < a.N0) a.out0[(size_t)m * a.N0 + at] = y;
-    else if (at < a.N0 + a.N1) a.out1[(size_t)m * a.N1 + at - a.N0] = y;
-    else a.out2[(size_t)m * a.N2 + at - a.N0 - a.N1] = y;
+  store(a, red, T, n0, waves);
+}
+
+// One token: the operand of x is block diagonal. Its row 4 b + q holds digit q of the step's block b, in the k of lane
+// group b and zeros elsewhere, so lane 16 g + n gets its row's sums over block g, and the joining, scaling and adding
+// of sums (half of the instructions with four tokens, of which three would be missing) is a quarter. A lane needs the
+// words of its own block: what 16-byte loads of 64 contiguous bytes a row bring is transposed between lane groups.
+template <int G, bool MINS, bool F16>
+__global__ __launch_bounds__(64 * kWaves, 4) void gemv4_one_kernel(Gemv4Args a, int T) {
+  constexpr int NG = 128 / G;
+  constexpr int kRow = 144;                             // bytes of a (block, digit) row: 16 words of 8, and a pad
+  constexpr int kBytes = 16 * kRow + 128;               // then zeros
+  __shared__ __align__(16) char lds[kWaves * kBytes];
+  __shared__ float red[kWaves * kMaxTiles * 16];
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const int n = lane & 15, g = lane >> 4;
+  const int N = a.N0 + a.N1 + a.N2, n0 = blockIdx.x * 16 * T;
+  const int steps = (a.K + kStep - 1) / kStep, waves = blockDim.x >> 6;
+  const int blocks = a.K >> 7, words = a.K >> 3, groups = a.K / G;
+  char* dig = lds + wave * kBytes;
+  const int rows = min(16 * T, N - n0);
+  constexpr int kScale = F16 ? 2 : 4;
+  const auto rw = buffer(a.codes + (size_t)n0 * words, (size_t)rows * words * 4);
+  const auto rs = buffer((const char*)a.scales + (size_t)n0 * groups * kScale, (size_t)rows * groups * kScale);
+  const auto rm = buffer((const char*)(MINS ? a.mins : a.scales) + (size_t)n0 * groups * kScale, (size_t)rows * groups * kScale);
+
+  i32x4_t xd[8];       // the operand of x: words 2 i, 2 i + 1 of the lane's block
+  int ex = 0;          // the block's power of two
+  float xs[NG];        // the sums of x over the block's groups, as row 0 of an operand
+  bool odd_any = false;
+  f32x4_t x0, x1;
+  u32x4_t w[4];
+  Scales<G, F16> sc, lo;
+  auto load_x = [&](int step) {
+    const float* xp = a.x + 128 * min(4 * step + g, blocks - 1) + 8 * n;
+    x0 = *(const f32x4_t*)xp;
+    x1 = *(const f32x4_t*)(xp + 4);
+  };
+  auto load = [&](int step, int t) {
+    const int r = min(16 * t + n, rows - 1);
+#pragma unroll
+    for (int b = 0; b < 4; b++)  // past the end: x counts as zero there
+      w[b] = __builtin_bit_cast(u32x4_t, __builtin_amdgcn_raw_buffer_load_b128(rw, r * words * 4 + 16 * g, 64 * min(4 * step + b, blocks - 1), 0));
+    const int at = kScale * (r * groups + NG * min(4 * step + g, blocks - 1));
+    sc.load(rs, at, 0);
+    if constexpr (MINS) lo.load(rm, at, 0);
+  };
+  if (wave < steps) {
+    load_x(wave);
+    __builtin_amdgcn_sched_barrier(0);
+    load(wave, 0);
+    __builtin_amdgcn_sched_barrier(0);
+    if (lane < 8) *(uint4*)(dig + 16 * kRow + 16 * lane) = make_uint4(0, 0, 0, 0);
+#pragma unroll 1
+    for (int step = wave, t = 0; step < steps;) {
+      if (t == 0) {
+        if (step != wave) load_x(step);
+        const bool on = 4 * step + g < blocks;
+        uint32_t d[2][4];
+        int e;
+        const bool odd = digits(x0, x1, on, d, e);
+        odd_any = odd_any || (on && odd);
+        ex = odd ? 0 : e - (MINS ? 30 : 34);
+        if constexpr (MINS) {
+          float v = ((x0[0] + x0[1]) + (x0[2] + x0[3])) + ((x1[0] + x1[1]) + (x1[2] + x1[3]));
+          v = group_sum<G / 8>(v);
+          v = on && !odd ? v : 0.0f;
+#pragma unroll
+          for (int i = 0; i < NG; i++) {
+            const float all = __shfl(v, 16 * g + (G / 8) * i);
+            xs[i] = n == 0 ? all : 0.0f;
+          }
+        }
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll
+        for (int q = 0; q < 4; q++) *(uint2*)(dig + (4 * g + q) * kRow + 8 * n) = make_uint2(d[0][q], d[1][q]);
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+        const char* src = dig + ((n >> 2) == g ? n * kRow : 16 * kRow);
+#pragma unroll
+        for (int i = 0; i < 8; i++) xd[i] = *(const i32x4_t*)(src + 16 * i);
+      }
+      const bool end = t + 1 == T;
+      const int step1 = end ? step + waves : step, t1 = end ? 0 : t + 1;
+      u32x4_t v[4];
+      float s[NG], m[NG];
+#pragma unroll
+      for (int b = 0; b < 4; b++) v[b] = w[b];
+#pragma unroll
+      for (int i = 0; i < NG; i++) {
+        s[i] = sc.get(i);
+        m[i] = MINS ? lo.get(i) : 0.0f;
+      }
+#pragma unroll
+      for (int j = 0; j < 4; j++) {
+        uint32_t p0 = v[0][j], p1 = v[1][j], p2 = v[2][j], p3 = v[3][j];
+        transpose(p0, p1, p2, p3);
+        v[0][j] = p0;
+        v[1][j] = p1;
+        v[2][j] = p2;
+        v[3][j] = p3;
+      }
+      if (step1 < steps) load(step1, t1);
+      float acc = 0.0f;
+#pragma unroll
+      for (int i = 0; i < NG; i++) {
+        i32x4_t d = {0, 0, 0, 0};
+#pragma unroll
+        for (int j = i * G / 16; j < (i + 1) * G / 16; j++)
+          d = __builtin_amdgcn_mfma_i32_16x16x64_i8(xd[j], pair(weight_operand<MINS>(v[j >> 1][2 * (j & 1)]), weight_operand<MINS>(v[j >> 1][2 * (j & 1) + 1])), d, 0, 0, 0);
+        const float all = fmaf((float)(d[2] + (d[3] << 8)), 65536.0f, (float)(d[0] + (d[1] << 8)));
+        acc = i ? fmaf(all, s[i], acc) : all * s[i];
+      }
+      acc = ldexpf(acc, ex);
+      float2 r = pair16(acc);
+      r = pair32(r.x + r.y);
+      acc = r.x + r.y;  // the step's four blocks
+      if constexpr (MINS) {
+        f32x4_t d = {0, 0, 0, 0};
+#pragma unroll
+        for (int i = 0; i < NG; i++) d = __builtin_amdgcn_mfma_f32_16x16x4f32(xs[i], m[i], d, 0, 0, 0);
+        acc += d[0];  // (of lanes 0 to 15)
+      }
+      float* to = red + (wave * T + t) * 16 + n;
+      if (g == 0) *to = step == wave ? acc : *to + acc;
+      step = step1;
+      t = t1;
+    }
+    if (__any(odd_any)) odd_blocks<G, MINS, F16>(a, red, T, n0, wave, waves, lane);
   }
+  __syncthreads();
+  store(a, red, T, n0, waves);
 }
 
 template <int P, int G, bool MINS, bool F16>
@@ -373,6 +555,20 @@ hipError_t launch_t(const Gemv4Args& a, hipStream_t st) {
   return hipGetLastError();
 }
 
+template <int G, bool MINS, bool F16>
+hipError_t launch_one_t(const Gemv4Args& a, hipStream_t st) {
+  const int tiles = (a.N0 + a.N1 + a.N2 + 15) / 16, waves = std::min((a.K + kStep - 1) / kStep, kWaves);
+  const int T = std::min(kMaxTiles, (tiles + kTargetOne - 1) / kTargetOne);
+  hipLaunchKernelGGL((gemv4_one_kernel<G, MINS, F16>), dim3((tiles + T - 1) / T), dim3(64 * waves), 0, st, a, T);
+  return hipGetLastError();
+}
+
+template <int G>
+hipError_t launch_one(const Gemv4Args& a, hipStream_t st) {
+  if (a.mins) return a.scale_f16 ? launch_one_t<G, true, true>(a, st) : launch_one_t<G, true, false>(a, st);
+  return a.scale_f16 ? launch_one_t<G, false, true>(a, st) : launch_one_t<G, false, false>(a, st);
+}
+
 template <int P, int G>
 hipError_t launch_p(const Gemv4Args& a, hipStream_t st) {
   if (a.mins) return a.scale_f16 ? launch_t<P, G, true, true>(a, st) : launch_t<P, G, true, false>(a, st);
@@ -381,6 +577,7 @@ hipError_t launch_p(const Gemv4Args& a, hipStream_t st) {
 
 template <int G>
 hipError_t launch_g(const Gemv4Args& a, hipStream_t st) {
+  if (a.M == 1) return launch_one<G>(a, st);
   switch ((a.M + 3) / 4) {
     case 1: return launch_p<1, G>(a, st);
     case 2: return launch_p<2, G>(a, st);
