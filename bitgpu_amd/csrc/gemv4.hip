@@ -1,21 +1,26 @@
 // 4-bit projections of up to 16 rows (bg_linear.h states the weight's format).
 //
-//   contraction  on the int8 matrix cores (v_mfma_i32_16x16x32_i8), exactly: a row of x becomes, 128 weights at a time,
-//           a 31-bit fixed-point number over the block's largest power of two in four signed int8 digits; a
-//           weight's code, its top bit turned, is 16 (c - 8) as the high half of a signed byte (two bit operations
-//           a word give its odd codes and, shifted, its even ones). The operand of x has four rows a token, one a
-//           digit, so a product takes four tokens; its result leaves lane 16 g + n with the four digit sums of
-//           weight row n and token g, exact integers that are joined in f32 once a scale group, scaled back and
-//           multiplied by the group's scale. With minima, codes enter as they are (c), and the minima times the
-//           groups' sums of x, 16 tokens at once, are a product on the f32 matrix cores. What a row of x gives does
-//           not depend on the rows beside it: how K is split depends on K alone, and the rest is exact.
+//   contraction  on the int8 matrix cores, exactly: a row of x becomes, 128 weights at a time, a 31-bit fixed-point
+//           number over the block's largest power of two in four signed int8 digits (x is rounded to 2^-31 of its
+//           block's largest, below the rounding of an f32 sum over the block); a weight's code, its top bit turned, is
+//           16 (c - 8) as the high half of a signed byte (two bit operations a word give its odd codes and, shifted,
+//           its even ones). The operand of x has four rows a token, one a digit, so a product takes four tokens; its
+//           result leaves lane 16 g + n with the four digit sums of weight row n and token g, exact integers that are
+//           joined in f32 once a scale group, multiplied by the group's scale and scaled back once a block. With
+//           minima, codes enter as they are (c), and the minima times the groups' sums of x, 16 tokens at once, are a
+//           product on the f32 matrix cores.
+//   order   what a row of x gives does not depend on the rows beside it: how K is split depends on K alone, the integers
+//           are exact, and the f32 sums are taken in one order, groups, blocks (0 + 1) + (2 + 3), steps, waves.
 //   lanes   16 weight rows x 128 weights: lane 16 g + n holds words 4 g .. 4 g + 3 of row n (one 16-byte load). A
-//           product contracts one word of each of the four lane groups: of the same scale group with groups of 128;
-//           for 64 and 32 the words change lane groups (v_permlane32_swap, v_permlane16_swap) until that holds. The
-//           digits of x are read in the order that this gives.
+//           product contracts words of the four lane groups: of the same scale group with groups of 128; for 64 and 32
+//           the words change lane groups (v_permlane32_swap, v_permlane16_swap) until that holds. The digits of x are
+//           read in the order that this gives.
 //   split   the waves of a workgroup split K, 512 weights at a time. A wave prepares x for its 512 once, through LDS
 //           into registers, and runs the workgroup's tiles of 16 rows over it, the next tile's weights and scales in
 //           flight while one is multiplied; the parts meet in LDS at the end.
+//   bounds  one token: 24576 rows of K = 4096 in groups of 32 with minima (63 MB) 13.4 us, 4.7 TB/s, what a large copy
+//           reaches; 4096 x 4096 in groups of 128 (8.7 MB) 5.1 us, the latency of a launch and one pass over K. More tokens:
+//           instructions, a third of them x's digits: ten rows of K = 4096, N = 16480 18 us.
 //   values  a block of x with an infinity or a NaN is summed directly in f32.
 #include <hip/hip_fp16.h>
 
@@ -35,7 +40,9 @@ typedef float f32x4_t __attribute__((ext_vector_type(4)));
 
 constexpr int kStep = 512;            // weights of a wave's step: four blocks of 128
 constexpr int kWaves = 8;
-// Workgroups that a launch aims at, with up to kMaxTiles tiles of 16 rows each: two a CU for one token, one otherwise
+// Workgroups that a launch aims at, with up to kMaxTiles tiles of 16 rows each. One token, two a CU: 4096 x 4096 takes
+// 5.1 us and 6176 x 2048 6.5 us, with half as many 5.1 and 7.0, with twice as many 5.1 and 6.3 (but 24576 rows of 4096
+// 13.9 against 13.4). More tokens prepare x longer, so one a CU: ten rows of 16480 x 4096 18 us, with half 23, twice 25.
 constexpr int kTargetOne = 512, kTarget = 256, kMaxTiles = 8;
 constexpr int kDigit = 528;           // bytes of a digit's row: 64 words of 8, and a pad that spreads 16 rows over the banks
 constexpr int kToken = 4 * kDigit;
