@@ -37,11 +37,11 @@ try:
 except ImportError:  # the host-only functions (tables, plans, snapshot checks) need no torch
     torch = None
 
-from ._args import _f32, _int32, _ptr, _rows_ptr, _stream
+from ._args import _f32, _getDevice, _int32, _ptr, _rows_ptr, _stream
 from ._lib import (BG_E_INVALID, BG_E_STATE, BG_K, BG_KSCALE, BG_ROPE_ABSOLUTE, BG_ROPE_SLOT, BG_V, BG_VSCALE,
                    KV_DTYPES, BitgpuError, check, lib)
-from .linear import (FourBitWeight, LinearBatch, LinearStateCache, _fused_mm4, _resid_mm4, linear_attention,
-                     linear_layer_attention, linear_prologue)
+from .linear import (FourBitWeight, LinearBatch, LinearStateCache, _between, _fused_mm4, _layer_ptrs, _on, _resid_mm4,
+                     linear_attention, linear_layer_attention, linear_prologue)
 
 __all__ = ["KvCache", "attention", "qkv_prologue", "layer_attention", "hybrid_full_attention",
            "rope_tables", "evict_plan", "ring_map", "validate_snapshot", "OneBitWeight", "fused_mm", "resid_mm",
@@ -795,8 +795,43 @@ def linear_block(cache: LinearStateCache, li: int, batch: LinearBatch, n1, h, w_
     M = 1 if n1.dim() == 1 else n1.shape[0]
     if M != batch.n_tokens:
         raise ValueError(f"bitgpu_amd: n1 holds {M} rows, the batch has {batch.n_tokens} new rows")
-    new = n1.new_empty
-    qkv, z, ba = new((M, cache.channels)), new((M, Hv, DV)), new((M, 2 * Hv))
-    fused_mm(w_in, n1, [qkv, z, ba])
-    att = linear_layer_attention(cache, li, batch, qkv, ba[:, Hv:], ba[:, :Hv], conv_weight, a_log, dt_bias, z, norm, eps)
-    return resid_mm(w_out, att.view(*n1.shape[:-1], Hv * DV), h)
+    _f32(n1, "n1")
+    _f32(h, "h")
+    dev, st, L = cache.index, _stream(), lib()
+    if n1.get_device() != dev or h.get_device() != dev or dev != _getDevice():
+        raise ValueError(f"bitgpu_amd: expected tensors on cuda:{dev}, the current device")
+    if n1.shape[-1] != w_in.K or h.numel() != M * w_out.N:
+        raise ValueError(f"bitgpu_amd: n1 must hold [{M}, {w_in.K}] and h [{M}, {w_out.N}], got {list(n1.shape)} and {list(h.shape)}")
+    x, res = _ptr(n1), _ptr(h)
+    weights = _layer_ptrs(cache, conv_weight, a_log, dt_bias, norm)
+    # one piece of memory for what lies between the launches: qkv, z, att | b, a (interleaved rows) and the prologue's
+    out, wide, Z = n1.new_empty((*n1.shape[:-1], w_out.N)), cache.channels, Hv * DV
+    room = n1.new_empty(M * (2 * wide + 2 * Z + 4 * Hv))
+    qkv = room.data_ptr()
+    z = qkv + 4 * M * wide
+    att = z + 4 * M * Z
+    inner = att + 4 * M * Z
+    ba = inner + 4 * M * (wide + 2 * Hv)
+    if isinstance(w_in, FourBitWeight):
+        _on(w_in)
+        rc = L.bg_gemv4_split(x, M, w_in.K, *w_in._w, wide, Z, 2 * Hv, qkv, z, ba, st)
+    else:
+        _one_row(M)
+        rc = L.bg_gemv_split(x, w_in.K, _ptr(w_in.sign), _ptr(w_in.scales), wide, Z, 2 * Hv, qkv, z, ba, st)
+    if rc:
+        check(rc)
+    _between(cache, li, batch, qkv, ba + 4 * Hv, ba, 2 * Hv, weights, z, eps, inner, att, st)
+    if isinstance(w_out, FourBitWeight):
+        _on(w_out)
+        rc = L.bg_gemv4_resid(att, M, Z, *w_out._w, w_out.N, res, out.data_ptr(), st)
+    else:
+        _one_row(M)
+        rc = L.bg_gemv_resid(att, Z, _ptr(w_out.sign), _ptr(w_out.scales), w_out.N, res, out.data_ptr(), st)
+    if rc:
+        check(rc)
+    return out
+
+
+def _one_row(M):
+    if M != 1:
+        raise ValueError(f"bitgpu_amd: a 1-bit weight's product takes one row, got {M}")
