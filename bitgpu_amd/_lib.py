@@ -87,8 +87,9 @@ SIGNATURES = [
     ("bg_linear_batch_set", _i32, [_vp, _i32, _vp, _vp, _vp, _vp]),
     ("bg_linear_prologue", _i32, [_vp, _i32, _vp, _vp, _vp, _vp, _vp, _i32] + [_vp] * 8),
     ("bg_linear_attention", _i32, [_vp, _i32, _vp, _vp, _vp, _vp, _vp, _i32, _vp, _f32, _vp, _vp, _f32, _vp, _vp]),
-    ("bg_gemv4_split", _i32, [_vp, _i32, _i32, _vp, _vp, _vp, _i32, _i32, _i32, _i32, _i32, _vp, _vp, _vp, _vp]),
-    ("bg_gemv4_resid", _i32, [_vp, _i32, _i32, _vp, _vp, _vp, _i32, _i32, _i32, _vp, _vp, _vp]),
+    ("bg_gemv4_workspace", C.c_int64, [_i32, _i32]),
+    ("bg_gemv4_split", _i32, [_vp, _i32, _i32, _vp, _vp, _vp, _i32, _i32, _i32, _i32, _i32, _vp, _vp, _vp, _vp, _vp]),
+    ("bg_gemv4_resid", _i32, [_vp, _i32, _i32, _vp, _vp, _vp, _i32, _i32, _i32, _vp, _vp, _vp, _vp]),
 ]
 
 

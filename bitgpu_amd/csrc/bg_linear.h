@@ -93,7 +93,9 @@ struct Gemv4Args {
   int N0, N1, N2;
   float *out0, *out1, *out2;
   const float* resid;
+  char* room;  // of gemv4_room bytes: x prepared for more than four rows
 };
+size_t gemv4_room(int M, int K);
 hipError_t launch_gemv4(const Gemv4Args& a, hipStream_t st);
 
 }  // namespace bg

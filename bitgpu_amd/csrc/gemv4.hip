@@ -15,12 +15,16 @@
 //           product contracts words of the four lane groups: of the same scale group with groups of 128; for 64 and 32
 //           the words change lane groups (v_permlane32_swap, v_permlane16_swap) until that holds. The digits of x are
 //           read in the order that this gives.
-//   split   the waves of a workgroup split K, 512 weights at a time. A wave prepares x for its 512 once, through LDS
-//           into registers, and runs the workgroup's tiles of 16 rows over it, the next tile's weights and scales in
-//           flight while one is multiplied; the parts meet in LDS at the end.
+//   split   the waves of a workgroup split K, 512 weights at a time. A wave has x for its 512 in registers (or LDS) and
+//           runs the workgroup's tiles of 16 rows over it, the next tile's weights and scales in flight while one is
+//           multiplied; the parts meet in LDS at the end.
+//   x       up to four tokens: every wave prepares x for its 512, through LDS. More: a kernel of its own does, once for
+//           all workgroups, in the order in which they read it. That launch takes 2.5 us (five rows of 4096 x 4096 8.4
+//           us, four 6.5), but 16 rows prepared in every workgroup took longer than all products: 15 rows of K = 6144,
+//           N = 4096 22 us, so 11 + 4.7.
 //   bounds  one token: 24576 rows of K = 4096 in groups of 32 with minima (63 MB) 13.4 us, 4.7 TB/s, what a large copy
 //           reaches; 4096 x 4096 in groups of 128 (8.7 MB) 5.1 us, the latency of a launch and one pass over K. More tokens:
-//           instructions, a third of them x's digits: ten rows of K = 4096, N = 16480 18 us.
+//           the joining of the integers: ten rows of K = 4096, N = 16480 16.6 + 2.6 us.
 //   values  a block of x with an infinity or a NaN is summed directly in f32.
 #include <hip/hip_fp16.h>
 
@@ -42,10 +46,16 @@ constexpr int kStep = 512;            // weights of a wave's step: four blocks o
 constexpr int kWaves = 8;
 // Workgroups that a launch aims at, with up to kMaxTiles tiles of 16 rows each. One token, two a CU: 4096 x 4096 takes
 // 5.1 us and 6176 x 2048 6.5 us, with half as many 5.1 and 7.0, with twice as many 5.1 and 6.3 (but 24576 rows of 4096
-// 13.9 against 13.4). More tokens prepare x longer, so one a CU: ten rows of 16480 x 4096 18 us, with half 23, twice 25.
+// 13.9 against 13.4). More tokens prepare x longer, so one a CU: 16 rows of 16480 x 4096 21 us, with twice as many 28;
+// waves of half as many: 25.
 constexpr int kTargetOne = 512, kTarget = 256, kMaxTiles = 8;
 constexpr int kDigit = 528;           // bytes of a digit's row: 64 words of 8, and a pad that spreads 16 rows over the banks
 constexpr int kToken = 4 * kDigit;
+// x prepared for more than four tokens: of a step of 512 weights, kPassBytes for every four tokens (operands
+// [block][word pair][lane], 16 bytes each, then powers of two [token][block]), behind all of them kSumBytes a step (the
+// groups' sums [16 rows][block][group])
+constexpr int kOperand = 8192, kPassBytes = kOperand + 64, kSumBytes = 1024;
+constexpr int kOdd = 0x7fffffff;      // the power of two of a block with an infinity or a NaN (its digits are zero)
 
 // The word of a 128-weight block (0 to 15) that lane group g holds as its j-th after the exchange.
 template <int G>
@@ -170,6 +180,12 @@ __device__ inline bool digits(f32x4_t x0, f32x4_t x1, bool on, uint32_t (&d)[2][
   return odd;
 }
 
+// the sum over a lane's scale group, in all of the group's lanes
+template <int G>
+__device__ inline float block_sums(f32x4_t x0, f32x4_t x1) {
+  return group_sum<G / 8>(((x0[0] + x0[1]) + (x0[2] + x0[3])) + ((x1[0] + x1[1]) + (x1[2] + x1[3])));
+}
+
 // four registers of the four lane groups transposed: afterwards w[i] of group g is what w[g] of group i was
 __device__ inline void transpose(uint32_t& a, uint32_t& b, uint32_t& c, uint32_t& d) {
   auto ac = __builtin_amdgcn_permlane32_swap(a, c, false, false);
@@ -226,13 +242,43 @@ __device__ __forceinline__ void store(const Gemv4Args& a, const float* red, int 
   }
 }
 
+// x of more than four tokens, prepared once for all workgroups in the order in which they read it: a wave takes 512
+// weights of a token (of 4 P, those behind the last are zero).
+template <int G, bool MINS>
+__global__ __launch_bounds__(64) void gemv4_digits_kernel(Gemv4Args a, int P) {
+  constexpr int NG = 128 / G;
+  const int lane = threadIdx.x, n = lane & 15, g = lane >> 4, step = blockIdx.x, token = blockIdx.y;
+  const int steps = (a.K + kStep - 1) / kStep, blocks = a.K >> 7;
+  const bool on = token < a.M && 4 * step + g < blocks;
+  const float* xp = a.x + (size_t)min(token, a.M - 1) * a.K + 128 * min(4 * step + g, blocks - 1) + 8 * n;
+  const f32x4_t x0 = *(const f32x4_t*)xp, x1 = *(const f32x4_t*)(xp + 4);
+  uint32_t d[2][4];
+  int e;
+  const bool odd = digits(x0, x1, on, d, e);
+  char* to = a.room + ((size_t)step * P + (token >> 2)) * kPassBytes;
+  // word n of block g: the j-th that lane group `at` holds (word_of)
+  const int j = G == 128 ? n & 3 : G == 64 ? 2 * (n >> 3) + (n & 1) : n >> 2;
+  const int at = G == 128 ? n >> 2 : G == 64 ? ((n >> 2) & 1) + 2 * ((n >> 1) & 1) : n & 3;
+  if (token < 4 * P) {
+#pragma unroll
+    for (int q = 0; q < 4; q++)
+      *(uint2*)(to + (2 * g + (j >> 1)) * 1024 + (16 * at + 4 * (token & 3) + q) * 16 + 8 * (j & 1)) = make_uint2(d[0][q], d[1][q]);
+    if (n == 0) ((int*)(to + kOperand))[4 * (token & 3) + g] = on && odd ? kOdd : odd ? 0 : e - (MINS ? 30 : 34);
+  }
+  if constexpr (MINS) {
+    const float t = block_sums<G>(x0, x1);
+    float* sums = (float*)(a.room + (size_t)steps * P * kPassBytes + (size_t)step * kSumBytes);
+    if (n % (G / 8) == 0) sums[((4 * (token & 3) + (token >> 2)) * 4 + g) * NG + n / (G / 8)] = on && !odd ? t : 0.0f;
+  }
+}
+
 // P: groups of four tokens.
 template <int P, int G, bool MINS, bool F16>
 __global__ __launch_bounds__(64 * kWaves, P == 1 ? 4 : 2) void gemv4_kernel(Gemv4Args a, int T) {
   constexpr int NG = 128 / G;
   extern __shared__ __align__(16) char lds[];
   __shared__ int exps[kWaves][4][4];
-  __shared__ float xsum[MINS ? kWaves : 1][16][4 * NG];
+  __shared__ float xsum[MINS && P == 1 ? kWaves : 1][4][4 * NG];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int n = lane & 15, g = lane >> 4;
   const int N = a.N0 + a.N1 + a.N2, n0 = blockIdx.x * 16 * T;
@@ -240,70 +286,76 @@ __global__ __launch_bounds__(64 * kWaves, P == 1 ? 4 : 2) void gemv4_kernel(Gemv
   const int blocks = a.K >> 7, words = a.K >> 3, groups = a.K / G;
   const int held = min(a.M, 4);                         // tokens of the digits in LDS, then zeros for the others
   char* dig = lds + wave * (held * kToken + kDigit);
-  float* red = (float*)(lds + waves * (held * kToken + kDigit));  // [wave][tile][16 rows][M]
+  float* red = (float*)(lds + (P == 1 ? waves * (held * kToken + kDigit) : 0));  // [wave][tile][16 rows][M]
 
-  long xd[P == 1 ? 1 : P][4][4];  // the operand of x: four words of each of the step's blocks (of one pass: read where used)
+  long xd[P][4][4];    // the operand of x: four words of each of the step's blocks (of one pass: read where used)
   int ex[P][4];        // the blocks' powers of two, of this lane's token 4 p + g
   float xs[NG];        // the groups' sums of x: token 4 (n % 4) + n / 4, group i of the step's block g
   bool odd_any = false;
-  f32x4_t x0[4], x1[4];  // a pass's rows of x as loaded: lane 16 b + l has weights 8 l .. + 7 of block b
-  auto load_x = [&](int step, int p) {
+  f32x4_t x0[4], x1[4];  // the rows of x as loaded: lane 16 b + l has weights 8 l .. + 7 of block b
+  auto load_x = [&](int step) {
 #pragma unroll
     for (int m = 0; m < 4; m++) {
-      if (4 * p + m >= a.M) break;
-      const float* xp = a.x + (size_t)(4 * p + m) * a.K + 128 * min(4 * step + g, blocks - 1) + 8 * n;
+      if (m >= a.M) break;
+      const float* xp = a.x + (size_t)m * a.K + 128 * min(4 * step + g, blocks - 1) + 8 * n;
       x0[m] = *(const f32x4_t*)xp;
       x1[m] = *(const f32x4_t*)(xp + 4);
     }
   };
-  auto prepare = [&](int step) {  // x of its first pass is loaded
+  auto prepare = [&](int step) {  // four tokens: x is loaded
     for (int i = lane; i < kDigit / 4; i += 64) ((int*)(dig + held * kToken))[i] = 0;
+#pragma unroll
+    for (int m = 0; m < 4; m++) {
+      if (m >= a.M) {
+        if constexpr (MINS)
+          if (lane < 4 * NG) xsum[wave][m][lane] = 0.0f;
+        continue;
+      }
+      const bool on = 4 * step + g < blocks;
+      uint32_t d[2][4];
+      int e;
+      const bool odd = digits(x0[m], x1[m], on, d, e);
+      odd_any = odd_any || (on && odd);
+      if constexpr (MINS) {
+        const float t = block_sums<G>(x0[m], x1[m]);
+        if (n % (G / 8) == 0) xsum[wave][m][NG * g + n / (G / 8)] = on && !odd ? t : 0.0f;
+      }
+#pragma unroll
+      for (int q = 0; q < 4; q++) *(uint2*)(dig + m * kToken + q * kDigit + 128 * g + 8 * n) = make_uint2(d[0][q], d[1][q]);
+      if (n == 0) exps[wave][m][g] = odd ? 0 : e - (MINS ? 30 : 34);
+    }
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+#pragma unroll
+    for (int b = 0; b < 4; b++) ex[0][b] = g < a.M ? exps[wave][g][b] : 0;
+    if constexpr (MINS)
+#pragma unroll
+      for (int i = 0; i < NG; i++) xs[i] = (n & 3) == 0 ? xsum[wave][n >> 2][NG * g + i] : 0.0f;
+  };
+  auto take = [&](int step) {  // more tokens: as gemv4_digits_kernel left it
+    const char* at = a.room + (size_t)step * P * kPassBytes;
 #pragma unroll
     for (int p = 0; p < P; p++) {
 #pragma unroll
-      for (int m = 0; m < 4; m++) {
-        if (4 * p + m >= a.M) {
-          if constexpr (MINS)
-            if (lane < 4 * NG) xsum[wave][4 * m + p][lane] = 0.0f;
-          continue;
-        }
-        const bool on = 4 * step + g < blocks;
-        uint32_t d[2][4];
-        int e;
-        const bool odd = digits(x0[m], x1[m], on, d, e);
-        odd_any = odd_any || (on && odd);
-        if constexpr (MINS) {
-          float t = ((x0[m][0] + x0[m][1]) + (x0[m][2] + x0[m][3])) + ((x1[m][0] + x1[m][1]) + (x1[m][2] + x1[m][3]));
-          t = group_sum<G / 8>(t);
-          if (n % (G / 8) == 0) xsum[wave][4 * m + p][NG * g + n / (G / 8)] = on && !odd ? t : 0.0f;
-        }
+      for (int b = 0; b < 4; b++)
 #pragma unroll
-        for (int q = 0; q < 4; q++) *(uint2*)(dig + m * kToken + q * kDigit + 128 * g + 8 * n) = make_uint2(d[0][q], d[1][q]);
-        if (n == 0) exps[wave][m][g] = odd ? 0 : e - (MINS ? 30 : 34);
-      }
-      __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-      __builtin_amdgcn_wave_barrier();
-      __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-      if (p + 1 < P) load_x(step, p + 1);
-      const int token = n >> 2;  // of the operand's row n; its digit is n & 3
-      const bool there = token < held && 4 * p + token < a.M;
-      const char* src = dig + (there ? token * kToken + (n & 3) * kDigit : held * kToken);
+        for (int j = 0; j < 4; j += 2) {
+          const i32x4_t v = *(const i32x4_t*)(at + p * kPassBytes + (2 * b + j / 2) * 1024 + lane * 16);
+          xd[p][b][j] = (long)((uint64_t)(uint32_t)v[1] << 32 | (uint32_t)v[0]);
+          xd[p][b][j + 1] = (long)((uint64_t)(uint32_t)v[3] << 32 | (uint32_t)v[2]);
+        }
+      const i32x4_t e = *(const i32x4_t*)(at + p * kPassBytes + kOperand + g * 16);
 #pragma unroll
       for (int b = 0; b < 4; b++) {
-#pragma unroll
-        for (int j = 0; j < 4; j++)
-          if constexpr (P > 1) xd[p][b][j] = *(const long*)(src + 128 * b + 8 * word_of<G>(j, g));
-        ex[p][b] = 4 * p + g < a.M ? exps[wave][g][b] : 0;
+        ex[p][b] = e[b];
+        odd_any = odd_any || e[b] == kOdd;
       }
-      __builtin_amdgcn_sched_barrier(0);
-      // read before the next pass writes: a wave's LDS accesses complete in order
-      __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-      __builtin_amdgcn_wave_barrier();
     }
     if constexpr (MINS) {
-      __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+      const float* sums = (const float*)(a.room + (size_t)steps * P * kPassBytes + (size_t)step * kSumBytes) + (n * 4 + g) * NG;
 #pragma unroll
-      for (int i = 0; i < NG; i++) xs[i] = (n & 3) < P ? xsum[wave][n][NG * g + i] : 0.0f;  // (row n: token 4 (n % 4) + n / 4)
+      for (int i = 0; i < NG; i++) xs[i] = sums[i];
     }
   };
 
@@ -396,7 +448,8 @@ __global__ __launch_bounds__(64 * kWaves, P == 1 ? 4 : 2) void gemv4_kernel(Gemv
   if (wave < steps) {
     // x first: it is needed first, and loads arrive in order
     Tile x;
-    load_x(wave, 0);
+    if constexpr (P == 1) load_x(wave);
+    else take(wave);
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int b = 0; b < 4; b++) load(x, wave, 0, b);
@@ -405,8 +458,12 @@ __global__ __launch_bounds__(64 * kWaves, P == 1 ? 4 : 2) void gemv4_kernel(Gemv
 #pragma unroll 1
     for (int step = wave, t = 0; step < steps;) {
       if (t == 0) {
-        if (step != wave) load_x(step, 0);
-        prepare(step);
+        if constexpr (P == 1) {
+          if (step != wave) load_x(step);
+          prepare(step);
+        } else if (step != wave) {
+          take(step);
+        }
       }
       const bool end = t + 1 == T;
       const int step1 = end ? step + waves : step, t1 = end ? 0 : t + 1;
@@ -481,8 +538,7 @@ __global__ __launch_bounds__(64 * kWaves, 4) void gemv4_one_kernel(Gemv4Args a, 
         odd_any = odd_any || (on && odd);
         ex = odd ? 0 : e - (MINS ? 30 : 34);
         if constexpr (MINS) {
-          float v = ((x0[0] + x0[1]) + (x0[2] + x0[3])) + ((x1[0] + x1[1]) + (x1[2] + x1[3]));
-          v = group_sum<G / 8>(v);
+          float v = block_sums<G>(x0, x1);
           v = on && !odd ? v : 0.0f;
 #pragma unroll
           for (int i = 0; i < NG; i++) {
@@ -557,7 +613,13 @@ template <int P, int G, bool MINS, bool F16>
 hipError_t launch_t(const Gemv4Args& a, hipStream_t st) {
   const int tiles = (a.N0 + a.N1 + a.N2 + 15) / 16, waves = std::min((a.K + kStep - 1) / kStep, kWaves);
   const int T = std::min(kMaxTiles, (tiles + kTarget - 1) / kTarget);
-  const size_t lds = waves * ((size_t)(std::min(a.M, 4) * kToken + kDigit) + (size_t)T * 16 * a.M * sizeof(float));
+  const size_t lds = waves * ((P == 1 ? (size_t)(a.M * kToken + kDigit) : 0) + (size_t)T * 16 * a.M * sizeof(float));
+  if constexpr (P > 1) {
+    // (the sums are an operand of 16 rows)
+    hipLaunchKernelGGL((gemv4_digits_kernel<G, MINS>), dim3((a.K + kStep - 1) / kStep, MINS ? 16 : 4 * P), dim3(64), 0, st, a, P);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+  }
   hipLaunchKernelGGL((gemv4_kernel<P, G, MINS, F16>), dim3((tiles + T - 1) / T), dim3(64 * waves), lds, st, a, T);
   return hipGetLastError();
 }
@@ -594,6 +656,10 @@ hipError_t launch_g(const Gemv4Args& a, hipStream_t st) {
 }
 
 }  // namespace
+
+size_t gemv4_room(int M, int K) {
+  return M <= 4 ? 0 : (size_t)((K + kStep - 1) / kStep) * ((size_t)(M + 3) / 4 * kPassBytes + kSumBytes);
+}
 
 hipError_t launch_gemv4(const Gemv4Args& a, hipStream_t st) {
   if (a.N0 + a.N1 + a.N2 <= 0 || a.M <= 0) return hipSuccess;

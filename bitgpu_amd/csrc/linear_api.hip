@@ -470,25 +470,30 @@ static int32_t check_gemv4(const char* who, const bg::Gemv4Args& a, int32_t scal
   if (!a.x || !a.codes || !a.scales) return fail(BG_E_INVALID, "%s: NULL argument", who);
   if ((a.N0 && !a.out0) || (a.N1 && !a.out1) || (a.N2 && !a.out2))
     return fail(BG_E_INVALID, "%s: output ranges %d/%d/%d need their buffers", who, a.N0, a.N1, a.N2);
-  if (((uintptr_t)a.x | (uintptr_t)a.codes | (uintptr_t)a.scales | (uintptr_t)a.mins) & 15)
-    return fail(BG_E_INVALID, "%s: x, codes, scales and mins must be 16-byte aligned", who);
+  const size_t room = bg::gemv4_room(a.M, a.K) / 4;
+  if (room && !a.room) return fail(BG_E_INVALID, "%s: %d rows need a workspace", who, a.M);
+  if (((uintptr_t)a.x | (uintptr_t)a.codes | (uintptr_t)a.scales | (uintptr_t)a.mins | (uintptr_t)(room ? a.room : nullptr)) & 15)
+    return fail(BG_E_INVALID, "%s: x, codes, scales, mins and the workspace must be 16-byte aligned", who);
   const size_t M = a.M, K = a.K, N = (size_t)a.N0 + a.N1 + a.N2;
-  const struct { const void* p; size_t n; } o[] = {{a.out0, M * a.N0}, {a.out1, M * a.N1}, {a.out2, M * a.N2}};
+  const struct { const void* p; size_t n; } o[] = {{a.out0, M * a.N0}, {a.out1, M * a.N1}, {a.out2, M * a.N2}, {a.room, room}};
   const size_t sc = (N * (K / a.group) * (a.scale_f16 ? 2 : 4) + 3) / 4;
-  for (int i = 0; i < 3; i++) {
+  for (int i = 0; i < 4; i++) {
     if (overlap(o[i].p, o[i].n, a.x, M * K) || overlap(o[i].p, o[i].n, a.codes, N * K / 8) || overlap(o[i].p, o[i].n, a.scales, sc) ||
         overlap(o[i].p, o[i].n, a.mins, sc))
-      return fail(BG_E_INVALID, "%s: an output overlaps an input", who);
+      return fail(BG_E_INVALID, "%s: an output or the workspace overlaps an input", who);
     for (int j = 0; j < i; j++)
-      if (overlap(o[i].p, o[i].n, o[j].p, o[j].n)) return fail(BG_E_INVALID, "%s: two outputs overlap", who);
+      if (overlap(o[i].p, o[i].n, o[j].p, o[j].n)) return fail(BG_E_INVALID, "%s: two outputs, or one and the workspace, overlap", who);
   }
+  if (overlap(a.room, room, a.resid, M * N)) return fail(BG_E_INVALID, "%s: the workspace overlaps resid", who);
   return BG_OK;
 }
 
+int64_t bg_gemv4_workspace(int32_t rows, int32_t K) { return rows > 16 || K < 1 ? 0 : (int64_t)bg::gemv4_room(rows, K); }
+
 int32_t bg_gemv4_split(const float* x, int32_t rows, int32_t K, const uint32_t* codes, const void* scales, const void* mins,
                        int32_t scale_type, int32_t group, int32_t N0, int32_t N1, int32_t N2, float* out0, float* out1, float* out2,
-                       void* stream) {
-  const bg::Gemv4Args a{x, rows, K, codes, scales, mins, scale_type == BG_KV_F16, group, N0, N1, N2, out0, out1, out2, nullptr};
+                       void* workspace, void* stream) {
+  const bg::Gemv4Args a{x, rows, K, codes, scales, mins, scale_type == BG_KV_F16, group, N0, N1, N2, out0, out1, out2, nullptr, (char*)workspace};
   const int32_t rc = check_gemv4("bg_gemv4_split", a, scale_type);
   if (rc != BG_OK) return rc;
   const hipError_t e = bg::launch_gemv4(a, (hipStream_t)stream);
@@ -496,8 +501,9 @@ int32_t bg_gemv4_split(const float* x, int32_t rows, int32_t K, const uint32_t* 
 }
 
 int32_t bg_gemv4_resid(const float* x, int32_t rows, int32_t K, const uint32_t* codes, const void* scales, const void* mins,
-                       int32_t scale_type, int32_t group, int32_t N, const float* resid, float* y, void* stream) {
-  const bg::Gemv4Args a{x, rows, K, codes, scales, mins, scale_type == BG_KV_F16, group, N, 0, 0, y, nullptr, nullptr, resid};
+                       int32_t scale_type, int32_t group, int32_t N, const float* resid, float* y, void* workspace,
+                       void* stream) {
+  const bg::Gemv4Args a{x, rows, K, codes, scales, mins, scale_type == BG_KV_F16, group, N, 0, 0, y, nullptr, nullptr, resid, (char*)workspace};
   const int32_t rc = check_gemv4("bg_gemv4_resid", a, scale_type);
   if (rc != BG_OK) return rc;
   if (rows && N && !resid) return fail(BG_E_INVALID, "bg_gemv4_resid: resid is NULL");

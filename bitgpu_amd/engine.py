@@ -806,15 +806,17 @@ def linear_block(cache: LinearStateCache, li: int, batch: LinearBatch, n1, h, w_
     weights = _layer_ptrs(cache, conv_weight, a_log, dt_bias, norm)
     # one piece of memory for what lies between the launches: qkv, z, att | b, a (interleaved rows) and the prologue's
     out, wide, Z = n1.new_empty((*n1.shape[:-1], w_out.N)), cache.channels, Hv * DV
-    room = n1.new_empty(M * (2 * wide + 2 * Z + 4 * Hv))
-    qkv = room.data_ptr()
+    four = [L.bg_gemv4_workspace(M, w.K) // 4 for w in (w_in, w_out)] if 4 < M <= 16 else (0, 0)
+    room = n1.new_empty(M * (2 * wide + 2 * Z + 4 * Hv) + max(four))
+    space = room.data_ptr()  # the projections' workspace
+    qkv = space + 4 * max(four)
     z = qkv + 4 * M * wide
     att = z + 4 * M * Z
     inner = att + 4 * M * Z
     ba = inner + 4 * M * (wide + 2 * Hv)
     if isinstance(w_in, FourBitWeight):
         _on(w_in)
-        rc = L.bg_gemv4_split(x, M, w_in.K, *w_in._w, wide, Z, 2 * Hv, qkv, z, ba, st)
+        rc = L.bg_gemv4_split(x, M, w_in.K, *w_in._w, wide, Z, 2 * Hv, qkv, z, ba, space, st)
     else:
         _one_row(M)
         rc = L.bg_gemv_split(x, w_in.K, _ptr(w_in.sign), _ptr(w_in.scales), wide, Z, 2 * Hv, qkv, z, ba, st)
@@ -823,7 +825,7 @@ def linear_block(cache: LinearStateCache, li: int, batch: LinearBatch, n1, h, w_
     _between(cache, li, batch, qkv, ba + 4 * Hv, ba, 2 * Hv, weights, z, eps, inner, att, st)
     if isinstance(w_out, FourBitWeight):
         _on(w_out)
-        rc = L.bg_gemv4_resid(att, M, Z, *w_out._w, w_out.N, res, out.data_ptr(), st)
+        rc = L.bg_gemv4_resid(att, M, Z, *w_out._w, w_out.N, res, out.data_ptr(), space, st)
     else:
         _one_row(M)
         rc = L.bg_gemv_resid(att, Z, _ptr(w_out.sign), _ptr(w_out.scales), w_out.N, res, out.data_ptr(), st)

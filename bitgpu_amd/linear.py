@@ -63,6 +63,13 @@ def _on(w):
         raise ValueError(f"bitgpu_amd: the weight is on cuda:{w.index}, the current device is {_getDevice()}")
 
 
+def _room(w, x, M):
+    """The workspace of M rows, or None."""
+    if not 4 < M <= 16:
+        return None
+    return x.new_empty(lib().bg_gemv4_workspace(M, w.K) // 4, dtype=torch.float32)
+
+
 def _fused_mm4(w, x, outs):
     M, dev = _rows_of(w, x), w.index
     _on(w)
@@ -72,7 +79,9 @@ def _fused_mm4(w, x, outs):
         if i > 2 or (t is not None and t.numel() != M * ns[i]):
             raise ValueError(f"bitgpu_amd: outs must hold [{M}, N] rows of the weight's ranges {ns}")
         o[i] = _rows_ptr(t, "an output", M, ns[i], dev)
-    rc = lib().bg_gemv4_split(_rows_ptr(x, "x", M, w.K, dev), M, w.K, *w._w, *ns, *o, _stream())
+    room = _room(w, x, M)
+    rc = lib().bg_gemv4_split(_rows_ptr(x, "x", M, w.K, dev), M, w.K, *w._w, *ns, *o, None if room is None else room.data_ptr(),
+                              _stream())
     if rc:
         check(rc)
 
@@ -86,8 +95,9 @@ def _resid_mm4(w, x, resid, out):
         out = x.new_empty((*x.shape[:-1], w.N))
     elif out.numel() != M * w.N:
         raise ValueError(f"bitgpu_amd: out must hold [{M}, {w.N}], got {list(out.shape)}")
+    room = _room(w, x, M)
     rc = lib().bg_gemv4_resid(_rows_ptr(x, "x", M, w.K, dev), M, w.K, *w._w, w.N, _rows_ptr(resid, "resid", M, w.N, dev),
-                              _rows_ptr(out, "out", M, w.N, dev), _stream())
+                              _rows_ptr(out, "out", M, w.N, dev), None if room is None else room.data_ptr(), _stream())
     if rc:
         check(rc)
     return out

@@ -464,12 +464,16 @@ int32_t bg_linear_attention(const bg_linear_cache* cache, int32_t layer, bg_line
  * c = bits 4 (k % 8) .. + 3 of codes[n][k / 8] (u32) and, with the scale (and min) [n][k / group], the value
  * (c - 8) * scale, or c * scale + min where mins is not NULL. scale_type (scales and mins): BG_KV_F32 or BG_KV_F16.
  * K a multiple of 128, group 32, 64 or 128; x, codes, scales and mins 16-byte aligned. Outputs [rows, N0], [rows, N1],
- * [rows, N2]; resid, y [rows, N], y may be resid; otherwise no output overlaps an input or another. */
+ * [rows, N2]; resid, y [rows, N], y may be resid; otherwise no output overlaps an input or another. A product of two values may reach 2^126 and their scales 2^90; K at most
+ * 2^24. More than four rows need a workspace of bg_gemv4_workspace(rows, K) bytes, 16-byte aligned, that no other stream
+ * uses meanwhile (four or fewer: 0 bytes, NULL). What a row gives does not depend on the rows beside it. */
+int64_t bg_gemv4_workspace(int32_t rows, int32_t K);
 int32_t bg_gemv4_split(const float* x, int32_t rows, int32_t K, const uint32_t* codes, const void* scales, const void* mins,
                        int32_t scale_type, int32_t group, int32_t N0, int32_t N1, int32_t N2, float* out0, float* out1, float* out2,
-                       void* stream);
+                       void* workspace, void* stream);
 int32_t bg_gemv4_resid(const float* x, int32_t rows, int32_t K, const uint32_t* codes, const void* scales, const void* mins,
-                       int32_t scale_type, int32_t group, int32_t N, const float* resid, float* y, void* stream);
+                       int32_t scale_type, int32_t group, int32_t N, const float* resid, float* y, void* workspace,
+                       void* stream);
 
 #ifdef __cplusplus
 }

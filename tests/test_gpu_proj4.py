@@ -161,3 +161,24 @@ def test_no_rows(dev):
     w = Weight(rng, 10, 128, 32).handle()
     E.fused_mm(w, torch.empty(0, 128, device="cuda"), [torch.empty(0, 10, device="cuda")])
     assert E.resid_mm(w, torch.empty(0, 128, device="cuda"), torch.empty(0, 10, device="cuda")).shape == (0, 10)
+
+
+@pytest.mark.parametrize("group,mins", [(32, True), (64, False), (128, True)])
+@pytest.mark.parametrize("M", [1, 3, 6, 16])
+def test_many_rows_of_weights(dev, M, group, mins):
+    """As many tiles a workgroup as there are, over more than eight steps of 512 weights: the bits of every 5000 rows
+    alone."""
+    N, K = 40000, 4736
+    g = torch.Generator(device="cuda").manual_seed(M + group)
+    codes = torch.randint(-2**31, 2**31 - 1, (N, K // 8), device="cuda", generator=g).to(torch.int32)
+    scales, lo = ((torch.rand((N, K // group), device="cuda", generator=g) - 0.5).half() for _ in range(2))
+    x = torch.randn((M, K), device="cuda", generator=g)
+
+    def rows(a, b):
+        out = torch.full((M, b - a), float("nan"), device="cuda")
+        E.fused_mm(E.FourBitWeight(codes[a:b], scales[a:b], K, b - a, group=group, mins=lo[a:b] if mins else None), x, [out])
+        return out
+
+    out = rows(0, N)
+    for a in range(0, N, 5000):
+        assert torch.equal(out[:, a:a + 5000], rows(a, a + 5000)), a
