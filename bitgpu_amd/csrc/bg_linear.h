@@ -49,7 +49,7 @@ struct LinBatchView {
   const LinSeq* seqs;
   const LinUnit* units;
   int n_seqs, n_tokens, n_units;
-  int most;                       // rows of the longest sequence
+  int most;                       // rows of the longest sequence that is not chunked, at most
   int n_chunked, n_chunk_units;
   int window;                     // chunks that the workspace holds
   char* ws;                       // NULL under capture: hdr's

@@ -43,7 +43,7 @@ constexpr int kSlots = 2;
 struct Plan {
   std::vector<bg::LinSeq> seqs;    // those with new rows, the longest first
   std::vector<bg::LinUnit> units;
-  int n_tokens = 0, most = 0;
+  int n_tokens = 0;
   int n_chunked = 0, n_chunk_units = 0;
 };
 
@@ -85,15 +85,16 @@ struct bg_linear_batch {
     b.n_tokens = plan.n_tokens;
     b.n_seqs = captured ? std::min(max_seqs, plan.n_tokens) : (int)plan.seqs.size();
     b.n_units = captured ? b.n_seqs + plan.n_tokens / bg::kLinChunk : (int)plan.units.size();
-    b.most = plan.most;
     b.window = window;
     if (captured) {
+      b.most = std::min(plan.n_tokens, bg::kLinChunkFrom - 1);
       b.n_chunked = std::min(max_seqs, plan.n_tokens / bg::kLinChunkFrom);
       b.n_chunk_units = b.n_chunked ? b.n_chunked + plan.n_tokens / bg::kLinChunk : 0;
     } else {
       b.n_chunked = plan.n_chunked;
       b.n_chunk_units = plan.n_chunk_units;
       b.ws = ws;
+      b.most = b.n_seqs > b.n_chunked ? plan.seqs[b.n_chunked].rows : 0;
     }
     return b;
   }
@@ -159,7 +160,7 @@ int32_t make_plan(bg_linear_batch* b, int32_t n_seqs, const int32_t* rows, const
   Plan& p = b->next;
   p.seqs.clear();
   p.units.clear();
-  p.most = p.n_chunked = p.n_chunk_units = 0;
+  p.n_chunked = p.n_chunk_units = 0;
   long long T = 0;
   b->writer.assign(b->n_slots, -1);
   for (int s = 0; s < n_seqs; s++) {
@@ -178,7 +179,6 @@ int32_t make_plan(bg_linear_batch* b, int32_t n_seqs, const int32_t* rows, const
       return fail(BG_E_INVALID, "bg_linear_batch_set: %lld new rows up to sequence %d, the batch holds %d", T + rows[s], s, b->max_tokens);
     if (rows[s] > 0) p.seqs.push_back(bg::LinSeq{(int)T, rows[s], src, slots[s], s, 0, {}});
     T += rows[s];
-    p.most = std::max(p.most, rows[s]);
   }
   for (const bg::LinSeq& q : p.seqs)
     if (q.src >= 0 && b->writer[q.src] >= 0 && b->writer[q.src] != q.unit0)

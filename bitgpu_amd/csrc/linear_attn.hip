@@ -28,13 +28,31 @@ __global__ __launch_bounds__(kThreads) void linear_recurrent_kernel(LinLayer L, 
   constexpr int NI = DK / 32;
   constexpr int WAVES = kThreads / 64;
   static_assert(CPL >= 1 && NI >= 1, "state split");
-  __shared__ float part[2][WAVES];
+  constexpr int ROW = 2 * DK + DV, PIECES = ROW / 4;      // of a row in LDS: k | q | v
+  constexpr int EACH = DV / 64;                           // values of a lane that normalizes a row
+  constexpr int HELD = (kLinChunkFrom - 2) * PIECES / kThreads + 1;
   const int s_at = first + blockIdx.y;
   const LinSeq s = b.seqs[s_at];
   if (s_at >= b.hdr->n_seqs || s.rows >= kLinChunkFrom) return;
+  extern __shared__ __align__(16) float lds[];
+  float* made = lds;                                      // the rows' outputs, where they are to be normalized
+  float* rows = lds + (a.norm ? s.rows * DV : 0);   // the rows behind the first
   const int h = blockIdx.x, kh = h / (L.v_heads / L.k_heads);
   const int l = threadIdx.x & 7, col = (threadIdx.x >> 3) * CPL, wave = threadIdx.x >> 6;
 
+  // all rows but the first through LDS: of the sequence's own order the loop below could keep only one row in flight
+  // (five rows of three sequences 13.6 us so, XXX us from LDS)
+  f4 held[HELD];
+  const int pieces = (s.rows - 1) * PIECES;
+#pragma unroll
+  for (int i = 0; i < HELD; i++) {
+    const int at = i * kThreads + threadIdx.x, t = at / PIECES, e = at % PIECES * 4;
+    if (at >= pieces) continue;
+    const size_t row = s.row0 + 1 + t;
+    held[i] = e < 2 * DK ? *(const f4*)((e < DK ? a.k : a.q) + (row * L.k_heads + kh) * DK + (e & (DK - 1)))
+                         : *(const f4*)(a.v + (row * L.v_heads + h) * DV + e - 2 * DK);
+  }
+  __builtin_amdgcn_sched_barrier(0);
   f4 S[CPL][NI];
 #pragma unroll
   for (int c = 0; c < CPL; c++)
@@ -47,41 +65,64 @@ __global__ __launch_bounds__(kThreads) void linear_recurrent_kernel(LinLayer L, 
 #pragma unroll
       for (int i = 0; i < NI; i++) S[c][i] = *(const f4*)(p + c * DK + 32 * i);
   }
-  float weight[CPL];
-#pragma unroll
-  for (int c = 0; c < CPL; c++) weight[c] = a.norm ? a.norm[col + c] : 1.0f;
-
-  const size_t kstride = (size_t)L.k_heads * DK, vstride = (size_t)L.v_heads * DV;
-  const float* kp = a.k + (size_t)s.row0 * kstride + kh * DK + 4 * l;
-  const float* qp = a.q + (size_t)s.row0 * kstride + kh * DK + 4 * l;
-  const float* vp = a.v + (size_t)s.row0 * vstride + h * DV + col;
   RowIn<DK> in;
-  float v[CPL], z[CPL], g, beta;
-  auto load = [&](int t) {
+  float v[CPL];
+  {
+    const float* kp = a.k + ((size_t)s.row0 * L.k_heads + kh) * DK + 4 * l;
+    const float* qp = a.q + ((size_t)s.row0 * L.k_heads + kh) * DK + 4 * l;
+    const size_t vat = ((size_t)s.row0 * L.v_heads + h) * DV + col;
 #pragma unroll
     for (int i = 0; i < NI; i++) {
-      in.k[i] = *(const f4*)(kp + t * kstride + 32 * i);
-      in.q[i] = *(const f4*)(qp + t * kstride + 32 * i);
+      in.k[i] = *(const f4*)(kp + 32 * i);
+      in.q[i] = *(const f4*)(qp + 32 * i);
     }
 #pragma unroll
-    for (int c = 0; c < CPL; c++) v[c] = vp[t * vstride + c];
+    for (int c = 0; c < CPL; c++) v[c] = a.v[vat + c];
+  }
+  // a wave normalizes rows wave, wave + 8 ..: the first one's gate, and the weight
+  const int mine = EACH * (threadIdx.x & 63);
+  float weight[EACH], z[EACH];
+  auto load_gate = [&](int t) {
 #pragma unroll
-    for (int c = 0; c < CPL; c++) z[c] = a.gate ? a.gate[((size_t)(s.row0 + t) * L.v_heads + h) * DV + col + c] : 0.0f;
-    g = a.g[(a.g_stride ? (size_t)(s.row0 + t) * a.g_stride : 0) + h];
-    beta = DELTA ? a.beta[(size_t)(s.row0 + t) * L.v_heads + h] : 1.0f;
+    for (int c = 0; c < EACH; c++) z[c] = a.gate[((size_t)(s.row0 + t) * L.v_heads + h) * DV + mine + c];
   };
-  load(0);
+  if (a.norm && wave < s.rows) {
+#pragma unroll
+    for (int c = 0; c < EACH; c++) weight[c] = a.norm[mine + c];
+    if (a.gate) load_gate(wave);
+  }
+  // the rows' decays and write strengths: lane t has row t's (an exponential in 64 bits a wave, not one a row)
+  static_assert(kLinChunkFrom <= 64, "a lane a row");
+  float fades, rests, betas = 1.0f;
+  {
+    const size_t t = s.row0 + min((int)(threadIdx.x & 63), s.rows - 1);
+    if constexpr (DELTA) betas = a.beta[t * L.v_heads + h];
+    fade_of(a.g[(a.g_stride ? t * a.g_stride : 0) + h], fades, rests);
+  }
+  auto of_row = [&](float x, int t) { return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(x), t)); };
+  __builtin_amdgcn_sched_barrier(0);
+  if (pieces) {
+#pragma unroll
+    for (int i = 0; i < HELD; i++)
+      if (i * kThreads + (int)threadIdx.x < pieces) *(f4*)(rows + 4 * (i * kThreads + threadIdx.x)) = held[i];
+    __syncthreads();
+  }
+  auto load = [&](int t) {
+    const float* r = rows + (t - 1) * ROW;
+#pragma unroll
+    for (int i = 0; i < NI; i++) {
+      in.k[i] = *(const f4*)(r + 4 * l + 32 * i);
+      in.q[i] = *(const f4*)(r + DK + 4 * l + 32 * i);
+    }
+#pragma unroll
+    for (int c = 0; c < CPL; c++) v[c] = r[2 * DK + col + c];
+  };
   for (int t = 0; t < s.rows; t++) {
     const RowIn<DK> x = in;
-    float vv[CPL], zz[CPL];
+    float vv[CPL];
 #pragma unroll
-    for (int c = 0; c < CPL; c++) {
-      vv[c] = v[c];
-      zz[c] = z[c];
-    }
-    float fade, rest;
-    fade_of(g, fade, rest);
-    const float strength = beta;
+    for (int c = 0; c < CPL; c++) vv[c] = v[c];
+    const float fade = of_row(fades, t), rest = of_row(rests, t), strength = of_row(betas, t);
     if (t + 1 < s.rows) load(t + 1);
     float ks[CPL], qs[CPL], qk = 0.0f;
 #pragma unroll
@@ -98,39 +139,20 @@ __global__ __launch_bounds__(kThreads) void linear_recurrent_kernel(LinLayer L, 
         }
       }
     qk = group_sum<8>(qk);
-    float o[CPL], ss = 0.0f;
+    float o[CPL];
 #pragma unroll
     for (int c = 0; c < CPL; c++) {
       qs[c] = group_sum<8>(qs[c]);
       float delta = vv[c];
       if constexpr (DELTA) delta = strength * (vv[c] - fade * group_sum<8>(ks[c]));
       o[c] = a.scale * fmaf(qk, delta, fade * qs[c]);
-      ss = fmaf(o[c], o[c], ss);
 #pragma unroll
       for (int i = 0; i < NI; i++)
 #pragma unroll
         for (int e = 0; e < 4; e++) S[c][i][e] = fmaf(fade, S[c][i][e], fmaf(rest, S[c][i][e], x.k[i][e] * delta));
     }
-    if (a.norm) {
-      // the eight lanes of a column hold the same value: sum over the wave's eight groups, then its waves
-      ss += dpp_mov<0x128>(ss);  // row_ror:8: the row's other group
-      float2 r = pair16(ss);
-      r = pair32(r.x + r.y);
-      ss = r.x + r.y;
-      if ((threadIdx.x & 63) == 0) part[t & 1][wave] = ss;
-      __syncthreads();
-      ss = 0.0f;
-#pragma unroll
-      for (int w = 0; w < WAVES; w++) ss += part[t & 1][w];
-      const float inv = 1.0f / sqrtf(ss / DV + a.eps);
-#pragma unroll
-      for (int c = 0; c < CPL; c++) {
-        o[c] = o[c] * inv * weight[c];
-        if (a.gate) o[c] *= zz[c] / (1.0f + expf(-zz[c]));
-      }
-    }
     if (l == 0) {
-      float* op = a.out + ((size_t)(s.row0 + t) * L.v_heads + h) * DV + col;
+      float* op = a.norm ? made + t * DV + col : a.out + ((size_t)(s.row0 + t) * L.v_heads + h) * DV + col;
 #pragma unroll
       for (int c = 0; c < CPL; c++) op[c] = o[c];
     }
@@ -140,14 +162,33 @@ __global__ __launch_bounds__(kThreads) void linear_recurrent_kernel(LinLayer L, 
   for (int c = 0; c < CPL; c++)
 #pragma unroll
     for (int i = 0; i < NI; i++) *(f4*)(p + c * DK + 32 * i) = S[c][i];
+  if (!a.norm) return;
+  __syncthreads();
+  for (int t = wave; t < s.rows; t += WAVES) {
+    if (t != wave && a.gate) load_gate(t);
+    float o[EACH], ss = 0.0f;
+#pragma unroll
+    for (int c = 0; c < EACH; c++) {
+      o[c] = made[t * DV + mine + c];
+      ss = fmaf(o[c], o[c], ss);
+    }
+    const float inv = 1.0f / sqrtf(wave_sum(ss) / DV + a.eps);
+    float* op = a.out + ((size_t)(s.row0 + t) * L.v_heads + h) * DV + mine;
+#pragma unroll
+    for (int c = 0; c < EACH; c++) {
+      const float y = o[c] * inv * weight[c];
+      op[c] = a.gate ? y * (z[c] / (1.0f + expf(-z[c]))) : y;
+    }
+  }
 }
 
 template <int DK, int DV>
 hipError_t launch_t(const LinLayer& L, const LinBatchView& b, const LinAttnArgs& a, hipStream_t st) {
   const int first = b.ws || !b.n_chunked ? b.n_chunked : 0;  // (under capture the counts are of the replay)
   const dim3 g(L.v_heads, b.n_seqs - first);
-  if (a.beta) hipLaunchKernelGGL((linear_recurrent_kernel<DK, DV, true>), g, dim3(kThreads), 0, st, L, b, a, first);
-  else hipLaunchKernelGGL((linear_recurrent_kernel<DK, DV, false>), g, dim3(kThreads), 0, st, L, b, a, first);
+  const size_t lds = ((size_t)(b.most - 1) * (2 * DK + DV) + (a.norm ? b.most * DV : 0)) * sizeof(float);
+  if (a.beta) hipLaunchKernelGGL((linear_recurrent_kernel<DK, DV, true>), g, dim3(kThreads), lds, st, L, b, a, first);
+  else hipLaunchKernelGGL((linear_recurrent_kernel<DK, DV, false>), g, dim3(kThreads), lds, st, L, b, a, first);
   return hipGetLastError();
 }
 
