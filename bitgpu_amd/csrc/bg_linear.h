@@ -12,8 +12,11 @@
 namespace bg {
 
 constexpr int kLinChunk = 64;     // rows of a unit
-// Sequences of at least this many new rows are done in chunks of 64, shorter ones row by row.
-constexpr int kLinChunkFrom = 24;
+// Sequences of at least this many new rows are done in chunks of 64, shorter ones row by row. With 32 heads of 128 x 128
+// one sequence of the delta rule takes 4.9 + 0.87 us a row so and 30 us as a chunk (4 sequences 6 + 0.87 and 41, 64 of
+// them 50 + 7.2 and 280: they meet at 29, 41 and 32 rows), one of the sum rule 5 + 0.75 and 20.5 (64: 45 + 6.2 and 177:
+// at 21). A batch does not know the rule: a number between.
+constexpr int kLinChunkFrom = 28;
 constexpr size_t kLinSpace = (size_t)256 << 20;  // most bytes of chunk operands at a time
 
 // a row's decay as hi + lo: the rounding of one float would add up over the rows of a constant decay

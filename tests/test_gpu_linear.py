@@ -261,3 +261,11 @@ def test_long_prompts(dev, rows, Hv):
     for rule in ("delta", "sum"):
         c = Case(rows, Hk=1, Hv=Hv, rule=rule, gate=rule == "sum", seed=7)
         c.check(*c.run())
+
+
+@pytest.mark.parametrize("how", ["plain", "norm", "gate"])
+@pytest.mark.parametrize("rule", ["delta", "sum"])
+def test_lengths_beside_the_chunked_ones(dev, rule, how):
+    """Sequences of two dozen rows, some row by row and some as a chunk, in one batch."""
+    c = Case([29, 3, 27, 26, 1, 28, 23, 24, 31], rule=rule, gate=how == "gate", norm=how != "plain", seed=11)
+    c.check(*c.run())
