@@ -795,14 +795,12 @@ def linear_block(cache: LinearStateCache, li: int, batch: LinearBatch, n1, h, w_
     M = 1 if n1.dim() == 1 else n1.shape[0]
     if M != batch.n_tokens:
         raise ValueError(f"bitgpu_amd: n1 holds {M} rows, the batch has {batch.n_tokens} new rows")
-    _f32(n1, "n1")
-    _f32(h, "h")
     dev, st, L = cache.index, _stream(), lib()
-    if n1.get_device() != dev or h.get_device() != dev or dev != _getDevice():
-        raise ValueError(f"bitgpu_amd: expected tensors on cuda:{dev}, the current device")
+    if dev != _getDevice():
+        raise ValueError(f"bitgpu_amd: the cache lives on cuda:{dev}, the current device is {_getDevice()}")
     if n1.shape[-1] != w_in.K or h.numel() != M * w_out.N:
         raise ValueError(f"bitgpu_amd: n1 must hold [{M}, {w_in.K}] and h [{M}, {w_out.N}], got {list(n1.shape)} and {list(h.shape)}")
-    x, res = _ptr(n1), _ptr(h)
+    x, res = _rows_ptr(n1, "n1", M, w_in.K, dev), _rows_ptr(h, "h", M, w_out.N, dev)
     weights = _layer_ptrs(cache, conv_weight, a_log, dt_bias, norm)
     # one piece of memory for what lies between the launches: qkv, z, att | b, a (interleaved rows) and the prologue's
     out, wide, Z = n1.new_empty((*n1.shape[:-1], w_out.N)), cache.channels, Hv * DV
