@@ -434,7 +434,9 @@ int32_t bg_linear_batch_destroy(bg_linear_batch* batch);
  * on from the state in slot sources[s] (NULL: slots[s]; -1: a new conversation, zeros) and leaves it in slot
  * slots[s]. Sequences may share a source (a fork); no slot is written by two, or written by one and read by
  * another (BG_E_INVALID, the batch before stays set). A sequence without new rows touches no slot. Rows are
- * numbered sequence by sequence. Not under graph capture (BG_E_STATE). */
+ * numbered sequence by sequence. Not under graph capture (BG_E_STATE). Sequences of 28 new rows and more are done in
+ * chunks of 64, whose operands take a workspace of at most 256 MiB (or one chunk's): it grows here (BG_E_OOM: the batch
+ * before stays set), never in a layer's call. */
 int32_t bg_linear_batch_set(bg_linear_batch* batch, int32_t n_seqs, const int32_t* rows, const int32_t* slots,
                             const int32_t* sources, void* stream);
 
@@ -453,8 +455,9 @@ int32_t bg_linear_prologue(const bg_linear_cache* cache, int32_t layer, bg_linea
  * k_heads, k_dim], v, out [rows, v_heads, v_dim], g [rows, v_heads] with rows g_stride values apart (0: [v_heads], one
  * decay a head), beta [rows, v_heads] or NULL. norm (nullable, [v_dim]): out = o / sqrt(mean o^2 + eps) * norm, and
  * with gate [rows, v_heads, v_dim] times gate / (1 + exp(-gate)). q, k, v, gate, norm, out 16-byte aligned; out
- * overlaps no input. Rows of out beyond the batch's are left as they are. A value that is not finite reaches its own
- * head's later rows and state. */
+ * overlaps no input. Rows of out beyond the batch's are left as they are. A v that is not finite reaches its value dim's
+ * row, later rows and state; a q its row of its heads; a k, g or beta its heads' row, later rows and states (g of minus
+ * infinity is a decay to zero). Norms spread what is in a row over its head. */
 int32_t bg_linear_attention(const bg_linear_cache* cache, int32_t layer, bg_linear_batch* batch, const float* q, const float* k,
                             const float* v, const float* g, int32_t g_stride, const float* beta, float scale, const float* gate,
                             const float* norm, float eps, float* out, void* stream);
