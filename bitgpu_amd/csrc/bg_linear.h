@@ -52,7 +52,8 @@ struct LinBatchView {
   const LinSeq* seqs;
   const LinUnit* units;
   int n_seqs, n_tokens, n_units;
-  int most;                       // rows of the longest sequence that is not chunked, at most
+  int longest;                    // rows of the longest sequence as the batch is set (not a bound)
+  int most;                       // of the longest one that is not chunked, at most
   int n_chunked, n_chunk_units;
   int window;                     // chunks that the workspace holds
   char* ws;                       // NULL under capture: hdr's

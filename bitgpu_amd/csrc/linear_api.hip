@@ -86,6 +86,7 @@ struct bg_linear_batch {
     b.n_seqs = captured ? std::min(max_seqs, plan.n_tokens) : (int)plan.seqs.size();
     b.n_units = captured ? b.n_seqs + plan.n_tokens / bg::kLinChunk : (int)plan.units.size();
     b.window = window;
+    b.longest = plan.seqs.empty() ? 0 : plan.seqs[0].rows;
     if (captured) {
       b.most = std::min(plan.n_tokens, bg::kLinChunkFrom - 1);
       b.n_chunked = std::min(max_seqs, plan.n_tokens / bg::kLinChunkFrom);

@@ -6,7 +6,7 @@
 //   g = -exp(a_log) softplus(a + dt_bias), beta = sigmoid(b)
 //
 // Bound by memory: every input row is read and every output row written once. A group of D / 4 lanes owns a
-// head's channels, four a lane, and walks a run of up to 8 rows whose inputs (and the taps - 1 before them)
+// head's channels, four a lane, and walks a run of up to 4 rows whose inputs (and the taps - 1 before them)
 // are all loaded before the first is used. The lanes that hold a sequence's first run also read its kept
 // inputs and, behind that, store the new ones: the sequence's other runs never look at them, so one slot may
 // be both source and destination.
@@ -15,7 +15,7 @@
 
 namespace bg {
 
-constexpr int kRun = 8;
+constexpr int kRun = 4;
 constexpr float kUnitEps = 1e-6f;  // under the root of the q / k norm
 
 typedef float f4 __attribute__((ext_vector_type(4)));
@@ -81,15 +81,18 @@ __device__ __forceinline__ void conv_run(const LinLayer& L, const LinBatchView& 
 }
 
 // blockIdx.x: a unit; blockIdx.y: blocks of q and k heads, of v heads, then one of the gates. WIDE: a block is
-// one head and its lane groups are runs of a unit; otherwise its groups are heads and each walks all runs
-// (units of few rows).
+// one head and its lane groups are a unit's runs (512 threads: all 16 at head dims of 128); otherwise its groups are heads
+// and each walks all runs, which is for sequences of one run. 10,240 channels, one sequence of 1, 8, 64 rows 3.7, 4.5, 7.7 us
+// wide, 3.8, 6.3, 31 not (there with runs of 8); 32 sequences of 1, 4, 8, 16 rows 6.0, 10.0, 11.3, 15.2 wide, 4.8, 7.5,
+// 11.1, 16.1 not. Of 4,096 rows 81 us, 4.2 TB/s (runs of 8 and 256 threads 85, runs of 2 106).
 template <int DK, int DV, int TAPS, bool WIDE>
-__global__ __launch_bounds__(256) void linear_prologue_kernel(LinLayer L, LinBatchView b, LinPrologueArgs a, int qk_blocks, int v_blocks) {
+__global__ __launch_bounds__(WIDE ? 512 : 256) void linear_prologue_kernel(LinLayer L, LinBatchView b, LinPrologueArgs a, int qk_blocks, int v_blocks) {
+  constexpr int THREADS = WIDE ? 512 : 256;
   if ((int)blockIdx.x >= b.hdr->n_units) return;
   const LinUnit u = b.units[blockIdx.x];
   const int y = blockIdx.y;
   if (y < qk_blocks) {
-    constexpr int LG = DK / 4, GROUPS = 256 / LG;
+    constexpr int LG = DK / 4, GROUPS = THREADS / LG;
     const int grp = threadIdx.x / LG, c = 4 * (threadIdx.x % LG);
     const int head = WIDE ? y : y * GROUPS + grp;
     if (head >= 2 * L.k_heads) return;
@@ -98,14 +101,14 @@ __global__ __launch_bounds__(256) void linear_prologue_kernel(LinLayer L, LinBat
     for (int r0 = WIDE ? kRun * grp : 0; r0 < u.n; r0 += WIDE ? kRun * GROUPS : kRun)
       conv_run<DK, TAPS, true>(L, b, a, u, r0, head * DK + c, (isq ? a.q : a.k) + h * DK + c, L.k_heads * DK);
   } else if (y < qk_blocks + v_blocks) {
-    constexpr int LG = DV / 4, GROUPS = 256 / LG;
+    constexpr int LG = DV / 4, GROUPS = THREADS / LG;
     const int grp = threadIdx.x / LG, c = 4 * (threadIdx.x % LG);
     const int head = WIDE ? y - qk_blocks : (y - qk_blocks) * GROUPS + grp;
     if (head >= L.v_heads) return;
     for (int r0 = WIDE ? kRun * grp : 0; r0 < u.n; r0 += WIDE ? kRun * GROUPS : kRun)
       conv_run<DV, TAPS, false>(L, b, a, u, r0, 2 * L.k_heads * DK + head * DV + c, a.v + head * DV + c, L.v_heads * DV);
   } else {
-    for (int i = threadIdx.x; i < u.n * L.v_heads; i += 256) {
+    for (int i = threadIdx.x; i < u.n * L.v_heads; i += THREADS) {
       const int r = u.row0 + i / L.v_heads, h = i % L.v_heads;
       const size_t at = (size_t)r * a.ab_stride + h, to = (size_t)r * L.v_heads + h;
       if (a.g) {
@@ -120,9 +123,9 @@ __global__ __launch_bounds__(256) void linear_prologue_kernel(LinLayer L, LinBat
 template <int DK, int DV, int TAPS>
 static hipError_t launch_t(const LinLayer& L, const LinBatchView& b, const LinPrologueArgs& a, hipStream_t st) {
   const int gates = a.g || a.beta;
-  if (b.most > 2 * kRun) {
+  if (b.longest > kRun) {
     const int qk = 2 * L.k_heads, v = L.v_heads;
-    hipLaunchKernelGGL((linear_prologue_kernel<DK, DV, TAPS, true>), dim3(b.n_units, qk + v + gates), dim3(256), 0, st, L, b, a, qk, v);
+    hipLaunchKernelGGL((linear_prologue_kernel<DK, DV, TAPS, true>), dim3(b.n_units, qk + v + gates), dim3(512), 0, st, L, b, a, qk, v);
   } else {
     const int per_k = 1024 / DK, per_v = 1024 / DV;
     const int qk = (2 * L.k_heads + per_k - 1) / per_k, v = (L.v_heads + per_v - 1) / per_v;
