@@ -462,7 +462,7 @@ int32_t bg_linear_attention(const bg_linear_cache* c, int32_t layer, bg_linear_b
 static int32_t check_gemv4(const char* who, const bg::Gemv4Args& a, int32_t scale_type) {
   if (a.M < 0 || a.M > 16) return fail(BG_E_UNSUPPORTED, "%s: %d rows (at most 16)", who, a.M);
   if (a.K < 128 || a.K % 128) return fail(BG_E_INVALID, "%s: K %d must be a positive multiple of 128", who, a.K);
-  if (a.K > (1 << 24)) return fail(BG_E_UNSUPPORTED, "%s: K %d too large", who, a.K);  // a workgroup's 64 rows in 32-bit offsets
+  if (a.K > (1 << 24)) return fail(BG_E_UNSUPPORTED, "%s: K %d too large", who, a.K);  // a workgroup's 128 rows in 32-bit offsets
   if (a.group != 32 && a.group != 64 && a.group != 128) return fail(BG_E_UNSUPPORTED, "%s: group %d unsupported (32, 64 or 128)", who, a.group);
   if (scale_type != BG_KV_F32 && scale_type != BG_KV_F16) return fail(BG_E_INVALID, "%s: unknown scale type %d", who, scale_type);
   if (a.N0 < 0 || a.N1 < 0 || a.N2 < 0 || (long long)a.N0 + a.N1 + a.N2 > INT_MAX / 16)

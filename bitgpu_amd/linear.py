@@ -43,7 +43,14 @@ class FourBitWeight:
         self.codes, self.scales, self.mins, self.group = codes, scales, mins, group
         self.K, self.N0, self.N1, self.N2 = K, N0, N1, N2
         self.index = codes.get_device()
-        self._w = (_ptr(codes), _ptr(scales), _ptr(mins), BG_KV_F16 if scales.dtype is torch.float16 else BG_KV_F32, group)
+        self._type = BG_KV_F16 if scales.dtype is torch.float16 else BG_KV_F32
+        for t in (codes, scales, mins):
+            _ptr(t)
+
+    @property
+    def _w(self):
+        """codes .. group of the C calls."""
+        return (self.codes.data_ptr(), self.scales.data_ptr(), None if self.mins is None else self.mins.data_ptr(), self._type, self.group)
 
     @property
     def N(self) -> int:

@@ -50,7 +50,8 @@ def test_weights():
 def four(N0, N1=0, N2=0, K=256):
     w = object.__new__(E.FourBitWeight)
     w.K, w.N0, w.N1, w.N2, w.index, w.group = K, N0, N1, N2, -1, 64
-    w._w = (None, None, None, _lib.BG_KV_F16, 64)
+    w.codes = w.scales = torch.zeros(0)
+    w.mins, w._type = None, _lib.BG_KV_F16
     return w
 
 
