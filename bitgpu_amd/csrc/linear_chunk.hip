@@ -40,12 +40,12 @@ constexpr double kLowest = -1e4;  // of a log decay: e^g is 0 in f32 from -104 o
 
 // What the scan needs of a chunk and head beside its operands. Operands are held times 2^shift.
 struct ChunkMeta {
-  int kshift, qshift[4], tshift[4], pshift[4], wshift[4];
+  int kshift, qshift[4], tshift[4], pshift[4];
   float whole;                 // e^G_n
-  // What the scan's bounds are made of, as powers of two: w of DK kmax T e^G's largest row sum (of a state's share of
-  // V'), t of T's, f of the largest e^(G_n - G_i), s of e^G_n, k of 64 kmax. bad in w: something is not finite
-  int ew, et, ef, es, ek;
-  int pad[9];
+  // What the scan's bounds are made of, as powers of two: y of gmax DK kmax (of a state's share of Y), t of T's
+  // largest row sum, f of the largest e^(G_n - G_i), s of e^G_n, k of 64 kmax. bad in y: something is not finite
+  int ey, et, ef, es, ek;
+  int pad[13];
 };
 static_assert(sizeof(ChunkMeta) == 128, "meta");
 
@@ -55,9 +55,8 @@ static_assert(sizeof(ChunkMeta) == 128, "meta");
 template <int DK>
 struct ChunkSpace {
   static constexpr int NKB = DK / 32;
-  static constexpr int Q = 0, KT = Q + 4 * NKB * 2 * 64, PER_K = KT + (DK / 16) * 2 * 2 * 64;  // in half8
-  static constexpr int T = 0, P = T + 4 * 2 * 2 * 64, W = P + 4 * 2 * 2 * 64, G = W + 4 * NKB * 2 * 64, META = G + 128 / 4,
-                       PER_H = META + 8;                                                      // in 16 bytes
+  static constexpr int K = 0, Q = K + 4 * NKB * 2 * 64, KT = Q + 4 * NKB * 2 * 64, PER_K = KT + (DK / 16) * 2 * 2 * 64;  // in half8
+  static constexpr int T = 0, P = T + 4 * 2 * 2 * 64, G = P + 4 * 2 * 2 * 64, META = G + 128 / 4, PER_H = META + 8;       // in 16 bytes
 };
 
 // The workspace, as memory that is known to be the device's: through a pointer of no known kind its loads would
@@ -68,8 +67,6 @@ __device__ inline ghalf8* workspace(const LinBatchView& b) { return (ghalf8*)(b.
 
 __device__ inline int top_exponent(float x) { return __builtin_amdgcn_frexp_expf(x); }  // x < 2^e; 0 for 0
 __device__ inline int shift_for(float most) { return kTop - top_exponent(most); }
-// of a row tile of W = T e^G K, from its largest row sum of T e^G
-__device__ inline int wshift_of(float sum, float kmax) { return kTop - top_exponent(sum) - top_exponent(kmax); }
 __device__ inline uint32_t mag(float x) { return __float_as_uint(x) & 0x7fffffffu; }
 constexpr uint32_t kInf = 0x7f800000u;
 
@@ -171,11 +168,10 @@ __global__ __launch_bounds__(256, 4) void linear_chunk_prepare(LinLayer L, LinBa
   constexpr int kMat = 64 * kPad * 4, kFrag = 4 * NKB * 2 * 64 * 16;
   __shared__ __align__(16) char mem[2 * kMat > kFrag ? 2 * kMat : kFrag];
   __shared__ double gsums[4][64];            // of four value heads at a time, a wave each
-  __shared__ float strengths[4][64], fades[4][64], gtop[4][2];
+  __shared__ float strengths[4][64], gtop[4][3];
   __shared__ int gbad[4];
   __shared__ uint32_t most[4], bits[4];
-  __shared__ float sums[4], wsums[4];
-  __shared__ int wheld[4];
+  __shared__ float sums[4];
   half8* frag = (half8*)mem;                 // K, while products with it run
   float* Am = (float*)mem;                   // then A
   float* Tm = (float*)(mem + kMat);          // P, then T
@@ -238,6 +234,10 @@ __global__ __launch_bounds__(256, 4) void linear_chunk_prepare(LinLayer L, LinBa
     const int i = (wave * NKB + kb) * 2 * 64 + lane;
     frag[i] = kh8[kb];
     frag[i + 64] = kl8[kb];
+    if constexpr (DELTA) {
+      wk[W::K + i] = kh8[kb];
+      wk[W::K + i + 64] = kl8[kb];
+    }
     wk[W::Q + i] = qh[kb];
     wk[W::Q + i + 64] = ql[kb];
   }
@@ -309,13 +309,13 @@ __global__ __launch_bounds__(256, 4) void linear_chunk_prepare(LinLayer L, LinBa
         const float eg = expf((float)s), fg = expf((float)(end - s));
         BG_GLOBAL float* gg = (BG_GLOBAL float*)(wh + (size_t)wave * W::PER_H + W::G);
         gg[lane] = eg;
-        fades[wave][lane] = eg;
         gg[64 + lane] = on ? fg : 0.0f;
-        const float fm = __uint_as_float(wave_umax(mag(fg)));
+        const float gm = __uint_as_float(wave_umax(mag(eg))), fm = __uint_as_float(wave_umax(mag(fg)));
         const bool odd = __any(mag(eg) >= kInf || mag(fg) >= kInf || mag(be) >= kInf);
         if (lane == 0) {
-          gtop[wave][0] = fm;
-          gtop[wave][1] = expf((float)end);
+          gtop[wave][0] = gm;
+          gtop[wave][1] = fm;
+          gtop[wave][2] = expf((float)end);
           gbad[wave] = odd;
         }
       }
@@ -323,7 +323,7 @@ __global__ __launch_bounds__(256, 4) void linear_chunk_prepare(LinLayer L, LinBa
     }
     const double* gsum = gsums[i & 3];
     const float* strength = strengths[i & 3];
-    const float fmax_ = gtop[i & 3][0], whole = gtop[i & 3][1];
+    const float gmax = gtop[i & 3][0], fmax_ = gtop[i & 3][1], whole = gtop[i & 3][2];
     bool bad = bad_k || gbad[i & 3];
     // A and P of this wave's rows
     uint32_t pm = 0;
@@ -382,7 +382,7 @@ __global__ __launch_bounds__(256, 4) void linear_chunk_prepare(LinLayer L, LinBa
       put(W::P, kb, ps, x);
     }
     int ts = 0;
-    float tsum = 1.0f, wtop = 0.0f;
+    float tsum = 1.0f;
     if constexpr (DELTA) {
       __syncthreads();  // P is read; A is there
       {  // the diagonal block of this wave, a column a lane (four lanes alike)
@@ -445,79 +445,10 @@ __global__ __launch_bounds__(256, 4) void linear_chunk_prepare(LinLayer L, LinBa
       for (int kb = 0; kb < 2; kb++)
         if (2 * kb <= wave) put(W::T, kb, ts, x[kb]);
       sum = __uint_as_float(wave_umax(mag(groups_sum(sum))));  // (a NaN counts as the largest)
-      // T e^G of this wave's rows, in A's place
-      const float* fade = fades[i & 3];
-      float wsum = 0.0f;
-      big = 0;
-#pragma unroll
-      for (int kb = 0; kb < 2; kb++)
-        if (2 * kb <= wave)
-#pragma unroll
-          for (int e = 0; e < 8; e++) {
-            x[kb][e] *= fade[32 * kb + 16 * (e >> 2) + 4 * g + (e & 3)];
-            wsum += fabsf(x[kb][e]);
-            big = max(big, mag(x[kb][e]));
-          }
-      big = wave_umax(big);
-      const int ys = shift_for(__uint_as_float(big));
-      half8* wt = (half8*)Am;
-#pragma unroll
-      for (int kb = 0; kb < 2; kb++)
-        if (2 * kb <= wave) {
-          half8 hi, lo;
-#pragma unroll
-          for (int e = 0; e < 8; e++) x[kb][e] = ldexpf(x[kb][e], ys);
-          split8(x[kb], hi, lo);
-          wt[((wave * 2 + kb) * 2 + 0) * 64 + lane] = hi;
-          wt[((wave * 2 + kb) * 2 + 1) * 64 + lane] = lo;
-        }
-      wsum = ldexpf(__uint_as_float(wave_umax(mag(groups_sum(wsum)))), -ts);
-      if (lane == 0) {
-        sums[wave] = sum;
-        wsums[wave] = wsum;
-        wheld[wave] = ts + ys;
-      }
+      if (lane == 0) sums[wave] = sum;
       __syncthreads();
-      {  // W = T e^G K, transposed: this wave's key dims of all rows
-        const auto rk = buffer((const void*)wk, 16 * W::PER_K);
-        half8 kt[DK / 64][2][2];
-#pragma unroll
-        for (int td = 0; td < DK / 64; td++)
-#pragma unroll
-          for (int kb = 0; kb < 2; kb++)
-#pragma unroll
-            for (int hl = 0; hl < 2; hl++) kt[td][kb][hl] = load8(rk, 16 * lane + wave * (DK / 64 * 2 * 2 * 64 * 16), W::KT + ((td * 2 + kb) * 2 + hl) * 64);
-#pragma unroll
-        for (int rt = 0; rt < 4; rt++) {
-          f4 acc[DK / 64] = {};
-#pragma unroll
-          for (int kb = 0; kb < 2; kb++) {
-            if (2 * kb > rt) continue;
-            const half8 bh = wt[((rt * 2 + kb) * 2 + 0) * 64 + lane], bl = wt[((rt * 2 + kb) * 2 + 1) * 64 + lane];
-#pragma unroll
-            for (int td = 0; td < DK / 64; td++) acc[td] = product3(kt[td][kb][0], kt[td][kb][1], bh, bl, acc[td]);
-          }
-          const int by = wshift_of(wsums[rt], kmax) - ks - wheld[rt];
-          if constexpr (DK == 128) {
-            float y[8];
-            half8 hi, lo;
-#pragma unroll
-            for (int e = 0; e < 8; e++) y[e] = ldexpf(acc[e >> 2][e & 3], by);
-            split8(y, hi, lo);
-            __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u4, hi), rh, 16 * lane + 2048 * wave, 16 * (W::W + rt * NKB * 128), 0);
-            __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u4, lo), rh, 16 * lane + 2048 * wave, 16 * (W::W + rt * NKB * 128 + 64), 0);
-          } else {
-            u2 hi, lo;
-            split4(ldexpf(acc[0][0], by), ldexpf(acc[0][1], by), ldexpf(acc[0][2], by), ldexpf(acc[0][3], by), hi, lo);
-            const int at = 16 * lane + 2048 * (wave >> 1) + 8 * (wave & 1);
-            __builtin_amdgcn_raw_buffer_store_b64(hi, rh, at, 16 * (W::W + rt * NKB * 128), 0);
-            __builtin_amdgcn_raw_buffer_store_b64(lo, rh, at, 16 * (W::W + rt * NKB * 128 + 64), 0);
-          }
-        }
-      }
       tsum = fmaxf(fmaxf(sums[0], sums[1]), fmaxf(sums[2], sums[3]));
-      wtop = fmaxf(fmaxf(wsums[0], wsums[1]), fmaxf(wsums[2], wsums[3]));
-      for (int w = 0; w < 4; w++) bad = bad || !(sums[w] < 0x1p60f) || !(wsums[w] < 0x1p60f);
+      for (int w = 0; w < 4; w++) bad = bad || !(sums[w] < 0x1p60f);
     } else {
       __syncthreads();
     }
@@ -527,11 +458,10 @@ __global__ __launch_bounds__(256, 4) void linear_chunk_prepare(LinLayer L, LinBa
       meta->qshift[wave] = qs;
       meta->tshift[wave] = ts;
       meta->pshift[wave] = ps;
-      if constexpr (DELTA) meta->wshift[wave] = wshift_of(wsums[wave], kmax);
       if (wave == 0) {
         meta->kshift = ks;
         meta->whole = whole;
-        meta->ew = bad ? kBad : top_exponent(wtop) + top_exponent(DK * kmax);
+        meta->ey = bad ? kBad : top_exponent(gmax) + top_exponent(DK * kmax);
         meta->et = top_exponent(tsum);
         meta->ef = top_exponent(fmax_);
         meta->es = whole > 0.0f ? top_exponent(whole) : -200;
@@ -541,7 +471,7 @@ __global__ __launch_bounds__(256, 4) void linear_chunk_prepare(LinLayer L, LinBa
   }
 }
 
-enum { M_KSHIFT = 0, M_QSHIFT = 1, M_TSHIFT = 5, M_PSHIFT = 9, M_WSHIFT = 13, M_WHOLE = 17, M_EW, M_ET, M_EF, M_ES, M_EK };
+enum { M_KSHIFT = 0, M_QSHIFT = 1, M_TSHIFT = 5, M_PSHIFT = 9, M_WHOLE = 13, M_EY, M_ET, M_EF, M_ES, M_EK };
 static_assert(offsetof(ChunkMeta, ek) == 4 * M_EK && offsetof(ChunkMeta, pshift) == 4 * M_PSHIFT, "meta words");
 
 // A sequence's chunks from u0 up to u1 (its window of the workspace) for 16 NT value dims of a head. Four waves carry
@@ -558,7 +488,7 @@ __global__ __launch_bounds__(512, NT == 1 ? 4 : 2) void linear_chunk_scan(LinLay
   constexpr int NKB = W::NKB, MT = DK / 64, kCols = 16 * NT, SLICES = DV / kCols;
   __shared__ half8 Sb[NKB * NT * 2 * 64];        // the state as an operand
   __shared__ half8 Yb[2 * NT * 2 * 64], Vb[2][2 * NT * 2 * 64], Fb[2 * NT * 2 * 64];  // Y, V' (of this chunk and the one before), e^(G_n - G) V'
-  __shared__ uint32_t smax[4][kCols], vmax[2][4][kCols];
+  __shared__ uint32_t smax[4][kCols], vmax[4][kCols];
   __shared__ float plain[kCols][DK + 4];        // columns that are done row by row: the state before
   __shared__ int slow_from[kCols];              // this chunk of the sequence
   // a key head's value heads and slices, which read the same operands, run on one XCD
@@ -599,32 +529,26 @@ __global__ __launch_bounds__(512, NT == 1 ? 4 : 2) void linear_chunk_scan(LinLay
   // The powers of two of a chunk's columns (this lane's two), from what is noted of S and V; next_m bounds the
   // next state. `out`: columns that are not for these products.
   struct Shifts {
-    int u[NT], v[NT], f[NT], s_next[NT];
+    int y[NT], v[NT], f[NT], s_next[NT];
     uint32_t out;
   };
-  auto noted_v = [&](int u, int nt) {
-    const int c = 16 * nt + n;
-    const auto& m = vmax[u & 1];
-    return max(max(m[0][c], m[1][c]), max(m[2][c], m[3][c]));
-  };
-  // a power of two above what is noted (of nothing: what adds nothing to a maximum)
-  auto above = [&](uint32_t m) { return m ? top_exponent(__uint_as_float(m)) : -200; };
-  auto shifts = [&](int u) {
+  auto shifts = [&]() {
     Shifts t;
     t.out = 0;
-    const int cw = word(M_EW), ct = word(M_ET), cf = word(M_EF), cs = word(M_ES), ck = word(M_EK);
+    const int cy = word(M_EY), ct = word(M_ET), cf = word(M_EF), cs = word(M_ES), ck = word(M_EK);
 #pragma unroll
     for (int nt = 0; nt < NT; nt++) {
       const int c = 16 * nt + n;
       const uint32_t sm = max(max(smax[0][c], smax[1][c]), max(smax[2][c], smax[3][c]));
-      const uint32_t vm = noted_v(u, nt);
-      const int es = above(sm), ev = above(vm);
-      const int evp = DELTA ? max(ev + ct, es + cw) + 1 : ev, ef = evp + cf, en = max(es + cs, ef + ck) + 1;
-      t.u[nt] = kTop - ev;
+      const uint32_t vm = max(max(vmax[0][c], vmax[1][c]), max(vmax[2][c], vmax[3][c]));
+      // powers of two above them (of nothing: what adds nothing to a maximum)
+      const int es = sm ? top_exponent(__uint_as_float(sm)) : -200, ev = vm ? top_exponent(__uint_as_float(vm)) : -200;
+      const int ey = DELTA ? max(ev, es + cy) + 1 : ev, evp = ey + ct, ef = evp + cf, en = max(es + cs, ef + ck) + 1;
+      t.y[nt] = kTop - ey;
       t.v[nt] = kTop - evp;
       t.f[nt] = kTop - ef;
       t.s_next[nt] = kTop - en;
-      const bool out = max(sm, vm) >= kInf || max(max(es, ev), max(evp, en)) >= 120 || cw >= kBad / 2;
+      const bool out = max(sm, vm) >= kInf || max(max(es, ey), max(evp, en)) >= 120 || cy >= kBad / 2;
       t.out |= (uint32_t)(__ballot(out) & 0xffffu) << (16 * nt);
     }
     t.out = uniform(t.out);
@@ -649,29 +573,22 @@ __global__ __launch_bounds__(512, NT == 1 ? 4 : 2) void linear_chunk_scan(LinLay
       lo[nt] = from[((kb * NT + nt) * 2 + 1) * 64 + lane];
     }
   };
-  auto put4 = [&](half8* to, int tile, int nt, float a, float b, float c, float d) {
-    u2 hi, lo;
-    split4(a, b, c, d, hi, lo);
-    char* p = (char*)(to + (((tile >> 1) * NT + nt) * 2) * 64 + lane) + 8 * (tile & 1);
-    *(u2*)p = hi;
-    *(u2*)(p + 64 * 16) = lo;
-  };
   uint32_t slow = 0;  // the columns that are done row by row
   int sshift[NT];
   f4 S[MT][NT];
 
   if (role == 0) {
     __builtin_amdgcn_s_setprio(2);  // the state is what everything waits for
-    half8 fw[NKB][2], ft[2][2], fkt[MT][2][2];
-    float v[2][NT][4];  // this chunk's and the next one's (sum rule)
-    f4 fg;
-    auto load_w = [&](int u) {
-      const auto r = head(u);
+    half8 fk[NKB][2], ft[2][2], fkt[MT][2][2];
+    float v[2][NT][4];  // this chunk's and the next one's
+    f4 eg, fg;
+    auto load_k = [&](int u) {
+      const auto r = keys(u);
       if constexpr (DELTA)
 #pragma unroll
         for (int kb = 0; kb < NKB; kb++)
 #pragma unroll
-          for (int hl = 0; hl < 2; hl++) fw[kb][hl] = load8(r, at_k, W::W + (kb * 2 + hl) * 64);
+          for (int hl = 0; hl < 2; hl++) fk[kb][hl] = load8(r, at_k, W::K + (kb * 2 + hl) * 64);
     };
     auto load_t = [&](int u) {
       const auto r = head(u);
@@ -696,6 +613,13 @@ __global__ __launch_bounds__(512, NT == 1 ? 4 : 2) void linear_chunk_scan(LinLay
       const int l = afresh(lane);
       if (l < 16) smax[wave][16 * nt + l] = t;
     };
+    auto put4 = [&](half8* to, int tile, int nt, float a, float b, float c, float d) {
+      u2 hi, lo;
+      split4(a, b, c, d, hi, lo);
+      char* p = (char*)(to + (((tile >> 1) * NT + nt) * 2) * 64 + lane) + 8 * (tile & 1);
+      *(u2*)p = hi;
+      *(u2*)(p + 64 * 16) = lo;
+    };
     auto put_state = [&]() {
 #pragma unroll
       for (int i = 0; i < MT; i++)
@@ -709,13 +633,14 @@ __global__ __launch_bounds__(512, NT == 1 ? 4 : 2) void linear_chunk_scan(LinLay
       for (int nt = 0; nt < NT; nt++)
         S[i][nt] = from >= 0 ? *(const f4*)(L.state + (((size_t)from * L.v_heads + h) * DV + col0 + 16 * nt + n) * DK + 16 * (wave * MT + i) + 4 * g)
                              : f4{0, 0, 0, 0};
-    if constexpr (!DELTA) load_v(first, v[0]);
+    load_v(first, v[0]);
     load_meta(first);
-    load_w(first);
-    load_t(first);
+    load_k(first);
+    eg = load_fade(first, 0);
     fg = load_fade(first, 256);
+    load_t(first);
     load_kt(first);
-    if constexpr (!DELTA) load_v(min(first + 1, last - 1), v[1]);
+    load_v(min(first + 1, last - 1), v[1]);
 #pragma unroll
     for (int nt = 0; nt < NT; nt++) {
       uint32_t t = 0;
@@ -739,40 +664,45 @@ __global__ __launch_bounds__(512, NT == 1 ? 4 : 2) void linear_chunk_scan(LinLay
 #pragma unroll 1
     for (int u = first; u < last; u++) {
       const int next = min(u + 1, last - 1);
-      const int kshift = word(M_KSHIFT), tshift = word(M_TSHIFT + wave), wshift = word(M_WSHIFT + wave);
+      const int kshift = word(M_KSHIFT), tshift = word(M_TSHIFT + wave);
       const float whole = fword(M_WHOLE);
-      __syncthreads();  // the state, V, and what is noted of them
-      const Shifts sh = shifts(u);
+      __syncthreads();  // the state, and what is noted of it and of V
+      const Shifts sh = shifts();
       load_meta(next);
       f4 vp[NT];
       if constexpr (DELTA) {
-        f4 ks[NT] = {}, tv[NT] = {};
+        f4 ks[NT] = {};
 #pragma unroll
         for (int kb = 0; kb < NKB; kb++) {
           half8 hi[NT], lo[NT];
           operands(Sb, kb, hi, lo);
-          products3(fw[kb][0], fw[kb][1], hi, lo, ks);
+          products3(fk[kb][0], fk[kb][1], hi, lo, ks);
         }
         __builtin_amdgcn_sched_barrier(0);
-        load_w(next);
+        load_k(next);
         __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++) {
+          // Y 2^y, the product's own powers in one factor: below 2^-149 its share is nothing beside Y's bound
+          const float f = ldexpf(1.0f, sh.y[nt] - kshift - sshift[nt]);
+          float y[4];
+#pragma unroll
+          for (int r = 0; r < 4; r++) y[r] = fmaf(-(eg[r] * f), ks[nt][r], ldexpf(v[0][nt][r], sh.y[nt]));
+          put4(Yb, wave, nt, y[0], y[1], y[2], y[3]);
+        }
+        eg = load_fade(next, 0);
+        __syncthreads();
+        for (int nt = 0; nt < NT; nt++) vp[nt] = f4{0, 0, 0, 0};
 #pragma unroll
         for (int kb = 0; kb < 2; kb++)
           if (2 * kb <= wave) {
             half8 hi[NT], lo[NT];
             operands(Yb, kb, hi, lo);
-            products3(ft[kb][0], ft[kb][1], hi, lo, tv);
+            products3(ft[kb][0], ft[kb][1], hi, lo, vp);
           }
         __builtin_amdgcn_sched_barrier(0);
         load_t(next);
         __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-        for (int nt = 0; nt < NT; nt++) {
-          // V' 2^v, the products' own powers in a factor each: below 2^-149 a share is nothing beside V's bound
-          const float ft = ldexpf(1.0f, sh.v[nt] - tshift - sh.u[nt]), fs = ldexpf(1.0f, sh.v[nt] - wshift - sshift[nt]);
-#pragma unroll
-          for (int r = 0; r < 4; r++) vp[nt][r] = fmaf(ft, tv[nt][r], -(fs * ks[nt][r]));
-        }
       } else {
 #pragma unroll
         for (int nt = 0; nt < NT; nt++)
@@ -782,7 +712,7 @@ __global__ __launch_bounds__(512, NT == 1 ? 4 : 2) void linear_chunk_scan(LinLay
       // V' as it is held: times 2^held
       int held[NT];
 #pragma unroll
-      for (int nt = 0; nt < NT; nt++) held[nt] = DELTA ? sh.v[nt] : 0;
+      for (int nt = 0; nt < NT; nt++) held[nt] = DELTA ? tshift + sh.y[nt] : 0;
 #pragma unroll
       for (int nt = 0; nt < NT; nt++) {
         const float f = ldexpf(1.0f, sh.f[nt] - held[nt]);
@@ -828,9 +758,8 @@ __global__ __launch_bounds__(512, NT == 1 ? 4 : 2) void linear_chunk_scan(LinLay
         }
         sshift[nt] = sh.s_next[nt];
         note(nt, __float_as_uint(ldexpf(t, -sshift[nt])));
-        if constexpr (!DELTA)
 #pragma unroll
-          for (int r = 0; r < 4; r++) v[0][nt][r] = moved(v[1][nt][r]);
+        for (int r = 0; r < 4; r++) v[0][nt][r] = moved(v[1][nt][r]);
       }
       put_state();
       // V' for the output waves, which take it behind the next barrier
@@ -839,11 +768,9 @@ __global__ __launch_bounds__(512, NT == 1 ? 4 : 2) void linear_chunk_scan(LinLay
         const int e = sh.v[nt] - held[nt];
         put4(Vb[u & 1], wave, nt, ldexpf(vp[nt][0], e), ldexpf(vp[nt][1], e), ldexpf(vp[nt][2], e), ldexpf(vp[nt][3], e));
       }
-      if constexpr (!DELTA) {
-        __builtin_amdgcn_sched_barrier(0);
-        load_v(min(u + 2, last - 1), v[1]);
-        __builtin_amdgcn_sched_barrier(0);
-      }
+      __builtin_amdgcn_sched_barrier(0);
+      load_v(min(u + 2, last - 1), v[1]);
+      __builtin_amdgcn_sched_barrier(0);
     }
     __syncthreads();
   } else {
@@ -864,7 +791,7 @@ __global__ __launch_bounds__(512, NT == 1 ? 4 : 2) void linear_chunk_scan(LinLay
         for (int hl = 0; hl < 2; hl++)
           if (2 * kb <= wave) fp[kb][hl] = load8(r, at_t, W::P + (kb * 2 + hl) * 64);
     };
-    auto note_v = [&](int u, const float (&of)[NT][4]) {
+    auto note_v = [&](const float (&of)[NT][4]) {
 #pragma unroll
       for (int nt = 0; nt < NT; nt++) {
         uint32_t t = 0;
@@ -872,7 +799,7 @@ __global__ __launch_bounds__(512, NT == 1 ? 4 : 2) void linear_chunk_scan(LinLay
         for (int r = 0; r < 4; r++) t = max(t, mag(of[nt][r]));
         t = groups_max(t);
         const int l = afresh(lane);
-        if (l < 16) vmax[u & 1][wave][16 * nt + l] = t;
+        if (l < 16) vmax[wave][16 * nt + l] = t;
       }
     };
     float v[NT][4];
@@ -906,18 +833,9 @@ __global__ __launch_bounds__(512, NT == 1 ? 4 : 2) void linear_chunk_scan(LinLay
     load_q(first);
     eg = load_fade(first, 0);
     load_p(first);
-    note_v(first, v);
-    auto put_v = [&](int u) {  // V of chunk u, noted before the last barrier, for the state waves
-      if constexpr (DELTA)
-#pragma unroll
-        for (int nt = 0; nt < NT; nt++) {
-          const int e = kTop - above(noted_v(u, nt));
-          put4(Yb, wave, nt, ldexpf(v[nt][0], e), ldexpf(v[nt][1], e), ldexpf(v[nt][2], e), ldexpf(v[nt][3], e));
-        }
-    };
-    __syncthreads();
-    put_v(first);
+    note_v(v);
     load_v(min(first + 1, last - 1), v);
+    __syncthreads();
 #pragma unroll
     for (int nt = 0; nt < NT; nt++) sshift[nt] = first_shift(nt);
     int vshift[NT] = {}, pshift = 0;
@@ -925,7 +843,7 @@ __global__ __launch_bounds__(512, NT == 1 ? 4 : 2) void linear_chunk_scan(LinLay
     for (int u = first; u < last; u++) {
       const int next = min(u + 1, last - 1);
       __syncthreads();
-      const Shifts sh = shifts(u);
+      const Shifts sh = shifts();
       const int qshift = word(M_QSHIFT + wave), pshift_now = word(M_PSHIFT + wave);
       load_meta(next);
       f4 now[NT] = {};
@@ -938,7 +856,8 @@ __global__ __launch_bounds__(512, NT == 1 ? 4 : 2) void linear_chunk_scan(LinLay
       __builtin_amdgcn_sched_barrier(0);
       load_q(next);
       __builtin_amdgcn_sched_barrier(0);
-      // the state waves hurry from here to the second barrier: the chunk before is finished behind it
+      if constexpr (DELTA) __syncthreads();
+      // the state waves hurry from here to the third barrier: the chunk before is finished behind it
 #pragma unroll
       for (int nt = 0; nt < NT; nt++) {
         const float f = a.scale * ldexpf(1.0f, -qshift - sshift[nt]);
@@ -946,9 +865,8 @@ __global__ __launch_bounds__(512, NT == 1 ? 4 : 2) void linear_chunk_scan(LinLay
         for (int r = 0; r < 4; r++) now[nt][r] = eg[r] * (f * now[nt][r]);
       }
       eg = load_fade(next, 0);
-      note_v(u + 1, v);
       __syncthreads();
-      put_v(u + 1);
+      note_v(v);
       __builtin_amdgcn_sched_barrier(0);
       load_v(min(u + 2, last - 1), v);
       __builtin_amdgcn_sched_barrier(0);

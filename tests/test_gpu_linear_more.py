@@ -22,9 +22,9 @@ def inputs(T, Hk, Hv, seed, rule="delta"):
 @pytest.mark.parametrize("rows", [[6000], [3000, 3000]])
 @pytest.mark.parametrize("rule", ["delta", "sum"])
 def test_prompts_longer_than_the_workspace(dev, rule, rows):
-    """Of 16 key and 48 value heads a chunk's operands take 16 x 65,536 + 48 x 66,176 bytes: 63 chunks fit 256 MiB. A
+    """Of 16 key and 48 value heads a chunk's operands take 16 x 98,304 + 48 x 33,408 bytes: 84 chunks fit 256 MiB. A
     prompt that goes on behind them has the bits of two calls with the state carried, cut there."""
-    Hk, Hv, window = 16, 48, (256 << 20) // (16 * 65536 + 48 * 66176)
+    Hk, Hv, window = 16, 48, (256 << 20) // (16 * 98304 + 48 * 33408)
     x = inputs(sum(rows), Hk, Hv, 5, rule)
     cut = 64 * window - (0 if len(rows) == 1 else 64 * ((rows[0] + 63) // 64) - rows[0])
     start = torch.randn(1, 2, Hv, 128, 128, device="cuda") * 0.1
