@@ -17,7 +17,10 @@ constexpr int kLinChunk = 64;     // rows of a unit
 // them 50 + 7.2 and 280: they meet at 29, 41 and 32 rows), one of the sum rule 5 + 0.75 and 20.5 (64: 45 + 6.2 and 177:
 // at 21). A batch does not know the rule: a number between.
 constexpr int kLinChunkFrom = 28;
-constexpr size_t kLinSpace = (size_t)256 << 20;  // most bytes of chunk operands at a time
+// Most bytes of chunk operands at a time: what the scan reads should still be in the 256 MiB behind the L2s that the
+// preparation wrote it to, beside the rows themselves. 8192 rows of 48 heads (3.2 MB a chunk): 64 MiB 602 us (passes of 19
+// chunks), 80 530, 104 489, 128 488, 160 489, 208 525, 400 525.
+constexpr size_t kLinSpace = (size_t)128 << 20;
 
 // a row's decay as hi + lo: the rounding of one float would add up over the rows of a constant decay
 __device__ inline void fade_of(float g, float& hi, float& lo) {

@@ -596,8 +596,7 @@ __global__ __launch_bounds__(512, NT == 1 ? 4 : 2) void linear_chunk_scan(LinLay
 #pragma unroll
         for (int kb = 0; kb < 2; kb++)
 #pragma unroll
-          for (int hl = 0; hl < 2; hl++)
-            if (2 * kb <= wave) ft[kb][hl] = load8(r, at_t, W::T + (kb * 2 + hl) * 64);
+          for (int hl = 0; hl < 2; hl++) ft[kb][hl] = load8(r, at_t, W::T + (kb * 2 + hl) * 64);  // (also what no product takes)
     };
     auto load_kt = [&](int u) {
       const auto r = keys(u);
@@ -788,8 +787,7 @@ __global__ __launch_bounds__(512, NT == 1 ? 4 : 2) void linear_chunk_scan(LinLay
 #pragma unroll
       for (int kb = 0; kb < 2; kb++)
 #pragma unroll
-        for (int hl = 0; hl < 2; hl++)
-          if (2 * kb <= wave) fp[kb][hl] = load8(r, at_t, W::P + (kb * 2 + hl) * 64);
+        for (int hl = 0; hl < 2; hl++) fp[kb][hl] = load8(r, at_t, W::P + (kb * 2 + hl) * 64);
     };
     auto note_v = [&](const float (&of)[NT][4]) {
 #pragma unroll
@@ -803,16 +801,16 @@ __global__ __launch_bounds__(512, NT == 1 ? 4 : 2) void linear_chunk_scan(LinLay
       }
     };
     float v[NT][4];
-    f4 o[NT];
-    // what V' adds to the rows of chunk u, and their store, but for the columns `left_out`
-    auto finish = [&](int u, int pshift, const int (&vshift)[NT], uint32_t left_out) {
+    f4 o[NT] = {};
+    // what V' (in Vb[half]) adds to the rows of chunk u, and their store, but for the columns `left_out`
+    auto finish = [&](int u, int half, int pshift, const int (&vshift)[NT], uint32_t left_out) {
       const auto ro = values(a.out, u);
       f4 acc[NT] = {};
 #pragma unroll
       for (int kb = 0; kb < 2; kb++)
         if (2 * kb <= wave) {
           half8 hi[NT], lo[NT];
-          operands(Vb[u & 1], kb, hi, lo);
+          operands(Vb[half], kb, hi, lo);
           products3(fp[kb][0], fp[kb][1], hi, lo, acc);
         }
 #pragma unroll
@@ -821,12 +819,16 @@ __global__ __launch_bounds__(512, NT == 1 ? 4 : 2) void linear_chunk_scan(LinLay
 #pragma unroll
         for (int r = 0; r < 4; r++) acc[nt][r] = fmaf(f, acc[nt][r], o[nt][r]);
       }
-      int at = afresh(vlane);
+      // (A column that is left out, and with the first chunk every one, is stored past the buffer's end, which drops it:
+      // with a branch there a wait for what was loaded before would not know how many stores came after, and wait for them.)
+      int at[NT];
 #pragma unroll
-      for (int r = 0; r < 4; r++, at += vrow)
+      for (int nt = 0; nt < NT; nt++) at[nt] = left_out >> (16 * nt + n) & 1 ? 0x40000000 : afresh(vlane) + 64 * nt;
 #pragma unroll
-        for (int nt = 0; nt < NT; nt++)
-          if (!(left_out >> (16 * nt + n) & 1)) __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(acc[nt][r]), ro, at + 64 * nt, 0, 0);
+      for (int r = 0; r < 4; r++)
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++, at[nt - 1] += vrow)
+          __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(acc[nt][r]), ro, at[nt], 0, 0);
     };
     load_v(first, v);
     load_meta(first);
@@ -862,20 +864,21 @@ __global__ __launch_bounds__(512, NT == 1 ? 4 : 2) void linear_chunk_scan(LinLay
       for (int nt = 0; nt < NT; nt++) {
         const float f = a.scale * ldexpf(1.0f, -qshift - sshift[nt]);
 #pragma unroll
-        for (int r = 0; r < 4; r++) now[nt][r] = eg[r] * (f * now[nt][r]);
+        for (int r = 0; r < 4; r++) {
+          now[nt][r] = eg[r] * (f * now[nt][r]);
+          asm volatile("" : "+v"(now[nt][r]));  // here: moved to where it is read next, it would keep eg from its next load
+        }
       }
       eg = load_fade(next, 0);
       __syncthreads();
       note_v(v);
+      finish(max(u - 1, first), u & 1 ^ 1, pshift, vshift, u > first ? slow : ~0u);
+      __builtin_amdgcn_sched_barrier(0);
+      load_p(u);
+      __builtin_amdgcn_sched_barrier(0);
       __builtin_amdgcn_sched_barrier(0);
       load_v(min(u + 2, last - 1), v);
       __builtin_amdgcn_sched_barrier(0);
-      if (u > first) {
-        finish(u - 1, pshift, vshift, slow);
-        __builtin_amdgcn_sched_barrier(0);
-        load_p(u);
-        __builtin_amdgcn_sched_barrier(0);
-      }
 #pragma unroll
       for (int nt = 0; nt < NT; nt++) {
         o[nt] = now[nt];
@@ -886,7 +889,7 @@ __global__ __launch_bounds__(512, NT == 1 ? 4 : 2) void linear_chunk_scan(LinLay
       slow |= sh.out;
     }
     __syncthreads();
-    finish(last - 1, pshift, vshift, slow);
+    finish(last - 1, (last - 1) & 1, pshift, vshift, slow);
   }
   float* left = L.state + (((size_t)uniform(sp->dst) * L.v_heads + h) * DV + col0) * DK;
   if (role == 0)
@@ -970,8 +973,10 @@ void launch_scan(const LinLayer& L, const LinBatchView& b, const LinAttnArgs& a,
 
 template <int DK, int DV, bool DELTA>
 hipError_t launch_t(const LinLayer& L, const LinBatchView& b, const LinAttnArgs& a, hipStream_t st) {
-  for (int u0 = 0; u0 < b.n_chunk_units; u0 += b.window) {
-    const int u1 = std::min(u0 + b.window, b.n_chunk_units);
+  // as few passes as the workspace allows, of one size
+  const int passes = (b.n_chunk_units + b.window - 1) / b.window, step = (b.n_chunk_units + passes - 1) / passes;
+  for (int u0 = 0; u0 < b.n_chunk_units; u0 += step) {
+    const int u1 = std::min(u0 + step, b.n_chunk_units);
     hipLaunchKernelGGL((linear_chunk_prepare<DK, DELTA>), dim3(u1 - u0, L.k_heads), dim3(256), 0, st, L, b, a, u0);
     // 32 value dims a workgroup; of the sum rule, whose chain is short, 16 where that still fits the GPU twice (2 x
     // 2048 rows of 16 heads, 128 workgroups of 32: 59 us, 256 of 16: 50; more workgroups than 512 of 16, each

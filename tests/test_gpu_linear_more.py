@@ -9,6 +9,7 @@ from tests.linear_helpers import Case, cuda
 from tests.test_gpu_proj4 import Weight, check
 
 pytestmark = pytest.mark.gpu
+SPACE = 128 << 20  # kLinSpace in bg_linear.h
 
 
 def inputs(T, Hk, Hv, seed, rule="delta"):
@@ -19,29 +20,35 @@ def inputs(T, Hk, Hv, seed, rule="delta"):
     return [q, k, r(T, Hv, 128), -torch.exp(r(T, Hv) - 3), beta]
 
 
-@pytest.mark.parametrize("rows", [[6000], [3000, 3000]])
+@pytest.mark.parametrize("rows", [[6000], [2500, 3500], [12000]])
 @pytest.mark.parametrize("rule", ["delta", "sum"])
 def test_prompts_longer_than_the_workspace(dev, rule, rows):
-    """Of 16 key and 48 value heads a chunk's operands take 16 x 98,304 + 48 x 33,408 bytes: 84 chunks fit 256 MiB. A
-    prompt that goes on behind them has the bits of two calls with the state carried, cut there."""
-    Hk, Hv, window = 16, 48, (256 << 20) // (16 * 98304 + 48 * 33408)
+    """Of 16 key and 48 value heads a chunk's operands take 16 x 98,304 + 48 x 33,408 bytes: longer prompts go through
+    the workspace in equal passes, with the bits of calls that are cut there, the state carried."""
+    Hk, Hv, window = 16, 48, SPACE // (16 * 98304 + 48 * 33408)
     x = inputs(sum(rows), Hk, Hv, 5, rule)
-    cut = 64 * window - (0 if len(rows) == 1 else 64 * ((rows[0] + 63) // 64) - rows[0])
+    units = sum((r + 63) // 64 for r in rows)
+    passes = -(-units // window)
+    assert passes > 1
+    step = -(-units // passes)
+    at = [sum(rows[:i]) for i in range(len(rows))]
+    order = sorted(range(len(rows)), key=lambda i: -rows[i])  # the longest sequence's chunks are the first
+    chunks = [(i, r) for i in order for r in range(0, rows[i], 64)]
+    cut_up = []
+    for a in range(0, units, step):
+        mine = [[r for j, r in chunks[a:a + step] if j == i] for i in range(len(rows))]
+        cut_up.append([(i, r[0], min(r[-1] + 64, rows[i])) for i, r in enumerate(mine) if r])
     start = torch.randn(1, 2, Hv, 128, 128, device="cuda") * 0.1
     got = []
-    for pieces in ([(0, sum(rows))], [(0, cut), (cut, sum(rows))]):
+    for calls in ([[(i, 0, r) for i, r in enumerate(rows)]], cut_up):
         cache = E.LinearStateCache(1, Hk, Hv, 128, 128, n_slots=2, conv_width=0, state=start.clone())
         batch = E.LinearBatch(cache, 2, sum(rows))
-        outs = []
-        for i, (a, b) in enumerate(pieces):
-            if len(pieces) == 1:
-                batch.set(rows, [0, 1][:len(rows)])
-            elif i == 0:
-                batch.set([cut] if len(rows) == 1 else [rows[0], cut - rows[0]], [0, 1][:len(rows)])
-            else:
-                batch.set([b - a], [len(rows) - 1])
-            outs.append(E.linear_attention(cache, 0, batch, *[None if t is None else t[a:b] for t in x]))
-        got.append((torch.cat(outs), cache.state))
+        out = torch.zeros(sum(rows), Hv, 128, device="cuda")
+        for call in calls:
+            batch.set([b - a for _, a, b in call], [i for i, _, _ in call])
+            which = torch.cat([torch.arange(at[i] + a, at[i] + b, device="cuda") for i, a, b in call])
+            out[which] = E.linear_attention(cache, 0, batch, *[None if t is None else t[which] for t in x])
+        got.append((out, cache.state))
     assert torch.equal(got[0][1], got[1][1]) and torch.equal(got[0][0], got[1][0])
     assert torch.isfinite(got[0][0]).all() and not torch.equal(got[0][1], start)
 
