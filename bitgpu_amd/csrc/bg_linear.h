@@ -13,9 +13,9 @@ namespace bg {
 
 constexpr int kLinChunk = 64;     // rows of a unit
 // Sequences of at least this many new rows are done in chunks of 64, shorter ones row by row. With 32 heads of 128 x 128
-// one sequence of the delta rule takes 4.9 + 0.87 us a row so and 30 us as a chunk (4 sequences 6 + 0.87 and 41, 64 of
-// them 50 + 7.2 and 280: they meet at 29, 41 and 32 rows), one of the sum rule 5 + 0.75 and 20.5 (64: 45 + 6.2 and 177:
-// at 21). A batch does not know the rule: a number between.
+// one sequence of the delta rule takes 4.9 + 0.87 us a row so and 25 us as a chunk (4 sequences 6 + 0.87 and 35, 64 of
+// them 50 + 7.2 and 300: they meet at 23, 34 and 34 rows), one of the sum rule 5 + 0.75 and 18.5 (64: 45 + 6.2 and 192: at
+// 18 and 24). A batch does not know the rule: a number between.
 constexpr int kLinChunkFrom = 28;
 // Most bytes of chunk operands at a time: what the scan reads should still be in the 256 MiB behind the L2s that the
 // preparation wrote it to, beside the rows themselves. 8192 rows of 48 heads (3.2 MB a chunk): 64 MiB 602 us (passes of 19

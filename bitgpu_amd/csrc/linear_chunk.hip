@@ -35,6 +35,7 @@ typedef float f4 __attribute__((ext_vector_type(4)));
 constexpr int kTop = 14;      // an operand's largest value is below 2^kTop
 constexpr int kFewScans = 256;   // workgroups of 32 value dims of the sum rule's scan
 constexpr int kBad = 1 << 20;
+constexpr int kPrepared = 768;   // workgroups that the preparation is split into, at most
 constexpr int kPad = 68;      // row stride of 64 x 64 matrices in LDS
 constexpr double kLowest = -1e4;  // of a log decay: e^g is 0 in f32 from -104 on
 
@@ -160,9 +161,10 @@ __device__ inline int afresh(int x) {
   return x;
 }
 
-// One chunk and key head (and its value heads): blockIdx.x a unit from u0 on, blockIdx.y the key head.
+// One chunk and key head, and `each` of its value heads: blockIdx.x a unit from u0 on, blockIdx.y the key head and which of
+// its value heads.
 template <int DK, bool DELTA>
-__global__ __launch_bounds__(256, 4) void linear_chunk_prepare(LinLayer L, LinBatchView b, LinAttnArgs a, int u0) {
+__global__ __launch_bounds__(256, 4) void linear_chunk_prepare(LinLayer L, LinBatchView b, LinAttnArgs a, int u0, int each) {
   using W = ChunkSpace<DK>;
   constexpr int NKB = W::NKB;
   constexpr int kMat = 64 * kPad * 4, kFrag = 4 * NKB * 2 * 64 * 16;
@@ -177,7 +179,8 @@ __global__ __launch_bounds__(256, 4) void linear_chunk_prepare(LinLayer L, LinBa
   float* Tm = (float*)(mem + kMat);          // P, then T
   const LinUnit u = b.units[u0 + blockIdx.x];
   if (u0 + (int)blockIdx.x >= b.hdr->n_chunk_units) return;
-  const int kh = blockIdx.y, rep = L.v_heads / L.k_heads;
+  const int rep = L.v_heads / L.k_heads, parts = (rep + each - 1) / each, kh = blockIdx.y / parts;
+  const int i0 = blockIdx.y % parts * each, i1 = min(i0 + each, rep);
   const int wave = uniform(threadIdx.x >> 6), lane_ = threadIdx.x & 63;
   ghalf8* wk = workspace(b) + (size_t)blockIdx.x * (L.k_heads * W::PER_K + L.v_heads * W::PER_H);
   ghalf8* wh0 = wk + (size_t)L.k_heads * W::PER_K;
@@ -234,16 +237,18 @@ __global__ __launch_bounds__(256, 4) void linear_chunk_prepare(LinLayer L, LinBa
     const int i = (wave * NKB + kb) * 2 * 64 + lane;
     frag[i] = kh8[kb];
     frag[i + 64] = kl8[kb];
-    if constexpr (DELTA) {
-      wk[W::K + i] = kh8[kb];
-      wk[W::K + i + 64] = kl8[kb];
+    if (i0 == 0) {
+      if constexpr (DELTA) {
+        wk[W::K + i] = kh8[kb];
+        wk[W::K + i + 64] = kl8[kb];
+      }
+      wk[W::Q + i] = qh[kb];
+      wk[W::Q + i + 64] = ql[kb];
     }
-    wk[W::Q + i] = qh[kb];
-    wk[W::Q + i + 64] = ql[kb];
   }
   __syncthreads();
   // K^T: this wave's tiles of 16 key dims
-  {
+  if (i0 == 0) {
     const _Float16* e = (const _Float16*)frag;
 #pragma unroll
     for (int i = 0; i < DK / 64; i++) {
@@ -284,14 +289,14 @@ __global__ __launch_bounds__(256, 4) void linear_chunk_prepare(LinLayer L, LinBa
   }
 
 #pragma unroll 1
-  for (int i = 0; i < rep; i++) {
+  for (int i = i0; i < i1; i++) {
     const int h = kh * rep + i;
     ghalf8* wh = wh0 + (size_t)h * W::PER_H;
     const auto rh = buffer((const void*)wh, 16 * W::PER_H);
     const int lane = afresh(lane_), m = lane & 15, g = lane >> 4, row = 16 * wave + m;
     __syncthreads();  // the frag reads, or the head before
-    if ((i & 3) == 0) {
-      if (i + wave < rep) {  // the decays' sums: lane = row
+    if ((i - i0 & 3) == 0) {
+      if (i + wave < i1) {  // the decays' sums: lane = row
         const bool on = lane < u.n;
         const size_t rr = u.row0 + (on ? lane : 0);
         const int hh = h + wave;
@@ -321,10 +326,10 @@ __global__ __launch_bounds__(256, 4) void linear_chunk_prepare(LinLayer L, LinBa
       }
       __syncthreads();
     }
-    const double* gsum = gsums[i & 3];
-    const float* strength = strengths[i & 3];
-    const float gmax = gtop[i & 3][0], fmax_ = gtop[i & 3][1], whole = gtop[i & 3][2];
-    bool bad = bad_k || gbad[i & 3];
+    const double* gsum = gsums[i - i0 & 3];
+    const float* strength = strengths[i - i0 & 3];
+    const float gmax = gtop[i - i0 & 3][0], fmax_ = gtop[i - i0 & 3][1], whole = gtop[i - i0 & 3][2];
+    bool bad = bad_k || gbad[i - i0 & 3];
     // A and P of this wave's rows
     uint32_t pm = 0;
 #pragma unroll
@@ -481,7 +486,9 @@ static_assert(offsetof(ChunkMeta, ek) == 4 * M_EK && offsetof(ChunkMeta, pshift)
 // registers of this one's as soon as their last product has been issued: by buffer loads, whose one lane
 // offset and scalar rest leave the registers to the operands. (A register too many costs a wait for everything
 // in flight when it is read back: with 64-bit addresses in vector registers 14 us a chunk, with the row offsets
-// of V and the output kept through the loop 6.8, without 4.0; one set of waves for all of it.)
+// of V and the output kept through the loop 6.8, without 4.0; one set of waves for all of it.) 2.9 us a chunk, of which
+// operands that come from behind the L2 instead of from it take 0.8; the rest is the chain of three products, each with
+// its operand's way through LDS. No unit is more than a third busy.
 template <int DK, int DV, bool DELTA, int NT>
 __global__ __launch_bounds__(512, NT == 1 ? 4 : 2) void linear_chunk_scan(LinLayer L, LinBatchView b, LinAttnArgs a, int u0, int u1) {
   using W = ChunkSpace<DK>;
@@ -977,7 +984,12 @@ hipError_t launch_t(const LinLayer& L, const LinBatchView& b, const LinAttnArgs&
   const int passes = (b.n_chunk_units + b.window - 1) / b.window, step = (b.n_chunk_units + passes - 1) / passes;
   for (int u0 = 0; u0 < b.n_chunk_units; u0 += step) {
     const int u1 = std::min(u0 + step, b.n_chunk_units);
-    hipLaunchKernelGGL((linear_chunk_prepare<DK, DELTA>), dim3(u1 - u0, L.k_heads), dim3(256), 0, st, L, b, a, u0);
+    // A workgroup's value heads one after the other, or, where that leaves most of the GPU idle, workgroups of their own
+    // that share a key head's products (16 key and 48 value heads, one chunk: prompt of 64 rows 38 us, so 28; four
+    // prompts of 256, 16 chunks, 81 and 74; 32 chunks 124 and 125, 8192 rows 486 and 493).
+    const int rep = L.v_heads / L.k_heads, parts = std::max(1, std::min(rep, kPrepared / ((u1 - u0) * L.k_heads)));
+    const int each = (rep + parts - 1) / parts;
+    hipLaunchKernelGGL((linear_chunk_prepare<DK, DELTA>), dim3(u1 - u0, L.k_heads * ((rep + each - 1) / each)), dim3(256), 0, st, L, b, a, u0, each);
     // 32 value dims a workgroup; of the sum rule, whose chain is short, 16 where that still fits the GPU twice (2 x
     // 2048 rows of 16 heads, 128 workgroups of 32: 59 us, 256 of 16: 50; more workgroups than 512 of 16, each
     // reading the same operands, take longer). The delta rule's 192 of 32 over 8192 rows 435 us, 384 of 16 496.
