@@ -486,9 +486,9 @@ static_assert(offsetof(ChunkMeta, ek) == 4 * M_EK && offsetof(ChunkMeta, pshift)
 // registers of this one's as soon as their last product has been issued: by buffer loads, whose one lane
 // offset and scalar rest leave the registers to the operands. (A register too many costs a wait for everything
 // in flight when it is read back: with 64-bit addresses in vector registers 14 us a chunk, with the row offsets
-// of V and the output kept through the loop 6.8, without 4.0; one set of waves for all of it.) 2.9 us a chunk, of which
-// operands that come from behind the L2 instead of from it take 0.8; the rest is the chain of three products, each with
-// its operand's way through LDS. No unit is more than a third busy.
+// of V and the output kept through the loop 6.8, without 4.0; one set of waves for all of it.) 2.9 us a chunk: the
+// chain of three products, each with its operand's way through LDS (with one chunk's operands for all 2.9 too). No unit is
+// more than a third busy.
 template <int DK, int DV, bool DELTA, int NT>
 __global__ __launch_bounds__(512, NT == 1 ? 4 : 2) void linear_chunk_scan(LinLayer L, LinBatchView b, LinAttnArgs a, int u0, int u1) {
   using W = ChunkSpace<DK>;

@@ -800,8 +800,14 @@ def linear_block(cache: LinearStateCache, li: int, batch: LinearBatch, n1, h, w_
         raise ValueError(f"bitgpu_amd: the cache lives on cuda:{dev}, the current device is {_getDevice()}")
     if n1.shape[-1] != w_in.K or h.numel() != M * w_out.N:
         raise ValueError(f"bitgpu_amd: n1 must hold [{M}, {w_in.K}] and h [{M}, {w_out.N}], got {list(n1.shape)} and {list(h.shape)}")
+    # everything that a later launch would refuse, before the first one: the states have moved on behind it
+    for w in (w_in, w_out):
+        if isinstance(w, FourBitWeight):
+            _on(w)
+        elif M != 1:
+            raise ValueError(f"bitgpu_amd: a 1-bit weight's product takes one row, got {M}")
     x, res = _rows_ptr(n1, "n1", M, w_in.K, dev), _rows_ptr(h, "h", M, w_out.N, dev)
-    weights = _layer_ptrs(cache, conv_weight, a_log, dt_bias, norm)
+    weights = _layer_ptrs(cache, conv_weight, a_log, dt_bias, norm, eps)
     # one piece of memory for what lies between the launches: qkv, z, att | b, a (interleaved rows) and the prologue's
     out, wide, Z = n1.new_empty((*n1.shape[:-1], w_out.N)), cache.channels, Hv * DV
     four = [L.bg_gemv4_workspace(M, w.K) // 4 for w in (w_in, w_out)] if 4 < M <= 16 else (0, 0)
@@ -813,25 +819,16 @@ def linear_block(cache: LinearStateCache, li: int, batch: LinearBatch, n1, h, w_
     inner = att + 4 * M * Z
     ba = inner + 4 * M * (wide + 2 * Hv)
     if isinstance(w_in, FourBitWeight):
-        _on(w_in)
         rc = L.bg_gemv4_split(x, M, w_in.K, *w_in._w, wide, Z, 2 * Hv, qkv, z, ba, space, st)
     else:
-        _one_row(M)
         rc = L.bg_gemv_split(x, w_in.K, _ptr(w_in.sign), _ptr(w_in.scales), wide, Z, 2 * Hv, qkv, z, ba, st)
     if rc:
         check(rc)
     _between(cache, li, batch, qkv, ba + 4 * Hv, ba, 2 * Hv, weights, z, eps, inner, att, st)
     if isinstance(w_out, FourBitWeight):
-        _on(w_out)
         rc = L.bg_gemv4_resid(att, M, Z, *w_out._w, w_out.N, res, out.data_ptr(), space, st)
     else:
-        _one_row(M)
         rc = L.bg_gemv_resid(att, Z, _ptr(w_out.sign), _ptr(w_out.scales), w_out.N, res, out.data_ptr(), st)
     if rc:
         check(rc)
     return out
-
-
-def _one_row(M):
-    if M != 1:
-        raise ValueError(f"bitgpu_amd: a 1-bit weight's product takes one row, got {M}")

@@ -297,8 +297,10 @@ def linear_layer_attention(cache: LinearStateCache, li: int, batch: LinearBatch,
     (ap, stride), (bp, b_stride) = _columns_ptr(a, "a", T, Hv, dev), _columns_ptr(b, "b", T, Hv, dev)
     if b_stride != stride and T > 1:
         raise ValueError(f"bitgpu_amd: a and b must have one row stride, got {stride} and {b_stride}")
-    weights = _layer_ptrs(cache, conv_weight, a_log, dt_bias, norm)
+    weights = _layer_ptrs(cache, conv_weight, a_log, dt_bias, norm, eps)
     zp = _rows_ptr(z, "z", T, Hv * DV, dev)
+    if zp and zp & 15:
+        raise ValueError("bitgpu_amd: z must be 16-byte aligned")
     out = qkv.new_empty((qkv.numel() // cache.channels, Hv, DV))
     room = qkv.new_empty(T * (cache.channels + 2 * Hv))
     _between(cache, li, batch, qp, ap, bp, stride, weights, zp, eps, room.data_ptr(), out.data_ptr(), _stream())
@@ -308,12 +310,14 @@ def linear_layer_attention(cache: LinearStateCache, li: int, batch: LinearBatch,
 # What a layer keeps between its launches (q, k, v, the gates) is one piece of memory and goes from one call to the
 # next by address, checked once: a row of linear_layer_attention takes 14 us on the host instead of 22, of
 # engine.linear_block 25 instead of 48.
-def _layer_ptrs(cache, conv_weight, a_log, dt_bias, norm):
+def _layer_ptrs(cache, conv_weight, a_log, dt_bias, norm, eps):
     Hv, dev = cache.v_heads, cache.index
     if any(t is None for t in (conv_weight, a_log, dt_bias, norm)):
         raise ValueError("bitgpu_amd: the layer needs conv_weight, a_log, dt_bias and norm")
-    return (_conv_ptr(cache, conv_weight), _rows_ptr(a_log, "a_log", 1, Hv, dev), _rows_ptr(dt_bias, "dt_bias", 1, Hv, dev),
-            _rows_ptr(norm, "norm", 1, cache.v_dim, dev))
+    norm_at = _rows_ptr(norm, "norm", 1, cache.v_dim, dev)
+    if not eps >= 0 or norm_at & 15:  # (the prologue has moved the convolution's inputs on when the attention refuses them)
+        raise ValueError(f"bitgpu_amd: eps must not be negative and norm 16-byte aligned, got {eps}")
+    return _conv_ptr(cache, conv_weight), _rows_ptr(a_log, "a_log", 1, Hv, dev), _rows_ptr(dt_bias, "dt_bias", 1, Hv, dev), norm_at
 
 
 def _between(cache, li, batch, qkv, a, b, stride, weights, z, eps, room, out, stream):

@@ -186,8 +186,11 @@ def test_layers(host, monkeypatch):
             call(conv_weight=z(CH, 2))
         with pytest.raises(ValueError, match="norm holds"):
             call(norm=z(D - 1))
+        for bad in (dict(eps=-1e-6), dict(eps=float("nan")), dict(norm=z(D + 1)[1:])):
+            with pytest.raises(ValueError, match="eps must not be negative and norm 16-byte aligned"):
+                call(**bad)
     for k, match in ((dict(a=None), "needs a and b"), (dict(b=None), "needs a and b"), (dict(a=z(3, 2 * HV)[:, HV:]), "one row stride"),
-                     (dict(qkv=z(2, CH)), "qkv holds"), (dict(z=z(2, HV, D)), "z holds")):
+                     (dict(qkv=z(2, CH)), "qkv holds"), (dict(z=z(2, HV, D)), "z holds"), (dict(z=z(3 * HV * D + 1)[1:]), "z must be 16-byte")):
         with pytest.raises(ValueError, match=match):
             between(**k)
     for k, match in ((dict(w_in=four(CH, HV * D, HV)), "the weights' rows must be"), (dict(w_out=four(30, K=256)), "the weights' rows must be"),
@@ -200,6 +203,12 @@ def test_layers(host, monkeypatch):
     one = types.SimpleNamespace(N0=CH, N1=HV * D, N2=2 * HV, K=256, sign=None, scales=None)
     with pytest.raises(ValueError, match="takes one row, got 3"):
         block(w_in=one)
+    with pytest.raises(ValueError, match="takes one row, got 3"):
+        block(w_out=types.SimpleNamespace(N=30, K=HV * D, sign=None, scales=None))
+    away = four(30, K=HV * D)
+    away.index = 1
+    with pytest.raises(ValueError, match="the weight is on cuda:1"):
+        block(w_out=away)
     monkeypatch.setattr(E, "_getDevice", lambda: 0)
     with pytest.raises(ValueError, match="the cache lives on cuda:-1"):
         block()
