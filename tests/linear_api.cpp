@@ -117,7 +117,7 @@ hipError_t launch_linear_chunks(const LinLayer&, const LinBatchView& b, const Li
   note("chunks on %d", sid(st));
   return hipSuccess;
 }
-size_t linear_unit_bytes(int, int, int) { return (size_t)8 << 20; }  // 32 to a pass
+size_t linear_unit_bytes(int, int, int) { return bg::kLinSpace / 32; }
 size_t gemv4_room(int M, int) { return M <= 4 ? 0 : 4096; }
 hipError_t launch_gemv4(const Gemv4Args& a, hipStream_t st) {
   product = a;
@@ -388,11 +388,11 @@ static void capture() {
   CHECK(y.attend(0) == BG_OK);
 }
 
-// units of 8 MiB, 32 to a pass
+// 32 units to a pass
 static void workspace() {
   Batch x(4, 1 << 16);
   CHECK(x.set({27}, {0}) == BG_OK && x.attend(0) == BG_OK && !bg::seen.ws);
-  auto size = [&]() { return blocks.at(bg::seen.ws) >> 23; };
+  auto size = [&]() { return blocks.at(bg::seen.ws) / (bg::kLinSpace / 32); };
   CHECK(x.set({64}, {0}) == BG_OK && x.attend(0) == BG_OK && size() == 1 && bg::seen.window == 32);
   calls.clear();
   char* was = bg::seen.ws;
@@ -408,9 +408,9 @@ static void workspace() {
   Batch y;
   CHECK(y.set({64, 64}, {0, 1}) == BG_OK && y.attend(0) == BG_OK);
   was = bg::seen.ws;
-  most_memory = (size_t)20 << 20;
+  most_memory = bg::kLinSpace / 32 * 5 / 2;
   CHECK(y.set({64, 65}, {0, 1}) == BG_E_OOM);
-  most_memory = (size_t)24 << 20;                     // not twofold, but what is needed
+  most_memory = bg::kLinSpace / 32 * 3;                     // not twofold, but what is needed
   CHECK(y.attend(0) == BG_OK && bg::seen.ws == was && bg::seen.hdr->n_tokens == 128 && bg::seen.n_tokens == 128);
   CHECK(y.set({64, 65}, {0, 1}) == BG_OK && y.attend(0) == BG_OK && size() == 3);
   most_memory = ~(size_t)0;
