@@ -33,7 +33,7 @@ typedef _Float16 half8 __attribute__((ext_vector_type(8)));
 typedef float f4 __attribute__((ext_vector_type(4)));
 
 constexpr int kTop = 14;      // an operand's largest value is below 2^kTop
-constexpr int kFewScans = 256;   // workgroups of 32 value dims of the sum rule's scan
+constexpr int kFewScans[2] = {256, 128};  // workgroups of 32 value dims of the sum and the delta rule's scan
 constexpr int kBad = 1 << 20;
 constexpr int kPrepared = 768;   // workgroups that the preparation is split into, at most
 constexpr int kPad = 68;      // row stride of 64 x 64 matrices in LDS
@@ -490,7 +490,7 @@ static_assert(offsetof(ChunkMeta, ek) == 4 * M_EK && offsetof(ChunkMeta, pshift)
 // chain of three products, each with its operand's way through LDS (with one chunk's operands for all 2.9 too). No unit is
 // more than a third busy.
 template <int DK, int DV, bool DELTA, int NT>
-__global__ __launch_bounds__(512, NT == 1 ? 4 : 2) void linear_chunk_scan(LinLayer L, LinBatchView b, LinAttnArgs a, int u0, int u1) {
+__global__ __launch_bounds__(512, NT == 1 && !DELTA ? 4 : 2) void linear_chunk_scan(LinLayer L, LinBatchView b, LinAttnArgs a, int u0, int u1) {
   using W = ChunkSpace<DK>;
   constexpr int NKB = W::NKB, MT = DK / 64, kCols = 16 * NT, SLICES = DV / kCols;
   __shared__ half8 Sb[NKB * NT * 2 * 64];        // the state as an operand
@@ -990,13 +990,12 @@ hipError_t launch_t(const LinLayer& L, const LinBatchView& b, const LinAttnArgs&
     const int rep = L.v_heads / L.k_heads, parts = std::max(1, std::min(rep, kPrepared / ((u1 - u0) * L.k_heads)));
     const int each = (rep + parts - 1) / parts;
     hipLaunchKernelGGL((linear_chunk_prepare<DK, DELTA>), dim3(u1 - u0, L.k_heads * ((rep + each - 1) / each)), dim3(256), 0, st, L, b, a, u0, each);
-    // 32 value dims a workgroup; of the sum rule, whose chain is short, 16 where that still fits the GPU twice (2 x
-    // 2048 rows of 16 heads, 128 workgroups of 32: 59 us, 256 of 16: 50; more workgroups than 512 of 16, each
-    // reading the same operands, take longer). The delta rule's 192 of 32 over 8192 rows 435 us, 384 of 16 496.
-    bool narrow = false;
-    if constexpr (!DELTA) narrow = b.n_chunked * L.v_heads * (DV / 32) <= kFewScans;
-    if constexpr (!DELTA)
-      if (narrow) launch_scan<DK, DV, DELTA, 1>(L, b, a, u0, u1, st);
+    // 32 value dims a workgroup, or 16 where that still fits the GPU: of the sum rule, whose products need fewer
+    // registers, twice a CU (2 x 2048 rows of 16 heads, 128 workgroups of 32: 55 us, 256 of 16: 43), of the delta rule once
+    // (2048 rows of 16 heads, 64 workgroups of 32: 103 us, 128 of 16: 85; of two such prompts 118 and 101; of four of 1024
+    // rows 88 and 104). More workgroups, each reading the same operands, take longer.
+    const bool narrow = b.n_chunked * L.v_heads * (DV / 32) <= kFewScans[DELTA];
+    if (narrow) launch_scan<DK, DV, DELTA, 1>(L, b, a, u0, u1, st);
     if (!narrow) launch_scan<DK, DV, DELTA, 2>(L, b, a, u0, u1, st);
   }
   if (a.norm)
