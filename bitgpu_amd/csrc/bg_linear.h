@@ -17,10 +17,11 @@ constexpr int kLinChunk = 64;     // rows of a unit
 // them 50 + 7.2 and 300: they meet at 23, 34 and 34 rows), one of the sum rule 5 + 0.75 and 18.5 (64: 45 + 6.2 and 192: at
 // 18 and 24). A batch does not know the rule: a number between.
 constexpr int kLinChunkFrom = 28;
-// Most bytes of chunk operands at a time: what the scan reads should still be in the 256 MiB behind the L2s that the
-// preparation wrote it to, beside the rows themselves. 8192 rows of 48 heads (3.2 MB a chunk): 64 MiB 602 us (passes of 19
-// chunks), 80 530, 104 489, 128 488, 160 489, 208 525, 400 525.
-constexpr size_t kLinSpace = (size_t)128 << 20;
+// Most bytes of chunk operands at a time. Of one sequence: what the scan reads should still be in the 256 MiB behind the
+// L2s that the preparation wrote it to, beside the rows themselves (8192 rows of 48 heads, 3.2 MB a chunk: 64 MiB 602 us,
+// 80 530, 104 489, 128 488, 160 489, 208 525, 400 525). Of several: a pass should hold many sequences, whose scans run side
+// by side (2048 rows of 32 heads: two sequences 128 MiB 241 us, 400 181; four 408 and 374; eight 824 and 751, 800 723).
+constexpr size_t kLinCached = (size_t)128 << 20, kLinSpace = (size_t)384 << 20;
 
 // a row's decay as hi + lo: the rounding of one float would add up over the rows of a constant decay
 __device__ inline void fade_of(float g, float& hi, float& lo) {

@@ -981,7 +981,8 @@ void launch_scan(const LinLayer& L, const LinBatchView& b, const LinAttnArgs& a,
 template <int DK, int DV, bool DELTA>
 hipError_t launch_t(const LinLayer& L, const LinBatchView& b, const LinAttnArgs& a, hipStream_t st) {
   // as few passes as the workspace allows, of one size
-  const int passes = (b.n_chunk_units + b.window - 1) / b.window, step = (b.n_chunk_units + passes - 1) / passes;
+  const int most = b.n_chunked > 1 ? b.window : std::min<int>(b.window, std::max<size_t>(1, kLinCached / linear_unit_bytes(DK, L.k_heads, L.v_heads)));
+  const int passes = (b.n_chunk_units + most - 1) / most, step = (b.n_chunk_units + passes - 1) / passes;
   for (int u0 = 0; u0 < b.n_chunk_units; u0 += step) {
     const int u1 = std::min(u0 + step, b.n_chunk_units);
     // A workgroup's value heads one after the other, or, where that leaves most of the GPU idle, workgroups of their own

@@ -435,7 +435,7 @@ int32_t bg_linear_batch_destroy(bg_linear_batch* batch);
  * slots[s]. Sequences may share a source (a fork); no slot is written by two, or written by one and read by
  * another (BG_E_INVALID, the batch before stays set). A sequence without new rows touches no slot. Rows are
  * numbered sequence by sequence. Not under graph capture (BG_E_STATE). Sequences of 28 new rows and more are done in
- * chunks of 64, whose operands take a workspace of at most 128 MiB (or one chunk's): it grows here (BG_E_OOM: the batch
+ * chunks of 64, whose operands take a workspace of at most 384 MiB (or one chunk's): it grows here (BG_E_OOM: the batch
  * before stays set), never in a layer's call. */
 int32_t bg_linear_batch_set(bg_linear_batch* batch, int32_t n_seqs, const int32_t* rows, const int32_t* slots,
                             const int32_t* sources, void* stream);

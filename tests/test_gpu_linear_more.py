@@ -9,7 +9,7 @@ from tests.linear_helpers import Case, cuda
 from tests.test_gpu_proj4 import Weight, check
 
 pytestmark = pytest.mark.gpu
-SPACE = 128 << 20  # kLinSpace in bg_linear.h
+ONE, SEVERAL = 128 << 20, 384 << 20  # kLinCached and kLinSpace in bg_linear.h
 
 
 def inputs(T, Hk, Hv, seed, rule="delta"):
@@ -20,12 +20,12 @@ def inputs(T, Hk, Hv, seed, rule="delta"):
     return [q, k, r(T, Hv, 128), -torch.exp(r(T, Hv) - 3), beta]
 
 
-@pytest.mark.parametrize("rows", [[6000], [2500, 3500], [12000]])
+@pytest.mark.parametrize("rows", [[6000], [12000], [6000, 5000, 5000]])
 @pytest.mark.parametrize("rule", ["delta", "sum"])
 def test_prompts_longer_than_the_workspace(dev, rule, rows):
     """Of 16 key and 48 value heads a chunk's operands take 16 x 98,304 + 48 x 33,408 bytes: longer prompts go through
     the workspace in equal passes, with the bits of calls that are cut there, the state carried."""
-    Hk, Hv, window = 16, 48, SPACE // (16 * 98304 + 48 * 33408)
+    Hk, Hv, window = 16, 48, (ONE if len(rows) == 1 else SEVERAL) // (16 * 98304 + 48 * 33408)
     x = inputs(sum(rows), Hk, Hv, 5, rule)
     units = sum((r + 63) // 64 for r in rows)
     passes = -(-units // window)
@@ -38,11 +38,11 @@ def test_prompts_longer_than_the_workspace(dev, rule, rows):
     for a in range(0, units, step):
         mine = [[r for j, r in chunks[a:a + step] if j == i] for i in range(len(rows))]
         cut_up.append([(i, r[0], min(r[-1] + 64, rows[i])) for i, r in enumerate(mine) if r])
-    start = torch.randn(1, 2, Hv, 128, 128, device="cuda") * 0.1
+    start = torch.randn(1, 3, Hv, 128, 128, device="cuda") * 0.1
     got = []
     for calls in ([[(i, 0, r) for i, r in enumerate(rows)]], cut_up):
-        cache = E.LinearStateCache(1, Hk, Hv, 128, 128, n_slots=2, conv_width=0, state=start.clone())
-        batch = E.LinearBatch(cache, 2, sum(rows))
+        cache = E.LinearStateCache(1, Hk, Hv, 128, 128, n_slots=3, conv_width=0, state=start.clone())
+        batch = E.LinearBatch(cache, 3, sum(rows))
         out = torch.zeros(sum(rows), Hv, 128, device="cuda")
         for call in calls:
             batch.set([b - a for _, a, b in call], [i for i, _, _ in call])
