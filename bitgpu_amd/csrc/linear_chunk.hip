@@ -466,11 +466,11 @@ __global__ __launch_bounds__(256, 4) void linear_chunk_prepare(LinLayer L, LinBa
       if (wave == 0) {
         meta->kshift = ks;
         meta->whole = whole;
-        meta->ey = bad ? kBad : top_exponent(gmax) + top_exponent(DK * kmax);
+        meta->ey = bad ? kBad : (gmax > 0.0f ? top_exponent(gmax) : -200) + top_exponent(kmax) + (DK == 64 ? 6 : 7);
         meta->et = top_exponent(tsum);
         meta->ef = top_exponent(fmax_);
         meta->es = whole > 0.0f ? top_exponent(whole) : -200;
-        meta->ek = kmax > 0.0f ? top_exponent(kLinChunk * kmax) : -200;
+        meta->ek = kmax > 0.0f ? top_exponent(kmax) + 6 : -200;
       }
     }
   }
@@ -548,8 +548,8 @@ __global__ __launch_bounds__(512, NT == 1 && !DELTA ? 4 : 2) void linear_chunk_s
       const int c = 16 * nt + n;
       const uint32_t sm = max(max(smax[0][c], smax[1][c]), max(smax[2][c], smax[3][c]));
       const uint32_t vm = max(max(vmax[0][c], vmax[1][c]), max(vmax[2][c], vmax[3][c]));
-      // powers of two above them (of nothing: what adds nothing to a maximum)
-      const int es = sm ? top_exponent(__uint_as_float(sm)) : -200, ev = vm ? top_exponent(__uint_as_float(vm)) : -200;
+      // powers of two above them (a state that counts as nothing here may be held in values below the smallest float)
+      const int es = sm ? top_exponent(__uint_as_float(sm)) : -149, ev = vm ? top_exponent(__uint_as_float(vm)) : -200;
       const int ey = DELTA ? max(ev, es + cy) + 1 : ev, evp = ey + ct, ef = evp + cf, en = max(es + cs, ef + ck) + 1;
       t.y[nt] = kTop - ey;
       t.v[nt] = kTop - evp;
@@ -689,11 +689,12 @@ __global__ __launch_bounds__(512, NT == 1 && !DELTA ? 4 : 2) void linear_chunk_s
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int nt = 0; nt < NT; nt++) {
-          // Y 2^y, the product's own powers in one factor: below 2^-149 its share is nothing beside Y's bound
-          const float f = ldexpf(1.0f, sh.y[nt] - kshift - sshift[nt]);
+          // Y 2^y. Powers of two go to the values here and below: as a factor of its own one would overflow where the
+          // values that it belongs to are nothing, and zero times infinity is NaN.
+          const int e = sh.y[nt] - kshift - sshift[nt];
           float y[4];
 #pragma unroll
-          for (int r = 0; r < 4; r++) y[r] = fmaf(-(eg[r] * f), ks[nt][r], ldexpf(v[0][nt][r], sh.y[nt]));
+          for (int r = 0; r < 4; r++) y[r] = ldexpf(v[0][nt][r], sh.y[nt]) - ldexpf(eg[r] * ks[nt][r], e);
           put4(Yb, wave, nt, y[0], y[1], y[2], y[3]);
         }
         eg = load_fade(next, 0);
@@ -721,8 +722,8 @@ __global__ __launch_bounds__(512, NT == 1 && !DELTA ? 4 : 2) void linear_chunk_s
       for (int nt = 0; nt < NT; nt++) held[nt] = DELTA ? tshift + sh.y[nt] : 0;
 #pragma unroll
       for (int nt = 0; nt < NT; nt++) {
-        const float f = ldexpf(1.0f, sh.f[nt] - held[nt]);
-        put4(Fb, wave, nt, fg[0] * f * vp[nt][0], fg[1] * f * vp[nt][1], fg[2] * f * vp[nt][2], fg[3] * f * vp[nt][3]);
+        const int e = sh.f[nt] - held[nt];
+        put4(Fb, wave, nt, ldexpf(fg[0] * vp[nt][0], e), ldexpf(fg[1] * vp[nt][1], e), ldexpf(fg[2] * vp[nt][2], e), ldexpf(fg[3] * vp[nt][3], e));
       }
       fg = load_fade(next, 256);
       __syncthreads();
@@ -753,17 +754,17 @@ __global__ __launch_bounds__(512, NT == 1 && !DELTA ? 4 : 2) void linear_chunk_s
       }
 #pragma unroll
       for (int nt = 0; nt < NT; nt++) {
-        const float f = ldexpf(1.0f, sh.s_next[nt] - kshift - sh.f[nt]), w = ldexpf(whole, sh.s_next[nt] - sshift[nt]);
-        float t = 0.0f;
+        const int e = sh.s_next[nt] - kshift - sh.f[nt], w = sh.s_next[nt] - sshift[nt];
+        uint32_t t = 0;
 #pragma unroll
         for (int i = 0; i < MT; i++) {
 #pragma unroll
-          for (int r = 0; r < 4; r++) S[i][nt][r] = fmaf(f, acc[i][nt][r], w * S[i][nt][r]);
+          for (int r = 0; r < 4; r++) S[i][nt][r] = ldexpf(acc[i][nt][r], e) + ldexpf(whole * S[i][nt][r], w);
 #pragma unroll
-          for (int r = 0; r < 4; r++) t = fmaxf(t, fabsf(S[i][nt][r]));
+          for (int r = 0; r < 4; r++) t = max(t, mag(S[i][nt][r]));
         }
         sshift[nt] = sh.s_next[nt];
-        note(nt, __float_as_uint(ldexpf(t, -sshift[nt])));
+        note(nt, mag(ldexpf(__uint_as_float(t), -sshift[nt])));
 #pragma unroll
         for (int r = 0; r < 4; r++) v[0][nt][r] = moved(v[1][nt][r]);
       }
@@ -822,9 +823,8 @@ __global__ __launch_bounds__(512, NT == 1 && !DELTA ? 4 : 2) void linear_chunk_s
         }
 #pragma unroll
       for (int nt = 0; nt < NT; nt++) {
-        const float f = a.scale * ldexpf(1.0f, -pshift - vshift[nt]);
 #pragma unroll
-        for (int r = 0; r < 4; r++) acc[nt][r] = fmaf(f, acc[nt][r], o[nt][r]);
+        for (int r = 0; r < 4; r++) acc[nt][r] = fmaf(a.scale, ldexpf(acc[nt][r], -pshift - vshift[nt]), o[nt][r]);
       }
       // (A column that is left out, and with the first chunk every one, is stored past the buffer's end, which drops it:
       // with a branch there a wait for what was loaded before would not know how many stores came after, and wait for them.)
@@ -869,10 +869,9 @@ __global__ __launch_bounds__(512, NT == 1 && !DELTA ? 4 : 2) void linear_chunk_s
       // the state waves hurry from here to the third barrier: the chunk before is finished behind it
 #pragma unroll
       for (int nt = 0; nt < NT; nt++) {
-        const float f = a.scale * ldexpf(1.0f, -qshift - sshift[nt]);
 #pragma unroll
         for (int r = 0; r < 4; r++) {
-          now[nt][r] = eg[r] * (f * now[nt][r]);
+          now[nt][r] = a.scale * (eg[r] * ldexpf(now[nt][r], -qshift - sshift[nt]));
           asm volatile("" : "+v"(now[nt][r]));  // here: moved to where it is read next, it would keep eg from its next load
         }
       }
