@@ -18,10 +18,11 @@ constexpr int kLinChunk = 64;     // rows of a unit
 // 18 and 24). A batch does not know the rule: a number between.
 constexpr int kLinChunkFrom = 28;
 // Most bytes of chunk operands at a time. Of one sequence: what the scan reads should still be in the 256 MiB behind the
-// L2s that the preparation wrote it to, beside the rows themselves (8192 rows of 48 heads, 3.2 MB a chunk: 64 MiB 602 us,
-// 80 530, 104 489, 128 488, 160 489, 208 525, 400 525). Of several: a pass should hold many sequences, whose scans run side
-// by side (2048 rows of 32 heads: two sequences 128 MiB 241 us, 400 181; four 408 and 374; eight 824 and 751, 800 723).
-constexpr size_t kLinCached = (size_t)128 << 20, kLinSpace = (size_t)384 << 20;
+// L2s that the preparation wrote it to, beside the rows themselves (8192 rows of 48 heads, 4.7 MB a chunk: 64 MiB 751 us,
+// 96 706, 112 684, 128 651, 144 651, 160 626, 176 628, 208 684, 256 684). Of several: a pass should hold many sequences,
+// whose scans run side by side (2048 rows of 32 heads: two sequences 128 MiB 241 us, 400 181; four 408 and 374; eight 824
+// and 751, 800 723; with two f16 parts an operand).
+constexpr size_t kLinCached = (size_t)160 << 20, kLinSpace = (size_t)384 << 20;
 
 // a row's decay as hi + lo: the rounding of one float would add up over the rows of a constant decay
 __device__ inline void fade_of(float g, float& hi, float& lo) {

@@ -7,16 +7,15 @@
 // ("sum": V' = V). Everything that does not need S is one launch over all chunks (linear_chunk_prepare); the
 // scan (linear_chunk_scan) then walks a sequence's chunks with 32 value dims of a head a workgroup.
 //
-// Precision: products run on the f16 matrix cores with each f32 operand as two f16 parts, x = hi + lo, three
-// products of four (22 bits of the larger operands; what is left out is 2^-22 of a product), summed in f32.
-// Powers of two bring an operand's largest value to 2^14, so values down to 2^-16 of it keep all 22 bits: one
-// for a tile of K, Q, T, P; one for a value dim of S, Y = V - e^G K S and V', whose columns are independent and
-// may be of any size. Those follow from bounds (the column's largest |S| and |V|, K's largest value, T's largest
-// row sum), which may be 2^16 too large before that costs a bit. The decays' sums are taken in f64: their
-// differences over a chunk would lose 2^-24 of the sums. T is found in f32: its diagonal blocks of 16 rows by
+// Precision: products run on the bf16 matrix cores with each f32 operand as three bf16 parts, which hold all of its 24
+// bits and, down to 2^-109, its exponents: six products of nine, the others being below 2^-23 of a product, summed
+// in f32. Every row and value dim is as good as an f32 sum makes it, whatever its neighbours' sizes. (Two f16 parts
+// and three products are faster, prompt of 8192 rows 490 us instead of 617, but want one power of two for all rows of
+// a value dim: a large state or value that the rows behind it have forgotten leaves those with as many bits fewer.) The decays' sums are taken in
+// f64: their differences over a chunk would lose 2^-24 of the sums. T is found in f32: its diagonal blocks of 16 rows by
 // substitution, the others from them with f32 matrix products.
 //
-// A column whose V or S is not finite, or so large that a bound would overflow, and every column of a chunk
+// A column whose V or S is not finite, or so large that a sum on the way could overflow, and every column of a chunk
 // whose K, Q, decays or strengths are not finite, is done again row by row: zero times infinity would reach
 // rows before it. Its other columns keep their results (a matrix product's columns do not mix).
 #include <algorithm>
@@ -29,98 +28,95 @@ namespace bg {
 
 namespace {
 
-typedef _Float16 half8 __attribute__((ext_vector_type(8)));
+typedef __bf16 part8 __attribute__((ext_vector_type(8)));
 typedef float f4 __attribute__((ext_vector_type(4)));
 
-constexpr int kTop = 14;      // an operand's largest value is below 2^kTop
+constexpr int kParts = 3;     // of an operand: largest first
 constexpr int kFewScans[2] = {256, 128};  // workgroups of 32 value dims of the sum and the delta rule's scan
-constexpr int kBad = 1 << 20;
 constexpr int kPrepared = 768;   // workgroups that the preparation is split into, at most
 constexpr int kPad = 68;      // row stride of 64 x 64 matrices in LDS
 constexpr double kLowest = -1e4;  // of a log decay: e^g is 0 in f32 from -104 on
 
-// What the scan needs of a chunk and head beside its operands. Operands are held times 2^shift.
+// What the scan needs of a chunk and head beside its operands: e^G_n, and the size (as bits) from which on a value of S
+// or V could overflow a sum on its way; 0 where something is not finite.
 struct ChunkMeta {
-  int kshift, qshift[4], tshift[4], pshift[4];
-  float whole;                 // e^G_n
-  // What the scan's bounds are made of, as powers of two: y of gmax DK kmax (of a state's share of Y), t of T's
-  // largest row sum, f of the largest e^(G_n - G_i), s of e^G_n, k of 64 kmax. bad in y: something is not finite
-  int ey, et, ef, es, ek;
-  int pad[13];
+  float whole;
+  uint32_t limit;
+  int pad[30];
 };
 static_assert(sizeof(ChunkMeta) == 128, "meta");
 
-// Operands of a chunk in the order the matrix instructions take them: [tile of 16 rows][32 of k][hi, lo][lane], a
+// Operands of a chunk in the order the matrix instructions take them: [tile of 16 rows][32 of k][part][lane], a
 // lane's k values being 16 (j / 4) + 4 g + j % 4 of the 32 for j = 0..7 (g = lane / 16), so that a product's
 // result (rows 4 g + r of a tile) is the next one's operand without leaving its lane.
 template <int DK>
 struct ChunkSpace {
   static constexpr int NKB = DK / 32;
-  static constexpr int K = 0, Q = K + 4 * NKB * 2 * 64, KT = Q + 4 * NKB * 2 * 64, PER_K = KT + (DK / 16) * 2 * 2 * 64;  // in half8
-  static constexpr int T = 0, P = T + 4 * 2 * 2 * 64, G = P + 4 * 2 * 2 * 64, META = G + 128 / 4, PER_H = META + 8;       // in 16 bytes
+  static constexpr int K = 0, Q = K + 4 * NKB * kParts * 64, KT = Q + 4 * NKB * kParts * 64, PER_K = KT + (DK / 16) * 2 * kParts * 64;  // in part8
+  static constexpr int T = 0, P = T + 4 * 2 * kParts * 64, G = P + 4 * 2 * kParts * 64, META = G + 128 / 4, PER_H = META + 8;          // in 16 bytes
 };
 
 // The workspace, as memory that is known to be the device's: through a pointer of no known kind its loads would
 // count as LDS accesses too, and every barrier wait for them.
 #define BG_GLOBAL __attribute__((address_space(1)))
-typedef BG_GLOBAL half8 ghalf8;
-__device__ inline ghalf8* workspace(const LinBatchView& b) { return (ghalf8*)(b.ws ? b.ws : b.hdr->ws); }
+typedef BG_GLOBAL part8 gpart8;
+__device__ inline gpart8* workspace(const LinBatchView& b) { return (gpart8*)(b.ws ? b.ws : b.hdr->ws); }
 
 __device__ inline int top_exponent(float x) { return __builtin_amdgcn_frexp_expf(x); }  // x < 2^e; 0 for 0
-__device__ inline int shift_for(float most) { return kTop - top_exponent(most); }
 __device__ inline uint32_t mag(float x) { return __float_as_uint(x) & 0x7fffffffu; }
 constexpr uint32_t kInf = 0x7f800000u;
 
-// x less the low (high) half of h: one mixed-precision fma, exact
-__device__ inline float less_lo(float x, uint32_t h) {
-  float r;
-  asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel_hi:[1,0,0]" : "=v"(r) : "v"(h), "v"(x));
-  return r;
+// two values as bf16, rounded to nearest: the first in the low half
+__device__ inline uint32_t round2(float a, float b) {
+  typedef float f2 __attribute__((ext_vector_type(2)));
+  typedef __bf16 b2 __attribute__((ext_vector_type(2)));
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector((f2{a, b}), b2));
 }
-__device__ inline float less_hi(float x, uint32_t h) {
-  float r;
-  asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(r) : "v"(h), "v"(x));
-  return r;
-}
-// a, b as hi and lo f16 parts, each rounded to nearest
-__device__ inline void split2(float a, float b, uint32_t& hi, uint32_t& lo) {
-  typedef _Float16 half2_t __attribute__((ext_vector_type(2)));
-  const half2_t h = {(_Float16)a, (_Float16)b};
-  hi = __builtin_bit_cast(uint32_t, h);
-  const half2_t l = {(_Float16)less_lo(a, hi), (_Float16)less_hi(b, hi)};
-  lo = __builtin_bit_cast(uint32_t, l);
+__device__ inline void split2(float a, float b, uint32_t (&to)[kParts]) {
+#pragma unroll
+  for (int p = 0; p < kParts; p++) {
+    to[p] = round2(a, b);
+    a -= __uint_as_float(to[p] << 16);
+    b -= __uint_as_float(to[p] & 0xffff0000u);
+  }
 }
 typedef uint32_t u2 __attribute__((ext_vector_type(2)));
 typedef uint32_t u4 __attribute__((ext_vector_type(4)));
-__device__ inline void split4(float a, float b, float c, float d, u2& hi, u2& lo) {
-  uint32_t h[2], l[2];
-  split2(a, b, h[0], l[0]);
-  split2(c, d, h[1], l[1]);
-  hi = u2{h[0], h[1]};
-  lo = u2{l[0], l[1]};
-}
-__device__ inline void split8(const float (&x)[8], half8& hi, half8& lo) {
-  uint32_t h[4], l[4];
+__device__ inline void split4(float a, float b, float c, float d, u2 (&to)[kParts]) {
+  uint32_t x[kParts], y[kParts];
+  split2(a, b, x);
+  split2(c, d, y);
 #pragma unroll
-  for (int i = 0; i < 4; i++) split2(x[2 * i], x[2 * i + 1], h[i], l[i]);
-  hi = __builtin_bit_cast(half8, u4{h[0], h[1], h[2], h[3]});
-  lo = __builtin_bit_cast(half8, u4{l[0], l[1], l[2], l[3]});
+  for (int p = 0; p < kParts; p++) to[p] = u2{x[p], y[p]};
 }
-// c += (ah + al)(bh + bl) less al bl
-__device__ inline f4 product3(half8 ah, half8 al, half8 bh, half8 bl, f4 c) {
-  c = __builtin_amdgcn_mfma_f32_16x16x32_f16(al, bh, c, 0, 0, 0);
-  c = __builtin_amdgcn_mfma_f32_16x16x32_f16(ah, bl, c, 0, 0, 0);
-  return __builtin_amdgcn_mfma_f32_16x16x32_f16(ah, bh, c, 0, 0, 0);
+__device__ inline void split8(const float (&x)[8], part8 (&to)[kParts]) {
+  uint32_t h[4][kParts];
+#pragma unroll
+  for (int i = 0; i < 4; i++) split2(x[2 * i], x[2 * i + 1], h[i]);
+#pragma unroll
+  for (int p = 0; p < kParts; p++) to[p] = __builtin_bit_cast(part8, u4{h[0][p], h[1][p], h[2][p], h[3][p]});
 }
-// the same for N tiles of columns, their chains side by side
+// c += a b for N tiles of columns, their chains side by side, the smallest products first
 template <int N>
-__device__ inline void products3(half8 ah, half8 al, const half8 (&bh)[N], const half8 (&bl)[N], f4 (&c)[N]) {
+__device__ inline void products(const part8 (&a)[kParts], const part8 (&b)[N][kParts], f4 (&c)[N]) {
 #pragma unroll
-  for (int i = 0; i < N; i++) c[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(al, bh[i], c[i], 0, 0, 0);
+  for (int both = 2; both >= 0; both--)
 #pragma unroll
-  for (int i = 0; i < N; i++) c[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ah, bl[i], c[i], 0, 0, 0);
+    for (int p = both; p >= 0; p--)
 #pragma unroll
-  for (int i = 0; i < N; i++) c[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ah, bh[i], c[i], 0, 0, 0);
+      for (int i = 0; i < N; i++) c[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[p], b[i][both - p], c[i], 0, 0, 0);
+}
+__device__ inline f4 product(const part8 (&a)[kParts], const part8 (&b)[kParts], f4 c) {
+#pragma unroll
+  for (int both = 2; both >= 0; both--)
+#pragma unroll
+    for (int p = both; p >= 0; p--) c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[p], b[both - p], c, 0, 0, 0);
+  return c;
+}
+// e^x, x in 64 bits: the float next to x alone would leave 2^-25 of x
+__device__ inline float exp_of(double x) {
+  const float h = (float)x, e = expf(h);
+  return fmaf(e, (float)(x - (double)h), e);
 }
 // over the four lane groups that hold a column's rows (or a row's k values)
 __device__ inline uint32_t groups_max(uint32_t v) {
@@ -146,8 +142,8 @@ __device__ inline __amdgpu_buffer_rsrc_t buffer(const void* p, uint32_t bytes) {
   const uint64_t u = (uint64_t)(uint32_t)uniform((int)(uint32_t)a) | (uint64_t)(uint32_t)uniform((int)(uint32_t)(a >> 32)) << 32;
   return __builtin_amdgcn_make_buffer_rsrc((void*)u, (short)0, (int)bytes, 0x00020000);
 }
-__device__ inline half8 load8(__amdgpu_buffer_rsrc_t r, int offset, int at) {  // `at` half8s behind byte `offset`
-  return __builtin_bit_cast(half8, __builtin_amdgcn_raw_buffer_load_b128(r, offset, 16 * at, 0));
+__device__ inline part8 load8(__amdgpu_buffer_rsrc_t r, int offset, int at) {  // `at` part8s behind byte `offset`
+  return __builtin_bit_cast(part8, __builtin_amdgcn_raw_buffer_load_b128(r, offset, 16 * at, 0));
 }
 // x, copied here: a copy that the compiler puts at its next use would wait there for what x is loaded with anew
 __device__ inline float moved(float x) {
@@ -164,17 +160,17 @@ __device__ inline int afresh(int x) {
 // One chunk and key head, and `each` of its value heads: blockIdx.x a unit from u0 on, blockIdx.y the key head and which of
 // its value heads.
 template <int DK, bool DELTA>
-__global__ __launch_bounds__(256, 4) void linear_chunk_prepare(LinLayer L, LinBatchView b, LinAttnArgs a, int u0, int each) {
+__global__ __launch_bounds__(256, 3) void linear_chunk_prepare(LinLayer L, LinBatchView b, LinAttnArgs a, int u0, int each) {
   using W = ChunkSpace<DK>;
   constexpr int NKB = W::NKB;
-  constexpr int kMat = 64 * kPad * 4, kFrag = 4 * NKB * 2 * 64 * 16;
+  constexpr int kMat = 64 * kPad * 4, kFrag = 4 * NKB * kParts * 64 * 16;
   __shared__ __align__(16) char mem[2 * kMat > kFrag ? 2 * kMat : kFrag];
   __shared__ double gsums[4][64];            // of four value heads at a time, a wave each
   __shared__ float strengths[4][64], gtop[4][3];
   __shared__ int gbad[4];
   __shared__ uint32_t most[4], bits[4];
   __shared__ float sums[4];
-  half8* frag = (half8*)mem;                 // K, while products with it run
+  part8* frag = (part8*)mem;                 // K, while products with it run
   float* Am = (float*)mem;                   // then A
   float* Tm = (float*)(mem + kMat);          // P, then T
   const LinUnit u = b.units[u0 + blockIdx.x];
@@ -182,13 +178,12 @@ __global__ __launch_bounds__(256, 4) void linear_chunk_prepare(LinLayer L, LinBa
   const int rep = L.v_heads / L.k_heads, parts = (rep + each - 1) / each, kh = blockIdx.y / parts;
   const int i0 = blockIdx.y % parts * each, i1 = min(i0 + each, rep);
   const int wave = uniform(threadIdx.x >> 6), lane_ = threadIdx.x & 63;
-  ghalf8* wk = workspace(b) + (size_t)blockIdx.x * (L.k_heads * W::PER_K + L.v_heads * W::PER_H);
-  ghalf8* wh0 = wk + (size_t)L.k_heads * W::PER_K;
+  gpart8* wk = workspace(b) + (size_t)blockIdx.x * (L.k_heads * W::PER_K + L.v_heads * W::PER_H);
+  gpart8* wh0 = wk + (size_t)L.k_heads * W::PER_K;
   wk += (size_t)kh * W::PER_K;
 
   f4 kk[4], qk[4];
-  float kmax;
-  int ks, qs;
+  float kmax, qmax;
   bool bad_k;
   {
   const int lane = lane_, m = lane & 15, g = lane >> 4;
@@ -217,73 +212,66 @@ __global__ __launch_bounds__(256, 4) void linear_chunk_prepare(LinLayer L, LinBa
     most[wave] = km;
     bits[wave] = qm;
   }
+  const int mine = wave * NKB * kParts * 64 + lane;  // this wave's operands
+#pragma unroll
+  for (int kb = 0; kb < NKB; kb++) {
+    part8 x[kParts];
+    split8(kx[kb], x);
+#pragma unroll
+    for (int p = 0; p < kParts; p++) {
+      frag[mine + (kb * kParts + p) * 64] = x[p];
+      if constexpr (DELTA)
+        if (i0 == 0) wk[W::K + mine + (kb * kParts + p) * 64] = x[p];
+    }
+  }
   __syncthreads();
   const uint32_t kall = max(max(most[0], most[1]), max(most[2], most[3]));
   const uint32_t qall = max(max(bits[0], bits[1]), max(bits[2], bits[3]));
   bad_k = kall >= kInf || qall >= kInf;
   kmax = __uint_as_float(kall);
-  ks = shift_for(kmax);
-  qs = shift_for(__uint_as_float(qm));
-  half8 qh[NKB], ql[NKB], kh8[NKB], kl8[NKB];
-#pragma unroll
-  for (int kb = 0; kb < NKB; kb++) {
-#pragma unroll
-    for (int e = 0; e < 8; e++) {
-      kx[kb][e] = ldexpf(kx[kb][e], ks);
-      qx[kb][e] = ldexpf(qx[kb][e], qs);
-    }
-    split8(kx[kb], kh8[kb], kl8[kb]);
-    split8(qx[kb], qh[kb], ql[kb]);
-    const int i = (wave * NKB + kb) * 2 * 64 + lane;
-    frag[i] = kh8[kb];
-    frag[i + 64] = kl8[kb];
-    if (i0 == 0) {
-      if constexpr (DELTA) {
-        wk[W::K + i] = kh8[kb];
-        wk[W::K + i + 64] = kl8[kb];
-      }
-      wk[W::Q + i] = qh[kb];
-      wk[W::Q + i + 64] = ql[kb];
-    }
-  }
-  __syncthreads();
+  qmax = __uint_as_float(qall);
   // K^T: this wave's tiles of 16 key dims
   if (i0 == 0) {
-    const _Float16* e = (const _Float16*)frag;
+    const __bf16* e = (const __bf16*)frag;
 #pragma unroll
     for (int i = 0; i < DK / 64; i++) {
       const int td = wave * (DK / 64) + i;
 #pragma unroll
       for (int kb2 = 0; kb2 < 2; kb2++)
 #pragma unroll
-        for (int hl = 0; hl < 2; hl++) {
+        for (int p = 0; p < kParts; p++) {
           asm volatile("" ::: "memory");
-          half8 x;
+          part8 x;
 #pragma unroll
           for (int j = 0; j < 8; j++) {
             const int tile = 2 * kb2 + (j >> 2), from = 4 * g + (j & 3) + 16 * (m >> 2);
-            x[j] = e[(((tile * NKB + (td >> 1)) * 2 + hl) * 64 + from) * 8 + 4 * (td & 1) + (m & 3)];
+            x[j] = e[(((tile * NKB + (td >> 1)) * kParts + p) * 64 + from) * 8 + 4 * (td & 1) + (m & 3)];
           }
-          wk[W::KT + ((td * 2 + kb2) * 2 + hl) * 64 + lane] = x;
+          wk[W::KT + ((td * 2 + kb2) * kParts + p) * 64 + lane] = x;
         }
     }
   }
-  // row tile `wave` of K K^T and Q K^T
+  // row tile `wave` of K K^T and Q K^T (its operands made or read where they are used: kept through the loop they spilled)
 #pragma unroll
-  for (int ct = 0; ct < 4; ct++) {
-    kk[ct] = qk[ct] = f4{0, 0, 0, 0};
-    if (ct > wave) continue;
-    asm volatile("" ::: "memory");  // (one tile's operands at a time in registers)
+  for (int ct = 0; ct < 4; ct++) kk[ct] = qk[ct] = f4{0, 0, 0, 0};
 #pragma unroll
-    for (int kb = 0; kb < NKB; kb++) {
-      const half8 bh = frag[((ct * NKB + kb) * 2 + 0) * 64 + lane], bl = frag[((ct * NKB + kb) * 2 + 1) * 64 + lane];
-      if constexpr (DELTA) kk[ct] = product3(kh8[kb], kl8[kb], bh, bl, kk[ct]);
-      qk[ct] = product3(qh[kb], ql[kb], bh, bl, qk[ct]);
+  for (int kb = 0; kb < NKB; kb++) {
+    asm volatile("" ::: "memory");
+    part8 kp[kParts], qp[kParts];
+    split8(qx[kb], qp);
+#pragma unroll
+    for (int p = 0; p < kParts; p++) {
+      kp[p] = frag[mine + (kb * kParts + p) * 64];
+      if (i0 == 0) wk[W::Q + mine + (kb * kParts + p) * 64] = qp[p];
     }
 #pragma unroll
-    for (int r = 0; r < 4; r++) {
-      kk[ct][r] = ldexpf(kk[ct][r], -2 * ks);
-      qk[ct][r] = ldexpf(qk[ct][r], -ks - qs);
+    for (int ct = 0; ct < 4; ct++) {
+      if (ct > wave) continue;
+      part8 x[kParts];
+#pragma unroll
+      for (int p = 0; p < kParts; p++) x[p] = frag[((ct * NKB + kb) * kParts + p) * 64 + lane];
+      if constexpr (DELTA) kk[ct] = product(kp, x, kk[ct]);
+      qk[ct] = product(qp, x, qk[ct]);
     }
   }
   }
@@ -291,7 +279,7 @@ __global__ __launch_bounds__(256, 4) void linear_chunk_prepare(LinLayer L, LinBa
 #pragma unroll 1
   for (int i = i0; i < i1; i++) {
     const int h = kh * rep + i;
-    ghalf8* wh = wh0 + (size_t)h * W::PER_H;
+    gpart8* wh = wh0 + (size_t)h * W::PER_H;
     const auto rh = buffer((const void*)wh, 16 * W::PER_H);
     const int lane = afresh(lane_), m = lane & 15, g = lane >> 4, row = 16 * wave + m;
     __syncthreads();  // the frag reads, or the head before
@@ -311,7 +299,7 @@ __global__ __launch_bounds__(256, 4) void linear_chunk_prepare(LinLayer L, LinBa
         const float be = DELTA ? (on ? a.beta[rr * L.v_heads + hh] : 0.0f) : 1.0f;
         gsums[wave][lane] = s;
         strengths[wave][lane] = be;
-        const float eg = expf((float)s), fg = expf((float)(end - s));
+        const float eg = exp_of(s), fg = exp_of(end - s);
         BG_GLOBAL float* gg = (BG_GLOBAL float*)(wh + (size_t)wave * W::PER_H + W::G);
         gg[lane] = eg;
         gg[64 + lane] = on ? fg : 0.0f;
@@ -320,7 +308,7 @@ __global__ __launch_bounds__(256, 4) void linear_chunk_prepare(LinLayer L, LinBa
         if (lane == 0) {
           gtop[wave][0] = gm;
           gtop[wave][1] = fm;
-          gtop[wave][2] = expf((float)end);
+          gtop[wave][2] = exp_of(end);
           gbad[wave] = odd;
         }
       }
@@ -348,13 +336,12 @@ __global__ __launch_bounds__(256, 4) void linear_chunk_prepare(LinLayer L, LinBa
       }
     }
     pm = wave_umax(pm);
-    const int ps = shift_for(__uint_as_float(pm));
     if (lane == 0) bits[wave] = pm;
     // P's operands: rows written by this wave itself
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
     __builtin_amdgcn_wave_barrier();
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-    auto operand = [&](const float* M, int kb, bool strong, float& sum, uint32_t& big, float (&x)[8]) {
+    auto operand = [&](const float* M, int kb, bool strong, float& sum, float (&x)[8]) {
 #pragma unroll
       for (int half = 0; half < 2; half++) {
         const int ct = 2 * kb + half;
@@ -365,28 +352,24 @@ __global__ __launch_bounds__(256, 4) void linear_chunk_prepare(LinLayer L, LinBa
           const float y = ct <= wave && strong ? v[e] * strength[16 * ct + 4 * g + e] : v[e];
           x[4 * half + e] = y;
           sum += fabsf(y);
-          big = max(big, mag(y));
         }
       }
     };
-    auto put = [&](int base, int kb, int shift, float (&x)[8]) {
-      half8 hi, lo;
+    auto put = [&](int base, int kb, const float (&x)[8]) {
+      part8 parts[kParts];
+      split8(x, parts);
+      const int at = 16 * lane + 2 * kParts * 1024 * wave;
 #pragma unroll
-      for (int e = 0; e < 8; e++) x[e] = ldexpf(x[e], shift);
-      split8(x, hi, lo);
-      const int at = 16 * lane + 4096 * wave;
-      __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u4, hi), rh, at, 16 * (base + kb * 128), 0);
-      __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u4, lo), rh, at, 16 * (base + kb * 128 + 64), 0);
+      for (int p = 0; p < kParts; p++)
+        __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u4, parts[p]), rh, at, 16 * (base + (kb * kParts + p) * 64), 0);
     };
 #pragma unroll
     for (int kb = 0; kb < 2; kb++) {
       float x[8], none = 0;
-      uint32_t nil = 0;
       if (2 * kb > wave) continue;
-      operand(Tm, kb, false, none, nil, x);
-      put(W::P, kb, ps, x);
+      operand(Tm, kb, false, none, x);
+      put(W::P, kb, x);
     }
-    int ts = 0;
     float tsum = 1.0f;
     if constexpr (DELTA) {
       __syncthreads();  // P is read; A is there
@@ -439,16 +422,14 @@ __global__ __launch_bounds__(256, 4) void linear_chunk_prepare(LinLayer L, LinBa
         }
       }
       __syncthreads();
-      float x[2][8], sum = 0.0f;
-      uint32_t big = 0;
+      float sum = 0.0f;
 #pragma unroll
-      for (int kb = 0; kb < 2; kb++)
-        if (2 * kb <= wave) operand(Tm, kb, true, sum, big, x[kb]);
-      big = wave_umax(big);
-      ts = shift_for(__uint_as_float(big));
-#pragma unroll
-      for (int kb = 0; kb < 2; kb++)
-        if (2 * kb <= wave) put(W::T, kb, ts, x[kb]);
+      for (int kb = 0; kb < 2; kb++) {
+        float x[8];
+        if (2 * kb > wave) continue;
+        operand(Tm, kb, true, sum, x);
+        put(W::T, kb, x);
+      }
       sum = __uint_as_float(wave_umax(mag(groups_sum(sum))));  // (a NaN counts as the largest)
       if (lane == 0) sums[wave] = sum;
       __syncthreads();
@@ -458,26 +439,19 @@ __global__ __launch_bounds__(256, 4) void linear_chunk_prepare(LinLayer L, LinBa
       __syncthreads();
     }
     for (int w = 0; w < 4; w++) bad = bad || !(__uint_as_float(bits[w]) < 0x1p60f);
-    BG_GLOBAL ChunkMeta* meta = (BG_GLOBAL ChunkMeta*)(wh + W::META);
-    if (lane == 0) {
-      meta->qshift[wave] = qs;
-      meta->tshift[wave] = ts;
-      meta->pshift[wave] = ps;
-      if (wave == 0) {
-        meta->kshift = ks;
-        meta->whole = whole;
-        meta->ey = bad ? kBad : (gmax > 0.0f ? top_exponent(gmax) : -200) + top_exponent(kmax) + (DK == 64 ? 6 : 7);
-        meta->et = top_exponent(tsum);
-        meta->ef = top_exponent(fmax_);
-        meta->es = whole > 0.0f ? top_exponent(whole) : -200;
-        meta->ek = kmax > 0.0f ? top_exponent(kmax) + 6 : -200;
-      }
+    if (threadIdx.x == 0) {
+      // what a value of S or V may grow by: through e^G Q S; through Y, T and e^(G_n - G) to K^T V' or P V'
+      const float pmax = __uint_as_float(max(max(bits[0], bits[1]), max(bits[2], bits[3])));
+      constexpr int kSum = DK == 64 ? 6 : 7;
+      const int eg = max(0, top_exponent(gmax)), ek = top_exponent(kmax), y = max(0, kSum + ek + eg) + 1;
+      const int v = y + max(0, top_exponent(tsum)) + max(0, top_exponent(fmax_));
+      const int grow = max(max(eg, kSum + top_exponent(qmax) + eg), v + max(0, 6 + max(ek, top_exponent(pmax)))) + 1;
+      BG_GLOBAL ChunkMeta* meta = (BG_GLOBAL ChunkMeta*)(wh + W::META);
+      meta->whole = whole;
+      meta->limit = bad || grow > 220 ? 0 : __float_as_uint(ldexpf(1.0f, 126 - grow));
     }
   }
 }
-
-enum { M_KSHIFT = 0, M_QSHIFT = 1, M_TSHIFT = 5, M_PSHIFT = 9, M_WHOLE = 13, M_EY, M_ET, M_EF, M_ES, M_EK };
-static_assert(offsetof(ChunkMeta, ek) == 4 * M_EK && offsetof(ChunkMeta, pshift) == 4 * M_PSHIFT, "meta words");
 
 // A sequence's chunks from u0 up to u1 (its window of the workspace) for 16 NT value dims of a head. Four waves carry
 // the state: wave w has rows 16 w .. of K S, Y and V' and a quarter of the key dims of S, all in registers; what
@@ -485,17 +459,18 @@ static_assert(offsetof(ChunkMeta, ek) == 4 * M_EK && offsetof(ChunkMeta, pshift)
 // make the output from what lies in LDS between those barriers. The next chunk's operands are loaded into the
 // registers of this one's as soon as their last product has been issued: by buffer loads, whose one lane
 // offset and scalar rest leave the registers to the operands. (A register too many costs a wait for everything
-// in flight when it is read back: with 64-bit addresses in vector registers 14 us a chunk, with the row offsets
-// of V and the output kept through the loop 6.8, without 4.0; one set of waves for all of it.) 2.9 us a chunk: the
-// chain of three products, each with its operand's way through LDS (with one chunk's operands for all 2.9 too). No unit is
-// more than a third busy.
+// in flight when it is read back; with two f16 parts an operand: 64-bit addresses in vector registers 14 us a chunk, the
+// row offsets of V and the output kept through the loop 6.8, without 4.0, two sets of waves 2.9.) 4.1 us a chunk: the
+// chain of three products of six matrix instructions a tile and step, each with its operand's way through LDS. By
+// count the matrix cores and LDS are a third busy.
 template <int DK, int DV, bool DELTA, int NT>
 __global__ __launch_bounds__(512, NT == 1 && !DELTA ? 4 : 2) void linear_chunk_scan(LinLayer L, LinBatchView b, LinAttnArgs a, int u0, int u1) {
   using W = ChunkSpace<DK>;
   constexpr int NKB = W::NKB, MT = DK / 64, kCols = 16 * NT, SLICES = DV / kCols;
-  __shared__ half8 Sb[NKB * NT * 2 * 64];        // the state as an operand
-  __shared__ half8 Yb[2 * NT * 2 * 64], Vb[2][2 * NT * 2 * 64], Fb[2 * NT * 2 * 64];  // Y, V' (of this chunk and the one before), e^(G_n - G) V'
-  __shared__ uint32_t smax[4][kCols], vmax[4][kCols];
+  constexpr int kRows = 2 * NT * kParts * 64;    // of an operand whose k are the chunk's rows
+  __shared__ part8 Sb[NKB * NT * kParts * 64];   // the state as an operand
+  __shared__ part8 Yb[kRows], Vb[2][kRows], Fb[kRows];  // Y, V' (of this chunk and the one before), e^(G_n - G) V'
+  __shared__ uint32_t sout[4], vout[4];          // the waves' columns with a value of S, of V past the chunk's limit
   __shared__ float plain[kCols][DK + 4];        // columns that are done row by row: the state before
   __shared__ int slow_from[kCols];              // this chunk of the sequence
   // a key head's value heads and slices, which read the same operands, run on one XCD
@@ -512,9 +487,9 @@ __global__ __launch_bounds__(512, NT == 1 && !DELTA ? 4 : 2) void linear_chunk_s
   const int role = uniform(threadIdx.x >> 8), wave = uniform((threadIdx.x >> 6) & 3);
   const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
   const size_t per_unit = (size_t)L.k_heads * W::PER_K + (size_t)L.v_heads * W::PER_H;
-  const half8* ws = (const half8*)(b.ws ? b.ws : b.hdr->ws);
+  const part8* ws = (const part8*)(b.ws ? b.ws : b.hdr->ws);
 
-  const int at_k = 16 * lane + wave * (NKB * 2 * 64 * 16), at_t = 16 * lane + wave * (2 * 2 * 64 * 16);
+  const int at_k = 16 * lane + wave * (NKB * kParts * 64 * 16), at_t = 16 * lane + wave * (2 * kParts * 64 * 16);
   static_assert(NKB == 2 * MT, "the operands of a wave's rows and of its key dims lie alike");
   auto keys = [&](int u) { return buffer(ws + (size_t)(u - u0) * per_unit + (size_t)kh * W::PER_K, 16 * W::PER_K); };
   auto head = [&](int u) {
@@ -526,45 +501,24 @@ __global__ __launch_bounds__(512, NT == 1 && !DELTA ? 4 : 2) void linear_chunk_s
     const int r = kLinChunk * (u - unit0);
     return buffer(p + ((size_t)(row0 + r) * L.v_heads + h) * DV + col0, (min(kLinChunk, rows - r) - 1) * vrow + 4 * kCols);
   };
-  int meta;  // lane i: word i of the chunk's ChunkMeta
-  auto load_meta = [&](int u) { meta = __builtin_amdgcn_raw_buffer_load_b32(head(u), 4 * (afresh(lane) & 31), 16 * W::META, 0); };
+  u2 meta;  // the chunk's ChunkMeta, in every lane
+  auto load_meta = [&](int u) { meta = __builtin_bit_cast(u2, __builtin_amdgcn_raw_buffer_load_b64(head(u), 0, 16 * W::META, 0)); };
   auto load_fade = [&](int u, int at) {  // this wave's rows' e^G (at 0) or e^(G_n - G) (256)
     return __builtin_bit_cast(f4, __builtin_amdgcn_raw_buffer_load_b128(head(u), 64 * wave + 16 * (afresh(lane) >> 4), 16 * W::G + at, 0));
   };
-  auto word = [&](int i) { return __builtin_amdgcn_readlane(meta, i); };
-  auto fword = [&](int i) { return __builtin_bit_cast(float, __builtin_amdgcn_readlane(meta, i)); };
-  // The powers of two of a chunk's columns (this lane's two), from what is noted of S and V; next_m bounds the
-  // next state. `out`: columns that are not for these products.
-  struct Shifts {
-    int y[NT], v[NT], f[NT], s_next[NT];
-    uint32_t out;
-  };
-  auto shifts = [&]() {
-    Shifts t;
-    t.out = 0;
-    const int cy = word(M_EY), ct = word(M_ET), cf = word(M_EF), cs = word(M_ES), ck = word(M_EK);
+  // bit c: column c, of which a lane's largest value (as bits) is in top[c / 16], is not for the chunk's products
+  auto marked = [&](const uint32_t (&top)[NT]) {
+    const uint32_t limit = uniform((int)meta[1]);
+    uint32_t m = 0;
 #pragma unroll
     for (int nt = 0; nt < NT; nt++) {
-      const int c = 16 * nt + n;
-      const uint32_t sm = max(max(smax[0][c], smax[1][c]), max(smax[2][c], smax[3][c]));
-      const uint32_t vm = max(max(vmax[0][c], vmax[1][c]), max(vmax[2][c], vmax[3][c]));
-      // powers of two above them (a state that counts as nothing here may be held in values below the smallest float)
-      const int es = sm ? top_exponent(__uint_as_float(sm)) : -149, ev = vm ? top_exponent(__uint_as_float(vm)) : -200;
-      const int ey = DELTA ? max(ev, es + cy) + 1 : ev, evp = ey + ct, ef = evp + cf, en = max(es + cs, ef + ck) + 1;
-      t.y[nt] = kTop - ey;
-      t.v[nt] = kTop - evp;
-      t.f[nt] = kTop - ef;
-      t.s_next[nt] = kTop - en;
-      const bool out = max(sm, vm) >= kInf || max(max(es, ey), max(evp, en)) >= 120 || cy >= kBad / 2;
-      t.out |= (uint32_t)(__ballot(out) & 0xffffu) << (16 * nt);
+      const uint64_t b = __ballot(top[nt] >= limit);
+      const uint32_t w = (uint32_t)b | (uint32_t)(b >> 32);
+      m |= ((w | w >> 16) & 0xffffu) << (16 * nt);
     }
-    t.out = uniform(t.out);
-    return t;
+    return m;
   };
-  auto first_shift = [&](int nt) {
-    const int c = 16 * nt + n;
-    return shift_for(__uint_as_float(max(max(smax[0][c], smax[1][c]), max(smax[2][c], smax[3][c]))));
-  };
+  auto marks = [&]() { return (uint32_t)uniform((int)(sout[0] | sout[1] | sout[2] | sout[3] | vout[0] | vout[1] | vout[2] | vout[3])); };
   auto load_v = [&](int u, float (&to)[NT][4]) {
     const auto r = values(a.v, u);
     int at = afresh(vlane);
@@ -573,20 +527,18 @@ __global__ __launch_bounds__(512, NT == 1 && !DELTA ? 4 : 2) void linear_chunk_s
 #pragma unroll
       for (int nt = 0; nt < NT; nt++) to[nt][e] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(r, at + 64 * nt, 0, 0));
   };
-  auto operands = [&](const half8* from, int kb, half8 (&hi)[NT], half8 (&lo)[NT]) {  // both column tiles
+  auto operands = [&](const part8* from, int kb, part8 (&x)[NT][kParts]) {  // all column tiles
 #pragma unroll
-    for (int nt = 0; nt < NT; nt++) {
-      hi[nt] = from[((kb * NT + nt) * 2 + 0) * 64 + lane];
-      lo[nt] = from[((kb * NT + nt) * 2 + 1) * 64 + lane];
-    }
+    for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+      for (int p = 0; p < kParts; p++) x[nt][p] = from[((kb * NT + nt) * kParts + p) * 64 + lane];
   };
   uint32_t slow = 0;  // the columns that are done row by row
-  int sshift[NT];
   f4 S[MT][NT];
 
   if (role == 0) {
     __builtin_amdgcn_s_setprio(2);  // the state is what everything waits for
-    half8 fk[NKB][2], ft[2][2], fkt[MT][2][2];
+    part8 fk[NKB][kParts], ft[2][kParts], fkt[MT][2][kParts];
     float v[2][NT][4];  // this chunk's and the next one's
     f4 eg, fg;
     auto load_k = [&](int u) {
@@ -595,7 +547,7 @@ __global__ __launch_bounds__(512, NT == 1 && !DELTA ? 4 : 2) void linear_chunk_s
 #pragma unroll
         for (int kb = 0; kb < NKB; kb++)
 #pragma unroll
-          for (int hl = 0; hl < 2; hl++) fk[kb][hl] = load8(r, at_k, W::K + (kb * 2 + hl) * 64);
+          for (int p = 0; p < kParts; p++) fk[kb][p] = load8(r, at_k, W::K + (kb * kParts + p) * 64);
     };
     auto load_t = [&](int u) {
       const auto r = head(u);
@@ -603,7 +555,7 @@ __global__ __launch_bounds__(512, NT == 1 && !DELTA ? 4 : 2) void linear_chunk_s
 #pragma unroll
         for (int kb = 0; kb < 2; kb++)
 #pragma unroll
-          for (int hl = 0; hl < 2; hl++) ft[kb][hl] = load8(r, at_t, W::T + (kb * 2 + hl) * 64);  // (also what no product takes)
+          for (int p = 0; p < kParts; p++) ft[kb][p] = load8(r, at_t, W::T + (kb * kParts + p) * 64);  // (also what no product takes)
     };
     auto load_kt = [&](int u) {
       const auto r = keys(u);
@@ -612,19 +564,24 @@ __global__ __launch_bounds__(512, NT == 1 && !DELTA ? 4 : 2) void linear_chunk_s
 #pragma unroll
         for (int kb = 0; kb < 2; kb++)
 #pragma unroll
-          for (int hl = 0; hl < 2; hl++) fkt[i][kb][hl] = load8(r, at_k, W::KT + ((i * 2 + kb) * 2 + hl) * 64);
+          for (int p = 0; p < kParts; p++) fkt[i][kb][p] = load8(r, at_k, W::KT + ((i * 2 + kb) * kParts + p) * 64);
     };
-    auto note = [&](int nt, uint32_t t) {  // a column's largest over this wave's key dims
-      t = groups_max(t);
-      const int l = afresh(lane);
-      if (l < 16) smax[wave][16 * nt + l] = t;
+    auto note = [&]() {  // this wave's key dims
+      uint32_t top[NT] = {};
+#pragma unroll
+      for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+        for (int i = 0; i < MT; i++)
+#pragma unroll
+          for (int r = 0; r < 4; r++) top[nt] = max(top[nt], mag(S[i][nt][r]));
+      sout[wave] = marked(top);
     };
-    auto put4 = [&](half8* to, int tile, int nt, float a, float b, float c, float d) {
-      u2 hi, lo;
-      split4(a, b, c, d, hi, lo);
-      char* p = (char*)(to + (((tile >> 1) * NT + nt) * 2) * 64 + lane) + 8 * (tile & 1);
-      *(u2*)p = hi;
-      *(u2*)(p + 64 * 16) = lo;
+    auto put4 = [&](part8* to, int tile, int nt, float a, float b, float c, float d) {
+      u2 x[kParts];
+      split4(a, b, c, d, x);
+      char* at = (char*)(to + (((tile >> 1) * NT + nt) * kParts) * 64 + lane) + 8 * (tile & 1);
+#pragma unroll
+      for (int p = 0; p < kParts; p++) *(u2*)(at + p * 64 * 16) = x[p];
     };
     auto put_state = [&]() {
 #pragma unroll
@@ -647,54 +604,32 @@ __global__ __launch_bounds__(512, NT == 1 && !DELTA ? 4 : 2) void linear_chunk_s
     load_t(first);
     load_kt(first);
     load_v(min(first + 1, last - 1), v[1]);
-#pragma unroll
-    for (int nt = 0; nt < NT; nt++) {
-      uint32_t t = 0;
-#pragma unroll
-      for (int i = 0; i < MT; i++)
-#pragma unroll
-        for (int r = 0; r < 4; r++) t = max(t, mag(S[i][nt][r]));
-      note(nt, t);
-    }
-    __syncthreads();
-    // from here on S holds the state times 2^sshift
-#pragma unroll
-    for (int nt = 0; nt < NT; nt++) {
-      sshift[nt] = first_shift(nt);
-#pragma unroll
-      for (int i = 0; i < MT; i++)
-#pragma unroll
-        for (int r = 0; r < 4; r++) S[i][nt][r] = ldexpf(S[i][nt][r], sshift[nt]);
-    }
+    note();
     put_state();
 #pragma unroll 1
     for (int u = first; u < last; u++) {
       const int next = min(u + 1, last - 1);
-      const int kshift = word(M_KSHIFT), tshift = word(M_TSHIFT + wave);
-      const float whole = fword(M_WHOLE);
+      const float whole = __uint_as_float(uniform((int)meta[0]));
       __syncthreads();  // the state, and what is noted of it and of V
-      const Shifts sh = shifts();
+      const uint32_t out = marks();
       load_meta(next);
       f4 vp[NT];
       if constexpr (DELTA) {
         f4 ks[NT] = {};
 #pragma unroll
         for (int kb = 0; kb < NKB; kb++) {
-          half8 hi[NT], lo[NT];
-          operands(Sb, kb, hi, lo);
-          products3(fk[kb][0], fk[kb][1], hi, lo, ks);
+          part8 x[NT][kParts];
+          operands(Sb, kb, x);
+          products(fk[kb], x, ks);
         }
         __builtin_amdgcn_sched_barrier(0);
         load_k(next);
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int nt = 0; nt < NT; nt++) {
-          // Y 2^y. Powers of two go to the values here and below: as a factor of its own one would overflow where the
-          // values that it belongs to are nothing, and zero times infinity is NaN.
-          const int e = sh.y[nt] - kshift - sshift[nt];
           float y[4];
 #pragma unroll
-          for (int r = 0; r < 4; r++) y[r] = ldexpf(v[0][nt][r], sh.y[nt]) - ldexpf(eg[r] * ks[nt][r], e);
+          for (int r = 0; r < 4; r++) y[r] = fmaf(-eg[r], ks[nt][r], v[0][nt][r]);
           put4(Yb, wave, nt, y[0], y[1], y[2], y[3]);
         }
         eg = load_fade(next, 0);
@@ -703,9 +638,9 @@ __global__ __launch_bounds__(512, NT == 1 && !DELTA ? 4 : 2) void linear_chunk_s
 #pragma unroll
         for (int kb = 0; kb < 2; kb++)
           if (2 * kb <= wave) {
-            half8 hi[NT], lo[NT];
-            operands(Yb, kb, hi, lo);
-            products3(ft[kb][0], ft[kb][1], hi, lo, vp);
+            part8 x[NT][kParts];
+            operands(Yb, kb, x);
+            products(ft[kb], x, vp);
           }
         __builtin_amdgcn_sched_barrier(0);
         load_t(next);
@@ -716,29 +651,22 @@ __global__ __launch_bounds__(512, NT == 1 && !DELTA ? 4 : 2) void linear_chunk_s
 #pragma unroll
           for (int r = 0; r < 4; r++) vp[nt][r] = v[0][nt][r];
       }
-      // V' as it is held: times 2^held
-      int held[NT];
 #pragma unroll
-      for (int nt = 0; nt < NT; nt++) held[nt] = DELTA ? tshift + sh.y[nt] : 0;
-#pragma unroll
-      for (int nt = 0; nt < NT; nt++) {
-        const int e = sh.f[nt] - held[nt];
-        put4(Fb, wave, nt, ldexpf(fg[0] * vp[nt][0], e), ldexpf(fg[1] * vp[nt][1], e), ldexpf(fg[2] * vp[nt][2], e), ldexpf(fg[3] * vp[nt][3], e));
-      }
+      for (int nt = 0; nt < NT; nt++) put4(Fb, wave, nt, fg[0] * vp[nt][0], fg[1] * vp[nt][1], fg[2] * vp[nt][2], fg[3] * vp[nt][3]);
       fg = load_fade(next, 256);
       __syncthreads();
       f4 acc[MT][NT] = {};
 #pragma unroll
       for (int kb = 0; kb < 2; kb++) {
-        half8 hi[NT], lo[NT];
-        operands(Fb, kb, hi, lo);
+        part8 x[NT][kParts];
+        operands(Fb, kb, x);
 #pragma unroll
-        for (int i = 0; i < MT; i++) products3(fkt[i][kb][0], fkt[i][kb][1], hi, lo, acc[i]);
+        for (int i = 0; i < MT; i++) products(fkt[i][kb], x, acc[i]);
       }
       __builtin_amdgcn_sched_barrier(0);
       load_kt(next);
       __builtin_amdgcn_sched_barrier(0);
-      if (const uint32_t todo = sh.out & ~slow) {  // columns that leave the chunks here
+      if (const uint32_t todo = out & ~slow) {  // columns that leave the chunks here
         const int l = afresh(lane);
 #pragma unroll
         for (int nt = 0; nt < NT; nt++) {
@@ -747,84 +675,72 @@ __global__ __launch_bounds__(512, NT == 1 && !DELTA ? 4 : 2) void linear_chunk_s
 #pragma unroll
           for (int i = 0; i < MT; i++)
 #pragma unroll
-            for (int r = 0; r < 4; r++) plain[c][16 * (wave * MT + i) + 4 * (l >> 4) + r] = ldexpf(S[i][nt][r], -sshift[nt]);
+            for (int r = 0; r < 4; r++) plain[c][16 * (wave * MT + i) + 4 * (l >> 4) + r] = S[i][nt][r];
           if (wave == 0) slow_from[c] = u - unit0;
         }
         slow |= todo;
       }
 #pragma unroll
       for (int nt = 0; nt < NT; nt++) {
-        const int e = sh.s_next[nt] - kshift - sh.f[nt], w = sh.s_next[nt] - sshift[nt];
-        uint32_t t = 0;
 #pragma unroll
-        for (int i = 0; i < MT; i++) {
+        for (int i = 0; i < MT; i++)
 #pragma unroll
-          for (int r = 0; r < 4; r++) S[i][nt][r] = ldexpf(acc[i][nt][r], e) + ldexpf(whole * S[i][nt][r], w);
-#pragma unroll
-          for (int r = 0; r < 4; r++) t = max(t, mag(S[i][nt][r]));
-        }
-        sshift[nt] = sh.s_next[nt];
-        note(nt, mag(ldexpf(__uint_as_float(t), -sshift[nt])));
+          for (int r = 0; r < 4; r++) S[i][nt][r] = fmaf(whole, S[i][nt][r], acc[i][nt][r]);
 #pragma unroll
         for (int r = 0; r < 4; r++) v[0][nt][r] = moved(v[1][nt][r]);
       }
+      note();
       put_state();
       // V' for the output waves, which take it behind the next barrier
 #pragma unroll
-      for (int nt = 0; nt < NT; nt++) {
-        const int e = sh.v[nt] - held[nt];
-        put4(Vb[u & 1], wave, nt, ldexpf(vp[nt][0], e), ldexpf(vp[nt][1], e), ldexpf(vp[nt][2], e), ldexpf(vp[nt][3], e));
-      }
+      for (int nt = 0; nt < NT; nt++) put4(Vb[u & 1], wave, nt, vp[nt][0], vp[nt][1], vp[nt][2], vp[nt][3]);
       __builtin_amdgcn_sched_barrier(0);
       load_v(min(u + 2, last - 1), v[1]);
       __builtin_amdgcn_sched_barrier(0);
     }
     __syncthreads();
   } else {
-    half8 fq[NKB][2], fp[2][2];
+    part8 fq[NKB][kParts], fp[2][kParts];
     f4 eg;
     auto load_q = [&](int u) {
       const auto r = keys(u);
 #pragma unroll
       for (int kb = 0; kb < NKB; kb++)
 #pragma unroll
-        for (int hl = 0; hl < 2; hl++) fq[kb][hl] = load8(r, at_k, W::Q + (kb * 2 + hl) * 64);
+        for (int p = 0; p < kParts; p++) fq[kb][p] = load8(r, at_k, W::Q + (kb * kParts + p) * 64);
     };
     auto load_p = [&](int u) {
       const auto r = head(u);
 #pragma unroll
       for (int kb = 0; kb < 2; kb++)
 #pragma unroll
-        for (int hl = 0; hl < 2; hl++) fp[kb][hl] = load8(r, at_t, W::P + (kb * 2 + hl) * 64);
+        for (int p = 0; p < kParts; p++) fp[kb][p] = load8(r, at_t, W::P + (kb * kParts + p) * 64);
     };
     auto note_v = [&](const float (&of)[NT][4]) {
+      uint32_t top[NT] = {};
 #pragma unroll
-      for (int nt = 0; nt < NT; nt++) {
-        uint32_t t = 0;
+      for (int nt = 0; nt < NT; nt++)
 #pragma unroll
-        for (int r = 0; r < 4; r++) t = max(t, mag(of[nt][r]));
-        t = groups_max(t);
-        const int l = afresh(lane);
-        if (l < 16) vmax[wave][16 * nt + l] = t;
-      }
+        for (int r = 0; r < 4; r++) top[nt] = max(top[nt], mag(of[nt][r]));
+      vout[wave] = marked(top);
     };
     float v[NT][4];
     f4 o[NT] = {};
     // what V' (in Vb[half]) adds to the rows of chunk u, and their store, but for the columns `left_out`
-    auto finish = [&](int u, int half, int pshift, const int (&vshift)[NT], uint32_t left_out) {
+    auto finish = [&](int u, int half, uint32_t left_out) {
       const auto ro = values(a.out, u);
       f4 acc[NT] = {};
 #pragma unroll
       for (int kb = 0; kb < 2; kb++)
         if (2 * kb <= wave) {
-          half8 hi[NT], lo[NT];
-          operands(Vb[half], kb, hi, lo);
-          products3(fp[kb][0], fp[kb][1], hi, lo, acc);
+          part8 x[NT][kParts];
+          operands(Vb[half], kb, x);
+          products(fp[kb], x, acc);
         }
 #pragma unroll
       for (int nt = 0; nt < NT; nt++) {
 #pragma unroll
-        for (int r = 0; r < 4; r++) acc[nt][r] = fmaf(a.scale, ldexpf(acc[nt][r], -pshift - vshift[nt]), o[nt][r]);
+        for (int r = 0; r < 4; r++) acc[nt][r] = fmaf(a.scale, acc[nt][r], o[nt][r]);
       }
       // (A column that is left out, and with the first chunk every one, is stored past the buffer's end, which drops it:
       // with a branch there a wait for what was loaded before would not know how many stores came after, and wait for them.)
@@ -844,23 +760,18 @@ __global__ __launch_bounds__(512, NT == 1 && !DELTA ? 4 : 2) void linear_chunk_s
     load_p(first);
     note_v(v);
     load_v(min(first + 1, last - 1), v);
-    __syncthreads();
-#pragma unroll
-    for (int nt = 0; nt < NT; nt++) sshift[nt] = first_shift(nt);
-    int vshift[NT] = {}, pshift = 0;
 #pragma unroll 1
     for (int u = first; u < last; u++) {
       const int next = min(u + 1, last - 1);
       __syncthreads();
-      const Shifts sh = shifts();
-      const int qshift = word(M_QSHIFT + wave), pshift_now = word(M_PSHIFT + wave);
+      const uint32_t out = marks();
       load_meta(next);
       f4 now[NT] = {};
 #pragma unroll
       for (int kb = 0; kb < NKB; kb++) {
-        half8 hi[NT], lo[NT];
-        operands(Sb, kb, hi, lo);
-        products3(fq[kb][0], fq[kb][1], hi, lo, now);
+        part8 x[NT][kParts];
+        operands(Sb, kb, x);
+        products(fq[kb], x, now);
       }
       __builtin_amdgcn_sched_barrier(0);
       load_q(next);
@@ -871,31 +782,25 @@ __global__ __launch_bounds__(512, NT == 1 && !DELTA ? 4 : 2) void linear_chunk_s
       for (int nt = 0; nt < NT; nt++) {
 #pragma unroll
         for (int r = 0; r < 4; r++) {
-          now[nt][r] = a.scale * (eg[r] * ldexpf(now[nt][r], -qshift - sshift[nt]));
+          now[nt][r] = a.scale * (eg[r] * now[nt][r]);
           asm volatile("" : "+v"(now[nt][r]));  // here: moved to where it is read next, it would keep eg from its next load
         }
       }
       eg = load_fade(next, 0);
       __syncthreads();
       note_v(v);
-      finish(max(u - 1, first), u & 1 ^ 1, pshift, vshift, u > first ? slow : ~0u);
+      finish(max(u - 1, first), u & 1 ^ 1, u > first ? slow : ~0u);
       __builtin_amdgcn_sched_barrier(0);
       load_p(u);
-      __builtin_amdgcn_sched_barrier(0);
       __builtin_amdgcn_sched_barrier(0);
       load_v(min(u + 2, last - 1), v);
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-      for (int nt = 0; nt < NT; nt++) {
-        o[nt] = now[nt];
-        vshift[nt] = sh.v[nt];
-        sshift[nt] = sh.s_next[nt];
-      }
-      pshift = pshift_now;
-      slow |= sh.out;
+      for (int nt = 0; nt < NT; nt++) o[nt] = now[nt];
+      slow |= out;
     }
     __syncthreads();
-    finish(last - 1, (last - 1) & 1, pshift, vshift, slow);
+    finish(last - 1, (last - 1) & 1, slow);
   }
   float* left = L.state + (((size_t)uniform(sp->dst) * L.v_heads + h) * DV + col0) * DK;
   if (role == 0)
@@ -903,8 +808,7 @@ __global__ __launch_bounds__(512, NT == 1 && !DELTA ? 4 : 2) void linear_chunk_s
     for (int i = 0; i < MT; i++)
 #pragma unroll
       for (int nt = 0; nt < NT; nt++)
-        if (!(slow >> (16 * nt + n) & 1)) *(f4*)(left + (16 * nt + n) * DK + 16 * (wave * MT + i) + 4 * g) =
-              f4{ldexpf(S[i][nt][0], -sshift[nt]), ldexpf(S[i][nt][1], -sshift[nt]), ldexpf(S[i][nt][2], -sshift[nt]), ldexpf(S[i][nt][3], -sshift[nt])};
+        if (!(slow >> (16 * nt + n) & 1)) *(f4*)(left + (16 * nt + n) * DK + 16 * (wave * MT + i) + 4 * g) = S[i][nt];
   if (!slow) return;
   // the other columns, eight lanes each, as linear_attn.hip does them
   __syncthreads();

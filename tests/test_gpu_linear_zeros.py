@@ -1,5 +1,5 @@
 """GPU: linear attention where an operand of a prompt's chunk is nothing: value dims, keys, queries or states that are
-zero throughout, values near the smallest floats. Nothing in them is infinite, and nothing that they give."""
+zero throughout, values near the smallest floats. They are numbers like others (bounds: linear_helpers.py)."""
 import numpy as np
 import pytest
 
@@ -13,6 +13,7 @@ ROWS = pytest.mark.parametrize("rows", [[28], [64], [100], [150, 29]])
 def finite(c):
     out, state = c.run()
     assert np.isfinite(out).all() and np.isfinite(state).all()
+    c.check(out, state)
     return out, state
 
 
@@ -109,12 +110,19 @@ def test_decays_near_the_smallest_floats(dev, rule, first):
 @RULES
 @pytest.mark.parametrize("size", [1e-36, 1e-42, 1e-45])
 def test_values_near_the_smallest_floats(dev, rule, size):
+    """Beside the bound, in which sizes count: below 2^-126 a float keeps a step of 2^-149, the parts that products take
+    of one (the third is 2^-16 of it) a step of 2^-133, or of 2^-126 where subnormals are dropped. A row and key dim adds one
+    to a sum of at most 64 + 128."""
     c = Case([130], rule=rule, seed=9)
     c.v = (c.v * size).astype(np.float32)
     c.state = (c.state * size).astype(np.float32)
     c.v[..., ::4] = np.random.default_rng(1).standard_normal(c.v[..., ::4].shape)  # ordinary value dims beside them
     c.state[..., ::4, :] = 0
-    finite(c)
+    out, state = finite(c)
+    want, bound, S, S_bound = c.reference()
+    step = 2.0 ** -126 * 192 * c.growth() if rule == "delta" else 2.0 ** -126 * 192
+    assert np.all(np.abs(out - want) <= bound - 1e-30 + 4 * step)
+    assert np.all(np.sqrt(np.square(state - S).sum(-1)) <= S_bound - 1e-30 + 4 * step)
 
 
 @pytest.mark.parametrize("size", [1e-25, 1e-12, 1e12, 1e25])
