@@ -40,7 +40,7 @@ except ImportError:  # the host-only functions (tables, plans, snapshot checks) 
 from ._args import _f32, _getDevice, _int32, _ptr, _rows_ptr, _stream
 from ._lib import (BG_E_INVALID, BG_E_STATE, BG_K, BG_KSCALE, BG_ROPE_ABSOLUTE, BG_ROPE_SLOT, BG_V, BG_VSCALE,
                    KV_DTYPES, BitgpuError, check, lib)
-from .linear import (FourBitWeight, LinearBatch, LinearStateCache, _between, _fused_mm4, _layer_ptrs, _on, _resid_mm4,
+from .linear import (FourBitWeight, LinearBatch, LinearStateCache, _aligned, _between, _fused_mm4, _layer_ptrs, _on, _resid_mm4,
                      linear_attention, linear_layer_attention, linear_prologue)
 
 __all__ = ["KvCache", "attention", "qkv_prologue", "layer_attention", "hybrid_full_attention",
@@ -801,11 +801,16 @@ def linear_block(cache: LinearStateCache, li: int, batch: LinearBatch, n1, h, w_
     if n1.shape[-1] != w_in.K or h.numel() != M * w_out.N:
         raise ValueError(f"bitgpu_amd: n1 must hold [{M}, {w_in.K}] and h [{M}, {w_out.N}], got {list(n1.shape)} and {list(h.shape)}")
     # everything that a later launch would refuse, before the first one: the states have moved on behind it
+    at = []
     for w in (w_in, w_out):
         if isinstance(w, FourBitWeight):
             _on(w)
+            at.append(w._w)
         elif M != 1:
             raise ValueError(f"bitgpu_amd: a 1-bit weight's product takes one row, got {M}")
+        else:
+            at.append((_ptr(w.sign), _ptr(w.scales)))
+        _aligned(*at[-1][:3])
     x, res = _rows_ptr(n1, "n1", M, w_in.K, dev), _rows_ptr(h, "h", M, w_out.N, dev)
     weights = _layer_ptrs(cache, conv_weight, a_log, dt_bias, norm, eps)
     # one piece of memory for what lies between the launches: qkv, z, att | b, a (interleaved rows) and the prologue's
@@ -819,16 +824,16 @@ def linear_block(cache: LinearStateCache, li: int, batch: LinearBatch, n1, h, w_
     inner = att + 4 * M * Z
     ba = inner + 4 * M * (wide + 2 * Hv)
     if isinstance(w_in, FourBitWeight):
-        rc = L.bg_gemv4_split(x, M, w_in.K, *w_in._w, wide, Z, 2 * Hv, qkv, z, ba, space, st)
+        rc = L.bg_gemv4_split(x, M, w_in.K, *at[0], wide, Z, 2 * Hv, qkv, z, ba, space, st)
     else:
-        rc = L.bg_gemv_split(x, w_in.K, _ptr(w_in.sign), _ptr(w_in.scales), wide, Z, 2 * Hv, qkv, z, ba, st)
+        rc = L.bg_gemv_split(x, w_in.K, *at[0], wide, Z, 2 * Hv, qkv, z, ba, st)
     if rc:
         check(rc)
     _between(cache, li, batch, qkv, ba + 4 * Hv, ba, 2 * Hv, weights, z, eps, inner, att, st)
     if isinstance(w_out, FourBitWeight):
-        rc = L.bg_gemv4_resid(att, M, Z, *w_out._w, w_out.N, res, out.data_ptr(), space, st)
+        rc = L.bg_gemv4_resid(att, M, Z, *at[1], w_out.N, res, out.data_ptr(), space, st)
     else:
-        rc = L.bg_gemv_resid(att, Z, _ptr(w_out.sign), _ptr(w_out.scales), w_out.N, res, out.data_ptr(), st)
+        rc = L.bg_gemv_resid(att, Z, *at[1], w_out.N, res, out.data_ptr(), st)
     if rc:
         check(rc)
     return out

@@ -46,6 +46,7 @@ class FourBitWeight:
         self._type = BG_KV_F16 if scales.dtype is torch.float16 else BG_KV_F32
         for t in (codes, scales, mins):
             _ptr(t)
+        _aligned(*self._w[:3])
 
     @property
     def _w(self):
@@ -55,6 +56,11 @@ class FourBitWeight:
     @property
     def N(self) -> int:
         return self.N0 + self.N1 + self.N2
+
+
+def _aligned(*pointers):
+    if any(p and p & 15 for p in pointers):
+        raise ValueError("bitgpu_amd: a weight's tensors must be 16-byte aligned")
 
 
 def _rows_of(w, x):
