@@ -792,6 +792,8 @@ def linear_block(cache: LinearStateCache, li: int, batch: LinearBatch, n1, h, w_
     if (w_in.N0, w_in.N1, w_in.N2) != (cache.channels, Hv * DV, 2 * Hv) or w_out.K != Hv * DV:
         raise ValueError(f"bitgpu_amd: the weights' rows must be {cache.channels} | {Hv * DV} | {2 * Hv} from the hidden state "
                          f"and the hidden state from {Hv * DV}")
+    if n1.dim() not in (1, 2):
+        raise ValueError(f"bitgpu_amd: n1 must be [K] or [rows, K], got {list(n1.shape)}")
     M = 1 if n1.dim() == 1 else n1.shape[0]
     if M != batch.n_tokens:
         raise ValueError(f"bitgpu_amd: n1 holds {M} rows, the batch has {batch.n_tokens} new rows")

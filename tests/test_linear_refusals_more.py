@@ -90,3 +90,12 @@ def test_a_weight_that_no_product_takes(monkeypatch):
     for k in (dict(scales=scales[1:]), dict(mins=scales[1:]), dict(codes=Z(801, dtype=torch.int32)[1:].view(10, 80))):
         with pytest.raises(ValueError, match="16-byte aligned"):
             E.FourBitWeight(**{**dict(codes=codes[1:], scales=scales[:10], K=640, N0=10), **k})
+
+
+def test_hidden_rows_of_three_dims(launches):
+    """[3, 2, K] is not three rows: the result would be half uninitialized."""
+    cache, batch, calls = launches
+    for n1 in (Z(3, 2, 256), Z(3, 1, 256), Z(1, 3, 256)):
+        with pytest.raises(ValueError, match=r"n1 must be \[K\] or \[rows, K\]"):
+            block(cache, batch, n1=n1)
+    assert not calls
