@@ -811,6 +811,9 @@ def linear_block(cache: LinearStateCache, li: int, batch: LinearBatch, n1, h, w_
         elif M != 1:
             raise ValueError(f"bitgpu_amd: a 1-bit weight's product takes one row, got {M}")
         else:
+            for t in (w.sign, w.scales):
+                if t.get_device() != dev:
+                    raise ValueError(f"bitgpu_amd: a 1-bit weight is on cuda:{t.get_device()}, the cache on cuda:{dev}")
             at.append((_ptr(w.sign), _ptr(w.scales)))
         _aligned(*at[-1][:3])
     x, res = _rows_ptr(n1, "n1", M, w_in.K, dev), _rows_ptr(h, "h", M, w_out.N, dev)

@@ -99,3 +99,15 @@ def test_hidden_rows_of_three_dims(launches):
         with pytest.raises(ValueError, match=r"n1 must be \[K\] or \[rows, K\]"):
             block(cache, batch, n1=n1)
     assert not calls
+
+
+def test_one_bit_weights_of_another_device(launches, monkeypatch):
+    cache, batch, calls = launches
+    monkeypatch.setattr(E, "_ptr", _cpu_ptr)
+    batch.n_tokens = 1
+    away = types.SimpleNamespace(get_device=lambda: 1, is_contiguous=lambda: True, data_ptr=lambda: 256)
+    for which, w in (("w_in", lambda **k: one_bit(CH, HV * D, 2 * HV, **k)), ("w_out", lambda **k: one_bit(30, K=HV * D, **k))):
+        for k in (dict(sign=away), dict(scales=away)):
+            with pytest.raises(ValueError, match="cuda:1"):
+                block(cache, batch, 1, **{"w_in": one_bit(CH, HV * D, 2 * HV), "w_out": one_bit(30, K=HV * D), which: w(**k)})
+    assert not calls
