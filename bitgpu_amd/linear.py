@@ -215,7 +215,10 @@ def _columns_ptr(t, name, rows, width, device):
         raise ValueError(f"bitgpu_amd: expected {name} on cuda:{device}, got {t.device}")
     if t.dim() != 2 or t.shape[0] < rows or t.shape[1] != width or (t.stride(1) != 1 and width > 1):
         raise ValueError(f"bitgpu_amd: {name} must be [{rows} rows, {width}], got {list(t.shape)} with strides {list(t.stride())}")
-    return t.data_ptr(), t.stride(0) if t.shape[0] > 1 else width
+    stride = t.stride(0) if t.shape[0] > 1 else width
+    if stride > 0x7fffffff:
+        raise ValueError(f"bitgpu_amd: rows of {name} lie too far apart ({stride} values)")
+    return t.data_ptr(), stride
 
 
 def _conv_ptr(cache, w):

@@ -111,3 +111,17 @@ def test_one_bit_weights_of_another_device(launches, monkeypatch):
             with pytest.raises(ValueError, match="cuda:1"):
                 block(cache, batch, 1, **{"w_in": one_bit(CH, HV * D, 2 * HV), "w_out": one_bit(30, K=HV * D), which: w(**k)})
     assert not calls
+
+
+def test_row_strides_past_32_bits(host):  # noqa: F811
+    """The C entries take a row stride of 32 bits: a longer one had arrived as its low half."""
+    cache, batch = host
+    far = torch.empty(3, 2**32 + HV, device="meta")[:, :HV]
+    assert far.get_device() == -1 and far.stride(0) & 0xffffffff == HV
+    with pytest.raises(ValueError, match="rows of g lie too far apart"):
+        E.linear_attention(cache, 0, batch, Z(3, 1, D), Z(3, 1, D), Z(3, HV, D), far)
+    rows = dict(a=far, b=far, a_log=Z(HV), dt_bias=Z(HV))
+    with pytest.raises(ValueError, match="rows of a lie too far apart"):
+        E.linear_prologue(cache, 0, batch, Z(3, CH), Z(CH, 4), **rows)
+    with pytest.raises(ValueError, match="rows of a lie too far apart"):
+        E.linear_layer_attention(cache, 0, batch, Z(3, CH), conv_weight=Z(CH, 4), z=Z(3, HV, D), norm=Z(D), eps=1e-6, **rows)
