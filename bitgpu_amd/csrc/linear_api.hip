@@ -217,7 +217,8 @@ int32_t bg_linear_create(int32_t n_layers, int32_t k_heads, int32_t v_heads, int
     return fail(BG_E_UNSUPPORTED, "bg_linear_create: k_dim %d, v_dim %d unsupported (64 or 128)", k_dim, v_dim);
   if (conv_width != 0 && (conv_width < 2 || conv_width > 4))
     return fail(BG_E_UNSUPPORTED, "bg_linear_create: conv_width %d unsupported (2 to 4, 0: no convolution)", conv_width);
-  if (v_heads > 4096 || n_layers > (1 << 16) || n_slots > (1 << 24))  // a grid's heads; a state's values below 2^63
+  if (v_heads > 4096 || n_layers > (1 << 16) || n_slots > (1 << 24) ||  // a grid's heads; a state's bytes below 2^63
+      (long double)n_layers * n_slots * v_heads * v_dim * k_dim * sizeof(float) >= 0x1p63L)
     return fail(BG_E_UNSUPPORTED, "bg_linear_create: v_heads %d, n_layers %d or n_slots %d too large", v_heads, n_layers, n_slots);
   if (!state || (conv_width != 0) != (conv != nullptr))
     return fail(BG_E_INVALID, "bg_linear_create: state is NULL, or conv and conv_width do not belong together");
