@@ -130,6 +130,13 @@ int32_t check_pair(const char* who, const bg_linear_cache* c, const bg_linear_ba
   return BG_OK;
 }
 
+// Whether the scans of n chunked sequences are one launch: workgroups of 512 threads for 32 value dims of a head each,
+// rounded up to eight key heads (linear_chunk.hip), and fewer than 2^32 threads on a grid's axis
+bool one_launch(const bg_linear_batch* b, int n) {
+  const long long groups = ((long long)n * b->k_heads + 7) / 8 * 8;
+  return groups * (b->v_heads / b->k_heads) * (b->DV / 32) * 512 < 1ll << 32;
+}
+
 // Orders a call on `st` behind the batch's calls so far. (A launch under capture runs at replay: its order is
 // the caller's.)
 int32_t join_stream(const char* who, bg_linear_batch* b, hipStream_t st) {
@@ -318,6 +325,9 @@ int32_t bg_linear_batch_set(bg_linear_batch* b, int32_t n_seqs, const int32_t* r
   const Plan& p = b->next;
   if (p.n_tokens > b->cap_tokens)
     return fail(BG_E_STATE, "bg_linear_batch_set: %d new rows, but launches of this batch were captured with %d", p.n_tokens, b->cap_tokens);
+  if (!one_launch(b, p.n_chunked))
+    return fail(BG_E_UNSUPPORTED, "bg_linear_batch_set: %d sequences of at least %d new rows are too many at once for %d heads", p.n_chunked,
+                bg::kLinChunkFrom, b->v_heads);
   const int32_t rc = join_stream("bg_linear_batch_set", b, st);
   if (rc != BG_OK) return rc;
   const int slot = b->slot;
@@ -445,13 +455,16 @@ int32_t bg_linear_attention(const bg_linear_cache* c, int32_t layer, bg_linear_b
                                                     {beta, T * H}, {gate, nv}, {norm, (size_t)c->DV}};
   for (const auto& x : in)
     if (overlap(out, nv, x.p, x.n)) return fail(BG_E_INVALID, "bg_linear_attention: out overlaps an input");
+  const bg::LinBatchView batch = b->view(captured);
+  if (!one_launch(b, batch.n_chunked))
+    return fail(BG_E_UNSUPPORTED, "bg_linear_attention: any batch of %d new rows, for a graph, may be too many sequences for %d heads",
+                b->plan.n_tokens, c->v_heads);
   if (!captured) {
     const int32_t moved = join_stream("bg_linear_attention", b, st);
     if (moved != BG_OK) return moved;
   }
   const bg::LinAttnArgs args{q, k, v, g, g_stride, beta, scale, gate, norm, eps, out};
   const bg::LinLayer view = layer_view(c, layer);
-  const bg::LinBatchView batch = b->view(captured);
   hipError_t e = hipSuccess;
   if (captured || batch.n_seqs > batch.n_chunked) e = bg::launch_linear_rows(view, batch, args, st);
   if (e == hipSuccess && batch.n_chunk_units) e = bg::launch_linear_chunks(view, batch, args, st);
