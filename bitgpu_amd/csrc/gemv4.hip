@@ -55,6 +55,10 @@ constexpr int kToken = 4 * kDigit;
 // [block][word pair][lane], 16 bytes each, then powers of two [token][block]), behind all of them kSumBytes a step (the
 // groups' sums [16 rows][block][group])
 constexpr int kOperand = 8192, kPassBytes = kOperand + 64, kSumBytes = 1024;
+// A block's joined digits count 2^(e - kUnit) (codes without minima 16 times as much), |x| < 2^e there: a digit of weight
+// 2^0 counts 2^(e - 30), and digits 2 and 3 are the whole part. A group's sum is at most about 2^28 so, and may be multiplied by
+// a scale of 2^90.
+constexpr int kUnit = 14;
 constexpr int kOdd = 0x7fffffff;      // the power of two of a block with an infinity or a NaN (its digits are zero)
 
 // The word of a 128-weight block (0 to 15) that lane group g holds as its j-th after the exchange.
@@ -263,7 +267,7 @@ __global__ __launch_bounds__(64) void gemv4_digits_kernel(Gemv4Args a, int P) {
 #pragma unroll
     for (int q = 0; q < 4; q++)
       *(uint2*)(to + (2 * g + (j >> 1)) * 1024 + (16 * at + 4 * (token & 3) + q) * 16 + 8 * (j & 1)) = make_uint2(d[0][q], d[1][q]);
-    if (n == 0) ((int*)(to + kOperand))[4 * (token & 3) + g] = on && odd ? kOdd : odd ? 0 : e - (MINS ? 30 : 34);
+    if (n == 0) ((int*)(to + kOperand))[4 * (token & 3) + g] = on && odd ? kOdd : odd ? 0 : e - (MINS ? kUnit : kUnit + 4);
   }
   if constexpr (MINS) {
     const float t = block_sums<G>(x0, x1);
@@ -322,7 +326,7 @@ __global__ __launch_bounds__(64 * kWaves, P == 1 ? 4 : 2) void gemv4_kernel(Gemv
       }
 #pragma unroll
       for (int q = 0; q < 4; q++) *(uint2*)(dig + m * kToken + q * kDigit + 128 * g + 8 * n) = make_uint2(d[0][q], d[1][q]);
-      if (n == 0) exps[wave][m][g] = odd ? 0 : e - (MINS ? 30 : 34);
+      if (n == 0) exps[wave][m][g] = odd ? 0 : e - (MINS ? kUnit : kUnit + 4);
     }
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
     __builtin_amdgcn_wave_barrier();
@@ -420,7 +424,7 @@ __global__ __launch_bounds__(64 * kWaves, P == 1 ? 4 : 2) void gemv4_kernel(Gemv
 #pragma unroll
         for (int p = 0; p < P; p++) {  // digits 0, 1 and 2, 3 as integers (|d| <= 2^21), then in f32
           const float low = (float)(d[p][0] + (d[p][1] << 8)), hi = (float)(d[p][2] + (d[p][3] << 8));
-          const float all = fmaf(hi, 65536.0f, low);
+          const float all = fmaf(low, 0x1p-16f, hi);
           sum[p] = i ? fmaf(all, s, sum[p]) : all * s;
         }
       }
@@ -536,7 +540,7 @@ __global__ __launch_bounds__(64 * kWaves, 4) void gemv4_one_kernel(Gemv4Args a, 
         int e;
         const bool odd = digits(x0, x1, on, d, e);
         odd_any = odd_any || (on && odd);
-        ex = odd ? 0 : e - (MINS ? 30 : 34);
+        ex = odd ? 0 : e - (MINS ? kUnit : kUnit + 4);
         if constexpr (MINS) {
           float v = block_sums<G>(x0, x1);
           v = on && !odd ? v : 0.0f;
@@ -585,7 +589,7 @@ __global__ __launch_bounds__(64 * kWaves, 4) void gemv4_one_kernel(Gemv4Args a, 
 #pragma unroll
         for (int j = i * G / 16; j < (i + 1) * G / 16; j++)
           d = __builtin_amdgcn_mfma_i32_16x16x64_i8(xd[j], pair(weight_operand<MINS>(v[j >> 1][2 * (j & 1)]), weight_operand<MINS>(v[j >> 1][2 * (j & 1) + 1])), d, 0, 0, 0);
-        const float all = fmaf((float)(d[2] + (d[3] << 8)), 65536.0f, (float)(d[0] + (d[1] << 8)));
+        const float all = fmaf((float)(d[0] + (d[1] << 8)), 0x1p-16f, (float)(d[2] + (d[3] << 8)));
         acc = i ? fmaf(all, s[i], acc) : all * s[i];
       }
       acc = ldexpf(acc, ex);
