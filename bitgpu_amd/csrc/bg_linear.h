@@ -13,15 +13,15 @@ namespace bg {
 
 constexpr int kLinChunk = 64;     // rows of a unit
 // Sequences of at least this many new rows are done in chunks of 64, shorter ones row by row. With 32 heads of 128 x 128
-// one sequence of the delta rule takes 4.9 + 0.87 us a row so and 25 us as a chunk (4 sequences 6 + 0.87 and 35, 64 of
-// them 50 + 7.2 and 300: they meet at 23, 34 and 34 rows), one of the sum rule 5 + 0.75 and 18.5 (64: 45 + 6.2 and 192: at
-// 18 and 24). A batch does not know the rule: a number between.
+// one sequence of the delta rule takes 5.7 + 0.86 us a row so and 24 us as a chunk (4 sequences 6.1 + 0.92 and 36, 64 of
+// them 50 + 5.5 and 350: they meet at 22, 33 and 54 rows), one of the sum rule 5.9 + 0.66 and 17.6 (64: 50 + 4.8 and 254: at
+// 18 and 42). A batch does not know the rule: a number between.
 constexpr int kLinChunkFrom = 28;
 // Most bytes of chunk operands at a time. Of one sequence: what the scan reads should still be in the 256 MiB behind the
 // L2s that the preparation wrote it to, beside the rows themselves (8192 rows of 48 heads, 4.7 MB a chunk: 64 MiB 751 us,
 // 96 706, 112 684, 128 651, 144 651, 160 626, 176 628, 208 684, 256 684). Of several: a pass should hold many sequences,
-// whose scans run side by side (2048 rows of 32 heads: two sequences 128 MiB 241 us, 400 181; four 408 and 374; eight 824
-// and 751, 800 723; with two f16 parts an operand).
+// whose scans run side by side (2048 rows of 32 heads: two sequences 160 MiB 285 us, 384 225; four 570 and 441; eight 970
+// and 966).
 constexpr size_t kLinCached = (size_t)160 << 20, kLinSpace = (size_t)384 << 20;
 
 // a row's decay as hi + lo: the rounding of one float would add up over the rows of a constant decay

@@ -32,7 +32,7 @@ typedef __bf16 part8 __attribute__((ext_vector_type(8)));
 typedef float f4 __attribute__((ext_vector_type(4)));
 
 constexpr int kParts = 3;     // of an operand: largest first
-constexpr int kFewScans[2] = {256, 128};  // workgroups of 32 value dims of the sum and the delta rule's scan
+constexpr int kFewScans = 128;  // workgroups of 32 value dims
 constexpr int kPrepared = 768;   // workgroups that the preparation is split into, at most
 constexpr int kPad = 68;      // row stride of 64 x 64 matrices in LDS
 constexpr double kLowest = -1e4;  // of a log decay: e^g is 0 in f32 from -104 on
@@ -443,7 +443,7 @@ __global__ __launch_bounds__(256, 3) void linear_chunk_prepare(LinLayer L, LinBa
       // what a value of S or V may grow by: through e^G Q S; through Y, T and e^(G_n - G) to K^T V' or P V'
       const float pmax = __uint_as_float(max(max(bits[0], bits[1]), max(bits[2], bits[3])));
       constexpr int kSum = DK == 64 ? 6 : 7;
-      const int eg = max(0, top_exponent(gmax)), ek = top_exponent(kmax), y = max(0, kSum + ek + eg) + 1;
+      const int eg = max(0, top_exponent(gmax)), ek = top_exponent(kmax), y = DELTA ? max(0, kSum + ek + eg) + 1 : 0;
       const int v = y + max(0, top_exponent(tsum)) + max(0, top_exponent(fmax_));
       const int grow = max(max(eg, kSum + top_exponent(qmax) + eg), v + max(0, 6 + max(ek, top_exponent(pmax)))) + 1;
       BG_GLOBAL ChunkMeta* meta = (BG_GLOBAL ChunkMeta*)(wh + W::META);
@@ -464,7 +464,7 @@ __global__ __launch_bounds__(256, 3) void linear_chunk_prepare(LinLayer L, LinBa
 // chain of three products of six matrix instructions a tile and step, each with its operand's way through LDS. By
 // count the matrix cores and LDS are a third busy.
 template <int DK, int DV, bool DELTA, int NT>
-__global__ __launch_bounds__(512, NT == 1 && !DELTA ? 4 : 2) void linear_chunk_scan(LinLayer L, LinBatchView b, LinAttnArgs a, int u0, int u1) {
+__global__ __launch_bounds__(512, 2) void linear_chunk_scan(LinLayer L, LinBatchView b, LinAttnArgs a, int u0, int u1) {
   using W = ChunkSpace<DK>;
   constexpr int NKB = W::NKB, MT = DK / 64, kCols = 16 * NT, SLICES = DV / kCols;
   constexpr int kRows = 2 * NT * kParts * 64;    // of an operand whose k are the chunk's rows
@@ -889,18 +889,16 @@ hipError_t launch_t(const LinLayer& L, const LinBatchView& b, const LinAttnArgs&
   for (int u0 = 0; u0 < b.n_chunk_units; u0 += step) {
     const int u1 = std::min(u0 + step, b.n_chunk_units);
     // A workgroup's value heads one after the other, or, where that leaves most of the GPU idle, workgroups of their own
-    // that share a key head's products (16 key and 48 value heads, one chunk: prompt of 64 rows 38 us, so 28; four
-    // prompts of 256, 16 chunks, 81 and 74; 32 chunks 124 and 125, 8192 rows 486 and 493).
+    // that share a key head's products (16 key and 48 value heads, one chunk: prompt of 64 rows 36 us, so 27; four
+    // prompts of 256, 16 chunks, 91 and 88; 32 chunks 160 and 169, 8192 rows 604 and 637).
     const int rep = L.v_heads / L.k_heads, parts = std::max(1, std::min(rep, kPrepared / ((u1 - u0) * L.k_heads)));
     const int each = (rep + parts - 1) / parts;
     hipLaunchKernelGGL((linear_chunk_prepare<DK, DELTA>), dim3(u1 - u0, L.k_heads * ((rep + each - 1) / each)), dim3(256), 0, st, L, b, a, u0, each);
-    // 32 value dims a workgroup, or 16 where that still fits the GPU: of the sum rule, whose products need fewer
-    // registers, twice a CU (2 x 2048 rows of 16 heads, 128 workgroups of 32: 55 us, 256 of 16: 43), of the delta rule once
-    // (2048 rows of 16 heads, 64 workgroups of 32: 103 us, 128 of 16: 85; of two such prompts 118 and 101; of four of 1024
-    // rows 88 and 104). More workgroups, each reading the same operands, take longer.
-    const bool narrow = b.n_chunked * L.v_heads * (DV / 32) <= kFewScans[DELTA];
-    if (narrow) launch_scan<DK, DV, DELTA, 1>(L, b, a, u0, u1, st);
-    if (!narrow) launch_scan<DK, DV, DELTA, 2>(L, b, a, u0, u1, st);
+    // 32 value dims a workgroup, or 16 where that still leaves one workgroup a CU (delta rule, 2048 rows of 16 heads, 64
+    // workgroups of 32: 130 us, 128 of 16: 104; of two such prompts 176 and 163; three of 1024 rows 95 and 120. Sum, two of
+    // 2048, k_dim 64: 78 and 59; three 103 and 116). More workgroups, each reading the same operands, take longer.
+    if (b.n_chunked * L.v_heads * (DV / 32) <= kFewScans) launch_scan<DK, DV, DELTA, 1>(L, b, a, u0, u1, st);
+    else launch_scan<DK, DV, DELTA, 2>(L, b, a, u0, u1, st);
   }
   if (a.norm)
     hipLaunchKernelGGL((linear_norm_kernel<DV>), dim3(b.n_chunk_units, (kLinChunk * L.v_heads * DV / 4 + 1023) / 1024), dim3(256), 0, st, L, b, a);
