@@ -1,5 +1,5 @@
-// Linear attention with a decay for each head: what its kernels (linear_prologue.hip, linear_attn.hip) and
-// its entry points (linear_api.hip) share.
+// Linear attention with a decay for each head: what its kernels (linear_prologue.hip, linear_attn.hip,
+// linear_chunk.hip) and its entry points (linear_api.hip) share, and those of the 4-bit projections (gemv4.hip).
 //
 // Per layer, slot and value head one f32 matrix [v_dim][k_dim] (the state, transposed: a row holds what one
 // value dim has gathered over the key dims), and per layer and slot the convolution's last inputs,

@@ -1,8 +1,7 @@
 // 4-bit projections of up to 16 rows (bg_linear.h states the weight's format).
 //
 //   contraction  on the int8 matrix cores, exactly: a row of x becomes, 128 weights at a time, a 31-bit fixed-point
-//           number over the block's largest power of two in four signed int8 digits (x is rounded to 2^-31 of its
-//           block's largest, below the rounding of an f32 sum over the block); a weight's code, its top bit turned, is
+//           number over the block's largest power of two in four signed int8 digits; a weight's code, its top bit turned, is
 //           16 (c - 8) as the high half of a signed byte (two bit operations a word give its odd codes and, shifted,
 //           its even ones). The operand of x has four rows a token, one a digit, so a product takes four tokens; its
 //           result leaves lane 16 g + n with the four digit sums of weight row n and token g, exact integers that are
@@ -25,7 +24,10 @@
 //   bounds  one token: 24576 rows of K = 4096 in groups of 32 with minima (63 MB) 13.4 us, 4.7 TB/s, what a large copy
 //           reaches; 4096 x 4096 in groups of 128 (8.7 MB) 5.1 us, the latency of a launch and one pass over K. More tokens:
 //           the joining of the integers: ten rows of K = 4096, N = 16480 16.6 + 2.6 us.
-//   values  a block of x with an infinity or a NaN is summed directly in f32.
+//           (Of two to four tokens 24576 rows of K = 4096 take 19 to 20 us, of 16 30.)
+//   values  x is rounded to 2^-31 of its block's largest value: below the rounding of an f32 sum that this value takes part
+//           in. Where its weight is exactly zero (code 8, no minima) the others keep only that: values 2^-7 of the largest
+//           have an f32's 24 bits, smaller ones fewer. A block with an infinity or a NaN is summed directly in f32.
 #include <hip/hip_fp16.h>
 
 #include <algorithm>

@@ -1,6 +1,6 @@
 // C ABI of linear attention with a decay for each head (include/bitgpu_attn.h): the states' geometry over the
 // caller's device memory, the batch (its checks and its upload) and the launches; and of the 4-bit
-// projections. Host code only; the kernels live in linear_prologue.hip, linear_attn.hip and gemv4.hip.
+// projections. Host code only; the kernels live in linear_prologue.hip, linear_attn.hip, linear_chunk.hip and gemv4.hip.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>

@@ -422,7 +422,8 @@ int32_t bg_paged_attention(const bg_paged_kv* kv, int32_t layer, bg_paged_batch*
 typedef struct bg_linear_cache bg_linear_cache;
 typedef struct bg_linear_batch bg_linear_batch;
 
-/* k_dim, v_dim 64 or 128; v_heads a multiple of k_heads; conv_width 2 to 4, or 0 and conv NULL: no convolution. */
+/* k_dim, v_dim 64 or 128; v_heads a multiple of k_heads; conv_width 2 to 4, or 0 and conv NULL: no convolution. At most
+ * 4096 value heads, and states of less than 2^63 bytes. */
 int32_t bg_linear_create(int32_t n_layers, int32_t k_heads, int32_t v_heads, int32_t k_dim, int32_t v_dim, int32_t conv_width,
                          int32_t n_slots, float* state, float* conv, bg_linear_cache** out);
 int32_t bg_linear_destroy(bg_linear_cache* cache);
@@ -436,7 +437,8 @@ int32_t bg_linear_batch_destroy(bg_linear_batch* batch);
  * another (BG_E_INVALID, the batch before stays set). A sequence without new rows touches no slot. Rows are
  * numbered sequence by sequence. Not under graph capture (BG_E_STATE). Sequences of 28 new rows and more are done in
  * chunks of 64, whose operands take a workspace of at most 384 MiB (or one chunk's): it grows here (BG_E_OOM: the batch
- * before stays set), never in a layer's call. */
+ * before stays set), never in a layer's call. Their scans are one launch: sequences of that length times v_heads v_dim
+ * / 32 below 2^23 (BG_E_UNSUPPORTED, the batch before stays set), for a captured call any that its rows allow. */
 int32_t bg_linear_batch_set(bg_linear_batch* batch, int32_t n_seqs, const int32_t* rows, const int32_t* slots,
                             const int32_t* sources, void* stream);
 
@@ -457,7 +459,8 @@ int32_t bg_linear_prologue(const bg_linear_cache* cache, int32_t layer, bg_linea
  * with gate [rows, v_heads, v_dim] times gate / (1 + exp(-gate)). q, k, v, gate, norm, out 16-byte aligned; out
  * overlaps no input. Rows of out beyond the batch's are left as they are. A v that is not finite reaches its value dim's
  * row, later rows and state; a q its row of its heads; a k, g or beta its heads' row, later rows and states (g of minus
- * infinity is a decay to zero). Norms spread what is in a row over its head. */
+ * infinity is a decay to zero). Norms spread what is in a row over its head. Sums are f32 for any sizes of rows and value
+ * dims beside each other; in chunks, values below 2^-109 count in steps of 2^-133. */
 int32_t bg_linear_attention(const bg_linear_cache* cache, int32_t layer, bg_linear_batch* batch, const float* q, const float* k,
                             const float* v, const float* g, int32_t g_stride, const float* beta, float scale, const float* gate,
                             const float* norm, float eps, float* out, void* stream);
@@ -467,8 +470,9 @@ int32_t bg_linear_attention(const bg_linear_cache* cache, int32_t layer, bg_line
  * c = bits 4 (k % 8) .. + 3 of codes[n][k / 8] (u32) and, with the scale (and min) [n][k / group], the value
  * (c - 8) * scale, or c * scale + min where mins is not NULL. scale_type (scales and mins): BG_KV_F32 or BG_KV_F16.
  * K a multiple of 128, group 32, 64 or 128; x, codes, scales and mins 16-byte aligned. Outputs [rows, N0], [rows, N1],
- * [rows, N2]; resid, y [rows, N], y may be resid; otherwise no output overlaps an input or another. A product of two values may reach 2^126 and their scales 2^90; K at most
- * 2^24. More than four rows need a workspace of bg_gemv4_workspace(rows, K) bytes, 16-byte aligned, that no other stream
+ * [rows, N2]; resid, y [rows, N], y may be resid; otherwise no output overlaps an input or another. A product of two
+ * values may reach 2^126 and their scales 2^90; K at most 2^24. x counts to 2^-31 of the largest of its 128 (those from a
+ * multiple of 128 on), sums are f32. More than four rows need a workspace of bg_gemv4_workspace(rows, K) bytes, 16-byte aligned, that no other stream
  * uses meanwhile (four or fewer: 0 bytes, NULL). What a row gives does not depend on the rows beside it. */
 int64_t bg_gemv4_workspace(int32_t rows, int32_t K);
 int32_t bg_gemv4_split(const float* x, int32_t rows, int32_t K, const uint32_t* codes, const void* scales, const void* mins,
