@@ -11,9 +11,10 @@
 // bits and, down to 2^-109, its exponents: six products of nine, the others being below 2^-23 of a product, summed
 // in f32. Every row and value dim is as good as an f32 sum makes it, whatever its neighbours' sizes. (Two f16 parts
 // and three products are faster, prompt of 8192 rows 490 us instead of 617, but want one power of two for all rows of
-// a value dim: a large state or value that the rows behind it have forgotten leaves those with as many bits fewer.) The decays' sums are taken in
-// f64: their differences over a chunk would lose 2^-24 of the sums. T is found in f32: its diagonal blocks of 16 rows by
-// substitution, the others from them with f32 matrix products.
+// a value dim: a large state or value that the rows behind it have forgotten leaves those with as many bits fewer.) The
+// decays' sums are taken in f64: their differences over a chunk would lose 2^-24 of the sums. T is found in f32: its
+// diagonal blocks of 16 rows by substitution, the others from them with f32 matrix products. Values below 2^-109 count in
+// steps of 2^-133, the smallest bf16.
 //
 // A column whose V or S is not finite, or so large that a sum on the way could overflow, and every column of a chunk
 // whose K, Q, decays or strengths are not finite, is done again row by row: zero times infinity would reach
